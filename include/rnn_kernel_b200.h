@@ -117,6 +117,88 @@ int gru_mse_loss(const float* out, const float* target, long n, float* loss, voi
 int gru_mse_loss_backward(const float* out, const float* target, const float* grad_loss, float* dout, long n,
                           void* stream);
 
+/* ---- Element types of the entry points below ---- */
+#define GRU_F32 0
+#define GRU_BF16 1
+
+/* ---- AdamW over many tensors in one launch (the reference harness trains
+ * with torch.optim.AdamW: rnn_benchmark.py) ---- */
+
+/* One tensor (host struct).  param and grad are dense arrays of n elements of
+ * the call's dtype; its moments are elements [state_offset, state_offset + n)
+ * of the moment buffers, state_offset a multiple of 256; the elements up to
+ * the next multiple of 256 belong to it too and stay zero. */
+typedef struct {
+  void* param;
+  const void* grad;
+  long n;
+  long state_offset;
+  float decay;        /* 1 - lr * weight_decay */
+  float step_size;    /* lr / (1 - beta1^t); with device_step: lr */
+  float inv_sqrt_bc2; /* 1 / sqrt(1 - beta2^t); unused with device_step */
+} gru_adamw_tensor;
+
+/* One step on `count` tensors of one dtype (GRU_F32 or GRU_BF16), in place:
+ *   g *= grad_scale;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = decay p - step_size m / (sqrt(v) inv_sqrt_bc2 + eps)
+ * computed in FP32.  state_bits 32: exp_avg and exp_avg_sq hold state_elems
+ * floats.  state_bits 8: they hold one byte an element, and scale_avg /
+ * scale_sq one float per 256 elements (all zero-initialised).  8-bit moments
+ * are rounded stochastically from (seed, step, position), step the number of
+ * this step.  With device_scalars (3 device floats) the bias corrections and
+ * the rounding key come from there, and step_size holds lr; a call with
+ * device_step (a device counter) too first increments it and fills them, so
+ * that a CUDA graph can replay the step. */
+int gru_adamw_step(const gru_adamw_tensor* tensors, int count, int dtype, int state_bits, void* exp_avg,
+                   void* exp_avg_sq, float* scale_avg, float* scale_sq, long state_elems, double beta1, double beta2,
+                   double eps, double grad_scale, unsigned seed, long long step, long long* device_step,
+                   float* device_scalars, void* stream);
+
+/* The FP32 values that 8-bit moments stand for (state_elems floats each). */
+int gru_adamw_decode(const void* exp_avg, const void* exp_avg_sq, const float* scale_avg, const float* scale_sq,
+                     long state_elems, float* out_avg, float* out_avg_sq, void* stream);
+
+/* ---- Gated delta rule (no reference counterpart): a recurrent layer whose
+ * state is a matrix S [dk, dv] per batch row and value head.  Per token:
+ *   S' = e^g S;  u = beta (v - S'^T k);  S = S' + k u^T;  o = scale S^T q
+ * Value heads are shared out over the key heads in order: value head h reads
+ * key head h / (Hv / Hk).  g is the log of the decay (-inf resets the state);
+ * g, beta and states are FP32, q, k, v, out and their gradients of `dtype`. ---- */
+typedef struct {
+  int dtype; /* GRU_F32 or GRU_BF16 */
+  int B, T, Hk, Hv, dk, dv; /* 1 <= dk, dv <= 128; Hv a multiple of Hk */
+  float scale;
+  const void *q, *k, *v;       /* [B, T, Hk, dk], [B, T, Hk, dk], [B, T, Hv, dv] */
+  const float *g, *beta;       /* [B, T, Hv] */
+  const float* initial_state;  /* dense [B, Hv, dk, dv], or NULL for zeros */
+  /* elements between batch rows, tokens and heads; a head's elements are
+   * consecutive */
+  long q_stride[3], k_stride[3], v_stride[3], g_stride[3], beta_stride[3];
+} gru_delta_args; /* host struct */
+
+/* Bytes that gru_delta_forward leaves for gru_delta_backward (the forward
+ * needs them too when no backward follows), and each one's workspace; 0 and an
+ * error text for arguments that they refuse. */
+size_t gru_delta_stash_bytes(const gru_delta_args* args);
+size_t gru_delta_workspace_bytes(const gru_delta_args* args, int backward);
+
+/* All T tokens: out dense [B, T, Hv, dv], final_state dense [B, Hv, dk, dv]
+ * (which may be the initial state's memory). */
+int gru_delta_forward(const gru_delta_args* args, void* out, float* final_state, void* stash, size_t stash_bytes,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of q, k, v, g, beta (dense, overwritten; dq, dk and dv aligned to
+ * two elements) and of the initial state (or NULL), from dout dense
+ * [B, T, Hv, dv] and dfinal dense [B, Hv, dk, dv] (either NULL: zeros).  The
+ * arguments are the forward's, its inputs unchanged. */
+int gru_delta_backward(const gru_delta_args* args, const void* dout, const float* dfinal, const void* stash,
+                       size_t stash_bytes, void* dq, void* dk, void* dv, float* dg, float* dbeta, float* dinitial,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token (T = 1, initial_state unused): state dense [B, Hv, dk, dv] is
+ * updated in place, out is dense [B, Hv, dv]. */
+int gru_delta_step(const gru_delta_args* args, float* state, void* out, void* stream);
+
 /* Time chunks (no reference counterpart; a scheduling knob of this library).
  * When the time loops leave SMs idle (e.g. 104 of 148 at H = 256, B = 64),
  * gru_forward and gru_backward run the sequence as n consecutive chunks and
@@ -145,7 +227,7 @@ int gru_set_small_loops(int mode);
  * scripts/profile_a100_h256_step.py).  Kernel kinds: 0 input-projection GEMM,
  * 1 forward time loop, 2 backward time loop, 3 gradient products (dW, dx;
  * + split-K reduce), 4 bias-gradient column sums, 5 padding / transpose
- * copies, 6 MSE loss and its gradient. ---- */
+ * copies, 6 MSE loss and its gradient, 7 AdamW, 8 gated delta rule. ---- */
 
 /* Device status word of the current device: 0 when every kernel so far ran
  * to completion, else GRU_STATUS_* bits (a bounded wait inside a time-loop

@@ -7,8 +7,11 @@ if the library is missing the call raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
+
+import torch
 
 from . import build as _build
 
@@ -17,6 +20,9 @@ GRU_OK = 0
 GRU_ERR_INVALID = 1
 GRU_ERR_CUDA = 2
 GRU_ERR_UNSUPPORTED = 3
+# element types
+GRU_F32 = 0
+GRU_BF16 = 1
 
 _lock = threading.Lock()
 _lib = None
@@ -24,6 +30,11 @@ _lib = None
 _c_float_p = ctypes.c_void_p
 _size_t = ctypes.c_size_t
 _int = ctypes.c_int
+
+# gru_delta_args of include/rnn_kernel_b200.h, packed into bytes (which a call
+# takes as its pointer)
+DELTA_ARGS = struct.Struct("@7if6P15q")
+
 
 # name -> (restype, argtypes); mirrors include/rnn_kernel_b200.h
 SIGNATURES = {
@@ -44,11 +55,21 @@ SIGNATURES = {
     "gru_mse_loss": (_int, [_c_float_p, _c_float_p, ctypes.c_long, _c_float_p, ctypes.c_void_p, _size_t,
                             ctypes.c_void_p]),
     "gru_mse_loss_backward": (_int, [_c_float_p, _c_float_p, _c_float_p, _c_float_p, ctypes.c_long, ctypes.c_void_p]),
+    "gru_adamw_step": (_int, [ctypes.c_void_p, _int, _int, _int] + [ctypes.c_void_p] * 4 + [ctypes.c_long]
+                       + [ctypes.c_double] * 4 + [ctypes.c_uint, ctypes.c_longlong] + [ctypes.c_void_p] * 3),
+    "gru_adamw_decode": (_int, [ctypes.c_void_p] * 4 + [ctypes.c_long] + [ctypes.c_void_p] * 3),
+    "gru_delta_stash_bytes": (_size_t, [ctypes.c_void_p]),
+    "gru_delta_workspace_bytes": (_size_t, [ctypes.c_void_p, _int]),
+    "gru_delta_forward": (_int, [ctypes.c_void_p] * 4 + [_size_t, ctypes.c_void_p, _size_t, ctypes.c_void_p]),
+    "gru_delta_backward": (_int, [ctypes.c_void_p] * 4 + [_size_t] + [ctypes.c_void_p] * 7
+                           + [_size_t, ctypes.c_void_p]),
+    "gru_delta_step": (_int, [ctypes.c_void_p] * 4),
     "gru_timing_enable": (_int, [_int]),
     "gru_timing_collect": (_int, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int), _int]),
 }
 
-KERNEL_KINDS = ("input_gemm", "fwd_recurrent", "bwd_recurrent", "grad_gemm", "colsum", "layout", "loss")
+KERNEL_KINDS = ("input_gemm", "fwd_recurrent", "bwd_recurrent", "grad_gemm", "colsum", "layout", "loss", "optimizer",
+                "delta_rule")
 
 
 def timing_enable(on: bool) -> None:
@@ -121,6 +142,24 @@ def timeline_read():
     return buf
 
 
+class on_device:
+    """``torch.cuda.device`` that costs nothing where the device is current already."""
+
+    __slots__ = ("index", "guard")
+
+    def __init__(self, index: int) -> None:
+        self.index, self.guard = index, None
+
+    def __enter__(self) -> None:
+        if torch.cuda.current_device() != self.index:
+            self.guard = torch.cuda.device(self.index)
+            self.guard.__enter__()
+
+    def __exit__(self, *exc) -> None:
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
 def library_path() -> Path:
     return _build.LIB_PATH
 
@@ -128,6 +167,8 @@ def library_path() -> Path:
 def load(build_if_missing: bool = True) -> ctypes.CDLL:
     """Load (building first if needed and possible) the CUDA library."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

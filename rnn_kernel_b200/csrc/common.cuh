@@ -179,7 +179,9 @@ enum KernelKind {
   kKindColsum = 4,      // db_ih / db_hh
   kKindLayout = 5,      // padding / transpose copies feeding the tensor-core products
   kKindLoss = 6,        // MSE loss and its gradient
-  kKindCount = 7
+  kKindOptimizer = 7,   // AdamW
+  kKindDeltaRule = 8,   // gated delta rule: forward, gradient, step
+  kKindCount = 9
 };
 
 class LaunchScope {

@@ -1,0 +1,240 @@
+"""The gated delta rule on the CUDA library: a recurrent layer whose state is a matrix.
+
+Each batch row and value head keeps a state ``S [dk, dv]``; token t, with log
+decay ``g_t`` and writing strength ``beta_t``, does::
+
+    S' = exp(g_t) S;   u = beta_t (v_t - S'^T k_t);   S = S' + k_t u^T;   o_t = scale S^T q_t
+
+* :func:`gated_delta_rule` runs all tokens of a batch (in chunks of 64 on the
+  tensor cores) and has gradients for every input;
+* :func:`gated_delta_step` runs one token and updates the state in place;
+* :class:`GatedDelta` is the layer around them, with :class:`GRU`'s calling
+  convention: ``(input, state) -> (output, state)``.
+
+q, k and v are FP32 or bf16, gates and states FP32; products and sums are FP32
+throughout.  Value heads may outnumber key heads (``Hv = n Hk``: value head h
+reads key head ``h // n``).  Shape problems raise ``ValueError``, device and
+dtype problems and CUDA failures ``RuntimeError``; there is no CPU fallback.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from . import _lib
+from .gru import is_b200_available
+
+MAX_HEAD_SIZE = 128
+
+_DTYPES = {torch.float32: _lib.GRU_F32, torch.bfloat16: _lib.GRU_BF16}
+_supported: dict = {}  # device index -> whether it is a B200
+
+
+def _check(name, q, k, v, g, beta, state, lead):
+    """Sizes, types and devices of one call; ``lead`` is the number of leading dimensions."""
+    qs, vs = q.shape, v.shape
+    if len(qs) != lead + 2 or len(vs) != lead + 2:
+        dims = "batch" if lead == 1 else "batch, tokens"
+        raise ValueError(f"{name}: q, k, v must have shape [{dims}, heads, size] and g, beta [{dims}, value heads].")
+    if k.shape != qs:
+        raise ValueError(f"{name}: k must have q's shape.")
+    gates = vs[:-1]
+    if vs[:lead] != qs[:lead] or g.shape != gates or beta.shape != gates:
+        raise ValueError(f"{name}: v, g and beta must have q's leading dimensions and the same value heads.")
+    Hk, dk = qs[-2:]
+    Hv, dv = vs[-2:]
+    if Hk < 1 or Hv < 1 or Hv % Hk:
+        raise ValueError(f"{name}: the value heads must be a multiple of the key heads.")
+    if not 1 <= dk <= MAX_HEAD_SIZE or not 1 <= dv <= MAX_HEAD_SIZE:
+        raise ValueError(f"{name}: head sizes must be in [1, {MAX_HEAD_SIZE}].")
+    if state is not None and state.shape != (qs[0], Hv, dk, dv):
+        raise ValueError(f"{name}: the state must have shape {(qs[0], Hv, dk, dv)}.")
+    dev, dtype = q.get_device(), q.dtype
+    if k.get_device() != dev or v.get_device() != dev or g.get_device() != dev or beta.get_device() != dev \
+            or (state is not None and state.get_device() != dev):
+        raise ValueError(f"{name}: all tensors must be on the same CUDA device.")
+    if not q.is_cuda:
+        raise RuntimeError(f"{name} requires CUDA tensors.")
+    code = _DTYPES.get(dtype)
+    if code is None or k.dtype != dtype or v.dtype != dtype:
+        raise RuntimeError(f"{name}: q, k and v must all be float32 or all bfloat16.")
+    f32 = torch.float32
+    if g.dtype != f32 or beta.dtype != f32 or (state is not None and state.dtype != f32):
+        raise RuntimeError(f"{name}: g, beta and the state must be float32.")
+    ok = _supported.get(dev)
+    if ok is None:
+        ok = _supported[dev] = is_b200_available(dev)
+    if not ok:
+        raise RuntimeError("rnn_kernel_b200 requires a B200-class (sm_100) GPU.")
+    return code
+
+
+def _dense_heads(t):
+    """t itself if its last dimension is dense (other strides are free), else a contiguous copy."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _args(code, q, k, v, g, beta, state, scale):
+    """The C struct for [B, T, ...] tensors."""
+    B, T, Hk, dk = q.shape
+    Hv, dv = v.shape[2:]
+    return _lib.DELTA_ARGS.pack(code, B, T, Hk, Hv, dk, dv, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                g.data_ptr(), beta.data_ptr(), 0 if state is None else state.data_ptr(),
+                                *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *beta.stride())
+
+
+def _bytes(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def _forward(code, q, k, v, g, beta, state, scale):
+    """out, the last state and what the gradient needs besides the inputs."""
+    q, k, v = _dense_heads(q), _dense_heads(k), _dense_heads(v)
+    state = None if state is None else state.contiguous()
+    B, T, Hv, dv = v.shape
+    dev = q.device
+    lib = _lib.load()
+    a = _args(code, q, k, v, g, beta, state, scale)
+    with _lib.on_device(dev.index):
+        out = torch.empty(B, T, Hv, dv, dtype=v.dtype, device=dev)
+        last = torch.empty(B, Hv, q.shape[3], dv, device=dev)
+        stash, ws = _bytes(lib.gru_delta_stash_bytes(a), dev), _bytes(lib.gru_delta_workspace_bytes(a, 0), dev)
+        _lib.check(lib.gru_delta_forward(a, out.data_ptr(), last.data_ptr(), stash.data_ptr(), stash.numel(),
+                                         ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream),
+                   "gru_delta_forward")
+    return out, last, stash, (q, k, v)
+
+
+class GatedDeltaRuleFunction(torch.autograd.Function):
+    """``(q, k, v, g, beta, state or None, scale) -> (out, last state)``."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, state, scale):
+        code = _check("gated_delta_rule", q, k, v, g, beta, state, 2)
+        out, last, stash, (qd, kd, vd) = _forward(code, q, k, v, g, beta, state, scale)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(qd, kd, vd, g, beta, stash)
+        ctx.code, ctx.scale, ctx.has_state = code, scale, state is not None
+        return out, last
+
+    @staticmethod
+    def backward(ctx, dout, dlast):
+        q, k, v, g, beta, stash = ctx.saved_tensors
+        dev = q.device
+        lib = _lib.load()
+        with _lib.on_device(dev.index):
+            dout = None if dout is None else dout.contiguous()
+            dlast = None if dlast is None else dlast.contiguous()
+            a = _args(ctx.code, q, k, v, g, beta, None, ctx.scale)
+            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+            dg, dbeta = (torch.empty(t.shape, device=dev) for t in (g, beta))
+            ds = None
+            if ctx.has_state and ctx.needs_input_grad[5]:
+                ds = torch.empty(q.shape[0], v.shape[2], q.shape[3], v.shape[3], device=dev)
+            ws = _bytes(lib.gru_delta_workspace_bytes(a, 1), dev)
+            _lib.check(lib.gru_delta_backward(
+                a, None if dout is None else dout.data_ptr(), None if dlast is None else dlast.data_ptr(),
+                stash.data_ptr(), stash.numel(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
+                dbeta.data_ptr(), None if ds is None else ds.data_ptr(), ws.data_ptr(), ws.numel(),
+                torch.cuda.current_stream(dev).cuda_stream), "gru_delta_backward")
+        return dq, dk, dv, dg, dbeta, ds, None
+
+
+def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                     initial_state: Optional[torch.Tensor] = None, scale: Optional[float] = None):
+    """All tokens of a batch: ``(out [B, T, Hv, dv], last state [B, Hv, dk, dv])``.
+
+    ``q``, ``k``: [B, T, Hk, dk]; ``v``: [B, T, Hv, dv]; ``g`` (log of the decay, <= 0
+    in use; -inf forgets the state), ``beta``: [B, T, Hv].  ``scale`` defaults to
+    ``dk ** -0.5``.  Keys are used as given: normalise them for a stable rule.
+    The other strides than the last dimension's are free.
+    """
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if torch.is_grad_enabled():
+        return GatedDeltaRuleFunction.apply(q, k, v, g, beta, initial_state, scale)
+    code = _check("gated_delta_rule", q, k, v, g, beta, initial_state, 2)
+    out, last, _, _ = _forward(code, q, k, v, g, beta, initial_state, scale)
+    return out, last
+
+
+def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                     state: torch.Tensor, scale: Optional[float] = None) -> torch.Tensor:
+    """One token: ``out [B, Hv, dv]``; ``state`` [B, Hv, dk, dv] (contiguous) is updated in place.
+
+    ``q``, ``k``: [B, Hk, dk]; ``v``: [B, Hv, dv]; ``g``, ``beta``: [B, Hv].  No gradient.
+    """
+    code = _check("gated_delta_step", q, k, v, g, beta, state, 1)
+    if not state.is_contiguous():
+        raise ValueError("gated_delta_step: the state is updated in place and must be contiguous.")
+    q, k, v = _dense_heads(q), _dense_heads(k), _dense_heads(v)
+    B, Hk, dk = q.shape
+    Hv, dv = v.shape[1:]
+    dev = q.device
+    (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.stride(), k.stride(), v.stride()
+    (gb, gh), (bb, bh) = g.stride(), beta.stride()
+    a = _lib.DELTA_ARGS.pack(code, B, 1, Hk, Hv, dk, dv, dk ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(),
+                             v.data_ptr(), g.data_ptr(), beta.data_ptr(), 0, qb, 0, qh, kb, 0, kh, vb, 0, vh, gb, 0, gh,
+                             bb, 0, bh)
+    with _lib.on_device(dev.index):
+        out = torch.empty(B, Hv, dv, dtype=v.dtype, device=dev)
+        _lib.check(_lib.load().gru_delta_step(a, state.data_ptr(), out.data_ptr(),
+                                              torch.cuda.current_stream(dev).cuda_stream), "gru_delta_step")
+    torch.autograd.graph.increment_version(state)
+    return out
+
+
+class GatedDelta(nn.Module):
+    """A gated delta rule layer: ``(input [B, T, input_size], state) -> (output [B, T, output], state)``.
+
+    One projection makes q, k (L2-normalised), v, the decay and the writing
+    strength of every head; the heads' outputs, RMS-normalised per head, go
+    through an output projection back to ``output_size`` (default: the input's).
+    """
+
+    def __init__(self, input_size: int, num_heads: int = 4, head_size: int = 64, num_key_heads: Optional[int] = None,
+                 output_size: Optional[int] = None) -> None:
+        super().__init__()
+        num_key_heads = num_heads if num_key_heads is None else num_key_heads
+        if input_size < 1 or num_heads < 1 or num_key_heads < 1 or num_heads % num_key_heads:
+            raise ValueError("GatedDelta: num_heads must be a positive multiple of num_key_heads, input_size >= 1.")
+        if not 1 <= head_size <= MAX_HEAD_SIZE:
+            raise ValueError(f"GatedDelta: head_size must be in [1, {MAX_HEAD_SIZE}].")
+        self.input_size, self.num_heads, self.num_key_heads, self.head_size = input_size, num_heads, num_key_heads, head_size
+        self.output_size = input_size if output_size is None else output_size
+        self._split = (num_key_heads * head_size, num_key_heads * head_size, num_heads * head_size, num_heads, num_heads)
+        self.in_proj = nn.Linear(input_size, sum(self._split), bias=False)
+        self.out_proj = nn.Linear(num_heads * head_size, self.output_size, bias=False)
+        self.norm_weight = nn.Parameter(torch.ones(head_size))
+        # decays from a few tokens to a few hundred
+        self.log_rate = nn.Parameter(torch.linspace(-5.0, 0.0, num_heads))
+
+    def init_state(self, batch: int) -> torch.Tensor:
+        return torch.zeros(batch, self.num_heads, self.head_size, self.head_size, device=self.log_rate.device)
+
+    def _project(self, x):
+        q, k, v, a, b = self.in_proj(x).split(self._split, dim=-1)
+        keys, values = (self.num_key_heads, self.head_size), (self.num_heads, self.head_size)
+        q = F.normalize(q.unflatten(-1, keys).float(), dim=-1).to(x.dtype)
+        k = F.normalize(k.unflatten(-1, keys).float(), dim=-1).to(x.dtype)
+        g = -self.log_rate.float().exp() * F.softplus(a.float())
+        return q, k, v.unflatten(-1, values), g, b.float().sigmoid()
+
+    def _finish(self, o):
+        rms = o.float().square().mean(-1, keepdim=True).add(1e-6).rsqrt()
+        return self.out_proj((o * rms * self.norm_weight).to(o.dtype).flatten(-2))
+
+    def forward(self, x: torch.Tensor, state: Optional[torch.Tensor] = None):
+        if x.dim() != 3 or x.shape[-1] != self.input_size:
+            raise ValueError(f"x must have shape [batch, seq, {self.input_size}].")
+        o, last = gated_delta_rule(*self._project(x), initial_state=state)
+        return self._finish(o), last
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
+        """One token of every sequence, [batch, input_size]; ``state`` is updated in place."""
+        if x.dim() != 2 or x.shape[-1] != self.input_size:
+            raise ValueError(f"x must have shape [batch, {self.input_size}].")
+        return self._finish(gated_delta_step(*self._project(x), state))

@@ -1,0 +1,224 @@
+"""AdamW on the CUDA library: every tensor's step in one launch, moments in 32 or in 8 bits.
+
+The reference harness trains with ``torch.optim.AdamW`` (rnn_benchmark.py);
+:class:`AdamW` computes the same update (decoupled weight decay, bias
+correction) in FP32 for FP32 or bf16 weights::
+
+    m = b1 m + (1 - b1) g;   v = b2 v + (1 - b2) g^2
+    p = (1 - lr wd) p - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+``state_bits=8`` holds each moment in one byte: blocks of 256 elements share an
+FP32 scale, codes are logarithmic with 3 mantissa bits, and rounding is
+stochastic from ``(seed, step, position)``, so a run repeats bit for bit.  A
+block that meets a gradient that is not finite has NaN moments from then on,
+as 32-bit moments of those elements would.  CUDA tensors only; there is no
+fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Iterable, Optional
+
+import numpy as np
+import torch
+
+from . import _lib
+
+STATE_BLOCK = 256  # elements per 8-bit scale; every tensor's moments start a block
+
+_DTYPES = {torch.float32: _lib.GRU_F32, torch.bfloat16: _lib.GRU_BF16}
+# gru_adamw_tensor of include/rnn_kernel_b200.h
+_ENTRY = np.dtype([("param", "u8"), ("grad", "u8"), ("n", "i8"), ("state_offset", "i8"), ("decay", "f4"),
+                   ("step_size", "f4"), ("inv_sqrt_bc2", "f4"), ("pad", "f4")])
+
+
+def _at(array: np.ndarray) -> ctypes.c_void_p:
+    return ctypes.c_void_p(array.ctypes.data)
+
+
+class AdamW:
+    """``torch.optim.AdamW``'s update over all tensors at once.
+
+    ``params`` is an iterable of tensors, or of dicts with ``"params"`` and
+    optionally ``"lr"`` and ``"weight_decay"``; ``param_groups`` holds them, and
+    a schedule may set a group's ``"lr"`` between steps.  Parameters without a
+    gradient are skipped and keep their own step count.
+
+    ``capturable=True`` keeps the step count on the device, so that a step
+    captured in a CUDA graph advances with every replay; the learning rates
+    are those at capture, and every parameter needs its gradient.
+    """
+
+    def __init__(self, params: Iterable, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, state_bits: int = 32, seed: int = 0, capturable: bool = False) -> None:
+        if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
+            raise ValueError("betas must be in [0, 1).")
+        if not eps >= 0.0:
+            raise ValueError("eps must be >= 0.")
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32.")
+        self.betas, self.eps = (float(betas[0]), float(betas[1])), float(eps)
+        self.state_bits, self.seed, self.capturable = state_bits, int(seed) & 0xFFFFFFFF, bool(capturable)
+        groups = list(params)
+        if not groups:
+            raise ValueError("AdamW got no parameters.")
+        if not isinstance(groups[0], dict):
+            groups = [{"params": groups}]
+        self.param_groups = []
+        for g in groups:
+            ps = g["params"]
+            ps = [ps] if isinstance(ps, torch.Tensor) else list(ps)
+            group = {"params": ps, "lr": float(g.get("lr", lr)), "weight_decay": float(g.get("weight_decay", weight_decay))}
+            if not group["lr"] >= 0.0 or not group["weight_decay"] >= 0.0:
+                raise ValueError("lr and weight_decay must be >= 0.")
+            self.param_groups.append(group)
+        self.params = [p for g in self.param_groups for p in g["params"]]
+        if not self.params or len({id(p) for p in self.params}) != len(self.params):
+            raise ValueError("AdamW needs parameters, each of them once.")
+        for p in self.params:
+            if not isinstance(p, torch.Tensor) or not p.is_cuda or p.dtype not in _DTYPES:
+                raise RuntimeError("AdamW: FP32 or bf16 CUDA parameters are required.")
+            if not p.is_contiguous():
+                raise ValueError("AdamW: parameters must be contiguous.")
+        self.device = self.params[0].device
+        if any(p.device != self.device for p in self.params):
+            raise ValueError("AdamW: all parameters must be on the same CUDA device.")
+
+        sizes = np.array([p.numel() for p in self.params], dtype=np.int64)
+        ends = np.cumsum(-(-sizes // STATE_BLOCK) * STATE_BLOCK)
+        self.state_elems = int(ends[-1])
+        self._offsets = np.concatenate([np.zeros(1, np.int64), ends[:-1]])
+        self._sizes = sizes
+        n = max(self.state_elems, STATE_BLOCK)
+        kind = torch.float32 if state_bits == 32 else torch.uint8
+        self.exp_avg = torch.zeros(n, dtype=kind, device=self.device)[:self.state_elems]
+        self.exp_avg_sq = torch.zeros(n, dtype=kind, device=self.device)[:self.state_elems]
+        self.scale_avg = self.scale_sq = None
+        if state_bits == 8:
+            self.scale_avg = torch.zeros(n // STATE_BLOCK, device=self.device)
+            self.scale_sq = torch.zeros(n // STATE_BLOCK, device=self.device)
+        self._calls = 0
+        self._steps = np.zeros(len(self.params), dtype=np.int64)
+        self._device_step = torch.zeros(1, dtype=torch.int64, device=self.device) if capturable else None
+        self._scalars = torch.zeros(3, device=self.device) if capturable else None
+        group_of = [i for i, g in enumerate(self.param_groups) for _ in g["params"]]
+        self._tables = []
+        for dt, code in _DTYPES.items():
+            index = np.array([i for i, p in enumerate(self.params) if p.dtype == dt], dtype=np.int64)
+            if not index.size:
+                continue
+            table = np.zeros(index.size, dtype=_ENTRY)
+            table["n"], table["state_offset"] = sizes[index], self._offsets[index]
+            self._tables.append((dt, code, index, [self.params[i] for i in index], table,
+                                 np.array(group_of, dtype=np.int64)[index]))
+
+    def _gradients(self, dt, params, table):
+        """Fills the table's addresses; returns the mask of parameters that have a gradient, None where all have."""
+        ptrs = [p.data_ptr() for p in params]
+        if ptrs != table["param"].tolist():
+            for p, n in zip(params, table["n"].tolist()):
+                if p.dtype != dt or p.numel() != n or p.device != self.device or not p.is_contiguous():
+                    raise RuntimeError("AdamW: a parameter's type, size, device or layout has changed.")
+            table["param"] = ptrs
+        grads = [p.grad for p in params]
+        mask = None
+        if None in [g if g is None else 0 for g in grads]:
+            mask = np.array([g is not None for g in grads])
+        grads = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
+        for g in grads:
+            if g is not None and (g.dtype is not dt or g.layout is not torch.strided):
+                raise RuntimeError("AdamW: gradients must be dense and of their parameter's type.")
+        table["grad"] = [0 if g is None else g.data_ptr() for g in grads]
+        return mask, grads
+
+    @torch.no_grad()
+    def step(self, grad_scale: float = 1.0) -> None:
+        """Updates the parameters in place from their ``.grad`` times ``grad_scale``."""
+        lib = _lib.load()
+        b1, b2 = self.betas
+        filled = [self._gradients(t[0], t[3], t[4]) for t in self._tables]
+        if self.capturable and any(mask is not None for mask, _ in filled):
+            raise RuntimeError("AdamW(capturable=True): every parameter needs a gradient.")
+        self._calls += 1
+        lrs = np.array([g["lr"] for g in self.param_groups])
+        decay = 1.0 - lrs * np.array([g["weight_decay"] for g in self.param_groups])
+        dev = self.device.index
+        counted = self._device_step
+        with _lib.on_device(dev):
+            stream = torch.cuda.current_stream(dev).cuda_stream
+            for (dt, code, index, _, table, group), (mask, _keep) in zip(self._tables, filled):
+                if mask is not None:
+                    index, table, group = index[mask], table[mask], group[mask]
+                    if not index.size:
+                        continue
+                table["decay"] = decay[group]
+                if self.capturable:
+                    table["step_size"] = lrs[group]
+                else:
+                    self._steps[index] += 1
+                    t = self._steps[index]
+                    table["step_size"] = lrs[group] / (1.0 - b1 ** t)
+                    table["inv_sqrt_bc2"] = 1.0 / np.sqrt(1.0 - b2 ** t)
+                _lib.check(lib.gru_adamw_step(
+                    _at(table), len(table), code, self.state_bits, self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
+                    self.scale_avg.data_ptr() if self.scale_avg is not None else None,
+                    self.scale_sq.data_ptr() if self.scale_sq is not None else None, self.state_elems, b1, b2, self.eps,
+                    float(grad_scale), self.seed, self._calls, None if counted is None else counted.data_ptr(),
+                    None if self._scalars is None else self._scalars.data_ptr(), stream), "gru_adamw_step")
+                counted = None  # counted once for all element types
+        torch.autograd.graph.increment_version(self.params)
+
+    def zero_grad(self, set_to_none: bool = True) -> None:
+        for p in self.params:
+            if p.grad is not None:
+                if set_to_none:
+                    p.grad = None
+                else:
+                    p.grad.zero_()
+
+    def moments(self):
+        """Both moments as FP32 buffers: tensor i's at ``[offset_i, offset_i + numel_i)`` (:meth:`offsets`), zeros
+        between.  32-bit moments are the optimizer's own buffers, 8-bit ones are decoded into new ones."""
+        if self.state_bits == 32:
+            return self.exp_avg, self.exp_avg_sq
+        m = torch.empty(self.state_elems, device=self.device)
+        v = torch.empty(self.state_elems, device=self.device)
+        dev = self.device.index
+        with _lib.on_device(dev):
+            _lib.check(_lib.load().gru_adamw_decode(
+                self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), self.scale_avg.data_ptr(), self.scale_sq.data_ptr(),
+                self.state_elems, m.data_ptr(), v.data_ptr(), torch.cuda.current_stream(dev).cuda_stream),
+                "gru_adamw_decode")
+        return m, v
+
+    def offsets(self):
+        """(offset, elements) of each parameter's moments in :meth:`moments`' buffers, in order."""
+        return list(zip(self._offsets.tolist(), self._sizes.tolist()))
+
+    def state_dict(self) -> dict:
+        """What continues this run bit for bit: moments as they are held, counts, and the groups' rates."""
+        calls = self._calls if self._device_step is None else int(self._device_step)
+        steps = self._steps.tolist() if self._device_step is None else [calls] * len(self.params)
+        return {"state_bits": self.state_bits, "seed": self.seed, "sizes": self._sizes.tolist(), "calls": calls,
+                "steps": steps, "exp_avg": self.exp_avg.clone(), "exp_avg_sq": self.exp_avg_sq.clone(),
+                "scale_avg": None if self.scale_avg is None else self.scale_avg.clone(),
+                "scale_sq": None if self.scale_sq is None else self.scale_sq.clone(),
+                "groups": [{"lr": g["lr"], "weight_decay": g["weight_decay"]} for g in self.param_groups]}
+
+    @torch.no_grad()
+    def load_state_dict(self, state: dict) -> None:
+        if state["state_bits"] != self.state_bits or list(state["sizes"]) != self._sizes.tolist() \
+                or len(state["groups"]) != len(self.param_groups):
+            raise ValueError("AdamW: the state belongs to other parameters or another state_bits.")
+        if self._device_step is not None:
+            if any(t != state["calls"] for t in state["steps"]):
+                raise ValueError("AdamW(capturable=True): the state's parameters have different step counts.")
+            self._device_step.fill_(state["calls"])
+        self._calls, self.seed = int(state["calls"]), int(state["seed"])
+        self._steps[:] = state["steps"]
+        for name in ("exp_avg", "exp_avg_sq", "scale_avg", "scale_sq"):
+            mine: Optional[torch.Tensor] = getattr(self, name)
+            if mine is not None:
+                mine.copy_(state[name])
+        for g, s in zip(self.param_groups, state["groups"]):
+            g.update(lr=float(s["lr"]), weight_decay=float(s["weight_decay"]))

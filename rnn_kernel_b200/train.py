@@ -13,7 +13,8 @@ layer's gradients into that buffer in place, so a step is::
     flat_params.add_(grad, alpha=-lr / world)  # SGD on the mean gradient
 
 i.e. one collective and one fused update kernel per step, independent of the
-number of layers.  With ``overlap=True`` (default) and several layers, the
+number of layers (``optimizer="adamw"``: :class:`AdamW`'s one launch instead of
+the SGD update).  With ``overlap=True`` (default) and several layers, the
 gradient buffer is reduced per layer instead: each layer's slice is
 all-reduced asynchronously as soon as autograd has accumulated all of its
 gradients (a post-accumulate-grad hook per parameter), so the upper layers'
@@ -32,6 +33,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .loss import mse_loss
+from .optim import AdamW
 
 
 def flatten_parameters_(module: nn.Module):
@@ -55,15 +57,28 @@ def flatten_parameters_(module: nn.Module):
 
 
 class DataParallelTrainer:
-    """SGD data-parallel trainer: shard-local fwd/bwd, one all-reduce, one update."""
+    """Data-parallel trainer: shard-local fwd/bwd, one all-reduce, one update.
+
+    ``optimizer`` is ``"sgd"`` or ``"adamw"`` (:class:`AdamW` on the flat
+    parameter buffer, CUDA only; ``weight_decay`` and ``state_bits`` are its).
+    """
 
     def __init__(self, module: nn.Module, lr: float = 1e-2,
-                 process_group: Optional[dist.ProcessGroup] = None, overlap: bool = True) -> None:
+                 process_group: Optional[dist.ProcessGroup] = None, overlap: bool = True,
+                 optimizer: str = "sgd", weight_decay: float = 1e-2, state_bits: int = 32) -> None:
+        if optimizer not in ("sgd", "adamw"):
+            raise ValueError('optimizer must be "sgd" or "adamw".')
         self.module = module
         self.lr = float(lr)
         self.group = process_group
         self.world = dist.get_world_size(process_group) if dist.is_available() and dist.is_initialized() else 1
         self.flat, self.grad = flatten_parameters_(module)
+        self.optimizer = None
+        if optimizer == "adamw":
+            # the step count lives on the device, so that a captured step advances with every replay
+            self.flat.grad = self.grad
+            self.optimizer = AdamW([self.flat], lr=self.lr, weight_decay=weight_decay, state_bits=state_bits,
+                                   capturable=True)
         self._buckets: list = []   # [lo, hi) slices of the gradient buffer, one per layer
         self._pending: list = []   # parameters of each bucket not yet accumulated this step
         self._works: list = []
@@ -140,7 +155,7 @@ class DataParallelTrainer:
         return loss.detach()
 
     def reduce_and_update(self) -> None:
-        """Finish the gradient all-reduce and apply the SGD update."""
+        """Finish the gradient all-reduce and apply the update."""
         if self.world > 1 and self.overlap_active:
             for w in self._works:
                 w.wait()
@@ -151,6 +166,9 @@ class DataParallelTrainer:
             self._works = []
         elif self.world > 1:
             dist.all_reduce(self.grad, op=dist.ReduceOp.SUM, group=self.group)
+        if self.optimizer is not None:
+            self.optimizer.step(grad_scale=1.0 / self.world)
+            return
         with torch.no_grad():
             self.flat.add_(self.grad, alpha=-self.lr / self.world)
 
