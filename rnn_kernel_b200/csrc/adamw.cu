@@ -6,7 +6,7 @@
 // in FP32 whatever the weights' type (FP32 or bf16, rounded once when stored).
 // All tensors' moments live in one buffer each, in which every tensor starts at
 // a multiple of 256 elements (one quantisation block); a CTA updates 2048
-// consecutive elements of one tensor, a warp one block, a lane 2 x 4 elements,
+// (with 8-bit moments up to 16384) consecutive elements of one tensor, a warp a block at a time, a lane 2 x 4 elements,
 // so every access is a coalesced 16-byte one (8 for bf16, 4 for codes).  The
 // tensor table travels in the kernel's parameters: no copy, no device table.
 //
@@ -40,7 +40,7 @@ namespace {
 
 constexpr int kBlock = 256;         // elements per quantisation block = per warp
 constexpr int kThreads = 256;
-constexpr int kChunk = kBlock * (kThreads / 32);  // elements per CTA
+constexpr int kRow = kBlock * (kThreads / 32);  // elements that a CTA's warps take at a time
 constexpr float kInvTop = (float)(1.0 / 1.875);  // the largest code stands for 1.875 scales
 
 struct Entry {
@@ -70,46 +70,54 @@ struct Common {
   float b1, omb1, b2, omb2, eps, gscale;
   unsigned key;
   int count;
+  int rows;  // kRow elements that a CTA takes, one after the other
 };
 
 __device__ __forceinline__ float code_value(unsigned low, int ebits) {
   return low ? __uint_as_float((low << 20) + ((128u - (1u << ebits)) << 23)) : 0.0f;
 }
 
-__device__ __forceinline__ float decode_m(unsigned c, float scale) {
+__device__ __forceinline__ float value_m(unsigned c) {
   const float x = code_value(c & 0x7fu, 4);
-  return __fmul_rn((c & 0x80u) ? -x : x, scale);
+  return (c & 0x80u) ? -x : x;
+}
+__device__ __forceinline__ float value_v(unsigned c) { return code_value(c, 5); }
+__device__ __forceinline__ float decode_m(unsigned c, float scale) { return __fmul_rn(value_m(c), scale); }
+__device__ __forceinline__ float decode_v(unsigned c, float scale) { return __fmul_rn(value_v(c), scale); }
+
+// The larger of two magnitudes; a NaN wins.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
 }
 
-__device__ __forceinline__ float decode_v(unsigned c, float scale) { return __fmul_rn(code_value(c, 5), scale); }
-
-// 32 random bits of a position: 16 for each moment.
-__device__ __forceinline__ unsigned noise_bits(long i, unsigned key) {
-  unsigned h = (unsigned)i * 0x9E3779B1u + key + (unsigned)((unsigned long long)i >> 32) * 0xC2B2AE3Du;
+// 32 random bits of a position, 16 for each moment.  noise_base is linear in
+// the position (inside a block, whose elements share their upper 32 bits).
+__device__ __forceinline__ unsigned noise_base(long i, unsigned key) {
+  return (unsigned)i * 0x9E3779B1u + key + (unsigned)((unsigned long long)i >> 32) * 0xC2B2AE3Du;
+}
+__device__ __forceinline__ unsigned noise_bits(unsigned h) {
   h = (h ^ (h >> 15)) * 0xB5297A4Du;
   h = (h ^ (h >> 13)) * 0x68E31DA5u;
   return h ^ (h >> 16);
 }
 
-// The code whose value is r rounded up or down at random (16 random bits
-// below the 3 mantissa bits; the 4 bits below those are truncated).
-__device__ __forceinline__ int round_code(float r, unsigned n16, int ebits) {
-  const int c = (int)((__float_as_uint(r) + (n16 << 4)) >> 20) - (int)((128u - (1u << ebits)) << 3);
-  return min(c, (1 << (ebits + 3)) - 1);
+// The code whose value is r rounded up or down at random, from 16 random bits
+// (shifted to `noise`) below the 3 mantissa bits; the 4 bits below those are
+// truncated.  Below 1 where r is below the least code.
+__device__ __forceinline__ int round_code(float r, unsigned noise, int ebits) {
+  const unsigned base = (128u - (1u << ebits)) << 23;
+  return min((int)(__float_as_uint(r) + noise - base) >> 20, (1 << (ebits + 3)) - 1);
 }
 
-__device__ __forceinline__ unsigned encode_m(float m, float inv, unsigned n16) {
-  constexpr float least = 1.125f / 32768.0f;
-  const float r = __fmul_rn(fabsf(m), inv);
-  int c = round_code(r, n16, 4);
-  if (r < least) c = r > __fmul_rn((float)n16, least / 65536.0f) ? 1 : 0;
-  return (unsigned)c | (m < 0.0f ? 0x80u : 0u);
-}
+constexpr float kLeast = 1.125f / 32768.0f;  // the least first moment that a code stands for
 
-__device__ __forceinline__ unsigned encode_v(float v, float inv, unsigned n16) {
-  const float r = __fmul_rn(v, inv);
-  const int c = max(round_code(r, n16, 5), 1);
-  return r > 0.0f ? (unsigned)c : 0u;
+// A first moment below that: the least code or zero, at random.
+__device__ __forceinline__ int round_least(float r, unsigned n16) {
+  // n16 / 65536, exactly, without the slow integer conversion
+  const float u = __uint_as_float(0x3f800000u | (n16 << 7)) - 1.0f;
+  return r > __fmul_rn(u, kLeast) ? 1 : 0;
 }
 
 // A block's scale from the warp's largest magnitude (as bits: for
@@ -120,11 +128,13 @@ __device__ __forceinline__ float block_scale(unsigned amax_bits) {
   return s < 0x1p-100f ? 0.0f : s;
 }
 
+// Four consecutive elements: `vec` where all four exist and one access can
+// take them, else those of them that exist (zeros for the others).
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, long left, int vec, float (&x)[4]);
+__device__ __forceinline__ void load4(const T* p, int left, bool vec, float (&x)[4]);
 template <>
-__device__ __forceinline__ void load4<float>(const float* p, long left, int vec, float (&x)[4]) {
-  if (vec && left >= 4) {
+__device__ __forceinline__ void load4<float>(const float* p, int left, bool vec, float (&x)[4]) {
+  if (vec) {
     const float4 f = __ldcs(reinterpret_cast<const float4*>(p));
     x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
   } else {
@@ -133,8 +143,8 @@ __device__ __forceinline__ void load4<float>(const float* p, long left, int vec,
   }
 }
 template <>
-__device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16* p, long left, int vec, float (&x)[4]) {
-  if (vec && left >= 4) {
+__device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16* p, int left, bool vec, float (&x)[4]) {
+  if (vec) {
     const uint2 u = __ldcs(reinterpret_cast<const uint2*>(p));
     x[0] = __uint_as_float(u.x << 16), x[1] = __uint_as_float(u.x & 0xffff0000u);
     x[2] = __uint_as_float(u.y << 16), x[3] = __uint_as_float(u.y & 0xffff0000u);
@@ -145,10 +155,10 @@ __device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16* p, lon
 }
 
 template <typename T>
-__device__ __forceinline__ void store4(T* p, long left, int vec, const float (&x)[4]);
+__device__ __forceinline__ void store4(T* p, int left, bool vec, const float (&x)[4]);
 template <>
-__device__ __forceinline__ void store4<float>(float* p, long left, int vec, const float (&x)[4]) {
-  if (vec && left >= 4) {
+__device__ __forceinline__ void store4<float>(float* p, int left, bool vec, const float (&x)[4]) {
+  if (vec) {
     __stcs(reinterpret_cast<float4*>(p), make_float4(x[0], x[1], x[2], x[3]));
   } else {
 #pragma unroll
@@ -157,8 +167,8 @@ __device__ __forceinline__ void store4<float>(float* p, long left, int vec, cons
   }
 }
 template <>
-__device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16* p, long left, int vec, const float (&x)[4]) {
-  if (vec && left >= 4) {
+__device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16* p, int left, bool vec, const float (&x)[4]) {
+  if (vec) {
     const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
     uint2 u;
     u.x = *reinterpret_cast<const unsigned*>(&a);
@@ -171,10 +181,41 @@ __device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16* p, long lef
   }
 }
 
+// The step's square root and quotient.  With 8-bit moments the kernel is near
+// its instruction limit (86 slots an element at copy bandwidth), so it takes
+// the hardware's approximations, good to 2 ulp of a step that the moments
+// themselves know to 4 bits; codes and scales do not depend on them.
+template <int kBits>
+__device__ __forceinline__ float root(float x) {
+  if (kBits == 32) return __fsqrt_rn(x);
+  float y;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <int kBits>
+__device__ __forceinline__ float ratio(float x, float y) {
+  if (kBits == 32) return __fdiv_rn(x, y);
+  float z;  // y is a normal number, or zero where v and eps are
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(z) : "f"(y));
+  return __fmul_rn(x, z);
+}
+
 // kBits: 32 or 8.
+//
+// What bounds it: memory with 32-bit moments; with 8-bit ones the integer pipe
+// (two instructions a cycle and SM) comes close: the codes' values come from
+// a table in shared memory instead of integer arithmetic, codes are packed by
+// multiply-adds (another pipe), and a first moment below the least code is the
+// rare case of a branch over a lane's eight elements.
 template <typename T, int kBits, int N>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<N> tab,
+__global__ void __launch_bounds__(kThreads, kBits == 8 ? 5 : 4) adamw_kernel(const __grid_constant__ Table<N> tab,
                                                          const __grid_constant__ Common c) {
+  __shared__ float lut[kBits == 8 ? 512 : 1];
+  if (kBits == 8) {
+    lut[threadIdx.x] = value_m(threadIdx.x);
+    lut[256 + threadIdx.x] = value_v(threadIdx.x);
+    __syncthreads();
+  }
   // the last tensor whose first CTA is not after this one
   int lo = 0, hi = c.count - 1;
   while (lo < hi) {
@@ -183,38 +224,6 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
   }
   const Entry& e = tab.e[lo];
   const int lane = threadIdx.x & 31;
-  // first element of this warp's block, in the tensor and in the moments
-  const long at = (long)(blockIdx.x - e.chunk) * kChunk + (threadIdx.x >> 5) * kBlock;
-  if (at >= e.n) return;
-  const long so = e.off + at;
-
-  float p[2][4], g[2][4], m[2][4], v[2][4];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const long i = at + h * 128 + lane * 4;
-    load4<T>(static_cast<const T*>(e.g) + i, e.n - i, e.vec, g[h]);
-    load4<T>(static_cast<const T*>(e.p) + i, e.n - i, e.vec, p[h]);
-    if (kBits == 32) {
-      load4<float>(static_cast<const float*>(c.m) + so + h * 128 + lane * 4, 4, 1, m[h]);
-      load4<float>(static_cast<const float*>(c.v) + so + h * 128 + lane * 4, 4, 1, v[h]);
-    }
-  }
-  if (kBits == 8) {
-    unsigned cm[2], cv[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      cm[h] = reinterpret_cast<const unsigned*>(static_cast<const unsigned char*>(c.m) + so)[h * 32 + lane];
-      cv[h] = reinterpret_cast<const unsigned*>(static_cast<const unsigned char*>(c.v) + so)[h * 32 + lane];
-    }
-    const float sm = c.sm[so / kBlock], sv = c.sv[so / kBlock];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        m[h][i] = decode_m((cm[h] >> (8 * i)) & 0xffu, sm);
-        v[h][i] = decode_v((cv[h] >> (8 * i)) & 0xffu, sv);
-      }
-  }
   float step = e.step, inv_bc2 = e.inv_bc2;
   unsigned key = c.key;
   if (c.scal) {
@@ -222,47 +231,114 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     inv_bc2 = c.scal[1];
     key = __float_as_uint(c.scal[2]);
   }
-  unsigned am = 0, av = 0;
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float gg = __fmul_rn(g[h][i], c.gscale);
-      m[h][i] = __fadd_rn(__fmul_rn(m[h][i], c.b1), __fmul_rn(gg, c.omb1));
-      v[h][i] = __fadd_rn(__fmul_rn(v[h][i], c.b2), __fmul_rn(__fmul_rn(gg, gg), c.omb2));
-      const float den = __fadd_rn(__fmul_rn(__fsqrt_rn(v[h][i]), inv_bc2), c.eps);
-      p[h][i] = __fsub_rn(__fmul_rn(p[h][i], e.decay), __fdiv_rn(__fmul_rn(m[h][i], step), den));
-      am = max(am, __float_as_uint(m[h][i]) & 0x7fffffffu);
-      av = max(av, __float_as_uint(v[h][i]) & 0x7fffffffu);
-    }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const long i = at + h * 128 + lane * 4;
-    store4<T>(static_cast<T*>(e.p) + i, e.n - i, e.vec, p[h]);
-    if (kBits == 32) {
-      // the elements between the tensor's end and its block's are zero: g is
-      store4<float>(static_cast<float*>(c.m) + so + h * 128 + lane * 4, 4, 1, m[h]);
-      store4<float>(static_cast<float*>(c.v) + so + h * 128 + lane * 4, 4, 1, v[h]);
-    }
-  }
-  if (kBits == 8) {
-    const float sm = block_scale(am), sv = block_scale(av);
-    const float im = sm == 0.0f ? 0.0f : __frcp_rn(sm), iv = sv == 0.0f ? 0.0f : __frcp_rn(sv);
+#pragma unroll 1
+  for (int w = 0; w < c.rows; ++w) {
+    // first element of this warp's block, in the tensor and in the moments
+    const long at = ((long)(blockIdx.x - e.chunk) * c.rows + w) * kRow + (threadIdx.x >> 5) * kBlock;
+    if (at >= e.n) return;
+    const long so = e.off + at;
+
+    float p[2][4], g[2][4], m[2][4], v[2][4];
+    const int there = (int)min((long)kBlock, e.n - at);
+    const bool vec = e.vec && there == kBlock;  // the same for the whole warp
+    T* bp = static_cast<T*>(e.p) + at + lane * 4;
+    const T* bg = static_cast<const T*>(e.g) + at + lane * 4;
+    float* fm = static_cast<float*>(c.m) + so + lane * 4;
+    float* fv = static_cast<float*>(c.v) + so + lane * 4;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      unsigned cm = 0, cv = 0;
+      load4<T>(bg + h * 128, there - h * 128 - lane * 4, vec, g[h]);
+      load4<T>(bp + h * 128, there - h * 128 - lane * 4, vec, p[h]);
+      if (kBits == 32) {
+        load4<float>(fm + h * 128, 4, true, m[h]);
+        load4<float>(fv + h * 128, 4, true, v[h]);
+      }
+    }
+    unsigned* bm = reinterpret_cast<unsigned*>(static_cast<unsigned char*>(c.m) + so) + lane;
+    unsigned* bv = reinterpret_cast<unsigned*>(static_cast<unsigned char*>(c.v) + so) + lane;
+    if (kBits == 8) {
+      unsigned cm[2], cv[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        cm[h] = bm[h * 32];
+        cv[h] = bv[h * 32];
+      }
+      const float sm = c.sm[so / kBlock], sv = c.sv[so / kBlock];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          m[h][i] = __fmul_rn(lut[(cm[h] >> (8 * i)) & 0xffu], sm);
+          v[h][i] = __fmul_rn(lut[256 + ((cv[h] >> (8 * i)) & 0xffu)], sv);
+        }
+    }
+    float am = 0.0f, av = 0.0f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const unsigned r = noise_bits(so + h * 128 + lane * 4 + i, key);
-        cm |= encode_m(m[h][i], im, r >> 16) << (8 * i);
-        cv |= encode_v(v[h][i], iv, r & 0xffffu) << (8 * i);
+        const float gg = __fmul_rn(g[h][i], c.gscale);
+        m[h][i] = __fadd_rn(__fmul_rn(m[h][i], c.b1), __fmul_rn(gg, c.omb1));
+        v[h][i] = __fadd_rn(__fmul_rn(v[h][i], c.b2), __fmul_rn(__fmul_rn(gg, gg), c.omb2));
+        const float den = __fadd_rn(__fmul_rn(root<kBits>(v[h][i]), inv_bc2), c.eps);
+        p[h][i] = __fsub_rn(__fmul_rn(p[h][i], e.decay), ratio<kBits>(__fmul_rn(m[h][i], step), den));
+        if (kBits == 8) {
+          am = max_nan(am, fabsf(m[h][i]));
+          av = max_nan(av, v[h][i]);
+        }
       }
-      reinterpret_cast<unsigned*>(static_cast<unsigned char*>(c.m) + so)[h * 32 + lane] = cm;
-      reinterpret_cast<unsigned*>(static_cast<unsigned char*>(c.v) + so)[h * 32 + lane] = cv;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      store4<T>(bp + h * 128, there - h * 128 - lane * 4, vec, p[h]);
+      if (kBits == 32) {
+        // the elements between the tensor's end and its block's are zero: g is
+        store4<float>(fm + h * 128, 4, true, m[h]);
+        store4<float>(fv + h * 128, 4, true, v[h]);
+      }
     }
-    if (lane == 0) {
-      c.sm[so / kBlock] = sm;
-      c.sv[so / kBlock] = sv;
+    if (kBits == 8) {
+      const float sm = block_scale(__float_as_uint(am)), sv = block_scale(__float_as_uint(av));
+      const float im = sm == 0.0f ? 0.0f : __frcp_rn(sm), iv = sv == 0.0f ? 0.0f : __frcp_rn(sv);
+      int km[2][4];
+      unsigned rnd[2][4];
+      bool low = false;
+      const unsigned base = noise_base(so + lane * 4, key);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        unsigned cv = 0;
+#pragma unroll
+        for (int i = 3; i >= 0; --i) {
+          rnd[h][i] = noise_bits(base + (unsigned)(h * 128 + i) * 0x9E3779B1u);
+          const float r = __fmul_rn(fabsf(m[h][i]), im), q = __fmul_rn(v[h][i], iv);
+          km[h][i] = round_code(r, (rnd[h][i] >> 12) & 0xffff0u, 4);
+          low |= r < kLeast;
+          // a nonzero second moment is never coded as zero: it divides
+          const int k = max(round_code(q, (rnd[h][i] << 4) & 0xffff0u, 5), (int)min(__float_as_uint(q), 1u));
+          cv = cv * 256u + (unsigned)k;
+        }
+        bv[h * 32] = cv;
+      }
+      if (low) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float r = __fmul_rn(fabsf(m[h][i]), im);
+            if (r < kLeast) km[h][i] = round_least(r, rnd[h][i] >> 16);
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        unsigned cm = 0;
+#pragma unroll
+        for (int i = 3; i >= 0; --i)
+          cm = cm * 256u + ((unsigned)km[h][i] | ((__float_as_uint(m[h][i]) >> 24) & 0x80u));
+        bm[h * 32] = cm;
+      }
+      if (lane == 0) {
+        c.sm[so / kBlock] = sm;
+        c.sv[so / kBlock] = sv;
+      }
     }
   }
 }
@@ -311,7 +387,7 @@ int run(const gru_adamw_tensor* ts, int count, Common c, cudaStream_t stream) {
   long ctas = 0;
   for (int i = 0; i < count; ++i) {
     if (ts[i].n == 0) continue;
-    const long need = (ts[i].n + kChunk - 1) / kChunk;
+    const long chunk = (long)kRow * c.rows, need = (ts[i].n + chunk - 1) / chunk;
     if (k == N || ctas + need > (1L << 30)) {
       c.count = k;
       if (const int rc = launch<T, kBits, N>(t, c, (int)ctas, stream)) return rc;
@@ -327,12 +403,12 @@ int run(const gru_adamw_tensor* ts, int count, Common c, cudaStream_t stream) {
   return launch<T, kBits, N>(t, c, (int)ctas, stream);
 }
 
-// Tables of 32 tensors (1.8 KB of kernel parameters) or of 512 (28 KB, of
-// the 32 KB a launch may carry): a launch's parameters are copied whole.
+// Tables of 32 tensors (1.8 KB of kernel parameters) or of 256 (14 KB): a
+// launch's parameters are copied whole, so a few tensors get the small one.
 template <typename T, int kBits>
 int run_sized(const gru_adamw_tensor* ts, int count, const Common& c, cudaStream_t stream) {
   if (count <= 32) return run<T, kBits, 32>(ts, count, c, stream);
-  return run<T, kBits, 512>(ts, count, c, stream);
+  return run<T, kBits, 256>(ts, count, c, stream);
 }
 
 }  // namespace
@@ -361,7 +437,7 @@ extern "C" int gru_adamw_step(const gru_adamw_tensor* tensors, int count, int dt
     set_error("gru_adamw_step: device_step needs device_scalars");
     return GRU_ERR_INVALID;
   }
-  bool any = false;
+  long total = 0;
   for (int i = 0; i < count; ++i) {
     const gru_adamw_tensor& t = tensors[i];
     if (t.n < 0 || (t.n > 0 && (!t.param || !t.grad))) {
@@ -378,9 +454,9 @@ extern "C" int gru_adamw_step(const gru_adamw_tensor* tensors, int count, int dt
       set_error("gru_adamw_step: a tensor's moments must start at a multiple of 256 and end inside the buffers");
       return GRU_ERR_INVALID;
     }
-    any = any || t.n > 0;
+    total += t.n;
   }
-  if (any && (!exp_avg || !exp_avg_sq || (state_bits == 8 && (!scale_avg || !scale_sq)) || state_elems % kBlock != 0 ||
+  if (total > 0 && (!exp_avg || !exp_avg_sq || (state_bits == 8 && (!scale_avg || !scale_sq)) || state_elems % kBlock != 0 ||
               !aligned(exp_avg, 16) || !aligned(exp_avg_sq, 16))) {
     set_error("gru_adamw_step: moments (and 8-bit scales) must be non-null, 16-byte aligned, a multiple of 256 long");
     return GRU_ERR_INVALID;
@@ -391,10 +467,17 @@ extern "C" int gru_adamw_step(const gru_adamw_tensor* tensors, int count, int dt
     adamw_scalars_kernel<<<1, 1, 0, stream>>>(device_step, beta1, beta2, seed, device_scalars);
     GRU_CUDA_TRY(cudaGetLastError());
   }
-  if (!any) return GRU_OK;
+  if (total == 0) return GRU_OK;
+  // With 8-bit moments a CTA first builds its decoding table, so a large step
+  // lets it take up to eight rows while two waves of CTAs remain (201 M
+  // weights: 1027 us with eight rows, 1074 with one); a small one, and 32-bit
+  // moments, spread over as many CTAs as there are.
+  const long all = total / (kRow * 2L * 5 * 148);
+  const int rows = state_bits == 8 ? (int)std::min(std::max(all, 1L), 8L) : 1;
   const Common c{exp_avg, exp_avg_sq, scale_avg, scale_sq, device_scalars, (float)beta1, (float)(1.0 - beta1),
-                 (float)beta2, (float)(1.0 - beta2), (float)eps, (float)grad_scale,
-                 seed * 0x8DA6B343u + (unsigned)step * 0xD8163841u, 0};
+                 (float)beta2, (float)(1.0 - beta2), eps > 0.0 ? std::max((float)eps, 1.17549435e-38f) : 0.0f,
+                 (float)grad_scale,
+                 seed * 0x8DA6B343u + (unsigned)step * 0xD8163841u, 0, rows};
   if (dtype == GRU_F32)
     return state_bits == 32 ? run_sized<float, 32>(tensors, count, c, stream)
                             : run_sized<float, 8>(tensors, count, c, stream);

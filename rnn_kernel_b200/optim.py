@@ -16,7 +16,8 @@ fallback.
 """
 from __future__ import annotations
 
-import ctypes
+import math
+import operator
 from typing import Iterable, Optional
 
 import numpy as np
@@ -32,8 +33,49 @@ _ENTRY = np.dtype([("param", "u8"), ("grad", "u8"), ("n", "i8"), ("state_offset"
                    ("step_size", "f4"), ("inv_sqrt_bc2", "f4"), ("pad", "f4")])
 
 
-def _at(array: np.ndarray) -> ctypes.c_void_p:
-    return ctypes.c_void_p(array.ctypes.data)
+_address = torch.Tensor.data_ptr
+_is_dense = torch.Tensor.is_contiguous
+_gradient, _dtype = operator.attrgetter("grad"), operator.attrgetter("dtype")
+
+
+class _TypeTable:
+    """The C call's table of the parameters of one element type."""
+
+    def __init__(self, opt: "AdamW", dt: torch.dtype, group_of: np.ndarray) -> None:
+        self.dtype, self.code = dt, _DTYPES[dt]
+        self.index = np.array([i for i, p in enumerate(opt.params) if p.dtype == dt], dtype=np.int64)
+        self.params = [opt.params[i] for i in self.index]
+        self.group = group_of[self.index]
+        cuts = [0] + (np.flatnonzero(np.diff(self.group)) + 1).tolist() + [len(self.index)]
+        self.groups = [(lo, hi, int(self.group[lo])) for lo, hi in zip(cuts[:-1], cuts[1:])]
+        self.entries = np.zeros(len(self.index), dtype=_ENTRY)
+        self.entries["n"], self.entries["state_offset"] = opt._sizes[self.index], opt._offsets[self.index]
+        self.addresses: list = []  # of the parameters, as in the entries
+        self.copies = None         # dense copies of gradients that are not, until the launch
+
+    def gather(self, device: torch.device) -> Optional[np.ndarray]:
+        """Fills in this step's addresses; the mask of parameters without a gradient, None where all have one."""
+        addresses = list(map(_address, self.params))
+        if addresses != self.addresses:
+            for p, n in zip(self.params, self.entries["n"].tolist()):
+                if p.dtype != self.dtype or p.numel() != n or p.device != device or not p.is_contiguous():
+                    raise RuntimeError("AdamW: a parameter's type, size, device or layout has changed.")
+            self.entries["param"] = self.addresses = addresses
+        grads = list(map(_gradient, self.params))
+        try:
+            where = np.fromiter(map(_address, grads), np.uint64, len(grads))
+            if all(map(_is_dense, grads)) and set(map(_dtype, grads)) == {self.dtype}:
+                self.entries["grad"] = where
+                return None
+        except TypeError:  # None has no address
+            pass
+        without = np.array([g is None for g in grads])
+        have = [g for g in grads if g is not None]
+        if any(g.layout is not torch.strided or g.dtype != self.dtype for g in have):
+            raise RuntimeError("AdamW: gradients must be dense and of their parameter's type.")
+        self.copies = grads = [g if g is None else g.contiguous() for g in grads]
+        self.entries["grad"] = [0 if g is None else g.data_ptr() for g in grads]
+        return without if without.any() else None
 
 
 class AdamW:
@@ -101,72 +143,64 @@ class AdamW:
         self._steps = np.zeros(len(self.params), dtype=np.int64)
         self._device_step = torch.zeros(1, dtype=torch.int64, device=self.device) if capturable else None
         self._scalars = torch.zeros(3, device=self.device) if capturable else None
-        group_of = [i for i, g in enumerate(self.param_groups) for _ in g["params"]]
-        self._tables = []
-        for dt, code in _DTYPES.items():
-            index = np.array([i for i, p in enumerate(self.params) if p.dtype == dt], dtype=np.int64)
-            if not index.size:
-                continue
-            table = np.zeros(index.size, dtype=_ENTRY)
-            table["n"], table["state_offset"] = sizes[index], self._offsets[index]
-            self._tables.append((dt, code, index, [self.params[i] for i in index], table,
-                                 np.array(group_of, dtype=np.int64)[index]))
-
-    def _gradients(self, dt, params, table):
-        """Fills the table's addresses; returns the mask of parameters that have a gradient, None where all have."""
-        ptrs = [p.data_ptr() for p in params]
-        if ptrs != table["param"].tolist():
-            for p, n in zip(params, table["n"].tolist()):
-                if p.dtype != dt or p.numel() != n or p.device != self.device or not p.is_contiguous():
-                    raise RuntimeError("AdamW: a parameter's type, size, device or layout has changed.")
-            table["param"] = ptrs
-        grads = [p.grad for p in params]
-        mask = None
-        if None in [g if g is None else 0 for g in grads]:
-            mask = np.array([g is not None for g in grads])
-        grads = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
-        for g in grads:
-            if g is not None and (g.dtype is not dt or g.layout is not torch.strided):
-                raise RuntimeError("AdamW: gradients must be dense and of their parameter's type.")
-        table["grad"] = [0 if g is None else g.data_ptr() for g in grads]
-        return mask, grads
+        group_of = np.array([i for i, g in enumerate(self.param_groups) for _ in g["params"]], dtype=np.int64)
+        # one table per element type, its entries in the parameters' order
+        self._tables = [_TypeTable(self, dt, group_of) for dt in _DTYPES if any(p.dtype == dt for p in self.params)]
+        self._steady = True  # every parameter has had its gradient in every step
 
     @torch.no_grad()
     def step(self, grad_scale: float = 1.0) -> None:
         """Updates the parameters in place from their ``.grad`` times ``grad_scale``."""
         lib = _lib.load()
-        b1, b2 = self.betas
-        filled = [self._gradients(t[0], t[3], t[4]) for t in self._tables]
-        if self.capturable and any(mask is not None for mask, _ in filled):
-            raise RuntimeError("AdamW(capturable=True): every parameter needs a gradient.")
+        missing = [t.gather(self.device) for t in self._tables]
+        if any(m is not None for m in missing):
+            if self.capturable:
+                raise RuntimeError("AdamW(capturable=True): every parameter needs a gradient.")
+            self._steady = False
         self._calls += 1
-        lrs = np.array([g["lr"] for g in self.param_groups])
-        decay = 1.0 - lrs * np.array([g["weight_decay"] for g in self.param_groups])
+        b1, b2 = self.betas
         dev = self.device.index
-        counted = self._device_step
+        scales = (None, None) if self.scale_avg is None else (self.scale_avg.data_ptr(), self.scale_sq.data_ptr())
+        counter = None if self._device_step is None else self._device_step.data_ptr()
+        scalars = None if self._scalars is None else self._scalars.data_ptr()
         with _lib.on_device(dev):
             stream = torch.cuda.current_stream(dev).cuda_stream
-            for (dt, code, index, _, table, group), (mask, _keep) in zip(self._tables, filled):
-                if mask is not None:
-                    index, table, group = index[mask], table[mask], group[mask]
-                    if not index.size:
-                        continue
-                table["decay"] = decay[group]
-                if self.capturable:
-                    table["step_size"] = lrs[group]
-                else:
-                    self._steps[index] += 1
-                    t = self._steps[index]
-                    table["step_size"] = lrs[group] / (1.0 - b1 ** t)
-                    table["inv_sqrt_bc2"] = 1.0 / np.sqrt(1.0 - b2 ** t)
+            for table, without in zip(self._tables, missing):
+                entries = table.entries if without is None else table.entries[~without]
+                if not len(entries):
+                    continue
+                self._rates(table, entries, without)
                 _lib.check(lib.gru_adamw_step(
-                    _at(table), len(table), code, self.state_bits, self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
-                    self.scale_avg.data_ptr() if self.scale_avg is not None else None,
-                    self.scale_sq.data_ptr() if self.scale_sq is not None else None, self.state_elems, b1, b2, self.eps,
-                    float(grad_scale), self.seed, self._calls, None if counted is None else counted.data_ptr(),
-                    None if self._scalars is None else self._scalars.data_ptr(), stream), "gru_adamw_step")
-                counted = None  # counted once for all element types
+                    entries.ctypes.data, len(entries), table.code, self.state_bits, self.exp_avg.data_ptr(),
+                    self.exp_avg_sq.data_ptr(), *scales, self.state_elems, b1, b2, self.eps, grad_scale, self.seed,
+                    self._calls, counter, scalars, stream), "gru_adamw_step")
+                counter = None  # counted once for all element types
+                table.copies = None
         torch.autograd.graph.increment_version(self.params)
+
+    def _rates(self, table, entries, without) -> None:
+        """Writes the learning rates, decays and bias corrections of this step; counts it."""
+        b1, b2 = self.betas
+        if self._steady:
+            # all parameters are at the same step
+            t = self._calls
+            r1, r2 = (1.0, 0.0) if self.capturable else (1.0 - b1 ** t, 1.0 / math.sqrt(1.0 - b2 ** t))
+            for lo, hi, i in table.groups:
+                lr = self.param_groups[i]["lr"]
+                part = entries[lo:hi]
+                part["decay"] = 1.0 - lr * self.param_groups[i]["weight_decay"]
+                part["step_size"] = lr / r1
+                part["inv_sqrt_bc2"] = r2
+            self._steps[table.index] += 1
+            return
+        index = table.index if without is None else table.index[~without]
+        group = table.group if without is None else table.group[~without]
+        self._steps[index] += 1
+        t = self._steps[index]
+        lr = np.array([g["lr"] for g in self.param_groups])
+        entries["decay"] = (1.0 - lr * np.array([g["weight_decay"] for g in self.param_groups]))[group]
+        entries["step_size"] = lr[group] / (1.0 - b1 ** t)
+        entries["inv_sqrt_bc2"] = 1.0 / np.sqrt(1.0 - b2 ** t)
 
     def zero_grad(self, set_to_none: bool = True) -> None:
         for p in self.params:
@@ -216,6 +250,7 @@ class AdamW:
             self._device_step.fill_(state["calls"])
         self._calls, self.seed = int(state["calls"]), int(state["seed"])
         self._steps[:] = state["steps"]
+        self._steady = all(t == self._calls for t in state["steps"])
         for name in ("exp_avg", "exp_avg_sq", "scale_avg", "scale_sq"):
             mine: Optional[torch.Tensor] = getattr(self, name)
             if mine is not None:
