@@ -1,7 +1,7 @@
 // The gated delta rule over chunks of 64 tokens: gradient.
 //
 // In the notation of the forward, with dS1 the gradient of the state after a
-// chunk and P = scale lower(Q K^T o D):
+// chunk:
 //
 //   dU = P^T dO + diag(e^(G_end - G)) K dS1        Z = dU - W^T (B dU)
 //   dV = B Z            dbeta_i = Z_i . E_i
@@ -17,269 +17,299 @@
 // decay of token t multiplies, and nothing besides (running sums of q . dq -
 // k . dk would do, but cancel most of their digits).
 //
-// The chunks' products of queries, keys and W are computed again (`prepare`)
-// rather than kept from the forward.  `dout` (all chunks) computes P^T dO;
-// `scan` walks the chunks backwards as the forward's scan does, a CTA per head
-// and 32 value columns, and leaves dS1 and Z; `grads` (all chunks) does the
-// rest, a CTA per key head, over its value heads in a fixed order.
+// W and P are computed again (`prepare`) rather than kept from the forward.
+// `scan` walks the chunks backwards as the forward's scan does and leaves dS1,
+// Z and dO as planes; `grads` (all chunks at once) does the rest, a CTA per key
+// head, over its value heads in a fixed order.
 
-#include "delta_common.cuh"
+#include "delta_scan.cuh"
 
 namespace gru {
 namespace delta {
 namespace {
 
-template <typename T>
-__device__ __forceinline__ bool vec4_ok(const T* p, long stride) {
-  return ((reinterpret_cast<uintptr_t>(p) | (stride * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
-}
-
-// A chunk's rows of the output gradient, kSlice columns from c0, as planes.
-template <typename T>
-__device__ __forceinline__ void load_dout(bf16* dst, const T* p, long stride, int rows, int cols, bool vec) {
-  constexpr int NP = Planes<T>::n;
-  for (int i = threadIdx.x; i < kC * (kSlice / 4); i += kThreads) {
-    const int r = i / (kSlice / 4), c = (i % (kSlice / 4)) * 4;
-    const float4 f = get4<T>(p + r * stride + c, r < rows ? cols - c : 0, vec);
-    put2<NP>(dst, kC * pitch(kSlice), pitch(kSlice), r, c, f.x, f.y);
-    put2<NP>(dst, kC * pitch(kSlice), pitch(kSlice), r, c + 2, f.z, f.w);
-  }
-}
-
 // ---------------------------------------------------------------------------
-// dout: P^T dO, one CTA per (batch, value head, chunk).
+// scan: one CTA per (batch, value head, 32 value columns), last chunk first, in
+// the forward scan's division of work: eight warps, four quarters of the rows x
+// two groups of 16 columns, dS in registers, planes through shared memory
+// between three barriers a chunk.
 // ---------------------------------------------------------------------------
 
-template <typename T>
-struct DoutSmem {
-  static constexpr int p = 3 * kC * pitch(kC), d = Planes<T>::n * kC * pitch(kSlice);
-  static constexpr int bytes = (p + d) * 2;
-};
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) delta_dout_kernel(const Problem a) {
-  constexpr int NP = Planes<T>::n;
-  using L = DoutSmem<T>;
-  extern __shared__ __align__(16) unsigned char smem[];
-  bf16* pp = reinterpret_cast<bf16*>(smem);
-  bf16* op = pp + L::p;
-  constexpr int ldx = pitch(kSlice), plx = kC * ldx;
-  const int chunk = blockIdx.x % a.nc, bh = blockIdx.x / a.nc;
-  const int hv = bh % a.Hv, b = bh / a.Hv;
-  const int t0 = chunk * kC, rows = min(kC, a.T - t0);
-  const long nv = blockIdx.x, stride = (long)a.Hv * a.dv;
-  const T* dout = static_cast<const T*>(a.dout) + ((long)b * a.T + t0) * stride + (long)hv * a.dv;
-  const bool vec = vec4_ok(dout, a.dv);
-  copy_rows<kC>(pp, a.pp + nv * 3 * kC * kC, 3 * kC);
-  cp_async_commit();
-  cp_async_wait<0>();
-  const int warp = threadIdx.x >> 5;
-  const int m0 = (warp >> 1) * 16, n0 = (warp & 1) * 16;
-  for (int c0 = 0; c0 < a.dvp; c0 += kSlice) {
-    load_dout<T>(op, dout + c0, stride, rows, a.dv - c0, vec);
-    __syncthreads();
-    float acc[2][4];
-    zero(acc);
-    mma_tile<3, NP, true, true, 2>(acc, pp, kC * pitch(kC), pitch(kC), m0, op, plx, ldx, n0, m0, kC);
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        *reinterpret_cast<float2*>(a.du0 + (nv * kC + frag_row(m0, e)) * a.dvp + c0 + frag_col(n0 + n * 8)) =
-            make_float2(acc[n][2 * e], acc[n][2 * e + 1]);
-    __syncthreads();
-  }
-}
-
-// ---------------------------------------------------------------------------
-// scan: one CTA per (batch, value head, 32 value columns), last chunk first.
-// ---------------------------------------------------------------------------
-
-template <int NP, int DK>
+template <int NP, int DK, int STAGES>
 struct BackSmem {
-  static constexpr int k = NP * kC * pitch(DK);
-  static constexpr int w = 3 * kC * pitch(kC);
-  static constexpr int stage = (2 * k + w) * 2 + 3 * kC * 4;
-  static constexpr int stages = NP == 3 && DK == 128 ? 1 : 2;  // two do not fit there
-  static constexpr int s = 3 * DK * pitch(kSlice);
-  static constexpr int x = 3 * kC * pitch(kSlice);
-  static constexpr int bytes = stages * stage + (s + 3 * x) * 2;
+  static constexpr int k = NP * kC * DK, w = 2 * kTile;  // elements; K, Q, W, P
+  static constexpr int stage = 2 * (k + w) * 2 + kGates * kC * 4;
+  // two planes of two groups (of dO, NP): dS, B dU, e^G B Z; dO; e^G dO twice
+  static constexpr int s = 4 * kGroup * DK, x = 4 * kGroup * kC, o = NP * 2 * kGroup * kC;
+  static constexpr int bytes = STAGES * stage + (s + 4 * x + o) * 2 + 6 * 8 * 4;
 };
 
 template <int NP, int DK>
 __device__ __forceinline__ void back_load(unsigned char* stage, const Problem& a, long nk, long nv) {
-  using L = BackSmem<NP, DK>;
-  bf16* k = reinterpret_cast<bf16*>(stage);
-  copy_rows<DK>(k, a.kp + nk * NP * kC * DK, NP * kC);
-  copy_rows<DK>(k + L::k, a.qp + nk * NP * kC * DK, NP * kC);
-  copy_rows<kC>(k + 2 * L::k, a.wp + nv * 3 * kC * kC, 3 * kC);
-  float* sc = reinterpret_cast<float*>(k + 2 * L::k + L::w);
-  if (threadIdx.x < 3 * kC / 4) cp_async16(sc + threadIdx.x * 4, a.gates + nv * kGates * kC + threadIdx.x * 4);
+  using L = BackSmem<NP, DK, 1>;
+  f16* p = reinterpret_cast<f16*>(stage);
+  copy_async(p, a.kp + nk * L::k, L::k * 2);
+  copy_async(p + L::k, a.qp + nk * L::k, L::k * 2);
+  copy_async(p + 2 * L::k, a.wp + nv * L::w, L::w * 2);
+  copy_async(p + 2 * L::k + L::w, a.pp + nv * L::w, L::w * 2);
+  copy_async(p + 2 * (L::k + L::w), a.gates + nv * kGates * kC, kGates * kC * 4);
   cp_async_commit();
 }
 
-template <typename T, int DK>
-__global__ void __launch_bounds__(kThreads) delta_back_scan_kernel(const Problem a) {
-  constexpr int NP = Planes<T>::n;
-  constexpr int NT = DK / 32;
-  using L = BackSmem<NP, DK>;
-  extern __shared__ __align__(16) unsigned char smem[];
-  bf16* sp = reinterpret_cast<bf16*>(smem + L::stages * L::stage);
-  bf16* xp = sp + L::s;
-  bf16* yp = xp + L::x;
-  bf16* op = yp + L::x;
-  constexpr int ldx = pitch(kSlice), plx = kC * ldx, pls = DK * ldx;
-
-  const int slices = a.dvp / kSlice;
-  const int slice = blockIdx.x % slices, bh = blockIdx.x / slices;
-  const int hv = bh % a.Hv, b = bh / a.Hv;
-  const int c0 = slice * kSlice;
-  const int warp = threadIdx.x >> 5;
-  const int m0 = (warp >> 1) * 16, n0 = (warp & 1) * 16;
-  const int ms = DK == 128 ? warp * 16 : m0, ns = DK == 128 ? 0 : n0;
-  const long nv0 = (long)bh * a.nc, nk0 = ((long)b * a.Hk + hv / a.rep) * a.nc;
-
-  float d[NT][4];  // the gradient of the state after the chunk
+// A warp's 16 tokens x 16 columns as NP planes in shared memory (and `out`,
+// if any), with their scale.
+template <int NP>
+__device__ __forceinline__ void put_tokens(const float (&x)[2][4], int quarter, f16* tile, float* scale, f16* out,
+                                           long plane, float* out_scale) {
+  const float inv = plane_inv(warp_max(x));
+  if ((threadIdx.x & 31) == 0) {
+    if (tile) scale[quarter] = plane_scale(inv);
+    if (out) out_scale[quarter] = plane_scale(inv);
+  }
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int n = 0; n < 2; ++n)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = frag_row(ms, e >> 1), c = c0 + frag_col(ns + n * 8) + (e & 1);
-      d[n][e] = (a.ds_out && r < a.dk && c < a.dv) ? a.ds_out[((long)bh * a.dk + r) * a.dv + c] : 0.0f;
+    for (int e = 0; e < 2; ++e) {
+      uint32_t w[NP];
+      split2<NP>(x[n][2 * e], x[n][2 * e + 1], inv, w);
+      if (tile) store_pair<NP>(tile, 2 * kGroup * kC, quarter * 2 + e, n, w);
+      if (out) store_pair<NP>(out, plane, quarter * 2 + e, n, w);
     }
+}
+
+// STAGES: with two the next chunk's tiles load during this one; with one they
+// load between chunks, and two CTAs fit on an SM.
+template <typename T, int DK, int STAGES>
+__global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Problem a) {
+  constexpr int NP = Planes<T>::n, MT = DK / 64;
+  using L = BackSmem<NP, DK, STAGES>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int slices = a.dvp / kSlice, groups = a.dvp / kGroup;
+  const int bh = blockIdx.x / slices, hv = bh % a.Hv, b = bh / a.Hv;
+  const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3, pair = threadIdx.x >> 7;
+  const int group = (blockIdx.x % slices) * 2 + pair, c0 = group * kGroup;
+  const long nv0 = (long)bh * a.nc, nk0 = ((long)b * a.Hk + hv / a.rep) * a.nc;
+  f16* base = reinterpret_cast<f16*>(smem + STAGES * L::stage);
+  f16* sp = base + pair * kGroup * DK;
+  f16* up = base + L::s + pair * kGroup * kC;  // B dU
+  f16* zp = up + L::x;                         // -e^G B Z
+  f16* qop = zp + L::x;                        // scale e^G dO, of this chunk and of the next
+  f16* op = base + L::s + 4 * L::x + pair * kGroup * kC;
+  float* scales = reinterpret_cast<float*>(base + L::s + 4 * L::x + L::o) + pair * 4;
+  float *ssc = scales, *usc = scales + 8, *zsc = scales + 16, *qosc = scales + 24, *osc = scales + 40;
+
+  float d[MT][2][4];  // the gradient of the state after the chunk
+  const float* ds = a.ds_out ? a.ds_out + (long)bh * a.dk * a.dv : nullptr;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = frag_row((quarter * MT + m) * 16, e >> 1), c = c0 + frag_col(n * 8) + (e & 1);
+        d[m][n][e] = ds && r < a.dk && c < a.dv ? ds[(long)r * a.dv + c] : 0.0f;
+      }
   const long stride = (long)a.Hv * a.dv;
   const long at = (long)b * a.T * stride + (long)hv * a.dv + c0;
   const T* dout = a.dout ? static_cast<const T*>(a.dout) + at : nullptr;
   T* dv = static_cast<T*>(a.dv_) + at;
-  const bool vec = a.dv % 2 == 0;
-  float dr[2][4], ur[2][4];
-  auto load_rows = [&](int chunk) {
+  const int cols = a.dv - c0;
+  const bool vec = pairs_ok<T>(a.dout, 0, 0, 0, a.dv);
+  Columns<T> od;
+  auto load_dout = [&](int chunk) {
+    const int t = chunk * kC + quarter * 16;
+    od.start(dout + (dout ? t * stride : 0), stride, dout ? a.T - t : 0, cols, vec);
+  };
+  // dO of a chunk, whose e^G must be there, as planes: as it is, and for Q^T
+  auto put_dout = [&](int chunk, const float* gate) {
+    float x[2][4];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = frag_row(m0, e), t = chunk * kC + row, c = frag_col(n0 + n * 8);
-        const bool in = dout && t < a.T;
-        dr[n][2 * e] = in && c0 + c < a.dv ? as_float(dout[t * stride + c]) : 0.0f;
-        dr[n][2 * e + 1] = in && c0 + c + 1 < a.dv ? as_float(dout[t * stride + c + 1]) : 0.0f;
-        const float2 u = dout ? *reinterpret_cast<const float2*>(a.du0 + ((nv0 + chunk) * kC + row) * a.dvp + c0 + c)
-                              : make_float2(0.0f, 0.0f);
-        ur[n][2 * e] = u.x;
-        ur[n][2 * e + 1] = u.y;
+        const float2 f = od.get(n, e);
+        x[n][2 * e] = f.x;
+        x[n][2 * e + 1] = f.y;
       }
-  };
-  auto put_state = [&]() {
+    const long nv = nv0 + chunk;
+    put_tokens<NP>(x, quarter, op, osc, a.dop + (nv * NP * groups + group) * kGroup * kC, (long)a.dvp * kC,
+                   a.doscale + (nv * groups + group) * 4);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        put2<3>(sp, pls, ldx, frag_row(ms, e), frag_col(ns + n * 8), d[n][2 * e], d[n][2 * e + 1]);
+      for (int e = 0; e < 4; ++e) x[n][e] *= a.scale * gate[frag_row(quarter * 16, e >> 1)];
+    put_tokens<2>(x, quarter, qop + (chunk & 1) * L::x, qosc + (chunk & 1) * 8, nullptr, 0, nullptr);
   };
-
-  int buf = 0;
+  auto state_out = [&](int chunk) {
+    const long nv = nv0 + chunk;
+    put_state<DK>(d, quarter, sp, ssc, chunk >= 0 ? a.dstates + (nv * 2 * groups + group) * kGroup * DK : nullptr,
+                  (long)a.dvp * DK, a.dsscale + (nv * groups + group) * 4);
+  };
   back_load<NP, DK>(smem, a, nk0 + a.nc - 1, nv0 + a.nc - 1);
-  load_rows(a.nc - 1);
-  put_state();
+  load_dout(a.nc - 1);
+  state_out(a.nc - 1);
+  int buf = 0;
   for (int chunk = a.nc - 1; chunk >= 0; --chunk) {
-    unsigned char* stage = smem + buf * L::stage;
-    const bf16* kp = reinterpret_cast<const bf16*>(stage);
-    const bf16* qp = kp + L::k;
-    const bf16* wp = qp + L::k;
-    const float* gate = reinterpret_cast<const float*>(wp + L::w);
+    const f16* kp = reinterpret_cast<const f16*>(smem + buf * L::stage);
+    const f16* qp = kp + L::k;
+    const f16* wp = qp + L::k;
+    const f16* pp = wp + L::w;
+    const float* gate = reinterpret_cast<const float*>(pp + L::w);
     const long nv = nv0 + chunk;
     cp_async_wait<0>();
     __syncthreads();
-    if (L::stages == 2 && chunk > 0) {
+    if (STAGES == 2 && chunk > 0) {
       buf ^= 1;
       back_load<NP, DK>(smem + buf * L::stage, a, nk0 + chunk - 1, nv - 1);
     }
+    const float sw = gate[5 * kC], sP = gate[5 * kC + 1], sk = gate[5 * kC + 2], sq = gate[5 * kC + 3];
+    const int row[2] = {frag_row(quarter * 16, 0), frag_row(quarter * 16, 1)};
+    put_dout(chunk, gate);
+    if (chunk > 0) load_dout(chunk - 1);
+    // dU
+    float x[2][4], y[2][4];
+    times_state<NP, DK>(x, kp, quarter * 2, sp, ssc);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        *reinterpret_cast<float2*>(a.dstates + (nv * DK + frag_row(ms, e)) * a.dvp + c0 + frag_col(ns + n * 8)) =
-            make_float2(d[n][2 * e], d[n][2 * e + 1]);
-
-    float acc[2][4], du[2][4];
-    zero(acc);
-    mma_tile<NP, 3, false, true, 2>(acc, kp, kC * pitch(DK), pitch(DK), m0, sp, pls, ldx, n0, 0, DK);
+      for (int e = 0; e < 4; ++e) x[n][e] *= sk * gate[kC + row[e >> 1]];
+    __syncthreads();
+    times_tokens<2, NP, true>(x, pp, quarter * 2, op, 2 * kGroup * kC * 2, osc, sP, quarter, 4);
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[n][e] = x[n][e] * gate[2 * kC + row[e >> 1]];
+    put_tokens<2>(y, quarter, up, usc, nullptr, 0, nullptr);
+    __syncthreads();
+    // Z and dV
+    times_tokens<2, 2, true>(x, wp, quarter * 2, up, 2 * kGroup * kC * 2, usc, -sw, quarter, 4);
+    put_tokens<2>(x, quarter, nullptr, nullptr, a.z + (nv * 2 * groups + group) * kGroup * kC, (long)a.dvp * kC,
+                  a.zscale + (nv * groups + group) * 4);
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = frag_row(m0, e), col = frag_col(n0 + n * 8);
-        const float er = gate[kC + row], be = gate[2 * kC + row], f = gate[row] * a.scale;
-        du[n][2 * e] = ur[n][2 * e] + er * acc[n][2 * e];
-        du[n][2 * e + 1] = ur[n][2 * e + 1] + er * acc[n][2 * e + 1];
-        put2<3>(xp, plx, ldx, row, col, be * du[n][2 * e], be * du[n][2 * e + 1]);
-        put2<3>(op, plx, ldx, row, col, f * dr[n][2 * e], f * dr[n][2 * e + 1]);
+        const int t = chunk * kC + row[e], c = frag_col(n * 8);
+        const float be = gate[2 * kC + row[e]], eg = gate[row[e]];
+        x[n][2 * e] *= be;
+        x[n][2 * e + 1] *= be;
+        if (t < a.T) set2<T>(dv + t * stride + c, cols - c, a.dv % 2 == 0, x[n][2 * e], x[n][2 * e + 1]);
+        y[n][2 * e] = -eg * x[n][2 * e];
+        y[n][2 * e + 1] = -eg * x[n][2 * e + 1];
       }
-    if (chunk > 0) load_rows(chunk - 1);
+    put_tokens<2>(y, quarter, zp, zsc, nullptr, 0, nullptr);
     __syncthreads();
-    zero(acc);
-    mma_tile<3, 3, true, true, 2>(acc, wp, kC * pitch(kC), pitch(kC), m0, xp, plx, ldx, n0, m0, kC);
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = frag_row(m0, e), col = frag_col(n0 + n * 8), t = chunk * kC + row;
-        const float z0 = du[n][2 * e] - acc[n][2 * e], z1 = du[n][2 * e + 1] - acc[n][2 * e + 1];
-        const float be = gate[2 * kC + row], f = -gate[row] * be;
-        *reinterpret_cast<float2*>(a.z + (nv * kC + row) * a.dvp + c0 + col) = make_float2(z0, z1);
-        put2<3>(yp, plx, ldx, row, col, f * z0, f * z1);
-        if (t < a.T) set2<T>(dv + t * stride + col, a.dv - c0 - col, vec, be * z0, be * z1);
-      }
-    __syncthreads();
-    float x[NT][4];
-    zero(x);
-    mma_tile<NP, 3, true, true, NT>(x, qp, kC * pitch(DK), pitch(DK), ms, op, plx, ldx, ns, 0, kC);
-    mma_tile<NP, 3, true, true, NT>(x, kp, kC * pitch(DK), pitch(DK), ms, yp, plx, ldx, ns, 0, kC);
     const float decay = gate[kC - 1];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) d[n][e] = decay * d[n][e] + x[n][e];
-    put_state();
-    if (L::stages == 1 && chunk > 0) {
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[m][n][e] *= decay;
+    add_to_state<NP, DK>(d, qp, quarter, qop + (chunk & 1) * L::x, qosc + (chunk & 1) * 8, sq);
+    add_to_state<NP, DK>(d, kp, quarter, zp, zsc, sk);
+    state_out(chunk - 1);
+    if (STAGES == 1 && chunk > 0) {
       __syncthreads();
       back_load<NP, DK>(smem, a, nk0 + chunk - 1, nv - 1);
     }
   }
-  if (a.ds0) {
+  if (!a.ds0) return;
+  float* out = a.ds0 + (long)bh * a.dk * a.dv;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int r = frag_row(ms, e >> 1), c = c0 + frag_col(ns + n * 8) + (e & 1);
-        if (r < a.dk && c < a.dv) a.ds0[((long)bh * a.dk + r) * a.dv + c] = d[n][e];
+        const int r = frag_row((quarter * MT + m) * 16, e >> 1), c = c0 + frag_col(n * 8) + (e & 1);
+        if (r < a.dk && c < a.dv) out[(long)r * a.dv + c] = d[m][n][e];
       }
-  }
 }
 
 // ---------------------------------------------------------------------------
-// grads: one CTA per (batch, key head, chunk).
+// grads: one CTA per (batch, key head, chunk).  It walks the value columns in
+// steps of 16 (one step of the products' inner dimension, one scale), three
+// steps in flight; a warp keeps 16 tokens x half of the key columns of dQ,
+// dK_row and dK_col, and of 32 tokens of dO U^T and Z U^T, in registers.
 // ---------------------------------------------------------------------------
 
 template <int NP, int DK>
 struct GradSmem {
-  static constexpr int qk = NP * kC * pitch(DK);
-  static constexpr int s = 3 * DK * pitch(kSlice), x = 3 * kC * pitch(kSlice), o = NP * kC * pitch(kSlice);
-  static constexpr int slices = 2 * s + 2 * x + o;   // while walking the value columns
-  static constexpr int tiles = 2 * 3 * kC * pitch(kC) + 2 * kC * (kC + 1);  // afterwards; y in FP32
-  static constexpr int bytes = (2 * qk + (slices > tiles ? slices : tiles)) * 2 + kGates * kC * 4 + (5 * kC + 16) * 4;
+  static constexpr int qk = NP * kC * DK;  // elements
+  static constexpr int s = 2 * kGroup * DK, x = 2 * kGroup * kC, o = NP * kGroup * kC;
+  static constexpr int stage = 2 * s + 2 * x + o;  // S, dS, E, Z, dO of 16 columns
+  static constexpr int stages = 3;
+  static constexpr int tiles = 4 * kTile * 2 + kC * (kC + 1) * 4;  // bytes: dP', M; y in FP32; over the stages
+  static constexpr int main = stages * stage * 2 > tiles ? stages * stage * 2 : tiles;
+  static constexpr int bytes = 2 * qk * 2 + (main + 15) / 16 * 16 + kGates * kC * 4 + (5 * kC + 32) * 4;
 };
 
-// The value at (row, col) and (row, col + 1) of a tile held as planes.
-template <int NP>
-__device__ __forceinline__ float2 take2(const bf16* p, int plane, int ld, int row, int col) {
-  float2 f = make_float2(0.0f, 0.0f);
+template <int NP, int DK>
+__device__ __forceinline__ void grad_load(f16* dst, const Problem& a, long nv, int c0) {
+  using L = GradSmem<NP, DK>;
 #pragma unroll
-  for (int i = NP - 1; i >= 0; --i) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(p + i * plane + row * ld + col);
-    f.x += __uint_as_float(w << 16);
-    f.y += __uint_as_float(w & 0xffff0000u);
+  for (int p = 0; p < 2; ++p) {
+    copy_async(dst + p * kGroup * DK, a.states + (nv * 2 + p) * a.dvp * DK + (long)c0 * DK, kGroup * DK * 2);
+    copy_async(dst + L::s + p * kGroup * DK, a.dstates + (nv * 2 + p) * a.dvp * DK + (long)c0 * DK, kGroup * DK * 2);
+    copy_async(dst + 2 * L::s + p * kGroup * kC, a.e + (nv * 2 + p) * a.dvp * kC + (long)c0 * kC, kGroup * kC * 2);
+    copy_async(dst + 2 * L::s + L::x + p * kGroup * kC, a.z + (nv * 2 + p) * a.dvp * kC + (long)c0 * kC, kGroup * kC * 2);
+  }
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+    copy_async(dst + 2 * L::s + 2 * L::x + p * kGroup * kC, a.dop + (nv * NP + p) * a.dvp * kC + (long)c0 * kC,
+               kGroup * kC * 2);
+}
+
+// The value pair `word` of a tile held as planes, without its scale.
+template <int NP>
+__device__ __forceinline__ float2 take2(const f16* p, int plane, int word) {
+  float2 f = __half22float2(reinterpret_cast<const __half2*>(p)[word]);
+  if (NP == 2) {
+    const float2 l = __half22float2(reinterpret_cast<const __half2*>(p + plane)[word]);
+    f.x += l.x;
+    f.y += l.y;
   }
   return f;
+}
+__device__ __forceinline__ float2 pair(uint32_t h, uint32_t l) {
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&l));
+  return make_float2(x.x + y.x, x.y + y.y);
+}
+
+// acc[n ..] += A B, one step of 16 and four tiles, times f0 (the first two
+// tiles) or f1.
+template <int NA, int NB, int NT>
+__device__ __forceinline__ void step_add(float (&acc)[NT][4], int n, float f0, float f1, const uint32_t (&fa)[NA][4],
+                                         const uint32_t (&fb)[NB][4][2]) {
+  float t[4][4];
+  zero(t);
+  mma_terms<NA, NB, 4>(t, fa, fb);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[n + i][e] += (i < 2 ? f0 : f1) * t[i][e];
+}
+
+// acc += f A B over steps [k0, k1) of the tokens: A a 64 x 64 tile (rows m, or
+// transposed), B a [64 x DK] tile from column block n8.
+template <int NP, int DK, bool TA, int NT>
+__device__ __forceinline__ void token_product(float (&acc)[NT][4], float f, const f16* A, int m8, const f16* B, int n8,
+                                              int k0, int k1) {
+  for (int kk = k0; kk < k1; ++kk) {
+    uint32_t fa[2][4];
+    const uint32_t pa = addr_a<kC, TA>(A, m8, 2 * kk);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) ldm4<TA>(fa[p], pa + p * kTile * 2);
+    const uint32_t pb = addr_b<DK, true>(B, 2 * kk, n8);
+#pragma unroll
+    for (int n = 0; n < NT; n += 4) {
+      uint32_t fb[NP][4][2];
+      load_b<NP, 4, true>(fb, pb + n * 128, 256, kC * DK * 2);
+      step_add<2, NP, NT>(acc, n, f, f, fa, fb);
+    }
+  }
 }
 
 template <typename T, int DK>
@@ -288,41 +318,35 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
   constexpr int NT = DK / 16;  // a warp's half of the key columns, in 8-column tiles
   using L = GradSmem<NP, DK>;
   extern __shared__ __align__(16) unsigned char smem[];
-  bf16* qp = reinterpret_cast<bf16*>(smem);
-  bf16* kp = qp + L::qk;
-  bf16* s0p = kp + L::qk;
-  bf16* dsp = s0p + L::s;
-  bf16* up = dsp + L::s;
-  bf16* zp = up + L::x;
-  bf16* op = zp + L::x;
-  bf16* dpp = s0p;  // over the slices
-  bf16* mp = dpp + 3 * kC * pitch(kC);
-  float* gate = reinterpret_cast<float*>(s0p + (L::slices > L::tiles ? L::slices : L::tiles));
-  float* y = reinterpret_cast<float*>(mp + 3 * kC * pitch(kC));  // [64][65]
-  float* red = gate + kGates * kC;  // x and z of the two column halves, F; then one value per warp
+  f16* qp = reinterpret_cast<f16*>(smem);
+  f16* kp = qp + L::qk;
+  f16* main = kp + L::qk;
+  f16* dpp = main;  // over the stages
+  f16* mp = dpp + 2 * kTile;
+  float* y = reinterpret_cast<float*>(mp + 2 * kTile);  // [64][65]
+  float* gate = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(main) + (L::main + 15) / 16 * 16);
+  float* red = gate + kGates * kC;  // x and z of the two column halves, F; then values per warp
   float* wred = red + 5 * kC;
-  constexpr int ldx = pitch(kSlice), plx = kC * ldx, pls = DK * ldx;
-  constexpr int ldq = pitch(DK), plq = kC * ldq, ldc = pitch(kC), plc = kC * ldc;
 
   const int chunk = blockIdx.x % a.nc, bh = blockIdx.x / a.nc;
   const int hk = bh % a.Hk, b = bh / a.Hk;
   const int t0 = chunk * kC, rows = min(kC, a.T - t0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int m0 = (warp >> 1) * 16, half = warp & 1;
-  const long stride = (long)a.Hv * a.dv;
+  const int groups = a.dvp / kGroup;
 
-  copy_rows<DK>(qp, a.qp + (long)blockIdx.x * NP * kC * DK, NP * kC);
-  copy_rows<DK>(kp, a.kp + (long)blockIdx.x * NP * kC * DK, NP * kC);
-  cp_async_commit();
-  cp_async_wait<0>();
+  copy_async(qp, a.qp + (long)blockIdx.x * L::qk, L::qk * 2);
+  copy_async(kp, a.kp + (long)blockIdx.x * L::qk, L::qk * 2);
 
   for (int r = 0; r < a.rep; ++r) {
     const int hv = hk * a.rep + r;
     const long nv = ((long)b * a.Hv + hv) * a.nc + chunk;
-    const T* dout = a.dout ? static_cast<const T*>(a.dout) + ((long)b * a.T + t0) * stride + (long)hv * a.dv : nullptr;
-    const bool vec = vec4_ok(dout, a.dv);
     __syncthreads();
-    for (int i = threadIdx.x; i < kGates * kC; i += kThreads) gate[i] = a.gates[nv * kGates * kC + i];
+    copy_async(gate, a.gates + nv * kGates * kC, kGates * kC * 4);
+    grad_load<NP, DK>(main, a, nv, 0);
+    cp_async_commit();
+    grad_load<NP, DK>(main + L::stage, a, nv, kGroup);  // dvp is a multiple of two groups
+    cp_async_commit();
     float dp[4][4], da[4][4], dq[NT][4], dkr[NT][4], dkc[NT][4];
     zero(dp);
     zero(da);
@@ -330,67 +354,112 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
     zero(dkr);
     zero(dkc);
     float sdot = 0.0f, bdot[2] = {0.0f, 0.0f};
-    __syncthreads();
-    for (int c0 = 0; c0 < a.dvp; c0 += kSlice) {
-      for (int i = threadIdx.x; i < DK * (kSlice / 4); i += kThreads) {
-        const int x = i / (kSlice / 4), c = (i % (kSlice / 4)) * 4;
-        const float4 f = *reinterpret_cast<const float4*>(a.states + (nv * DK + x) * a.dvp + c0 + c);
-        const float4 g = *reinterpret_cast<const float4*>(a.dstates + (nv * DK + x) * a.dvp + c0 + c);
-        put2<3>(s0p, pls, ldx, x, c, f.x, f.y);
-        put2<3>(s0p, pls, ldx, x, c + 2, f.z, f.w);
-        put2<3>(dsp, pls, ldx, x, c, g.x, g.y);
-        put2<3>(dsp, pls, ldx, x, c + 2, g.z, g.w);
-        sdot += (f.x * g.x + f.y * g.y) + (f.z * g.z + f.w * g.w);
+    for (int g = 0; g < groups; ++g) {
+      cp_async_wait<1>();
+      __syncthreads();
+      if (g + 2 < groups) grad_load<NP, DK>(main + (g + 2) % L::stages * L::stage, a, nv, (g + 2) * kGroup);
+      cp_async_commit();
+      const f16* sp = main + g % L::stages * L::stage;
+      const f16* dsp = sp + L::s;
+      const f16* ep = dsp + L::s;
+      const f16* zp = ep + L::x;
+      const f16* op = zp + L::x;
+      // scales: of this warp's 16 tokens, of its 32 columns of tokens, and of the
+      // quarters of the key columns
+      const long sg = (nv * groups + g) * 4;
+      const int mq = m0 / 16;
+      const float se = fabsf(a.escale[sg + mq]), sz = a.zscale[sg + mq], so = a.doscale[sg + mq];
+      const float se0 = fabsf(a.escale[sg + 2 * half]), se1 = fabsf(a.escale[sg + 2 * half + 1]);
+      const float4 ss = *reinterpret_cast<const float4*>(a.sscale + sg);
+      const float4 sd = *reinterpret_cast<const float4*>(a.dsscale + sg);
+      uint32_t fo[NP][4], fz[2][4], fe[2][4];
+#pragma unroll
+      for (int p = 0; p < NP; ++p) ldm4<false>(fo[p], addr_a<kGroup, false>(op, m0 / 8, 0) + p * kGroup * kC * 2);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        ldm4<false>(fz[p], addr_a<kGroup, false>(zp, m0 / 8, 0) + p * kGroup * kC * 2);
+        ldm4<false>(fe[p], addr_a<kGroup, false>(ep, m0 / 8, 0) + p * kGroup * kC * 2);
+      }
+      if (half * 32 <= m0) {
+        uint32_t fb[2][4][2];
+        load_b<2, 4, false>(fb, addr_b<kGroup, false>(ep, 0, half * 4), 512, kGroup * kC * 2);
+        step_add<NP, 2, 4>(dp, 0, so * se0, so * se1, fo, fb);
+        step_add<2, 2, 4>(da, 0, sz * se0, sz * se1, fz, fb);
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int i = threadIdx.x + j * kThreads;
-        const int x = i / (kSlice / 4), c = (i % (kSlice / 4)) * 4;
-        const float4 f = *reinterpret_cast<const float4*>(a.e + (nv * kC + x) * a.dvp + c0 + c);
-        const float4 g = *reinterpret_cast<const float4*>(a.z + (nv * kC + x) * a.dvp + c0 + c);
-        const float be = gate[2 * kC + x];
-        put2<3>(up, plx, ldx, x, c, be * f.x, be * f.y);
-        put2<3>(up, plx, ldx, x, c + 2, be * f.z, be * f.w);
-        put2<3>(zp, plx, ldx, x, c, g.x, g.y);
-        put2<3>(zp, plx, ldx, x, c + 2, g.z, g.w);
-        bdot[j] += (f.x * g.x + f.y * g.y) + (f.z * g.z + f.w * g.w);
+      for (int n = 0; n < NT; n += 4) {
+        // tiles n, n + 2 of this half lie in these quarters (of DK / 32 tiles)
+        const bool odd = DK == 128 ? n >= 4 : false;
+        const float s0 = half ? (odd ? ss.w : ss.z) : (odd ? ss.y : ss.x);
+        const float s1 = DK == 128 ? s0 : (half ? ss.w : ss.y);
+        const float d0 = half ? (odd ? sd.w : sd.z) : (odd ? sd.y : sd.x);
+        const float d1 = DK == 128 ? d0 : (half ? sd.w : sd.y);
+        uint32_t fb[2][4][2];
+        load_b<2, 4, false>(fb, addr_b<kGroup, false>(sp, 0, half * NT + n), 512, kGroup * DK * 2);
+        step_add<NP, 2, NT>(dq, n, so * s0, so * s1, fo, fb);
+        step_add<2, 2, NT>(dkr, n, sz * s0, sz * s1, fz, fb);
+        load_b<2, 4, false>(fb, addr_b<kGroup, false>(dsp, 0, half * NT + n), 512, kGroup * DK * 2);
+        step_add<2, 2, NT>(dkc, n, se * d0, se * d1, fe, fb);
       }
-      load_dout<T>(op, dout + c0, stride, dout ? rows : 0, a.dv - c0, vec);
-      __syncthreads();
-      if (half * 32 <= m0) {
-        mma_tile<NP, 3, false, false, 4>(dp, op, plx, ldx, m0, up, plx, ldx, half * 32, 0, kSlice);
-        mma_tile<3, 3, false, false, 4>(da, zp, plx, ldx, m0, up, plx, ldx, half * 32, 0, kSlice);
+      if (half == 0) {
+        // Z . E of this lane's two tokens
+        const float f = sz * se;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 u = pair(fz[0][j], fz[1][j]), w = pair(fe[0][j], fe[1][j]);
+          bdot[j & 1] += f * (u.x * w.x + u.y * w.y);
+        }
       }
-      mma_tile<NP, 3, false, false, NT>(dq, op, plx, ldx, m0, s0p, pls, ldx, half * (DK / 2), 0, kSlice);
-      mma_tile<3, 3, false, false, NT>(dkr, zp, plx, ldx, m0, s0p, pls, ldx, half * (DK / 2), 0, kSlice);
-      mma_tile<3, 3, false, false, NT>(dkc, up, plx, ldx, m0, dsp, pls, ldx, half * (DK / 2), 0, kSlice);
-      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kGroup * DK / 2 / kThreads; ++i) {
+        // block warp + 8 i is of the rows 8 (warp / 2 + 4 i) ..., in this quarter
+        const int w = threadIdx.x + i * kThreads, q = (warp / 2 + 4 * i) * 8 / (DK / 4);
+        const float2 u = take2<2>(sp, kGroup * DK, w), v = take2<2>(dsp, kGroup * DK, w);
+        const float fs = q == 0 ? ss.x : q == 1 ? ss.y : q == 2 ? ss.z : ss.w;
+        const float fd = q == 0 ? sd.x : q == 1 ? sd.y : q == 2 ? sd.z : sd.w;
+        sdot += (fs * fd) * (u.x * v.x + u.y * v.y);
+      }
     }
-    // the masked 64 x 64 products, over the slices' memory
+    __syncthreads();
+    // the masked 64 x 64 products, over the stages' memory
+    const float sk = gate[5 * kC + 2], sq = gate[5 * kC + 3];
+    float mu = 0.0f, mw = 0.0f;
     {
       float qk[4][4], kk[4][4];
       zero(qk);
       zero(kk);
       if (half * 32 <= m0) {
-        mma_tile<NP, NP, false, false, 4>(qk, qp, plq, ldq, m0, kp, plq, ldq, half * 32, 0, DK);
-        mma_tile<NP, NP, false, false, 4>(kk, kp, plq, ldq, m0, kp, plq, ldq, half * 32, 0, DK);
+#pragma unroll
+        for (int k = 0; k < DK / 16; ++k) {
+          uint32_t fq[NP][4], fk[NP][4], fb[NP][4][2];
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            ldm4<false>(fq[p], addr_a<DK, false>(qp, m0 / 8, 2 * k) + p * kC * DK * 2);
+            ldm4<false>(fk[p], addr_a<DK, false>(kp, m0 / 8, 2 * k) + p * kC * DK * 2);
+          }
+          load_b<NP, 4, false>(fb, addr_b<DK, false>(kp, 2 * k, half * 4), 32 * DK, kC * DK * 2);
+          step_add<NP, NP, 4>(qk, 0, sq * sk, sq * sk, fq, fb);
+          step_add<NP, NP, 4>(kk, 0, sk * sk, sk * sk, fk, fb);
+        }
       }
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int i = frag_row(m0, e), j = frag_col(half * 32 + n * 8);
-          float u[2], w[2];
 #pragma unroll
           for (int l = 0; l < 2; ++l) {
             const float dec = j + l <= i ? expf((gate[3 * kC + i] - gate[3 * kC + j + l]) +
-                                                (gate[4 * kC + i] - gate[4 * kC + j + l])) : 0.0f;
-            u[l] = j + l <= i ? a.scale * dec * dp[n][2 * e + l] : 0.0f;
-            w[l] = j + l < i ? -gate[2 * kC + i] * dec * da[n][2 * e + l] : 0.0f;
-            y[i * (kC + 1) + j + l] = j + l < i ? u[l] * qk[n][2 * e + l] + w[l] * kk[n][2 * e + l] : 0.0f;
+                                                (gate[4 * kC + i] - gate[4 * kC + j + l])) * gate[2 * kC + j + l]
+                                         : 0.0f;
+            float& u = dp[n][2 * e + l];
+            float& w = da[n][2 * e + l];
+            u = j + l <= i ? a.scale * dec * u : 0.0f;
+            w = j + l < i ? -gate[2 * kC + i] * dec * w : 0.0f;
+            y[i * (kC + 1) + j + l] = j + l < i ? u * qk[n][2 * e + l] + w * kk[n][2 * e + l] : 0.0f;
+            mu = max_finite(mu, u);
+            mw = max_finite(mw, w);
           }
-          put2<3>(dpp, plc, ldc, i, j, u[0], u[1]);
-          put2<3>(mp, plc, ldc, i, j, w[0], w[1]);
         }
     }
     float xs[2] = {0.0f, 0.0f}, zs[2] = {0.0f, 0.0f};
@@ -398,17 +467,19 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = frag_row(m0, e), col = frag_col(half * (DK / 2) + n * 8);
+        const int row = frag_row(m0, e);
+        const int word = ((m0 / 8 + e) * (DK / 8) + half * NT + n) * 32 + lane;
         const float eg = gate[row], er = gate[kC + row], be = gate[2 * kC + row];
-        const float2 kv = take2<NP>(kp, plq, ldq, row, col), qv = take2<NP>(qp, plq, ldq, row, col);
+        const float2 kv = take2<NP>(kp, kC * DK, word), qv = take2<NP>(qp, kC * DK, word);
 #pragma unroll
         for (int l = 0; l < 2; ++l) {
           dq[n][2 * e + l] *= a.scale * eg;
           dkr[n][2 * e + l] *= -eg * be;
-          dkc[n][2 * e + l] *= er;
+          dkc[n][2 * e + l] *= er * be;
         }
-        xs[e] += (qv.x * dq[n][2 * e] + qv.y * dq[n][2 * e + 1]) + (kv.x * dkr[n][2 * e] + kv.y * dkr[n][2 * e + 1]);
-        zs[e] += kv.x * dkc[n][2 * e] + kv.y * dkc[n][2 * e + 1];
+        xs[e] += sq * (qv.x * dq[n][2 * e] + qv.y * dq[n][2 * e + 1]) +
+                 sk * (kv.x * dkr[n][2 * e] + kv.y * dkr[n][2 * e + 1]);
+        zs[e] += sk * (kv.x * dkc[n][2 * e] + kv.y * dkc[n][2 * e + 1]);
       }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -416,18 +487,47 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
       for (int o = 1; o < 4; o <<= 1) {
         xs[e] += __shfl_xor_sync(0xffffffffu, xs[e], o);
         zs[e] += __shfl_xor_sync(0xffffffffu, zs[e], o);
+        bdot[e] += __shfl_xor_sync(0xffffffffu, bdot[e], o);
       }
+      const int row = frag_row(m0, e);
       if ((lane & 3) == 0) {
-        red[half * kC + frag_row(m0, e)] = xs[e];
-        red[(2 + half) * kC + frag_row(m0, e)] = zs[e];
+        red[half * kC + row] = xs[e];
+        red[(2 + half) * kC + row] = zs[e];
+        if (half == 0 && row < rows) a.dbeta[((long)b * a.T + t0 + row) * a.Hv + hv] = bdot[e];
       }
     }
+    float end = gate[kC - 1] * sdot;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) end += __shfl_xor_sync(0xffffffffu, end, o);
+    const unsigned um = __reduce_max_sync(0xffffffffu, __float_as_uint(mu));
+    const unsigned wm = __reduce_max_sync(0xffffffffu, __float_as_uint(mw));
+    if (lane == 0) {
+      wred[warp] = end;
+      wred[8 + warp] = __uint_as_float(um);
+      wred[16 + warp] = __uint_as_float(wm);
+    }
     __syncthreads();
-    const int nb = half * (DK / 2);
-    mma_tile<3, NP, false, true, NT>(dq, dpp, plc, ldc, m0, kp, plq, ldq, nb, 0, m0 + 16);
-    mma_tile<3, NP, false, true, NT>(dkr, mp, plc, ldc, m0, kp, plq, ldq, nb, 0, m0 + 16);
-    mma_tile<3, NP, true, true, NT>(dkc, dpp, plc, ldc, m0, qp, plq, ldq, nb, m0, kC);
-    mma_tile<3, NP, true, true, NT>(dkc, mp, plc, ldc, m0, kp, plq, ldq, nb, m0, kC);
+    mu = wred[8], mw = wred[16];
+#pragma unroll
+    for (int w = 1; w < kThreads / 32; ++w) {
+      mu = fmaxf(mu, wred[8 + w]);
+      mw = fmaxf(mw, wred[16 + w]);
+    }
+    const float iu = plane_inv(mu), iw = plane_inv(mw);
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int word = ((m0 / 8 + e) * (kC / 8) + half * 4 + n) * 32 + lane;
+        uint32_t u[2], w[2];
+        split2<2>(dp[n][2 * e], dp[n][2 * e + 1], iu, u);
+        split2<2>(da[n][2 * e], da[n][2 * e + 1], iw, w);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          reinterpret_cast<uint32_t*>(dpp + p * kTile)[word] = u[p];
+          reinterpret_cast<uint32_t*>(mp + p * kTile)[word] = w[p];
+        }
+      }
     if (threadIdx.x < kC) {
       // y_ij -> sum over the columns before j
       float* row = y + threadIdx.x * (kC + 1);
@@ -439,6 +539,11 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
       }
     }
     __syncthreads();
+    const float su = plane_scale(iu), sw = plane_scale(iw);
+    token_product<NP, DK, false, NT>(dq, su * sk, dpp, m0 / 8, kp, half * NT, 0, m0 / 16 + 1);
+    token_product<NP, DK, false, NT>(dkr, sw * sk, mp, m0 / 8, kp, half * NT, 0, m0 / 16 + 1);
+    token_product<NP, DK, true, NT>(dkc, su * sq, dpp, m0 / 8, qp, half * NT, m0 / 16, kC / 16);
+    token_product<NP, DK, true, NT>(dkc, sw * sk, mp, m0 / 8, kp, half * NT, m0 / 16, kC / 16);
     {
       const int t = threadIdx.x >> 2;
       float f = 0.0f;
@@ -446,18 +551,6 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
       f += __shfl_xor_sync(0xffffffffu, f, 1);
       f += __shfl_xor_sync(0xffffffffu, f, 2);
       if ((threadIdx.x & 3) == 0) red[4 * kC + t] = f;
-    }
-    float end = gate[kC - 1] * sdot;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) end += __shfl_xor_sync(0xffffffffu, end, o);
-    if (lane == 0) wred[warp] = end;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      bdot[j] += __shfl_xor_sync(0xffffffffu, bdot[j], 1);
-      bdot[j] += __shfl_xor_sync(0xffffffffu, bdot[j], 2);
-      bdot[j] += __shfl_xor_sync(0xffffffffu, bdot[j], 4);
-      const int x = (threadIdx.x + j * kThreads) / (kSlice / 4);
-      if ((lane & 7) == 0 && x < rows) a.dbeta[((long)b * a.T + t0 + x) * a.Hv + hv] = bdot[j];
     }
     __syncthreads();
     if (warp == 0) {
@@ -492,47 +585,58 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
     // dq and dk of a key head are the sums over its value heads
     float* accq = a.dqk + (long)blockIdx.x * 2 * kC * DK;
     float* acck = accq + kC * DK;
-    const bool pair = a.dk % 2 == 0;
+    const bool even = a.dk % 2 == 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = frag_row(m0, e), col = frag_col(nb + n * 8);
+        const int row = frag_row(m0, e), col = frag_col((half * NT + n) * 8);
         float2 x = make_float2(dq[n][2 * e], dq[n][2 * e + 1]);
-        float2 y = make_float2(dkr[n][2 * e] + dkc[n][2 * e], dkr[n][2 * e + 1] + dkc[n][2 * e + 1]);
+        float2 z = make_float2(dkr[n][2 * e] + dkc[n][2 * e], dkr[n][2 * e + 1] + dkc[n][2 * e + 1]);
         float2* px = reinterpret_cast<float2*>(accq + row * DK + col);
-        float2* py = reinterpret_cast<float2*>(acck + row * DK + col);
+        float2* pz = reinterpret_cast<float2*>(acck + row * DK + col);
         if (r > 0) {
           x.x += px->x, x.y += px->y;
-          y.x += py->x, y.y += py->y;
+          z.x += pz->x, z.y += pz->y;
         }
         if (r + 1 < a.rep) {
           *px = x;
-          *py = y;
+          *pz = z;
         } else if (row < rows) {
           const long o = (((long)b * a.T + t0 + row) * a.Hk + hk) * a.dk + col;
-          set2<T>(static_cast<T*>(a.dq) + o, a.dk - col, pair, x.x, x.y);
-          set2<T>(static_cast<T*>(a.dk_) + o, a.dk - col, pair, y.x, y.y);
+          set2<T>(static_cast<T*>(a.dq) + o, a.dk - col, even, x.x, x.y);
+          set2<T>(static_cast<T*>(a.dk_) + o, a.dk - col, even, z.x, z.y);
         }
       }
   }
 }
 
+template <typename T, int DK, int STAGES>
+int launch_scan(const Problem& a, cudaStream_t stream) {
+  constexpr int bytes = BackSmem<Planes<T>::n, DK, STAGES>::bytes;
+  if (const int rc = with_smem(delta_back_scan_kernel<T, DK, STAGES>, bytes)) return rc;
+  delta_back_scan_kernel<T, DK, STAGES>
+      <<<(unsigned)((long)a.B * a.Hv * (a.dvp / kSlice)), kThreads, bytes, stream>>>(a);
+  GRU_CUDA_TRY(cudaGetLastError());
+  return GRU_OK;
+}
+
 template <typename T, int DK>
 int backward_typed(const Problem& a, cudaStream_t stream) {
-  using D = DoutSmem<T>;
-  using S = BackSmem<Planes<T>::n, DK>;
   using G = GradSmem<Planes<T>::n, DK>;
-  if (const int rc = with_smem(delta_dout_kernel<T>, D::bytes)) return rc;
-  if (const int rc = with_smem(delta_back_scan_kernel<T, DK>, S::bytes)) return rc;
   if (const int rc = with_smem(delta_grads_kernel<T, DK>, G::bytes)) return rc;
-  LaunchScope scope(kKindDeltaRule, stream, a.dout ? 3 : 2);
-  if (a.dout) {
-    delta_dout_kernel<T><<<(unsigned)((long)a.B * a.Hv * a.nc), kThreads, D::bytes, stream>>>(a);
-    GRU_CUDA_TRY(cudaGetLastError());
+  LaunchScope scope(kKindDeltaRule, stream, 2);
+  // one stage where two CTAs then share an SM and there are that many, or
+  // where two stages do not fit (FP32 inputs of 128 key columns)
+  constexpr int kMost = 227 * 1024;
+  constexpr bool fits = BackSmem<Planes<T>::n, DK, 2>::bytes <= kMost;
+  constexpr bool share = 2 * (BackSmem<Planes<T>::n, DK, 1>::bytes + 1024) <= 228 * 1024;
+  const bool many = (long)a.B * a.Hv * (a.dvp / kSlice) > 148;
+  if constexpr (fits) {
+    if (const int rc = many && share ? launch_scan<T, DK, 1>(a, stream) : launch_scan<T, DK, 2>(a, stream)) return rc;
+  } else {
+    if (const int rc = launch_scan<T, DK, 1>(a, stream)) return rc;
   }
-  delta_back_scan_kernel<T, DK><<<(unsigned)((long)a.B * a.Hv * (a.dvp / kSlice)), kThreads, S::bytes, stream>>>(a);
-  GRU_CUDA_TRY(cudaGetLastError());
   delta_grads_kernel<T, DK><<<(unsigned)((long)a.B * a.Hk * a.nc), kThreads, G::bytes, stream>>>(a);
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
@@ -541,7 +645,7 @@ int backward_typed(const Problem& a, cudaStream_t stream) {
 }  // namespace
 
 int backward(const Problem& a, int dtype, cudaStream_t stream) {
-  if (const int rc = prepare(a, dtype, stream)) return rc;
+  if (const int rc = prepare(a, dtype, false, stream)) return rc;
   if (dtype == GRU_F32)
     return a.dk <= 64 ? backward_typed<float, 64>(a, stream) : backward_typed<float, 128>(a, stream);
   return a.dk <= 64 ? backward_typed<bf16, 64>(a, stream) : backward_typed<bf16, 128>(a, stream);

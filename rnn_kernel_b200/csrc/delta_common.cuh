@@ -1,13 +1,20 @@
 // Shared device code of the gated delta rule's kernels (sm_100a).
 //
-// The chunked kernels need FP32-grade products (the states, the gates' and the
-// FP32 inputs' gradients are FP32), on tensor cores that multiply bf16: an FP32
-// operand is held as three bf16 planes x = x0 + x1 + x2 (x0 = bf16(x), x1 =
-// bf16(x - x0), x2 = bf16(x - x0 - x1): the residue is below 2^-26 |x|), and a
-// product of two such operands is the six plane products whose weight is above
-// 2^-24, a product with a bf16 operand (which is one plane, exactly) three.
+// The chunked kernels need FP32-grade products (states, gates' gradients and
+// FP32 tensors are FP32) from tensor cores that multiply 16-bit numbers.  An
+// FP32 tile is held as two FP16 planes with a common power of two, x = s (h + l),
+// h = fp16(x / s), l = fp16(x / s - h): s puts the tile's largest magnitude in
+// [2^14, 2^15), so a value keeps 22 bits down to 2^-17 of the largest, and
+// 2^-39 of the largest below.  A product of two such tiles is three plane
+// products (l h', h l', h h'; l l' is below 2^-22 of the result), half the work
+// of three bf16 planes.  bf16 inputs are one plane, exactly.
+//
+// Tiles in memory are made of 8 x 8 blocks of 128 consecutive bytes, the unit
+// that ldmatrix reads (transposed or not, without bank conflicts) and that a
+// warp's accumulators write as 32 x 4 bytes.
 #pragma once
 
+#include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -18,27 +25,28 @@
 namespace gru {
 namespace delta {
 
-constexpr int kC = 64;         // tokens per chunk
-constexpr int kSlice = 32;     // value columns that one CTA of a scan (one pass of a loop) works on
-constexpr int kThreads = 256;  // 8 warps: 4 tiles of 16 rows x 2 halves of the columns
+constexpr int kC = 64;      // tokens per chunk
+constexpr int kGroup = 16;  // value columns to a tile of states, errors and their gradients
+constexpr int kSlice = 32;  // value columns of a scan's CTA; they are padded to a multiple of this
+constexpr int kThreads = 256;
+constexpr int kTile = kC * kC;  // elements of a token x token tile
 
-constexpr int kGates = 5;      // rows of Problem::gates
+// Rows of Problem::gates, 64 floats each: e^G_i, e^(G_end - G_i), beta_i, G_i as
+// two floats, and the scales of the planes of W, P, K and Q.
+constexpr int kGates = 6;
+
 // Log decays below this count as this: e^-1000 is zero in FP32, and sums of 64
 // of them (in FP64) still tell neighbouring tokens apart, which -inf would not.
 constexpr float kNoDecay = -1000.0f;
 
 typedef __nv_bfloat16 bf16;
-
-// Rows of 16-bit elements in shared memory are padded by 16 bytes: the eight
-// 16-byte rows of an ldmatrix then fall into eight different bank groups for
-// every row length used here (32, 64, 128).
-__host__ __device__ constexpr int pitch(int cols) { return cols + 8; }
+typedef __half f16;
 
 template <typename T>
-struct Planes;  // planes that hold a value of the input type exactly
+struct Planes;  // planes of an input tensor
 template <>
 struct Planes<float> {
-  static constexpr int n = 3;
+  static constexpr int n = 2;
 };
 template <>
 struct Planes<bf16> {
@@ -55,28 +63,36 @@ struct Problem {
   int B, T, Hk, Hv, dk, dv;
   int rep;   // value heads per key head
   int nc;    // chunks
-  int dvp;   // dv rounded up to whole slices
+  int dvp;   // dv rounded up to a multiple of kSlice
   float scale;
-  // workspace; n = (b * H + h) * nc + chunk
-  bf16* kp;      // [n over Hk][NP][64][DK]
-  bf16* qp;      // [n over Hk][NP][64][DK]
-  bf16* wp;      // [n over Hv][3][64][64]
-  bf16* pp;      // [n over Hv][3][64][64]
-  float* gates;  // [n over Hv][kGates][64]: e^G_i, e^(G_end - G_i), beta_i, G_i as two floats
-  float* states; // [n over Hv][DK][dvp]: the state before the chunk
-  float* e;      // [n over Hv][64][dvp]: v - S'^T k, so that u = beta e
+  // workspace; n = (b * H + h) * nc + chunk, tiles of 8 x 8 blocks
+  f16* kp;       // [n over Hk][NP][64 x DK]
+  f16* qp;       // [n over Hk][NP][64 x DK]
+  f16* wp;       // [n over Hv][2][64 x 64]
+  f16* pp;       // [n over Hv][2][64 x 64]: P, for the output P B
+  float* gates;  // [n over Hv][kGates][64]
+  // Tiles of 16 value columns each, [n over Hv][plane][group][rows x 16], rows
+  // the key columns of a state or the tokens; every quarter of a tile's rows
+  // has its own scale, [n over Hv][group][4].
+  f16* states;   // the state before the chunk
+  float* sscale;
+  f16* e;        // v - S'^T k, so that u = beta e
+  float* escale;
   // gradient
   const void* dout;
   const float* ds_out;
   void *dq, *dk_, *dv_;
   float *dg, *dbeta, *ds0;
-  float* du0;    // [n over Hv][64][dvp]: P^T dO
-  float* z;      // [n over Hv][64][dvp]
-  float* dstates;// [n over Hv][DK][dvp]: the gradient of the state after the chunk
+  f16* z;
+  float* zscale;
+  f16* dstates;  // the gradient of the state after the chunk
+  float* dsscale;
+  f16* dop;      // the output's gradient, one plane if it is bf16
+  float* doscale;
   float* dqk;    // [n over Hk][2][64][DK]: dq and dk summed over a key head's value heads
 };
 
-int prepare(const Problem& a, int dtype, cudaStream_t stream);
+int prepare(const Problem& a, int dtype, bool fold_beta, cudaStream_t stream);
 int forward(const Problem& a, int dtype, cudaStream_t stream);
 int backward(const Problem& a, int dtype, cudaStream_t stream);
 
@@ -92,107 +108,88 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N));
 }
+// `bytes` (a multiple of 16) from global to shared memory, by all threads.
+__device__ __forceinline__ void copy_async(void* dst, const void* src, int bytes) {
+  for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16)
+    cp_async16(static_cast<char*>(dst) + i, static_cast<const char*>(src) + i);
+}
 
+template <bool TRANS>
 __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+  if (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
 }
-__device__ __forceinline__ void ldm4t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
+
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Two values as planes, packed {low half: a, high half: b}.
-template <int NP>
-__device__ __forceinline__ void split2(float a, float b, uint32_t (&w)[NP]) {
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    if (i + 1 < NP) {
-      a -= __uint_as_float(w[i] << 16);
-      b -= __uint_as_float(w[i] & 0xffff0000u);
-    }
-  }
+// ---------------------------------------------------------------------------
+// Operands in shared memory, COLS elements to a row of blocks.  Each function
+// gives this lane's address for the first block; moving by whole blocks adds
+// 128 bytes a column of blocks, 16 * COLS a row of blocks.
+// ---------------------------------------------------------------------------
+
+template <int COLS>
+__device__ __forceinline__ uint32_t block_addr(const f16* p, int r8, int c8) {
+  return smem_addr(p) + ((r8 * (COLS / 8) + c8) * 64 + (threadIdx.x & 7) * 8) * 2;
+}
+// A (16 rows m, 16 of k): stored [m][k], or [k][m] (TRANS).
+template <int COLS, bool TRANS>
+__device__ __forceinline__ uint32_t addr_a(const f16* p, int m8, int k8) {
+  const int i = (threadIdx.x >> 3) & 3;
+  return TRANS ? block_addr<COLS>(p, k8 + (i >> 1), m8 + (i & 1)) : block_addr<COLS>(p, m8 + (i & 1), k8 + (i >> 1));
+}
+// B (16 of k, two 8-column tiles n): stored [k][n] (TRANS), or [n][k].
+template <int COLS, bool TRANS>
+__device__ __forceinline__ uint32_t addr_b(const f16* p, int k8, int n8) {
+  const int i = (threadIdx.x >> 3) & 3;
+  return TRANS ? block_addr<COLS>(p, k8 + (i & 1), n8 + (i >> 1)) : block_addr<COLS>(p, n8 + (i >> 1), k8 + (i & 1));
 }
 
-// A tile in shared memory, as planes: `stride` elements from plane to plane.
-template <int NP, int PITCH>
-struct Tile {
-  bf16* p;
-  static constexpr int np = NP;
-  static constexpr int ld = PITCH;
-  template <int ROWS>
-  __device__ static constexpr int elems() { return NP * ROWS * PITCH; }
-};
-
-// acc[NT][4] += A (16 rows from m0) x B (NT * 8 columns from n0) over k in
-// [k0, k1) (multiples of 16).  A's planes hold [m][k] (TA false) or [k][m];
-// B's hold [k][n] (TB true) or [n][k].  sa / sb: elements between planes.
-//
-// The tensor core truncates when it adds into its accumulator.  So every 32 of
-// k go into fresh accumulators, smallest plane products first, and those are
-// added to acc in FP32 (rounded to nearest).
-template <int NA, int NB, bool TA, bool TB, int NT>
-__device__ __forceinline__ void mma_tile(float (&acc)[NT][4], const bf16* a, int sa, int lda, int m0, const bf16* b,
-                                         int sb, int ldb, int n0, int k0, int k1) {
-  static_assert(NT % 2 == 0, "pairs of 8-column tiles");
-  const int lane = threadIdx.x & 31;
-  const uint32_t pa = smem_addr(a) + 2 * (TA ? ((lane & 7) + (lane >> 4) * 8) * lda + m0 + ((lane >> 3) & 1) * 8
-                                             : (m0 + (lane & 15)) * lda + (lane >> 4) * 8);
-  const uint32_t pb = smem_addr(b) + 2 * (TB ? (lane & 15) * ldb + n0 + (lane >> 4) * 8
-                                             : (n0 + (lane & 7) + (lane >> 4) * 8) * ldb + ((lane >> 3) & 1) * 8);
-  constexpr int kTop = (NA > NB ? NA : NB) - 1;  // planes i, j with i + j <= kTop
-  for (int kb = k0; kb < k1; kb += 32) {
-    float t[NT][4];
+// t[n] += A B_n over one step of 16 in k, smallest plane products first.  The
+// tensor core truncates when it adds into its accumulator, so callers give
+// every step fresh accumulators and add those up in FP32 (rounded to nearest).
+template <int NA, int NB, int NT>
+__device__ __forceinline__ void mma_terms(float (&t)[NT][4], const uint32_t (&fa)[NA][4], const uint32_t (&fb)[NB][NT][2]) {
+  constexpr int kTop = (NA > NB ? NA : NB) - 1;
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+  for (int s = kTop; s >= 0; --s)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) t[i][j] = 0.0f;
+    for (int i = 0; i <= s; ++i)
+      if (i < NA && s - i < NB) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = kb + 16 * h;
-      if (k < k1) {
-        uint32_t fa[NA][4];
-#pragma unroll
-        for (int i = 0; i < NA; ++i) {
-          const uint32_t at = pa + 2 * (i * sa + (TA ? k * lda : k));
-          if (TA) ldm4t(fa[i], at); else ldm4(fa[i], at);
-        }
-#pragma unroll
-        for (int n = 0; n < NT; n += 2) {
-          uint32_t fb[NB][4];
-#pragma unroll
-          for (int i = 0; i < NB; ++i) {
-            const uint32_t at = pb + 2 * (i * sb + (TB ? k * ldb + n * 8 : n * 8 * ldb + k));
-            if (TB) ldm4t(fb[i], at); else ldm4(fb[i], at);
-          }
-#pragma unroll
-          for (int s = kTop; s >= 0; --s)
-#pragma unroll
-            for (int i = 0; i <= s; ++i) {
-              const int j = s - i;
-              if (i < NA && j < NB) {
-                mma(t[n], fa[i], fb[j][0], fb[j][1]);
-                mma(t[n + 1], fa[i], fb[j][2], fb[j][3]);
-              }
-            }
-        }
+        for (int n = 0; n < NT; ++n) mma(t[n], fa[i], fb[s - i][n][0], fb[s - i][n][1]);
       }
+}
+
+// B fragments of NT (even) tiles: `next` bytes from one pair of tiles to the
+// next, `plane` bytes from plane to plane.
+template <int NB, int NT, bool TRANS>
+__device__ __forceinline__ void load_b(uint32_t (&fb)[NB][NT][2], uint32_t addr, int next, int plane) {
+#pragma unroll
+  for (int p = 0; p < NB; ++p)
+#pragma unroll
+    for (int n = 0; n < NT; n += 2) {
+      uint32_t r[4];
+      ldm4<TRANS>(r, addr + p * plane + (n / 2) * next);
+      fb[p][n][0] = r[0], fb[p][n][1] = r[1], fb[p][n + 1][0] = r[2], fb[p][n + 1][1] = r[3];
     }
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] += t[i][j];
-  }
 }
 
 template <int NT>
@@ -208,36 +205,76 @@ __device__ __forceinline__ void zero(float (&acc)[NT][4]) {
 __device__ __forceinline__ int frag_row(int m0, int h) { return m0 + ((threadIdx.x & 31) >> 2) + 8 * h; }
 __device__ __forceinline__ int frag_col(int n0) { return n0 + (threadIdx.x & 3) * 2; }
 
-// Stores (a, b) at [row][col], [row][col + 1] of each plane.
+// ---------------------------------------------------------------------------
+// Planes.
+// ---------------------------------------------------------------------------
+
+// 1 / s for a tile whose largest magnitude is m (a finite number).  Tiles
+// below 2^-100 share the scale of 2^-100.
+__device__ __forceinline__ float plane_inv(float m) {
+  const int eb = max((int)(__float_as_uint(m) >> 23), 27);
+  return __uint_as_float((unsigned)(268 - eb) << 23);
+}
+__device__ __forceinline__ float plane_scale(float inv) { return __uint_as_float((254u << 23) - __float_as_uint(inv)); }
+
+// Two values (times inv) as planes, packed {low half: a, high half: b}.
 template <int NP>
-__device__ __forceinline__ void put2(bf16* p, int plane, int ld, int row, int col, float a, float b) {
-  uint32_t w[NP];
-  split2<NP>(a, b, w);
-#pragma unroll
-  for (int i = 0; i < NP; ++i) *reinterpret_cast<uint32_t*>(p + i * plane + row * ld + col) = w[i];
+__device__ __forceinline__ void split2(float a, float b, float inv, uint32_t (&w)[NP]) {
+  a *= inv;
+  b *= inv;
+  const __half2 h = __floats2half2_rn(a, b);
+  w[0] = *reinterpret_cast<const uint32_t*>(&h);
+  if (NP == 2) {
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    w[NP - 1] = *reinterpret_cast<const uint32_t*>(&l);
+  }
 }
 
-// Four consecutive values, zero past `left`.
-template <typename T>
-__device__ __forceinline__ float4 get4(const T* p, int left, bool vec);
-template <>
-__device__ __forceinline__ float4 get4<float>(const float* p, int left, bool vec) {
-  if (vec && left >= 4) return *reinterpret_cast<const float4*>(p);
-  return make_float4(left > 0 ? p[0] : 0.f, left > 1 ? p[1] : 0.f, left > 2 ? p[2] : 0.f, left > 3 ? p[3] : 0.f);
+// The larger magnitude of two numbers, NaN and infinities aside (they must not
+// take the other values' scale).
+__device__ __forceinline__ float max_finite(float m, float x) {
+  const float y = fabsf(x);
+  return fmaxf(m, y <= 3.4028235e38f ? y : 0.0f);
 }
-template <>
-__device__ __forceinline__ float4 get4<bf16>(const bf16* p, int left, bool vec) {
-  if (vec && left >= 4) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                       __uint_as_float(u.y & 0xffff0000u));
-  }
-  return make_float4(left > 0 ? __bfloat162float(p[0]) : 0.f, left > 1 ? __bfloat162float(p[1]) : 0.f,
-                     left > 2 ? __bfloat162float(p[2]) : 0.f, left > 3 ? __bfloat162float(p[3]) : 0.f);
+// Writes an accumulator pair (row block r8, column tile n) of a tile of 16
+// columns, `plane` elements between planes.
+template <int NP>
+__device__ __forceinline__ void store_pair(f16* tile, long plane, int r8, int n, const uint32_t (&w)[NP]) {
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+    reinterpret_cast<uint32_t*>(tile + p * plane)[(r8 * 2 + n) * 32 + (threadIdx.x & 31)] = w[p];
+}
+
+// ---------------------------------------------------------------------------
+// Elements of either input type.
+// ---------------------------------------------------------------------------
+
+// Four consecutive values of a row, aligned to four, zero where `in` is false.
+// No branch, so that a thread's loads are all in flight together: a value
+// that is not there is read from `safe` and dropped.
+__device__ __forceinline__ float4 load4(const float* p, const float* safe, bool in) {
+  const float4 f = *reinterpret_cast<const float4*>(in ? p : safe);
+  return in ? f : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+}
+__device__ __forceinline__ float4 load4(const bf16* p, const bf16* safe, bool in) {
+  const uint2 u = *reinterpret_cast<const uint2*>(in ? p : safe);
+  return in ? make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                          __uint_as_float(u.y & 0xffff0000u))
+            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 }
 
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(bf16 x) { return __bfloat162float(x); }
+// The same element by element, for rows that are not aligned or not a multiple
+// of four long; `left` elements are there.
+template <typename T>
+__device__ __forceinline__ float4 load4_any(const T* p, const T* safe, int left) {
+  const float x = as_float(*(left > 0 ? p : safe)), y = as_float(*(left > 1 ? p + 1 : safe));
+  const float z = as_float(*(left > 2 ? p + 2 : safe)), w = as_float(*(left > 3 ? p + 3 : safe));
+  return make_float4(left > 0 ? x : 0.0f, left > 1 ? y : 0.0f, left > 2 ? z : 0.0f, left > 3 ? w : 0.0f);
+}
+
 template <typename T>
 __device__ __forceinline__ T as_type(float x);
 template <>
@@ -267,31 +304,75 @@ __device__ __forceinline__ void set2<bf16>(bf16* p, int left, bool vec, float a,
   }
 }
 
+// A warp's 16 tokens x 16 value columns of a [token][column] tensor, as
+// accumulator tiles.  `start` issues the loads and `get` gives a value pair,
+// zero where the tensor has none: nothing between the two waits for memory.
+template <typename T>
+struct PairOf;
+template <>
+struct PairOf<float> {
+  typedef float2 type;
+  static __device__ __forceinline__ float2 make(float x, float y) { return make_float2(x, y); }
+  static __device__ __forceinline__ float2 get(float2 r) { return r; }
+};
+template <>
+struct PairOf<bf16> {
+  typedef uint32_t type;
+  static __device__ __forceinline__ uint32_t make(bf16 x, bf16 y) {
+    return __bfloat16_as_ushort(x) | (uint32_t)__bfloat16_as_ushort(y) << 16;
+  }
+  static __device__ __forceinline__ float2 get(uint32_t r) {
+    return make_float2(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
+  }
+};
+template <typename T>
+struct Columns {
+  typename PairOf<T>::type raw[2][2];
+  int tokens, cols;  // that there are from the tile's first on
+  // vec: columns and strides are even and p is aligned to two elements
+  __device__ __forceinline__ void start(const T* p, long stride, int tokens_, int cols_, bool vec) {
+    tokens = tokens_;
+    cols = cols_;
+    if (tokens <= 0 || cols <= 0) return;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int c = frag_col(n * 8);
+        const T* q = p + min(frag_row(0, e), tokens - 1) * stride;
+        if (vec) raw[n][e] = *reinterpret_cast<const typename PairOf<T>::type*>(q + (c < cols ? c : 0));
+        else raw[n][e] = PairOf<T>::make(q[min(c, cols - 1)], q[min(c + 1, cols - 1)]);
+      }
+  }
+  __device__ __forceinline__ float2 get(int n, int e) const {
+    float2 f = PairOf<T>::get(raw[n][e]);
+    const int c = frag_col(n * 8);
+    const bool in = frag_row(0, e) < tokens;
+    f.x = in && c < cols ? f.x : 0.0f;
+    f.y = in && c + 1 < cols ? f.y : 0.0f;
+    return f;
+  }
+};
+template <typename T>
+__device__ __forceinline__ bool pairs_ok(const void* p, long s0, long s1, long s2, int cols) {
+  return (reinterpret_cast<uintptr_t>(p) & (2 * sizeof(T) - 1)) == 0 && ((s0 | s1 | s2 | cols) & 1) == 0;
+}
+
+// The largest finite magnitude of a warp's tile.
+template <int NT>
+__device__ __forceinline__ float warp_max(const float (&x)[NT][4]) {
+  float m = 0.0f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = max_finite(m, x[n][e]);
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+}
+
 template <typename K>
 inline int with_smem(K kernel, int bytes) {
   GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   return GRU_OK;
-}
-
-// Rows of `cols` 16-bit elements from a dense array into padded shared rows.
-template <int COLS>
-__device__ __forceinline__ void copy_rows(bf16* dst, const bf16* src, int rows) {
-  constexpr int per = COLS / 8;
-  for (int i = threadIdx.x; i < rows * per; i += kThreads) {
-    const int r = i / per, c = i % per;
-    cp_async16(dst + r * pitch(COLS) + c * 8, src + (long)r * COLS + c * 8);
-  }
-}
-
-// rows x kSlice FP32 values (row stride ld) as planes in padded shared rows.
-template <int NP>
-__device__ __forceinline__ void load_slice(bf16* dst, int plane, const float* src, long ld, int rows) {
-  for (int i = threadIdx.x; i < rows * (kSlice / 4); i += kThreads) {
-    const int r = i / (kSlice / 4), c = (i % (kSlice / 4)) * 4;
-    const float4 f = *reinterpret_cast<const float4*>(src + r * ld + c);
-    put2<NP>(dst, plane, pitch(kSlice), r, c, f.x, f.y);
-    put2<NP>(dst, plane, pitch(kSlice), r, c + 2, f.z, f.w);
-  }
 }
 
 }  // namespace delta

@@ -44,10 +44,15 @@ __global__ void __launch_bounds__(kThreads) delta_step_kernel(const Step a) {
   float* s = a.s + (long)bh * a.dk * a.dv + c;
   const int left = a.dv - c;
   float4 x[kMaxD / 32];
+  const float* safe = a.s + (long)bh * a.dk * a.dv;
+  if (a.vec) {
 #pragma unroll
-  for (int i = 0; i < kMaxD / 32; ++i) {
-    const int r = row0 + 32 * i;
-    x[i] = get4<float>(s + (long)r * a.dv, r < a.dk ? left : 0, a.vec);
+    for (int i = 0; i < kMaxD / 32; ++i)
+      x[i] = load4(s + (long)(row0 + 32 * i) * a.dv, safe, row0 + 32 * i < a.dk && left > 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kMaxD / 32; ++i)
+      x[i] = load4_any(s + (long)(row0 + 32 * i) * a.dv, safe, row0 + 32 * i < a.dk ? left : 0);
   }
   if (threadIdx.x < kMaxD) {
     const int d = threadIdx.x;
@@ -107,7 +112,8 @@ __global__ void __launch_bounds__(kThreads) delta_step_kernel(const Step a) {
     const float kr = ks[r];
     const float4 y = make_float4(x[i].x + kr * u.x, x[i].y + kr * u.y, x[i].z + kr * u.z, x[i].w + kr * u.w);
     float* p = s + (long)r * a.dv;
-    if (a.vec && left >= 4) {
+    if (a.vec) {
+      if (left <= 0) continue;
       *reinterpret_cast<float4*>(p) = y;
     } else {
       if (left > 0) p[0] = y.x;
@@ -174,23 +180,28 @@ void fill(Problem& a, const gru_delta_args& p) {
 }
 
 void lay_stash(Problem& a, const gru_delta_args& p, Arena& m) {
-  const size_t n = (size_t)a.B * a.Hv * a.nc;
-  a.states = m.take<float>(n * key_width(p) * a.dvp);
-  a.e = m.take<float>(n * kC * a.dvp);
+  const size_t n = (size_t)a.B * a.Hv * a.nc, groups = a.dvp / kGroup;
+  a.states = m.take<f16>(n * 2 * a.dvp * key_width(p));
+  a.sscale = m.take<float>(n * groups * 4);
+  a.e = m.take<f16>(n * 2 * a.dvp * kC);
+  a.escale = m.take<float>(n * groups * 4);
 }
 
 void lay_workspace(Problem& a, const gru_delta_args& p, Arena& m, bool backward) {
   const size_t nk = (size_t)a.B * a.Hk * a.nc, nv = (size_t)a.B * a.Hv * a.nc, w = key_width(p);
-  const size_t np = p.dtype == GRU_F32 ? 3 : 1;
-  a.kp = m.take<bf16>(nk * np * kC * w);
-  a.qp = m.take<bf16>(nk * np * kC * w);
-  a.wp = m.take<bf16>(nv * 3 * kC * kC);
-  a.pp = m.take<bf16>(nv * 3 * kC * kC);
+  const size_t np = p.dtype == GRU_F32 ? 2 : 1, groups = a.dvp / kGroup;
+  a.kp = m.take<f16>(nk * np * kC * w);
+  a.qp = m.take<f16>(nk * np * kC * w);
+  a.wp = m.take<f16>(nv * 2 * kTile);
+  a.pp = m.take<f16>(nv * 2 * kTile);
   a.gates = m.take<float>(nv * kGates * kC);
   if (!backward) return;
-  a.du0 = m.take<float>(nv * kC * a.dvp);
-  a.z = m.take<float>(nv * kC * a.dvp);
-  a.dstates = m.take<float>(nv * w * a.dvp);
+  a.z = m.take<f16>(nv * 2 * a.dvp * kC);
+  a.zscale = m.take<float>(nv * groups * 4);
+  a.dstates = m.take<f16>(nv * 2 * a.dvp * w);
+  a.dsscale = m.take<float>(nv * groups * 4);
+  a.dop = m.take<f16>(nv * np * a.dvp * kC);
+  a.doscale = m.take<float>(nv * groups * 4);
   a.dqk = m.take<float>(a.rep > 1 ? nk * 2 * kC * w : 0);
 }
 
