@@ -39,9 +39,9 @@ template <int NP, int DK, int STAGES>
 struct BackSmem {
   static constexpr int k = NP * kC * DK, w = 2 * kTile;  // elements; K, Q, W, P
   static constexpr int stage = 2 * (k + w) * 2 + kGates * kC * 4;
-  // two planes of two groups (of dO, NP): dS, B dU, e^G B Z; dO; e^G dO twice
+  // two planes of two groups (of dO, NP): dS, B dU, e^G B Z, e^G dO; dO
   static constexpr int s = 4 * kGroup * DK, x = 4 * kGroup * kC, o = NP * 2 * kGroup * kC;
-  static constexpr int bytes = STAGES * stage + (s + 4 * x + o) * 2 + 6 * 8 * 4;
+  static constexpr int bytes = STAGES * stage + (s + 3 * x + o) * 2 + 5 * 8 * 4;
 };
 
 template <int NP, int DK>
@@ -86,17 +86,17 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
   extern __shared__ __align__(16) unsigned char smem[];
   const int slices = a.dvp / kSlice, groups = a.dvp / kGroup;
   const int bh = blockIdx.x / slices, hv = bh % a.Hv, b = bh / a.Hv;
-  const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3, pair = threadIdx.x >> 7;
+  const int quarter = (threadIdx.x >> 5) & 3, pair = threadIdx.x >> 7;
   const int group = (blockIdx.x % slices) * 2 + pair, c0 = group * kGroup;
   const long nv0 = (long)bh * a.nc, nk0 = ((long)b * a.Hk + hv / a.rep) * a.nc;
   f16* base = reinterpret_cast<f16*>(smem + STAGES * L::stage);
   f16* sp = base + pair * kGroup * DK;
   f16* up = base + L::s + pair * kGroup * kC;  // B dU
   f16* zp = up + L::x;                         // -e^G B Z
-  f16* qop = zp + L::x;                        // scale e^G dO, of this chunk and of the next
-  f16* op = base + L::s + 4 * L::x + pair * kGroup * kC;
-  float* scales = reinterpret_cast<float*>(base + L::s + 4 * L::x + L::o) + pair * 4;
-  float *ssc = scales, *usc = scales + 8, *zsc = scales + 16, *qosc = scales + 24, *osc = scales + 40;
+  f16* qop = zp + L::x;                        // scale e^G dO
+  f16* op = base + L::s + 3 * L::x + pair * kGroup * kC;
+  float* scales = reinterpret_cast<float*>(base + L::s + 3 * L::x + L::o) + pair * 4;
+  float *ssc = scales, *usc = scales + 8, *zsc = scales + 16, *qosc = scales + 24, *osc = scales + 32;
 
   float d[MT][2][4];  // the gradient of the state after the chunk
   const float* ds = a.ds_out ? a.ds_out + (long)bh * a.dk * a.dv : nullptr;
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[n][e] *= a.scale * gate[frag_row(quarter * 16, e >> 1)];
-    put_tokens<2>(x, quarter, qop + (chunk & 1) * L::x, qosc + (chunk & 1) * 8, nullptr, 0, nullptr);
+    put_tokens<2>(x, quarter, qop, qosc, nullptr, 0, nullptr);
   };
   auto state_out = [&](int chunk) {
     const long nv = nv0 + chunk;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[m][n][e] *= decay;
-    add_to_state<NP, DK>(d, qp, quarter, qop + (chunk & 1) * L::x, qosc + (chunk & 1) * 8, sq);
+    add_to_state<NP, DK>(d, qp, quarter, qop, qosc, sq);
     add_to_state<NP, DK>(d, kp, quarter, zp, zsc, sk);
     state_out(chunk - 1);
     if (STAGES == 1 && chunk > 0) {
@@ -229,20 +229,25 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
 
 // ---------------------------------------------------------------------------
 // grads: one CTA per (batch, key head, chunk).  It walks the value columns in
-// steps of 16 (one step of the products' inner dimension, one scale), three
-// steps in flight; a warp keeps 16 tokens x half of the key columns of dQ,
-// dK_row and dK_col, and of 32 tokens of dO U^T and Z U^T, in registers.
+// steps of 16 (one step of the products' inner dimension), three steps in
+// flight; each of 16 warps keeps 16 tokens x a quarter of the key columns of dQ,
+// dK_row and dK_col, and of 16 tokens of dO U^T and Z U^T, in registers.  (Eight
+// warps of twice the tile had one CTA an SM as well, at 255 registers: 373 us for
+// train 4 x 2048 x 16 heads of 128.)
 // ---------------------------------------------------------------------------
+
+constexpr int kGradThreads = 512;
 
 template <int NP, int DK>
 struct GradSmem {
   static constexpr int qk = NP * kC * DK;  // elements
   static constexpr int s = 2 * kGroup * DK, x = 2 * kGroup * kC, o = NP * kGroup * kC;
-  static constexpr int stage = 2 * s + 2 * x + o;  // S, dS, E, Z, dO of 16 columns
+  static constexpr int planes = 2 * s + 2 * x + o;  // S, dS, E, Z, dO of 16 columns
+  static constexpr int stage = planes + 5 * 8;       // and their scales
   static constexpr int stages = 3;
   static constexpr int tiles = 4 * kTile * 2 + kC * (kC + 1) * 4;  // bytes: dP', M; y in FP32; over the stages
   static constexpr int main = stages * stage * 2 > tiles ? stages * stage * 2 : tiles;
-  static constexpr int bytes = 2 * qk * 2 + (main + 15) / 16 * 16 + kGates * kC * 4 + (5 * kC + 32) * 4;
+  static constexpr int bytes = 2 * qk * 2 + (main + 15) / 16 * 16 + kGates * kC * 4 + (9 * kC + 48) * 4;
 };
 
 template <int NP, int DK>
@@ -259,6 +264,12 @@ __device__ __forceinline__ void grad_load(f16* dst, const Problem& a, long nv, i
   for (int p = 0; p < NP; ++p)
     copy_async(dst + 2 * L::s + 2 * L::x + p * kGroup * kC, a.dop + (nv * NP + p) * a.dvp * kC + (long)c0 * kC,
                kGroup * kC * 2);
+  const long g = (nv * (a.dvp / kGroup) + c0 / kGroup) * 4;
+  if (threadIdx.x < 5) {
+    const float* from = threadIdx.x == 0 ? a.sscale : threadIdx.x == 1 ? a.dsscale : threadIdx.x == 2 ? a.escale
+                      : threadIdx.x == 3 ? a.zscale : a.doscale;
+    cp_async16(dst + L::planes + threadIdx.x * 8, from + g);
+  }
 }
 
 // The value pair `word` of a tile held as planes, without its scale.
@@ -278,18 +289,16 @@ __device__ __forceinline__ float2 pair(uint32_t h, uint32_t l) {
   return make_float2(x.x + y.x, x.y + y.y);
 }
 
-// acc[n ..] += A B, one step of 16 and four tiles, times f0 (the first two
-// tiles) or f1.
+// acc += f A B, one step of 16.
 template <int NA, int NB, int NT>
-__device__ __forceinline__ void step_add(float (&acc)[NT][4], int n, float f0, float f1, const uint32_t (&fa)[NA][4],
-                                         const uint32_t (&fb)[NB][4][2]) {
-  float t[4][4];
-  zero(t);
-  mma_terms<NA, NB, 4>(t, fa, fb);
+__device__ __forceinline__ void step_add(float (&acc)[NT][4], float f, const uint32_t (&fa)[NA][4],
+                                         const uint32_t (&fb)[NB][NT][2]) {
+  float t[NT][4];
+  mma_terms<NA, NB, NT>(t, fa, fb);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[n + i][e] += (i < 2 ? f0 : f1) * t[i][e];
+    for (int e = 0; e < 4; ++e) acc[i][e] += f * t[i][e];
 }
 
 // acc += f A B over steps [k0, k1) of the tokens: A a 64 x 64 tile (rows m, or
@@ -298,24 +307,19 @@ template <int NP, int DK, bool TA, int NT>
 __device__ __forceinline__ void token_product(float (&acc)[NT][4], float f, const f16* A, int m8, const f16* B, int n8,
                                               int k0, int k1) {
   for (int kk = k0; kk < k1; ++kk) {
-    uint32_t fa[2][4];
+    uint32_t fa[2][4], fb[NP][NT][2];
     const uint32_t pa = addr_a<kC, TA>(A, m8, 2 * kk);
 #pragma unroll
     for (int p = 0; p < 2; ++p) ldm4<TA>(fa[p], pa + p * kTile * 2);
-    const uint32_t pb = addr_b<DK, true>(B, 2 * kk, n8);
-#pragma unroll
-    for (int n = 0; n < NT; n += 4) {
-      uint32_t fb[NP][4][2];
-      load_b<NP, 4, true>(fb, pb + n * 128, 256, kC * DK * 2);
-      step_add<2, NP, NT>(acc, n, f, f, fa, fb);
-    }
+    load_b<NP, NT, true>(fb, addr_b<DK, true>(B, 2 * kk, n8), 256, kC * DK * 2);
+    step_add<2, NP, NT>(acc, f, fa, fb);
   }
 }
 
 template <typename T, int DK>
-__global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) {
+__global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem a) {
   constexpr int NP = Planes<T>::n;
-  constexpr int NT = DK / 16;  // a warp's half of the key columns, in 8-column tiles
+  constexpr int NT = DK / 32;  // a warp's quarter of the key columns, in 8-column tiles
   using L = GradSmem<NP, DK>;
   extern __shared__ __align__(16) unsigned char smem[];
   f16* qp = reinterpret_cast<f16*>(smem);
@@ -325,14 +329,14 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
   f16* mp = dpp + 2 * kTile;
   float* y = reinterpret_cast<float*>(mp + 2 * kTile);  // [64][65]
   float* gate = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(main) + (L::main + 15) / 16 * 16);
-  float* red = gate + kGates * kC;  // x and z of the two column halves, F; then values per warp
-  float* wred = red + 5 * kC;
+  float* red = gate + kGates * kC;  // x and z of the four column quarters, F; then values per warp
+  float* wred = red + 9 * kC;
 
   const int chunk = blockIdx.x % a.nc, bh = blockIdx.x / a.nc;
   const int hk = bh % a.Hk, b = bh / a.Hk;
   const int t0 = chunk * kC, rows = min(kC, a.T - t0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m0 = (warp >> 1) * 16, half = warp & 1;
+  const int m0 = (warp >> 2) * 16, col = warp & 3;  // this warp's tokens; its quarter of the columns
   const int groups = a.dvp / kGroup;
 
   copy_async(qp, a.qp + (long)blockIdx.x * L::qk, L::qk * 2);
@@ -347,7 +351,7 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
     cp_async_commit();
     grad_load<NP, DK>(main + L::stage, a, nv, kGroup);  // dvp is a multiple of two groups
     cp_async_commit();
-    float dp[4][4], da[4][4], dq[NT][4], dkr[NT][4], dkc[NT][4];
+    float dp[2][4], da[2][4], dq[NT][4], dkr[NT][4], dkc[NT][4];
     zero(dp);
     zero(da);
     zero(dq);
@@ -366,42 +370,16 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
       const f16* op = zp + L::x;
       // scales: of this warp's 16 tokens, of its 32 columns of tokens, and of the
       // quarters of the key columns
-      const long sg = (nv * groups + g) * 4;
+      const float* scales = reinterpret_cast<const float*>(sp + L::planes);  // of S, dS, E, Z, dO
       const int mq = m0 / 16;
-      const float se = fabsf(a.escale[sg + mq]), sz = a.zscale[sg + mq], so = a.doscale[sg + mq];
-      const float se0 = fabsf(a.escale[sg + 2 * half]), se1 = fabsf(a.escale[sg + 2 * half + 1]);
-      const float4 ss = *reinterpret_cast<const float4*>(a.sscale + sg);
-      const float4 sd = *reinterpret_cast<const float4*>(a.dsscale + sg);
-      uint32_t fo[NP][4], fz[2][4], fe[2][4];
-#pragma unroll
-      for (int p = 0; p < NP; ++p) ldm4<false>(fo[p], addr_a<kGroup, false>(op, m0 / 8, 0) + p * kGroup * kC * 2);
+      const float se = fabsf(scales[8 + mq]), sz = scales[12 + mq], so = scales[16 + mq];
+      uint32_t fz[2][4], fe[2][4];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         ldm4<false>(fz[p], addr_a<kGroup, false>(zp, m0 / 8, 0) + p * kGroup * kC * 2);
         ldm4<false>(fe[p], addr_a<kGroup, false>(ep, m0 / 8, 0) + p * kGroup * kC * 2);
       }
-      if (half * 32 <= m0) {
-        uint32_t fb[2][4][2];
-        load_b<2, 4, false>(fb, addr_b<kGroup, false>(ep, 0, half * 4), 512, kGroup * kC * 2);
-        step_add<NP, 2, 4>(dp, 0, so * se0, so * se1, fo, fb);
-        step_add<2, 2, 4>(da, 0, sz * se0, sz * se1, fz, fb);
-      }
-#pragma unroll
-      for (int n = 0; n < NT; n += 4) {
-        // tiles n, n + 2 of this half lie in these quarters (of DK / 32 tiles)
-        const bool odd = DK == 128 ? n >= 4 : false;
-        const float s0 = half ? (odd ? ss.w : ss.z) : (odd ? ss.y : ss.x);
-        const float s1 = DK == 128 ? s0 : (half ? ss.w : ss.y);
-        const float d0 = half ? (odd ? sd.w : sd.z) : (odd ? sd.y : sd.x);
-        const float d1 = DK == 128 ? d0 : (half ? sd.w : sd.y);
-        uint32_t fb[2][4][2];
-        load_b<2, 4, false>(fb, addr_b<kGroup, false>(sp, 0, half * NT + n), 512, kGroup * DK * 2);
-        step_add<NP, 2, NT>(dq, n, so * s0, so * s1, fo, fb);
-        step_add<2, 2, NT>(dkr, n, sz * s0, sz * s1, fz, fb);
-        load_b<2, 4, false>(fb, addr_b<kGroup, false>(dsp, 0, half * NT + n), 512, kGroup * DK * 2);
-        step_add<2, 2, NT>(dkc, n, se * d0, se * d1, fe, fb);
-      }
-      if (half == 0) {
+      if (col == 0) {
         // Z . E of this lane's two tokens
         const float f = sz * se;
 #pragma unroll
@@ -410,14 +388,33 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
           bdot[j & 1] += f * (u.x * w.x + u.y * w.y);
         }
       }
+      {
+        uint32_t fb[2][NT][2];
+        load_b<2, NT, false>(fb, addr_b<kGroup, false>(dsp, 0, col * NT), 512, kGroup * DK * 2);
+        step_add<2, 2, NT>(dkc, se * scales[4 + col], fe, fb);
+      }
+      uint32_t fo[NP][4];
 #pragma unroll
-      for (int i = 0; i < kGroup * DK / 2 / kThreads; ++i) {
-        // block warp + 8 i is of the rows 8 (warp / 2 + 4 i) ..., in this quarter
-        const int w = threadIdx.x + i * kThreads, q = (warp / 2 + 4 * i) * 8 / (DK / 4);
+      for (int p = 0; p < NP; ++p) ldm4<false>(fo[p], addr_a<kGroup, false>(op, m0 / 8, 0) + p * kGroup * kC * 2);
+      {
+        uint32_t fb[2][NT][2];
+        load_b<2, NT, false>(fb, addr_b<kGroup, false>(sp, 0, col * NT), 512, kGroup * DK * 2);
+        step_add<NP, 2, NT>(dq, so * scales[col], fo, fb);
+        step_add<2, 2, NT>(dkr, sz * scales[col], fz, fb);
+      }
+      if (col <= mq) {
+        uint32_t fb[2][2][2];
+        load_b<2, 2, false>(fb, addr_b<kGroup, false>(ep, 0, col * 2), 512, kGroup * kC * 2);
+        const float f = fabsf(scales[8 + col]);
+        step_add<NP, 2, 2>(dp, so * f, fo, fb);
+        step_add<2, 2, 2>(da, sz * f, fz, fb);
+      }
+#pragma unroll
+      for (int i = 0; i < kGroup * DK / 2 / kGradThreads; ++i) {
+        // block warp + 16 i is of the rows 8 (warp / 2 + 8 i) ..., in this quarter
+        const int w = threadIdx.x + i * kGradThreads, q = (warp / 2 + 8 * i) * 8 / (DK / 4);
         const float2 u = take2<2>(sp, kGroup * DK, w), v = take2<2>(dsp, kGroup * DK, w);
-        const float fs = q == 0 ? ss.x : q == 1 ? ss.y : q == 2 ? ss.z : ss.w;
-        const float fd = q == 0 ? sd.x : q == 1 ? sd.y : q == 2 ? sd.z : sd.w;
-        sdot += (fs * fd) * (u.x * v.x + u.y * v.y);
+        sdot += (scales[q] * scales[4 + q]) * (u.x * v.x + u.y * v.y);
       }
     }
     __syncthreads();
@@ -425,28 +422,27 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
     const float sk = gate[5 * kC + 2], sq = gate[5 * kC + 3];
     float mu = 0.0f, mw = 0.0f;
     {
-      float qk[4][4], kk[4][4];
+      float qk[2][4], kk[2][4];
       zero(qk);
       zero(kk);
-      if (half * 32 <= m0) {
+      if (col <= m0 / 16) {
 #pragma unroll
         for (int k = 0; k < DK / 16; ++k) {
-          uint32_t fq[NP][4], fk[NP][4], fb[NP][4][2];
+          uint32_t fa[NP][4], fb[NP][2][2];
+          load_b<NP, 2, false>(fb, addr_b<DK, false>(kp, 2 * k, col * 2), 0, kC * DK * 2);
 #pragma unroll
-          for (int p = 0; p < NP; ++p) {
-            ldm4<false>(fq[p], addr_a<DK, false>(qp, m0 / 8, 2 * k) + p * kC * DK * 2);
-            ldm4<false>(fk[p], addr_a<DK, false>(kp, m0 / 8, 2 * k) + p * kC * DK * 2);
-          }
-          load_b<NP, 4, false>(fb, addr_b<DK, false>(kp, 2 * k, half * 4), 32 * DK, kC * DK * 2);
-          step_add<NP, NP, 4>(qk, 0, sq * sk, sq * sk, fq, fb);
-          step_add<NP, NP, 4>(kk, 0, sk * sk, sk * sk, fk, fb);
+          for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], addr_a<DK, false>(qp, m0 / 8, 2 * k) + p * kC * DK * 2);
+          step_add<NP, NP, 2>(qk, sq * sk, fa, fb);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], addr_a<DK, false>(kp, m0 / 8, 2 * k) + p * kC * DK * 2);
+          step_add<NP, NP, 2>(kk, sk * sk, fa, fb);
         }
       }
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int i = frag_row(m0, e), j = frag_col(half * 32 + n * 8);
+          const int i = frag_row(m0, e), j = frag_col(col * 16 + n * 8);
 #pragma unroll
           for (int l = 0; l < 2; ++l) {
             const float dec = j + l <= i ? expf((gate[3 * kC + i] - gate[3 * kC + j + l]) +
@@ -468,7 +464,7 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = frag_row(m0, e);
-        const int word = ((m0 / 8 + e) * (DK / 8) + half * NT + n) * 32 + lane;
+        const int word = ((m0 / 8 + e) * (DK / 8) + col * NT + n) * 32 + lane;
         const float eg = gate[row], er = gate[kC + row], be = gate[2 * kC + row];
         const float2 kv = take2<NP>(kp, kC * DK, word), qv = take2<NP>(qp, kC * DK, word);
 #pragma unroll
@@ -491,9 +487,9 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
       }
       const int row = frag_row(m0, e);
       if ((lane & 3) == 0) {
-        red[half * kC + row] = xs[e];
-        red[(2 + half) * kC + row] = zs[e];
-        if (half == 0 && row < rows) a.dbeta[((long)b * a.T + t0 + row) * a.Hv + hv] = bdot[e];
+        red[col * kC + row] = xs[e];
+        red[(4 + col) * kC + row] = zs[e];
+        if (col == 0 && row < rows) a.dbeta[((long)b * a.T + t0 + row) * a.Hv + hv] = bdot[e];
       }
     }
     float end = gate[kC - 1] * sdot;
@@ -503,22 +499,22 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
     const unsigned wm = __reduce_max_sync(0xffffffffu, __float_as_uint(mw));
     if (lane == 0) {
       wred[warp] = end;
-      wred[8 + warp] = __uint_as_float(um);
-      wred[16 + warp] = __uint_as_float(wm);
+      wred[16 + warp] = __uint_as_float(um);
+      wred[32 + warp] = __uint_as_float(wm);
     }
     __syncthreads();
-    mu = wred[8], mw = wred[16];
+    mu = wred[16], mw = wred[32];
 #pragma unroll
-    for (int w = 1; w < kThreads / 32; ++w) {
-      mu = fmaxf(mu, wred[8 + w]);
-      mw = fmaxf(mw, wred[16 + w]);
+    for (int w = 1; w < kGradThreads / 32; ++w) {
+      mu = fmaxf(mu, wred[16 + w]);
+      mw = fmaxf(mw, wred[32 + w]);
     }
     const float iu = plane_inv(mu), iw = plane_inv(mw);
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int word = ((m0 / 8 + e) * (kC / 8) + half * 4 + n) * 32 + lane;
+        const int word = ((m0 / 8 + e) * (kC / 8) + col * 2 + n) * 32 + lane;
         uint32_t u[2], w[2];
         split2<2>(dp[n][2 * e], dp[n][2 * e + 1], iu, u);
         split2<2>(da[n][2 * e], da[n][2 * e + 1], iw, w);
@@ -528,29 +524,40 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
           reinterpret_cast<uint32_t*>(mp + p * kTile)[word] = w[p];
         }
       }
-    if (threadIdx.x < kC) {
-      // y_ij -> sum over the columns before j
-      float* row = y + threadIdx.x * (kC + 1);
-      float run = 0.0f;
-      for (int j = 0; j < kC; ++j) {
-        const float t = row[j];
-        row[j] = run;
-        run += t;
+    {
+      // y_ij -> sum over the columns before j, eight threads to a row
+      float* part = y + (threadIdx.x >> 3) * (kC + 1) + (threadIdx.x & 7) * 8;
+      float v[8], sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = part[j];
+        sum += v[j];
+      }
+      float run = 0.0f;  // of the parts before
+#pragma unroll
+      for (int k = 0; k < 7; ++k) {
+        const float f = __shfl_sync(0xffffffffu, sum, k, 8);
+        if ((threadIdx.x & 7) > k) run += f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        part[j] = run;
+        run += v[j];
       }
     }
     __syncthreads();
     const float su = plane_scale(iu), sw = plane_scale(iw);
-    token_product<NP, DK, false, NT>(dq, su * sk, dpp, m0 / 8, kp, half * NT, 0, m0 / 16 + 1);
-    token_product<NP, DK, false, NT>(dkr, sw * sk, mp, m0 / 8, kp, half * NT, 0, m0 / 16 + 1);
-    token_product<NP, DK, true, NT>(dkc, su * sq, dpp, m0 / 8, qp, half * NT, m0 / 16, kC / 16);
-    token_product<NP, DK, true, NT>(dkc, sw * sk, mp, m0 / 8, kp, half * NT, m0 / 16, kC / 16);
+    token_product<NP, DK, false, NT>(dq, su * sk, dpp, m0 / 8, kp, col * NT, 0, m0 / 16 + 1);
+    token_product<NP, DK, false, NT>(dkr, sw * sk, mp, m0 / 8, kp, col * NT, 0, m0 / 16 + 1);
+    token_product<NP, DK, true, NT>(dkc, su * sq, dpp, m0 / 8, qp, col * NT, m0 / 16, kC / 16);
+    token_product<NP, DK, true, NT>(dkc, sw * sk, mp, m0 / 8, kp, col * NT, m0 / 16, kC / 16);
     {
-      const int t = threadIdx.x >> 2;
+      const int t = threadIdx.x >> 3;
       float f = 0.0f;
-      for (int i = t + (threadIdx.x & 3); i < kC; i += 4) f += y[i * (kC + 1) + t];
-      f += __shfl_xor_sync(0xffffffffu, f, 1);
-      f += __shfl_xor_sync(0xffffffffu, f, 2);
-      if ((threadIdx.x & 3) == 0) red[4 * kC + t] = f;
+      for (int i = t + (threadIdx.x & 7); i < kC; i += 8) f += y[i * (kC + 1) + t];
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) f += __shfl_xor_sync(0xffffffffu, f, o);
+      if ((threadIdx.x & 7) == 0) red[8 * kC + t] = f;
     }
     __syncthreads();
     if (warp == 0) {
@@ -559,8 +566,8 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int i = 2 * lane + e;
-        x[e] = (double)red[i] + red[kC + i];
-        z[e] = (double)red[2 * kC + i] + red[3 * kC + i];
+        x[e] = ((double)red[i] + red[kC + i]) + ((double)red[2 * kC + i] + red[3 * kC + i]);
+        z[e] = ((double)red[4 * kC + i] + red[5 * kC + i]) + ((double)red[6 * kC + i] + red[7 * kC + i]);
       }
       double sx = x[0] + x[1], sz = z[0] + z[1];
 #pragma unroll
@@ -569,7 +576,7 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
         if (lane + o < 32) sx += u;
         if (lane >= o) sz += w;
       }
-      for (int w = 0; w < kThreads / 32; ++w) last += wred[w];
+      for (int w = 0; w < kGradThreads / 32; ++w) last += wred[w];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int i = 2 * lane + e;
@@ -578,7 +585,7 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
           const double from = e ? sx - x[0] : sx, before = e ? sz - z[1] : sz - z[0] - z[1];
           // a decay of zero passes no gradient
           a.dg[((long)b * a.T + t0 + i) * a.Hv + hv] =
-              gv < kNoDecay ? 0.0f : (float)(from + before + red[4 * kC + i] + last);
+              gv < kNoDecay ? 0.0f : (float)(from + before + red[8 * kC + i] + last);
         }
       }
     }
@@ -590,11 +597,11 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = frag_row(m0, e), col = frag_col((half * NT + n) * 8);
+        const int row = frag_row(m0, e), c = frag_col((col * NT + n) * 8);
         float2 x = make_float2(dq[n][2 * e], dq[n][2 * e + 1]);
         float2 z = make_float2(dkr[n][2 * e] + dkc[n][2 * e], dkr[n][2 * e + 1] + dkc[n][2 * e + 1]);
-        float2* px = reinterpret_cast<float2*>(accq + row * DK + col);
-        float2* pz = reinterpret_cast<float2*>(acck + row * DK + col);
+        float2* px = reinterpret_cast<float2*>(accq + row * DK + c);
+        float2* pz = reinterpret_cast<float2*>(acck + row * DK + c);
         if (r > 0) {
           x.x += px->x, x.y += px->y;
           z.x += pz->x, z.y += pz->y;
@@ -603,9 +610,9 @@ __global__ void __launch_bounds__(kThreads) delta_grads_kernel(const Problem a) 
           *px = x;
           *pz = z;
         } else if (row < rows) {
-          const long o = (((long)b * a.T + t0 + row) * a.Hk + hk) * a.dk + col;
-          set2<T>(static_cast<T*>(a.dq) + o, a.dk - col, even, x.x, x.y);
-          set2<T>(static_cast<T*>(a.dk_) + o, a.dk - col, even, z.x, z.y);
+          const long o = (((long)b * a.T + t0 + row) * a.Hk + hk) * a.dk + c;
+          set2<T>(static_cast<T*>(a.dq) + o, a.dk - c, even, x.x, x.y);
+          set2<T>(static_cast<T*>(a.dk_) + o, a.dk - c, even, z.x, z.y);
         }
       }
   }
@@ -637,7 +644,7 @@ int backward_typed(const Problem& a, cudaStream_t stream) {
   } else {
     if (const int rc = launch_scan<T, DK, 1>(a, stream)) return rc;
   }
-  delta_grads_kernel<T, DK><<<(unsigned)((long)a.B * a.Hk * a.nc), kThreads, G::bytes, stream>>>(a);
+  delta_grads_kernel<T, DK><<<(unsigned)((long)a.B * a.Hk * a.nc), kGradThreads, G::bytes, stream>>>(a);
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
 }

@@ -126,15 +126,19 @@ __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
                  : "r"(addr));
 }
 
+// d = A B + d, and d = A B.
+__device__ __forceinline__ void mma_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -162,19 +166,24 @@ __device__ __forceinline__ uint32_t addr_b(const f16* p, int k8, int n8) {
   return TRANS ? block_addr<COLS>(p, k8 + (i & 1), n8 + (i >> 1)) : block_addr<COLS>(p, n8 + (i >> 1), k8 + (i & 1));
 }
 
-// t[n] += A B_n over one step of 16 in k, smallest plane products first.  The
-// tensor core truncates when it adds into its accumulator, so callers give
-// every step fresh accumulators and add those up in FP32 (rounded to nearest).
+// t[n] = A B_n over one step of 16 in k, smallest plane products first.  The
+// tensor core truncates when it adds into its accumulator, so every step has
+// fresh ones and callers add those up in FP32 (rounded to nearest).
 template <int NA, int NB, int NT>
 __device__ __forceinline__ void mma_terms(float (&t)[NT][4], const uint32_t (&fa)[NA][4], const uint32_t (&fb)[NB][NT][2]) {
   constexpr int kTop = (NA > NB ? NA : NB) - 1;
+  bool first = true;
 #pragma unroll
   for (int s = kTop; s >= 0; --s)
 #pragma unroll
     for (int i = 0; i <= s; ++i)
       if (i < NA && s - i < NB) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma(t[n], fa[i], fb[s - i][n][0], fb[s - i][n][1]);
+        for (int n = 0; n < NT; ++n) {
+          if (first) mma_zero(t[n], fa[i], fb[s - i][n][0], fb[s - i][n][1]);
+          else mma(t[n], fa[i], fb[s - i][n][0], fb[s - i][n][1]);
+        }
+        first = false;
       }
 }
 
@@ -231,12 +240,46 @@ __device__ __forceinline__ void split2(float a, float b, float inv, uint32_t (&w
   }
 }
 
-// The larger magnitude of two numbers, NaN and infinities aside (they must not
-// take the other values' scale).
-__device__ __forceinline__ float max_finite(float m, float x) {
-  const float y = fabsf(x);
-  return fmaxf(m, y <= 3.4028235e38f ? y : 0.0f);
+// The larger of m and |x|; a NaN wins.
+__device__ __forceinline__ float max_mag(float m, float x) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(m), "f"(fabsf(x)));
+  return y;
 }
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e38f; }
+// The larger of m and |x| if that is finite: what is not must not take the
+// other values' scale.
+__device__ __forceinline__ float max_finite(float m, float x) { return fmaxf(m, finite(x) ? fabsf(x) : 0.0f); }
+// The largest of non-negative numbers over the warp; a NaN wins.
+__device__ __forceinline__ float warp_largest(float m) {
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+}
+// The largest finite magnitude of a warp's tile, and whether all are finite.
+template <int NT>
+__device__ __forceinline__ float warp_max(const float (&x)[NT][4], bool& all_finite) {
+  float m = 0.0f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = max_mag(m, x[n][e]);
+  m = warp_largest(m);
+  all_finite = finite(m);
+  if (!all_finite) {
+    m = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = max_finite(m, x[n][e]);
+    m = warp_largest(m);
+  }
+  return m;
+}
+template <int NT>
+__device__ __forceinline__ float warp_max(const float (&x)[NT][4]) {
+  bool all_finite;
+  return warp_max<NT>(x, all_finite);
+}
+
 // Writes an accumulator pair (row block r8, column tile n) of a tile of 16
 // columns, `plane` elements between planes.
 template <int NP>
@@ -356,17 +399,6 @@ struct Columns {
 template <typename T>
 __device__ __forceinline__ bool pairs_ok(const void* p, long s0, long s1, long s2, int cols) {
   return (reinterpret_cast<uintptr_t>(p) & (2 * sizeof(T) - 1)) == 0 && ((s0 | s1 | s2 | cols) & 1) == 0;
-}
-
-// The largest finite magnitude of a warp's tile.
-template <int NT>
-__device__ __forceinline__ float warp_max(const float (&x)[NT][4]) {
-  float m = 0.0f;
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m = max_finite(m, x[n][e]);
-  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
 }
 
 template <typename K>

@@ -40,15 +40,15 @@ struct PrepareSmem {
   static constexpr int planes = 2 * NP * kC * DK * 2;
   static constexpr int tiles = (2 * kC * kLd + kC * kLx) * 4;  // N, W and X, over the planes once those are used up
   static constexpr int main = planes > tiles ? planes : tiles;
-  static constexpr int bytes = main + kC * 8 + kGates * kC * 4 + kC * 4 + 64 * 4;
+  static constexpr int bytes = main + 2 * kGates * kC * 4 + kC * 4 + 64 * 4;
 };
 
-// acc[n] += A B_n of FP32 tiles in shared memory, A's columns times colscale[k]
-// (SCALED): operands as three bf16 planes, which need no scale.  k0, k1: a range
-// of k in multiples of 16; A at (m0, k), B at (k, n0).
-template <int NT, bool SCALED>
-__device__ __forceinline__ void mma_f32(float (&acc)[NT][4], const float* A, int lda, int m0, const float* B, int ldb,
-                                        int n0, int k0, int k1, const float* colscale) {
+// acc += A B of FP32 tiles in shared memory, 16 rows from m0 and 8 columns
+// from n0, A's columns times colscale[k] (SCALED): operands as three bf16
+// planes, which need no scale.  k0, k1: a range of k in multiples of 16.
+template <bool SCALED>
+__device__ __forceinline__ void mma_f32(float (&acc)[4], const float* A, int lda, int m0, const float* B, int ldb, int n0,
+                                        int k0, int k1, const float* colscale) {
   const int g = (threadIdx.x & 31) >> 2, c = (threadIdx.x & 3) * 2;
   auto planes = [](float x, float y, uint32_t (&w)[3]) {
 #pragma unroll
@@ -59,8 +59,9 @@ __device__ __forceinline__ void mma_f32(float (&acc)[NT][4], const float* A, int
       y -= __uint_as_float(w[p] & 0xffff0000u);
     }
   };
+#pragma unroll 2
   for (int k = k0; k < k1; k += 16) {
-    uint32_t fa[3][4];
+    uint32_t fa[3][4], fb[2][3];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int kk = k + c + 8 * (j >> 1);
@@ -72,56 +73,91 @@ __device__ __forceinline__ void mma_f32(float (&acc)[NT][4], const float* A, int
       for (int p = 0; p < 3; ++p) fa[p][j] = w[p];
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      uint32_t fb[2][3];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float* q = B + (k + c + 8 * j) * ldb + n0 + n * 8 + g;
-        planes(q[0], q[ldb], fb[j]);
-      }
-      float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int s = 2; s >= 0; --s)
-#pragma unroll
-        for (int i = 0; i <= s; ++i) mma_bf16(t, fa[i], fb[0][s - i], fb[1][s - i]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[n][e] += t[e];
+    for (int j = 0; j < 2; ++j) {
+      const float* q = B + (k + c + 8 * j) * ldb + n0 + g;
+      planes(q[0], q[ldb], fb[j]);
     }
+    // two chains: the larger products apart from the smaller
+    float t[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    mma_bf16(t, fa[0], fb[0][2], fb[1][2]);
+    mma_bf16(u, fa[0], fb[0][1], fb[1][1]);
+    mma_bf16(t, fa[1], fb[0][1], fb[1][1]);
+    mma_bf16(u, fa[1], fb[0][0], fb[1][0]);
+    mma_bf16(t, fa[2], fb[0][0], fb[1][0]);
+    mma_bf16(u, fa[0], fb[0][0], fb[1][0]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += t[e] + u[e];
   }
 }
 
-// One doubling of W's diagonal blocks, for 16 rows of it from m0 on by one
-// warp: with the blocks W0 (rows o.. ) and W1 (rows s..) done, the block below
-// W0 is X - W1 (B1 X), X = N10 - (N10 B0) W0.  First half: X into `x` and B1 X
-// into shared memory; second half: the block into W.
-template <int NT>
-__device__ __forceinline__ void join_first(float (&x)[NT][4], const float* N, const float* W, float* X, int m0, int o,
-                                           int s, const float* beta) {
-  float t[NT][4];
-  zero(t);
-  mma_f32<NT, true>(t, N, kLd, m0, W, kLd, o, o, s, beta);
+// One doubling of W's diagonal blocks: with the blocks W0 (rows and columns o
+// to s) and W1 (from s on) done, the block of W1's rows and W0's columns is X - W1
+// (B1 X), X = N10 - (N10 B0) W0.  A warp does 16 rows (from m0) x 8 columns (from
+// o + n0) of it: first X, into `x`, and B1 X into shared memory, then the block.
+__device__ __forceinline__ void join_first(float (&x)[4], const float* N, const float* W, float* X, int m0, int o, int s,
+                                           int n0, const float* beta) {
+  float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  mma_f32<true>(t, N, kLd, m0, W, kLd, o + n0, o, s, beta);
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = frag_row(m0, e), c = frag_col(n * 8);
-      const float2 f = *reinterpret_cast<const float2*>(N + r * kLd + o + c);
-      x[n][2 * e] = f.x - t[n][2 * e];
-      x[n][2 * e + 1] = f.y - t[n][2 * e + 1];
-      *reinterpret_cast<float2*>(X + r * kLx + c) = make_float2(beta[r] * x[n][2 * e], beta[r] * x[n][2 * e + 1]);
-    }
+  for (int e = 0; e < 2; ++e) {
+    const int r = frag_row(m0, e), c = frag_col(n0);
+    const float2 f = *reinterpret_cast<const float2*>(N + r * kLd + o + c);
+    x[2 * e] = f.x - t[2 * e];
+    x[2 * e + 1] = f.y - t[2 * e + 1];
+    *reinterpret_cast<float2*>(X + r * kLx + c) = make_float2(beta[r] * x[2 * e], beta[r] * x[2 * e + 1]);
+  }
 }
-template <int NT>
-__device__ __forceinline__ void join_second(const float (&x)[NT][4], float* W, const float* X, int m0, int o, int s) {
-  float t[NT][4];
-  zero(t);
-  mma_f32<NT, false>(t, W, kLd, m0, X, kLx, 0, s, m0 + 16, nullptr);
+__device__ __forceinline__ void join_second(const float (&x)[4], float* W, const float* X, int m0, int o, int s, int n0) {
+  float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  mma_f32<false>(t, W, kLd, m0, X, kLx, n0, s, m0 + 16, nullptr);
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int e = 0; e < 2; ++e)
+    *reinterpret_cast<float2*>(W + frag_row(m0, e) * kLd + o + frag_col(n0)) =
+        make_float2(x[2 * e] - t[2 * e], x[2 * e + 1] - t[2 * e + 1]);
+}
+
+// The gates of one value head's chunk, by one warp.  `bad`: tokens whose key is
+// not finite.
+__device__ __forceinline__ void chunk_gates(const Problem& a, int b, int hv, int t0, int rows, const int* bad, float* gates) {
+  const int lane = threadIdx.x & 31;
+  // sums of log decays in FP64: differences of neighbours stay exact to FP32
+  // where the sums are large
+  double x[2];
+  float be[2];
+  unsigned lost[2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-      *reinterpret_cast<float2*>(W + frag_row(m0, e) * kLd + o + frag_col(n * 8)) =
-          make_float2(x[n][2 * e] - t[n][2 * e], x[n][2 * e + 1] - t[n][2 * e + 1]);
+  for (int e = 0; e < 2; ++e) {
+    const int i = 2 * lane + e, t = t0 + min(i, rows - 1);
+    float gv = a.g[b * a.sg[0] + t * a.sg[1] + hv * a.sg[2]];
+    be[e] = a.beta[b * a.sb[0] + t * a.sb[1] + hv * a.sb[2]];
+    if (i >= rows) gv = be[e] = 0.0f;
+    const bool off = bad[i] != 0 || !(gv <= 3.4028235e38f) || !finite(be[e]);
+    lost[e] = __ballot_sync(0xffffffffu, off);
+    if (!(gv <= 3.4028235e38f)) gv = 0.0f;
+    if (!finite(be[e])) be[e] = 0.0f;
+    if (gv < kNoDecay) gv = kNoDecay;
+    x[e] = gv;
+  }
+  // The first token with a key, decay or strength that is not finite: it and
+  // those after it get NaN through e^G, those before it nothing.
+  const int first = min(lost[0] ? 2 * (__ffs(lost[0]) - 1) : kC, lost[1] ? 2 * (__ffs(lost[1]) - 1) + 1 : kC);
+  double s = x[0] + x[1];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += y;
+  }
+  const double end = __shfl_sync(0xffffffffu, s, 31);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int i = 2 * lane + e;
+    const double gi = e ? s : s - x[1];
+    gates[i] = i < first ? expf((float)gi) : __uint_as_float(0x7fffffffu);
+    gates[kC + i] = expf((float)(end - gi));
+    gates[2 * kC + i] = be[e];
+    gates[3 * kC + i] = (float)gi;
+    gates[4 * kC + i] = (float)(gi - (double)(float)gi);
+  }
 }
 
 // The largest of a value over the CTA (after a barrier).
@@ -137,7 +173,7 @@ __device__ __forceinline__ float get_max(const float* red) {
 }
 
 template <typename T, int DK>
-__global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const Problem a, const bool fold_beta) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_prepare_kernel(const Problem a, const bool fold_beta) {
   constexpr int NP = Planes<T>::n;
   constexpr int NQ = kC * DK / 4 / kThreads;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -147,9 +183,8 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const Problem a
   float* N = reinterpret_cast<float*>(smem);  // over the planes
   float* W = N + kC * kLd;
   float* X = W + kC * kLd;
-  double* G = reinterpret_cast<double*>(smem + L::main);
-  float* gates = reinterpret_cast<float*>(G + kC);
-  int* bad = reinterpret_cast<int*>(gates + kGates * kC);  // tokens whose key is not finite
+  float* gates2 = reinterpret_cast<float*>(smem + L::main);   // of this value head and of the next
+  int* bad = reinterpret_cast<int*>(gates2 + 2 * kGates * kC);  // tokens whose key is not finite
   float* red = reinterpret_cast<float*>(bad + kC);         // [4][8] and scales
 
   const int chunk = blockIdx.x % a.nc, bh = blockIdx.x / a.nc;
@@ -207,7 +242,7 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const Problem a
         float* f = &kx[x].x;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (!(fabsf(f[i]) <= 3.4028235e38f)) f[i] = 0.0f, lost = true;
+          if (!finite(f[i])) f[i] = 0.0f, lost = true;
         if (lost) bad[r] = 1;
       }
     }
@@ -261,8 +296,6 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const Problem a
       }
       load_b<NP, 4, false>(fb, pb + kk * 256, 32 * DK, kC * DK * 2);
       float t[4][4], u[4][4];
-      zero(t);
-      zero(u);
       mma_terms<NP, NP, 4>(t, fk, fb);
       mma_terms<NP, NP, 4>(u, fq, fb);
 #pragma unroll
@@ -284,51 +317,12 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const Problem a
     }
   __syncthreads();
   for (int x = threadIdx.x; x < kC * kLd; x += kThreads) W[x] = 0.0f;  // above its diagonal blocks it stays zero
+  if (warp == 7) chunk_gates(a, b, h * a.rep, t0, rows, bad, gates2);
 
   for (int r = 0; r < a.rep; ++r) {
     const int hv = h * a.rep + r;
     const long nv = ((long)b * a.Hv + hv) * a.nc + chunk;
-    if (warp == 0) {
-      // sums of log decays in FP64: differences of neighbours stay exact to
-      // FP32 where the sums are large
-      double x[2];
-      float be[2];
-      unsigned lost[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = 2 * lane + e;
-        float gv = i < rows ? a.g[b * a.sg[0] + (t0 + i) * a.sg[1] + hv * a.sg[2]] : 0.0f;
-        be[e] = i < rows ? a.beta[b * a.sb[0] + (t0 + i) * a.sb[1] + hv * a.sb[2]] : 0.0f;
-        const bool off = bad[i] != 0 || !(gv <= 3.4028235e38f) || !(fabsf(be[e]) <= 3.4028235e38f);
-        lost[e] = __ballot_sync(0xffffffffu, off);
-        if (!(gv <= 3.4028235e38f)) gv = 0.0f;
-        if (!(fabsf(be[e]) <= 3.4028235e38f)) be[e] = 0.0f;
-        if (gv < kNoDecay) gv = kNoDecay;
-        x[e] = gv;
-      }
-      // The first token with a key, decay or strength that is not finite: it
-      // and those after it get NaN through e^G, those before it nothing.
-      const int first = min(lost[0] ? 2 * (__ffs(lost[0]) - 1) : kC, lost[1] ? 2 * (__ffs(lost[1]) - 1) + 1 : kC);
-      double s = x[0] + x[1];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += y;
-      }
-      const double end = __shfl_sync(0xffffffffu, s, 31);
-      const float nan = __uint_as_float(0x7fffffffu);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = 2 * lane + e;
-        const double gi = e ? s : s - x[1];
-        G[i] = gi;
-        gates[i] = i < first ? expf((float)gi) : nan;
-        gates[kC + i] = expf((float)(end - gi));
-        gates[2 * kC + i] = be[e];
-        gates[3 * kC + i] = (float)gi;
-        gates[4 * kC + i] = (float)(gi - (double)(float)gi);
-      }
-    }
+    const float* gates = gates2 + (r & 1) * kGates * kC;
     __syncthreads();
     float mp = 0.0f;
     float pv[4][4];
@@ -340,7 +334,9 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const Problem a
         float nn[2];
 #pragma unroll
         for (int l = 0; l < 2; ++l) {
-          const float d = j + l <= i ? expf((float)(G[i] - G[j + l])) : 0.0f;
+          const float d = j + l <= i ? expf((gates[3 * kC + i] - gates[3 * kC + j + l]) +
+                                            (gates[4 * kC + i] - gates[4 * kC + j + l]))
+                                     : 0.0f;
           nn[l] = j + l < i ? ak[n][2 * e + l] * d : 0.0f;
           const float p = j + l <= i ? aq[n][2 * e + l] * d * a.scale : 0.0f;
           pv[n][2 * e + l] = fold_beta ? p * gates[2 * kC + j + l] : p;
@@ -379,24 +375,22 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const Problem a
     }
     __syncthreads();
     const float* beta = gates + 2 * kC;
-    {
-      float x[2][4];
-      if (warp == 2) join_first<2>(x, N, W, X, 16, 0, 16, beta);
-      if (warp == 6) join_first<2>(x, N, W, X, 48, 32, 48, beta);
-      __syncthreads();
-      if (warp == 2) join_second<2>(x, W, X, 16, 0, 16);
-      if (warp == 6) join_second<2>(x, W, X, 48, 32, 48);
-      __syncthreads();
-    }
-    {
-      float x[4][4];
-      if (warp == 4) join_first<4>(x, N, W, X, 32, 0, 32, beta);
-      if (warp == 6) join_first<4>(x, N, W, X, 48, 0, 32, beta);
-      __syncthreads();
-      if (warp == 4) join_second<4>(x, W, X, 32, 0, 32);
-      if (warp == 6) join_second<4>(x, W, X, 48, 0, 32);
-      __syncthreads();
-    }
+    float jx[4];
+    // 16 -> 32: two blocks, two column tiles each; the last warp makes the
+    // next value head's gates meanwhile
+    const int o1 = (warp >> 1) * 32, n1 = (warp & 1) * 8;
+    if (warp < 4) join_first(jx, N, W, X, o1 + 16, o1, o1 + 16, n1, beta);
+    if (warp == 7 && r + 1 < a.rep)
+      chunk_gates(a, b, hv + 1, t0, rows, bad, gates2 + ((r + 1) & 1) * kGates * kC);
+    __syncthreads();
+    if (warp < 4) join_second(jx, W, X, o1 + 16, o1, o1 + 16, n1);
+    __syncthreads();
+    // 32 -> 64: two row tiles, four column tiles
+    const int m2 = 32 + (warp >> 2) * 16, n2 = (warp & 3) * 8;
+    join_first(jx, N, W, X, m2, 0, 32, n2, beta);
+    __syncthreads();
+    join_second(jx, W, X, m2, 0, 32, n2);
+    __syncthreads();
     // W's planes: a thread takes two rows of eight elements of the tile's blocks
     float4 wx[2][2];
     float mw = 0.0f;
@@ -547,19 +541,24 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
           y[n][2 * e + 1] = be * x[n][2 * e + 1];
         }
       if (chunk + 1 < a.nc) load_v(chunk + 1);
-      const float inv = plane_inv(warp_max(y));
+      bool all_finite;
+      const float inv = plane_inv(warp_max(y, all_finite));
       if (lane == 0) xsc[quarter] = plane_scale(inv);
+      if (!all_finite) {
+        // What is not finite is left out, since a zero of W times it would
+        // reach earlier tokens, and put back below.
+        off = true;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[n][e] = finite(y[n][e]) && finite(x[n][e]) ? y[n][e] : 0.0f;
+      }
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          // What is not finite is left out, since a zero of W times it would
-          // reach earlier tokens, and put back below.
-          const bool bad0 = !(fabsf(x[n][2 * e]) <= 3.4028235e38f) || !(fabsf(y[n][2 * e]) <= 3.4028235e38f);
-          const bool bad1 = !(fabsf(x[n][2 * e + 1]) <= 3.4028235e38f) || !(fabsf(y[n][2 * e + 1]) <= 3.4028235e38f);
-          off |= bad0 || bad1;
           uint32_t w[2];
-          split2<2>(bad0 ? 0.0f : y[n][2 * e], bad1 ? 0.0f : y[n][2 * e + 1], inv, w);
+          split2<2>(y[n][2 * e], y[n][2 * e + 1], inv, w);
           store_pair<2>(xp, 2 * kGroup * kC, quarter * 2 + e, n, w);
         }
     }
@@ -569,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (!(fabsf(x[n][e]) <= 3.4028235e38f)) atomicMin(first + pair * kGroup + frag_col(n * 8) + (e & 1), row[e >> 1]);
+          if (!finite(x[n][e])) atomicMin(first + pair * kGroup + frag_col(n * 8) + (e & 1), row[e >> 1]);
       __syncthreads();
     }
     // E
@@ -583,17 +582,10 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
           if (row[e >> 1] > first[pair * kGroup + frag_col(n * 8) + (e & 1)]) x[n][e] = __uint_as_float(0x7fffffffu);
     }
     {
-      const float inv = plane_inv(warp_max(x));
+      bool all_finite;
+      const float inv = plane_inv(warp_max(x, all_finite));
       // a scale below zero marks a quarter that holds something not finite
-      bool lost = false;
-      if (off) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) lost |= !(fabsf(x[n][e]) <= 3.4028235e38f);
-        lost = __any_sync(0xffffffffu, lost);
-      }
-      if (lane == 0) a.escale[(nv * groups + group) * 4 + quarter] = lost ? -plane_scale(inv) : plane_scale(inv);
+      if (lane == 0) a.escale[(nv * groups + group) * 4 + quarter] = all_finite ? plane_scale(inv) : -plane_scale(inv);
       f16* out = a.e + (nv * 2 * groups + group) * kGroup * kC;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -646,79 +638,88 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
 }
 
 // ---------------------------------------------------------------------------
-// output: one CTA per (batch, value head, chunk); a warp takes 16 tokens x 16
-// of a slice's 32 value columns, the next slice loads meanwhile.  bf16 outputs
-// take the first plane only (2^-12 of the operands' size, against 2^-9 from
-// rounding the output), which halves the reading: it is bound by memory.
+// output: one CTA per (batch, value head, chunk), 64 value columns at a time; a
+// warp takes 16 tokens x 32 columns.  bf16 outputs take the first plane only
+// (2^-12 of the operands' size, against 2^-9 from rounding the output), which
+// halves the reading: it is bound by memory.
 // ---------------------------------------------------------------------------
 
 template <typename T, int DK>
 struct OutputSmem {
   static constexpr int NP = Planes<T>::n;  // planes used, of every operand
-  static constexpr int q = NP * kC * DK, p = NP * kTile;
-  static constexpr int s = NP * kSlice * DK, e = NP * kSlice * kC;
-  static constexpr int bytes = (q + p + 2 * (s + e)) * 2 + kGates * kC * 4;
+  static constexpr int cols = 64;
+  static constexpr int q = NP * kC * DK, p = NP * kTile;  // elements
+  static constexpr int s = NP * cols * DK, e = NP * cols * kC;
+  static constexpr int slice = s + e + 2 * 32;  // and the scales of S and E, four groups and quarters
+  static constexpr int buffers = (q + p + 2 * slice) * 2 > 96 * 1024 ? 1 : 2;
+  static constexpr int bytes = (q + p + buffers * slice) * 2 + kGates * kC * 4;
 };
 
 template <typename T, int DK>
 __device__ __forceinline__ void output_load(f16* dst, const Problem& a, long nv, int c0) {
   using L = OutputSmem<T, DK>;
+  const int cols = min(L::cols, a.dvp - c0);
 #pragma unroll
   for (int p = 0; p < L::NP; ++p) {
-    copy_async(dst + p * kSlice * DK, a.states + (nv * 2 + p) * a.dvp * DK + (long)c0 * DK, kSlice * DK * 2);
-    copy_async(dst + L::s + p * kSlice * kC, a.e + (nv * 2 + p) * a.dvp * kC + (long)c0 * kC, kSlice * kC * 2);
+    copy_async(dst + p * L::cols * DK, a.states + (nv * 2 + p) * a.dvp * DK + (long)c0 * DK, cols * DK * 2);
+    copy_async(dst + L::s + p * L::cols * kC, a.e + (nv * 2 + p) * a.dvp * kC + (long)c0 * kC, cols * kC * 2);
   }
+  const long g = (nv * (a.dvp / kGroup) + c0 / kGroup) * 4;
+  copy_async(dst + L::s + L::e, a.sscale + g, cols);
+  copy_async(dst + L::s + L::e + 32, a.escale + g, cols);
   cp_async_commit();
 }
 
-// acc += A B over `steps` of 16, of which the first nk count; two at a time
-// for four independent chains of products.  scale: one for `per` steps.
+// acc (two groups of 16 columns) += A B over nk <= STEPS steps of 16.  Both
+// groups' scales of a quarter (PER steps) are scale[4 g + quarter]; `group`: bytes
+// from one group's B to the next.
 template <int NP, int STEPS, int PER>
-__device__ __forceinline__ void output_product(float (&acc)[2][4], uint32_t pa, int plane_a, uint32_t pb, int plane_b,
-                                               int nk, const float (&scale)[4]) {
+__device__ __forceinline__ void output_product(float (&acc)[4][4], uint32_t pa, int plane_a, uint32_t pb, int plane_b,
+                                               int group, int nk, const float* scale) {
 #pragma unroll
-  for (int kk = 0; kk < STEPS; kk += 2) {
-    if (kk >= nk) break;
-    float t[2][2][4];
-    zero(t[0]);
-    zero(t[1]);
+  for (int k0 = 0; k0 < STEPS; k0 += PER) {
+    if (k0 >= nk) break;
+    float t[4][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (kk + h >= nk) break;
-      uint32_t fa[NP][4], fb[NP][2][2];
+    for (int h = 0; h < PER; ++h) {
+      const int kk = k0 + h;
+      uint32_t fa[NP][4], fb[NP][4][2];
 #pragma unroll
-      for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], pa + (kk + h) * 256 + p * plane_a);
-      load_b<NP, 2, true>(fb, pb + (kk + h) * 512, 0, plane_b);
-      mma_terms<NP, NP, 2>(t[h], fa, fb);
+      for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], pa + kk * 256 + p * plane_a);
+      load_b<NP, 4, true>(fb, pb + kk * 512, group, plane_b);
+      if (NP == 1 && h > 0) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) mma(t[n], fa[0], fb[0][n][0], fb[0][n][1]);
+      } else {
+        mma_terms<NP, NP, 4>(t, fa, fb);
+      }
+      if (NP == 1 && h + 1 < PER) continue;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const float f = scale[(n >> 1) * 4 + k0 / PER];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][e] += f * t[n][e];
+      }
     }
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[n][e] += scale[kk / PER] * t[0][n][e] + scale[(kk + 1) / PER] * t[1][n][e];
   }
 }
 
-// y = P E where an error is not finite: element by element, because the zeros
+// An element of P E, for a chunk with an error that is not finite: the zeros
 // of P above its diagonal would spread it to earlier tokens.
 template <int NP>
-__device__ __noinline__ void output_by_element(float (&y)[2][4], const f16* pp, int m0, const f16* ep, float4 scale) {
-  const float s[4] = {fabsf(scale.x), fabsf(scale.y), fabsf(scale.z), fabsf(scale.w)};
-  for (int x = 0; x < 8; ++x) {
-    const int n = x >> 2, e = x & 3;
-    const int i = frag_row(m0, e >> 1), c = frag_col(n * 8) + (e & 1);
-    float sum = 0.0f;
-    for (int j = 0; j <= i; ++j) {
-      const int ip = ((i >> 3) * 8 + (j >> 3)) * 64 + (i & 7) * 8 + (j & 7);
-      const int ie = ((j >> 3) * 2 + (c >> 3)) * 64 + (j & 7) * 8 + (c & 7);
-      float u = 0.0f, w = 0.0f;
-      for (int p = 0; p < NP; ++p) {
-        u += __half2float(pp[p * kTile + ip]);
-        w += __half2float(ep[p * kSlice * kC + ie]);
-      }
-      sum += s[j >> 4] * (u * w);
+__device__ __noinline__ float output_element(const f16* pp, const f16* ep, int plane, const float* scale, int i, int c) {
+  float sum = 0.0f;
+  for (int j = 0; j <= i; ++j) {
+    const int ip = ((i >> 3) * 8 + (j >> 3)) * 64 + (i & 7) * 8 + (j & 7);
+    const int ie = ((j >> 3) * 2 + (c >> 3)) * 64 + (j & 7) * 8 + (c & 7);
+    float u = 0.0f, w = 0.0f;
+    for (int p = 0; p < NP; ++p) {
+      u += __half2float(pp[p * kTile + ip]);
+      w += __half2float(ep[p * plane + ie]);
     }
-    y[n][e] = sum;
+    sum += fabsf(scale[j >> 4]) * (u * w);
   }
+  return sum;
 }
 
 template <typename T, int DK>
@@ -729,7 +730,7 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a)
   f16* qp = reinterpret_cast<f16*>(smem);
   f16* pp = qp + L::q;
   f16* slices = pp + L::p;
-  float* gate = reinterpret_cast<float*>(slices + 2 * (L::s + L::e));
+  float* gate = reinterpret_cast<float*>(slices + L::buffers * L::slice);
 
   const int chunk = blockIdx.x % a.nc, bh = blockIdx.x / a.nc;
   const int hv = bh % a.Hv, b = bh / a.Hv;
@@ -740,42 +741,61 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a)
   output_load<T, DK>(slices, a, nv, 0);
   const int warp = threadIdx.x >> 5;
   const int m0 = (warp >> 1) * 16, half = warp & 1;
-  T* o = static_cast<T*>(a.o);
+  T* o = static_cast<T*>(a.o) + (((long)b * a.T + (long)chunk * kC) * a.Hv + hv) * a.dv;
+  const int rows = a.T - chunk * kC;
   const bool vec = a.dv % 2 == 0 && (reinterpret_cast<uintptr_t>(o) & (2 * sizeof(T) - 1)) == 0;
-  for (int c0 = 0, buf = 0; c0 < a.dvp; c0 += kSlice, buf ^= 1) {
+  for (int c0 = 0, buf = 0; c0 < a.dvp; c0 += L::cols) {
     cp_async_wait<0>();
     __syncthreads();
-    if (c0 + kSlice < a.dvp) output_load<T, DK>(slices + (buf ^ 1) * (L::s + L::e), a, nv, c0 + kSlice);
-    const f16* sp = slices + buf * (L::s + L::e);
+    const f16* sp = slices + buf * L::slice;
     const f16* ep = sp + L::s;
-    const long g = nv * (a.dvp / kGroup) + c0 / kGroup + half;
-    const float4 fs = *reinterpret_cast<const float4*>(a.sscale + g * 4);
-    const float4 fe = *reinterpret_cast<const float4*>(a.escale + g * 4);
-    float x[2][4], y[2][4];
-    zero(x);
-    zero(y);
-    output_product<NP, DK / 16, DK / 64>(x, addr_a<DK, false>(qp, m0 / 8, 0), kC * DK * 2,
-                                         addr_b<kGroup, true>(sp + half * kGroup * DK, 0, 0), kSlice * DK * 2, DK / 16,
-                                         {fs.x, fs.y, fs.z, fs.w});
-    if (fminf(fminf(fe.x, fe.y), fminf(fe.z, fe.w)) < 0.0f) {
-      output_by_element<NP>(y, pp, m0, ep + half * kGroup * kC, fe);
-    } else {
-      output_product<NP, 4, 1>(y, addr_a<kC, false>(pp, m0 / 8, 0), kTile * 2,
-                             addr_b<kGroup, true>(ep + half * kGroup * kC, 0, 0), kSlice * kC * 2, m0 / 16 + 1,
-                               {fe.x, fe.y, fe.z, fe.w});
+    if (L::buffers == 2 && c0 + L::cols < a.dvp) {
+      buf ^= 1;
+      output_load<T, DK>(slices + buf * L::slice, a, nv, c0 + L::cols);
     }
-    const float fx = a.scale * gate[5 * kC + 3], fy = gate[5 * kC + 1];
+    const int cw = c0 + half * 32;  // this warp's columns; those it has are whole slices
+    if (cw < a.dvp) {
+      const float* fs = reinterpret_cast<const float*>(ep + L::e) + half * 8;
+      const float* fe = fs + 16;
+      const f16* sg = sp + half * 2 * kGroup * DK;
+      const f16* eg = ep + half * 2 * kGroup * kC;
+      float x[4][4], y[4][4];
+      zero(x);
+      zero(y);
+      output_product<NP, DK / 16, DK / 64>(x, addr_a<DK, false>(qp, m0 / 8, 0), kC * DK * 2,
+                                           addr_b<kGroup, true>(sg, 0, 0), L::cols * DK * 2, kGroup * DK * 2, DK / 16, fs);
+      bool lost = false;
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+      for (int i = 0; i < 8; ++i) lost |= fe[i] < 0.0f;
+      if (lost) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            y[n][e] = output_element<NP>(pp, eg + (n >> 1) * kGroup * kC, L::cols * kC, fe + (n >> 1) * 4,
+                                         frag_row(m0, e >> 1), frag_col((n & 1) * 8) + (e & 1));
+      } else {
+        output_product<NP, 4, 1>(y, addr_a<kC, false>(pp, m0 / 8, 0), kTile * 2, addr_b<kGroup, true>(eg, 0, 0),
+                                 L::cols * kC * 2, kGroup * kC * 2, m0 / 16 + 1, fe);
+      }
+      const float fx = a.scale * gate[5 * kC + 3], fy = gate[5 * kC + 1];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = frag_row(m0, e), c = c0 + frag_col(half * 16 + n * 8), t = chunk * kC + row;
-        if (t < a.T) {
+        const int row = frag_row(m0, e);
+        if (row < rows) {
           const float f = gate[row] * fx;
-          set2<T>(o + (((long)b * a.T + t) * a.Hv + hv) * a.dv + c, a.dv - c, vec, f * x[n][2 * e] + fy * y[n][2 * e],
-                  f * x[n][2 * e + 1] + fy * y[n][2 * e + 1]);
+          T* p = o + (long)row * a.Hv * a.dv + cw + frag_col(0);
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            set2<T>(p + n * 8, a.dv - cw - frag_col(n * 8), vec, f * x[n][2 * e] + fy * y[n][2 * e],
+                    f * x[n][2 * e + 1] + fy * y[n][2 * e + 1]);
         }
       }
+    }
+    if (L::buffers == 1 && c0 + L::cols < a.dvp) {
+      __syncthreads();
+      output_load<T, DK>(slices, a, nv, c0 + L::cols);
+    }
   }
 }
 

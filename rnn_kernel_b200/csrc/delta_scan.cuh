@@ -23,7 +23,6 @@ __device__ __forceinline__ void times_state(float (&x)[2][4], const f16* kp, int
 #pragma unroll
       for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], pa + (kk + h) * 256 + p * kC * DK * 2);
       load_b<2, 2, true>(fb, pb + (kk + h) * 512, 0, 2 * kGroup * DK * 2);
-      zero(t[h]);
       mma_terms<NP, 2, 2>(t[h], fa, fb);
     }
     const float f0 = scale[kk / per], f1 = scale[(kk + 1) / per];
@@ -49,7 +48,6 @@ __device__ __forceinline__ void times_tokens(float (&x)[2][4], const f16* A, int
     for (int p = 0; p < NA; ++p) ldm4<TA>(fa[p], pa + p * kTile * 2);
     load_b<NB, 2, true>(fb, addr_b<kGroup, true>(B, 2 * kk, 0), 0, plane);
     float t[2][4];
-    zero(t);
     mma_terms<NA, NB, 2>(t, fa, fb);
     const float f = factor * scale[kk];
 #pragma unroll
@@ -77,7 +75,6 @@ __device__ __forceinline__ void add_to_state(float (&s)[DK / 64][2][4], const f1
       const uint32_t pa = addr_a<DK, true>(kp, (quarter * MT + m) * 2, 2 * kk);
 #pragma unroll
       for (int p = 0; p < NP; ++p) ldm4<true>(fa[p], pa + p * kC * DK * 2);
-      zero(t[m]);
       mma_terms<NP, 2, 2>(t[m], fa, fb);
     }
 #pragma unroll
@@ -100,8 +97,19 @@ __device__ __forceinline__ void put_state(const float (&s)[DK / 64][2][4], int q
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) m = max_finite(m, s[i][n][e]);
-  const float inv = plane_inv(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))));
+      for (int e = 0; e < 4; ++e) m = max_mag(m, s[i][n][e]);
+  m = warp_largest(m);
+  if (!finite(m)) {
+    m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = max_finite(m, s[i][n][e]);
+    m = warp_largest(m);
+  }
+  const float inv = plane_inv(m);
   if ((threadIdx.x & 31) == 0) {
     scale[quarter] = plane_scale(inv);
     if (out) out_scale[quarter] = plane_scale(inv);
