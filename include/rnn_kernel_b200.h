@@ -177,8 +177,9 @@ typedef struct {
 } gru_delta_args; /* host struct */
 
 /* Bytes that gru_delta_forward leaves for gru_delta_backward (the forward
- * needs them too when no backward follows), and each one's workspace; 0 and an
- * error text for arguments that they refuse. */
+ * needs them too when no backward follows), and each one's workspace, from
+ * the sizes alone (the tensors may be NULL); 0 and an error text for sizes that
+ * they refuse. */
 size_t gru_delta_stash_bytes(const gru_delta_args* args);
 size_t gru_delta_workspace_bytes(const gru_delta_args* args, int backward);
 

@@ -6,6 +6,7 @@ if the library is missing the call raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import struct
 import threading
@@ -142,22 +143,25 @@ def timeline_read():
     return buf
 
 
-class on_device:
-    """``torch.cuda.device`` that costs nothing where the device is current already."""
+def on_device(index: int):
+    """``torch.cuda.device(index)``, or a context that does nothing where that device is current."""
+    return _NOTHING if torch.cuda.current_device() == index else torch.cuda.device(index)
 
-    __slots__ = ("index", "guard")
 
-    def __init__(self, index: int) -> None:
-        self.index, self.guard = index, None
+_NOTHING = contextlib.nullcontext()
 
-    def __enter__(self) -> None:
-        if torch.cuda.current_device() != self.index:
-            self.guard = torch.cuda.device(self.index)
-            self.guard.__enter__()
 
-    def __exit__(self, *exc) -> None:
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def raw_stream(index: int) -> int:
+    """The ``cudaStream_t`` of the current stream of a device."""
+    return _raw_stream(index)
+
+
+try:
+    # torch's own short way, without a Stream object (1 us less a call)
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:  # a torch built without CUDA
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
 
 
 def library_path() -> Path:

@@ -129,7 +129,8 @@ int bad(const char* what, const char* msg, int code = GRU_ERR_INVALID) {
   return code;
 }
 
-int check_args(const char* what, const gru_delta_args* p) {
+// sizes_only: the tensors are not looked at.
+int check_args(const char* what, const gru_delta_args* p, bool sizes_only = false) {
   if (!p) return bad(what, "null arguments");
   if (p->dtype != GRU_F32 && p->dtype != GRU_BF16)
     return bad(what, "dtype must be GRU_F32 or GRU_BF16", GRU_ERR_UNSUPPORTED);
@@ -144,7 +145,7 @@ int check_args(const char* what, const gru_delta_args* p) {
         reinterpret_cast<uintptr_t>(p->initial_state)) & 3) != 0)
     return bad(what, "a tensor is not aligned to its element size");
   const bool any = p->B > 0 && p->T > 0;
-  if (any && (!p->q || !p->k || !p->v || !p->g || !p->beta)) return bad(what, "null tensor");
+  if (!sizes_only && any && (!p->q || !p->k || !p->v || !p->g || !p->beta)) return bad(what, "null tensor");
   const long nc = ((long)p->T + kC - 1) / kC;
   if ((long)p->B * p->Hv > (1L << 28) || (long)p->B * p->Hv * (nc > 4 ? nc : 4) > 0x7fffffffL)
     return bad(what, "too many chunks for one launch", GRU_ERR_UNSUPPORTED);
@@ -213,7 +214,7 @@ using namespace gru;
 using namespace gru::delta;
 
 extern "C" size_t gru_delta_stash_bytes(const gru_delta_args* p) {
-  if (check_args("gru_delta_stash_bytes", p)) return 0;
+  if (check_args("gru_delta_stash_bytes", p, true)) return 0;
   Problem a{};
   fill(a, *p);
   Arena m{nullptr};
@@ -222,7 +223,7 @@ extern "C" size_t gru_delta_stash_bytes(const gru_delta_args* p) {
 }
 
 extern "C" size_t gru_delta_workspace_bytes(const gru_delta_args* p, int backward) {
-  if (check_args("gru_delta_workspace_bytes", p)) return 0;
+  if (check_args("gru_delta_workspace_bytes", p, true)) return 0;
   Problem a{};
   fill(a, *p);
   Arena m{nullptr};

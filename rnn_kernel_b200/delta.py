@@ -18,6 +18,7 @@ dtype problems and CUDA failures ``RuntimeError``; there is no CPU fallback.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -86,25 +87,29 @@ def _args(code, q, k, v, g, beta, state, scale):
                                 *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *beta.stride())
 
 
-def _bytes(n, device):
-    return torch.empty(n, dtype=torch.uint8, device=device)
+@functools.lru_cache(maxsize=4096)
+def _sizes(code, B, T, Hk, Hv, dk, dv):
+    """Bytes of the stash, the forward's workspace and the backward's."""
+    lib = _lib.load()
+    a = _lib.DELTA_ARGS.pack(code, B, T, Hk, Hv, dk, dv, 1.0, *[0] * 21)
+    return lib.gru_delta_stash_bytes(a), lib.gru_delta_workspace_bytes(a, 0), lib.gru_delta_workspace_bytes(a, 1)
 
 
 def _forward(code, q, k, v, g, beta, state, scale):
     """out, the last state and what the gradient needs besides the inputs."""
     q, k, v = _dense_heads(q), _dense_heads(k), _dense_heads(v)
     state = None if state is None else state.contiguous()
-    B, T, Hv, dv = v.shape
-    dev = q.device
-    lib = _lib.load()
-    a = _args(code, q, k, v, g, beta, state, scale)
-    with _lib.on_device(dev.index):
-        out = torch.empty(B, T, Hv, dv, dtype=v.dtype, device=dev)
-        last = torch.empty(B, Hv, q.shape[3], dv, device=dev)
-        stash, ws = _bytes(lib.gru_delta_stash_bytes(a), dev), _bytes(lib.gru_delta_workspace_bytes(a, 0), dev)
-        _lib.check(lib.gru_delta_forward(a, out.data_ptr(), last.data_ptr(), stash.data_ptr(), stash.numel(),
-                                         ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream),
-                   "gru_delta_forward")
+    B, T, Hk, dk = q.shape
+    Hv, dv = v.shape[2:]
+    dev = q.get_device()
+    stash_bytes, ws_bytes, _ = _sizes(code, B, T, Hk, Hv, dk, dv)
+    with _lib.on_device(dev):
+        out = v.new_empty((B, T, Hv, dv))
+        last = g.new_empty((B, Hv, dk, dv))
+        stash, ws = g.new_empty(stash_bytes // 4), g.new_empty(ws_bytes // 4)
+        _lib.check(_lib.load().gru_delta_forward(
+            _args(code, q, k, v, g, beta, state, scale), out.data_ptr(), last.data_ptr(), stash.data_ptr(), stash_bytes,
+            ws.data_ptr(), ws_bytes, _lib.raw_stream(dev)), "gru_delta_forward")
     return out, last, stash, (q, k, v)
 
 
@@ -123,24 +128,23 @@ class GatedDeltaRuleFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout, dlast):
         q, k, v, g, beta, stash = ctx.saved_tensors
-        dev = q.device
-        lib = _lib.load()
-        with _lib.on_device(dev.index):
+        B, T, Hk, dk = q.shape
+        Hv, dv = v.shape[2:]
+        dev = q.get_device()
+        stash_bytes, _, ws_bytes = _sizes(ctx.code, B, T, Hk, Hv, dk, dv)
+        with _lib.on_device(dev):
             dout = None if dout is None else dout.contiguous()
             dlast = None if dlast is None else dlast.contiguous()
-            a = _args(ctx.code, q, k, v, g, beta, None, ctx.scale)
-            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-            dg, dbeta = (torch.empty(t.shape, device=dev) for t in (g, beta))
-            ds = None
-            if ctx.has_state and ctx.needs_input_grad[5]:
-                ds = torch.empty(q.shape[0], v.shape[2], q.shape[3], v.shape[3], device=dev)
-            ws = _bytes(lib.gru_delta_workspace_bytes(a, 1), dev)
-            _lib.check(lib.gru_delta_backward(
-                a, None if dout is None else dout.data_ptr(), None if dlast is None else dlast.data_ptr(),
-                stash.data_ptr(), stash.numel(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
-                dbeta.data_ptr(), None if ds is None else ds.data_ptr(), ws.data_ptr(), ws.numel(),
-                torch.cuda.current_stream(dev).cuda_stream), "gru_delta_backward")
-        return dq, dk, dv, dg, dbeta, ds, None
+            gq, gk, gv = q.new_empty((B, T, Hk, dk)), q.new_empty((B, T, Hk, dk)), q.new_empty((B, T, Hv, dv))
+            gg, gb = g.new_empty((B, T, Hv)), g.new_empty((B, T, Hv))
+            gs = g.new_empty((B, Hv, dk, dv)) if ctx.has_state and ctx.needs_input_grad[5] else None
+            ws = g.new_empty(ws_bytes // 4)
+            _lib.check(_lib.load().gru_delta_backward(
+                _args(ctx.code, q, k, v, g, beta, None, ctx.scale), 0 if dout is None else dout.data_ptr(),
+                0 if dlast is None else dlast.data_ptr(), stash.data_ptr(), stash_bytes, gq.data_ptr(), gk.data_ptr(),
+                gv.data_ptr(), gg.data_ptr(), gb.data_ptr(), 0 if gs is None else gs.data_ptr(), ws.data_ptr(), ws_bytes,
+                _lib.raw_stream(dev)), "gru_delta_backward")
+        return gq, gk, gv, gg, gb, gs, None
 
 
 def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
@@ -172,16 +176,15 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     q, k, v = _dense_heads(q), _dense_heads(k), _dense_heads(v)
     B, Hk, dk = q.shape
     Hv, dv = v.shape[1:]
-    dev = q.device
+    dev = q.get_device()
     (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.stride(), k.stride(), v.stride()
     (gb, gh), (bb, bh) = g.stride(), beta.stride()
     a = _lib.DELTA_ARGS.pack(code, B, 1, Hk, Hv, dk, dv, dk ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(),
                              v.data_ptr(), g.data_ptr(), beta.data_ptr(), 0, qb, 0, qh, kb, 0, kh, vb, 0, vh, gb, 0, gh,
                              bb, 0, bh)
-    with _lib.on_device(dev.index):
-        out = torch.empty(B, Hv, dv, dtype=v.dtype, device=dev)
-        _lib.check(_lib.load().gru_delta_step(a, state.data_ptr(), out.data_ptr(),
-                                              torch.cuda.current_stream(dev).cuda_stream), "gru_delta_step")
+    with _lib.on_device(dev):
+        out = v.new_empty((B, Hv, dv))
+        _lib.check(_lib.load().gru_delta_step(a, state.data_ptr(), out.data_ptr(), _lib.raw_stream(dev)), "gru_delta_step")
     torch.autograd.graph.increment_version(state)
     return out
 

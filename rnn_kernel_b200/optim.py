@@ -50,6 +50,7 @@ class _TypeTable:
         self.groups = [(lo, hi, int(self.group[lo])) for lo, hi in zip(cuts[:-1], cuts[1:])]
         self.entries = np.zeros(len(self.index), dtype=_ENTRY)
         self.entries["n"], self.entries["state_offset"] = opt._sizes[self.index], opt._offsets[self.index]
+        self.address = self.entries.ctypes.data
         self.addresses: list = []  # of the parameters, as in the entries
         self.copies = None         # dense copies of gradients that are not, until the launch
 
@@ -146,9 +147,8 @@ class AdamW:
         group_of = np.array([i for i, g in enumerate(self.param_groups) for _ in g["params"]], dtype=np.int64)
         # one table per element type, its entries in the parameters' order
         self._tables = [_TypeTable(self, dt, group_of) for dt in _DTYPES if any(p.dtype == dt for p in self.params)]
-        self._steady = True  # every parameter has had its gradient in every step
+        self._steady = True  # every parameter has had its gradient in every step: _steps is not kept up
 
-    @torch.no_grad()
     def step(self, grad_scale: float = 1.0) -> None:
         """Updates the parameters in place from their ``.grad`` times ``grad_scale``."""
         lib = _lib.load()
@@ -156,6 +156,8 @@ class AdamW:
         if any(m is not None for m in missing):
             if self.capturable:
                 raise RuntimeError("AdamW(capturable=True): every parameter needs a gradient.")
+            if self._steady:
+                self._steps[:] = self._calls
             self._steady = False
         self._calls += 1
         b1, b2 = self.betas
@@ -164,14 +166,17 @@ class AdamW:
         counter = None if self._device_step is None else self._device_step.data_ptr()
         scalars = None if self._scalars is None else self._scalars.data_ptr()
         with _lib.on_device(dev):
-            stream = torch.cuda.current_stream(dev).cuda_stream
+            stream = _lib.raw_stream(dev)
             for table, without in zip(self._tables, missing):
-                entries = table.entries if without is None else table.entries[~without]
+                entries, address = table.entries, table.address
+                if without is not None:
+                    entries = entries[~without]
+                    address = entries.ctypes.data
                 if not len(entries):
                     continue
                 self._rates(table, entries, without)
                 _lib.check(lib.gru_adamw_step(
-                    entries.ctypes.data, len(entries), table.code, self.state_bits, self.exp_avg.data_ptr(),
+                    address, len(entries), table.code, self.state_bits, self.exp_avg.data_ptr(),
                     self.exp_avg_sq.data_ptr(), *scales, self.state_elems, b1, b2, self.eps, grad_scale, self.seed,
                     self._calls, counter, scalars, stream), "gru_adamw_step")
                 counter = None  # counted once for all element types
@@ -191,7 +196,6 @@ class AdamW:
                 part["decay"] = 1.0 - lr * self.param_groups[i]["weight_decay"]
                 part["step_size"] = lr / r1
                 part["inv_sqrt_bc2"] = r2
-            self._steps[table.index] += 1
             return
         index = table.index if without is None else table.index[~without]
         group = table.group if without is None else table.group[~without]
@@ -221,7 +225,7 @@ class AdamW:
         with _lib.on_device(dev):
             _lib.check(_lib.load().gru_adamw_decode(
                 self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), self.scale_avg.data_ptr(), self.scale_sq.data_ptr(),
-                self.state_elems, m.data_ptr(), v.data_ptr(), torch.cuda.current_stream(dev).cuda_stream),
+                self.state_elems, m.data_ptr(), v.data_ptr(), _lib.raw_stream(dev)),
                 "gru_adamw_decode")
         return m, v
 
@@ -232,7 +236,7 @@ class AdamW:
     def state_dict(self) -> dict:
         """What continues this run bit for bit: moments as they are held, counts, and the groups' rates."""
         calls = self._calls if self._device_step is None else int(self._device_step)
-        steps = self._steps.tolist() if self._device_step is None else [calls] * len(self.params)
+        steps = [calls] * len(self.params) if self._steady else self._steps.tolist()
         return {"state_bits": self.state_bits, "seed": self.seed, "sizes": self._sizes.tolist(), "calls": calls,
                 "steps": steps, "exp_avg": self.exp_avg.clone(), "exp_avg_sq": self.exp_avg_sq.clone(),
                 "scale_avg": None if self.scale_avg is None else self.scale_avg.clone(),
