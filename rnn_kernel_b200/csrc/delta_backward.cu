@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
         x[n][2 * e + 1] = f.y;
       }
     const long nv = nv0 + chunk;
-    put_tokens<NP>(x, quarter, op, osc, a.dop + (nv * NP * groups + group) * kGroup * kC, (long)a.dvp * kC,
+    put_tokens<NP>(x, quarter, op, osc, a.dop + (nv * groups + group) * NP * kGroup * kC, kGroup * kC,
                    a.doscale + (nv * groups + group) * 4);
 #pragma unroll
     for (int n = 0; n < 2; ++n)
@@ -142,8 +142,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
   };
   auto state_out = [&](int chunk) {
     const long nv = nv0 + chunk;
-    put_state<DK>(d, quarter, sp, ssc, chunk >= 0 ? a.dstates + (nv * 2 * groups + group) * kGroup * DK : nullptr,
-                  (long)a.dvp * DK, a.dsscale + (nv * groups + group) * 4);
+    put_state<DK>(d, quarter, sp, ssc, chunk >= 0 ? a.dstates + (nv * groups + group) * 2 * kGroup * DK : nullptr,
+                  kGroup * DK, a.dsscale + (nv * groups + group) * 4);
   };
   back_load<NP, DK>(smem, a, nk0 + a.nc - 1, nv0 + a.nc - 1);
   load_dout(a.nc - 1);
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
     __syncthreads();
     // Z and dV
     times_tokens<2, 2, true>(x, wp, quarter * 2, up, 2 * kGroup * kC * 2, usc, -sw, quarter, 4);
-    put_tokens<2>(x, quarter, nullptr, nullptr, a.z + (nv * 2 * groups + group) * kGroup * kC, (long)a.dvp * kC,
+    put_tokens<2>(x, quarter, nullptr, nullptr, a.z + (nv * groups + group) * 2 * kGroup * kC, kGroup * kC,
                   a.zscale + (nv * groups + group) * 4);
 #pragma unroll
     for (int n = 0; n < 2; ++n)
@@ -229,8 +229,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
 
 // ---------------------------------------------------------------------------
 // grads: one CTA per (batch, key head, chunk).  It walks the value columns in
-// steps of 16 (one step of the products' inner dimension), three steps in
-// flight; each of 16 warps keeps 16 tokens x a quarter of the key columns of dQ,
+// steps of 16 (one step of the products' inner dimension), the next 32 loading
+// meanwhile; each of 16 warps keeps 16 tokens x a quarter of the key columns of dQ,
 // dK_row and dK_col, and of 16 tokens of dO U^T and Z U^T, in registers.  (Eight
 // warps of twice the tile had one CTA an SM as well, at 255 registers: 373 us for
 // train 4 x 2048 x 16 heads of 128.)
@@ -242,34 +242,29 @@ template <int NP, int DK>
 struct GradSmem {
   static constexpr int qk = NP * kC * DK;  // elements
   static constexpr int s = 2 * kGroup * DK, x = 2 * kGroup * kC, o = NP * kGroup * kC;
-  static constexpr int planes = 2 * s + 2 * x + o;  // S, dS, E, Z, dO of 16 columns
-  static constexpr int stage = planes + 5 * 8;       // and their scales
-  static constexpr int stages = 3;
+  // a stage: S, dS, E, Z, dO of two groups of 16 columns, each [group][plane], and their scales
+  static constexpr int planes = 2 * (2 * s + 2 * x + o);
+  static constexpr int stage = planes + 5 * 16;
   static constexpr int tiles = 4 * kTile * 2 + kC * (kC + 1) * 4;  // bytes: dP', M; y in FP32; over the stages
-  static constexpr int main = stages * stage * 2 > tiles ? stages * stage * 2 : tiles;
+  static constexpr int main = 2 * stage * 2 > tiles ? 2 * stage * 2 : tiles;
   static constexpr int bytes = 2 * qk * 2 + (main + 15) / 16 * 16 + kGates * kC * 4 + (9 * kC + 48) * 4;
 };
 
+// Two groups from the g-th on (of all chunks' groups).
 template <int NP, int DK>
-__device__ __forceinline__ void grad_load(f16* dst, const Problem& a, long nv, int c0) {
+__device__ __forceinline__ void grad_load(f16* dst, const Problem& a, long g) {
   using L = GradSmem<NP, DK>;
-#pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    copy_async(dst + p * kGroup * DK, a.states + (nv * 2 + p) * a.dvp * DK + (long)c0 * DK, kGroup * DK * 2);
-    copy_async(dst + L::s + p * kGroup * DK, a.dstates + (nv * 2 + p) * a.dvp * DK + (long)c0 * DK, kGroup * DK * 2);
-    copy_async(dst + 2 * L::s + p * kGroup * kC, a.e + (nv * 2 + p) * a.dvp * kC + (long)c0 * kC, kGroup * kC * 2);
-    copy_async(dst + 2 * L::s + L::x + p * kGroup * kC, a.z + (nv * 2 + p) * a.dvp * kC + (long)c0 * kC, kGroup * kC * 2);
+  copy_async(dst, a.states + g * L::s, 2 * L::s * 2);
+  copy_async(dst + 2 * L::s, a.dstates + g * L::s, 2 * L::s * 2);
+  copy_async(dst + 4 * L::s, a.e + g * L::x, 2 * L::x * 2);
+  copy_async(dst + 4 * L::s + 2 * L::x, a.z + g * L::x, 2 * L::x * 2);
+  copy_async(dst + 4 * L::s + 4 * L::x, a.dop + g * L::o, 2 * L::o * 2);
+  if (threadIdx.x < 10) {
+    const int t = threadIdx.x >> 1, i = threadIdx.x & 1;
+    const float* from = t == 0 ? a.sscale : t == 1 ? a.dsscale : t == 2 ? a.escale : t == 3 ? a.zscale : a.doscale;
+    cp_async16(dst + L::planes + (t * 2 + i) * 8, from + (g + i) * 4);
   }
-#pragma unroll
-  for (int p = 0; p < NP; ++p)
-    copy_async(dst + 2 * L::s + 2 * L::x + p * kGroup * kC, a.dop + (nv * NP + p) * a.dvp * kC + (long)c0 * kC,
-               kGroup * kC * 2);
-  const long g = (nv * (a.dvp / kGroup) + c0 / kGroup) * 4;
-  if (threadIdx.x < 5) {
-    const float* from = threadIdx.x == 0 ? a.sscale : threadIdx.x == 1 ? a.dsscale : threadIdx.x == 2 ? a.escale
-                      : threadIdx.x == 3 ? a.zscale : a.doscale;
-    cp_async16(dst + L::planes + threadIdx.x * 8, from + g);
-  }
+  cp_async_commit();
 }
 
 // The value pair `word` of a tile held as planes, without its scale.
@@ -347,10 +342,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
     const long nv = ((long)b * a.Hv + hv) * a.nc + chunk;
     __syncthreads();
     copy_async(gate, a.gates + nv * kGates * kC, kGates * kC * 4);
-    grad_load<NP, DK>(main, a, nv, 0);
-    cp_async_commit();
-    grad_load<NP, DK>(main + L::stage, a, nv, kGroup);  // dvp is a multiple of two groups
-    cp_async_commit();
+    grad_load<NP, DK>(main, a, nv * groups);
     float dp[2][4], da[2][4], dq[NT][4], dkr[NT][4], dkc[NT][4];
     zero(dp);
     zero(da);
@@ -359,20 +351,21 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
     zero(dkc);
     float sdot = 0.0f, bdot[2] = {0.0f, 0.0f};
     for (int g = 0; g < groups; ++g) {
-      cp_async_wait<1>();
-      __syncthreads();
-      if (g + 2 < groups) grad_load<NP, DK>(main + (g + 2) % L::stages * L::stage, a, nv, (g + 2) * kGroup);
-      cp_async_commit();
-      const f16* sp = main + g % L::stages * L::stage;
-      const f16* dsp = sp + L::s;
-      const f16* ep = dsp + L::s;
-      const f16* zp = ep + L::x;
-      const f16* op = zp + L::x;
-      // scales: of this warp's 16 tokens, of its 32 columns of tokens, and of the
-      // quarters of the key columns
-      const float* scales = reinterpret_cast<const float*>(sp + L::planes);  // of S, dS, E, Z, dO
+      const f16* stage = main + ((g >> 1) & 1) * L::stage;
+      if ((g & 1) == 0) {
+        cp_async_wait<0>();
+        __syncthreads();
+        if (g + 2 < groups) grad_load<NP, DK>(main + (((g >> 1) + 1) & 1) * L::stage, a, nv * groups + g + 2);
+      }
+      const f16* sp = stage + (g & 1) * L::s;
+      const f16* dsp = sp + 2 * L::s;
+      const f16* ep = stage + 4 * L::s + (g & 1) * L::x;
+      const f16* zp = ep + 2 * L::x;
+      const f16* op = stage + 4 * L::s + 4 * L::x + (g & 1) * L::o;
+      // scales: of the quarters of the key columns (S, dS) and of the tokens
+      const float* scales = reinterpret_cast<const float*>(stage + L::planes) + (g & 1) * 4;
       const int mq = m0 / 16;
-      const float se = fabsf(scales[8 + mq]), sz = scales[12 + mq], so = scales[16 + mq];
+      const float se = fabsf(scales[16 + mq]), sz = scales[24 + mq], so = scales[32 + mq];
       uint32_t fz[2][4], fe[2][4];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
@@ -391,7 +384,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
       {
         uint32_t fb[2][NT][2];
         load_b<2, NT, false>(fb, addr_b<kGroup, false>(dsp, 0, col * NT), 512, kGroup * DK * 2);
-        step_add<2, 2, NT>(dkc, se * scales[4 + col], fe, fb);
+        step_add<2, 2, NT>(dkc, se * scales[8 + col], fe, fb);
       }
       uint32_t fo[NP][4];
 #pragma unroll
@@ -405,7 +398,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
       if (col <= mq) {
         uint32_t fb[2][2][2];
         load_b<2, 2, false>(fb, addr_b<kGroup, false>(ep, 0, col * 2), 512, kGroup * kC * 2);
-        const float f = fabsf(scales[8 + col]);
+        const float f = fabsf(scales[16 + col]);
         step_add<NP, 2, 2>(dp, so * f, fo, fb);
         step_add<2, 2, 2>(da, sz * f, fz, fb);
       }
@@ -414,7 +407,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
         // block warp + 16 i is of the rows 8 (warp / 2 + 8 i) ..., in this quarter
         const int w = threadIdx.x + i * kGradThreads, q = (warp / 2 + 8 * i) * 8 / (DK / 4);
         const float2 u = take2<2>(sp, kGroup * DK, w), v = take2<2>(dsp, kGroup * DK, w);
-        sdot += (scales[q] * scales[4 + q]) * (u.x * v.x + u.y * v.y);
+        sdot += (scales[q] * scales[8 + q]) * (u.x * v.x + u.y * v.y);
       }
     }
     __syncthreads();
@@ -445,8 +438,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
           const int i = frag_row(m0, e), j = frag_col(col * 16 + n * 8);
 #pragma unroll
           for (int l = 0; l < 2; ++l) {
-            const float dec = j + l <= i ? expf((gate[3 * kC + i] - gate[3 * kC + j + l]) +
-                                                (gate[4 * kC + i] - gate[4 * kC + j + l])) * gate[2 * kC + j + l]
+            const float dec = j + l <= i ? decay_between(gate, i, j + l) * gate[2 * kC + j + l]
                                          : 0.0f;
             float& u = dp[n][2 * e + l];
             float& w = da[n][2 * e + l];

@@ -31,8 +31,8 @@ constexpr int kSlice = 32;  // value columns of a scan's CTA; they are padded to
 constexpr int kThreads = 256;
 constexpr int kTile = kC * kC;  // elements of a token x token tile
 
-// Rows of Problem::gates, 64 floats each: e^G_i, e^(G_end - G_i), beta_i, G_i as
-// two floats, and the scales of the planes of W, P, K and Q.
+// Rows of Problem::gates, 64 floats each: e^G_i, e^(G_end - G_i), beta_i, G_i /
+// log 2 as two floats, and the scales of the planes of W, P, K and Q.
 constexpr int kGates = 6;
 
 // Log decays below this count as this: e^-1000 is zero in FP32, and sums of 64
@@ -71,7 +71,7 @@ struct Problem {
   f16* wp;       // [n over Hv][2][64 x 64]
   f16* pp;       // [n over Hv][2][64 x 64]: P, for the output P B
   float* gates;  // [n over Hv][kGates][64]
-  // Tiles of 16 value columns each, [n over Hv][plane][group][rows x 16], rows
+  // Tiles of 16 value columns each, [n over Hv][group][plane][rows x 16], rows
   // the key columns of a state or the tokens; every quarter of a tile's rows
   // has its own scale, [n over Hv][group][4].
   f16* states;   // the state before the chunk
@@ -199,6 +199,11 @@ __device__ __forceinline__ void load_b(uint32_t (&fb)[NB][NT][2], uint32_t addr,
       ldm4<TRANS>(r, addr + p * plane + (n / 2) * next);
       fb[p][n][0] = r[0], fb[p][n][1] = r[1], fb[p][n + 1][0] = r[2], fb[p][n + 1][1] = r[3];
     }
+}
+
+// e^(G_i - G_j) from the gates.
+__device__ __forceinline__ float decay_between(const float* gates, int i, int j) {
+  return exp2f((gates[3 * kC + i] - gates[3 * kC + j]) + (gates[4 * kC + i] - gates[4 * kC + j]));
 }
 
 template <int NT>

@@ -155,8 +155,9 @@ __device__ __forceinline__ void chunk_gates(const Problem& a, int b, int hv, int
     gates[i] = i < first ? expf((float)gi) : __uint_as_float(0x7fffffffu);
     gates[kC + i] = expf((float)(end - gi));
     gates[2 * kC + i] = be[e];
-    gates[3 * kC + i] = (float)gi;
-    gates[4 * kC + i] = (float)(gi - (double)(float)gi);
+    const double g2 = gi * 1.4426950408889634;
+    gates[3 * kC + i] = (float)g2;
+    gates[4 * kC + i] = (float)(g2 - (double)(float)g2);
   }
 }
 
@@ -334,11 +335,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
         float nn[2];
 #pragma unroll
         for (int l = 0; l < 2; ++l) {
-          const float d = j + l <= i ? expf((gates[3 * kC + i] - gates[3 * kC + j + l]) +
-                                            (gates[4 * kC + i] - gates[4 * kC + j + l]))
-                                     : 0.0f;
+          const float d = j + l <= i ? decay_between(gates, i, j + l) : 0.0f;
           nn[l] = j + l < i ? ak[n][2 * e + l] * d : 0.0f;
-          const float p = j + l <= i ? aq[n][2 * e + l] * d * a.scale : 0.0f;
+          const float p = j + l <= i ? aq[n][2 * e + l] * (d * a.scale) : 0.0f;
           pv[n][2 * e + l] = fold_beta ? p * gates[2 * kC + j + l] : p;
           mp = max_finite(mp, pv[n][2 * e + l]);
         }
@@ -505,8 +504,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
   };
   auto state_out = [&](int chunk) {
     const long nv = nv0 + chunk;
-    put_state<DK>(s, quarter, sp, ssc, chunk < a.nc ? a.states + (nv * 2 * groups + group) * kGroup * DK : nullptr,
-                  (long)a.dvp * DK, a.sscale + (nv * groups + group) * 4);
+    put_state<DK>(s, quarter, sp, ssc, chunk < a.nc ? a.states + (nv * groups + group) * 2 * kGroup * DK : nullptr,
+                  kGroup * DK, a.sscale + (nv * groups + group) * 4);
   };
   scan_load<NP, DK>(smem, a, nk0, nv0);
   load_v(0);
@@ -586,14 +585,14 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
       const float inv = plane_inv(warp_max(x, all_finite));
       // a scale below zero marks a quarter that holds something not finite
       if (lane == 0) a.escale[(nv * groups + group) * 4 + quarter] = all_finite ? plane_scale(inv) : -plane_scale(inv);
-      f16* out = a.e + (nv * 2 * groups + group) * kGroup * kC;
+      f16* out = a.e + (nv * groups + group) * 2 * kGroup * kC;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           uint32_t w[2];
           split2<2>(x[n][2 * e], x[n][2 * e + 1], inv, w);
-          store_pair<2>(out, (long)a.dvp * kC, quarter * 2 + e, n, w);
+          store_pair<2>(out, kGroup * kC, quarter * 2 + e, n, w);
         }
     }
     // S <- e^G S + K^T (e^(G_end - G) U)
@@ -659,10 +658,15 @@ template <typename T, int DK>
 __device__ __forceinline__ void output_load(f16* dst, const Problem& a, long nv, int c0) {
   using L = OutputSmem<T, DK>;
   const int cols = min(L::cols, a.dvp - c0);
-#pragma unroll
-  for (int p = 0; p < L::NP; ++p) {
-    copy_async(dst + p * L::cols * DK, a.states + (nv * 2 + p) * a.dvp * DK + (long)c0 * DK, cols * DK * 2);
-    copy_async(dst + L::s + p * L::cols * kC, a.e + (nv * 2 + p) * a.dvp * kC + (long)c0 * kC, cols * kC * 2);
+  const long first = nv * (a.dvp / kGroup) + c0 / kGroup;
+  // of both planes of a group in memory the first NP, in the order [group][plane]
+  for (int i = threadIdx.x; i < cols * L::NP * DK / 8; i += kThreads) {
+    constexpr int per = L::NP * kGroup * DK / 8;
+    cp_async16(dst + i * 8, a.states + (first + i / per) * 2 * kGroup * DK + (i % per) * 8);
+  }
+  for (int i = threadIdx.x; i < cols * L::NP * kC / 8; i += kThreads) {
+    constexpr int per = L::NP * kGroup * kC / 8;
+    cp_async16(dst + L::s + i * 8, a.e + (first + i / per) * 2 * kGroup * kC + (i % per) * 8);
   }
   const long g = (nv * (a.dvp / kGroup) + c0 / kGroup) * 4;
   copy_async(dst + L::s + L::e, a.sscale + g, cols);
@@ -757,13 +761,13 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a)
     if (cw < a.dvp) {
       const float* fs = reinterpret_cast<const float*>(ep + L::e) + half * 8;
       const float* fe = fs + 16;
-      const f16* sg = sp + half * 2 * kGroup * DK;
-      const f16* eg = ep + half * 2 * kGroup * kC;
+      const f16* sg = sp + half * 2 * NP * kGroup * DK;
+      const f16* eg = ep + half * 2 * NP * kGroup * kC;
       float x[4][4], y[4][4];
       zero(x);
       zero(y);
       output_product<NP, DK / 16, DK / 64>(x, addr_a<DK, false>(qp, m0 / 8, 0), kC * DK * 2,
-                                           addr_b<kGroup, true>(sg, 0, 0), L::cols * DK * 2, kGroup * DK * 2, DK / 16, fs);
+                                           addr_b<kGroup, true>(sg, 0, 0), kGroup * DK * 2, NP * kGroup * DK * 2, DK / 16, fs);
       bool lost = false;
 #pragma unroll
       for (int i = 0; i < 8; ++i) lost |= fe[i] < 0.0f;
@@ -772,11 +776,11 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a)
         for (int n = 0; n < 4; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            y[n][e] = output_element<NP>(pp, eg + (n >> 1) * kGroup * kC, L::cols * kC, fe + (n >> 1) * 4,
+            y[n][e] = output_element<NP>(pp, eg + (n >> 1) * NP * kGroup * kC, kGroup * kC, fe + (n >> 1) * 4,
                                          frag_row(m0, e >> 1), frag_col((n & 1) * 8) + (e & 1));
       } else {
         output_product<NP, 4, 1>(y, addr_a<kC, false>(pp, m0 / 8, 0), kTile * 2, addr_b<kGroup, true>(eg, 0, 0),
-                                 L::cols * kC * 2, kGroup * kC * 2, m0 / 16 + 1, fe);
+                                 kGroup * kC * 2, NP * kGroup * kC * 2, m0 / 16 + 1, fe);
       }
       const float fx = a.scale * gate[5 * kC + 3], fy = gate[5 * kC + 1];
 #pragma unroll

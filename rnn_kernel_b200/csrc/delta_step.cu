@@ -9,7 +9,8 @@
 // reduction over dk, for both sums, before the writes.  A CTA owns 32 value
 // columns of one head: a warp takes four rows of 128 bytes at a time, a thread
 // keeps its (up to four) float4 of the state in registers from read to write.
-// HBM-bound: 8 dk dv bytes a head.
+// HBM-bound: 8 dk dv bytes a head, which are loaded and stored as used once
+// (64 sequences x 32 heads of 128 x 128: 54.1 -> 49.2 us, 85 % of the copy rate).
 
 #include <string>
 
@@ -31,8 +32,11 @@ struct Step {
   float scale;
 };
 
-template <typename T>
+// ROWS: the rows of a thread where the key columns are that many times 32 and
+// four value columns make an aligned access; 0: any sizes.
+template <typename T, int ROWS>
 __global__ void __launch_bounds__(kThreads) delta_step_kernel(const Step a) {
+  constexpr int R = ROWS ? ROWS : kMaxD / 32;
   __shared__ float ks[kMaxD], qs[kMaxD];
   __shared__ __align__(16) float part[2][8][kSlice];
   __shared__ __align__(16) float us[kSlice];
@@ -43,16 +47,16 @@ __global__ void __launch_bounds__(kThreads) delta_step_kernel(const Step a) {
   const int row0 = warp * 4 + (lane >> 3);        // and rows row0, row0 + 32, ...
   float* s = a.s + (long)bh * a.dk * a.dv + c;
   const int left = a.dv - c;
-  float4 x[kMaxD / 32];
-  const float* safe = a.s + (long)bh * a.dk * a.dv;
-  if (a.vec) {
+  float4 x[R];
+  if (ROWS) {
 #pragma unroll
-    for (int i = 0; i < kMaxD / 32; ++i)
-      x[i] = load4(s + (long)(row0 + 32 * i) * a.dv, safe, row0 + 32 * i < a.dk && left > 0);
+    for (int i = 0; i < R; ++i)
+      x[i] = left > 0 ? __ldcs(reinterpret_cast<const float4*>(s + (row0 + 32 * i) * a.dv)) : make_float4(0.f, 0.f, 0.f, 0.f);
   } else {
+    const float* safe = a.s + (long)bh * a.dk * a.dv;
 #pragma unroll
-    for (int i = 0; i < kMaxD / 32; ++i)
-      x[i] = load4_any(s + (long)(row0 + 32 * i) * a.dv, safe, row0 + 32 * i < a.dk ? left : 0);
+    for (int i = 0; i < R; ++i)
+      x[i] = load4_any(s + (row0 + 32 * i) * a.dv, safe, row0 + 32 * i < a.dk ? left : 0);
   }
   if (threadIdx.x < kMaxD) {
     const int d = threadIdx.x;
@@ -66,7 +70,7 @@ __global__ void __launch_bounds__(kThreads) delta_step_kernel(const Step a) {
   __syncthreads();
   float4 sk = make_float4(0.f, 0.f, 0.f, 0.f), sq = sk;
 #pragma unroll
-  for (int i = 0; i < kMaxD / 32; ++i) {
+  for (int i = 0; i < R; ++i) {
     const float kr = ks[row0 + 32 * i], qr = qs[row0 + 32 * i];
     x[i].x *= decay, x[i].y *= decay, x[i].z *= decay, x[i].w *= decay;
     sk.x += x[i].x * kr, sk.y += x[i].y * kr, sk.z += x[i].z * kr, sk.w += x[i].w * kr;
@@ -106,22 +110,33 @@ __global__ void __launch_bounds__(kThreads) delta_step_kernel(const Step a) {
   __syncthreads();
   const float4 u = *reinterpret_cast<const float4*>(&us[(lane & 7) * 4]);
 #pragma unroll
-  for (int i = 0; i < kMaxD / 32; ++i) {
+  for (int i = 0; i < R; ++i) {
     const int r = row0 + 32 * i;
-    if (r >= a.dk) continue;
     const float kr = ks[r];
     const float4 y = make_float4(x[i].x + kr * u.x, x[i].y + kr * u.y, x[i].z + kr * u.z, x[i].w + kr * u.w);
-    float* p = s + (long)r * a.dv;
-    if (a.vec) {
-      if (left <= 0) continue;
-      *reinterpret_cast<float4*>(p) = y;
-    } else {
+    float* p = s + r * a.dv;
+    if (ROWS) {
+      if (left > 0) __stcs(reinterpret_cast<float4*>(p), y);
+    } else if (r < a.dk) {
       if (left > 0) p[0] = y.x;
       if (left > 1) p[1] = y.y;
       if (left > 2) p[2] = y.z;
       if (left > 3) p[3] = y.w;
     }
   }
+}
+
+template <typename T>
+int launch_step(const Step& a, unsigned ctas, cudaStream_t stream) {
+  const int rows = a.vec && a.dk % 32 == 0 ? a.dk / 32 : 0;
+  LaunchScope scope(kKindDeltaRule, stream);
+  if (rows == 1) delta_step_kernel<T, 1><<<ctas, kThreads, 0, stream>>>(a);
+  else if (rows == 2) delta_step_kernel<T, 2><<<ctas, kThreads, 0, stream>>>(a);
+  else if (rows == 3) delta_step_kernel<T, 3><<<ctas, kThreads, 0, stream>>>(a);
+  else if (rows == 4) delta_step_kernel<T, 4><<<ctas, kThreads, 0, stream>>>(a);
+  else delta_step_kernel<T, 0><<<ctas, kThreads, 0, stream>>>(a);
+  GRU_CUDA_TRY(cudaGetLastError());
+  return GRU_OK;
 }
 
 int bad(const char* what, const char* msg, int code = GRU_ERR_INVALID) {
@@ -311,9 +326,5 @@ extern "C" int gru_delta_step(const gru_delta_args* p, float* state, void* out, 
          p->Hv, p->Hv / p->Hk, p->dk, p->dv, (p->dv + kSlice - 1) / kSlice,
          p->dv % 4 == 0 && (reinterpret_cast<uintptr_t>(state) & 15) == 0, p->scale};
   const unsigned ctas = (unsigned)((long)p->B * p->Hv * a.slices);
-  LaunchScope scope(kKindDeltaRule, stream);
-  if (p->dtype == GRU_F32) delta_step_kernel<float><<<ctas, kThreads, 0, stream>>>(a);
-  else delta_step_kernel<bf16><<<ctas, kThreads, 0, stream>>>(a);
-  GRU_CUDA_TRY(cudaGetLastError());
-  return GRU_OK;
+  return p->dtype == GRU_F32 ? launch_step<float>(a, ctas, stream) : launch_step<bf16>(a, ctas, stream);
 }
