@@ -48,11 +48,11 @@ template <int NP, int DK>
 __device__ __forceinline__ void back_load(unsigned char* stage, const Problem& a, long nk, long nv) {
   using L = BackSmem<NP, DK, 1>;
   f16* p = reinterpret_cast<f16*>(stage);
-  copy_async(p, a.kp + nk * L::k, L::k * 2);
-  copy_async(p + L::k, a.qp + nk * L::k, L::k * 2);
-  copy_async(p + 2 * L::k, a.wp + nv * L::w, L::w * 2);
-  copy_async(p + 2 * L::k + L::w, a.pp + nv * L::w, L::w * 2);
-  copy_async(p + 2 * (L::k + L::w), a.gates + nv * kGates * kC, kGates * kC * 4);
+  copy_async<L::k * 2, kThreads>(p, a.kp + nk * L::k);
+  copy_async<L::k * 2, kThreads>(p + L::k, a.qp + nk * L::k);
+  copy_async<L::w * 2, kThreads>(p + 2 * L::k, a.wp + nv * L::w);
+  copy_async<L::w * 2, kThreads>(p + 2 * L::k + L::w, a.pp + nv * L::w);
+  copy_async<kGates * kC * 4, kThreads>(p + 2 * (L::k + L::w), a.gates + nv * kGates * kC);
   cp_async_commit();
 }
 
@@ -254,11 +254,11 @@ struct GradSmem {
 template <int NP, int DK>
 __device__ __forceinline__ void grad_load(f16* dst, const Problem& a, long g) {
   using L = GradSmem<NP, DK>;
-  copy_async(dst, a.states + g * L::s, 2 * L::s * 2);
-  copy_async(dst + 2 * L::s, a.dstates + g * L::s, 2 * L::s * 2);
-  copy_async(dst + 4 * L::s, a.e + g * L::x, 2 * L::x * 2);
-  copy_async(dst + 4 * L::s + 2 * L::x, a.z + g * L::x, 2 * L::x * 2);
-  copy_async(dst + 4 * L::s + 4 * L::x, a.dop + g * L::o, 2 * L::o * 2);
+  copy_async<4 * L::s, kGradThreads>(dst, a.states + g * L::s);
+  copy_async<4 * L::s, kGradThreads>(dst + 2 * L::s, a.dstates + g * L::s);
+  copy_async<4 * L::x, kGradThreads>(dst + 4 * L::s, a.e + g * L::x);
+  copy_async<4 * L::x, kGradThreads>(dst + 4 * L::s + 2 * L::x, a.z + g * L::x);
+  copy_async<4 * L::o, kGradThreads>(dst + 4 * L::s + 4 * L::x, a.dop + g * L::o);
   if (threadIdx.x < 10) {
     const int t = threadIdx.x >> 1, i = threadIdx.x & 1;
     const float* from = t == 0 ? a.sscale : t == 1 ? a.dsscale : t == 2 ? a.escale : t == 3 ? a.zscale : a.doscale;
@@ -334,14 +334,14 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
   const int m0 = (warp >> 2) * 16, col = warp & 3;  // this warp's tokens; its quarter of the columns
   const int groups = a.dvp / kGroup;
 
-  copy_async(qp, a.qp + (long)blockIdx.x * L::qk, L::qk * 2);
-  copy_async(kp, a.kp + (long)blockIdx.x * L::qk, L::qk * 2);
+  copy_async<L::qk * 2, kGradThreads>(qp, a.qp + (long)blockIdx.x * L::qk);
+  copy_async<L::qk * 2, kGradThreads>(kp, a.kp + (long)blockIdx.x * L::qk);
 
   for (int r = 0; r < a.rep; ++r) {
     const int hv = hk * a.rep + r;
     const long nv = ((long)b * a.Hv + hv) * a.nc + chunk;
     __syncthreads();
-    copy_async(gate, a.gates + nv * kGates * kC, kGates * kC * 4);
+    copy_async<kGates * kC * 4, kGradThreads>(gate, a.gates + nv * kGates * kC);
     grad_load<NP, DK>(main, a, nv * groups);
     float dp[2][4], da[2][4], dq[NT][4], dkr[NT][4], dkc[NT][4];
     zero(dp);

@@ -108,10 +108,16 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N));
 }
-// `bytes` (a multiple of 16) from global to shared memory, by all threads.
-__device__ __forceinline__ void copy_async(void* dst, const void* src, int bytes) {
-  for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16)
-    cp_async16(static_cast<char*>(dst) + i, static_cast<const char*>(src) + i);
+// BYTES (a multiple of 16) from global to shared memory by THREADS threads:
+// one address each, the rest constant offsets.
+template <int BYTES, int THREADS>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  constexpr int n = BYTES / 16, full = n / THREADS, rest = n % THREADS;
+  char* d = static_cast<char*>(dst) + threadIdx.x * 16;
+  const char* s = static_cast<const char*>(src) + threadIdx.x * 16;
+#pragma unroll
+  for (int i = 0; i < full; ++i) cp_async16(d + i * THREADS * 16, s + i * THREADS * 16);
+  if (rest > 0 && threadIdx.x < rest) cp_async16(d + full * THREADS * 16, s + full * THREADS * 16);
 }
 
 template <bool TRANS>

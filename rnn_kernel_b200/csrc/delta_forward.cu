@@ -458,9 +458,9 @@ template <int NP, int DK>
 __device__ __forceinline__ void scan_load(unsigned char* stage, const Problem& a, long nk, long nv) {
   using L = ScanSmem<NP, DK>;
   f16* k = reinterpret_cast<f16*>(stage);
-  copy_async(k, a.kp + nk * L::k, L::k * 2);
-  copy_async(k + L::k, a.wp + nv * L::w, L::w * 2);
-  copy_async(k + L::k + L::w, a.gates + nv * kGates * kC, kGates * kC * 4);
+  copy_async<L::k * 2, kThreads>(k, a.kp + nk * L::k);
+  copy_async<L::w * 2, kThreads>(k + L::k, a.wp + nv * L::w);
+  copy_async<kGates * kC * 4, kThreads>(k + L::k + L::w, a.gates + nv * kGates * kC);
   cp_async_commit();
 }
 
@@ -657,20 +657,19 @@ struct OutputSmem {
 template <typename T, int DK>
 __device__ __forceinline__ void output_load(f16* dst, const Problem& a, long nv, int c0) {
   using L = OutputSmem<T, DK>;
-  const int cols = min(L::cols, a.dvp - c0);
   const long first = nv * (a.dvp / kGroup) + c0 / kGroup;
   // of both planes of a group in memory the first NP, in the order [group][plane]
-  for (int i = threadIdx.x; i < cols * L::NP * DK / 8; i += kThreads) {
-    constexpr int per = L::NP * kGroup * DK / 8;
-    cp_async16(dst + i * 8, a.states + (first + i / per) * 2 * kGroup * DK + (i % per) * 8);
+#pragma unroll
+  for (int g = 0; g < L::cols / kGroup; ++g) {
+    if (c0 + g * kGroup >= a.dvp) break;
+    copy_async<L::NP * kGroup * DK * 2, kThreads>(dst + g * L::NP * kGroup * DK, a.states + (first + g) * 2 * kGroup * DK);
+    copy_async<L::NP * kGroup * kC * 2, kThreads>(dst + L::s + g * L::NP * kGroup * kC, a.e + (first + g) * 2 * kGroup * kC);
   }
-  for (int i = threadIdx.x; i < cols * L::NP * kC / 8; i += kThreads) {
-    constexpr int per = L::NP * kGroup * kC / 8;
-    cp_async16(dst + L::s + i * 8, a.e + (first + i / per) * 2 * kGroup * kC + (i % per) * 8);
+  if (threadIdx.x < 8) {
+    const int g = threadIdx.x & 3;
+    if (c0 + g * kGroup < a.dvp)
+      cp_async16(dst + L::s + L::e + threadIdx.x * 8, (threadIdx.x < 4 ? a.sscale : a.escale) + (first + g) * 4);
   }
-  const long g = (nv * (a.dvp / kGroup) + c0 / kGroup) * 4;
-  copy_async(dst + L::s + L::e, a.sscale + g, cols);
-  copy_async(dst + L::s + L::e + 32, a.escale + g, cols);
   cp_async_commit();
 }
 
@@ -739,9 +738,9 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a)
   const int chunk = blockIdx.x % a.nc, bh = blockIdx.x / a.nc;
   const int hv = bh % a.Hv, b = bh / a.Hv;
   const long nv = blockIdx.x, nk = ((long)b * a.Hk + hv / a.rep) * a.nc + chunk;
-  copy_async(qp, a.qp + nk * L::q, L::q * 2);
-  copy_async(pp, a.pp + nv * 2 * kTile, L::p * 2);
-  copy_async(gate, a.gates + nv * kGates * kC, kGates * kC * 4);
+  copy_async<L::q * 2, kThreads>(qp, a.qp + nk * L::q);
+  copy_async<L::p * 2, kThreads>(pp, a.pp + nv * 2 * kTile);
+  copy_async<kGates * kC * 4, kThreads>(gate, a.gates + nv * kGates * kC);
   output_load<T, DK>(slices, a, nv, 0);
   const int warp = threadIdx.x >> 5;
   const int m0 = (warp >> 1) * 16, half = warp & 1;
