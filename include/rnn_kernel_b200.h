@@ -176,15 +176,16 @@ typedef struct {
   long q_stride[3], k_stride[3], v_stride[3], g_stride[3], beta_stride[3];
 } gru_delta_args; /* host struct */
 
-/* Bytes that gru_delta_forward leaves for gru_delta_backward (the forward
- * needs them too when no backward follows), and each one's workspace, from
- * the sizes alone (the tensors may be NULL); 0 and an error text for sizes that
- * they refuse. */
+/* Bytes that a training forward leaves for gru_delta_backward, and the
+ * workspace of that (backward != 0) or of a forward without a stash, from the
+ * sizes alone (the tensors may be NULL); 0 and an error text for sizes that they
+ * refuse. */
 size_t gru_delta_stash_bytes(const gru_delta_args* args);
 size_t gru_delta_workspace_bytes(const gru_delta_args* args, int backward);
 
 /* All T tokens: out dense [B, T, Hv, dv], final_state dense [B, Hv, dk, dv]
- * (which may be the initial state's memory). */
+ * (which may be the initial state's memory).  stash: gru_delta_stash_bytes()
+ * bytes for a training forward, which needs no workspace, or NULL. */
 int gru_delta_forward(const gru_delta_args* args, void* out, float* final_state, void* stash, size_t stash_bytes,
                       void* workspace, size_t workspace_bytes, void* stream);
 

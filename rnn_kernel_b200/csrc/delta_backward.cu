@@ -17,8 +17,7 @@
 // decay of token t multiplies, and nothing besides (running sums of q . dq -
 // k . dk would do, but cancel most of their digits).
 //
-// W and P are computed again (`prepare`) rather than kept from the forward.
-// `scan` walks the chunks backwards as the forward's scan does and leaves dS1,
+// K, Q, W and P come as the forward left them.  `scan` walks the chunks backwards as the forward's scan does and leaves dS1,
 // Z and dO as planes; `grads` (all chunks at once) does the rest, a CTA per key
 // head, over its value heads in a fixed order.
 
@@ -142,8 +141,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
   };
   auto state_out = [&](int chunk) {
     const long nv = nv0 + chunk;
-    put_state<DK>(d, quarter, sp, ssc, chunk >= 0 ? a.dstates + (nv * groups + group) * 2 * kGroup * DK : nullptr,
-                  kGroup * DK, a.dsscale + (nv * groups + group) * 4);
+    put_state<DK, 2>(d, quarter, sp, ssc, chunk >= 0 ? a.dstates + (nv * groups + group) * 2 * kGroup * DK : nullptr,
+                     a.dsscale + (nv * groups + group) * 4);
   };
   back_load<NP, DK>(smem, a, nk0 + a.nc - 1, nv0 + a.nc - 1);
   load_dout(a.nc - 1);
@@ -644,7 +643,6 @@ int backward_typed(const Problem& a, cudaStream_t stream) {
 }  // namespace
 
 int backward(const Problem& a, int dtype, cudaStream_t stream) {
-  if (const int rc = prepare(a, dtype, false, stream)) return rc;
   if (dtype == GRU_F32)
     return a.dk <= 64 ? backward_typed<float, 64>(a, stream) : backward_typed<float, 128>(a, stream);
   return a.dk <= 64 ? backward_typed<bf16, 64>(a, stream) : backward_typed<bf16, 128>(a, stream);

@@ -32,7 +32,8 @@ constexpr int kThreads = 256;
 constexpr int kTile = kC * kC;  // elements of a token x token tile
 
 // Rows of Problem::gates, 64 floats each: e^G_i, e^(G_end - G_i), beta_i, G_i /
-// log 2 as two floats, and the scales of the planes of W, P, K and Q.
+// log 2 as two floats, and the scales of the planes of W, P, K and Q and a power
+// of two above every |beta|.
 constexpr int kGates = 6;
 
 // Log decays below this count as this: e^-1000 is zero in FP32, and sums of 64
@@ -69,8 +70,9 @@ struct Problem {
   f16* kp;       // [n over Hk][NP][64 x DK]
   f16* qp;       // [n over Hk][NP][64 x DK]
   f16* wp;       // [n over Hv][2][64 x 64]
-  f16* pp;       // [n over Hv][2][64 x 64]: P, for the output P B
+  f16* pp;       // [n over Hv][2][64 x 64]
   float* gates;  // [n over Hv][kGates][64]
+  int planes;    // of states and e in memory: 2, or 1 where only a bf16 output reads them
   // Tiles of 16 value columns each, [n over Hv][group][plane][rows x 16], rows
   // the key columns of a state or the tokens; every quarter of a tile's rows
   // has its own scale, [n over Hv][group][4].
@@ -92,7 +94,6 @@ struct Problem {
   float* dqk;    // [n over Hk][2][64][DK]: dq and dk summed over a key head's value heads
 };
 
-int prepare(const Problem& a, int dtype, bool fold_beta, cudaStream_t stream);
 int forward(const Problem& a, int dtype, cudaStream_t stream);
 int backward(const Problem& a, int dtype, cudaStream_t stream);
 
@@ -292,36 +293,45 @@ __device__ __forceinline__ float warp_max(const float (&x)[NT][4]) {
 }
 
 // Writes an accumulator pair (row block r8, column tile n) of a tile of 16
-// columns, `plane` elements between planes.
+// columns, `plane` elements between planes; the first `np` of the NP planes.
 template <int NP>
-__device__ __forceinline__ void store_pair(f16* tile, long plane, int r8, int n, const uint32_t (&w)[NP]) {
+__device__ __forceinline__ void store_pair(f16* tile, long plane, int r8, int n, const uint32_t (&w)[NP], int np = NP) {
 #pragma unroll
   for (int p = 0; p < NP; ++p)
-    reinterpret_cast<uint32_t*>(tile + p * plane)[(r8 * 2 + n) * 32 + (threadIdx.x & 31)] = w[p];
+    if (p < np) reinterpret_cast<uint32_t*>(tile + p * plane)[(r8 * 2 + n) * 32 + (threadIdx.x & 31)] = w[p];
 }
 
 // ---------------------------------------------------------------------------
 // Elements of either input type.
 // ---------------------------------------------------------------------------
 
-// Four consecutive values of a row, aligned to four, zero where `in` is false.
-// No branch, so that a thread's loads are all in flight together: a value
-// that is not there is read from `safe` and dropped.
-__device__ __forceinline__ float4 load4(const float* p, const float* safe, bool in) {
-  const float4 f = *reinterpret_cast<const float4*>(in ? p : safe);
-  return in ? f : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-}
-__device__ __forceinline__ float4 load4(const bf16* p, const bf16* safe, bool in) {
-  const uint2 u = *reinterpret_cast<const uint2*>(in ? p : safe);
-  return in ? make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                          __uint_as_float(u.y & 0xffff0000u))
-            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-}
+// Four consecutive elements as they lie in memory, and as numbers.
+template <typename T>
+struct Quad;
+template <>
+struct Quad<float> {
+  typedef float4 type;
+  static __device__ __forceinline__ float4 get(const float4& r) { return r; }
+  static __device__ __forceinline__ float4 make(float x, float y, float z, float w) { return make_float4(x, y, z, w); }
+};
+template <>
+struct Quad<bf16> {
+  typedef uint2 type;
+  static __device__ __forceinline__ float4 get(const uint2& r) {
+    return make_float4(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16),
+                       __uint_as_float(r.y & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint2 make(bf16 x, bf16 y, bf16 z, bf16 w) {
+    return make_uint2(__bfloat16_as_ushort(x) | (uint32_t)__bfloat16_as_ushort(y) << 16,
+                      __bfloat16_as_ushort(z) | (uint32_t)__bfloat16_as_ushort(w) << 16);
+  }
+};
 
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(bf16 x) { return __bfloat162float(x); }
-// The same element by element, for rows that are not aligned or not a multiple
-// of four long; `left` elements are there.
+// Four elements one by one, of which `left` are there: the others are read
+// from `safe`, so that there is no branch and all loads are in flight together,
+// and count as zero.
 template <typename T>
 __device__ __forceinline__ float4 load4_any(const T* p, const T* safe, int left) {
   const float x = as_float(*(left > 0 ? p : safe)), y = as_float(*(left > 1 ? p + 1 : safe));

@@ -148,6 +148,8 @@ __device__ __forceinline__ void chunk_gates(const Problem& a, int b, int hv, int
     if (lane >= o) s += y;
   }
   const double end = __shfl_sync(0xffffffffu, s, 31);
+  const float top = warp_largest(fmaxf(fabsf(be[0]), fabsf(be[1])));
+  if (lane == 0) gates[5 * kC + 4] = plane_scale(plane_inv(top)) * 32768.0f;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int i = 2 * lane + e;
@@ -174,7 +176,7 @@ __device__ __forceinline__ float get_max(const float* red) {
 }
 
 template <typename T, int DK>
-__global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_prepare_kernel(const Problem a, const bool fold_beta) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_prepare_kernel(const Problem a) {
   constexpr int NP = Planes<T>::n;
   constexpr int NQ = kC * DK / 4 / kThreads;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -200,51 +202,76 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
   if (threadIdx.x < kC) bad[threadIdx.x] = 0;
   __syncthreads();
   {
-    // a thread's four elements are half a row of a block: item j is elements
-    // [4 j, 4 j + 4) of the tile as it lies in memory
-    float4 kx[NQ], qx[NQ];
-    float mk = 0.0f, mq = 0.0f;
-    const bool whole = vq && vk && a.dk % 4 == 0;
+    // A thread's four elements are half a row of a block: item j is elements
+    // [4 j, 4 j + 4) of the tile as it lies in memory.  They stay as loaded until
+    // all are there: a conversion in between would wait for each.
+    typedef typename Quad<T>::type Raw;
+    Raw kr[NQ], qr[NQ];
     auto place = [&](int x, int& r, int& c) {
       const int j = threadIdx.x + x * kThreads, blk = j >> 4;
       r = (blk / (DK / 8)) * 8 + ((j >> 1) & 7), c = (blk % (DK / 8)) * 8 + (j & 1) * 4;
     };
-    if (whole) {
+    if (vq && vk && a.dk % 4 == 0) {
 #pragma unroll
       for (int x = 0; x < NQ; ++x) {
         int r, c;
         place(x, r, c);
         const bool in = r < rows && c < a.dk;
-        kx[x] = load4(k + r * a.sk[1] + c, k, in);
-        qx[x] = load4(q + r * a.sq[1] + c, q, in);
+        kr[x] = *reinterpret_cast<const Raw*>(in ? k + r * a.sk[1] + c : k);
+        qr[x] = *reinterpret_cast<const Raw*>(in ? q + r * a.sq[1] + c : q);
       }
     } else {
 #pragma unroll
       for (int x = 0; x < NQ; ++x) {
         int r, c;
         place(x, r, c);
-        const int left = r < rows ? a.dk - c : 0;
-        kx[x] = load4_any(k + r * a.sk[1] + c, k, left);
-        qx[x] = load4_any(q + r * a.sq[1] + c, q, left);
+        auto some = [&](const T* p, long stride) {
+          const T* row = p + min(r, rows - 1) * stride;
+          const int last = a.dk - 1;
+          return Quad<T>::make(row[min(c, last)], row[min(c + 1, last)], row[min(c + 2, last)], row[min(c + 3, last)]);
+        };
+        kr[x] = some(k, a.sk[1]);
+        qr[x] = some(q, a.sq[1]);
       }
     }
-#pragma unroll
-    for (int x = 0; x < NQ; ++x) {
+    const bool whole = rows == kC && a.dk == DK;
+    auto value = [&](const Raw& raw, int x) {
+      float4 f = Quad<T>::get(raw);
+      if (whole) return f;
       int r, c;
       place(x, r, c);
-      float m = max_finite(max_finite(0.0f, kx[x].x), kx[x].y);
-      mk = fmaxf(mk, max_finite(max_finite(m, kx[x].z), kx[x].w));
-      m = max_finite(max_finite(0.0f, qx[x].x), qx[x].y);
-      mq = fmaxf(mq, max_finite(max_finite(m, qx[x].z), qx[x].w));
-      // A key that is not finite spoils its own token and the later ones (see
-      // the gates); inside the products it would reach earlier ones too.
-      if (!(fabsf(kx[x].x) + fabsf(kx[x].y) + fabsf(kx[x].z) + fabsf(kx[x].w) <= 3.4028235e38f)) {
-        bool lost = false;
-        float* f = &kx[x].x;
+      const int left = r < rows ? a.dk - c : 0;
+      f.x = left > 0 ? f.x : 0.0f, f.y = left > 1 ? f.y : 0.0f, f.z = left > 2 ? f.z : 0.0f, f.w = left > 3 ? f.w : 0.0f;
+      return f;
+    };
+    float mk = 0.0f, mq = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!finite(f[i])) f[i] = 0.0f, lost = true;
-        if (lost) bad[r] = 1;
+    for (int x = 0; x < NQ; ++x) {
+      const float4 f = value(kr[x], x), g = value(qr[x], x);
+      mk = max_mag(max_mag(max_mag(max_mag(mk, f.x), f.y), f.z), f.w);
+      mq = max_mag(max_mag(max_mag(max_mag(mq, g.x), g.y), g.z), g.w);
+    }
+    // A key that is not finite spoils its own token and the later ones (see the
+    // gates); inside the products it would reach earlier ones too, so there it
+    // counts as zero.
+    const bool lost = !finite(mk);
+    if (lost) {
+      mk = 0.0f;
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) {
+        const float4 f = value(kr[x], x);
+        mk = max_finite(max_finite(max_finite(max_finite(mk, f.x), f.y), f.z), f.w);
+        int r, c;
+        place(x, r, c);
+        if (!(finite(f.x) && finite(f.y) && finite(f.z) && finite(f.w))) bad[r] = 1;
+      }
+    }
+    if (!finite(mq)) {
+      mq = 0.0f;
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) {
+        const float4 f = value(qr[x], x);
+        mq = max_finite(max_finite(max_finite(max_finite(mq, f.x), f.y), f.z), f.w);
       }
     }
     put_max(red, mk);
@@ -260,16 +287,22 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
       const int at = (threadIdx.x + x * kThreads) * 4;
+      float4 f = value(kr[x], x);
+      if (lost) {
+        f.x = finite(f.x) ? f.x : 0.0f, f.y = finite(f.y) ? f.y : 0.0f;
+        f.z = finite(f.z) ? f.z : 0.0f, f.w = finite(f.w) ? f.w : 0.0f;
+      }
       uint32_t w0[NP], w1[NP];
-      split2<NP>(kx[x].x, kx[x].y, ik, w0);
-      split2<NP>(kx[x].z, kx[x].w, ik, w1);
+      split2<NP>(f.x, f.y, ik, w0);
+      split2<NP>(f.z, f.w, ik, w1);
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         *reinterpret_cast<uint2*>(ks + p * kC * DK + at) = make_uint2(w0[p], w1[p]);
         *reinterpret_cast<uint2*>(ko + p * kC * DK + at) = make_uint2(w0[p], w1[p]);
       }
-      split2<NP>(qx[x].x, qx[x].y, iq, w0);
-      split2<NP>(qx[x].z, qx[x].w, iq, w1);
+      f = value(qr[x], x);
+      split2<NP>(f.x, f.y, iq, w0);
+      split2<NP>(f.z, f.w, iq, w1);
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         *reinterpret_cast<uint2*>(qs + p * kC * DK + at) = make_uint2(w0[p], w1[p]);
@@ -284,7 +317,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
   float ak[4][4], aq[4][4];
   zero(ak);
   zero(aq);
-  if (n0 <= m0) {  // the rest is above the diagonal
+  // warp 1's tiles are above the diagonal: it makes the first gates meanwhile
+  if (warp == 1) chunk_gates(a, b, h * a.rep, t0, rows, bad, gates2);
+  if (n0 <= m0) {
     const uint32_t pk = addr_a<DK, false>(ks, m0 / 8, 0), pq = addr_a<DK, false>(qs, m0 / 8, 0);
     const uint32_t pb = addr_b<DK, false>(ks, 0, n0 / 8);
 #pragma unroll
@@ -318,7 +353,6 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
     }
   __syncthreads();
   for (int x = threadIdx.x; x < kC * kLd; x += kThreads) W[x] = 0.0f;  // above its diagonal blocks it stays zero
-  if (warp == 7) chunk_gates(a, b, h * a.rep, t0, rows, bad, gates2);
 
   for (int r = 0; r < a.rep; ++r) {
     const int hv = h * a.rep + r;
@@ -337,8 +371,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
         for (int l = 0; l < 2; ++l) {
           const float d = j + l <= i ? decay_between(gates, i, j + l) : 0.0f;
           nn[l] = j + l < i ? ak[n][2 * e + l] * d : 0.0f;
-          const float p = j + l <= i ? aq[n][2 * e + l] * (d * a.scale) : 0.0f;
-          pv[n][2 * e + l] = fold_beta ? p * gates[2 * kC + j + l] : p;
+          pv[n][2 * e + l] = j + l <= i ? aq[n][2 * e + l] * (d * a.scale) : 0.0f;
           mp = max_finite(mp, pv[n][2 * e + l]);
         }
         *reinterpret_cast<float2*>(N + i * kLd + j) = make_float2(nn[0], nn[1]);
@@ -421,8 +454,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
             make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
     }
     for (int x = threadIdx.x; x < 5 * kC; x += kThreads) a.gates[nv * kGates * kC + x] = gates[x];
-    if (threadIdx.x < 4) {
-      const float v[4] = {plane_scale(iw), plane_scale(ip), red[32], red[33]};
+    if (threadIdx.x < 5) {
+      const float v[5] = {plane_scale(iw), plane_scale(ip), red[32], red[33], gates[5 * kC + 4]};
       a.gates[nv * kGates * kC + 5 * kC + threadIdx.x] = v[threadIdx.x];
     }
     __syncthreads();
@@ -464,7 +497,8 @@ __device__ __forceinline__ void scan_load(unsigned char* stage, const Problem& a
   cp_async_commit();
 }
 
-template <typename T, int DK>
+// PO: planes of the states and errors that are kept.
+template <typename T, int DK, int PO>
 __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a) {
   constexpr int NP = Planes<T>::n, MT = DK / 64;
   using L = ScanSmem<NP, DK>;
@@ -504,8 +538,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
   };
   auto state_out = [&](int chunk) {
     const long nv = nv0 + chunk;
-    put_state<DK>(s, quarter, sp, ssc, chunk < a.nc ? a.states + (nv * groups + group) * 2 * kGroup * DK : nullptr,
-                  kGroup * DK, a.sscale + (nv * groups + group) * 4);
+    put_state<DK, PO>(s, quarter, sp, ssc, chunk < a.nc ? a.states + (nv * groups + group) * PO * kGroup * DK : nullptr,
+                      a.sscale + (nv * groups + group) * 4);
   };
   scan_load<NP, DK>(smem, a, nk0, nv0);
   load_v(0);
@@ -585,14 +619,14 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
       const float inv = plane_inv(warp_max(x, all_finite));
       // a scale below zero marks a quarter that holds something not finite
       if (lane == 0) a.escale[(nv * groups + group) * 4 + quarter] = all_finite ? plane_scale(inv) : -plane_scale(inv);
-      f16* out = a.e + (nv * groups + group) * 2 * kGroup * kC;
+      f16* out = a.e + (nv * groups + group) * PO * kGroup * kC;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           uint32_t w[2];
           split2<2>(x[n][2 * e], x[n][2 * e + 1], inv, w);
-          store_pair<2>(out, kGroup * kC, quarter * 2 + e, n, w);
+          store_pair<2>(out, kGroup * kC, quarter * 2 + e, n, w, PO);
         }
     }
     // S <- e^G S + K^T (e^(G_end - G) U)
@@ -662,8 +696,8 @@ __device__ __forceinline__ void output_load(f16* dst, const Problem& a, long nv,
 #pragma unroll
   for (int g = 0; g < L::cols / kGroup; ++g) {
     if (c0 + g * kGroup >= a.dvp) break;
-    copy_async<L::NP * kGroup * DK * 2, kThreads>(dst + g * L::NP * kGroup * DK, a.states + (first + g) * 2 * kGroup * DK);
-    copy_async<L::NP * kGroup * kC * 2, kThreads>(dst + L::s + g * L::NP * kGroup * kC, a.e + (first + g) * 2 * kGroup * kC);
+    copy_async<L::NP * kGroup * DK * 2, kThreads>(dst + g * L::NP * kGroup * DK, a.states + (first + g) * a.planes * kGroup * DK);
+    copy_async<L::NP * kGroup * kC * 2, kThreads>(dst + L::s + g * L::NP * kGroup * kC, a.e + (first + g) * a.planes * kGroup * kC);
   }
   if (threadIdx.x < 8) {
     const int g = threadIdx.x & 3;
@@ -673,44 +707,35 @@ __device__ __forceinline__ void output_load(f16* dst, const Problem& a, long nv,
   cp_async_commit();
 }
 
-// acc (two groups of 16 columns) += A B over nk <= STEPS steps of 16.  Both
-// groups' scales of a quarter (PER steps) are scale[4 g + quarter]; `group`: bytes
-// from one group's B to the next.
-template <int NP, int STEPS, int PER>
-__device__ __forceinline__ void output_product(float (&acc)[4][4], uint32_t pa, int plane_a, uint32_t pb, int plane_b,
-                                               int group, int nk, const float* scale) {
+// acc (two groups of 16 columns, NP * `tile` elements each) += A B, one step of
+// 16; both groups' scales are scale[0] and scale[4].  A bf16 output adds
+// consecutive steps of one scale up on the tensor core: `begin` and `end` say
+// where such a run does.
+template <int NP, int TILE>
+__device__ __forceinline__ void output_step(float (&acc)[4][4], float (&t)[4][4], const uint32_t (&fa)[NP][4], uint32_t pb,
+                                            const float* scale, bool begin, bool end) {
+  uint32_t fb[NP][4][2];
+  load_b<NP, 4, true>(fb, pb, NP * TILE * 2, TILE * 2);
+  if (NP == 1 && !begin) {
 #pragma unroll
-  for (int k0 = 0; k0 < STEPS; k0 += PER) {
-    if (k0 >= nk) break;
-    float t[4][4];
+    for (int n = 0; n < 4; ++n) mma(t[n], fa[0], fb[0][n][0], fb[0][n][1]);
+  } else {
+    mma_terms<NP, NP, 4>(t, fa, fb);
+  }
+  if (NP == 1 && !end) return;
 #pragma unroll
-    for (int h = 0; h < PER; ++h) {
-      const int kk = k0 + h;
-      uint32_t fa[NP][4], fb[NP][4][2];
+  for (int n = 0; n < 4; ++n) {
+    const float f = scale[(n >> 1) * 4];
 #pragma unroll
-      for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], pa + kk * 256 + p * plane_a);
-      load_b<NP, 4, true>(fb, pb + kk * 512, group, plane_b);
-      if (NP == 1 && h > 0) {
-#pragma unroll
-        for (int n = 0; n < 4; ++n) mma(t[n], fa[0], fb[0][n][0], fb[0][n][1]);
-      } else {
-        mma_terms<NP, NP, 4>(t, fa, fb);
-      }
-      if (NP == 1 && h + 1 < PER) continue;
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const float f = scale[(n >> 1) * 4 + k0 / PER];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[n][e] += f * t[n][e];
-      }
-    }
+    for (int e = 0; e < 4; ++e) acc[n][e] += f * t[n][e];
   }
 }
 
-// An element of P E, for a chunk with an error that is not finite: the zeros
-// of P above its diagonal would spread it to earlier tokens.
+// An element of P U (without the scales of P and B), for a chunk with an error that is not
+// finite: the zeros of P above its diagonal would spread it to earlier tokens.
 template <int NP>
-__device__ __noinline__ float output_element(const f16* pp, const f16* ep, int plane, const float* scale, int i, int c) {
+__device__ __noinline__ float output_element(const f16* pp, const f16* ep, int plane, const float* scale,
+                                             int i, int c) {
   float sum = 0.0f;
   for (int j = 0; j <= i; ++j) {
     const int ip = ((i >> 3) * 8 + (j >> 3)) * 64 + (i & 7) * 8 + (j & 7);
@@ -750,6 +775,38 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a)
   for (int c0 = 0, buf = 0; c0 < a.dvp; c0 += L::cols) {
     cp_async_wait<0>();
     __syncthreads();
+    if (c0 == 0) {
+      // P -> P B in place, eight columns at a time
+      const float ib = 1.0f / gate[5 * kC + 4];  // a power of two
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = threadIdx.x + i * kThreads;  // of 8 elements
+        const float* be = gate + 2 * kC + ((row >> 3) & 7) * 8;
+        uint32_t r[NP][4];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          const uint4 u = reinterpret_cast<const uint4*>(pp + p * kTile)[row];
+          r[p][0] = u.x, r[p][1] = u.y, r[p][2] = u.z, r[p][3] = u.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r[0][j]));
+          if (NP == 2) {
+            const float2 l = __half22float2(*reinterpret_cast<const __half2*>(&r[NP - 1][j]));
+            f.x += l.x;
+            f.y += l.y;
+          }
+          uint32_t w[NP];
+          split2<NP>(f.x * be[2 * j], f.y * be[2 * j + 1], ib, w);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) r[p][j] = w[p];
+        }
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          reinterpret_cast<uint4*>(pp + p * kTile)[row] = make_uint4(r[p][0], r[p][1], r[p][2], r[p][3]);
+      }
+      __syncthreads();
+    }
     const f16* sp = slices + buf * L::slice;
     const f16* ep = sp + L::s;
     if (L::buffers == 2 && c0 + L::cols < a.dvp) {
@@ -765,11 +822,22 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a)
       float x[4][4], y[4][4];
       zero(x);
       zero(y);
-      output_product<NP, DK / 16, DK / 64>(x, addr_a<DK, false>(qp, m0 / 8, 0), kC * DK * 2,
-                                           addr_b<kGroup, true>(sg, 0, 0), kGroup * DK * 2, NP * kGroup * DK * 2, DK / 16, fs);
+      {
+        const uint32_t pa = addr_a<DK, false>(qp, m0 / 8, 0), pb = addr_b<kGroup, true>(sg, 0, 0);
+        constexpr int per = DK / 64;  // steps to a scale
+        float t[4][4];
+#pragma unroll
+        for (int kk = 0; kk < DK / 16; ++kk) {
+          uint32_t fa[NP][4];
+#pragma unroll
+          for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], pa + kk * 256 + p * kC * DK * 2);
+          output_step<NP, kGroup * DK>(x, t, fa, pb + kk * 512, fs + kk / per, kk % per == 0, kk % per == per - 1);
+        }
+      }
       bool lost = false;
 #pragma unroll
       for (int i = 0; i < 8; ++i) lost |= fe[i] < 0.0f;
+      const float fy = gate[5 * kC + 1] * gate[5 * kC + 4];
       if (lost) {
 #pragma unroll
         for (int n = 0; n < 4; ++n)
@@ -778,10 +846,18 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a)
             y[n][e] = output_element<NP>(pp, eg + (n >> 1) * NP * kGroup * kC, kGroup * kC, fe + (n >> 1) * 4,
                                          frag_row(m0, e >> 1), frag_col((n & 1) * 8) + (e & 1));
       } else {
-        output_product<NP, 4, 1>(y, addr_a<kC, false>(pp, m0 / 8, 0), kTile * 2, addr_b<kGroup, true>(eg, 0, 0),
-                                 kGroup * kC * 2, NP * kGroup * kC * 2, m0 / 16 + 1, fe);
+        const uint32_t pa = addr_a<kC, false>(pp, m0 / 8, 0), pb = addr_b<kGroup, true>(eg, 0, 0);
+        float t[4][4];
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          if (kk > m0 / 16) break;
+          uint32_t fa[NP][4];
+#pragma unroll
+          for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], pa + kk * 256 + p * kTile * 2);
+          output_step<NP, kGroup * kC>(y, t, fa, pb + kk * 512, fe + kk, true, true);
+        }
       }
-      const float fx = a.scale * gate[5 * kC + 3], fy = gate[5 * kC + 1];
+      const float fx = a.scale * gate[5 * kC + 3];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = frag_row(m0, e);
@@ -802,38 +878,33 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a)
   }
 }
 
-template <typename T, int DK>
-int prepare_typed(const Problem& a, bool fold_beta, cudaStream_t stream) {
-  using L = PrepareSmem<T, DK>;
-  if (const int rc = with_smem(delta_prepare_kernel<T, DK>, L::bytes)) return rc;
-  LaunchScope scope(kKindDeltaRule, stream);
-  delta_prepare_kernel<T, DK><<<(unsigned)((long)a.B * a.Hk * a.nc), kThreads, L::bytes, stream>>>(a, fold_beta);
+template <typename T, int DK, int PO>
+int launch_scan(const Problem& a, cudaStream_t stream) {
+  constexpr int bytes = ScanSmem<Planes<T>::n, DK>::bytes;
+  if (const int rc = with_smem(delta_scan_kernel<T, DK, PO>, bytes)) return rc;
+  delta_scan_kernel<T, DK, PO><<<(unsigned)((long)a.B * a.Hv * (a.dvp / kSlice)), kThreads, bytes, stream>>>(a);
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
 }
 
 template <typename T, int DK>
 int forward_typed(const Problem& a, cudaStream_t stream) {
-  if (const int rc = prepare_typed<T, DK>(a, true, stream)) return rc;
-  using S = ScanSmem<Planes<T>::n, DK>;
+  using P = PrepareSmem<T, DK>;
   using O = OutputSmem<T, DK>;
-  if (const int rc = with_smem(delta_scan_kernel<T, DK>, S::bytes)) return rc;
+  if (const int rc = with_smem(delta_prepare_kernel<T, DK>, P::bytes)) return rc;
   if (const int rc = with_smem(delta_output_kernel<T, DK>, O::bytes)) return rc;
-  LaunchScope scope(kKindDeltaRule, stream, 2);
-  delta_scan_kernel<T, DK><<<(unsigned)((long)a.B * a.Hv * (a.dvp / kSlice)), kThreads, S::bytes, stream>>>(a);
+  LaunchScope scope(kKindDeltaRule, stream, 3);
+  delta_prepare_kernel<T, DK><<<(unsigned)((long)a.B * a.Hk * a.nc), kThreads, P::bytes, stream>>>(a);
   GRU_CUDA_TRY(cudaGetLastError());
+  // FP32 inputs keep both planes always, since their outputs read both
+  constexpr int least = Planes<T>::n;
+  if (const int rc = a.planes == 2 ? launch_scan<T, DK, 2>(a, stream) : launch_scan<T, DK, least>(a, stream)) return rc;
   delta_output_kernel<T, DK><<<(unsigned)((long)a.B * a.Hv * a.nc), kThreads, O::bytes, stream>>>(a);
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
 }
 
 }  // namespace
-
-int prepare(const Problem& a, int dtype, bool fold_beta, cudaStream_t stream) {
-  if (dtype == GRU_F32)
-    return a.dk <= 64 ? prepare_typed<float, 64>(a, fold_beta, stream) : prepare_typed<float, 128>(a, fold_beta, stream);
-  return a.dk <= 64 ? prepare_typed<bf16, 64>(a, fold_beta, stream) : prepare_typed<bf16, 128>(a, fold_beta, stream);
-}
 
 int forward(const Problem& a, int dtype, cudaStream_t stream) {
   if (dtype == GRU_F32)

@@ -86,10 +86,11 @@ __device__ __forceinline__ void add_to_state(float (&s)[DK / 64][2][4], const f1
   }
 }
 
-// Planes of this warp's quarter of the state into shared and global memory.
-template <int DK>
+// Planes of this warp's quarter of the state into shared memory, and the first
+// PO of them into `out`, if any.
+template <int DK, int PO>
 __device__ __forceinline__ void put_state(const float (&s)[DK / 64][2][4], int quarter, f16* sp, float* scale, f16* out,
-                                          long plane, float* out_scale) {
+                                          float* out_scale) {
   constexpr int MT = DK / 64;
   float m = 0.0f;
 #pragma unroll
@@ -124,7 +125,7 @@ __device__ __forceinline__ void put_state(const float (&s)[DK / 64][2][4], int q
         split2<2>(s[i][n][2 * e], s[i][n][2 * e + 1], inv, w);
         const int r8 = (quarter * MT + i) * 2 + e;
         store_pair<2>(sp, 2 * kGroup * DK, r8, n, w);
-        if (out) store_pair<2>(out, plane, r8, n, w);
+        if (out) store_pair<2>(out, kGroup * DK, r8, n, w, PO);
       }
 }
 

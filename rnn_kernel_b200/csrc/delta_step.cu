@@ -195,23 +195,25 @@ void fill(Problem& a, const gru_delta_args& p) {
   a.scale = p.scale;
 }
 
-void lay_stash(Problem& a, const gru_delta_args& p, Arena& m) {
-  const size_t n = (size_t)a.B * a.Hv * a.nc, groups = a.dvp / kGroup;
-  a.states = m.take<f16>(n * 2 * a.dvp * key_width(p));
-  a.sscale = m.take<float>(n * groups * 4);
-  a.e = m.take<f16>(n * 2 * a.dvp * kC);
-  a.escale = m.take<float>(n * groups * 4);
-}
-
-void lay_workspace(Problem& a, const gru_delta_args& p, Arena& m, bool backward) {
+// What the forward computes; `keep`: for a gradient.
+void lay_forward(Problem& a, const gru_delta_args& p, Arena& m, bool keep) {
   const size_t nk = (size_t)a.B * a.Hk * a.nc, nv = (size_t)a.B * a.Hv * a.nc, w = key_width(p);
   const size_t np = p.dtype == GRU_F32 ? 2 : 1, groups = a.dvp / kGroup;
+  a.planes = keep || p.dtype == GRU_F32 ? 2 : 1;
   a.kp = m.take<f16>(nk * np * kC * w);
   a.qp = m.take<f16>(nk * np * kC * w);
   a.wp = m.take<f16>(nv * 2 * kTile);
   a.pp = m.take<f16>(nv * 2 * kTile);
   a.gates = m.take<float>(nv * kGates * kC);
-  if (!backward) return;
+  a.states = m.take<f16>(nv * a.planes * a.dvp * w);
+  a.sscale = m.take<float>(nv * groups * 4);
+  a.e = m.take<f16>(nv * a.planes * a.dvp * kC);
+  a.escale = m.take<float>(nv * groups * 4);
+}
+
+void lay_backward(Problem& a, const gru_delta_args& p, Arena& m) {
+  const size_t nk = (size_t)a.B * a.Hk * a.nc, nv = (size_t)a.B * a.Hv * a.nc, w = key_width(p);
+  const size_t np = p.dtype == GRU_F32 ? 2 : 1, groups = a.dvp / kGroup;
   a.z = m.take<f16>(nv * 2 * a.dvp * kC);
   a.zscale = m.take<float>(nv * groups * 4);
   a.dstates = m.take<f16>(nv * 2 * a.dvp * w);
@@ -233,7 +235,7 @@ extern "C" size_t gru_delta_stash_bytes(const gru_delta_args* p) {
   Problem a{};
   fill(a, *p);
   Arena m{nullptr};
-  lay_stash(a, *p, m);
+  lay_forward(a, *p, m, true);
   return m.used;
 }
 
@@ -242,7 +244,8 @@ extern "C" size_t gru_delta_workspace_bytes(const gru_delta_args* p, int backwar
   Problem a{};
   fill(a, *p);
   Arena m{nullptr};
-  lay_workspace(a, *p, m, backward != 0);
+  if (backward) lay_backward(a, *p, m);
+  else lay_forward(a, *p, m, false);
   return m.used;
 }
 
@@ -264,12 +267,10 @@ extern "C" int gru_delta_forward(const gru_delta_args* p, void* out, float* fina
     return GRU_OK;
   }
   if (!out || (reinterpret_cast<uintptr_t>(out) & (p->dtype == GRU_F32 ? 3 : 1))) return bad(me, "null or misaligned out");
-  Arena s{static_cast<char*>(stash)}, w{static_cast<char*>(workspace)};
-  lay_stash(a, *p, s);
-  lay_workspace(a, *p, w, false);
-  if (!stash || stash_bytes < s.used || !workspace || workspace_bytes < w.used ||
-      ((reinterpret_cast<uintptr_t>(stash) | reinterpret_cast<uintptr_t>(workspace)) & 15))
-    return bad(me, "stash or workspace too small or not 16-byte aligned");
+  Arena m{static_cast<char*>(stash ? stash : workspace)};
+  lay_forward(a, *p, m, stash != nullptr);
+  if (!m.base || (stash ? stash_bytes : workspace_bytes) < m.used || (reinterpret_cast<uintptr_t>(m.base) & 15))
+    return bad(me, "stash (or workspace without one) too small or not 16-byte aligned");
   a.o = out;
   a.s_out = final_state;
   return forward(a, p->dtype, stream);
@@ -300,8 +301,8 @@ extern "C" int gru_delta_backward(const gru_delta_args* p, const void* dout, con
         reinterpret_cast<uintptr_t>(dfinal)) & 3))
     return bad(me, "null gradient, or one not aligned to two of its elements");
   Arena s{static_cast<char*>(const_cast<void*>(stash))}, w{static_cast<char*>(workspace)};
-  lay_stash(a, *p, s);
-  lay_workspace(a, *p, w, true);
+  lay_forward(a, *p, s, true);
+  lay_backward(a, *p, w);
   if (!stash || stash_bytes < s.used || !workspace || workspace_bytes < w.used ||
       ((reinterpret_cast<uintptr_t>(stash) | reinterpret_cast<uintptr_t>(workspace)) & 15))
     return bad(me, "stash or workspace too small or not 16-byte aligned");

@@ -95,8 +95,8 @@ def _sizes(code, B, T, Hk, Hv, dk, dv):
     return lib.gru_delta_stash_bytes(a), lib.gru_delta_workspace_bytes(a, 0), lib.gru_delta_workspace_bytes(a, 1)
 
 
-def _forward(code, q, k, v, g, beta, state, scale):
-    """out, the last state and what the gradient needs besides the inputs."""
+def _forward(code, q, k, v, g, beta, state, scale, train):
+    """out, the last state and, to train, what the gradient needs besides the inputs."""
     q, k, v = _dense_heads(q), _dense_heads(k), _dense_heads(v)
     state = None if state is None else state.contiguous()
     B, T, Hk, dk = q.shape
@@ -106,11 +106,11 @@ def _forward(code, q, k, v, g, beta, state, scale):
     with _lib.on_device(dev):
         out = v.new_empty((B, T, Hv, dv))
         last = g.new_empty((B, Hv, dk, dv))
-        stash, ws = g.new_empty(stash_bytes // 4), g.new_empty(ws_bytes // 4)
-        _lib.check(_lib.load().gru_delta_forward(
-            _args(code, q, k, v, g, beta, state, scale), out.data_ptr(), last.data_ptr(), stash.data_ptr(), stash_bytes,
-            ws.data_ptr(), ws_bytes, _lib.raw_stream(dev)), "gru_delta_forward")
-    return out, last, stash, (q, k, v)
+        memory = g.new_empty((stash_bytes if train else ws_bytes) // 4)
+        where = (memory.data_ptr(), stash_bytes, 0, 0) if train else (0, 0, memory.data_ptr(), ws_bytes)
+        _lib.check(_lib.load().gru_delta_forward(_args(code, q, k, v, g, beta, state, scale), out.data_ptr(), last.data_ptr(),
+                                                 *where, _lib.raw_stream(dev)), "gru_delta_forward")
+    return out, last, memory, (q, k, v)
 
 
 class GatedDeltaRuleFunction(torch.autograd.Function):
@@ -119,7 +119,7 @@ class GatedDeltaRuleFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, state, scale):
         code = _check("gated_delta_rule", q, k, v, g, beta, state, 2)
-        out, last, stash, (qd, kd, vd) = _forward(code, q, k, v, g, beta, state, scale)
+        out, last, stash, (qd, kd, vd) = _forward(code, q, k, v, g, beta, state, scale, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(qd, kd, vd, g, beta, stash)
         ctx.code, ctx.scale, ctx.has_state = code, scale, state is not None
@@ -160,7 +160,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     if torch.is_grad_enabled():
         return GatedDeltaRuleFunction.apply(q, k, v, g, beta, initial_state, scale)
     code = _check("gated_delta_rule", q, k, v, g, beta, initial_state, 2)
-    out, last, _, _ = _forward(code, q, k, v, g, beta, initial_state, scale)
+    out, last, _, _ = _forward(code, q, k, v, g, beta, initial_state, scale, False)
     return out, last
 
 
