@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
   T* dv = static_cast<T*>(a.dv_) + at;
   const int cols = a.dv - c0;
   const bool vec = pairs_ok<T>(a.dout, 0, 0, 0, a.dv);
-  Columns<T> od;
+  Columns<T, 2> od;
   auto load_dout = [&](int chunk) {
     const int t = chunk * kC + quarter * 16;
     od.start(dout + (dout ? t * stride : 0), stride, dout ? a.T - t : 0, cols, vec);

@@ -368,7 +368,7 @@ __device__ __forceinline__ void set2<bf16>(bf16* p, int left, bool vec, float a,
   }
 }
 
-// A warp's 16 tokens x 16 value columns of a [token][column] tensor, as
+// A warp's 16 tokens x 8 or 16 value columns of a [token][column] tensor, as
 // accumulator tiles.  `start` issues the loads and `get` gives a value pair,
 // zero where the tensor has none: nothing between the two waits for memory.
 template <typename T>
@@ -389,27 +389,39 @@ struct PairOf<bf16> {
     return make_float2(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
   }
 };
-template <typename T>
+// NT column tiles of 8.
+template <typename T, int NT>
 struct Columns {
-  typename PairOf<T>::type raw[2][2];
+  typename PairOf<T>::type raw[NT][2];
   int tokens, cols;  // that there are from the tile's first on
+  bool whole;        // all of the tile is there, the same for the warp
   // vec: columns and strides are even and p is aligned to two elements
   __device__ __forceinline__ void start(const T* p, long stride, int tokens_, int cols_, bool vec) {
     tokens = tokens_;
     cols = cols_;
+    whole = tokens >= 16 && cols >= NT * 8;
+    if (whole && vec) {
+      const T* q = p + frag_row(0, 0) * stride + frag_col(0);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          raw[n][e] = *reinterpret_cast<const typename PairOf<T>::type*>(q + e * 8 * stride + n * 8);
+      return;
+    }
     if (tokens <= 0 || cols <= 0) return;
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int c = frag_col(n * 8);
         const T* q = p + min(frag_row(0, e), tokens - 1) * stride;
-        if (vec) raw[n][e] = *reinterpret_cast<const typename PairOf<T>::type*>(q + (c < cols ? c : 0));
-        else raw[n][e] = PairOf<T>::make(q[min(c, cols - 1)], q[min(c + 1, cols - 1)]);
+        raw[n][e] = PairOf<T>::make(q[min(c, cols - 1)], q[min(c + 1, cols - 1)]);
       }
   }
   __device__ __forceinline__ float2 get(int n, int e) const {
     float2 f = PairOf<T>::get(raw[n][e]);
+    if (whole) return f;
     const int c = frag_col(n * 8);
     const bool in = frag_row(0, e) < tokens;
     f.x = in && c < cols ? f.x : 0.0f;

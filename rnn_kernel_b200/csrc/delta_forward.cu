@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
       }
   const T* v = static_cast<const T*>(a.v) + b * a.sv[0] + hv * a.sv[2] + c0;
   const bool vec = pairs_ok<T>(a.v, a.sv[0], a.sv[1], a.sv[2], a.dv);
-  Columns<T> vt;
+  Columns<T, 2> vt;
   auto load_v = [&](int chunk) {
     const int t = chunk * kC + quarter * 16;
     vt.start(v + t * a.sv[1], a.sv[1], a.T - t, a.dv - c0, vec);
