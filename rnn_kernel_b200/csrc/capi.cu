@@ -16,6 +16,34 @@
 namespace gru {
 
 namespace {
+thread_local std::map<int, Side> t_side;
+}
+
+int side_stream(int device, cudaStream_t main, Side** out) {
+  *out = nullptr;
+  auto it = t_side.find(device);
+  if (it != t_side.end()) {
+    *out = &it->second;
+    return GRU_OK;
+  }
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  GRU_CUDA_TRY(cudaStreamIsCapturing(main, &cs));
+  if (cs != cudaStreamCaptureStatusNone) return GRU_OK;
+  Side sd;
+  GRU_CUDA_TRY(cudaStreamCreateWithFlags(&sd.s, cudaStreamNonBlocking));
+  GRU_CUDA_TRY(cudaEventCreateWithFlags(&sd.fork, cudaEventDisableTiming));
+  GRU_CUDA_TRY(cudaEventCreateWithFlags(&sd.join, cudaEventDisableTiming));
+  *out = &(t_side[device] = sd);
+  return GRU_OK;
+}
+// `to` waits for everything issued so far on `from`.
+int stream_after(cudaStream_t to, cudaStream_t from, cudaEvent_t ev) {
+  GRU_CUDA_TRY(cudaEventRecord(ev, from));
+  GRU_CUDA_TRY(cudaStreamWaitEvent(to, ev, 0));
+  return GRU_OK;
+}
+
+namespace {
 thread_local std::string g_last_error;
 std::mutex g_mu;
 std::map<std::tuple<int, int, int, int, int>, RecGeom> g_geom;  // (device, kind, B, H, small-loops mode)
@@ -60,40 +88,6 @@ int time_chunks(const RecGeom& g, int device, double side_flops) {
   const double loop_half = 0.5 * g.T * (g.bcp / g.R) * kStepSecondsPerSubchunk;
   const double gain = on_all - std::max(0.0, on_free - loop_half) - kBoundarySeconds;
   return gain > 0.0 ? 2 : 1;
-}
-
-// One non-blocking side stream per host thread and device (default, i.e.
-// lowest, priority) with a fork and a join event.  Created outside stream
-// capture only: while the caller's stream is capturing and no side stream
-// exists yet, the call runs without time chunks.
-struct Side {
-  cudaStream_t s = nullptr;
-  cudaEvent_t fork = nullptr, join = nullptr;
-};
-thread_local std::map<int, Side> t_side;
-
-int side_stream(int device, cudaStream_t main, Side** out) {
-  *out = nullptr;
-  auto it = t_side.find(device);
-  if (it != t_side.end()) {
-    *out = &it->second;
-    return GRU_OK;
-  }
-  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-  GRU_CUDA_TRY(cudaStreamIsCapturing(main, &cs));
-  if (cs != cudaStreamCaptureStatusNone) return GRU_OK;
-  Side sd;
-  GRU_CUDA_TRY(cudaStreamCreateWithFlags(&sd.s, cudaStreamNonBlocking));
-  GRU_CUDA_TRY(cudaEventCreateWithFlags(&sd.fork, cudaEventDisableTiming));
-  GRU_CUDA_TRY(cudaEventCreateWithFlags(&sd.join, cudaEventDisableTiming));
-  *out = &(t_side[device] = sd);
-  return GRU_OK;
-}
-// `to` waits for everything issued so far on `from`.
-int stream_after(cudaStream_t to, cudaStream_t from, cudaEvent_t ev) {
-  GRU_CUDA_TRY(cudaEventRecord(ev, from));
-  GRU_CUDA_TRY(cudaStreamWaitEvent(to, ev, 0));
-  return GRU_OK;
 }
 
 int geometry(int kind, int B, int T, int H, int device, RecGeom* out) {

@@ -159,6 +159,18 @@ int bias_grads_finish(const double* part, int nparts, int H, float* db_ih, float
 
 int sm_count(int device);
 
+// One non-blocking side stream per host thread and device (default, i.e.
+// lowest, priority) with a fork and a join event.  Created outside stream
+// capture only: while the caller's stream is capturing and no side stream
+// exists yet, *out is null and the call runs without it.
+struct Side {
+  cudaStream_t s = nullptr;
+  cudaEvent_t fork = nullptr, join = nullptr;
+};
+int side_stream(int device, cudaStream_t main, Side** out);
+// `to` waits for everything issued so far on `from`.
+int stream_after(cudaStream_t to, cudaStream_t from, cudaEvent_t ev);
+
 // gru_forward's body; overlap = false keeps the whole forward on `stream`
 // (no time chunks, no side stream), as the allocation-free entry point needs.
 int forward_impl(const float* x, const float* h0, const float* w_ih, const float* w_hh, const float* b_ih,

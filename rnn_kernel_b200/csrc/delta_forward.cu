@@ -25,6 +25,11 @@ namespace gru {
 namespace delta {
 namespace {
 
+// The chunks of every sequence that a launch works on.
+struct Range {
+  int first, n;
+};
+
 // ---------------------------------------------------------------------------
 // prepare: one CTA per (batch, key head, chunk), over the head's value heads.
 // Latency-bound (a chain of small products between barriers), so it keeps its
@@ -176,7 +181,7 @@ __device__ __forceinline__ float get_max(const float* red) {
 }
 
 template <typename T, int DK>
-__global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_prepare_kernel(const Problem a) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_prepare_kernel(const Problem a, const Range range) {
   constexpr int NP = Planes<T>::n;
   constexpr int NQ = kC * DK / 4 / kThreads;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -190,8 +195,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
   int* bad = reinterpret_cast<int*>(gates2 + 2 * kGates * kC);  // tokens whose key is not finite
   float* red = reinterpret_cast<float*>(bad + kC);         // [4][8] and scales
 
-  const int chunk = blockIdx.x % a.nc, bh = blockIdx.x / a.nc;
+  const int chunk = range.first + blockIdx.x % range.n, bh = blockIdx.x / range.n;
   const int h = bh % a.Hk, b = bh / a.Hk;
+  const long nk = (long)bh * a.nc + chunk;
   const int t0 = chunk * kC, rows = min(kC, a.T - t0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T* q = static_cast<const T*>(a.q) + b * a.sq[0] + t0 * a.sq[1] + h * a.sq[2];
@@ -282,8 +288,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
       red[32] = plane_scale(ik);
       red[33] = plane_scale(iq);
     }
-    f16* ko = a.kp + (long)blockIdx.x * NP * kC * DK;
-    f16* qo = a.qp + (long)blockIdx.x * NP * kC * DK;
+    f16* ko = a.kp + nk * NP * kC * DK;
+    f16* qo = a.qp + nk * NP * kC * DK;
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
       const int at = (threadIdx.x + x * kThreads) * 4;
@@ -499,7 +505,7 @@ __device__ __forceinline__ void scan_load(unsigned char* stage, const Problem& a
 
 // PO: planes of the states and errors that are kept.
 template <typename T, int DK, int PO>
-__global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a) {
+__global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a, const Range range) {
   constexpr int NP = Planes<T>::n, MT = DK / 64;
   using L = ScanSmem<NP, DK>;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -519,7 +525,9 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
   int* first = reinterpret_cast<int*>(scales + 24);  // of each column, the first token that is not finite
 
   float s[MT][2][4];
-  const float* s0 = a.s0 ? a.s0 + (long)bh * a.dk * a.dv : nullptr;
+  // a later range goes on from what the one before it left
+  const float* from = range.first ? a.s_out : a.s0;
+  const float* s0 = from ? from + (long)bh * a.dk * a.dv : nullptr;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -538,21 +546,22 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
   };
   auto state_out = [&](int chunk) {
     const long nv = nv0 + chunk;
-    put_state<DK, PO>(s, quarter, sp, ssc, chunk < a.nc ? a.states + (nv * groups + group) * PO * kGroup * DK : nullptr,
+    put_state<DK, PO>(s, quarter, sp, ssc, chunk < range.first + range.n ? a.states + (nv * groups + group) * PO * kGroup * DK : nullptr,
                       a.sscale + (nv * groups + group) * 4);
   };
-  scan_load<NP, DK>(smem, a, nk0, nv0);
-  load_v(0);
+  const int end = range.first + range.n;
+  scan_load<NP, DK>(smem + (range.first & 1) * L::stage, a, nk0 + range.first, nv0 + range.first);
+  load_v(range.first);
   if (threadIdx.x < kSlice) first[threadIdx.x] = kC;
-  state_out(0);
-  for (int chunk = 0; chunk < a.nc; ++chunk) {
+  state_out(range.first);
+  for (int chunk = range.first; chunk < end; ++chunk) {
     const f16* kp = reinterpret_cast<const f16*>(smem + (chunk & 1) * L::stage);
     const f16* wp = kp + L::k;
     const float* gate = reinterpret_cast<const float*>(wp + L::w);
     const long nv = nv0 + chunk;
     cp_async_wait<0>();
     __syncthreads();
-    if (chunk + 1 < a.nc) scan_load<NP, DK>(smem + ((chunk + 1) & 1) * L::stage, a, nk0 + chunk + 1, nv + 1);
+    if (chunk + 1 < end) scan_load<NP, DK>(smem + ((chunk + 1) & 1) * L::stage, a, nk0 + chunk + 1, nv + 1);
     const float sw = gate[5 * kC], sk = gate[5 * kC + 2];
     const int row[2] = {frag_row(quarter * 16, 0), frag_row(quarter * 16, 1)};  // this lane's tokens
 
@@ -573,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
           y[n][2 * e] = be * x[n][2 * e];
           y[n][2 * e + 1] = be * x[n][2 * e + 1];
         }
-      if (chunk + 1 < a.nc) load_v(chunk + 1);
+      if (chunk + 1 < end) load_v(chunk + 1);
       bool all_finite;
       const float inv = plane_inv(warp_max(y, all_finite));
       if (lane == 0) xsc[quarter] = plane_scale(inv);
@@ -751,7 +760,7 @@ __device__ __noinline__ float output_element(const f16* pp, const f16* ep, int p
 }
 
 template <typename T, int DK>
-__global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a) {
+__global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a, const Range range) {
   constexpr int NP = Planes<T>::n;
   using L = OutputSmem<T, DK>;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -760,9 +769,9 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a)
   f16* slices = pp + L::p;
   float* gate = reinterpret_cast<float*>(slices + L::buffers * L::slice);
 
-  const int chunk = blockIdx.x % a.nc, bh = blockIdx.x / a.nc;
+  const int chunk = range.first + blockIdx.x % range.n, bh = blockIdx.x / range.n;
   const int hv = bh % a.Hv, b = bh / a.Hv;
-  const long nv = blockIdx.x, nk = ((long)b * a.Hk + hv / a.rep) * a.nc + chunk;
+  const long nv = (long)bh * a.nc + chunk, nk = ((long)b * a.Hk + hv / a.rep) * a.nc + chunk;
   copy_async<L::q * 2, kThreads>(qp, a.qp + nk * L::q);
   copy_async<L::p * 2, kThreads>(pp, a.pp + nv * 2 * kTile);
   copy_async<kGates * kC * 4, kThreads>(gate, a.gates + nv * kGates * kC);
@@ -878,30 +887,69 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a)
   }
 }
 
+template <typename T, int DK>
+int run_prepare(const Problem& a, Range r, cudaStream_t stream) {
+  constexpr int bytes = PrepareSmem<T, DK>::bytes;
+  if (const int rc = with_smem(delta_prepare_kernel<T, DK>, bytes)) return rc;
+  LaunchScope scope(kKindDeltaRule, stream);
+  delta_prepare_kernel<T, DK><<<(unsigned)((long)a.B * a.Hk * r.n), kThreads, bytes, stream>>>(a, r);
+  GRU_CUDA_TRY(cudaGetLastError());
+  return GRU_OK;
+}
 template <typename T, int DK, int PO>
-int launch_scan(const Problem& a, cudaStream_t stream) {
+int run_scan(const Problem& a, Range r, cudaStream_t stream) {
   constexpr int bytes = ScanSmem<Planes<T>::n, DK>::bytes;
   if (const int rc = with_smem(delta_scan_kernel<T, DK, PO>, bytes)) return rc;
-  delta_scan_kernel<T, DK, PO><<<(unsigned)((long)a.B * a.Hv * (a.dvp / kSlice)), kThreads, bytes, stream>>>(a);
+  LaunchScope scope(kKindDeltaRule, stream);
+  delta_scan_kernel<T, DK, PO><<<(unsigned)((long)a.B * a.Hv * (a.dvp / kSlice)), kThreads, bytes, stream>>>(a, r);
+  GRU_CUDA_TRY(cudaGetLastError());
+  return GRU_OK;
+}
+template <typename T, int DK>
+int run_output(const Problem& a, Range r, cudaStream_t stream) {
+  constexpr int bytes = OutputSmem<T, DK>::bytes;
+  if (const int rc = with_smem(delta_output_kernel<T, DK>, bytes)) return rc;
+  LaunchScope scope(kKindDeltaRule, stream);
+  delta_output_kernel<T, DK><<<(unsigned)((long)a.B * a.Hv * r.n), kThreads, bytes, stream>>>(a, r);
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
 }
 
+// A scan of few CTAs leaves most of every SM idle, so a long sequence is cut
+// into ranges of chunks: while one is scanned, the next is prepared and the one
+// before it gets its outputs on a side stream, joined before the call returns.
+// Worth its launches where those two take long themselves, from 2048 chunks of
+// heads on (about 0.1 ms of them at 128 x 128).
+constexpr int kRanges = 4;
 template <typename T, int DK>
 int forward_typed(const Problem& a, cudaStream_t stream) {
-  using P = PrepareSmem<T, DK>;
-  using O = OutputSmem<T, DK>;
-  if (const int rc = with_smem(delta_prepare_kernel<T, DK>, P::bytes)) return rc;
-  if (const int rc = with_smem(delta_output_kernel<T, DK>, O::bytes)) return rc;
-  LaunchScope scope(kKindDeltaRule, stream, 3);
-  delta_prepare_kernel<T, DK><<<(unsigned)((long)a.B * a.Hk * a.nc), kThreads, P::bytes, stream>>>(a);
-  GRU_CUDA_TRY(cudaGetLastError());
-  // FP32 inputs keep both planes always, since their outputs read both
-  constexpr int least = Planes<T>::n;
-  if (const int rc = a.planes == 2 ? launch_scan<T, DK, 2>(a, stream) : launch_scan<T, DK, least>(a, stream)) return rc;
-  delta_output_kernel<T, DK><<<(unsigned)((long)a.B * a.Hv * a.nc), kThreads, O::bytes, stream>>>(a);
-  GRU_CUDA_TRY(cudaGetLastError());
-  return GRU_OK;
+  constexpr int least = Planes<T>::n;  // FP32 outputs read both planes
+  auto scan = [&](Range r) {
+    return a.planes == 2 ? run_scan<T, DK, 2>(a, r, stream) : run_scan<T, DK, least>(a, r, stream);
+  };
+  int rc, device;
+  Side* side = nullptr;
+  if ((long)a.B * a.Hv * (a.dvp / kSlice) <= 148 && (long)a.B * a.Hv * a.nc >= 2048 && a.nc >= 4 * kRanges) {
+    GRU_CUDA_TRY(cudaGetDevice(&device));
+    if ((rc = side_stream(device, stream, &side))) return rc;
+  }
+  const int step = side ? (a.nc + kRanges - 1) / kRanges : a.nc;
+  Range r{0, step}, before{0, 0};
+  if ((rc = run_prepare<T, DK>(a, r, stream))) return rc;
+  if (side && (rc = stream_after(side->s, stream, side->fork))) return rc;
+  if ((rc = scan(r))) return rc;
+  for (before = r; before.first + before.n < a.nc; before = r) {
+    r.first += r.n;
+    r.n = step < a.nc - r.first ? step : a.nc - r.first;
+    if ((rc = run_prepare<T, DK>(a, r, side->s))) return rc;
+    GRU_CUDA_TRY(cudaEventRecord(side->fork, stream));  // the scan of the range before
+    if ((rc = stream_after(stream, side->s, side->join))) return rc;
+    if ((rc = scan(r))) return rc;
+    GRU_CUDA_TRY(cudaStreamWaitEvent(side->s, side->fork, 0));
+    if ((rc = run_output<T, DK>(a, before, side->s))) return rc;
+  }
+  if ((rc = run_output<T, DK>(a, r, stream))) return rc;
+  return side ? stream_after(stream, side->s, side->join) : GRU_OK;
 }
 
 }  // namespace

@@ -215,6 +215,40 @@ def test_nan_stays_with_its_head():
     assert torch.isnan(out[1, 50:, 3, 7]).all() and torch.isnan(last[1, 3, :, 7]).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("what", ["q", "k", "v", "g", "beta", "state"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_is_not_finite_reaches_no_earlier_token(dtype, what, bad):
+    """A token's output does not depend on later tokens, not even on a NaN in them (an infinite g aside, which is none)."""
+    x = list(R.inputs(1, 140, 1, 2, 48, 32, dtype=dtype, seed=15))
+    i, t = NAMES.index(what), 75
+    clean, _ = gated_delta_rule(*x[:5], initial_state=x[5])
+    x[i] = x[i].clone()
+    if what == "state":
+        x[i][0, 1, 3, 5] = bad
+    elif what in ("g", "beta"):
+        x[i][0, t, 1] = bad
+    else:
+        x[i][0, t, -1, 5] = bad
+    out, last = gated_delta_rule(*x[:5], initial_state=x[5])
+    if what == "state":
+        assert torch.isnan(out[0, :, 1, 5]).all()
+        # the column of the state that is not finite, and no other
+        rest = [c for c in range(32) if c != 5]
+        assert rel(out[..., 1, rest], clean[..., 1, rest]) <= TOL[dtype]
+        assert torch.equal(out[:, :, 0], clean[:, :, 0])
+        return
+    heads = slice(0, 2) if what in ("q", "k") else slice(1, 2)  # of one key head, both value heads
+    assert rel(out[:, :t, heads], clean[:, :t, heads]) <= TOL[dtype] and torch.isfinite(out[:, :t]).all()
+    assert not torch.isfinite(out[0, t, 1]).all()
+    if what == "q":
+        assert rel(out[:, t + 1:], clean[:, t + 1:]) <= TOL[dtype]
+    else:
+        assert not torch.isfinite(last[0, 1]).all()
+    if what not in ("q", "k"):
+        assert torch.equal(out[:, :, 0], clean[:, :, 0])
+
+
 def test_repeats_bit_for_bit_and_on_another_stream():
     x = R.inputs(3, 190, 2, 6, 128, 64, dtype=torch.bfloat16, seed=13)
 
@@ -264,6 +298,33 @@ def test_steps_continue_a_prompt():
         o = gated_delta_step(*(y[:, t] for y in x[:5]), state)
         assert rel(o, out[:, t]) <= 2e-6
     assert rel(state, last) <= 2e-6
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_sequence_in_ranges(dtype):
+    """Many chunks of many heads are worked on in overlapped ranges; pieces of the same sequence, one after the other,
+    give the same bits."""
+    x = R.inputs(1, 4101, 4, 32, 32, 32, dtype=dtype, seed=14)
+    with torch.no_grad():
+        out, last = gated_delta_rule(*x[:5], initial_state=x[5])
+        state, parts = x[5], []
+        for a in range(0, 4101, 1024):
+            o, state = gated_delta_rule(*(t[:, a:a + 1024] for t in x[:5]), initial_state=state)
+            parts.append(o)
+        assert torch.equal(torch.cat(parts, 1), out) and torch.equal(state, last)
+        out_r, last_r = R.rule(*x)
+    close(out, out_r, dtype)
+    close(last, last_r, torch.float32)
+    mine = with_grad(x)
+    out_t, last_t = gated_delta_rule(*mine[:5], initial_state=mine[5])
+    assert torch.equal(last_t, last)
+    close(out_t.detach(), out_r, dtype)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph), torch.no_grad():
+        out_g, last_g = gated_delta_rule(*x[:5], initial_state=x[5])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out_g, out) and torch.equal(last_g, last)
 
 
 def test_refusals():
