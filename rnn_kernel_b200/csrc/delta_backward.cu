@@ -246,7 +246,12 @@ struct GradSmem {
   static constexpr int stage = planes + 5 * 16;
   static constexpr int tiles = 4 * kTile * 2 + kC * (kC + 1) * 4;  // bytes: dP', M; y in FP32; over the stages
   static constexpr int main = 2 * stage * 2 > tiles ? 2 * stage * 2 : tiles;
-  static constexpr int bytes = 2 * qk * 2 + (main + 15) / 16 * 16 + kGates * kC * 4 + (9 * kC + 48) * 4;
+  static constexpr int least = 2 * qk * 2 + (main + 15) / 16 * 16 + kGates * kC * 4 + (9 * kC + 48) * 4;
+  // dq and dk of the value heads so far, every thread's own, where that fits
+  // (not for FP32 inputs of 128 key columns: in global memory there)
+  static constexpr int sums = 2 * kC * DK * 4;
+  static constexpr bool sums_fit = least + sums <= 227 * 1024;
+  static constexpr int bytes = least + (sums_fit ? sums : 0);
 };
 
 // Two groups from the g-th on (of all chunks' groups).
@@ -580,9 +585,10 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
         }
       }
     }
-    // dq and dk of a key head are the sums over its value heads
-    float* accq = a.dqk + (long)blockIdx.x * 2 * kC * DK;
-    float* acck = accq + kC * DK;
+    // dq and dk of a key head are the sums over its value heads: a thread's
+    // pair i is sum[i * kGradThreads]
+    float2* sum = reinterpret_cast<float2*>(L::sums_fit ? reinterpret_cast<float*>(smem + L::least)
+                                                        : a.dqk + (long)blockIdx.x * 2 * kC * DK) + threadIdx.x;
     const bool even = a.dk % 2 == 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -591,8 +597,8 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
         const int row = frag_row(m0, e), c = frag_col((col * NT + n) * 8);
         float2 x = make_float2(dq[n][2 * e], dq[n][2 * e + 1]);
         float2 z = make_float2(dkr[n][2 * e] + dkc[n][2 * e], dkr[n][2 * e + 1] + dkc[n][2 * e + 1]);
-        float2* px = reinterpret_cast<float2*>(accq + row * DK + c);
-        float2* pz = reinterpret_cast<float2*>(acck + row * DK + c);
+        float2* px = sum + (n * 4 + e * 2) * kGradThreads;
+        float2* pz = px + kGradThreads;
         if (r > 0) {
           x.x += px->x, x.y += px->y;
           z.x += pz->x, z.y += pz->y;
@@ -622,7 +628,8 @@ int launch_scan(const Problem& a, cudaStream_t stream) {
 template <typename T, int DK>
 int backward_typed(const Problem& a, cudaStream_t stream) {
   using G = GradSmem<Planes<T>::n, DK>;
-  if (const int rc = with_smem(delta_grads_kernel<T, DK>, G::bytes)) return rc;
+  const int grad_bytes = a.rep > 1 ? G::bytes : G::least;  // one value head has nothing to add up
+  if (const int rc = with_smem(delta_grads_kernel<T, DK>, grad_bytes)) return rc;
   LaunchScope scope(kKindDeltaRule, stream, 2);
   // one stage where two CTAs then share an SM and there are that many, or
   // where two stages do not fit (FP32 inputs of 128 key columns)
@@ -635,7 +642,7 @@ int backward_typed(const Problem& a, cudaStream_t stream) {
   } else {
     if (const int rc = launch_scan<T, DK, 1>(a, stream)) return rc;
   }
-  delta_grads_kernel<T, DK><<<(unsigned)((long)a.B * a.Hk * a.nc), kGradThreads, G::bytes, stream>>>(a);
+  delta_grads_kernel<T, DK><<<(unsigned)((long)a.B * a.Hk * a.nc), kGradThreads, grad_bytes, stream>>>(a);
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
 }
