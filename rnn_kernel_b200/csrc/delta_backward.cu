@@ -228,25 +228,26 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
 
 // ---------------------------------------------------------------------------
 // grads: one CTA per (batch, key head, chunk).  It walks the value columns in
-// steps of 16 (one step of the products' inner dimension), the next 32 loading
-// meanwhile; each of 16 warps keeps 16 tokens x a quarter of the key columns of dQ,
-// dK_row and dK_col, and of 16 tokens of dO U^T and Z U^T, in registers.  (Eight
-// warps of twice the tile had one CTA an SM as well, at 255 registers: 373 us for
-// train 4 x 2048 x 16 heads of 128.)
+// steps of 16 (one step of the products' inner dimension), the next stage of one
+// or two steps loading meanwhile.  A warp keeps 16 tokens x 32 key columns of
+// dQ, dK_row and dK_col, and of 16 or 32 tokens of dO U^T and Z U^T, in
+// registers: sixteen warps for 128 key columns, eight for 64, where two CTAs
+// then share an SM.
 // ---------------------------------------------------------------------------
-
-constexpr int kGradThreads = 512;
 
 template <int NP, int DK>
 struct GradSmem {
+  static constexpr int split = DK / 32;           // warps that share 16 tokens' columns
+  static constexpr int threads = 128 * split;
+  static constexpr int steps = split / 2;         // of 16 value columns to a stage
   static constexpr int qk = NP * kC * DK;  // elements
   static constexpr int s = 2 * kGroup * DK, x = 2 * kGroup * kC, o = NP * kGroup * kC;
-  // a stage: S, dS, E, Z, dO of two groups of 16 columns, each [group][plane], and their scales
-  static constexpr int planes = 2 * (2 * s + 2 * x + o);
-  static constexpr int stage = planes + 5 * 16;
+  // a stage: S, dS, E, Z, dO, each [step][plane], and their scales
+  static constexpr int planes = steps * (2 * s + 2 * x + o);
+  static constexpr int stage = planes + 5 * steps * 8;
   static constexpr int tiles = 4 * kTile * 2 + kC * (kC + 1) * 4;  // bytes: dP', M; y in FP32; over the stages
   static constexpr int main = 2 * stage * 2 > tiles ? 2 * stage * 2 : tiles;
-  static constexpr int least = 2 * qk * 2 + (main + 15) / 16 * 16 + kGates * kC * 4 + (9 * kC + 48) * 4;
+  static constexpr int least = 2 * qk * 2 + (main + 15) / 16 * 16 + kGates * kC * 4 + ((2 * split + 1) * kC + 12 * split) * 4;
   // dq and dk of the value heads so far, every thread's own, where that fits
   // (not for FP32 inputs of 128 key columns: in global memory there)
   static constexpr int sums = 2 * kC * DK * 4;
@@ -254,19 +255,20 @@ struct GradSmem {
   static constexpr int bytes = least + (sums_fit ? sums : 0);
 };
 
-// Two groups from the g-th on (of all chunks' groups).
+// A stage from the g-th group on (of all chunks' groups).
 template <int NP, int DK>
 __device__ __forceinline__ void grad_load(f16* dst, const Problem& a, long g) {
   using L = GradSmem<NP, DK>;
-  copy_async<4 * L::s, kGradThreads>(dst, a.states + g * L::s);
-  copy_async<4 * L::s, kGradThreads>(dst + 2 * L::s, a.dstates + g * L::s);
-  copy_async<4 * L::x, kGradThreads>(dst + 4 * L::s, a.e + g * L::x);
-  copy_async<4 * L::x, kGradThreads>(dst + 4 * L::s + 2 * L::x, a.z + g * L::x);
-  copy_async<4 * L::o, kGradThreads>(dst + 4 * L::s + 4 * L::x, a.dop + g * L::o);
-  if (threadIdx.x < 10) {
-    const int t = threadIdx.x >> 1, i = threadIdx.x & 1;
+  constexpr int n = L::steps, threads = L::threads;
+  copy_async<n * L::s * 2, threads>(dst, a.states + g * L::s);
+  copy_async<n * L::s * 2, threads>(dst + n * L::s, a.dstates + g * L::s);
+  copy_async<n * L::x * 2, threads>(dst + 2 * n * L::s, a.e + g * L::x);
+  copy_async<n * L::x * 2, threads>(dst + n * (2 * L::s + L::x), a.z + g * L::x);
+  copy_async<n * L::o * 2, threads>(dst + n * (2 * L::s + 2 * L::x), a.dop + g * L::o);
+  if (threadIdx.x < 5 * n) {
+    const int t = threadIdx.x / n, i = threadIdx.x % n;
     const float* from = t == 0 ? a.sscale : t == 1 ? a.dsscale : t == 2 ? a.escale : t == 3 ? a.zscale : a.doscale;
-    cp_async16(dst + L::planes + (t * 2 + i) * 8, from + (g + i) * 4);
+    cp_async16(dst + L::planes + threadIdx.x * 8, from + (g + i) * 4);
   }
   cp_async_commit();
 }
@@ -288,16 +290,16 @@ __device__ __forceinline__ float2 pair(uint32_t h, uint32_t l) {
   return make_float2(x.x + y.x, x.y + y.y);
 }
 
-// acc += f A B, one step of 16.
+// acc += A B, one step of 16, times f0 (the first half of the tiles) or f1.
 template <int NA, int NB, int NT>
-__device__ __forceinline__ void step_add(float (&acc)[NT][4], float f, const uint32_t (&fa)[NA][4],
+__device__ __forceinline__ void step_add(float (&acc)[NT][4], float f0, float f1, const uint32_t (&fa)[NA][4],
                                          const uint32_t (&fb)[NB][NT][2]) {
   float t[NT][4];
   mma_terms<NA, NB, NT>(t, fa, fb);
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[i][e] += f * t[i][e];
+    for (int e = 0; e < 4; ++e) acc[i][e] += (2 * i < NT ? f0 : f1) * t[i][e];
 }
 
 // acc += f A B over steps [k0, k1) of the tokens: A a 64 x 64 tile (rows m, or
@@ -311,15 +313,18 @@ __device__ __forceinline__ void token_product(float (&acc)[NT][4], float f, cons
 #pragma unroll
     for (int p = 0; p < 2; ++p) ldm4<TA>(fa[p], pa + p * kTile * 2);
     load_b<NP, NT, true>(fb, addr_b<DK, true>(B, 2 * kk, n8), 256, kC * DK * 2);
-    step_add<2, NP, NT>(acc, f, fa, fb);
+    step_add<2, NP, NT>(acc, f, f, fa, fb);
   }
 }
 
 template <typename T, int DK>
-__global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem a) {
+__global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 ? 2 : 1)
+    delta_grads_kernel(const Problem a) {
   constexpr int NP = Planes<T>::n;
-  constexpr int NT = DK / 32;  // a warp's quarter of the key columns, in 8-column tiles
   using L = GradSmem<NP, DK>;
+  constexpr int split = L::split, threads = L::threads;
+  constexpr int NT = 4;          // a warp's 32 key columns, in 8-column tiles
+  constexpr int NC = 8 / split;  // its columns of the 64 x 64 products
   extern __shared__ __align__(16) unsigned char smem[];
   f16* qp = reinterpret_cast<f16*>(smem);
   f16* kp = qp + L::qk;
@@ -328,26 +333,27 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
   f16* mp = dpp + 2 * kTile;
   float* y = reinterpret_cast<float*>(mp + 2 * kTile);  // [64][65]
   float* gate = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(main) + (L::main + 15) / 16 * 16);
-  float* red = gate + kGates * kC;  // x and z of the four column quarters, F; then values per warp
-  float* wred = red + 9 * kC;
+  float* red = gate + kGates * kC;  // x and z of the warps that share tokens, F; then values per warp
+  float* wred = red + (2 * split + 1) * kC;
 
   const int chunk = blockIdx.x % a.nc, bh = blockIdx.x / a.nc;
   const int hk = bh % a.Hk, b = bh / a.Hk;
   const int t0 = chunk * kC, rows = min(kC, a.T - t0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m0 = (warp >> 2) * 16, col = warp & 3;  // this warp's tokens; its quarter of the columns
+  const int m0 = warp / split * 16, col = warp % split;  // this warp's tokens; its part of the columns
+  const bool below = col * NC * 8 <= m0;                 // whether that holds any of the 64 x 64 products' lower half
   const int groups = a.dvp / kGroup;
 
-  copy_async<L::qk * 2, kGradThreads>(qp, a.qp + (long)blockIdx.x * L::qk);
-  copy_async<L::qk * 2, kGradThreads>(kp, a.kp + (long)blockIdx.x * L::qk);
+  copy_async<L::qk * 2, threads>(qp, a.qp + (long)blockIdx.x * L::qk);
+  copy_async<L::qk * 2, threads>(kp, a.kp + (long)blockIdx.x * L::qk);
 
   for (int r = 0; r < a.rep; ++r) {
     const int hv = hk * a.rep + r;
     const long nv = ((long)b * a.Hv + hv) * a.nc + chunk;
     __syncthreads();
-    copy_async<kGates * kC * 4, kGradThreads>(gate, a.gates + nv * kGates * kC);
+    copy_async<kGates * kC * 4, threads>(gate, a.gates + nv * kGates * kC);
     grad_load<NP, DK>(main, a, nv * groups);
-    float dp[2][4], da[2][4], dq[NT][4], dkr[NT][4], dkc[NT][4];
+    float dp[NC][4], da[NC][4], dq[NT][4], dkr[NT][4], dkc[NT][4];
     zero(dp);
     zero(da);
     zero(dq);
@@ -355,21 +361,25 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
     zero(dkc);
     float sdot = 0.0f, bdot[2] = {0.0f, 0.0f};
     for (int g = 0; g < groups; ++g) {
-      const f16* stage = main + ((g >> 1) & 1) * L::stage;
-      if ((g & 1) == 0) {
+      constexpr int n = L::steps;
+      const int i = g % n, at = g / n & 1;
+      const f16* stage = main + at * L::stage;
+      if (i == 0) {
         cp_async_wait<0>();
         __syncthreads();
-        if (g + 2 < groups) grad_load<NP, DK>(main + (((g >> 1) + 1) & 1) * L::stage, a, nv * groups + g + 2);
+        if (g + n < groups) grad_load<NP, DK>(main + (at ^ 1) * L::stage, a, nv * groups + g + n);
       }
-      const f16* sp = stage + (g & 1) * L::s;
-      const f16* dsp = sp + 2 * L::s;
-      const f16* ep = stage + 4 * L::s + (g & 1) * L::x;
-      const f16* zp = ep + 2 * L::x;
-      const f16* op = stage + 4 * L::s + 4 * L::x + (g & 1) * L::o;
+      const f16* sp = stage + i * L::s;
+      const f16* dsp = sp + n * L::s;
+      const f16* ep = stage + 2 * n * L::s + i * L::x;
+      const f16* zp = ep + n * L::x;
+      const f16* op = stage + n * (2 * L::s + 2 * L::x) + i * L::o;
       // scales: of the quarters of the key columns (S, dS) and of the tokens
-      const float* scales = reinterpret_cast<const float*>(stage + L::planes) + (g & 1) * 4;
-      const int mq = m0 / 16;
-      const float se = fabsf(scales[16 + mq]), sz = scales[24 + mq], so = scales[32 + mq];
+      const float* ss = reinterpret_cast<const float*>(stage + L::planes) + i * 4;
+      const float *sds = ss + 4 * n, *se = ss + 8 * n, *sz = ss + 12 * n, *so = ss + 16 * n;
+      const int mq = m0 / 16, kq = col * 4 / split;  // quarters of this warp's tokens and of its first key column
+      constexpr int k2 = split == 4 ? 0 : 1;         // and of its last
+      const float fE = fabsf(se[mq]), fZ = sz[mq], fO = so[mq];
       uint32_t fz[2][4], fe[2][4];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
@@ -378,7 +388,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
       }
       if (col == 0) {
         // Z . E of this lane's two tokens
-        const float f = sz * se;
+        const float f = fZ * fE;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float2 u = pair(fz[0][j], fz[1][j]), w = pair(fe[0][j], fe[1][j]);
@@ -388,7 +398,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
       {
         uint32_t fb[2][NT][2];
         load_b<2, NT, false>(fb, addr_b<kGroup, false>(dsp, 0, col * NT), 512, kGroup * DK * 2);
-        step_add<2, 2, NT>(dkc, se * scales[8 + col], fe, fb);
+        step_add<2, 2, NT>(dkc, fE * sds[kq], fE * sds[kq + k2], fe, fb);
       }
       uint32_t fo[NP][4];
 #pragma unroll
@@ -396,22 +406,22 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
       {
         uint32_t fb[2][NT][2];
         load_b<2, NT, false>(fb, addr_b<kGroup, false>(sp, 0, col * NT), 512, kGroup * DK * 2);
-        step_add<NP, 2, NT>(dq, so * scales[col], fo, fb);
-        step_add<2, 2, NT>(dkr, sz * scales[col], fz, fb);
+        step_add<NP, 2, NT>(dq, fO * ss[kq], fO * ss[kq + k2], fo, fb);
+        step_add<2, 2, NT>(dkr, fZ * ss[kq], fZ * ss[kq + k2], fz, fb);
       }
-      if (col <= mq) {
-        uint32_t fb[2][2][2];
-        load_b<2, 2, false>(fb, addr_b<kGroup, false>(ep, 0, col * 2), 512, kGroup * kC * 2);
-        const float f = fabsf(scales[16 + col]);
-        step_add<NP, 2, 2>(dp, so * f, fo, fb);
-        step_add<2, 2, 2>(da, sz * f, fz, fb);
+      if (below) {
+        uint32_t fb[2][NC][2];
+        load_b<2, NC, false>(fb, addr_b<kGroup, false>(ep, 0, col * NC), 512, kGroup * kC * 2);
+        const float f0 = fabsf(se[kq]), f1 = fabsf(se[kq + k2]);
+        step_add<NP, 2, NC>(dp, fO * f0, fO * f1, fo, fb);
+        step_add<2, 2, NC>(da, fZ * f0, fZ * f1, fz, fb);
       }
 #pragma unroll
-      for (int i = 0; i < kGroup * DK / 2 / kGradThreads; ++i) {
-        // block warp + 16 i is of the rows 8 (warp / 2 + 8 i) ..., in this quarter
-        const int w = threadIdx.x + i * kGradThreads, q = (warp / 2 + 8 * i) * 8 / (DK / 4);
-        const float2 u = take2<2>(sp, kGroup * DK, w), v = take2<2>(dsp, kGroup * DK, w);
-        sdot += (scales[q] * scales[8 + q]) * (u.x * v.x + u.y * v.y);
+      for (int j = 0; j < kGroup * DK / 2 / threads; ++j) {
+        // block warp + 4 split j is of the rows 8 (warp / 2 + 2 split j) ..., in quarter q
+        const int word = threadIdx.x + j * threads, q = (warp / 2 + 2 * split * j) * 8 / (DK / 4);
+        const float2 u = take2<2>(sp, kGroup * DK, word), v = take2<2>(dsp, kGroup * DK, word);
+        sdot += (ss[q] * sds[q]) * (u.x * v.x + u.y * v.y);
       }
     }
     __syncthreads();
@@ -419,27 +429,27 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
     const float sk = gate[5 * kC + 2], sq = gate[5 * kC + 3];
     float mu = 0.0f, mw = 0.0f;
     {
-      float qk[2][4], kk[2][4];
+      float qk[NC][4], kk[NC][4];
       zero(qk);
       zero(kk);
-      if (col <= m0 / 16) {
+      if (below) {
 #pragma unroll
         for (int k = 0; k < DK / 16; ++k) {
-          uint32_t fa[NP][4], fb[NP][2][2];
-          load_b<NP, 2, false>(fb, addr_b<DK, false>(kp, 2 * k, col * 2), 0, kC * DK * 2);
+          uint32_t fa[NP][4], fb[NP][NC][2];
+          load_b<NP, NC, false>(fb, addr_b<DK, false>(kp, 2 * k, col * NC), 32 * DK, kC * DK * 2);
 #pragma unroll
           for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], addr_a<DK, false>(qp, m0 / 8, 2 * k) + p * kC * DK * 2);
-          step_add<NP, NP, 2>(qk, sq * sk, fa, fb);
+          step_add<NP, NP, NC>(qk, sq * sk, sq * sk, fa, fb);
 #pragma unroll
           for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], addr_a<DK, false>(kp, m0 / 8, 2 * k) + p * kC * DK * 2);
-          step_add<NP, NP, 2>(kk, sk * sk, fa, fb);
+          step_add<NP, NP, NC>(kk, sk * sk, sk * sk, fa, fb);
         }
       }
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NC; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int i = frag_row(m0, e), j = frag_col(col * 16 + n * 8);
+          const int i = frag_row(m0, e), j = frag_col((col * NC + n) * 8);
 #pragma unroll
           for (int l = 0; l < 2; ++l) {
             const float dec = j + l <= i ? decay_between(gate, i, j + l) * gate[2 * kC + j + l]
@@ -484,7 +494,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
       const int row = frag_row(m0, e);
       if ((lane & 3) == 0) {
         red[col * kC + row] = xs[e];
-        red[(4 + col) * kC + row] = zs[e];
+        red[(split + col) * kC + row] = zs[e];
         if (col == 0 && row < rows) a.dbeta[((long)b * a.T + t0 + row) * a.Hv + hv] = bdot[e];
       }
     }
@@ -495,22 +505,22 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
     const unsigned wm = __reduce_max_sync(0xffffffffu, __float_as_uint(mw));
     if (lane == 0) {
       wred[warp] = end;
-      wred[16 + warp] = __uint_as_float(um);
-      wred[32 + warp] = __uint_as_float(wm);
+      wred[4 * split + warp] = __uint_as_float(um);
+      wred[8 * split + warp] = __uint_as_float(wm);
     }
     __syncthreads();
-    mu = wred[16], mw = wred[32];
+    mu = wred[4 * split], mw = wred[8 * split];
 #pragma unroll
-    for (int w = 1; w < kGradThreads / 32; ++w) {
-      mu = fmaxf(mu, wred[16 + w]);
-      mw = fmaxf(mw, wred[32 + w]);
+    for (int w = 1; w < 4 * split; ++w) {
+      mu = fmaxf(mu, wred[4 * split + w]);
+      mw = fmaxf(mw, wred[8 * split + w]);
     }
     const float iu = plane_inv(mu), iw = plane_inv(mw);
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < NC; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int word = ((m0 / 8 + e) * (kC / 8) + col * 2 + n) * 32 + lane;
+        const int word = ((m0 / 8 + e) * (kC / 8) + col * NC + n) * 32 + lane;
         uint32_t u[2], w[2];
         split2<2>(dp[n][2 * e], dp[n][2 * e + 1], iu, u);
         split2<2>(da[n][2 * e], da[n][2 * e + 1], iw, w);
@@ -521,22 +531,23 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
         }
       }
     {
-      // y_ij -> sum over the columns before j, eight threads to a row
-      float* part = y + (threadIdx.x >> 3) * (kC + 1) + (threadIdx.x & 7) * 8;
-      float v[8], sum = 0.0f;
+      // y_ij -> sum over the columns before j, `per` threads to a row
+      constexpr int per = threads / kC, n = kC / per;
+      float* part = y + (threadIdx.x / per) * (kC + 1) + (threadIdx.x % per) * n;
+      float v[n], sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < n; ++j) {
         v[j] = part[j];
         sum += v[j];
       }
       float run = 0.0f;  // of the parts before
 #pragma unroll
-      for (int k = 0; k < 7; ++k) {
-        const float f = __shfl_sync(0xffffffffu, sum, k, 8);
-        if ((threadIdx.x & 7) > k) run += f;
+      for (int k = 0; k < per - 1; ++k) {
+        const float f = __shfl_sync(0xffffffffu, sum, k, per);
+        if (threadIdx.x % per > k) run += f;
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < n; ++j) {
         part[j] = run;
         run += v[j];
       }
@@ -548,12 +559,13 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
     token_product<NP, DK, true, NT>(dkc, su * sq, dpp, m0 / 8, qp, col * NT, m0 / 16, kC / 16);
     token_product<NP, DK, true, NT>(dkc, sw * sk, mp, m0 / 8, kp, col * NT, m0 / 16, kC / 16);
     {
-      const int t = threadIdx.x >> 3;
+      constexpr int per = threads / kC;
+      const int t = threadIdx.x / per;
       float f = 0.0f;
-      for (int i = t + (threadIdx.x & 7); i < kC; i += 8) f += y[i * (kC + 1) + t];
+      for (int i = t + threadIdx.x % per; i < kC; i += per) f += y[i * (kC + 1) + t];
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) f += __shfl_xor_sync(0xffffffffu, f, o);
-      if ((threadIdx.x & 7) == 0) red[8 * kC + t] = f;
+      for (int o = 1; o < per; o <<= 1) f += __shfl_xor_sync(0xffffffffu, f, o);
+      if (threadIdx.x % per == 0) red[2 * split * kC + t] = f;
     }
     __syncthreads();
     if (warp == 0) {
@@ -562,8 +574,12 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int i = 2 * lane + e;
-        x[e] = ((double)red[i] + red[kC + i]) + ((double)red[2 * kC + i] + red[3 * kC + i]);
-        z[e] = ((double)red[4 * kC + i] + red[5 * kC + i]) + ((double)red[6 * kC + i] + red[7 * kC + i]);
+        x[e] = z[e] = 0.0;
+#pragma unroll
+        for (int c = 0; c < split; ++c) {
+          x[e] += red[c * kC + i];
+          z[e] += red[(split + c) * kC + i];
+        }
       }
       double sx = x[0] + x[1], sz = z[0] + z[1];
 #pragma unroll
@@ -572,7 +588,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
         if (lane + o < 32) sx += u;
         if (lane >= o) sz += w;
       }
-      for (int w = 0; w < kGradThreads / 32; ++w) last += wred[w];
+      for (int w = 0; w < 4 * split; ++w) last += wred[w];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int i = 2 * lane + e;
@@ -581,12 +597,12 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
           const double from = e ? sx - x[0] : sx, before = e ? sz - z[1] : sz - z[0] - z[1];
           // a decay of zero passes no gradient
           a.dg[((long)b * a.T + t0 + i) * a.Hv + hv] =
-              gv < kNoDecay ? 0.0f : (float)(from + before + red[8 * kC + i] + last);
+              gv < kNoDecay ? 0.0f : (float)(from + before + red[2 * split * kC + i] + last);
         }
       }
     }
     // dq and dk of a key head are the sums over its value heads: a thread's
-    // pair i is sum[i * kGradThreads]
+    // pair i is sum[i * threads]
     float2* sum = reinterpret_cast<float2*>(L::sums_fit ? reinterpret_cast<float*>(smem + L::least)
                                                         : a.dqk + (long)blockIdx.x * 2 * kC * DK) + threadIdx.x;
     const bool even = a.dk % 2 == 0;
@@ -597,8 +613,8 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const Problem
         const int row = frag_row(m0, e), c = frag_col((col * NT + n) * 8);
         float2 x = make_float2(dq[n][2 * e], dq[n][2 * e + 1]);
         float2 z = make_float2(dkr[n][2 * e] + dkc[n][2 * e], dkr[n][2 * e + 1] + dkc[n][2 * e + 1]);
-        float2* px = sum + (n * 4 + e * 2) * kGradThreads;
-        float2* pz = px + kGradThreads;
+        float2* px = sum + (n * 4 + e * 2) * threads;
+        float2* pz = px + threads;
         if (r > 0) {
           x.x += px->x, x.y += px->y;
           z.x += pz->x, z.y += pz->y;
@@ -642,7 +658,7 @@ int backward_typed(const Problem& a, cudaStream_t stream) {
   } else {
     if (const int rc = launch_scan<T, DK, 1>(a, stream)) return rc;
   }
-  delta_grads_kernel<T, DK><<<(unsigned)((long)a.B * a.Hk * a.nc), kGradThreads, grad_bytes, stream>>>(a);
+  delta_grads_kernel<T, DK><<<(unsigned)((long)a.B * a.Hk * a.nc), G::threads, grad_bytes, stream>>>(a);
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
 }
