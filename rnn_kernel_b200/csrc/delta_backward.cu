@@ -232,7 +232,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
 // or two steps loading meanwhile.  A warp keeps 16 tokens x 32 key columns of
 // dQ, dK_row and dK_col, and of 16 or 32 tokens of dO U^T and Z U^T, in
 // registers: sixteen warps for 128 key columns, eight for 64, where two CTAs
-// then share an SM.
+// then share an SM (2048 chunks of heads of 64, FP32: 170 us, against 205 with
+// sixteen warps of half the tile; of 128, bf16: 334 us).
 // ---------------------------------------------------------------------------
 
 template <int NP, int DK>
