@@ -192,7 +192,7 @@ int gru_delta_forward(const gru_delta_args* args, void* out, float* final_state,
 /* Gradients of q, k, v, g, beta (dense, overwritten; dq, dk and dv aligned to
  * two elements) and of the initial state (or NULL), from dout dense
  * [B, T, Hv, dv] and dfinal dense [B, Hv, dk, dv] (either NULL: zeros).  The
- * arguments are the forward's, its inputs unchanged. */
+ * sizes, scale and g are the forward's; its other tensors are not read. */
 int gru_delta_backward(const gru_delta_args* args, const void* dout, const float* dfinal, const void* stash,
                        size_t stash_bytes, void* dq, void* dk, void* dv, float* dg, float* dbeta, float* dinitial,
                        void* workspace, size_t workspace_bytes, void* stream);

@@ -144,8 +144,9 @@ int bad(const char* what, const char* msg, int code = GRU_ERR_INVALID) {
   return code;
 }
 
-// sizes_only: the tensors are not looked at.
-int check_args(const char* what, const gru_delta_args* p, bool sizes_only = false) {
+// Which of the tensors have to be there.
+enum Needs { kSizesOnly, kDecays, kInputs };
+int check_args(const char* what, const gru_delta_args* p, Needs needs) {
   if (!p) return bad(what, "null arguments");
   if (p->dtype != GRU_F32 && p->dtype != GRU_BF16)
     return bad(what, "dtype must be GRU_F32 or GRU_BF16", GRU_ERR_UNSUPPORTED);
@@ -160,7 +161,8 @@ int check_args(const char* what, const gru_delta_args* p, bool sizes_only = fals
         reinterpret_cast<uintptr_t>(p->initial_state)) & 3) != 0)
     return bad(what, "a tensor is not aligned to its element size");
   const bool any = p->B > 0 && p->T > 0;
-  if (!sizes_only && any && (!p->q || !p->k || !p->v || !p->g || !p->beta)) return bad(what, "null tensor");
+  if (any && ((needs != kSizesOnly && !p->g) || (needs == kInputs && (!p->q || !p->k || !p->v || !p->beta))))
+    return bad(what, "null tensor");
   const long nc = ((long)p->T + kC - 1) / kC;
   if ((long)p->B * p->Hv > (1L << 28) || (long)p->B * p->Hv * (nc > 4 ? nc : 4) > 0x7fffffffL)
     return bad(what, "too many chunks for one launch", GRU_ERR_UNSUPPORTED);
@@ -231,7 +233,7 @@ using namespace gru;
 using namespace gru::delta;
 
 extern "C" size_t gru_delta_stash_bytes(const gru_delta_args* p) {
-  if (check_args("gru_delta_stash_bytes", p, true)) return 0;
+  if (check_args("gru_delta_stash_bytes", p, kSizesOnly)) return 0;
   Problem a{};
   fill(a, *p);
   Arena m{nullptr};
@@ -240,7 +242,7 @@ extern "C" size_t gru_delta_stash_bytes(const gru_delta_args* p) {
 }
 
 extern "C" size_t gru_delta_workspace_bytes(const gru_delta_args* p, int backward) {
-  if (check_args("gru_delta_workspace_bytes", p, true)) return 0;
+  if (check_args("gru_delta_workspace_bytes", p, kSizesOnly)) return 0;
   Problem a{};
   fill(a, *p);
   Arena m{nullptr};
@@ -253,7 +255,7 @@ extern "C" int gru_delta_forward(const gru_delta_args* p, void* out, float* fina
                                  size_t stash_bytes, void* workspace, size_t workspace_bytes, void* stream_) {
   clear_error();
   const char* me = "gru_delta_forward";
-  if (const int rc = check_args(me, p)) return rc;
+  if (const int rc = check_args(me, p, kInputs)) return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (p->B == 0) return GRU_OK;
   if (!final_state || (reinterpret_cast<uintptr_t>(final_state) & 3)) return bad(me, "null or misaligned final_state");
@@ -281,7 +283,7 @@ extern "C" int gru_delta_backward(const gru_delta_args* p, const void* dout, con
                                   float* dinitial, void* workspace, size_t workspace_bytes, void* stream_) {
   clear_error();
   const char* me = "gru_delta_backward";
-  if (const int rc = check_args(me, p)) return rc;
+  if (const int rc = check_args(me, p, kDecays)) return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (p->B == 0) return GRU_OK;
   Problem a{};
@@ -314,7 +316,7 @@ extern "C" int gru_delta_backward(const gru_delta_args* p, const void* dout, con
 extern "C" int gru_delta_step(const gru_delta_args* p, float* state, void* out, void* stream_) {
   clear_error();
   const char* me = "gru_delta_step";
-  if (const int rc = check_args(me, p)) return rc;
+  if (const int rc = check_args(me, p, kInputs)) return rc;
   if (p->T != 1) return bad(me, "T must be 1");
   if (p->B == 0) return GRU_OK;
   if (!state || !out || (reinterpret_cast<uintptr_t>(state) & 3) ||

@@ -110,7 +110,7 @@ def _forward(code, q, k, v, g, beta, state, scale, train):
         where = (memory.data_ptr(), stash_bytes, 0, 0) if train else (0, 0, memory.data_ptr(), ws_bytes)
         _lib.check(_lib.load().gru_delta_forward(_args(code, q, k, v, g, beta, state, scale), out.data_ptr(), last.data_ptr(),
                                                  *where, _lib.raw_stream(dev)), "gru_delta_forward")
-    return out, last, memory, (q, k, v)
+    return out, last, memory
 
 
 class GatedDeltaRuleFunction(torch.autograd.Function):
@@ -119,31 +119,32 @@ class GatedDeltaRuleFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, state, scale):
         code = _check("gated_delta_rule", q, k, v, g, beta, state, 2)
-        out, last, stash, (qd, kd, vd) = _forward(code, q, k, v, g, beta, state, scale, True)
+        out, last, stash = _forward(code, q, k, v, g, beta, state, scale, True)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(qd, kd, vd, g, beta, stash)
-        ctx.code, ctx.scale, ctx.has_state = code, scale, state is not None
+        ctx.save_for_backward(g, stash)  # which holds what the gradient needs of the other inputs
+        B, T, Hk, dk = q.shape
+        ctx.sizes, ctx.scale, ctx.dtype = (code, B, T, Hk, v.shape[2], dk, v.shape[3]), scale, q.dtype
         return out, last
 
     @staticmethod
     def backward(ctx, dout, dlast):
-        q, k, v, g, beta, stash = ctx.saved_tensors
-        B, T, Hk, dk = q.shape
-        Hv, dv = v.shape[2:]
-        dev = q.get_device()
-        stash_bytes, _, ws_bytes = _sizes(ctx.code, B, T, Hk, Hv, dk, dv)
+        g, stash = ctx.saved_tensors
+        _, B, T, Hk, Hv, dk, dv = ctx.sizes
+        dev = g.get_device()
+        stash_bytes, _, ws_bytes = _sizes(*ctx.sizes)
         with _lib.on_device(dev):
             dout = None if dout is None else dout.contiguous()
             dlast = None if dlast is None else dlast.contiguous()
-            gq, gk, gv = q.new_empty((B, T, Hk, dk)), q.new_empty((B, T, Hk, dk)), q.new_empty((B, T, Hv, dv))
+            gq, gk = (g.new_empty((B, T, Hk, dk), dtype=ctx.dtype) for _ in range(2))
+            gv = g.new_empty((B, T, Hv, dv), dtype=ctx.dtype)
             gg, gb = g.new_empty((B, T, Hv)), g.new_empty((B, T, Hv))
-            gs = g.new_empty((B, Hv, dk, dv)) if ctx.has_state and ctx.needs_input_grad[5] else None
+            gs = g.new_empty((B, Hv, dk, dv)) if ctx.needs_input_grad[5] else None
             ws = g.new_empty(ws_bytes // 4)
+            a = _lib.DELTA_ARGS.pack(*ctx.sizes, ctx.scale, 0, 0, 0, g.data_ptr(), 0, 0, *[0] * 9, *g.stride(), 0, 0, 0)
             _lib.check(_lib.load().gru_delta_backward(
-                _args(ctx.code, q, k, v, g, beta, None, ctx.scale), 0 if dout is None else dout.data_ptr(),
-                0 if dlast is None else dlast.data_ptr(), stash.data_ptr(), stash_bytes, gq.data_ptr(), gk.data_ptr(),
-                gv.data_ptr(), gg.data_ptr(), gb.data_ptr(), 0 if gs is None else gs.data_ptr(), ws.data_ptr(), ws_bytes,
-                _lib.raw_stream(dev)), "gru_delta_backward")
+                a, 0 if dout is None else dout.data_ptr(), 0 if dlast is None else dlast.data_ptr(), stash.data_ptr(),
+                stash_bytes, gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), gg.data_ptr(), gb.data_ptr(),
+                0 if gs is None else gs.data_ptr(), ws.data_ptr(), ws_bytes, _lib.raw_stream(dev)), "gru_delta_backward")
         return gq, gk, gv, gg, gb, gs, None
 
 
@@ -160,7 +161,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     if torch.is_grad_enabled():
         return GatedDeltaRuleFunction.apply(q, k, v, g, beta, initial_state, scale)
     code = _check("gated_delta_rule", q, k, v, g, beta, initial_state, 2)
-    out, last, _, _ = _forward(code, q, k, v, g, beta, initial_state, scale, False)
+    out, last, _ = _forward(code, q, k, v, g, beta, initial_state, scale, False)
     return out, last
 
 
