@@ -55,25 +55,17 @@ __device__ __forceinline__ void back_load(unsigned char* stage, const Problem& a
   cp_async_commit();
 }
 
-// A warp's 16 tokens x 16 columns as NP planes in shared memory (and `out`,
-// if any), with their scale.
+// A warp's 16 tokens x 16 columns as NP planes in shared memory, with their
+// scale, and in `out`, if given.
 template <int NP>
 __device__ __forceinline__ void put_tokens(const float (&x)[2][4], int quarter, f16* tile, float* scale, f16* out,
-                                           long plane, float* out_scale) {
+                                           float* out_scale) {
   const float inv = plane_inv(warp_max(x));
   if ((threadIdx.x & 31) == 0) {
-    if (tile) scale[quarter] = plane_scale(inv);
+    scale[quarter] = plane_scale(inv);
     if (out) out_scale[quarter] = plane_scale(inv);
   }
-#pragma unroll
-  for (int n = 0; n < 2; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      uint32_t w[NP];
-      split2<NP>(x[n][2 * e], x[n][2 * e + 1], inv, w);
-      if (tile) store_pair<NP>(tile, 2 * kGroup * kC, quarter * 2 + e, n, w);
-      if (out) store_pair<NP>(out, plane, quarter * 2 + e, n, w);
-    }
+  store_rows<NP, NP>(tile, 2 * kGroup * kC, quarter * 2, x, inv, out, kGroup * kC);
 }
 
 // STAGES: with two the next chunk's tiles load during this one; with one they
@@ -119,9 +111,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
     const int t = chunk * kC + quarter * 16;
     od.start(dout + (dout ? t * stride : 0), stride, dout ? a.T - t : 0, cols, vec);
   };
-  // dO of a chunk, whose e^G must be there, as planes: as it is, and for Q^T
-  auto put_dout = [&](int chunk, const float* gate) {
-    float x[2][4];
+  auto dout_tile = [&](float (&x)[2][4]) {
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -130,14 +120,13 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
         x[n][2 * e] = f.x;
         x[n][2 * e + 1] = f.y;
       }
+  };
+  auto put_dout = [&](int chunk) {
+    float x[2][4];
+    dout_tile(x);
     const long nv = nv0 + chunk;
-    put_tokens<NP>(x, quarter, op, osc, a.dop + (nv * groups + group) * NP * kGroup * kC, kGroup * kC,
+    put_tokens<NP>(x, quarter, op, osc, a.dop + (nv * groups + group) * NP * kGroup * kC,
                    a.doscale + (nv * groups + group) * 4);
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[n][e] *= a.scale * gate[frag_row(quarter * 16, e >> 1)];
-    put_tokens<2>(x, quarter, qop, qosc, nullptr, 0, nullptr);
   };
   auto state_out = [&](int chunk) {
     const long nv = nv0 + chunk;
@@ -147,6 +136,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
   back_load<NP, DK>(smem, a, nk0 + a.nc - 1, nv0 + a.nc - 1);
   load_dout(a.nc - 1);
   state_out(a.nc - 1);
+  put_dout(a.nc - 1);
   int buf = 0;
   for (int chunk = a.nc - 1; chunk >= 0; --chunk) {
     const f16* kp = reinterpret_cast<const f16*>(smem + buf * L::stage);
@@ -163,27 +153,32 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
     }
     const float sw = gate[5 * kC], sP = gate[5 * kC + 1], sk = gate[5 * kC + 2], sq = gate[5 * kC + 3];
     const int row[2] = {frag_row(quarter * 16, 0), frag_row(quarter * 16, 1)};
-    put_dout(chunk, gate);
-    if (chunk > 0) load_dout(chunk - 1);
-    // dU
     float x[2][4], y[2][4];
+    // scale e^G dO, for Q^T
+    dout_tile(x);
+    if (chunk > 0) load_dout(chunk - 1);
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[n][e] *= a.scale * gate[row[e >> 1]];
+    put_tokens<2>(x, quarter, qop, qosc, nullptr, nullptr);
+    // dU
     times_state<NP, DK>(x, kp, quarter * 2, sp, ssc);
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[n][e] *= sk * gate[kC + row[e >> 1]];
-    __syncthreads();
     times_tokens<2, NP, true>(x, pp, quarter * 2, op, 2 * kGroup * kC * 2, osc, sP, quarter, 4);
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[n][e] = x[n][e] * gate[2 * kC + row[e >> 1]];
-    put_tokens<2>(y, quarter, up, usc, nullptr, 0, nullptr);
+    put_tokens<2>(y, quarter, up, usc, nullptr, nullptr);
     __syncthreads();
     // Z and dV
     times_tokens<2, 2, true>(x, wp, quarter * 2, up, 2 * kGroup * kC * 2, usc, -sw, quarter, 4);
-    put_tokens<2>(x, quarter, nullptr, nullptr, a.z + (nv * groups + group) * 2 * kGroup * kC, kGroup * kC,
-                  a.zscale + (nv * groups + group) * 4);
+    put_tokens<2>(x, quarter, zp, zsc, a.z + (nv * groups + group) * 2 * kGroup * kC,
+                  a.zscale + (nv * groups + group) * 4);  // zp: on the way only
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -196,7 +191,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
         y[n][2 * e] = -eg * x[n][2 * e];
         y[n][2 * e + 1] = -eg * x[n][2 * e + 1];
       }
-    put_tokens<2>(y, quarter, zp, zsc, nullptr, 0, nullptr);
+    __syncwarp();
+    put_tokens<2>(y, quarter, zp, zsc, nullptr, nullptr);
     __syncthreads();
     const float decay = gate[kC - 1];
 #pragma unroll
@@ -208,6 +204,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
     add_to_state<NP, DK>(d, qp, quarter, qop, qosc, sq);
     add_to_state<NP, DK>(d, kp, quarter, zp, zsc, sk);
     state_out(chunk - 1);
+    if (chunk > 0) put_dout(chunk - 1);
     if (STAGES == 1 && chunk > 0) {
       __syncthreads();
       back_load<NP, DK>(smem, a, nk0 + chunk - 1, nv - 1);

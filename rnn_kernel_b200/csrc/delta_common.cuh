@@ -292,13 +292,30 @@ __device__ __forceinline__ float warp_max(const float (&x)[NT][4]) {
   return warp_max<NT>(x, all_finite);
 }
 
-// Writes an accumulator pair (row block r8, column tile n) of a tile of 16
-// columns, `plane` elements between planes; the first `np` of the NP planes.
-template <int NP>
-__device__ __forceinline__ void store_pair(f16* tile, long plane, int r8, int n, const uint32_t (&w)[NP], int np = NP) {
+// Writes 16 rows (from row block r8) x 16 columns of accumulators, times inv, as
+// NP planes of a tile of 16 columns in shared memory (`plane` elements apart);
+// the first PO of them also into `out`, if given, 16 bytes a lane.  Four blocks
+// of 128 consecutive bytes, which is what stmatrix writes at once.
+template <int NP, int PO>
+__device__ __forceinline__ void store_rows(f16* tile, int plane, int r8, const float (&x)[2][4], float inv, f16* out,
+                                           int out_plane) {
+  uint32_t w[2][2][NP];
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) split2<NP>(x[n][2 * e], x[n][2 * e + 1], inv, w[e][n]);
+  const int at = r8 * 128 + (threadIdx.x & 31) * 8;
 #pragma unroll
   for (int p = 0; p < NP; ++p)
-    if (p < np) reinterpret_cast<uint32_t*>(tile + p * plane)[(r8 * 2 + n) * 32 + (threadIdx.x & 31)] = w[p];
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(smem_addr(tile + p * plane + at)),
+                 "r"(w[0][0][p]), "r"(w[0][1][p]), "r"(w[1][0][p]), "r"(w[1][1][p])
+                 : "memory");
+  if (out) {
+    __syncwarp();
+#pragma unroll
+    for (int p = 0; p < PO; ++p)
+      *reinterpret_cast<uint4*>(out + p * out_plane + at) = *reinterpret_cast<const uint4*>(tile + p * plane + at);
+  }
 }
 
 // ---------------------------------------------------------------------------

@@ -597,14 +597,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
 #pragma unroll
           for (int e = 0; e < 4; ++e) y[n][e] = finite(y[n][e]) && finite(x[n][e]) ? y[n][e] : 0.0f;
       }
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t w[2];
-          split2<2>(y[n][2 * e], y[n][2 * e + 1], inv, w);
-          store_pair<2>(xp, 2 * kGroup * kC, quarter * 2 + e, n, w);
-        }
+      store_rows<2, 0>(xp, 2 * kGroup * kC, quarter * 2, y, inv, nullptr, 0);
     }
     off = __syncthreads_or(off);
     if (off) {  // rare, and the same for the whole CTA
@@ -631,14 +624,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
       // a scale below zero marks a quarter that holds something not finite
       if (lane == 0) a.escale[(nv * groups + group) * 4 + quarter] = all_finite ? plane_scale(inv) : -plane_scale(inv);
       f16* out = a.e + (nv * groups + group) * PO * kGroup * kC;
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t w[2];
-          split2<2>(x[n][2 * e], x[n][2 * e + 1], inv, w);
-          store_pair<2>(out, kGroup * kC, quarter * 2 + e, n, w, PO);
-        }
+      store_rows<PO, PO>(yp, 2 * kGroup * kC, quarter * 2, x, inv, out, kGroup * kC);  // yp: on the way only
     }
     // S <- e^G S + K^T (e^(G_end - G) U)
     {
@@ -648,14 +634,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
         for (int e = 0; e < 4; ++e) x[n][e] *= gate[kC + row[e >> 1]] * gate[2 * kC + row[e >> 1]];
       const float inv = plane_inv(warp_max(x));
       if (lane == 0) ysc[quarter] = plane_scale(inv);
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t w[2];
-          split2<2>(x[n][2 * e], x[n][2 * e + 1], inv, w);
-          store_pair<2>(yp, 2 * kGroup * kC, quarter * 2 + e, n, w);
-        }
+      __syncwarp();
+      store_rows<2, 0>(yp, 2 * kGroup * kC, quarter * 2, x, inv, nullptr, 0);
     }
     __syncthreads();
     if (off && threadIdx.x < kSlice) first[threadIdx.x] = kC;

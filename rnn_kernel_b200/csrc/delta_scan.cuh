@@ -117,16 +117,7 @@ __device__ __forceinline__ void put_state(const float (&s)[DK / 64][2][4], int q
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        uint32_t w[2];
-        split2<2>(s[i][n][2 * e], s[i][n][2 * e + 1], inv, w);
-        const int r8 = (quarter * MT + i) * 2 + e;
-        store_pair<2>(sp, 2 * kGroup * DK, r8, n, w);
-        if (out) store_pair<2>(out, kGroup * DK, r8, n, w, PO);
-      }
+    store_rows<2, PO>(sp, 2 * kGroup * DK, (quarter * MT + i) * 2, s[i], inv, out, kGroup * DK);
 }
 
 }  // namespace delta
