@@ -292,12 +292,20 @@ __device__ __forceinline__ float2 pair(uint32_t h, uint32_t l) {
 template <int NA, int NB, int NT>
 __device__ __forceinline__ void step_add(float (&acc)[NT][4], float f0, float f1, const uint32_t (&fa)[NA][4],
                                          const uint32_t (&fb)[NB][NT][2]) {
-  float t[NT][4];
-  mma_terms<NA, NB, NT>(t, fa, fb);
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+  for (int h = 0; h < 2; ++h) {
+    float t[NT / 2][4];
+    uint32_t g[NB][NT / 2][2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[i][e] += (2 * i < NT ? f0 : f1) * t[i][e];
+    for (int p = 0; p < NB; ++p)
+#pragma unroll
+      for (int i = 0; i < NT / 2; ++i) g[p][i][0] = fb[p][h * NT / 2 + i][0], g[p][i][1] = fb[p][h * NT / 2 + i][1];
+    mma_terms<NA, NB, NT / 2>(t, fa, g);
+#pragma unroll
+    for (int i = 0; i < NT / 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[h * NT / 2 + i][e] += (h ? f1 : f0) * t[i][e];
+  }
 }
 
 // acc += f A B over steps [k0, k1) of the tokens: A a 64 x 64 tile (rows m, or

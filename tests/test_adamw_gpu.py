@@ -202,6 +202,26 @@ def test_many_tensors_of_two_types_groups_and_missing_gradients():
                 torch.testing.assert_close(p.detach().double(), w.detach(), rtol=3 * 2.0 ** -9, atol=1e-6)
 
 
+def test_gradients_that_are_not_dense():
+    torch.manual_seed(5)
+    ps = [torch.nn.Parameter(torch.randn(60, 80, device="cuda")) for _ in range(3)]
+    wide = [torch.nn.Parameter(p.detach().double()) for p in ps]
+    opt, ref = AdamW(ps), torch.optim.AdamW(wide, weight_decay=1e-2)
+    for step in range(3):
+        ps[0].grad = torch.randn(80, 60, device="cuda").t()
+        ps[1].grad = torch.randn(1, 80, device="cuda").expand(60, 80)
+        ps[2].grad = None if step == 1 else torch.randn(60, 80, device="cuda")
+        for p, w in zip(ps, wide):
+            w.grad = None if p.grad is None else p.grad.double()
+        opt.step()
+        ref.step()
+    for p, w in zip(ps, wide):
+        torch.testing.assert_close(p.detach().double(), w.detach(), rtol=2e-6, atol=2e-7)
+    ps[0].grad = torch.sparse_coo_tensor(torch.zeros(2, 1, dtype=torch.long), torch.ones(1), (60, 80)).cuda()
+    with pytest.raises(RuntimeError):
+        opt.step()
+
+
 def test_grad_scale_and_repeatability():
     runs = []
     for scale in (1.0, 0.25):
@@ -253,6 +273,23 @@ def test_state_dict_resumes_bit_for_bit(bits, capturable):
         assert torch.equal(p.detach(), q.detach())
     with pytest.raises(ValueError):
         AdamW(params_of([512, 40]), state_bits=bits).load_state_dict(saved)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_than_32_bits_of_elements(bits):
+    n = 2 ** 31 + 300
+    p = torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device="cuda"))
+    p.grad = torch.zeros_like(p)
+    tail = torch.linspace(-1, 1, 700, device="cuda")
+    p.grad[-700:] = tail.bfloat16()
+    p.grad[0] = 1.0
+    opt = AdamW([p], lr=1e-2, weight_decay=0.0, state_bits=bits)
+    opt.step()
+    # the first step is lr * sign(g)
+    got = p.detach()[-700:].float()
+    torch.testing.assert_close(got, -1e-2 * tail.bfloat16().float().sign(), rtol=2.0 ** -8, atol=0)
+    assert float(p.detach()[0]) == pytest.approx(-1e-2, rel=2.0 ** -8)
+    assert int((p.detach()[:-700] != 0).sum()) == 1
 
 
 def test_capturable_counts_on_the_device():

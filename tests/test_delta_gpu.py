@@ -327,6 +327,47 @@ def test_long_sequence_in_ranges(dtype):
     assert torch.equal(out_g, out) and torch.equal(last_g, last)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("power", [-60, -7, 40])
+def test_scaled_values_give_scaled_results(dtype, power):
+    """Tiles carry their own power of two, so values, states and queries of any size lose nothing: bit for bit."""
+    x = R.inputs(1, 150, 1, 2, 72, 40, dtype=dtype, seed=16)
+    f = 2.0 ** power
+    runs = []
+    for scale in (1.0, f):
+        q, k, v, g, beta, s = x
+        mine = with_grad((q * 2.0 ** 20 if scale != 1.0 else q, k, v * scale, g, beta, s * scale))
+        out, last = gated_delta_rule(*mine[:5], initial_state=mine[5])
+        do = torch.ones_like(out) * (k.new_tensor(1.5))
+        grads = torch.autograd.grad((out, last), mine, (do, torch.ones_like(last) * 2.0 ** 20 if scale != 1.0 else torch.ones_like(last)))
+        runs.append((out, last) + grads)
+    (o, l, dq, dk, dv, dg, db, ds), (o2, l2, dq2, dk2, dv2, dg2, db2, ds2) = runs
+    big = 2.0 ** 20
+    assert torch.equal(o2.float(), o.float() * (f * big)) and torch.equal(l2, l * f)
+    # out's gradient times q's factor, dS's likewise: all sums grow alike
+    assert torch.equal(dq2.float(), dq.float() * f) and torch.equal(dk2.float(), dk.float() * (f * big))
+    assert torch.equal(dv2.float(), dv.float() * big) and torch.equal(ds2, ds * big)
+    assert torch.equal(dg2, dg * (f * big)) and torch.equal(db2, db * (f * big))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides_and_offsets_past_32_bits(dtype):
+    x = R.inputs(2, 70, 1, 2, 16, 24, dtype=dtype, seed=17)
+    want = gated_delta_rule(*x[:5], initial_state=x[5])
+    far = 2 ** 31 + 64  # elements between the two sequences
+    base = torch.empty(far + 70 * 2 * 24, dtype=dtype, device="cuda")
+    wide = []
+    for t in x[:3]:
+        w = base.as_strided(t.shape, (far,) + t.stride()[1:])
+        wide.append(w.copy_(t))
+        got = gated_delta_rule(*(w if t is y else y for y in x[:3]), *x[3:5], initial_state=x[5])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        state, other = x[5].clone(), x[5].clone()
+        a = gated_delta_step(*((w if t is y else y)[:, 3] for y in x[:3]), x[3][:, 3], x[4][:, 3], state)
+        b = gated_delta_step(*(y[:, 3] for y in x[:5]), other)
+        assert torch.equal(a, b) and torch.equal(state, other)
+
+
 def test_refusals():
     q, k, v, g, beta, s = R.inputs(2, 5, 2, 4, 16, 8)
     with pytest.raises(ValueError, match="shape"):
