@@ -25,13 +25,15 @@ namespace gru {
 namespace delta {
 namespace {
 
-// The chunks of every sequence that a launch works on.
+// The chunks of every sequence that a launch works on; `parts`: CTAs of prepare
+// that share a key head's value heads.
 struct Range {
-  int first, n;
+  int first, n, parts;
 };
 
 // ---------------------------------------------------------------------------
-// prepare: one CTA per (batch, key head, chunk), over the head's value heads.
+// prepare: one CTA per (batch, key head, chunk), over the head's value heads; in
+// a small grid one for each of those.
 // Latency-bound (a chain of small products between barriers), so it keeps its
 // shared memory small enough for several CTAs on an SM (2048 chunks of heads of
 // 128, two to a key head: 67 us).
@@ -196,8 +198,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
   int* bad = reinterpret_cast<int*>(gates2 + 2 * kGates * kC);  // tokens whose key is not finite
   float* red = reinterpret_cast<float*>(bad + kC);         // [4][8] and scales
 
-  const int chunk = range.first + blockIdx.x % range.n, bh = blockIdx.x / range.n;
+  const int part = blockIdx.x % range.parts, block = blockIdx.x / range.parts;
+  const int chunk = range.first + block % range.n, bh = block / range.n;
   const int h = bh % a.Hk, b = bh / a.Hk;
+  const int r0 = part * (a.rep / range.parts), r1 = r0 + a.rep / range.parts;
   const long nk = (long)bh * a.nc + chunk;
   const int t0 = chunk * kC, rows = min(kC, a.T - t0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         *reinterpret_cast<uint2*>(ks + p * kC * DK + at) = make_uint2(w0[p], w1[p]);
-        *reinterpret_cast<uint2*>(ko + p * kC * DK + at) = make_uint2(w0[p], w1[p]);
+        if (part == 0) *reinterpret_cast<uint2*>(ko + p * kC * DK + at) = make_uint2(w0[p], w1[p]);
       }
       f = value(qr[x], x);
       split2<NP>(f.x, f.y, iq, w0);
@@ -313,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         *reinterpret_cast<uint2*>(qs + p * kC * DK + at) = make_uint2(w0[p], w1[p]);
-        *reinterpret_cast<uint2*>(qo + p * kC * DK + at) = make_uint2(w0[p], w1[p]);
+        if (part == 0) *reinterpret_cast<uint2*>(qo + p * kC * DK + at) = make_uint2(w0[p], w1[p]);
       }
     }
   }
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
   zero(ak);
   zero(aq);
   // warp 1's tiles are above the diagonal: it makes the first gates meanwhile
-  if (warp == 1) chunk_gates(a, b, h * a.rep, t0, rows, bad, gates2);
+  if (warp == 1) chunk_gates(a, b, h * a.rep + r0, t0, rows, bad, gates2 + (r0 & 1) * kGates * kC);
   if (n0 <= m0) {
     const uint32_t pk = addr_a<DK, false>(ks, m0 / 8, 0), pq = addr_a<DK, false>(qs, m0 / 8, 0);
     const uint32_t pb = addr_b<DK, false>(ks, 0, n0 / 8);
@@ -361,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
   __syncthreads();
   for (int x = threadIdx.x; x < kC * kLd; x += kThreads) W[x] = 0.0f;  // above its diagonal blocks it stays zero
 
-  for (int r = 0; r < a.rep; ++r) {
+  for (int r = r0; r < r1; ++r) {
     const int hv = h * a.rep + r;
     const long nv = ((long)b * a.Hv + hv) * a.nc + chunk;
     const float* gates = gates2 + (r & 1) * kGates * kC;
@@ -419,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
     // next value head's gates meanwhile
     const int o1 = (warp >> 1) * 32, n1 = (warp & 1) * 8;
     if (warp < 4) join_first(jx, N, W, X, o1 + 16, o1, o1 + 16, n1, beta);
-    if (warp == 7 && r + 1 < a.rep)
+    if (warp == 7 && r + 1 < r1)
       chunk_gates(a, b, hv + 1, t0, rows, bad, gates2 + ((r + 1) & 1) * kGates * kC);
     __syncthreads();
     if (warp < 4) join_second(jx, W, X, o1 + 16, o1, o1 + 16, n1);
@@ -874,7 +878,12 @@ int run_prepare(const Problem& a, Range r, cudaStream_t stream) {
   constexpr int bytes = PrepareSmem<T, DK>::bytes;
   if (const int rc = with_smem(delta_prepare_kernel<T, DK>, bytes)) return rc;
   LaunchScope scope(kKindDeltaRule, stream);
-  delta_prepare_kernel<T, DK><<<(unsigned)((long)a.B * a.Hk * r.n), kThreads, bytes, stream>>>(a, r);
+  const long ctas = (long)a.B * a.Hk * r.n;
+  // While SMs are left over, a value head of its own CTA costs only the products of
+  // keys once more (a prompt of 77, 4 key and 8 value heads: 48.7 us from call to
+  // result, 53.6 with both in turn); in a full grid that would be work for nothing.
+  r.parts = ctas * a.rep <= 148 ? a.rep : 1;
+  delta_prepare_kernel<T, DK><<<(unsigned)(ctas * r.parts), kThreads, bytes, stream>>>(a, r);
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
 }
@@ -916,7 +925,7 @@ int forward_typed(const Problem& a, cudaStream_t stream) {
     if ((rc = side_stream(device, stream, &side))) return rc;
   }
   const int step = side ? (a.nc + kRanges - 1) / kRanges : a.nc;
-  Range r{0, step}, before{0, 0};
+  Range r{0, step, 1}, before{0, 0, 1};
   if ((rc = run_prepare<T, DK>(a, r, stream))) return rc;
   if (side && (rc = stream_after(side->s, stream, side->fork))) return rc;
   if ((rc = scan(r))) return rc;
