@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
   const int quarter = (threadIdx.x >> 5) & 3, pair = threadIdx.x >> 7;
   const int group = (blockIdx.x % slices) * 2 + pair, c0 = group * kGroup;
   const long nv0 = (long)bh * a.nc, nk0 = ((long)b * a.Hk + hv / a.rep) * a.nc;
+  let_next_start();
   f16* base = reinterpret_cast<f16*>(smem + STAGES * L::stage);
   f16* sp = base + pair * kGroup * DK;
   f16* up = base + L::s + pair * kGroup * kC;  // B dU
@@ -352,6 +353,7 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
 
   copy_async<L::qk * 2, threads>(qp, a.qp + (long)blockIdx.x * L::qk);
   copy_async<L::qk * 2, threads>(kp, a.kp + (long)blockIdx.x * L::qk);
+  wait_for_before();
 
   for (int r = 0; r < a.rep; ++r) {
     const int hv = hk * a.rep + r;
@@ -664,9 +666,7 @@ int backward_typed(const Problem& a, cudaStream_t stream) {
   } else {
     if (const int rc = launch_scan<T, DK, 1>(a, stream)) return rc;
   }
-  delta_grads_kernel<T, DK><<<(unsigned)((long)a.B * a.Hk * a.nc), G::threads, grad_bytes, stream>>>(a);
-  GRU_CUDA_TRY(cudaGetLastError());
-  return GRU_OK;
+  return launch_after(delta_grads_kernel<T, DK>, (unsigned)((long)a.B * a.Hk * a.nc), G::threads, grad_bytes, stream, a);
 }
 
 }  // namespace

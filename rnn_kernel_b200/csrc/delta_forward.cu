@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
   int* bad = reinterpret_cast<int*>(gates2 + 2 * kGates * kC);  // tokens whose key is not finite
   float* red = reinterpret_cast<float*>(bad + kC);         // [4][8] and scales
 
+  let_next_start();
   const int part = blockIdx.x % range.parts, block = blockIdx.x / range.parts;
   const int chunk = range.first + block % range.n, bh = block / range.n;
   const int h = bh % a.Hk, b = bh / a.Hk;
@@ -556,8 +557,10 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
                       a.sscale + (nv * groups + group) * 4);
   };
   const int end = range.first + range.n;
-  scan_load<NP, DK>(smem + (range.first & 1) * L::stage, a, nk0 + range.first, nv0 + range.first);
   load_v(range.first);
+  wait_for_before();
+  let_next_start();
+  scan_load<NP, DK>(smem + (range.first & 1) * L::stage, a, nk0 + range.first, nv0 + range.first);
   if (threadIdx.x < kSlice) first[threadIdx.x] = kC;
   state_out(range.first);
   for (int chunk = range.first; chunk < end; ++chunk) {
@@ -758,6 +761,7 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
   const int chunk = range.first + blockIdx.x % range.n, bh = blockIdx.x / range.n;
   const int hv = bh % a.Hv, b = bh / a.Hv;
   const long nv = (long)bh * a.nc + chunk, nk = ((long)b * a.Hk + hv / a.rep) * a.nc + chunk;
+  wait_for_before();
   copy_async<L::q * 2, kThreads>(qp, a.qp + nk * L::q);
   copy_async<L::p * 2, kThreads>(pp, a.pp + nv * 2 * kTile);
   copy_async<kGates * kC * 4, kThreads>(gate, a.gates + nv * kGates * kC);
@@ -892,7 +896,9 @@ int run_scan(const Problem& a, Range r, cudaStream_t stream) {
   constexpr int bytes = ScanSmem<Planes<T>::n, DK>::bytes;
   if (const int rc = with_smem(delta_scan_kernel<T, DK, PO>, bytes)) return rc;
   LaunchScope scope(kKindDeltaRule, stream);
-  delta_scan_kernel<T, DK, PO><<<(unsigned)((long)a.B * a.Hv * (a.dvp / kSlice)), kThreads, bytes, stream>>>(a, r);
+  const unsigned ctas = (unsigned)((long)a.B * a.Hv * (a.dvp / kSlice));
+  if (r.n == a.nc) return launch_after(delta_scan_kernel<T, DK, PO>, ctas, kThreads, bytes, stream, a, r);
+  delta_scan_kernel<T, DK, PO><<<ctas, kThreads, bytes, stream>>>(a, r);
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
 }
@@ -901,7 +907,9 @@ int run_output(const Problem& a, Range r, cudaStream_t stream) {
   constexpr int bytes = OutputSmem<T, DK>::bytes;
   if (const int rc = with_smem(delta_output_kernel<T, DK>, bytes)) return rc;
   LaunchScope scope(kKindDeltaRule, stream);
-  delta_output_kernel<T, DK><<<(unsigned)((long)a.B * a.Hv * r.n), kThreads, bytes, stream>>>(a, r);
+  const unsigned ctas = (unsigned)((long)a.B * a.Hv * r.n);
+  if (r.n == a.nc) return launch_after(delta_output_kernel<T, DK>, ctas, kThreads, bytes, stream, a, r);
+  delta_output_kernel<T, DK><<<ctas, kThreads, bytes, stream>>>(a, r);
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
 }
