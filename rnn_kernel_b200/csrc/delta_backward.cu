@@ -347,8 +347,11 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
   const int hk = bh % a.Hk, b = bh / a.Hk;
   const int t0 = chunk * kC, rows = min(kC, a.T - t0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m0 = warp / split * 16, col = warp % split;  // this warp's tokens; its part of the columns
-  const bool below = col * NC * 8 <= m0;                 // whether that holds any of the 64 x 64 products' lower half
+  // This warp's tokens; its part of the columns, and whether that holds any of the
+  // 64 x 64 products' lower half.  The parts turn from row to row: were they the
+  // warp's remainder, one of the SM's quarters would have twice the others' products.
+  const int m0 = warp / split * 16, col = (warp - warp / split * split / 4) & (split - 1);
+  const bool below = col * NC * 8 <= m0;
   const int groups = a.dvp / kGroup;
 
   copy_async<L::qk * 2, threads>(qp, a.qp + (long)blockIdx.x * L::qk);
