@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
   extern __shared__ __align__(16) unsigned char smem[];
   const int slices = a.dvp / kSlice, groups = a.dvp / kGroup;
   const int bh = blockIdx.x / slices, hv = bh % a.Hv, b = bh / a.Hv;
-  const int quarter = (threadIdx.x >> 5) & 3, pair = threadIdx.x >> 7;
+  const int pair = threadIdx.x >> 7, quarter = quarter_of(threadIdx.x);
   const int group = (blockIdx.x % slices) * 2 + pair, c0 = group * kGroup;
   const long nv0 = (long)bh * a.nc, nk0 = ((long)b * a.Hk + hv / a.rep) * a.nc;
   let_next_start();

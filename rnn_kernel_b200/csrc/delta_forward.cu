@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
   extern __shared__ __align__(16) unsigned char smem[];
   const int slices = a.dvp / kSlice, groups = a.dvp / kGroup;
   const int bh = blockIdx.x / slices, hv = bh % a.Hv, b = bh / a.Hv;
-  const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3, pair = threadIdx.x >> 7;
+  const int lane = threadIdx.x & 31, pair = threadIdx.x >> 7, quarter = quarter_of(threadIdx.x);
   const int group = (blockIdx.x % slices) * 2 + pair, c0 = group * kGroup;
   const long nv0 = (long)bh * a.nc, nk0 = ((long)b * a.Hk + hv / a.rep) * a.nc;
   f16* base = reinterpret_cast<f16*>(smem + 2 * L::stage);
@@ -767,7 +767,8 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
   copy_async<kGates * kC * 4, kThreads>(gate, a.gates + nv * kGates * kC);
   output_load<T, DK>(slices, a, nv, 0);
   const int warp = threadIdx.x >> 5;
-  const int m0 = (warp >> 1) * 16, half = warp & 1;
+  // rows of 1 and 4 steps of P to two of the SM's quarters, of 2 and 3 to the others
+  const int m0 = (warp >> 1 ^ warp >> 2) * 16, half = warp & 1;
   T* o = static_cast<T*>(a.o) + (((long)b * a.T + (long)chunk * kC) * a.Hv + hv) * a.dv;
   const int rows = a.T - chunk * kC;
   const bool vec = a.dv % 2 == 0 && (reinterpret_cast<uintptr_t>(o) & (2 * sizeof(T) - 1)) == 0;

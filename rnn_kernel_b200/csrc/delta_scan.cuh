@@ -7,6 +7,15 @@
 namespace gru {
 namespace delta {
 
+// The quarter of the tokens (and of the key columns) of a scan's warp, among the
+// four of its value columns.  The second four take them the other way around:
+// quarters have 1 to 4 steps of a triangular product, and warps 4 apart share an
+// SM's quarter.
+__device__ __forceinline__ int quarter_of(int thread) {
+  const int warp = thread >> 5;
+  return (warp & 4 ? ~warp : warp) & 3;
+}
+
 // x (16 tokens x 16 columns) = K S of this warp's tokens; S as planes with a
 // scale for each quarter of its rows.
 template <int NP, int DK>
