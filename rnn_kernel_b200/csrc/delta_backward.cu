@@ -569,6 +569,11 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
     token_product<NP, DK, false, NT>(dkr, sw * sk, mp, m0 / 8, kp, col * NT, 0, m0 / 16 + 1);
     token_product<NP, DK, true, NT>(dkc, su * sq, dpp, m0 / 8, qp, col * NT, m0 / 16, kC / 16);
     token_product<NP, DK, true, NT>(dkc, sw * sk, mp, m0 / 8, kp, col * NT, m0 / 16, kC / 16);
+    float log_decay[2];  // of the two tokens that a lane of warp 0 ends with
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      log_decay[e] = warp == 0 && 2 * lane + e < rows
+                         ? a.g[b * a.sg[0] + (t0 + 2 * lane + e) * a.sg[1] + hv * a.sg[2]] : 0.0f;
     {
       constexpr int per = threads / kC;
       const int t = threadIdx.x / per;
@@ -581,7 +586,7 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
     __syncthreads();
     if (warp == 0) {
       // two tokens a lane: x summed from the end, z from the start
-      double x[2], z[2], last = 0.0;
+      double x[2], z[2], last = lane < 4 * split ? wred[lane] : 0.0f;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int i = 2 * lane + e;
@@ -598,17 +603,16 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
         const double u = __shfl_down_sync(0xffffffffu, sx, o), w = __shfl_up_sync(0xffffffffu, sz, o);
         if (lane + o < 32) sx += u;
         if (lane >= o) sz += w;
+        last += __shfl_xor_sync(0xffffffffu, last, o);
       }
-      for (int w = 0; w < 4 * split; ++w) last += wred[w];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int i = 2 * lane + e;
         if (i < rows) {
-          const float gv = a.g[b * a.sg[0] + (t0 + i) * a.sg[1] + hv * a.sg[2]];
           const double from = e ? sx - x[0] : sx, before = e ? sz - z[1] : sz - z[0] - z[1];
           // a decay of zero passes no gradient
           a.dg[((long)b * a.T + t0 + i) * a.Hv + hv] =
-              gv < kNoDecay ? 0.0f : (float)(from + before + red[2 * split * kC + i] + last);
+              log_decay[e] < kNoDecay ? 0.0f : (float)(from + before + red[2 * split * kC + i] + last);
         }
       }
     }
