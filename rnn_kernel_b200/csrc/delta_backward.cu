@@ -391,6 +391,20 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
       const int mq = m0 / 16, kq = col * 4 / split;  // quarters of this warp's tokens and of its first key column
       constexpr int k2 = split == 4 ? 0 : 1;         // and of its last
       const float fE = fabsf(se[mq]), fZ = sz[mq], fO = so[mq];
+      auto state_dot = [&] {
+#pragma unroll
+        for (int j = 0; j < kGroup * DK / 2 / threads; ++j) {
+          // block warp + 4 split j is of the rows 8 (warp / 2 + 2 split j) ..., in quarter q
+          const int word = threadIdx.x + j * threads, q = (warp / 2 + 2 * split * j) * 8 / (DK / 4);
+          const float2 u = take2<2>(sp, kGroup * DK, word), v = take2<2>(dsp, kGroup * DK, word);
+          sdot += (ss[q] * sds[q]) * (u.x * v.x + u.y * v.y);
+        }
+      };
+      // of eight warps, half begin with what takes shared memory and no tensor core
+      // (training 64 x 512 437 us, 441 where all end with it; sixteen are spread by
+      // themselves: training 4 x 2048 757 us, 768)
+      const bool early = split == 2 && (m0 & 16);
+      if (early) state_dot();
       uint32_t fz[2][4], fe[2][4];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
@@ -427,13 +441,7 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
         step_add<NP, 2, NC>(dp, fO * f0, fO * f1, fo, fb);
         step_add<2, 2, NC>(da, fZ * f0, fZ * f1, fz, fb);
       }
-#pragma unroll
-      for (int j = 0; j < kGroup * DK / 2 / threads; ++j) {
-        // block warp + 4 split j is of the rows 8 (warp / 2 + 2 split j) ..., in quarter q
-        const int word = threadIdx.x + j * threads, q = (warp / 2 + 2 * split * j) * 8 / (DK / 4);
-        const float2 u = take2<2>(sp, kGroup * DK, word), v = take2<2>(dsp, kGroup * DK, word);
-        sdot += (ss[q] * sds[q]) * (u.x * v.x + u.y * v.y);
-      }
+      if (!early) state_dot();
     }
     __syncthreads();
     // the masked 64 x 64 products, over the stages' memory
