@@ -629,28 +629,32 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
     float2* sum = reinterpret_cast<float2*>(L::sums_fit ? reinterpret_cast<float*>(smem + L::least)
                                                         : a.dqk + (long)blockIdx.x * 2 * kC * DK) + threadIdx.x;
     const bool even = a.dk % 2 == 0;
+    const bool whole = a.dk % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.dq) | reinterpret_cast<uintptr_t>(a.dk_)) & 15) == 0;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int e = 0; e < 2; ++e) {
+      float2 x[NT], z[NT];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = frag_row(m0, e), c = frag_col((col * NT + n) * 8);
-        float2 x = make_float2(dq[n][2 * e], dq[n][2 * e + 1]);
-        float2 z = make_float2(dkr[n][2 * e] + dkc[n][2 * e], dkr[n][2 * e + 1] + dkc[n][2 * e + 1]);
+      for (int n = 0; n < NT; ++n) {
+        x[n] = make_float2(dq[n][2 * e], dq[n][2 * e + 1]);
+        z[n] = make_float2(dkr[n][2 * e] + dkc[n][2 * e], dkr[n][2 * e + 1] + dkc[n][2 * e + 1]);
         float2* px = sum + (n * 4 + e * 2) * threads;
         float2* pz = px + threads;
         if (r > 0) {
-          x.x += px->x, x.y += px->y;
-          z.x += pz->x, z.y += pz->y;
+          x[n].x += px->x, x[n].y += px->y;
+          z[n].x += pz->x, z[n].y += pz->y;
         }
         if (r + 1 < a.rep) {
-          *px = x;
-          *pz = z;
-        } else if (row < rows) {
-          const long o = (((long)b * a.T + t0 + row) * a.Hk + hk) * a.dk + c;
-          set2<T>(static_cast<T*>(a.dq) + o, a.dk - c, even, x.x, x.y);
-          set2<T>(static_cast<T*>(a.dk_) + o, a.dk - c, even, z.x, z.y);
+          *px = x[n];
+          *pz = z[n];
         }
       }
+      if (r + 1 == a.rep) {
+        const int row = frag_row(m0, e), c = col * NT * 8;
+        const long o = (((long)b * a.T + t0 + row) * a.Hk + hk) * a.dk + c;
+        set_row<T>(static_cast<T*>(a.dq) + o, a.dk - c, even, whole, row < rows, x);
+        set_row<T>(static_cast<T*>(a.dk_) + o, a.dk - c, even, whole, row < rows, z);
+      }
+    }
   }
 }
 

@@ -385,6 +385,39 @@ __device__ __forceinline__ void set2<bf16>(bf16* p, int left, bool vec, float a,
   }
 }
 
+// A row of four accumulator tiles, 32 columns over four lanes, stored at p where
+// `in` and they exist (`left` of them do).  `pairs`: p allows two-element accesses;
+// `whole`: 16-byte ones too, and `left` is a multiple of 8.  Then bf16 goes between
+// the lanes first, so that each stores 16 bytes once instead of 4 four times.
+template <typename T>
+__device__ __forceinline__ void set_row(T* p, int left, bool pairs, bool whole, bool in, const float2 (&x)[4]) {
+  const int lane = threadIdx.x & 3;
+  if (sizeof(T) == 2 && whole) {
+    uint32_t w[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(x[n].x, x[n].y);
+      w[n] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    // lane i's word j becomes lane j's word i
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        if (!(n & o)) {
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, lane & o ? w[n] : w[n + o], o);
+          if (lane & o) w[n] = got; else w[n + o] = got;
+        }
+    if (in && lane * 8 < left) *reinterpret_cast<uint4*>(p + lane * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else if (in) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int c = n * 8 + lane * 2;
+      set2<T>(p + c, left - c, pairs, x[n].x, x[n].y);
+    }
+  }
+}
+
 // A warp's 16 tokens x 8 or 16 value columns of a [token][column] tensor, as
 // accumulator tiles.  `start` issues the loads and `get` gives a value pair,
 // zero where the tensor has none: nothing between the two waits for memory.

@@ -772,6 +772,7 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
   T* o = static_cast<T*>(a.o) + (((long)b * a.T + (long)chunk * kC) * a.Hv + hv) * a.dv;
   const int rows = a.T - chunk * kC;
   const bool vec = a.dv % 2 == 0 && (reinterpret_cast<uintptr_t>(o) & (2 * sizeof(T) - 1)) == 0;
+  const bool whole = a.dv % 8 == 0 && (reinterpret_cast<uintptr_t>(a.o) & 15) == 0;
   for (int c0 = 0, buf = 0; c0 < a.dvp; c0 += L::cols) {
     cp_async_wait<0>();
     __syncthreads();
@@ -861,14 +862,12 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = frag_row(m0, e);
-        if (row < rows) {
-          const float f = gate[row] * fx;
-          T* p = o + (long)row * a.Hv * a.dv + cw + frag_col(0);
+        const float f = gate[row] * fx;
+        float2 z[4];
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
-            set2<T>(p + n * 8, a.dv - cw - frag_col(n * 8), vec, f * x[n][2 * e] + fy * y[n][2 * e],
-                    f * x[n][2 * e + 1] + fy * y[n][2 * e + 1]);
-        }
+        for (int n = 0; n < 4; ++n)
+          z[n] = make_float2(f * x[n][2 * e] + fy * y[n][2 * e], f * x[n][2 * e + 1] + fy * y[n][2 * e + 1]);
+        set_row<T>(o + (long)row * a.Hv * a.dv + cw, a.dv - cw, vec, whole, row < rows, z);
       }
     }
     if (L::buffers == 1 && c0 + L::cols < a.dvp) {
