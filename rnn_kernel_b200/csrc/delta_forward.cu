@@ -67,7 +67,7 @@ __device__ __forceinline__ void mma_f32(float (&acc)[4], const float* A, int lda
       y -= __uint_as_float(w[p] & 0xffff0000u);
     }
   };
-#pragma unroll 2
+#pragma unroll 1
   for (int k = k0; k < k1; k += 16) {
     uint32_t fa[3][4], fb[2][3];
 #pragma unroll
@@ -334,7 +334,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
   if (n0 <= m0) {
     const uint32_t pk = addr_a<DK, false>(ks, m0 / 8, 0), pq = addr_a<DK, false>(qs, m0 / 8, 0);
     const uint32_t pb = addr_b<DK, false>(ks, 0, n0 / 8);
-#pragma unroll
+    // rolled, like the joins' steps: unrolled, a tenth of the stalls are for instructions
+#pragma unroll 1
     for (int kk = 0; kk < DK / 16; ++kk) {
       uint32_t fk[NP][4], fq[NP][4], fb[NP][4][2];
 #pragma unroll
