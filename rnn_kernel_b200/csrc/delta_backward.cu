@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[n][e] = x[n][e] * gate[2 * kC + row[e >> 1]];
     put_tokens<2>(y, quarter, up, usc, nullptr, nullptr);
-    __syncthreads();
+    group_sync(pair);
     // Z and dV
     times_tokens<2, 2, true>(x, wp, quarter * 2, up, 2 * kGroup * kC * 2, usc, -sw, quarter, 4);
     put_tokens<2>(x, quarter, zp, zsc, a.z + (nv * groups + group) * 2 * kGroup * kC,
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
       }
     __syncwarp();
     put_tokens<2>(y, quarter, zp, zsc, nullptr, nullptr);
-    __syncthreads();
+    group_sync(pair);
     const float decay = gate[kC - 1];
 #pragma unroll
     for (int m = 0; m < MT; ++m)

@@ -607,14 +607,14 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
       }
       store_rows<2, 0>(xp, 2 * kGroup * kC, quarter * 2, y, inv, nullptr, 0);
     }
-    off = __syncthreads_or(off);
-    if (off) {  // rare, and the same for the whole CTA
+    off = group_sync_or(pair, off);
+    if (off) {  // rare, and the same for the whole group
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (!finite(x[n][e])) atomicMin(first + pair * kGroup + frag_col(n * 8) + (e & 1), row[e >> 1]);
-      __syncthreads();
+      group_sync(pair);
     }
     // E
     times_tokens<2, 2, false>(x, wp, quarter * 2, xp, 2 * kGroup * kC * 2, xsc, -sw, 0, quarter + 1);
@@ -645,8 +645,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
       __syncwarp();
       store_rows<2, 0>(yp, 2 * kGroup * kC, quarter * 2, x, inv, nullptr, 0);
     }
-    __syncthreads();
-    if (off && threadIdx.x < kSlice) first[threadIdx.x] = kC;
+    group_sync(pair);
+    if (off && (threadIdx.x & 127) < kGroup) first[pair * kGroup + (threadIdx.x & 127)] = kC;
     const float decay = gate[kC - 1];
 #pragma unroll
     for (int m = 0; m < MT; ++m)

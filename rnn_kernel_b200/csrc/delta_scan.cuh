@@ -16,6 +16,22 @@ __device__ __forceinline__ int quarter_of(int thread) {
   return (warp & 4 ? ~warp : warp) & 3;
 }
 
+// Barriers of the four warps that share value columns: what one group writes the
+// other never reads, and groups apart from one another use the SM's pipes in turn.
+__device__ __forceinline__ void group_sync(int pair) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(pair + 1) : "memory"); }
+__device__ __forceinline__ bool group_sync_or(int pair, bool x) {
+  int y;
+  asm volatile(
+      "{\n.reg .pred p, q;\n"
+      "setp.ne.s32 p, %1, 0;\n"
+      "barrier.cta.red.or.pred q, %2, 128, p;\n"
+      "selp.s32 %0, 1, 0, q;\n}"
+      : "=r"(y)
+      : "r"((int)x), "r"(pair + 1)
+      : "memory");
+  return y != 0;
+}
+
 // x (16 tokens x 16 columns) = K S of this warp's tokens; S as planes with a
 // scale for each quarter of its rows.
 template <int NP, int DK>
