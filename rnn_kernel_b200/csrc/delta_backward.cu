@@ -31,7 +31,8 @@ namespace {
 // scan: one CTA per (batch, value head, 32 value columns), last chunk first, in
 // the forward scan's division of work: eight warps, four quarters of the rows x
 // two groups of 16 columns, dS in registers, planes through shared memory
-// between three barriers a chunk.
+// between three barriers a chunk (2048 chunks of heads of 128 x 128, bf16: 225 us;
+// bound by the chain of four dependent products a chunk).
 // ---------------------------------------------------------------------------
 
 template <int NP, int DK, int STAGES>
@@ -230,8 +231,10 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
 // or two steps loading meanwhile.  A warp keeps 16 tokens x 32 key columns of
 // dQ, dK_row and dK_col, and of 16 or 32 tokens of dO U^T and Z U^T, in
 // registers: sixteen warps for 128 key columns, eight for 64, where two CTAs
-// then share an SM (2048 chunks of heads of 64, FP32: 170 us, against 205 with
-// sixteen warps of half the tile; of 128, bf16: 334 us).
+// then share an SM (2048 chunks of heads of 64, FP32: 165 us, with sixteen warps
+// of half the tile a fifth more; of 128, bf16: 299 us).  Bound by the latency of
+// products and barriers; the tensor pipe is a third busy, the most of any of
+// these kernels.
 // ---------------------------------------------------------------------------
 
 template <int NP, int DK>

@@ -36,7 +36,7 @@ struct Range {
 // a small grid one for each of those.
 // Latency-bound (a chain of small products between barriers), so it keeps its
 // shared memory small enough for several CTAs on an SM (2048 chunks of heads of
-// 128, two to a key head: 67 us).
+// 128, two to a key head: 64 us).
 // ---------------------------------------------------------------------------
 
 constexpr int kLd = 68;  // row length of the FP32 64 x 64 tiles: a multiple of 4, not of 32
@@ -482,8 +482,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
 // Eight warps: four quarters of the rows (tokens, or key columns of the state)
 // x two groups of 16 columns.  The state stays in registers as FP32
 // accumulators; its planes, those of B R and of U go through shared memory
-// between three barriers a chunk, every warp's quarter with its own scale, so
-// that no scale needs an exchange of its own.  K, W and the gates are loaded a
+// between three barriers a chunk (two of them among a group's four warps only),
+// every warp's quarter with its own scale, so that no scale needs an exchange of
+// its own.  K, W and the gates are loaded a
 // chunk ahead; so are the warp's values of V, into registers.
 //
 // Bound by the chain of three dependent products a chunk (2.6 us at 128 x 128,
@@ -673,7 +674,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
 // output: one CTA per (batch, value head, chunk), 64 value columns at a time; a
 // warp takes 16 tokens x 32 columns.  bf16 outputs take the first plane only
 // (2^-12 of the operands' size, against 2^-9 from rounding the output), which
-// halves the reading: it is bound by memory.
+// halves the reading (2048 chunks of heads of 128 x 128: 47 us).  Bound by the
+// latency of its loads: memory is a quarter busy, the tensor pipe a fifth.
 // ---------------------------------------------------------------------------
 
 template <typename T, int DK>
