@@ -35,7 +35,7 @@ _ENTRY = np.dtype([("param", "u8"), ("grad", "u8"), ("n", "i8"), ("state_offset"
 
 _address = torch.Tensor.data_ptr
 _is_dense = torch.Tensor.is_contiguous
-_gradient, _dtype = operator.attrgetter("grad"), operator.attrgetter("dtype")
+_gradient, _dtype, _bytes = operator.attrgetter("grad"), operator.attrgetter("dtype"), operator.attrgetter("nbytes")
 
 
 class _TypeTable:
@@ -51,13 +51,15 @@ class _TypeTable:
         self.entries = np.zeros(len(self.index), dtype=_ENTRY)
         self.entries["n"], self.entries["state_offset"] = opt._sizes[self.index], opt._offsets[self.index]
         self.address = self.entries.ctypes.data
+        self.bytes = list(map(_bytes, self.params))
         self.addresses: list = []  # of the parameters, as in the entries
         self.copies = None         # dense copies of gradients that are not, until the launch
 
     def gather(self, device: torch.device) -> Optional[np.ndarray]:
         """Fills in this step's addresses; the mask of parameters without a gradient, None where all have one."""
         addresses = list(map(_address, self.params))
-        if addresses != self.addresses:
+        # a new .data may lie where the old one did
+        if addresses != self.addresses or not all(map(_is_dense, self.params)):
             for p, n in zip(self.params, self.entries["n"].tolist()):
                 if p.dtype != self.dtype or p.numel() != n or p.device != device or not p.is_contiguous():
                     raise RuntimeError("AdamW: a parameter's type, size, device or layout has changed.")
@@ -65,7 +67,8 @@ class _TypeTable:
         grads = list(map(_gradient, self.params))
         try:
             where = np.fromiter(map(_address, grads), np.uint64, len(grads))
-            if all(map(_is_dense, grads)) and set(map(_dtype, grads)) == {self.dtype}:
+            if (all(map(_is_dense, grads)) and list(map(_bytes, grads)) == self.bytes
+                    and set(map(_dtype, grads)) == {self.dtype}):
                 self.entries["grad"] = where
                 return None
         except TypeError:  # None has no address
@@ -74,6 +77,8 @@ class _TypeTable:
         have = [g for g in grads if g is not None]
         if any(g.layout is not torch.strided or g.dtype != self.dtype for g in have):
             raise RuntimeError("AdamW: gradients must be dense and of their parameter's type.")
+        if any(g is not None and g.nbytes != n for g, n in zip(grads, self.bytes)):
+            raise RuntimeError("AdamW: a gradient's size is not what its parameter's was.")
         self.copies = grads = [g if g is None else g.contiguous() for g in grads]
         self.entries["grad"] = [0 if g is None else g.data_ptr() for g in grads]
         return without if without.any() else None

@@ -354,3 +354,26 @@ def test_trainer_learns_with_adamw(make, bits):
             losses[graphed] = [float(trainer.step(x, y)) for _ in range(40)][2:]
     assert losses[False][-1] < 0.8 * losses[False][0]
     np.testing.assert_allclose(losses[True], losses[False], rtol=1e-3)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_that_become_others_in_the_same_place_are_refused(bits):
+    """A new .data may begin where the old one did, with other sizes or strides."""
+    def fresh():
+        p = [torch.nn.Parameter(torch.randn(12, 30, device="cuda")), torch.nn.Parameter(torch.randn(7, device="cuda"))]
+        opt = AdamW(p, lr=0.1, state_bits=bits)
+        for x in p:
+            x.grad = torch.randn_like(x)
+        opt.step()
+        return p, opt
+
+    for change in (lambda x: x.t(), lambda x: x[:5], lambda x: x[:, :10]):
+        p, opt = fresh()
+        p[0].grad = None
+        p[0].data = change(p[0].data)
+        p[0].grad = torch.randn(p[0].shape, device="cuda")
+        before = [x.detach().clone() for x in p]
+        with pytest.raises(RuntimeError, match="changed|size"):
+            opt.step()
+        assert all(torch.equal(a, b) for a, b in zip(before, p))
+
