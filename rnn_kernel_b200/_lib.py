@@ -191,6 +191,13 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         return lib
 
 
+def host():
+    """The Python module of csrc/host_tensors.cpp, built with the library."""
+    load()
+    from . import _host
+    return _host
+
+
 def last_error() -> str:
     msg = load().gru_last_error()
     return msg.decode() if msg else ""

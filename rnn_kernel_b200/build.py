@@ -3,13 +3,17 @@
 ``python -m rnn_kernel_b200.build`` (or ``build()``) compiles every ``.cu`` in
 ``csrc/`` with nvcc into one shared library next to this file.  The library
 has a plain C ABI (``include/rnn_kernel_b200.h``) and is loaded with ctypes.
+``csrc/host_tensors.cpp`` becomes the Python module ``_host`` beside it, which
+reads torch tensors' addresses and is built against the installed torch.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -24,6 +28,7 @@ if VARIANT not in ("", "timeline"):
     raise ValueError(f"RNN_KERNEL_B200_VARIANT must be unset or 'timeline', got {VARIANT!r}")
 LIB_NAME = "librnn_kernel_b200_timeline.so" if VARIANT else "librnn_kernel_b200.so"
 LIB_PATH = PKG / LIB_NAME
+HOST_SOURCE, HOST_PATH = CSRC / "host_tensors.cpp", PKG / "_host.so"
 VARIANT_FLAGS = ["-DGRU_TIMELINE"] if VARIANT == "timeline" else []
 
 NVCC_FLAGS = [
@@ -45,16 +50,41 @@ def sources() -> list[Path]:
     return sorted(CSRC.glob("*.cu"))
 
 
-def needs_build() -> bool:
-    if not LIB_PATH.exists():
+def _stale(built: Path, deps) -> bool:
+    if not built.exists():
         return True
-    mtime = LIB_PATH.stat().st_mtime
-    deps = list(CSRC.glob("*")) + list((ROOT / "include").glob("*.h"))
-    return any(p.stat().st_mtime > mtime for p in deps)
+    mtime = built.stat().st_mtime
+    return any(p.stat().st_mtime > mtime for p in [*deps, *(ROOT / "include").glob("*.h")])
+
+
+def _needs_library() -> bool:
+    return _stale(LIB_PATH, CSRC.glob("*.cu*"))
+
+
+def _needs_host() -> bool:
+    return _stale(HOST_PATH, [HOST_SOURCE])
+
+
+def needs_build() -> bool:
+    return _needs_library() or _needs_host()
+
+
+def _build_host(verbose: bool) -> None:
+    torch = Path(importlib.util.find_spec("torch").origin).parent
+    tmp = HOST_PATH.with_suffix(".so.tmp")
+    include = [torch / "include", torch / "include/torch/csrc/api/include", sysconfig.get_paths()["include"]]
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{i}" for i in include), str(HOST_SOURCE),
+           f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-o", str(tmp)]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, HOST_PATH)
 
 
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> Path:
-    if not force and not needs_build():
+    if force or _needs_host():
+        _build_host(verbose)
+    if not force and not _needs_library():
         return LIB_PATH
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [nvcc_path(), *NVCC_FLAGS, *VARIANT_FLAGS, *(extra or []), "-I", str(ROOT / "include"),

@@ -17,7 +17,6 @@ fallback.
 from __future__ import annotations
 
 import math
-import operator
 from typing import Iterable, Optional
 
 import numpy as np
@@ -33,11 +32,6 @@ _ENTRY = np.dtype([("param", "u8"), ("grad", "u8"), ("n", "i8"), ("state_offset"
                    ("step_size", "f4"), ("inv_sqrt_bc2", "f4"), ("pad", "f4")])
 
 
-_address = torch.Tensor.data_ptr
-_is_dense = torch.Tensor.is_contiguous
-_gradient, _dtype, _bytes = operator.attrgetter("grad"), operator.attrgetter("dtype"), operator.attrgetter("nbytes")
-
-
 class _TypeTable:
     """The C call's table of the parameters of one element type."""
 
@@ -51,35 +45,27 @@ class _TypeTable:
         self.entries = np.zeros(len(self.index), dtype=_ENTRY)
         self.entries["n"], self.entries["state_offset"] = opt._sizes[self.index], opt._offsets[self.index]
         self.address = self.entries.ctypes.data
-        self.bytes = list(map(_bytes, self.params))
-        self.addresses: list = []  # of the parameters, as in the entries
-        self.copies = None         # dense copies of gradients that are not, until the launch
+        self.addresses = _lib.host().adamw_addresses
+        self.copies = None  # dense copies of gradients that are not, until the launch
 
     def gather(self, device: torch.device) -> Optional[np.ndarray]:
         """Fills in this step's addresses; the mask of parameters without a gradient, None where all have one."""
-        addresses = list(map(_address, self.params))
+        if self.addresses(self.params, self.address, self.code, device.index):
+            return None
+        grads = []
         # a new .data may lie where the old one did
-        if addresses != self.addresses or not all(map(_is_dense, self.params)):
-            for p, n in zip(self.params, self.entries["n"].tolist()):
-                if p.dtype != self.dtype or p.numel() != n or p.device != device or not p.is_contiguous():
-                    raise RuntimeError("AdamW: a parameter's type, size, device or layout has changed.")
-            self.entries["param"] = self.addresses = addresses
-        grads = list(map(_gradient, self.params))
-        try:
-            where = np.fromiter(map(_address, grads), np.uint64, len(grads))
-            if (all(map(_is_dense, grads)) and list(map(_bytes, grads)) == self.bytes
-                    and set(map(_dtype, grads)) == {self.dtype}):
-                self.entries["grad"] = where
-                return None
-        except TypeError:  # None has no address
-            pass
+        for p, n in zip(self.params, self.entries["n"].tolist()):
+            if p.dtype != self.dtype or p.numel() != n or p.device != device or not p.is_contiguous():
+                raise RuntimeError("AdamW: a parameter's type, size, device or layout has changed.")
+            g = p.grad
+            if g is not None and (g.layout is not torch.strided or g.dtype != self.dtype or g.device != device):
+                raise RuntimeError("AdamW: gradients must be dense and of their parameter's type.")
+            if g is not None and g.numel() != n:
+                raise RuntimeError("AdamW: a gradient's size is not what its parameter's was.")
+            grads.append(g)
         without = np.array([g is None for g in grads])
-        have = [g for g in grads if g is not None]
-        if any(g.layout is not torch.strided or g.dtype != self.dtype for g in have):
-            raise RuntimeError("AdamW: gradients must be dense and of their parameter's type.")
-        if any(g is not None and g.nbytes != n for g, n in zip(grads, self.bytes)):
-            raise RuntimeError("AdamW: a gradient's size is not what its parameter's was.")
         self.copies = grads = [g if g is None else g.contiguous() for g in grads]
+        self.entries["param"] = [p.data_ptr() for p in self.params]
         self.entries["grad"] = [0 if g is None else g.data_ptr() for g in grads]
         return without if without.any() else None
 
