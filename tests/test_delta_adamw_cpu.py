@@ -106,3 +106,24 @@ def test_layer_state_dict_names():
     layer = GatedDelta(16, num_heads=4, head_size=8, num_key_heads=2, output_size=5)
     assert {k: tuple(v.shape) for k, v in layer.state_dict().items()} == {
         "in_proj.weight": (2 * 2 * 8 + 4 * 8 + 8, 16), "out_proj.weight": (5, 32), "norm_weight": (8,), "log_rate": (4,)}
+
+
+def test_tensor_addresses_only_of_what_the_table_holds():
+    """The C++ reader of parameters refuses, and reads nothing of, what is not a CUDA tensor of the entry's size."""
+    import numpy as np
+
+    from rnn_kernel_b200 import _lib, optim
+
+    read = _lib.host().adamw_addresses
+    p = torch.nn.Parameter(torch.zeros(5))
+    p.grad = torch.zeros(5)
+    entries = np.zeros(1, dtype=optim._ENTRY)
+    entries["n"] = 5
+    before = entries.copy()
+    assert read([p], entries.ctypes.data, _lib.GRU_F32, 0) is False  # not on the device
+    assert read(["p"], entries.ctypes.data, _lib.GRU_F32, 0) is False
+    assert read([], entries.ctypes.data, _lib.GRU_F32, 0) is True
+    assert (entries == before).all()
+    with pytest.raises(TypeError):
+        read((p,), entries.ctypes.data, _lib.GRU_F32, 0)
+
