@@ -110,10 +110,6 @@ def test_layer_state_dict_names():
 
 def test_tensor_addresses_only_of_what_the_table_holds():
     """The C++ reader of parameters refuses, and reads nothing of, what is not a CUDA tensor of the entry's size."""
-    import numpy as np
-
-    from rnn_kernel_b200 import _lib, optim
-
     read = _lib.host().adamw_addresses
     p = torch.nn.Parameter(torch.zeros(5))
     p.grad = torch.zeros(5)
