@@ -66,7 +66,7 @@ __device__ __forceinline__ void put_tokens(const float (&x)[2][4], int quarter, 
     scale[quarter] = plane_scale(inv);
     if (out) out_scale[quarter] = plane_scale(inv);
   }
-  store_rows<NP, NP>(tile, 2 * kGroup * kC, quarter * 2, x, inv, out, kGroup * kC);
+  store_rows<NP>(tile, 2 * kGroup * kC, quarter * 2, x, inv, out, kGroup * kC);
 }
 
 // STAGES: with two the next chunk's tiles load during this one; with one they
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
   };
   auto state_out = [&](int chunk) {
     const long nv = nv0 + chunk;
-    put_state<DK, 2>(d, quarter, sp, ssc, chunk >= 0 ? a.dstates + (nv * groups + group) * 2 * kGroup * DK : nullptr,
+    put_state<DK>(d, quarter, sp, ssc, chunk >= 0 ? a.dstates + (nv * groups + group) * 2 * kGroup * DK : nullptr,
                      a.dsscale + (nv * groups + group) * 4);
   };
   back_load<NP, DK>(smem, a, nk0 + a.nc - 1, nv0 + a.nc - 1);
@@ -285,11 +285,6 @@ __device__ __forceinline__ float2 take2(const f16* p, int plane, int word) {
     f.y += l.y;
   }
   return f;
-}
-__device__ __forceinline__ float2 pair(uint32_t h, uint32_t l) {
-  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h));
-  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&l));
-  return make_float2(x.x + y.x, x.y + y.y);
 }
 
 // acc += A B, one step of 16, times f0 (the first half of the tiles) or f1.

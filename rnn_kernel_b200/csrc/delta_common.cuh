@@ -72,10 +72,9 @@ struct Problem {
   f16* wp;       // [n over Hv][2][64 x 64]
   f16* pp;       // [n over Hv][2][64 x 64]
   float* gates;  // [n over Hv][kGates][64]
-  int planes;    // of states and e in memory: 2, or 1 where only a bf16 output reads them
-  // Tiles of 16 value columns each, [n over Hv][group][plane][rows x 16], rows
-  // the key columns of a state or the tokens; every quarter of a tile's rows
-  // has its own scale, [n over Hv][group][4].
+  // Tiles of 16 value columns each, [n over Hv][group][2][rows x 16], rows the
+  // key columns of a state or the tokens; every quarter of a tile's rows has its
+  // own scale, [n over Hv][group][4].
   f16* states;   // the state before the chunk
   float* sscale;
   f16* e;        // v - S'^T k, so that u = beta e
@@ -252,6 +251,13 @@ __device__ __forceinline__ void split2(float a, float b, float inv, uint32_t (&w
   }
 }
 
+// The numbers that two packed planes stand for.
+__device__ __forceinline__ float2 pair(uint32_t h, uint32_t l) {
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&l));
+  return make_float2(x.x + y.x, x.y + y.y);
+}
+
 // The larger of m and |x|; a NaN wins.
 __device__ __forceinline__ float max_mag(float m, float x) {
   float y;
@@ -293,10 +299,10 @@ __device__ __forceinline__ float warp_max(const float (&x)[NT][4]) {
 }
 
 // Writes 16 rows (from row block r8) x 16 columns of accumulators, times inv, as
-// NP planes of a tile of 16 columns in shared memory (`plane` elements apart);
-// the first PO of them also into `out`, if given, 16 bytes a lane.  Four blocks
-// of 128 consecutive bytes, which is what stmatrix writes at once.
-template <int NP, int PO>
+// NP planes of a tile of 16 columns in shared memory (`plane` elements apart),
+// and into `out`, if given, 16 bytes a lane.  Four blocks of 128 consecutive
+// bytes, which is what stmatrix writes at once.
+template <int NP>
 __device__ __forceinline__ void store_rows(f16* tile, int plane, int r8, const float (&x)[2][4], float inv, f16* out,
                                            int out_plane) {
   uint32_t w[2][2][NP];
@@ -313,7 +319,7 @@ __device__ __forceinline__ void store_rows(f16* tile, int plane, int r8, const f
   if (out) {
     __syncwarp();
 #pragma unroll
-    for (int p = 0; p < PO; ++p)
+    for (int p = 0; p < NP; ++p)
       *reinterpret_cast<uint4*>(out + p * out_plane + at) = *reinterpret_cast<const uint4*>(tile + p * plane + at);
   }
 }

@@ -512,8 +512,7 @@ __device__ __forceinline__ void scan_load(unsigned char* stage, const Problem& a
   cp_async_commit();
 }
 
-// PO: planes of the states and errors that are kept.
-template <typename T, int DK, int PO>
+template <typename T, int DK>
 __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a, const Range range) {
   constexpr int NP = Planes<T>::n, MT = DK / 64;
   using L = ScanSmem<NP, DK>;
@@ -555,8 +554,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
   };
   auto state_out = [&](int chunk) {
     const long nv = nv0 + chunk;
-    put_state<DK, PO>(s, quarter, sp, ssc, chunk < range.first + range.n ? a.states + (nv * groups + group) * PO * kGroup * DK : nullptr,
-                      a.sscale + (nv * groups + group) * 4);
+    put_state<DK>(s, quarter, sp, ssc, chunk < range.first + range.n ? a.states + (nv * groups + group) * 2 * kGroup * DK : nullptr,
+                  a.sscale + (nv * groups + group) * 4);
   };
   const int end = range.first + range.n;
   load_v(range.first);
@@ -606,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
 #pragma unroll
           for (int e = 0; e < 4; ++e) y[n][e] = finite(y[n][e]) && finite(x[n][e]) ? y[n][e] : 0.0f;
       }
-      store_rows<2, 0>(xp, 2 * kGroup * kC, quarter * 2, y, inv, nullptr, 0);
+      store_rows<2>(xp, 2 * kGroup * kC, quarter * 2, y, inv, nullptr, 0);
     }
     off = group_sync_or(pair, off);
     if (off) {  // rare, and the same for the whole group
@@ -632,8 +631,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
       const float inv = plane_inv(warp_max(x, all_finite));
       // a scale below zero marks a quarter that holds something not finite
       if (lane == 0) a.escale[(nv * groups + group) * 4 + quarter] = all_finite ? plane_scale(inv) : -plane_scale(inv);
-      f16* out = a.e + (nv * groups + group) * PO * kGroup * kC;
-      store_rows<PO, PO>(yp, 2 * kGroup * kC, quarter * 2, x, inv, out, kGroup * kC);  // yp: on the way only
+      f16* out = a.e + (nv * groups + group) * 2 * kGroup * kC;
+      store_rows<2>(yp, 2 * kGroup * kC, quarter * 2, x, inv, out, kGroup * kC);  // yp: on the way only
     }
     // S <- e^G S + K^T (e^(G_end - G) U)
     {
@@ -644,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
       const float inv = plane_inv(warp_max(x));
       if (lane == 0) ysc[quarter] = plane_scale(inv);
       __syncwarp();
-      store_rows<2, 0>(yp, 2 * kGroup * kC, quarter * 2, x, inv, nullptr, 0);
+      store_rows<2>(yp, 2 * kGroup * kC, quarter * 2, x, inv, nullptr, 0);
     }
     group_sync(pair);
     if (off && (threadIdx.x & 127) < kGroup) first[pair * kGroup + (threadIdx.x & 127)] = kC;
@@ -672,18 +671,17 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
 
 // ---------------------------------------------------------------------------
 // output: one CTA per (batch, value head, chunk), 64 value columns at a time; a
-// warp takes 16 tokens x 32 columns.  bf16 outputs take the first plane only
-// (2^-12 of the operands' size, against 2^-9 from rounding the output), which
-// halves the reading (2048 chunks of heads of 128 x 128: 47 us).  Bound by the
-// latency of its loads: memory is a quarter busy, the tensor pipe a fifth.
+// warp takes 16 tokens x 32 columns.  Every operand keeps both planes, whatever
+// the output's type: an FP32 result is rounded once, when it is stored (one
+// plane of each, 2^-12 of the operands' size, moved a tenth of the bf16 outputs
+// by their last bit).  Bound by the latency of its loads.
 // ---------------------------------------------------------------------------
 
 template <typename T, int DK>
 struct OutputSmem {
-  static constexpr int NP = Planes<T>::n;  // planes used, of every operand
   static constexpr int cols = 64;
-  static constexpr int q = NP * kC * DK, p = NP * kTile;  // elements
-  static constexpr int s = NP * cols * DK, e = NP * cols * kC;
+  static constexpr int q = Planes<T>::n * kC * DK, p = 2 * kTile;  // elements
+  static constexpr int s = 2 * cols * DK, e = 2 * cols * kC;
   static constexpr int slice = s + e + 2 * 32;  // and the scales of S and E, four groups and quarters
   static constexpr int buffers = (q + p + 2 * slice) * 2 > 96 * 1024 ? 1 : 2;
   static constexpr int bytes = (q + p + buffers * slice) * 2 + kGates * kC * 4;
@@ -693,12 +691,11 @@ template <typename T, int DK>
 __device__ __forceinline__ void output_load(f16* dst, const Problem& a, long nv, int c0) {
   using L = OutputSmem<T, DK>;
   const long first = nv * (a.dvp / kGroup) + c0 / kGroup;
-  // of both planes of a group in memory the first NP, in the order [group][plane]
 #pragma unroll
   for (int g = 0; g < L::cols / kGroup; ++g) {
     if (c0 + g * kGroup >= a.dvp) break;
-    copy_async<L::NP * kGroup * DK * 2, kThreads>(dst + g * L::NP * kGroup * DK, a.states + (first + g) * a.planes * kGroup * DK);
-    copy_async<L::NP * kGroup * kC * 2, kThreads>(dst + L::s + g * L::NP * kGroup * kC, a.e + (first + g) * a.planes * kGroup * kC);
+    copy_async<2 * kGroup * DK * 2, kThreads>(dst + g * 2 * kGroup * DK, a.states + (first + g) * 2 * kGroup * DK);
+    copy_async<2 * kGroup * kC * 2, kThreads>(dst + L::s + g * 2 * kGroup * kC, a.e + (first + g) * 2 * kGroup * kC);
   }
   if (threadIdx.x < 8) {
     const int g = threadIdx.x & 3;
@@ -708,22 +705,14 @@ __device__ __forceinline__ void output_load(f16* dst, const Problem& a, long nv,
   cp_async_commit();
 }
 
-// acc (two groups of 16 columns, NP * `tile` elements each) += A B, one step of
-// 16; both groups' scales are scale[0] and scale[4].  A bf16 output adds
-// consecutive steps of one scale up on the tensor core: `begin` and `end` say
-// where such a run does.
-template <int NP, int TILE>
-__device__ __forceinline__ void output_step(float (&acc)[4][4], float (&t)[4][4], const uint32_t (&fa)[NP][4], uint32_t pb,
-                                            const float* scale, bool begin, bool end) {
-  uint32_t fb[NP][4][2];
-  load_b<NP, 4, true>(fb, pb, NP * TILE * 2, TILE * 2);
-  if (NP == 1 && !begin) {
-#pragma unroll
-    for (int n = 0; n < 4; ++n) mma(t[n], fa[0], fb[0][n][0], fb[0][n][1]);
-  } else {
-    mma_terms<NP, NP, 4>(t, fa, fb);
-  }
-  if (NP == 1 && !end) return;
+// acc (two groups of 16 columns) += A B, one step of 16; both groups' scales are
+// scale[0] and scale[4].
+template <int NA, int TILE>
+__device__ __forceinline__ void output_step(float (&acc)[4][4], const uint32_t (&fa)[NA][4], uint32_t pb, const float* scale) {
+  uint32_t fb[2][4][2];
+  load_b<2, 4, true>(fb, pb, 2 * TILE * 2, TILE * 2);
+  float t[4][4];
+  mma_terms<NA, 2, 4>(t, fa, fb);
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
     const float f = scale[(n >> 1) * 4];
@@ -734,7 +723,6 @@ __device__ __forceinline__ void output_step(float (&acc)[4][4], float (&t)[4][4]
 
 // An element of P U (without the scales of P and B), for a chunk with an error that is not
 // finite: the zeros of P above its diagonal would spread it to earlier tokens.
-template <int NP>
 __device__ __noinline__ float output_element(const f16* pp, const f16* ep, int plane, const float* scale,
                                              int i, int c) {
   float sum = 0.0f;
@@ -742,7 +730,7 @@ __device__ __noinline__ float output_element(const f16* pp, const f16* ep, int p
     const int ip = ((i >> 3) * 8 + (j >> 3)) * 64 + (i & 7) * 8 + (j & 7);
     const int ie = ((j >> 3) * 2 + (c >> 3)) * 64 + (j & 7) * 8 + (c & 7);
     float u = 0.0f, w = 0.0f;
-    for (int p = 0; p < NP; ++p) {
+    for (int p = 0; p < 2; ++p) {
       u += __half2float(pp[p * kTile + ip]);
       w += __half2float(ep[p * plane + ie]);
     }
@@ -766,7 +754,7 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
   const long nv = (long)bh * a.nc + chunk, nk = ((long)b * a.Hk + hv / a.rep) * a.nc + chunk;
   wait_for_before();
   copy_async<L::q * 2, kThreads>(qp, a.qp + nk * L::q);
-  copy_async<L::p * 2, kThreads>(pp, a.pp + nv * 2 * kTile);
+  copy_async<L::p * 2, kThreads>(pp, a.pp + nv * L::p);
   copy_async<kGates * kC * 4, kThreads>(gate, a.gates + nv * kGates * kC);
   output_load<T, DK>(slices, a, nv, 0);
   const int warp = threadIdx.x >> 5;
@@ -786,27 +774,21 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
       for (int i = 0; i < 2; ++i) {
         const int row = threadIdx.x + i * kThreads;  // of 8 elements
         const float* be = gate + 2 * kC + ((row >> 3) & 7) * 8;
-        uint32_t r[NP][4];
+        uint32_t r[2][4];
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
+        for (int p = 0; p < 2; ++p) {
           const uint4 u = reinterpret_cast<const uint4*>(pp + p * kTile)[row];
           r[p][0] = u.x, r[p][1] = u.y, r[p][2] = u.z, r[p][3] = u.w;
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r[0][j]));
-          if (NP == 2) {
-            const float2 l = __half22float2(*reinterpret_cast<const __half2*>(&r[NP - 1][j]));
-            f.x += l.x;
-            f.y += l.y;
-          }
-          uint32_t w[NP];
-          split2<NP>(f.x * be[2 * j], f.y * be[2 * j + 1], ib, w);
-#pragma unroll
-          for (int p = 0; p < NP; ++p) r[p][j] = w[p];
+          const float2 f = pair(r[0][j], r[1][j]);
+          uint32_t w[2];
+          split2<2>(f.x * be[2 * j], f.y * be[2 * j + 1], ib, w);
+          r[0][j] = w[0], r[1][j] = w[1];
         }
 #pragma unroll
-        for (int p = 0; p < NP; ++p)
+        for (int p = 0; p < 2; ++p)
           reinterpret_cast<uint4*>(pp + p * kTile)[row] = make_uint4(r[p][0], r[p][1], r[p][2], r[p][3]);
       }
       __syncthreads();
@@ -821,21 +803,20 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
     if (cw < a.dvp) {
       const float* fs = reinterpret_cast<const float*>(ep + L::e) + half * 8;
       const float* fe = fs + 16;
-      const f16* sg = sp + half * 2 * NP * kGroup * DK;
-      const f16* eg = ep + half * 2 * NP * kGroup * kC;
+      const f16* sg = sp + half * 4 * kGroup * DK;
+      const f16* eg = ep + half * 4 * kGroup * kC;
       float x[4][4], y[4][4];
       zero(x);
       zero(y);
       {
         const uint32_t pa = addr_a<DK, false>(qp, m0 / 8, 0), pb = addr_b<kGroup, true>(sg, 0, 0);
         constexpr int per = DK / 64;  // steps to a scale
-        float t[4][4];
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
           uint32_t fa[NP][4];
 #pragma unroll
           for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], pa + kk * 256 + p * kC * DK * 2);
-          output_step<NP, kGroup * DK>(x, t, fa, pb + kk * 512, fs + kk / per, kk % per == 0, kk % per == per - 1);
+          output_step<NP, kGroup * DK>(x, fa, pb + kk * 512, fs + kk / per);
         }
       }
       bool lost = false;
@@ -847,18 +828,17 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
         for (int n = 0; n < 4; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            y[n][e] = output_element<NP>(pp, eg + (n >> 1) * NP * kGroup * kC, kGroup * kC, fe + (n >> 1) * 4,
+            y[n][e] = output_element(pp, eg + (n >> 1) * 2 * kGroup * kC, kGroup * kC, fe + (n >> 1) * 4,
                                          frag_row(m0, e >> 1), frag_col((n & 1) * 8) + (e & 1));
       } else {
         const uint32_t pa = addr_a<kC, false>(pp, m0 / 8, 0), pb = addr_b<kGroup, true>(eg, 0, 0);
-        float t[4][4];
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           if (kk > m0 / 16) break;
-          uint32_t fa[NP][4];
+          uint32_t fa[2][4];
 #pragma unroll
-          for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], pa + kk * 256 + p * kTile * 2);
-          output_step<NP, kGroup * kC>(y, t, fa, pb + kk * 512, fe + kk, true, true);
+          for (int p = 0; p < 2; ++p) ldm4<false>(fa[p], pa + kk * 256 + p * kTile * 2);
+          output_step<2, kGroup * kC>(y, fa, pb + kk * 512, fe + kk);
         }
       }
       const float fx = a.scale * gate[5 * kC + 3];
@@ -894,14 +874,14 @@ int run_prepare(const Problem& a, Range r, cudaStream_t stream) {
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
 }
-template <typename T, int DK, int PO>
+template <typename T, int DK>
 int run_scan(const Problem& a, Range r, cudaStream_t stream) {
   constexpr int bytes = ScanSmem<Planes<T>::n, DK>::bytes;
-  if (const int rc = with_smem(delta_scan_kernel<T, DK, PO>, bytes)) return rc;
+  if (const int rc = with_smem(delta_scan_kernel<T, DK>, bytes)) return rc;
   LaunchScope scope(kKindDeltaRule, stream);
   const unsigned ctas = (unsigned)((long)a.B * a.Hv * (a.dvp / kSlice));
-  if (r.n == a.nc) return launch_after(delta_scan_kernel<T, DK, PO>, ctas, kThreads, bytes, stream, a, r);
-  delta_scan_kernel<T, DK, PO><<<ctas, kThreads, bytes, stream>>>(a, r);
+  if (r.n == a.nc) return launch_after(delta_scan_kernel<T, DK>, ctas, kThreads, bytes, stream, a, r);
+  delta_scan_kernel<T, DK><<<ctas, kThreads, bytes, stream>>>(a, r);
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
 }
@@ -929,10 +909,7 @@ constexpr int kEnds[] = {1, 3, 5, 6};  // of the ranges, in sixths of the chunks
 constexpr int kRanges = sizeof(kEnds) / sizeof(int);
 template <typename T, int DK>
 int forward_typed(const Problem& a, cudaStream_t stream) {
-  constexpr int least = Planes<T>::n;  // FP32 outputs read both planes
-  auto scan = [&](Range r) {
-    return a.planes == 2 ? run_scan<T, DK, 2>(a, r, stream) : run_scan<T, DK, least>(a, r, stream);
-  };
+  auto scan = [&](Range r) { return run_scan<T, DK>(a, r, stream); };
   int rc, device;
   Side* side = nullptr;
   if ((long)a.B * a.Hv * (a.dvp / kSlice) <= 148 && (long)a.B * a.Hv * a.nc >= 2048 && a.nc >= 16) {

@@ -111,9 +111,9 @@ __device__ __forceinline__ void add_to_state(float (&s)[DK / 64][2][4], const f1
   }
 }
 
-// Planes of this warp's quarter of the state into shared memory, and the first
-// PO of them into `out`, if any.
-template <int DK, int PO>
+// Planes of this warp's quarter of the state into shared memory, and into `out`,
+// if any.
+template <int DK>
 __device__ __forceinline__ void put_state(const float (&s)[DK / 64][2][4], int quarter, f16* sp, float* scale, f16* out,
                                           float* out_scale) {
   constexpr int MT = DK / 64;
@@ -142,7 +142,7 @@ __device__ __forceinline__ void put_state(const float (&s)[DK / 64][2][4], int q
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i)
-    store_rows<2, PO>(sp, 2 * kGroup * DK, (quarter * MT + i) * 2, s[i], inv, out, kGroup * DK);
+    store_rows<2>(sp, 2 * kGroup * DK, (quarter * MT + i) * 2, s[i], inv, out, kGroup * DK);
 }
 
 }  // namespace delta

@@ -197,19 +197,18 @@ void fill(Problem& a, const gru_delta_args& p) {
   a.scale = p.scale;
 }
 
-// What the forward computes; `keep`: for a gradient.
-void lay_forward(Problem& a, const gru_delta_args& p, Arena& m, bool keep) {
+// What the forward computes, and a training one keeps.
+void lay_forward(Problem& a, const gru_delta_args& p, Arena& m) {
   const size_t nk = (size_t)a.B * a.Hk * a.nc, nv = (size_t)a.B * a.Hv * a.nc, w = key_width(p);
   const size_t np = p.dtype == GRU_F32 ? 2 : 1, groups = a.dvp / kGroup;
-  a.planes = keep || p.dtype == GRU_F32 ? 2 : 1;
   a.kp = m.take<f16>(nk * np * kC * w);
   a.qp = m.take<f16>(nk * np * kC * w);
   a.wp = m.take<f16>(nv * 2 * kTile);
   a.pp = m.take<f16>(nv * 2 * kTile);
   a.gates = m.take<float>(nv * kGates * kC);
-  a.states = m.take<f16>(nv * a.planes * a.dvp * w);
+  a.states = m.take<f16>(nv * 2 * a.dvp * w);
   a.sscale = m.take<float>(nv * groups * 4);
-  a.e = m.take<f16>(nv * a.planes * a.dvp * kC);
+  a.e = m.take<f16>(nv * 2 * a.dvp * kC);
   a.escale = m.take<float>(nv * groups * 4);
 }
 
@@ -237,7 +236,7 @@ extern "C" size_t gru_delta_stash_bytes(const gru_delta_args* p) {
   Problem a{};
   fill(a, *p);
   Arena m{nullptr};
-  lay_forward(a, *p, m, true);
+  lay_forward(a, *p, m);
   return m.used;
 }
 
@@ -247,7 +246,7 @@ extern "C" size_t gru_delta_workspace_bytes(const gru_delta_args* p, int backwar
   fill(a, *p);
   Arena m{nullptr};
   if (backward) lay_backward(a, *p, m);
-  else lay_forward(a, *p, m, false);
+  else lay_forward(a, *p, m);
   return m.used;
 }
 
@@ -270,7 +269,7 @@ extern "C" int gru_delta_forward(const gru_delta_args* p, void* out, float* fina
   }
   if (!out || (reinterpret_cast<uintptr_t>(out) & (p->dtype == GRU_F32 ? 3 : 1))) return bad(me, "null or misaligned out");
   Arena m{static_cast<char*>(stash ? stash : workspace)};
-  lay_forward(a, *p, m, stash != nullptr);
+  lay_forward(a, *p, m);
   if (!m.base || (stash ? stash_bytes : workspace_bytes) < m.used || (reinterpret_cast<uintptr_t>(m.base) & 15))
     return bad(me, "stash (or workspace without one) too small or not 16-byte aligned");
   a.o = out;
@@ -303,7 +302,7 @@ extern "C" int gru_delta_backward(const gru_delta_args* p, const void* dout, con
         reinterpret_cast<uintptr_t>(dfinal)) & 3))
     return bad(me, "null gradient, or one not aligned to two of its elements");
   Arena s{static_cast<char*>(const_cast<void*>(stash))}, w{static_cast<char*>(workspace)};
-  lay_forward(a, *p, s, true);
+  lay_forward(a, *p, s);
   lay_backward(a, *p, w);
   if (!stash || stash_bytes < s.used || !workspace || workspace_bytes < w.used ||
       ((reinterpret_cast<uintptr_t>(stash) | reinterpret_cast<uintptr_t>(workspace)) & 15))
