@@ -44,9 +44,21 @@ class _TypeTable:
         self.groups = [(lo, hi, int(self.group[lo])) for lo, hi in zip(cuts[:-1], cuts[1:])]
         self.entries = np.zeros(len(self.index), dtype=_ENTRY)
         self.entries["n"], self.entries["state_offset"] = opt._sizes[self.index], opt._offsets[self.index]
+        self._bind()
+
+    def _bind(self) -> None:
+        """What belongs to this object alone: the address of its own entries, which a copy of it does not share."""
         self.address = self.entries.ctypes.data
         self.addresses = _lib.host().adamw_addresses
         self.copies = None  # dense copies of gradients that are not, until the launch
+
+    def __getstate__(self) -> dict:
+        # for copy.deepcopy and pickle: they make new entries, elsewhere
+        return {k: v for k, v in self.__dict__.items() if k not in ("address", "addresses", "copies")}
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        self._bind()
 
     def gather(self, device: torch.device) -> Optional[np.ndarray]:
         """Fills in this step's addresses; the mask of parameters without a gradient, None where all have one."""
