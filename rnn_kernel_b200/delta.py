@@ -24,6 +24,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import _lib
 from .gru import is_b200_available
@@ -113,8 +114,20 @@ def _forward(code, q, k, v, g, beta, state, scale, train):
     return out, last, memory
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    """Passes gradients on; their own derivative raises, where without it they would count as constants."""
+
+    @staticmethod
+    def forward(ctx, anchor, *grads):
+        return tuple(None if g is None else g.clone() for g in grads)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("gated_delta_rule has no second derivative.")
+
+
 class GatedDeltaRuleFunction(torch.autograd.Function):
-    """``(q, k, v, g, beta, state or None, scale) -> (out, last state)``."""
+    """``(q, k, v, g, beta, state or None, scale) -> (out, last state)``; first derivatives, by backward only."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, state, scale):
@@ -145,7 +158,14 @@ class GatedDeltaRuleFunction(torch.autograd.Function):
                 a, 0 if dout is None else dout.data_ptr(), 0 if dlast is None else dlast.data_ptr(), stash.data_ptr(),
                 stash_bytes, gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), gg.data_ptr(), gb.data_ptr(),
                 0 if gs is None else gs.data_ptr(), ws.data_ptr(), ws_bytes, _lib.raw_stream(dev)), "gru_delta_backward")
+        if torch.is_grad_enabled():  # create_graph=True
+            gq, gk, gv, gg, gb, gs = _NoSecondDerivative.apply(torch.empty(0, requires_grad=True), gq, gk, gv, gg, gb, gs)
         return gq, gk, gv, gg, gb, gs, None
+
+
+def _forward_mode() -> bool:
+    """Inside a dual level: tensors may carry tangents, under no_grad too."""
+    return forward_ad._current_level >= 0
 
 
 def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
@@ -158,7 +178,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     The other strides than the last dimension's are free.
     """
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or _forward_mode():  # which refuses tangents
         return GatedDeltaRuleFunction.apply(q, k, v, g, beta, initial_state, scale)
     code = _check("gated_delta_rule", q, k, v, g, beta, initial_state, 2)
     out, last, _ = _forward(code, q, k, v, g, beta, initial_state, scale, False)
@@ -172,6 +192,8 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     ``q``, ``k``: [B, Hk, dk]; ``v``: [B, Hv, dv]; ``g``, ``beta``: [B, Hv].  No gradient.
     """
     code = _check("gated_delta_step", q, k, v, g, beta, state, 1)
+    if _forward_mode() and any(forward_ad.unpack_dual(t).tangent is not None for t in (q, k, v, g, beta, state)):
+        raise RuntimeError("gated_delta_step has no derivative.")
     if not state.is_contiguous():
         raise ValueError("gated_delta_step: the state is updated in place and must be contiguous.")
     q, k, v = _dense_heads(q), _dense_heads(k), _dense_heads(v)
