@@ -178,7 +178,9 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     The other strides than the last dimension's are free.
     """
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    if torch.is_grad_enabled() or _forward_mode():  # which refuses tangents
+    needed = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
+    if needed or _forward_mode():  # the Function refuses tangents
         return GatedDeltaRuleFunction.apply(q, k, v, g, beta, initial_state, scale)
     code = _check("gated_delta_rule", q, k, v, g, beta, initial_state, 2)
     out, last, _ = _forward(code, q, k, v, g, beta, initial_state, scale, False)

@@ -40,3 +40,28 @@ def test_forward_mode_raises(no_grad):
             y = [t[:, 0] for t in y[:5]] + [y[5].clone() if i < 5 else y[5]]
             with pytest.raises(RuntimeError, match="derivative"):
                 gated_delta_step(*y)
+
+
+def test_without_a_gradient_to_keep_for_the_forward_keeps_nothing():
+    """Gradients enabled, but no input asks for one: no more memory than under no_grad, and outputs without a graph."""
+    x = R.inputs(2, 512, 2, 4, 64, 64, dtype=torch.bfloat16, seed=3)
+
+    def peak(grad):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        with torch.set_grad_enabled(grad):
+            out, last = gated_delta_rule(*x[:5], initial_state=x[5])
+        held = torch.cuda.memory_allocated() - before
+        return torch.cuda.max_memory_allocated() - before, held, out, last
+
+    _, _, out, last = peak(False)
+    top, held, *_ = peak(False)
+    top_g, held_g, out_g, last_g = peak(True)
+    assert (top_g, held_g) == (top, held)
+    assert not out_g.requires_grad and torch.equal(out_g, out) and torch.equal(last_g, last)
+    for i in range(6):  # one input that does is enough
+        y = [t.clone().requires_grad_(j == i) for j, t in enumerate(x)]
+        out_y, last_y = gated_delta_rule(*y[:5], initial_state=y[5])
+        assert out_y.requires_grad and last_y.requires_grad
+        assert torch.autograd.grad(out_y.sum() + last_y.sum(), y[i])[0].shape == y[i].shape
