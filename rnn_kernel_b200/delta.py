@@ -245,8 +245,9 @@ class GatedDelta(nn.Module):
     def _project(self, x):
         q, k, v, a, b = self.in_proj(x).split(self._split, dim=-1)
         keys, values = (self.num_key_heads, self.head_size), (self.num_heads, self.head_size)
-        q = F.normalize(q.unflatten(-1, keys).float(), dim=-1).to(x.dtype)
-        k = F.normalize(k.unflatten(-1, keys).float(), dim=-1).to(x.dtype)
+        # back to v's type, which under autocast is the projection's and not x's
+        q = F.normalize(q.unflatten(-1, keys).float(), dim=-1).to(v.dtype)
+        k = F.normalize(k.unflatten(-1, keys).float(), dim=-1).to(v.dtype)
         g = -self.log_rate.float().exp() * F.softplus(a.float())
         return q, k, v.unflatten(-1, values), g, b.float().sigmoid()
 
