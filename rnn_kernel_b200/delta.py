@@ -240,7 +240,8 @@ class GatedDelta(nn.Module):
         self.log_rate = nn.Parameter(torch.linspace(-5.0, 0.0, num_heads))
 
     def init_state(self, batch: int) -> torch.Tensor:
-        return torch.zeros(batch, self.num_heads, self.head_size, self.head_size, device=self.log_rate.device)
+        return torch.zeros(batch, self.num_heads, self.head_size, self.head_size, dtype=torch.float32,
+                           device=self.log_rate.device)
 
     def _project(self, x):
         q, k, v, a, b = self.in_proj(x).split(self._split, dim=-1)

@@ -20,6 +20,15 @@ def test_projection_gives_one_type_under_autocast():
     assert g.dtype == beta.dtype == torch.float32
 
 
+def test_state_is_fp32_under_another_default_type():
+    m = layer()
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        assert m.init_state(2).dtype == torch.float32
+    finally:
+        torch.set_default_dtype(torch.float32)
+
+
 def plain(m, x, state):
     """The layer in 64 bits from the parameters and inputs as they are."""
     p = {n: t.detach().double() for n, t in m.named_parameters()}
