@@ -8,6 +8,8 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import importlib.machinery
+import importlib.util
 import struct
 import threading
 from pathlib import Path
@@ -27,6 +29,7 @@ GRU_BF16 = 1
 
 _lock = threading.Lock()
 _lib = None
+_host = None
 
 _c_float_p = ctypes.c_void_p
 _size_t = ctypes.c_size_t
@@ -192,10 +195,16 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
 
 
 def host():
-    """The Python module of csrc/host_tensors.cpp, built with the library."""
-    load()
-    from . import _host
-    return _host
+    """The Python module of csrc/host_tensors.cpp (built first if needed); raises where it cannot be built or loaded."""
+    global _host
+    with _lock:
+        if _host is None:
+            path = str(_build.build_host())
+            loader = importlib.machinery.ExtensionFileLoader("_host", path)
+            module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_host", path, loader=loader))
+            loader.exec_module(module)
+            _host = module
+        return _host
 
 
 def last_error() -> str:

@@ -3,12 +3,14 @@
 ``python -m rnn_kernel_b200.build`` (or ``build()``) compiles every ``.cu`` in
 ``csrc/`` with nvcc into one shared library next to this file.  The library
 has a plain C ABI (``include/rnn_kernel_b200.h``) and is loaded with ctypes.
-``csrc/host_tensors.cpp`` becomes the Python module ``_host`` beside it, which
-reads torch tensors' addresses and is built against the installed torch.
+``csrc/host_tensors.cpp`` becomes the Python module ``_host`` beside it
+(``build_host()``), which reads torch tensors' addresses for AdamW.  The library
+needs nvcc alone; the module needs a C++ compiler and the headers of the
+installed Python and torch, and carries both versions in its file's name, so
+that after an upgrade of either a new one is built and the old one left alone.
 """
 from __future__ import annotations
 
-import importlib.util
 import os
 import shutil
 import subprocess
@@ -28,7 +30,7 @@ if VARIANT not in ("", "timeline"):
     raise ValueError(f"RNN_KERNEL_B200_VARIANT must be unset or 'timeline', got {VARIANT!r}")
 LIB_NAME = "librnn_kernel_b200_timeline.so" if VARIANT else "librnn_kernel_b200.so"
 LIB_PATH = PKG / LIB_NAME
-HOST_SOURCE, HOST_PATH = CSRC / "host_tensors.cpp", PKG / "_host.so"
+HOST_SOURCE = CSRC / "host_tensors.cpp"
 VARIANT_FLAGS = ["-DGRU_TIMELINE"] if VARIANT == "timeline" else []
 
 NVCC_FLAGS = [
@@ -57,34 +59,40 @@ def _stale(built: Path, deps) -> bool:
     return any(p.stat().st_mtime > mtime for p in [*deps, *(ROOT / "include").glob("*.h")])
 
 
-def _needs_library() -> bool:
+def needs_build() -> bool:
     return _stale(LIB_PATH, CSRC.glob("*.cu*"))
 
 
-def _needs_host() -> bool:
-    return _stale(HOST_PATH, [HOST_SOURCE])
+def host_path() -> Path:
+    """The module's file for this Python and this torch."""
+    import torch
+
+    return PKG / f"_host-torch{torch.__version__}{sysconfig.get_config_var('EXT_SUFFIX')}"
 
 
-def needs_build() -> bool:
-    return _needs_library() or _needs_host()
+def build_host(force: bool = False, verbose: bool = False) -> Path:
+    """Compiles the module ``_host`` if it is missing or older than its source."""
+    import torch
 
-
-def _build_host(verbose: bool) -> None:
-    torch = Path(importlib.util.find_spec("torch").origin).parent
-    tmp = HOST_PATH.with_suffix(".so.tmp")
-    include = [torch / "include", torch / "include/torch/csrc/api/include", sysconfig.get_paths()["include"]]
-    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{i}" for i in include), str(HOST_SOURCE),
-           f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-o", str(tmp)]
+    path = host_path()
+    if not force and not _stale(path, [HOST_SOURCE]):
+        return path
+    base = Path(torch.__file__).parent
+    tmp = path.with_name(f"{path.name}.{os.getpid()}.so.tmp")  # ranks may build at the same time
+    include = [base / "include", base / "include/torch/csrc/api/include", sysconfig.get_paths()["include"]]
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{i}" for i in include),
+           str(HOST_SOURCE), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-o", str(tmp)]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)
-    os.replace(tmp, HOST_PATH)
+    os.replace(tmp, path)
+    return path
 
 
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> Path:
-    if force or _needs_host():
-        _build_host(verbose)
-    if not force and not _needs_library():
+    """Compiles the CUDA library if it is missing or older than a source."""
+    if not force and not needs_build():
         return LIB_PATH
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [nvcc_path(), *NVCC_FLAGS, *VARIANT_FLAGS, *(extra or []), "-I", str(ROOT / "include"),
@@ -99,3 +107,7 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
 if __name__ == "__main__":
     build(force="--force" in sys.argv, verbose=True,
           extra=["-Xptxas", "-v"] if "--ptxas" in sys.argv else None)
+    try:
+        build_host(force="--force" in sys.argv, verbose=True)
+    except (OSError, subprocess.CalledProcessError) as e:
+        print(f"the module _host was not built ({e}); AdamW reads its tensors in Python", file=sys.stderr)

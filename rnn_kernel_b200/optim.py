@@ -16,7 +16,9 @@ fallback.
 """
 from __future__ import annotations
 
+import functools
 import math
+import warnings
 from typing import Iterable, Optional
 
 import numpy as np
@@ -30,6 +32,16 @@ _DTYPES = {torch.float32: _lib.GRU_F32, torch.bfloat16: _lib.GRU_BF16}
 # gru_adamw_tensor of include/rnn_kernel_b200.h
 _ENTRY = np.dtype([("param", "u8"), ("grad", "u8"), ("n", "i8"), ("state_offset", "i8"), ("decay", "f4"),
                    ("step_size", "f4"), ("inv_sqrt_bc2", "f4"), ("pad", "f4")])
+
+
+@functools.lru_cache(maxsize=1)
+def _reader():
+    """The C++ reader of tensors, or None (said once) where it cannot be built: the Python below does the same."""
+    try:
+        return _lib.host().adamw_addresses
+    except Exception as e:  # no compiler, no headers, a module that does not load
+        warnings.warn(f"AdamW reads its tensors in Python, some 0.5 us each: the module _host is not available ({e})")
+        return None
 
 
 class _TypeTable:
@@ -49,7 +61,7 @@ class _TypeTable:
     def _bind(self) -> None:
         """What belongs to this object alone: the address of its own entries, which a copy of it does not share."""
         self.address = self.entries.ctypes.data
-        self.addresses = _lib.host().adamw_addresses
+        self.addresses = _reader()
         self.copies = None  # dense copies of gradients that are not, until the launch
 
     def __getstate__(self) -> dict:
@@ -62,7 +74,7 @@ class _TypeTable:
 
     def gather(self, device: torch.device) -> Optional[np.ndarray]:
         """Fills in this step's addresses; the mask of parameters without a gradient, None where all have one."""
-        if self.addresses(self.params, self.address, self.code, device.index):
+        if self.addresses is not None and self.addresses(self.params, self.address, self.code, device.index):
             return None
         grads = []
         # a new .data may lie where the old one did
