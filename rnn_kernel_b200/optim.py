@@ -249,10 +249,10 @@ class AdamW:
         return list(zip(self._offsets.tolist(), self._sizes.tolist()))
 
     def state_dict(self) -> dict:
-        """What continues this run bit for bit: moments as they are held, counts, and the groups' rates."""
+        """What continues this run bit for bit: moments as they are held, counts, betas, eps and the groups' rates."""
         calls = self._calls if self._device_step is None else int(self._device_step)
         steps = [calls] * len(self.params) if self._steady else self._steps.tolist()
-        return {"state_bits": self.state_bits, "seed": self.seed, "sizes": self._sizes.tolist(), "calls": calls,
+        return {"state_bits": self.state_bits, "betas": self.betas, "eps": self.eps, "seed": self.seed, "sizes": self._sizes.tolist(), "calls": calls,
                 "steps": steps, "exp_avg": self.exp_avg.clone(), "exp_avg_sq": self.exp_avg_sq.clone(),
                 "scale_avg": None if self.scale_avg is None else self.scale_avg.clone(),
                 "scale_sq": None if self.scale_sq is None else self.scale_sq.clone(),
@@ -268,6 +268,8 @@ class AdamW:
                 raise ValueError("AdamW(capturable=True): the state's parameters have different step counts.")
             self._device_step.fill_(state["calls"])
         self._calls, self.seed = int(state["calls"]), int(state["seed"])
+        if "betas" in state:  # states of before they were saved keep what this object was made with
+            self.betas, self.eps = (float(state["betas"][0]), float(state["betas"][1])), float(state["eps"])
         self._steps[:] = state["steps"]
         self._steady = all(t == self._calls for t in state["steps"])
         for name in ("exp_avg", "exp_avg_sq", "scale_avg", "scale_sq"):

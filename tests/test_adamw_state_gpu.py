@@ -1,0 +1,44 @@
+"""AdamW's saved state is all that a run's continuation depends on, and what the trainer's attributes do with it."""
+import pytest
+import torch
+
+from rnn_kernel_b200 import AdamW
+
+pytestmark = pytest.mark.gpu
+
+
+def params_of(sizes, seed=0):
+    torch.manual_seed(seed)
+    return [torch.nn.Parameter(torch.randn(n, device="cuda")) for n in sizes]
+
+
+def gradients(ps, step):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(step)
+    for p in ps:
+        p.grad = torch.randn(p.shape, device="cuda", generator=gen)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_state_brings_betas_and_eps(bits, capturable):
+    ps = params_of([513, 40])
+    opt = AdamW(ps, lr=1e-2, betas=(0.8, 0.95), eps=1e-4, weight_decay=0.1, state_bits=bits, seed=9, capturable=capturable)
+    for t in range(3):
+        gradients(ps, t)
+        opt.step()
+    saved = opt.state_dict()
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    other = AdamW(qs, lr=5.0, betas=(0.5, 0.5), eps=1e-8, state_bits=bits, capturable=capturable)
+    other.load_state_dict(saved)
+    for t in range(3, 6):
+        for x, o in ((ps, opt), (qs, other)):
+            gradients(x, t)
+            o.step()
+    for p, q in zip(ps, qs):
+        assert torch.equal(p.detach(), q.detach())
+    # a state of before betas and eps were part of it
+    old = {k: v for k, v in saved.items() if k not in ("betas", "eps")}
+    third = AdamW(params_of([513, 40]), betas=(0.7, 0.8), eps=1e-3, state_bits=bits, capturable=capturable)
+    third.load_state_dict(old)
+    assert third.betas == (0.7, 0.8) and third.eps == 1e-3
