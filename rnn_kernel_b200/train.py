@@ -61,6 +61,8 @@ class DataParallelTrainer:
 
     ``optimizer`` is ``"sgd"`` or ``"adamw"`` (:class:`AdamW` on the flat
     parameter buffer, CUDA only; ``weight_decay`` and ``state_bits`` are its).
+    ``lr`` may be set between steps, with either (a captured step keeps the one
+    at its capture).
     """
 
     def __init__(self, module: nn.Module, lr: float = 1e-2,
@@ -69,11 +71,11 @@ class DataParallelTrainer:
         if optimizer not in ("sgd", "adamw"):
             raise ValueError('optimizer must be "sgd" or "adamw".')
         self.module = module
+        self.optimizer = None
         self.lr = float(lr)
         self.group = process_group
         self.world = dist.get_world_size(process_group) if dist.is_available() and dist.is_initialized() else 1
         self.flat, self.grad = flatten_parameters_(module)
-        self.optimizer = None
         if optimizer == "adamw":
             # the step count lives on the device, so that a captured step advances with every replay
             self.flat.grad = self.grad
@@ -92,6 +94,17 @@ class DataParallelTrainer:
             dist.broadcast(self.flat, src=0, group=process_group)
             if overlap:
                 self._install_bucket_hooks()
+
+    @property
+    def lr(self) -> float:
+        return self._lr if self.optimizer is None else self.optimizer.param_groups[0]["lr"]
+
+    @lr.setter
+    def lr(self, value: float) -> None:
+        if self.optimizer is None:
+            self._lr = value
+        else:
+            self.optimizer.param_groups[0]["lr"] = value
 
     def _install_bucket_hooks(self) -> None:
         # Group the parameters by the layer suffix of their names (``_l{k}``,

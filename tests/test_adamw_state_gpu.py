@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from rnn_kernel_b200 import AdamW
+from rnn_kernel_b200 import GRU, AdamW, DataParallelTrainer
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,30 @@ def test_state_brings_betas_and_eps(bits, capturable):
     third = AdamW(params_of([513, 40]), betas=(0.7, 0.8), eps=1e-3, state_bits=bits, capturable=capturable)
     third.load_state_dict(old)
     assert third.betas == (0.7, 0.8) and third.eps == 1e-3
+
+
+@pytest.mark.parametrize("optimizer", ["sgd", "adamw"])
+def test_trainer_learning_rate_counts(optimizer):
+    torch.manual_seed(0)
+    x, y = torch.randn(4, 10, 8, device="cuda"), torch.randn(4, 10, 16, device="cuda")
+
+    def run(change):
+        torch.manual_seed(1)
+        trainer = DataParallelTrainer(GRU(8, 16).cuda(), lr=1e-2, optimizer=optimizer)
+        trainer.step(x, y)
+        change(trainer)
+        before = trainer.flat.clone()
+        trainer.step(x, y)
+        return trainer.lr, trainer.flat - before
+
+    def by_attribute(t):
+        t.lr = 0.0
+
+    def by_group(t):
+        t.optimizer.param_groups[0]["lr"] = 0.0
+
+    lr, moved = run(lambda t: None)
+    assert lr == 1e-2 and float(moved.abs().max()) > 0
+    for change in (by_attribute, by_group) if optimizer == "adamw" else (by_attribute,):
+        lr, moved = run(change)
+        assert lr == 0.0 and float(moved.abs().max()) == 0
