@@ -78,8 +78,14 @@ class DataParallelTrainer:
         self.flat, self.grad = flatten_parameters_(module)
         if optimizer == "adamw":
             # the step count lives on the device, so that a captured step advances with every replay
-            self.flat.grad = self.grad
-            self.optimizer = AdamW([self.flat], lr=self.lr, weight_decay=weight_decay, state_bits=state_bits,
+            parts = [self.flat]
+            if state_bits == 8:  # every parameter starts a block: a weight and the bias after it share no scale
+                parts = self.flat.split([p.numel() for p in module.parameters() if p.requires_grad])
+            at = 0
+            for part in parts:
+                part.grad = self.grad[at:at + part.numel()]
+                at += part.numel()
+            self.optimizer = AdamW(parts, lr=self.lr, weight_decay=weight_decay, state_bits=state_bits,
                                    capturable=True)
         self._buckets: list = []   # [lo, hi) slices of the gradient buffer, one per layer
         self._pending: list = []   # parameters of each bucket not yet accumulated this step

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from rnn_kernel_b200 import GRU, AdamW, DataParallelTrainer
+from rnn_kernel_b200 import GRU, AdamW, DataParallelTrainer, mse_loss
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +69,27 @@ def test_trainer_learning_rate_counts(optimizer):
     for change in (by_attribute, by_group) if optimizer == "adamw" else (by_attribute,):
         lr, moved = run(change)
         assert lr == 0.0 and float(moved.abs().max()) == 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_trainer_steps_as_the_optimizer_over_its_parameters(bits):
+    """8-bit moments: every parameter's blocks are its own, though all lie in one buffer."""
+    torch.manual_seed(0)
+    x, y = torch.randn(4, 10, 7, device="cuda"), torch.randn(4, 10, 13, device="cuda")
+
+    def module():
+        torch.manual_seed(1)
+        return GRU(7, 13, num_layers=2).cuda()
+
+    trainer = DataParallelTrainer(module(), lr=1e-2, optimizer="adamw", state_bits=bits)
+    m = module()
+    opt = AdamW(m.parameters(), lr=1e-2, state_bits=bits, capturable=True)
+    for _ in range(4):
+        trainer.step(x, y)
+        opt.zero_grad()
+        mse_loss(m(x)[0], y).backward()
+        opt.step()
+    for p, q in zip(trainer.module.parameters(), m.parameters()):
+        assert torch.equal(p.detach(), q.detach())
+    if bits == 8:
+        assert [n for _, n in trainer.optimizer.offsets()] == [p.numel() for p in m.parameters()]
