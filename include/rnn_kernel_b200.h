@@ -143,7 +143,8 @@ typedef struct {
  *   p = decay p - step_size m / (sqrt(v) inv_sqrt_bc2 + eps)
  * computed in FP32.  state_bits 32: exp_avg and exp_avg_sq hold state_elems
  * floats.  state_bits 8: they hold one byte an element, and scale_avg /
- * scale_sq one float per 256 elements (all zero-initialised).  8-bit moments
+ * scale_sq one float per 256 elements (all zero-initialised), and eps must be
+ * 2^-50 or more (second moments below 2^-100 are held as zero).  8-bit moments
  * are rounded stochastically from (seed, step, position), step the number of
  * this step.  With device_scalars (3 device floats) the bias corrections and
  * the rounding key come from there, and step_size holds lr; a call with

@@ -433,6 +433,12 @@ extern "C" int gru_adamw_step(const gru_adamw_tensor* tensors, int count, int dt
     set_error("gru_adamw_step: need 0 <= beta1, beta2 < 1 and eps >= 0");
     return GRU_ERR_INVALID;
   }
+  // a block of second moments below 2^-100 counts as zero: eps must not be
+  // smaller than their roots, or their step would be divided by next to nothing
+  if (state_bits == 8 && !(eps >= 0x1p-50)) {
+    set_error("gru_adamw_step: need eps >= 2^-50 with 8-bit moments");
+    return GRU_ERR_INVALID;
+  }
   if (device_step && !device_scalars) {
     set_error("gru_adamw_step: device_step needs device_scalars");
     return GRU_ERR_INVALID;

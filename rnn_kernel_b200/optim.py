@@ -27,6 +27,8 @@ import torch
 from . import _lib
 
 STATE_BLOCK = 256  # elements per 8-bit scale; every tensor's moments start a block
+# a block's second moments below 2^-100 are held as zero, so eps has to be at least their root
+MIN_EPS_8 = 2.0 ** -50
 
 _DTYPES = {torch.float32: _lib.GRU_F32, torch.bfloat16: _lib.GRU_BF16}
 # gru_adamw_tensor of include/rnn_kernel_b200.h
@@ -115,6 +117,8 @@ class AdamW:
             raise ValueError("eps must be >= 0.")
         if state_bits not in (8, 32):
             raise ValueError("state_bits must be 8 or 32.")
+        if state_bits == 8 and not eps >= MIN_EPS_8:
+            raise ValueError("eps must be >= 2^-50 with 8-bit moments: smaller second moments' roots count as zero.")
         self.betas, self.eps = (float(betas[0]), float(betas[1])), float(eps)
         self.state_bits, self.seed, self.capturable = state_bits, int(seed) & 0xFFFFFFFF, bool(capturable)
         groups = list(params)
