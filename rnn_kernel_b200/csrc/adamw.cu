@@ -16,7 +16,9 @@
 //   second moment  5 exponent bits:       2^-31 .. 1.875 (and zero)
 // A logarithmic code, because v spans many decades inside a block and a linear
 // one would round most of it to zero, and v divides: a nonzero v is never
-// coded as zero.  Rounding is stochastic, from a hash of (seed, step,
+// coded as zero, unless its quotient by the scale is below FP32's range, and
+// beside a v coded as zero (a gradient whose square vanishes) no m is rounded
+// up to the least code: eps alone would divide it.  Rounding is stochastic, from a hash of (seed, step,
 // position): an update moves v by 0.1 % where codes are 6 - 12 % apart, so
 // rounding to nearest would stop the average altogether, while here its
 // expectation is exact (above the least code).  The arithmetic up to the codes
@@ -300,12 +302,11 @@ __global__ void __launch_bounds__(kThreads, kBits == 8 ? 5 : 4) adamw_kernel(con
       const float sm = block_scale(__float_as_uint(am)), sv = block_scale(__float_as_uint(av));
       const float im = sm == 0.0f ? 0.0f : __frcp_rn(sm), iv = sv == 0.0f ? 0.0f : __frcp_rn(sv);
       int km[2][4];
-      unsigned rnd[2][4];
+      unsigned rnd[2][4], cv[2] = {0, 0};
       bool low = false;
       const unsigned base = noise_base(so + lane * 4, key);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        unsigned cv = 0;
 #pragma unroll
         for (int i = 3; i >= 0; --i) {
           rnd[h][i] = noise_bits(base + (unsigned)(h * 128 + i) * 0x9E3779B1u);
@@ -314,9 +315,9 @@ __global__ void __launch_bounds__(kThreads, kBits == 8 ? 5 : 4) adamw_kernel(con
           low |= r < kLeast;
           // a nonzero second moment is never coded as zero: it divides
           const int k = max(round_code(q, (rnd[h][i] << 4) & 0xffff0u, 5), (int)min(__float_as_uint(q), 1u));
-          cv = cv * 256u + (unsigned)k;
+          cv[h] = cv[h] * 256u + (unsigned)k;
         }
-        bv[h * 32] = cv;
+        bv[h * 32] = cv[h];
       }
       if (low) {
 #pragma unroll
@@ -324,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, kBits == 8 ? 5 : 4) adamw_kernel(con
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float r = __fmul_rn(fabsf(m[h][i]), im);
-            if (r < kLeast) km[h][i] = round_least(r, rnd[h][i] >> 16);
+            if (r < kLeast) km[h][i] = (cv[h] >> (8 * i)) & 0xffu ? round_least(r, rnd[h][i] >> 16) : 0;
           }
       }
 #pragma unroll
