@@ -38,10 +38,11 @@ namespace {
 template <int NP, int DK, int STAGES>
 struct BackSmem {
   static constexpr int k = NP * kC * DK, w = 2 * kTile;  // elements; K, Q, W, P
-  static constexpr int stage = 2 * (k + w) * 2 + kGates * kC * 4;
+  static constexpr int stage = 2 * (k + w) * 2 + kBackward * kC * 4;
   // two planes of two groups (of dO, NP): dS, B dU, e^G B Z, e^G dO; dO
   static constexpr int s = 4 * kGroup * DK, x = 4 * kGroup * kC, o = NP * 2 * kGroup * kC;
-  static constexpr int bytes = STAGES * stage + (s + 3 * x + o) * 2 + 5 * 8 * 4;
+  // scales of dS, e^G B Z and e^G dO, exponents of B dU's and dO's tokens
+  static constexpr int bytes = STAGES * stage + (s + 3 * x + o) * 2 + 3 * 8 * 4 + 4 * kC * 4;
 };
 
 template <int NP, int DK>
@@ -52,21 +53,8 @@ __device__ __forceinline__ void back_load(unsigned char* stage, const Problem& a
   copy_async<L::k * 2, kThreads>(p + L::k, a.qp + nk * L::k);
   copy_async<L::w * 2, kThreads>(p + 2 * L::k, a.wp + nv * L::w);
   copy_async<L::w * 2, kThreads>(p + 2 * L::k + L::w, a.pp + nv * L::w);
-  copy_async<kGates * kC * 4, kThreads>(p + 2 * (L::k + L::w), a.gates + nv * kGates * kC);
+  copy_async<kBackward * kC * 4, kThreads>(p + 2 * (L::k + L::w), a.gates + nv * kGates * kC);
   cp_async_commit();
-}
-
-// A warp's 16 tokens x 16 columns as NP planes in shared memory, with their
-// scale, and in `out`, if given.
-template <int NP>
-__device__ __forceinline__ void put_tokens(const float (&x)[2][4], int quarter, f16* tile, float* scale, f16* out,
-                                           float* out_scale) {
-  const float inv = plane_inv(warp_max(x));
-  if ((threadIdx.x & 31) == 0) {
-    scale[quarter] = plane_scale(inv);
-    if (out) out_scale[quarter] = plane_scale(inv);
-  }
-  store_rows<NP>(tile, 2 * kGroup * kC, quarter * 2, x, inv, out, kGroup * kC);
 }
 
 // STAGES: with two the next chunk's tiles load during this one; with one they
@@ -89,7 +77,10 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
   f16* qop = zp + L::x;                        // scale e^G dO
   f16* op = base + L::s + 3 * L::x + pair * kGroup * kC;
   float* scales = reinterpret_cast<float*>(base + L::s + 3 * L::x + L::o) + pair * 4;
-  float *ssc = scales, *usc = scales + 8, *zsc = scales + 16, *qosc = scales + 24, *osc = scales + 32;
+  float *ssc = scales, *zsc = scales + 8, *qosc = scales + 16;
+  int* uex = reinterpret_cast<int*>(scales - pair * 4 + 24) + pair * kC;
+  int* oex = uex + 2 * kC;
+  bool all_finite;
 
   float d[MT][2][4];  // the gradient of the state after the chunk
   const float* ds = a.ds_out ? a.ds_out + (long)bh * a.dk * a.dv : nullptr;
@@ -127,8 +118,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
     float x[2][4];
     dout_tile(x);
     const long nv = nv0 + chunk;
-    put_tokens<NP>(x, quarter, op, osc, a.dop + (nv * groups + group) * NP * kGroup * kC,
-                   a.doscale + (nv * groups + group) * 4);
+    put_tokens<NP>(x, quarter, op, oex, a.dop + (nv * groups + group) * NP * kGroup * kC,
+                   a.doscale + (nv * groups + group) * kC, all_finite);
   };
   auto state_out = [&](int chunk) {
     const long nv = nv0 + chunk;
@@ -153,8 +144,9 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
       buf ^= 1;
       back_load<NP, DK>(smem + buf * L::stage, a, nk0 + chunk - 1, nv - 1);
     }
-    const float sw = gate[5 * kC], sP = gate[5 * kC + 1], sk = gate[5 * kC + 2], sq = gate[5 * kC + 3];
+    const int* size = reinterpret_cast<const int*>(gate);
     const int row[2] = {frag_row(quarter * 16, 0), frag_row(quarter * 16, 1)};
+    const float sk[2] = {gate[kScaleK * kC + row[0]], gate[kScaleK * kC + row[1]]};
     float x[2][4], y[2][4];
     // scale e^G dO, for Q^T
     dout_tile(x);
@@ -162,31 +154,31 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[n][e] *= a.scale * gate[row[e >> 1]];
-    put_tokens<2>(x, quarter, qop, qosc, nullptr, nullptr);
+      for (int e = 0; e < 4; ++e) x[n][e] *= a.scale * gate[row[e >> 1]] * gate[kScaleQ * kC + row[e >> 1]];
+    put_sum(x, quarter, qop, qosc);
     // dU
     times_state<NP, DK>(x, kp, quarter * 2, sp, ssc);
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[n][e] *= sk * gate[kC + row[e >> 1]];
-    times_tokens<2, NP, true>(x, pp, quarter * 2, op, 2 * kGroup * kC * 2, osc, sP, quarter, 4);
+      for (int e = 0; e < 4; ++e) x[n][e] *= sk[e >> 1] * gate[kRest * kC + row[e >> 1]];
+    times_tokens<NP, true, false>(x, pp, gate + kScaleP * kC, size + kSizeP * kC, quarter, op, oex, 1.0f);
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[n][e] = x[n][e] * gate[2 * kC + row[e >> 1]];
-    put_tokens<2>(y, quarter, up, usc, nullptr, nullptr);
+      for (int e = 0; e < 4; ++e) y[n][e] = x[n][e] * gate[kBeta * kC + row[e >> 1]];
+    put_tokens<2>(y, quarter, up, uex, nullptr, nullptr, all_finite);
     group_sync(pair);
     // Z and dV
-    times_tokens<2, 2, true>(x, wp, quarter * 2, up, 2 * kGroup * kC * 2, usc, -sw, quarter, 4);
-    put_tokens<2>(x, quarter, zp, zsc, a.z + (nv * groups + group) * 2 * kGroup * kC,
-                  a.zscale + (nv * groups + group) * 4);  // zp: on the way only
+    times_tokens<2, true, true>(x, wp, gate + kScaleW * kC, size + kSizeW * kC, quarter, up, uex, -1.0f);
+    put_tokens<2>(x, quarter, zp, nullptr, a.z + (nv * groups + group) * 2 * kGroup * kC,
+                  a.zscale + (nv * groups + group) * kC, all_finite);  // zp: on the way only
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int t = chunk * kC + row[e], c = frag_col(n * 8);
-        const float be = gate[2 * kC + row[e]], eg = gate[row[e]];
+        const float be = gate[kBeta * kC + row[e]], eg = gate[row[e]] * sk[e];
         x[n][2 * e] *= be;
         x[n][2 * e + 1] *= be;
         if (t < a.T) set2<T>(dv + t * stride + c, cols - c, a.dv % 2 == 0, x[n][2 * e], x[n][2 * e + 1]);
@@ -194,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
         y[n][2 * e + 1] = -eg * x[n][2 * e + 1];
       }
     __syncwarp();
-    put_tokens<2>(y, quarter, zp, zsc, nullptr, nullptr);
+    put_sum(y, quarter, zp, zsc);
     group_sync(pair);
     const float decay = gate[kC - 1];
 #pragma unroll
@@ -203,8 +195,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[m][n][e] *= decay;
-    add_to_state<NP, DK>(d, qp, quarter, qop, qosc, sq);
-    add_to_state<NP, DK>(d, kp, quarter, zp, zsc, sk);
+    add_to_state<NP, DK>(d, qp, quarter, qop, qosc);
+    add_to_state<NP, DK>(d, kp, quarter, zp, zsc);
     state_out(chunk - 1);
     if (chunk > 0) put_dout(chunk - 1);
     if (STAGES == 1 && chunk > 0) {
@@ -237,6 +229,17 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
 // these kernels.
 // ---------------------------------------------------------------------------
 
+// A lower 64 x 64 matrix as its ten 16 x 16 tiles on and below the diagonal.
+constexpr int kLower = 10 * 256;
+__device__ __forceinline__ int lower_tile(int r16, int c16) { return r16 * (r16 + 1) / 2 + c16; }
+// A (16 rows m, 16 of k) of one: stored [m][k], or [k][m] (TRANS).
+template <bool TRANS>
+__device__ __forceinline__ uint32_t addr_lower(const f16* p, int m16, int k16) {
+  const int i = (threadIdx.x >> 3) & 3;
+  const int tile = TRANS ? lower_tile(k16, m16) : lower_tile(m16, k16);
+  return smem_addr(p) + (tile * 256 + (TRANS ? i : (i & 1) * 2 + (i >> 1)) * 64 + (threadIdx.x & 7) * 8) * 2;
+}
+
 template <int NP, int DK>
 struct GradSmem {
   static constexpr int split = DK / 32;           // warps that share 16 tokens' columns
@@ -246,10 +249,11 @@ struct GradSmem {
   static constexpr int s = 2 * kGroup * DK, x = 2 * kGroup * kC, o = NP * kGroup * kC;
   // a stage: S, dS, E, Z, dO, each [step][plane], and their scales
   static constexpr int planes = steps * (2 * s + 2 * x + o);
-  static constexpr int stage = planes + 5 * steps * 8;
-  static constexpr int tiles = 4 * kTile * 2 + kC * (kC + 1) * 4;  // bytes: dP', M; y in FP32; over the stages
+  static constexpr int stage = planes + steps * 2 * (2 * 4 + 3 * kC);
+  // bytes: dP' and M twice, scaled by rows and by columns; y in FP32; over the stages
+  static constexpr int tiles = 4 * 2 * kLower * 2 + kC * (kC + 1) * 4;
   static constexpr int main = 2 * stage * 2 > tiles ? 2 * stage * 2 : tiles;
-  static constexpr int least = 2 * qk * 2 + (main + 15) / 16 * 16 + kGates * kC * 4 + ((2 * split + 1) * kC + 12 * split) * 4;
+  static constexpr int least = 2 * qk * 2 + (main + 15) / 16 * 16 + kGates * kC * 4 + ((2 * split + 1 + 4) * kC + 4 * split) * 4;
   // dq and dk of the value heads so far, every thread's own, where that fits
   // (not for FP32 inputs of 128 key columns: in global memory there)
   static constexpr int sums = 2 * kC * DK * 4;
@@ -267,10 +271,12 @@ __device__ __forceinline__ void grad_load(f16* dst, const Problem& a, long g) {
   copy_async<n * L::x * 2, threads>(dst + 2 * n * L::s, a.e + g * L::x);
   copy_async<n * L::x * 2, threads>(dst + n * (2 * L::s + L::x), a.z + g * L::x);
   copy_async<n * L::o * 2, threads>(dst + n * (2 * L::s + 2 * L::x), a.dop + g * L::o);
-  if (threadIdx.x < 5 * n) {
-    const int t = threadIdx.x / n, i = threadIdx.x % n;
-    const float* from = t == 0 ? a.sscale : t == 1 ? a.dsscale : t == 2 ? a.escale : t == 3 ? a.zscale : a.doscale;
-    cp_async16(dst + L::planes + threadIdx.x * 8, from + (g + i) * 4);
+  // scales: of S and of dS, then of the tokens of E, Z and dO
+  if (threadIdx.x < n * (2 + 3 * 16)) {
+    const int t = threadIdx.x - 2 * n, what = t / (16 * n);
+    const float* from = t < 0 ? (threadIdx.x < n ? a.sscale + (g + threadIdx.x) * 4 : a.dsscale + (g + threadIdx.x - n) * 4)
+                              : (what == 0 ? a.escale : what == 1 ? a.zscale : a.doscale) + g * kC + t % (16 * n) * 4;
+    cp_async16(dst + L::planes + threadIdx.x * 8, from);
   }
   cp_async_commit();
 }
@@ -287,10 +293,10 @@ __device__ __forceinline__ float2 take2(const f16* p, int plane, int word) {
   return f;
 }
 
-// acc += A B, one step of 16, times f0 (the first half of the tiles) or f1.
+// acc += A B, one step of 16, times the scales of the rows and a lane's columns.
 template <int NA, int NB, int NT>
-__device__ __forceinline__ void step_add(float (&acc)[NT][4], float f0, float f1, const uint32_t (&fa)[NA][4],
-                                         const uint32_t (&fb)[NB][NT][2]) {
+__device__ __forceinline__ void step_add(float (&acc)[NT][4], const float (&row)[2], const float (&column)[NT][2],
+                                         const uint32_t (&fa)[NA][4], const uint32_t (&fb)[NB][NT][2]) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float t[NT / 2][4];
@@ -303,22 +309,32 @@ __device__ __forceinline__ void step_add(float (&acc)[NT][4], float f0, float f1
 #pragma unroll
     for (int i = 0; i < NT / 2; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[h * NT / 2 + i][e] += (h ? f1 : f0) * t[i][e];
+      for (int e = 0; e < 4; ++e) acc[h * NT / 2 + i][e] += row[e >> 1] * column[h * NT / 2 + i][e & 1] * t[i][e];
   }
 }
+// The same with one scale for the first half of the tiles' columns, and for the second.
+template <int NA, int NB, int NT>
+__device__ __forceinline__ void step_add(float (&acc)[NT][4], const float (&row)[2], float f0, float f1,
+                                         const uint32_t (&fa)[NA][4], const uint32_t (&fb)[NB][NT][2]) {
+  float column[NT][2];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) column[i][0] = column[i][1] = i < NT / 2 ? f0 : f1;
+  step_add<NA, NB, NT>(acc, row, column, fa, fb);
+}
 
-// acc += f A B over steps [k0, k1) of the tokens: A a 64 x 64 tile (rows m, or
-// transposed), B a [64 x DK] tile from column block n8.
+// acc += A B over steps [k0, k1) of the tokens, times the scales of A's rows: A a
+// lower 64 x 64 tile (rows m, or transposed), B a [64 x DK] tile from column block
+// n8, without its scales.
 template <int NP, int DK, bool TA, int NT>
-__device__ __forceinline__ void token_product(float (&acc)[NT][4], float f, const f16* A, int m8, const f16* B, int n8,
-                                              int k0, int k1) {
+__device__ __forceinline__ void token_product(float (&acc)[NT][4], const float (&row)[2], const f16* A, int m16, const f16* B,
+                                              int n8, int k0, int k1) {
   for (int kk = k0; kk < k1; ++kk) {
     uint32_t fa[2][4], fb[NP][NT][2];
-    const uint32_t pa = addr_a<kC, TA>(A, m8, 2 * kk);
+    const uint32_t pa = addr_lower<TA>(A, m16, kk);
 #pragma unroll
-    for (int p = 0; p < 2; ++p) ldm4<TA>(fa[p], pa + p * kTile * 2);
+    for (int p = 0; p < 2; ++p) ldm4<TA>(fa[p], pa + p * kLower * 2);
     load_b<NP, NT, true>(fb, addr_b<DK, true>(B, 2 * kk, n8), 256, kC * DK * 2);
-    step_add<2, NP, NT>(acc, f, f, fa, fb);
+    step_add<2, NP, NT>(acc, row, 1.0f, 1.0f, fa, fb);
   }
 }
 
@@ -334,17 +350,23 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
   f16* qp = reinterpret_cast<f16*>(smem);
   f16* kp = qp + L::qk;
   f16* main = kp + L::qk;
-  f16* dpp = main;  // over the stages
-  f16* mp = dpp + 2 * kTile;
-  float* y = reinterpret_cast<float*>(mp + 2 * kTile);  // [64][65]
+  // over the stages: dP' with K's scales and a scale a row, M likewise; dP' with
+  // Q's scales and a scale a column, M with K's
+  f16* dpr = main;
+  f16* mr = dpr + 2 * kLower;
+  f16* dpc = mr + 2 * kLower;
+  f16* mc = dpc + 2 * kLower;
+  float* y = reinterpret_cast<float*>(mc + 2 * kLower);  // [64][65]
   float* gate = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(main) + (L::main + 15) / 16 * 16);
-  float* red = gate + kGates * kC;  // x and z of the warps that share tokens, F; then values per warp
-  float* wred = red + (2 * split + 1) * kC;
+  float* red = gate + kGates * kC;  // x and z of the warps that share tokens, F
+  float* largest = red + (2 * split + 1) * kC;  // magnitudes of dP' and M, rows' and columns': [4][64]
+  float* wred = largest + 4 * kC;  // values per warp
 
   const int chunk = blockIdx.x % a.nc, bh = blockIdx.x / a.nc;
   const int hk = bh % a.Hk, b = bh / a.Hk;
   const int t0 = chunk * kC, rows = min(kC, a.T - t0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rw[2] = {frag_row(warp / split * 16, 0), frag_row(warp / split * 16, 1)};  // this lane's tokens
   // This warp's tokens; its part of the columns, and whether that holds any of the
   // 64 x 64 products' lower half.  The parts turn from row to row: were they the
   // warp's remainder, one of the SM's quarters would have twice the others' products.
@@ -362,6 +384,10 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
     __syncthreads();
     copy_async<kGates * kC * 4, threads>(gate, a.gates + nv * kGates * kC);
     grad_load<NP, DK>(main, a, nv * groups);
+    if (threadIdx.x < kC) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) largest[i * kC + threadIdx.x] = 0.0f;
+    }
     float dp[NC][4], da[NC][4], dq[NT][4], dkr[NT][4], dkc[NT][4];
     zero(dp);
     zero(da);
@@ -385,10 +411,12 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
       const f16* op = stage + n * (2 * L::s + 2 * L::x) + i * L::o;
       // scales: of the quarters of the key columns (S, dS) and of the tokens
       const float* ss = reinterpret_cast<const float*>(stage + L::planes) + i * 4;
-      const float *sds = ss + 4 * n, *se = ss + 8 * n, *sz = ss + 12 * n, *so = ss + 16 * n;
-      const int mq = m0 / 16, kq = col * 4 / split;  // quarters of this warp's tokens and of its first key column
-      constexpr int k2 = split == 4 ? 0 : 1;         // and of its last
-      const float fE = fabsf(se[mq]), fZ = sz[mq], fO = so[mq];
+      const float *sds = ss + 4 * n, *se = ss - i * 4 + 8 * n + i * kC, *sz = se + n * kC, *so = sz + n * kC;
+      const int kq = col * 4 / split;         // quarter of this warp's first key column
+      constexpr int k2 = split == 4 ? 0 : 1;  // and of its last
+      // a scale below zero only marks tokens
+      const float fE[2] = {fabsf(se[rw[0]]), fabsf(se[rw[1]])}, fZ[2] = {fabsf(sz[rw[0]]), fabsf(sz[rw[1]])};
+      const float fO[2] = {fabsf(so[rw[0]]), fabsf(so[rw[1]])};
       auto state_dot = [&] {
 #pragma unroll
         for (int j = 0; j < kGroup * DK / 2 / threads; ++j) {
@@ -411,17 +439,16 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
       }
       if (col == 0) {
         // Z . E of this lane's two tokens
-        const float f = fZ * fE;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float2 u = pair(fz[0][j], fz[1][j]), w = pair(fe[0][j], fe[1][j]);
-          bdot[j & 1] += f * (u.x * w.x + u.y * w.y);
+          bdot[j & 1] += fZ[j & 1] * fE[j & 1] * (u.x * w.x + u.y * w.y);
         }
       }
       {
         uint32_t fb[2][NT][2];
         load_b<2, NT, false>(fb, addr_b<kGroup, false>(dsp, 0, col * NT), 512, kGroup * DK * 2);
-        step_add<2, 2, NT>(dkc, fE * sds[kq], fE * sds[kq + k2], fe, fb);
+        step_add<2, 2, NT>(dkc, fE, sds[kq], sds[kq + k2], fe, fb);
       }
       uint32_t fo[NP][4];
 #pragma unroll
@@ -429,22 +456,31 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
       {
         uint32_t fb[2][NT][2];
         load_b<2, NT, false>(fb, addr_b<kGroup, false>(sp, 0, col * NT), 512, kGroup * DK * 2);
-        step_add<NP, 2, NT>(dq, fO * ss[kq], fO * ss[kq + k2], fo, fb);
-        step_add<2, 2, NT>(dkr, fZ * ss[kq], fZ * ss[kq + k2], fz, fb);
+        step_add<NP, 2, NT>(dq, fO, ss[kq], ss[kq + k2], fo, fb);
+        step_add<2, 2, NT>(dkr, fZ, ss[kq], ss[kq + k2], fz, fb);
       }
       if (below) {
         uint32_t fb[2][NC][2];
         load_b<2, NC, false>(fb, addr_b<kGroup, false>(ep, 0, col * NC), 512, kGroup * kC * 2);
-        const float f0 = fabsf(se[kq]), f1 = fabsf(se[kq + k2]);
-        step_add<NP, 2, NC>(dp, fO * f0, fO * f1, fo, fb);
-        step_add<2, 2, NC>(da, fZ * f0, fZ * f1, fz, fb);
+        float f[NC][2];
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+          for (int l = 0; l < 2; ++l) f[n][l] = fabsf(se[frag_col((col * NC + n) * 8) + l]);
+        step_add<NP, 2, NC>(dp, fO, f, fo, fb);
+        step_add<2, 2, NC>(da, fZ, f, fz, fb);
       }
       if (!early) state_dot();
     }
     __syncthreads();
     // the masked 64 x 64 products, over the stages' memory
-    const float sk = gate[5 * kC + 2], sq = gate[5 * kC + 3];
-    float mu = 0.0f, mw = 0.0f;
+    const float sk[2] = {gate[kScaleK * kC + rw[0]], gate[kScaleK * kC + rw[1]]};
+    const float sq[2] = {gate[kScaleQ * kC + rw[0]], gate[kScaleQ * kC + rw[1]]};
+    float sc[NC][2];  // K's scales of this lane's columns
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int l = 0; l < 2; ++l) sc[n][l] = gate[kScaleK * kC + frag_col((col * NC + n) * 8) + l];
     {
       float qk[NC][4], kk[NC][4];
       zero(qk);
@@ -456,10 +492,10 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
           load_b<NP, NC, false>(fb, addr_b<DK, false>(kp, 2 * k, col * NC), 32 * DK, kC * DK * 2);
 #pragma unroll
           for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], addr_a<DK, false>(qp, m0 / 8, 2 * k) + p * kC * DK * 2);
-          step_add<NP, NP, NC>(qk, sq * sk, sq * sk, fa, fb);
+          step_add<NP, NP, NC>(qk, sq, sc, fa, fb);
 #pragma unroll
           for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], addr_a<DK, false>(kp, m0 / 8, 2 * k) + p * kC * DK * 2);
-          step_add<NP, NP, NC>(kk, sk * sk, sk * sk, fa, fb);
+          step_add<NP, NP, NC>(kk, sk, sc, fa, fb);
         }
       }
 #pragma unroll
@@ -469,15 +505,54 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
           const int i = frag_row(m0, e), j = frag_col((col * NC + n) * 8);
 #pragma unroll
           for (int l = 0; l < 2; ++l) {
-            const float dec = j + l <= i ? decay_between(gate, i, j + l) * gate[2 * kC + j + l]
+            const float dec = j + l <= i ? decay_between(gate + kLog * kC, i, j + l) * gate[kBeta * kC + j + l]
                                          : 0.0f;
             float& u = dp[n][2 * e + l];
             float& w = da[n][2 * e + l];
             u = j + l <= i ? a.scale * dec * u : 0.0f;
-            w = j + l < i ? -gate[2 * kC + i] * dec * w : 0.0f;
+            w = j + l < i ? -gate[kBeta * kC + i] * dec * w : 0.0f;
             y[i * (kC + 1) + j + l] = j + l < i ? u * qk[n][2 * e + l] + w * kk[n][2 * e + l] : 0.0f;
-            mu = max_finite(mu, u);
-            mw = max_finite(mw, w);
+          }
+        }
+    }
+    // the largest of dP' and M of every row, with K's scales, and of every column,
+    // with Q's and K's
+    if (below) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mu = 0.0f, mw = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+          for (int l = 0; l < 2; ++l) {
+            mu = max_finite(mu, dp[n][2 * e + l] * sc[n][l]);
+            mw = max_finite(mw, da[n][2 * e + l] * sc[n][l]);
+          }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          mu = fmaxf(mu, __shfl_xor_sync(0xffffffffu, mu, o));
+          mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, o));
+        }
+        if ((lane & 3) == 0) {
+          atomicMax(reinterpret_cast<int*>(largest + rw[e]), __float_as_int(mu));
+          atomicMax(reinterpret_cast<int*>(largest + kC + rw[e]), __float_as_int(mw));
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int l = 0; l < 2; ++l) {
+          float mu = max_finite(max_finite(0.0f, dp[n][l] * sq[0]), dp[n][2 + l] * sq[1]);
+          float mw = max_finite(max_finite(0.0f, da[n][l] * sk[0]), da[n][2 + l] * sk[1]);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            mu = fmaxf(mu, __shfl_xor_sync(0xffffffffu, mu, o));
+            mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, o));
+          }
+          if (lane < 4) {
+            const int j = frag_col((col * NC + n) * 8) + l;
+            atomicMax(reinterpret_cast<int*>(largest + 2 * kC + j), __float_as_int(mu));
+            atomicMax(reinterpret_cast<int*>(largest + 3 * kC + j), __float_as_int(mw));
           }
         }
     }
@@ -488,7 +563,7 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
       for (int e = 0; e < 2; ++e) {
         const int row = frag_row(m0, e);
         const int word = ((m0 / 8 + e) * (DK / 8) + col * NT + n) * 32 + lane;
-        const float eg = gate[row], er = gate[kC + row], be = gate[2 * kC + row];
+        const float eg = gate[row], er = gate[kRest * kC + row], be = gate[kBeta * kC + row];
         const float2 kv = take2<NP>(kp, kC * DK, word), qv = take2<NP>(qp, kC * DK, word);
 #pragma unroll
         for (int l = 0; l < 2; ++l) {
@@ -496,9 +571,9 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
           dkr[n][2 * e + l] *= -eg * be;
           dkc[n][2 * e + l] *= er * be;
         }
-        xs[e] += sq * (qv.x * dq[n][2 * e] + qv.y * dq[n][2 * e + 1]) +
-                 sk * (kv.x * dkr[n][2 * e] + kv.y * dkr[n][2 * e + 1]);
-        zs[e] += sk * (kv.x * dkc[n][2 * e] + kv.y * dkc[n][2 * e + 1]);
+        xs[e] += sq[e] * (qv.x * dq[n][2 * e] + qv.y * dq[n][2 * e + 1]) +
+                 sk[e] * (kv.x * dkr[n][2 * e] + kv.y * dkr[n][2 * e + 1]);
+        zs[e] += sk[e] * (kv.x * dkc[n][2 * e] + kv.y * dkc[n][2 * e + 1]);
       }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -518,35 +593,41 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
     float end = gate[kC - 1] * sdot;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) end += __shfl_xor_sync(0xffffffffu, end, o);
-    const unsigned um = __reduce_max_sync(0xffffffffu, __float_as_uint(mu));
-    const unsigned wm = __reduce_max_sync(0xffffffffu, __float_as_uint(mw));
-    if (lane == 0) {
-      wred[warp] = end;
-      wred[4 * split + warp] = __uint_as_float(um);
-      wred[8 * split + warp] = __uint_as_float(wm);
-    }
+    if (lane == 0) wred[warp] = end;
     __syncthreads();
-    mu = wred[4 * split], mw = wred[8 * split];
+    // scales of the products' rows: of this lane's tokens as rows, and as columns
+    // of what is transposed
+    float scale[4][2];
 #pragma unroll
-    for (int w = 1; w < 4 * split; ++w) {
-      mu = fmaxf(mu, wred[4 * split + w]);
-      mw = fmaxf(mw, wred[8 * split + w]);
-    }
-    const float iu = plane_inv(mu), iw = plane_inv(mw);
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int n = 0; n < NC; ++n)
+      for (int e = 0; e < 2; ++e) scale[i][e] = plane_scale(plane_inv(largest[i * kC + rw[e]]));
+    const float iu[2] = {plane_inv(largest[rw[0]]), plane_inv(largest[rw[1]])};
+    const float iw[2] = {plane_inv(largest[kC + rw[0]]), plane_inv(largest[kC + rw[1]])};
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const int c8 = col * NC + n;
+      if (c8 / 2 > m0 / 16) continue;
+      const int j = frag_col(c8 * 8);
+      const float ju[2] = {plane_inv(largest[2 * kC + j]), plane_inv(largest[2 * kC + j + 1])};
+      const float jw[2] = {plane_inv(largest[3 * kC + j]), plane_inv(largest[3 * kC + j + 1])};
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int word = ((m0 / 8 + e) * (kC / 8) + col * NC + n) * 32 + lane;
-        uint32_t u[2], w[2];
-        split2<2>(dp[n][2 * e], dp[n][2 * e + 1], iu, u);
-        split2<2>(da[n][2 * e], da[n][2 * e + 1], iw, w);
+        const int word = lower_tile(m0 / 16, c8 / 2) * 128 + (e * 2 + (c8 & 1)) * 32 + lane;
+        uint32_t u[2], w[2], x[2], z[2];
+        split2<2>(dp[n][2 * e] * sc[n][0], dp[n][2 * e + 1] * sc[n][1], iu[e], u);
+        split2<2>(da[n][2 * e] * sc[n][0], da[n][2 * e + 1] * sc[n][1], iw[e], w);
+        split2<2>(dp[n][2 * e] * ju[0], dp[n][2 * e + 1] * ju[1], sq[e], x);
+        split2<2>(da[n][2 * e] * jw[0], da[n][2 * e + 1] * jw[1], sk[e], z);
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          reinterpret_cast<uint32_t*>(dpp + p * kTile)[word] = u[p];
-          reinterpret_cast<uint32_t*>(mp + p * kTile)[word] = w[p];
+          reinterpret_cast<uint32_t*>(dpr + p * kLower)[word] = u[p];
+          reinterpret_cast<uint32_t*>(mr + p * kLower)[word] = w[p];
+          reinterpret_cast<uint32_t*>(dpc + p * kLower)[word] = x[p];
+          reinterpret_cast<uint32_t*>(mc + p * kLower)[word] = z[p];
         }
       }
+    }
     {
       // y_ij -> sum over the columns before j, `per` threads to a row
       constexpr int per = threads / kC, n = kC / per;
@@ -570,11 +651,10 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
       }
     }
     __syncthreads();
-    const float su = plane_scale(iu), sw = plane_scale(iw);
-    token_product<NP, DK, false, NT>(dq, su * sk, dpp, m0 / 8, kp, col * NT, 0, m0 / 16 + 1);
-    token_product<NP, DK, false, NT>(dkr, sw * sk, mp, m0 / 8, kp, col * NT, 0, m0 / 16 + 1);
-    token_product<NP, DK, true, NT>(dkc, su * sq, dpp, m0 / 8, qp, col * NT, m0 / 16, kC / 16);
-    token_product<NP, DK, true, NT>(dkc, sw * sk, mp, m0 / 8, kp, col * NT, m0 / 16, kC / 16);
+    token_product<NP, DK, false, NT>(dq, scale[0], dpr, m0 / 16, kp, col * NT, 0, m0 / 16 + 1);
+    token_product<NP, DK, false, NT>(dkr, scale[1], mr, m0 / 16, kp, col * NT, 0, m0 / 16 + 1);
+    token_product<NP, DK, true, NT>(dkc, scale[2], dpc, m0 / 16, qp, col * NT, m0 / 16, kC / 16);
+    token_product<NP, DK, true, NT>(dkc, scale[3], mc, m0 / 16, kp, col * NT, m0 / 16, kC / 16);
     float log_decay[2];  // of the two tokens that a lane of warp 0 ends with
 #pragma unroll
     for (int e = 0; e < 2; ++e)
@@ -611,11 +691,16 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
         if (lane >= o) sz += w;
         last += __shfl_xor_sync(0xffffffffu, last, o);
       }
+      // of the lanes after this one, and of those before: nothing is taken off again
+      sx = __shfl_down_sync(0xffffffffu, sx, 1);
+      sz = __shfl_up_sync(0xffffffffu, sz, 1);
+      if (lane == 31) sx = 0.0;
+      if (lane == 0) sz = 0.0;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int i = 2 * lane + e;
         if (i < rows) {
-          const double from = e ? sx - x[0] : sx, before = e ? sz - z[1] : sz - z[0] - z[1];
+          const double from = e ? sx + x[1] : sx + x[0] + x[1], before = e ? sz + z[0] : sz;
           // a decay of zero passes no gradient
           a.dg[((long)b * a.T + t0 + i) * a.Hv + hv] =
               log_decay[e] < kNoDecay ? 0.0f : (float)(from + before + red[2 * split * kC + i] + last);

@@ -1,13 +1,21 @@
 // Shared device code of the gated delta rule's kernels (sm_100a).
 //
 // The chunked kernels need FP32-grade products (states, gates' gradients and
-// FP32 tensors are FP32) from tensor cores that multiply 16-bit numbers.  An
-// FP32 tile is held as two FP16 planes with a common power of two, x = s (h + l),
-// h = fp16(x / s), l = fp16(x / s - h): s puts the tile's largest magnitude in
-// [2^14, 2^15), so a value keeps 22 bits down to 2^-17 of the largest, and
-// 2^-39 of the largest below.  A product of two such tiles is three plane
-// products (l h', h l', h h'; l l' is below 2^-22 of the result), half the work
-// of three bf16 planes.  bf16 inputs are one plane, exactly.
+// FP32 tensors are FP32) from tensor cores that multiply 16-bit numbers.  FP32
+// numbers are held as two FP16 planes with a power of two that some of them
+// share, x = s (h + l), h = fp16(x / s), l = fp16(x / s - h): s puts the largest
+// magnitude in [2^14, 2^15), so a value keeps 22 bits down to 2^-17 of the
+// largest, and 2^-39 of the largest below.  A product of two such tiles is three
+// plane products (l h', h l', h h'; l l' is below 2^-22 of the result), half the
+// work of three bf16 planes.  bf16 inputs are one plane: exact down to 2^-31 of
+// the largest, and 2^-39 of it below.
+//
+// What shares a scale.  Of K, Q, the errors and the gradients of outputs: a
+// token's head, or 16 value columns of it.  Of W and P: a token's 16 earlier
+// tokens, without those tokens' own sizes (Weights, below).  So no token's
+// result depends on another's magnitude but through the rule itself.  Of a state
+// and its gradient, which have no tokens: a quarter of the key columns x 16 value
+// columns; of what a chunk adds to a state: 16 tokens x 16 value columns.
 //
 // Tiles in memory are made of 8 x 8 blocks of 128 consecutive bytes, the unit
 // that ldmatrix reads (transposed or not, without bank conflicts) and that a
@@ -31,10 +39,23 @@ constexpr int kSlice = 32;  // value columns of a scan's CTA; they are padded to
 constexpr int kThreads = 256;
 constexpr int kTile = kC * kC;  // elements of a token x token tile
 
-// Rows of Problem::gates, 64 floats each: e^G_i, e^(G_end - G_i), beta_i, G_i /
-// log 2 as two floats, and the scales of the planes of W, P, K and Q and a power
-// of two above every |beta|.
-constexpr int kGates = 6;
+// Rows of Problem::gates, 64 numbers each, one to a token.  A scan loads those
+// up to its last.
+enum Gate {
+  kDecay = 0,    // e^G_i
+  kRest = 1,     // e^(G_end - G_i)
+  kBeta = 2,
+  kScaleK = 3,   // of the planes of K
+  kSizeW = 4,    // the exponents (integers) that W's columns leave out, see Weights
+  kScaleW = 5,   // of the planes of W, 4 rows: 16 columns each
+  kForward = 9,  // rows that the forward scan needs
+  kScaleQ = 9,
+  kScaleP = 10,  // as W's
+  kSizeP = 14,
+  kBackward = 15,
+  kLog = 15,     // G_i / log 2 as two floats
+  kGates = 17
+};
 
 // Log decays below this count as this: e^-1000 is zero in FP32, and sums of 64
 // of them (in FP64) still tell neighbouring tokens apart, which -inf would not.
@@ -73,8 +94,8 @@ struct Problem {
   f16* pp;       // [n over Hv][2][64 x 64]
   float* gates;  // [n over Hv][kGates][64]
   // Tiles of 16 value columns each, [n over Hv][group][2][rows x 16], rows the
-  // key columns of a state or the tokens; every quarter of a tile's rows has its
-  // own scale, [n over Hv][group][4].
+  // key columns of a state or the tokens.  Scales: of a state's quarters, [n
+  // over Hv][group][4], of tokens, [n over Hv][group][64].
   f16* states;   // the state before the chunk
   float* sscale;
   f16* e;        // v - S'^T k, so that u = beta e
@@ -207,9 +228,9 @@ __device__ __forceinline__ void load_b(uint32_t (&fb)[NB][NT][2], uint32_t addr,
     }
 }
 
-// e^(G_i - G_j) from the gates.
-__device__ __forceinline__ float decay_between(const float* gates, int i, int j) {
-  return exp2f((gates[3 * kC + i] - gates[3 * kC + j]) + (gates[4 * kC + i] - gates[4 * kC + j]));
+// e^(G_i - G_j) from the two rows of logarithms.
+__device__ __forceinline__ float decay_between(const float* log, int i, int j) {
+  return exp2f((log[i] - log[j]) + (log[kC + i] - log[kC + j]));
 }
 
 template <int NT>
@@ -236,6 +257,10 @@ __device__ __forceinline__ float plane_inv(float m) {
   return __uint_as_float((unsigned)(268 - eb) << 23);
 }
 __device__ __forceinline__ float plane_scale(float inv) { return __uint_as_float((254u << 23) - __float_as_uint(inv)); }
+
+// A power of two's exponent, biased, and back, to the nearest that there is.
+__device__ __forceinline__ int exponent_of(float x) { return (int)((__float_as_uint(x) >> 23) & 0xffu); }
+__device__ __forceinline__ float power_of(int biased) { return __uint_as_float((unsigned)min(max(biased, 1), 254) << 23); }
 
 // Two values (times inv) as planes, packed {low half: a, high half: b}.
 template <int NP>
@@ -298,18 +323,40 @@ __device__ __forceinline__ float warp_max(const float (&x)[NT][4]) {
   return warp_max<NT>(x, all_finite);
 }
 
-// Writes 16 rows (from row block r8) x 16 columns of accumulators, times inv, as
-// NP planes of a tile of 16 columns in shared memory (`plane` elements apart),
+// The largest finite magnitudes of the two rows of a lane in a warp's 16 x 16
+// tile, and whether all of the tile is finite.
+__device__ __forceinline__ void row_max(const float (&x)[2][4], float (&m)[2], bool& all_finite) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    m[e] = max_mag(max_mag(max_mag(fabsf(x[0][2 * e]), x[0][2 * e + 1]), x[1][2 * e]), x[1][2 * e + 1]);
+    m[e] = max_mag(m[e], __shfl_xor_sync(0xffffffffu, m[e], 1));
+    m[e] = max_mag(m[e], __shfl_xor_sync(0xffffffffu, m[e], 2));
+  }
+  all_finite = !__any_sync(0xffffffffu, !finite(m[0]) || !finite(m[1]));
+  if (!all_finite) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      m[e] = 0.0f;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) m[e] = max_finite(max_finite(m[e], x[n][2 * e]), x[n][2 * e + 1]);
+      m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 1));
+      m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 2));
+    }
+  }
+}
+
+// Writes 16 rows (from row block r8) x 16 columns of accumulators, times their
+// row's inv, as NP planes of a tile of 16 columns in shared memory (`plane` elements apart),
 // and into `out`, if given, 16 bytes a lane.  Four blocks of 128 consecutive
 // bytes, which is what stmatrix writes at once.
 template <int NP>
-__device__ __forceinline__ void store_rows(f16* tile, int plane, int r8, const float (&x)[2][4], float inv, f16* out,
-                                           int out_plane) {
+__device__ __forceinline__ void store_rows(f16* tile, int plane, int r8, const float (&x)[2][4], const float (&inv)[2],
+                                           f16* out, int out_plane) {
   uint32_t w[2][2][NP];
 #pragma unroll
   for (int n = 0; n < 2; ++n)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) split2<NP>(x[n][2 * e], x[n][2 * e + 1], inv, w[e][n]);
+    for (int e = 0; e < 2; ++e) split2<NP>(x[n][2 * e], x[n][2 * e + 1], inv[e], w[e][n]);
   const int at = r8 * 128 + (threadIdx.x & 31) * 8;
 #pragma unroll
   for (int p = 0; p < NP; ++p)
@@ -321,6 +368,88 @@ __device__ __forceinline__ void store_rows(f16* tile, int plane, int r8, const f
 #pragma unroll
     for (int p = 0; p < NP; ++p)
       *reinterpret_cast<uint4*>(out + p * out_plane + at) = *reinterpret_cast<const uint4*>(tile + p * plane + at);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Products over tokens: sum_j A_ij x_j, A a token x token matrix (W or P, a 16 x
+// 16 tile of it), x_j tokens whose planes have a scale s_j each.
+//
+// The planes of A leave out c_j = 2^Size_j, about |k_j| e^(G_J - G_j) with J the
+// last of j's 16 tokens (in W, where keys of any size multiply one another, the
+// largest that a column without that decay has in the rows' own measure):
+// A_ij = r_i c_j A'_ij, where r_i is a row's scale, and |A'_ij| spans little.  A tile
+// is then multiplied as A'_ij 2^(w_j - w), w_j the exponent of s_j c_j (of s_j
+// r_j, for sums over A's rows), w the largest of those that the row adds up: in the
+// tile on the diagonal only the tokens up to i (from i on), without i itself in W,
+// whose diagonal is zero.  What falls below FP16's range there is below 2^-24 of a
+// term of the largest size.
+// ---------------------------------------------------------------------------
+
+// A lane's factors for an A fragment, {rows 0-7, 8-15} x {k = 0-7, 8-15}, and the
+// exponents w of its two rows.
+struct Weights {
+  __half2 f[2][2];
+  int top[2];
+};
+
+__device__ __forceinline__ __half2 two_powers(int a, int b) {
+  const float x = __uint_as_float((unsigned)(min(max(a, -60), 0) + 127) << 23);
+  const float y = __uint_as_float((unsigned)(min(max(b, -60), 0) + 127) << 23);
+  return __floats2half2_rn(x, y);
+}
+
+// w: of tokens 2c, 2c + 1, 2c + 8, 2c + 9, c = lane & 3.
+__device__ __forceinline__ Weights whole_weights(const int (&w)[4]) {
+  Weights r;
+  int top = max(max(w[0], w[1]), max(w[2], w[3]));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+#pragma unroll
+  for (int k = 0; k < 2; ++k) r.f[0][k] = r.f[1][k] = two_powers(w[2 * k] - top, w[2 * k + 1] - top);
+  r.top[0] = r.top[1] = top;
+  return r;
+}
+
+// own: of the lane's rows, lane / 4 and lane / 4 + 8.  The largest up to a row, or
+// from it on (DOWN), without it (STRICT).
+template <bool DOWN, bool STRICT>
+__device__ __forceinline__ Weights diagonal_weights(const int (&w)[4], const int (&own)[2]) {
+  Weights r;
+  const int lane = threadIdx.x & 31;
+  int a = own[DOWN ? 1 : 0], b = own[DOWN ? 0 : 1];  // the rows that count first, and the others
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) {
+    const int x = DOWN ? __shfl_down_sync(0xffffffffu, a, o) : __shfl_up_sync(0xffffffffu, a, o);
+    const int y = DOWN ? __shfl_down_sync(0xffffffffu, b, o) : __shfl_up_sync(0xffffffffu, b, o);
+    if (DOWN ? lane + o < 32 : lane >= o) {
+      a = max(a, x);
+      b = max(b, y);
+    }
+  }
+  const int all = __shfl_sync(0xffffffffu, a, DOWN ? 0 : 31);
+  b = max(b, all);
+  if (STRICT) {
+    const int x = DOWN ? __shfl_down_sync(0xffffffffu, a, 4) : __shfl_up_sync(0xffffffffu, a, 4);
+    const int y = DOWN ? __shfl_down_sync(0xffffffffu, b, 4) : __shfl_up_sync(0xffffffffu, b, 4);
+    const bool edge = DOWN ? lane >= 28 : lane < 4;
+    a = edge ? -1024 : x;  // nothing there
+    b = edge ? all : y;
+  }
+  r.top[0] = DOWN ? b : a;
+  r.top[1] = DOWN ? a : b;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) r.f[e][k] = two_powers(w[2 * k] - r.top[e], w[2 * k + 1] - r.top[e]);
+  return r;
+}
+
+__device__ __forceinline__ void weigh(uint32_t (&fa)[4], const Weights& w) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&fa[i]), w.f[i & 1][i >> 1]);
+    fa[i] = *reinterpret_cast<const uint32_t*>(&x);
   }
 }
 

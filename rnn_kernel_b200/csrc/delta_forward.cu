@@ -42,13 +42,19 @@ struct Range {
 constexpr int kLd = 68;  // row length of the FP32 64 x 64 tiles: a multiple of 4, not of 32
 constexpr int kLx = 36;
 
+// The gates that prepare makes, in shared memory: e^G, e^(G_end - G), beta, the
+// exponents of P's columns and of the decays in them, and the logarithms.
+enum Local { kLocalSize = 3, kLocalTail = 4, kLocalLog = 5, kLocal = 7 };
+
 template <typename T, int DK>
 struct PrepareSmem {
   static constexpr int NP = Planes<T>::n;
   static constexpr int planes = 2 * NP * kC * DK * 2;
   static constexpr int tiles = (2 * kC * kLd + kC * kLx) * 4;  // N, W and X, over the planes once those are used up
   static constexpr int main = planes > tiles ? planes : tiles;
-  static constexpr int bytes = main + 2 * kGates * kC * 4 + kC * 4 + 64 * 4;
+  // gates of two value heads, tokens whose key is not finite, the largest
+  // magnitudes of K's and Q's rows (then their scales), W's exponents
+  static constexpr int bytes = main + (2 * kLocal + 5) * kC * 4;
 };
 
 // acc += A B of FP32 tiles in shared memory, 16 rows from m0 and 8 columns
@@ -125,8 +131,9 @@ __device__ __forceinline__ void join_second(const float (&x)[4], float* W, const
 }
 
 // The gates of one value head's chunk, by one warp.  `bad`: tokens whose key is
-// not finite.
-__device__ __forceinline__ void chunk_gates(const Problem& a, int b, int hv, int t0, int rows, const int* bad, float* gates) {
+// not finite; `key`: scales of K's rows.
+__device__ __forceinline__ void chunk_gates(const Problem& a, int b, int hv, int t0, int rows, const int* bad,
+                                            const float* key, float* gates) {
   const int lane = threadIdx.x & 31;
   // sums of log decays in FP64: differences of neighbours stay exact to FP32
   // where the sums are large
@@ -156,8 +163,14 @@ __device__ __forceinline__ void chunk_gates(const Problem& a, int b, int hv, int
     if (lane >= o) s += y;
   }
   const double end = __shfl_sync(0xffffffffu, s, 31);
-  const float top = warp_largest(fmaxf(fabsf(be[0]), fabsf(be[1])));
-  if (lane == 0) gates[5 * kC + 4] = plane_scale(plane_inv(top)) * 32768.0f;
+  // what the planes of P leave out of a token's column: its key's size, in those
+  // of its 16 tokens, and its decay up to the last of them (within bounds that keep
+  // the quotients finite)
+  const int ke[2] = {exponent_of(key[2 * lane]), exponent_of(key[2 * lane + 1])};
+  int kmax = max(ke[0], ke[1]);
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) kmax = max(kmax, __shfl_xor_sync(0xffffffffu, kmax, o));
+  const double last = __shfl_sync(0xffffffffu, s, lane | 7);
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int i = 2 * lane + e;
@@ -166,21 +179,12 @@ __device__ __forceinline__ void chunk_gates(const Problem& a, int b, int hv, int
     gates[kC + i] = expf((float)(end - gi));
     gates[2 * kC + i] = be[e];
     const double g2 = gi * 1.4426950408889634;
-    gates[3 * kC + i] = (float)g2;
-    gates[4 * kC + i] = (float)(g2 - (double)(float)g2);
+    gates[kLocalLog * kC + i] = (float)g2;
+    gates[(kLocalLog + 1) * kC + i] = (float)(g2 - (double)(float)g2);
+    const int decay = (int)fmin(fmax((last - gi) * 1.4426950408889634, -60.0), 60.0);
+    reinterpret_cast<int*>(gates)[kLocalSize * kC + i] = max(decay + max(ke[e] - kmax, -60), -100);
+    reinterpret_cast<int*>(gates)[kLocalTail * kC + i] = max(decay, -30);
   }
-}
-
-// The largest of a value over the CTA (after a barrier).
-__device__ __forceinline__ void put_max(float* red, float m) {
-  const unsigned u = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = __uint_as_float(u);
-}
-__device__ __forceinline__ float get_max(const float* red) {
-  float m = red[0];
-#pragma unroll
-  for (int w = 1; w < kThreads / 32; ++w) m = fmaxf(m, red[w]);
-  return m;
 }
 
 template <typename T, int DK>
@@ -195,8 +199,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
   float* W = N + kC * kLd;
   float* X = W + kC * kLd;
   float* gates2 = reinterpret_cast<float*>(smem + L::main);   // of this value head and of the next
-  int* bad = reinterpret_cast<int*>(gates2 + 2 * kGates * kC);  // tokens whose key is not finite
-  float* red = reinterpret_cast<float*>(bad + kC);         // [4][8] and scales
+  int* bad = reinterpret_cast<int*>(gates2 + 2 * kLocal * kC);  // tokens whose key is not finite
+  float* ksc = reinterpret_cast<float*>(bad + kC);  // of K's rows and of Q's
+  float* qsc = ksc + kC;
+  int* wrow = reinterpret_cast<int*>(qsc + kC);  // exponents of the largest of W's rows, and of its columns
+  int* wcol = wrow + kC;
 
   let_next_start();
   const int part = blockIdx.x % range.parts, block = blockIdx.x / range.parts;
@@ -211,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
   constexpr int am = 4 * sizeof(T) - 1;  // 4-element accesses
   const bool vq = ((reinterpret_cast<uintptr_t>(q) | (a.sq[1] * sizeof(T))) & am) == 0;
   const bool vk = ((reinterpret_cast<uintptr_t>(k) | (a.sk[1] * sizeof(T))) & am) == 0;
-  if (threadIdx.x < kC) bad[threadIdx.x] = 0;
+  if (threadIdx.x < kC) bad[threadIdx.x] = 0, ksc[threadIdx.x] = 0.0f, qsc[threadIdx.x] = 0.0f;
   __syncthreads();
   {
     // A thread's four elements are half a row of a block: item j is elements
@@ -256,49 +263,52 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
       f.x = left > 0 ? f.x : 0.0f, f.y = left > 1 ? f.y : 0.0f, f.z = left > 2 ? f.z : 0.0f, f.w = left > 3 ? f.w : 0.0f;
       return f;
     };
-    float mk = 0.0f, mq = 0.0f;
+    // The largest magnitudes of the rows: those of a thread's items, then of the
+    // lanes that share them (bits 0 and 4), then of the warps.
+    auto largest = [](const float4& f) { return max_mag(max_mag(max_mag(fabsf(f.x), f.y), f.z), f.w); };
+    auto largest_finite = [](const float4& f) {
+      return max_finite(max_finite(max_finite(max_finite(0.0f, f.x), f.y), f.z), f.w);
+    };
+    bool lost = false;
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
       const float4 f = value(kr[x], x), g = value(qr[x], x);
-      mk = max_mag(max_mag(max_mag(max_mag(mk, f.x), f.y), f.z), f.w);
-      mq = max_mag(max_mag(max_mag(max_mag(mq, g.x), g.y), g.z), g.w);
-    }
-    // A key that is not finite spoils its own token and the later ones (see the
-    // gates); inside the products it would reach earlier ones too, so there it
-    // counts as zero.
-    const bool lost = !finite(mk);
-    if (lost) {
-      mk = 0.0f;
+      float mk = largest(f), mq = largest(g);
+      int r, c;
+      place(x, r, c);
+      // A key that is not finite spoils its own token and the later ones (see the
+      // gates); inside the products it would reach earlier ones too, so there it
+      // counts as zero.
+      if (!finite(mk)) {
+        lost = true;
+        bad[r] = 1;
+        mk = largest_finite(f);
+      }
+      if (!finite(mq)) mq = largest_finite(g);
 #pragma unroll
-      for (int x = 0; x < NQ; ++x) {
-        const float4 f = value(kr[x], x);
-        mk = max_finite(max_finite(max_finite(max_finite(mk, f.x), f.y), f.z), f.w);
-        int r, c;
-        place(x, r, c);
-        if (!(finite(f.x) && finite(f.y) && finite(f.z) && finite(f.w))) bad[r] = 1;
+      for (int o = 1; o <= 16; o *= 16) {
+        mk = fmaxf(mk, __shfl_xor_sync(0xffffffffu, mk, o));
+        mq = fmaxf(mq, __shfl_xor_sync(0xffffffffu, mq, o));
+      }
+      if (!(lane & 17)) {  // magnitudes: integer order is theirs
+        atomicMax(reinterpret_cast<int*>(ksc + r), __float_as_int(mk));
+        atomicMax(reinterpret_cast<int*>(qsc + r), __float_as_int(mq));
       }
     }
-    if (!finite(mq)) {
-      mq = 0.0f;
-#pragma unroll
-      for (int x = 0; x < NQ; ++x) {
-        const float4 f = value(qr[x], x);
-        mq = max_finite(max_finite(max_finite(max_finite(mq, f.x), f.y), f.z), f.w);
-      }
-    }
-    put_max(red, mk);
-    put_max(red + 8, mq);
     __syncthreads();
-    const float ik = plane_inv(get_max(red)), iq = plane_inv(get_max(red + 8));
-    if (threadIdx.x == 0) {
-      red[32] = plane_scale(ik);
-      red[33] = plane_scale(iq);
+    if (threadIdx.x < kC) {
+      ksc[threadIdx.x] = plane_scale(plane_inv(ksc[threadIdx.x]));
+      qsc[threadIdx.x] = plane_scale(plane_inv(qsc[threadIdx.x]));
     }
+    __syncthreads();
     f16* ko = a.kp + nk * NP * kC * DK;
     f16* qo = a.qp + nk * NP * kC * DK;
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
       const int at = (threadIdx.x + x * kThreads) * 4;
+      int r, c;
+      place(x, r, c);
+      const float ik = plane_scale(ksc[r]), iq = plane_scale(qsc[r]);  // a power of two's inverse
       float4 f = value(kr[x], x);
       if (lost) {
         f.x = finite(f.x) ? f.x : 0.0f, f.y = finite(f.y) ? f.y : 0.0f;
@@ -330,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
   zero(ak);
   zero(aq);
   // warp 1's tiles are above the diagonal: it makes the first gates meanwhile
-  if (warp == 1) chunk_gates(a, b, h * a.rep + r0, t0, rows, bad, gates2 + (r0 & 1) * kGates * kC);
+  if (warp == 1) chunk_gates(a, b, h * a.rep + r0, t0, rows, bad, ksc, gates2 + (r0 & 1) * kLocal * kC);
   if (n0 <= m0) {
     const uint32_t pk = addr_a<DK, false>(ks, m0 / 8, 0), pq = addr_a<DK, false>(qs, m0 / 8, 0);
     const uint32_t pb = addr_b<DK, false>(ks, 0, n0 / 8);
@@ -356,13 +366,13 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
         }
     }
   }
-  const float sk = red[32], sq = red[33];
 #pragma unroll
   for (int n = 0; n < 4; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      ak[n][e] *= sk * sk;
-      aq[n][e] *= sq * sk;
+      const int i = frag_row(m0, e >> 1), j = frag_col(n0 + n * 8) + (e & 1);
+      ak[n][e] = ak[n][e] * ksc[i] * ksc[j];
+      aq[n][e] = aq[n][e] * qsc[i] * ksc[j];
     }
   __syncthreads();
   for (int x = threadIdx.x; x < kC * kLd; x += kThreads) W[x] = 0.0f;  // above its diagonal blocks it stays zero
@@ -370,9 +380,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
   for (int r = r0; r < r1; ++r) {
     const int hv = h * a.rep + r;
     const long nv = ((long)b * a.Hv + hv) * a.nc + chunk;
-    const float* gates = gates2 + (r & 1) * kGates * kC;
+    const float* gates = gates2 + (r & 1) * kLocal * kC;
+    const int* size = reinterpret_cast<const int*>(gates + kLocalSize * kC);
+    const int* tail = reinterpret_cast<const int*>(gates + kLocalTail * kC);
+    float* out = a.gates + nv * kGates * kC;
     __syncthreads();
-    float mp = 0.0f;
     float pv[4][4];
 #pragma unroll
     for (int n = 0; n < 4; ++n)
@@ -382,27 +394,34 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
         float nn[2];
 #pragma unroll
         for (int l = 0; l < 2; ++l) {
-          const float d = j + l <= i ? decay_between(gates, i, j + l) : 0.0f;
+          const float d = j + l <= i ? decay_between(gates + kLocalLog * kC, i, j + l) : 0.0f;
           nn[l] = j + l < i ? ak[n][2 * e + l] * d : 0.0f;
-          pv[n][2 * e + l] = j + l <= i ? aq[n][2 * e + l] * (d * a.scale) : 0.0f;
-          mp = max_finite(mp, pv[n][2 * e + l]);
+          pv[n][2 * e + l] = j + l <= i ? aq[n][2 * e + l] * (d * a.scale) * power_of(127 - size[j + l]) : 0.0f;
         }
         *reinterpret_cast<float2*>(N + i * kLd + j) = make_float2(nn[0], nn[1]);
       }
-    put_max(red, mp);
-    __syncthreads();
-    const float ip = plane_inv(get_max(red));
     f16* pp = a.pp + nv * 2 * kTile;
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+    for (int n = 0; n < 4; n += 2)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        uint32_t w[2];
-        split2<2>(pv[n][2 * e], pv[n][2 * e + 1], ip, w);
-        const int at = ((m0 / 8 + e) * (kC / 8) + n0 / 8 + n) * 32 + lane;
-        reinterpret_cast<uint32_t*>(pp)[at] = w[0];
-        reinterpret_cast<uint32_t*>(pp + kTile)[at] = w[1];
+        // a row of a 16 x 16 tile, over four lanes
+        float m = max_finite(max_finite(0.0f, pv[n][2 * e]), pv[n][2 * e + 1]);
+        m = max_finite(max_finite(m, pv[n + 1][2 * e]), pv[n + 1][2 * e + 1]);
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const float inv = plane_inv(m);
+        if ((lane & 3) == 0) out[(kScaleP + (n0 + n * 8) / 16) * kC + frag_row(m0, e)] = plane_scale(inv);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[2];
+          split2<2>(pv[n + h][2 * e], pv[n + h][2 * e + 1], inv, w);
+          const int at = ((m0 / 8 + e) * (kC / 8) + n0 / 8 + n + h) * 32 + lane;
+          reinterpret_cast<uint32_t*>(pp)[at] = w[0];
+          reinterpret_cast<uint32_t*>(pp + kTile)[at] = w[1];
+        }
       }
+    __syncthreads();
     // W's 16 x 16 diagonal blocks, a thread per column: W_ic = N_ic - sum_j
     // N_ij beta_j W_jc, every row's term taken off as soon as it is known
     if (threadIdx.x < kC) {
@@ -426,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
     const int o1 = (warp >> 1) * 32, n1 = (warp & 1) * 8;
     if (warp < 4) join_first(jx, N, W, X, o1 + 16, o1, o1 + 16, n1, beta);
     if (warp == 7 && r + 1 < r1)
-      chunk_gates(a, b, hv + 1, t0, rows, bad, gates2 + ((r + 1) & 1) * kGates * kC);
+      chunk_gates(a, b, hv + 1, t0, rows, bad, ksc, gates2 + ((r + 1) & 1) * kLocal * kC);
     __syncthreads();
     if (warp < 4) join_second(jx, W, X, o1 + 16, o1, o1 + 16, n1);
     __syncthreads();
@@ -436,40 +455,71 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
     __syncthreads();
     join_second(jx, W, X, m2, 0, 32, n2);
     __syncthreads();
-    // W's planes: a thread takes two rows of eight elements of the tile's blocks
-    float4 wx[2][2];
-    float mw = 0.0f;
+    // The exponents that W's columns leave out: the decays, and the largest of a
+    // column in its rows' measure.  With keys of norm one that is about the key's
+    // part; a larger key multiplies what later rows hold of earlier columns.
+    {
+      const int row = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
+      int m = -1024;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int j = threadIdx.x + x * kThreads, blk = j >> 3;
-      const float* f = W + ((blk / 8) * 8 + (j & 7)) * kLd + (blk % 8) * 8;
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        wx[x][y] = *reinterpret_cast<const float4*>(f + 4 * y);
-        const float m = max_finite(max_finite(mw, wx[x][y].x), wx[x][y].y);
-        mw = max_finite(max_finite(m, wx[x][y].z), wx[x][y].w);
+      for (int y = 0; y < 16; y += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(W + row * kLd + c + y);
+        m = max(m, max(exponent_of(f.x) - tail[c + y], exponent_of(f.y) - tail[c + y + 1]));
+        m = max(m, max(exponent_of(f.z) - tail[c + y + 2], exponent_of(f.w) - tail[c + y + 3]));
       }
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      if ((threadIdx.x & 3) == 0) wrow[row] = m;
+      if (threadIdx.x < kC) wcol[threadIdx.x] = -1024;
     }
-    put_max(red + 8, mw);
     __syncthreads();
-    const float iw = plane_inv(get_max(red + 8));
+    {
+      const int c = threadIdx.x & (kC - 1), r1 = threadIdx.x / kC * 16;
+      int m = -1024;
+#pragma unroll
+      for (int y = 0; y < 16; ++y) {
+        const float f = W[(r1 + y) * kLd + c];
+        if (f != 0.0f) m = max(m, exponent_of(f) - wrow[r1 + y]);
+      }
+      if (m > -1024) atomicMax(wcol + c, m);
+    }
+    __syncthreads();
+    // (W over it is no larger than its rows' largest over the decays)
+    auto size_w = [&](int c) { return min(max(wcol[c], -100), 60); };
+    // W's planes: a thread takes two rows of eight elements of the tile's blocks;
+    // the next block's same row, of the same scale, is another lane's
     f16* wp = a.wp + nv * 2 * kTile;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
+      const int j = threadIdx.x + x * kThreads, blk = j >> 3, row = (blk / 8) * 8 + (j & 7), c8 = blk % 8;
+      const float* f = W + row * kLd + c8 * 8;
+      float v[8], m = 0.0f;
+#pragma unroll
+      for (int y = 0; y < 8; ++y) {
+        v[y] = f[y] * power_of(127 - size_w(c8 * 8 + y));
+        m = max_finite(m, v[y]);
+      }
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+      const float inv = plane_inv(m);
+      if (!(c8 & 1)) out[(kScaleW + c8 / 2) * kC + row] = plane_scale(inv);
       uint32_t w[4][2];
-      split2<2>(wx[x][0].x, wx[x][0].y, iw, w[0]);
-      split2<2>(wx[x][0].z, wx[x][0].w, iw, w[1]);
-      split2<2>(wx[x][1].x, wx[x][1].y, iw, w[2]);
-      split2<2>(wx[x][1].z, wx[x][1].w, iw, w[3]);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) split2<2>(v[2 * y], v[2 * y + 1], inv, w[y]);
 #pragma unroll
       for (int p = 0; p < 2; ++p)
-        reinterpret_cast<uint4*>(wp + p * kTile)[threadIdx.x + x * kThreads] =
-            make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
+        reinterpret_cast<uint4*>(wp + p * kTile)[j] = make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
     }
-    for (int x = threadIdx.x; x < 5 * kC; x += kThreads) a.gates[nv * kGates * kC + x] = gates[x];
-    if (threadIdx.x < 5) {
-      const float v[5] = {plane_scale(iw), plane_scale(ip), red[32], red[33], gates[5 * kC + 4]};
-      a.gates[nv * kGates * kC + 5 * kC + threadIdx.x] = v[threadIdx.x];
+    if (threadIdx.x < kC) {
+      const int i = threadIdx.x;
+      out[kDecay * kC + i] = gates[i];
+      out[kRest * kC + i] = gates[kC + i];
+      out[kBeta * kC + i] = gates[2 * kC + i];
+      out[kScaleK * kC + i] = ksc[i];
+      reinterpret_cast<int*>(out)[kSizeW * kC + i] = size_w(i);
+      out[kScaleQ * kC + i] = qsc[i];
+      reinterpret_cast<int*>(out)[kSizeP * kC + i] = size[i];
+      out[kLog * kC + i] = gates[kLocalLog * kC + i];
+      out[(kLog + 1) * kC + i] = gates[(kLocalLog + 1) * kC + i];
     }
     __syncthreads();
   }
@@ -497,9 +547,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
 template <int NP, int DK>
 struct ScanSmem {
   static constexpr int k = NP * kC * DK, w = 2 * kTile;  // elements
-  static constexpr int stage = (k + w) * 2 + kGates * kC * 4;
+  static constexpr int stage = (k + w) * 2 + kForward * kC * 4;
   static constexpr int s = 4 * kGroup * DK, x = 4 * kGroup * kC;  // two planes of two groups
-  static constexpr int bytes = 2 * stage + (s + 2 * x) * 2 + 3 * 8 * 4 + kSlice * 4;
+  // scales of S and of U, exponents of B R's tokens, a token for each column
+  static constexpr int bytes = 2 * stage + (s + 2 * x) * 2 + 2 * 8 * 4 + 2 * kC * 4 + kSlice * 4;
 };
 
 template <int NP, int DK>
@@ -508,7 +559,7 @@ __device__ __forceinline__ void scan_load(unsigned char* stage, const Problem& a
   f16* k = reinterpret_cast<f16*>(stage);
   copy_async<L::k * 2, kThreads>(k, a.kp + nk * L::k);
   copy_async<L::w * 2, kThreads>(k + L::k, a.wp + nv * L::w);
-  copy_async<kGates * kC * 4, kThreads>(k + L::k + L::w, a.gates + nv * kGates * kC);
+  copy_async<kForward * kC * 4, kThreads>(k + L::k + L::w, a.gates + nv * kGates * kC);
   cp_async_commit();
 }
 
@@ -519,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
   extern __shared__ __align__(16) unsigned char smem[];
   const int slices = a.dvp / kSlice, groups = a.dvp / kGroup;
   const int bh = blockIdx.x / slices, hv = bh % a.Hv, b = bh / a.Hv;
-  const int lane = threadIdx.x & 31, pair = threadIdx.x >> 7, quarter = quarter_of(threadIdx.x);
+  const int pair = threadIdx.x >> 7, quarter = quarter_of(threadIdx.x);
   const int group = (blockIdx.x % slices) * 2 + pair, c0 = group * kGroup;
   const long nv0 = (long)bh * a.nc, nk0 = ((long)b * a.Hk + hv / a.rep) * a.nc;
   f16* base = reinterpret_cast<f16*>(smem + 2 * L::stage);
@@ -528,9 +579,9 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
   f16* yp = xp + L::x;
   float* scales = reinterpret_cast<float*>(base + L::s + 2 * L::x);
   float* ssc = scales + pair * 4;
-  float* xsc = scales + 8 + pair * 4;
-  float* ysc = scales + 16 + pair * 4;
-  int* first = reinterpret_cast<int*>(scales + 24);  // of each column, the first token that is not finite
+  float* ysc = scales + 8 + pair * 4;
+  int* xex = reinterpret_cast<int*>(scales + 16) + pair * kC;
+  int* first = reinterpret_cast<int*>(scales + 16) + 2 * kC;  // of each column, the first token that is not finite
 
   float s[MT][2][4];
   // a later range goes on from what the one before it left
@@ -572,8 +623,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
     cp_async_wait<0>();
     __syncthreads();
     if (chunk + 1 < end) scan_load<NP, DK>(smem + ((chunk + 1) & 1) * L::stage, a, nk0 + chunk + 1, nv + 1);
-    const float sw = gate[5 * kC], sk = gate[5 * kC + 2];
     const int row[2] = {frag_row(quarter * 16, 0), frag_row(quarter * 16, 1)};  // this lane's tokens
+    const float sk[2] = {gate[kScaleK * kC + row[0]], gate[kScaleK * kC + row[1]]};
 
     float x[2][4];
     times_state<NP, DK>(x, kp, quarter * 2, sp, ssc);
@@ -585,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float eg = gate[row[e]] * sk, be = gate[2 * kC + row[e]];
+          const float eg = gate[row[e]] * sk[e], be = gate[kBeta * kC + row[e]];
           const float2 vv = vt.get(n, e);
           x[n][2 * e] = vv.x - eg * x[n][2 * e];
           x[n][2 * e + 1] = vv.y - eg * x[n][2 * e + 1];
@@ -593,19 +644,22 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
           y[n][2 * e + 1] = be * x[n][2 * e + 1];
         }
       if (chunk + 1 < end) load_v(chunk + 1);
-      bool all_finite;
-      const float inv = plane_inv(warp_max(y, all_finite));
-      if (lane == 0) xsc[quarter] = plane_scale(inv);
-      if (!all_finite) {
-        // What is not finite is left out, since a zero of W times it would
-        // reach earlier tokens, and put back below.
-        off = true;
+      // What is not finite is left out, since a zero of W times it would reach
+      // earlier tokens, and put back below.
+      float m = 0.0f;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = max_mag(m, y[n][e]);
+      off = __any_sync(0xffffffffu, !finite(m));
+      if (off) {
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) y[n][e] = finite(y[n][e]) && finite(x[n][e]) ? y[n][e] : 0.0f;
       }
-      store_rows<2>(xp, 2 * kGroup * kC, quarter * 2, y, inv, nullptr, 0);
+      bool all_finite;
+      put_tokens<2>(y, quarter, xp, xex, nullptr, nullptr, all_finite);
     }
     off = group_sync_or(pair, off);
     if (off) {  // rare, and the same for the whole group
@@ -617,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
       group_sync(pair);
     }
     // E
-    times_tokens<2, 2, false>(x, wp, quarter * 2, xp, 2 * kGroup * kC * 2, xsc, -sw, 0, quarter + 1);
+    times_tokens<2, false, true>(x, wp, gate + kScaleW * kC, reinterpret_cast<const int*>(gate) + kSizeW * kC, quarter, xp, xex, -1.0f);
     if (off) {
       // a later token's error holds every earlier one's
 #pragma unroll
@@ -628,22 +682,17 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
     }
     {
       bool all_finite;
-      const float inv = plane_inv(warp_max(x, all_finite));
-      // a scale below zero marks a quarter that holds something not finite
-      if (lane == 0) a.escale[(nv * groups + group) * 4 + quarter] = all_finite ? plane_scale(inv) : -plane_scale(inv);
-      f16* out = a.e + (nv * groups + group) * 2 * kGroup * kC;
-      store_rows<2>(yp, 2 * kGroup * kC, quarter * 2, x, inv, out, kGroup * kC);  // yp: on the way only
+      put_tokens<2>(x, quarter, yp, nullptr, a.e + (nv * groups + group) * 2 * kGroup * kC,
+                    a.escale + (nv * groups + group) * kC, all_finite);  // yp: on the way only
     }
     // S <- e^G S + K^T (e^(G_end - G) U)
     {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[n][e] *= gate[kC + row[e >> 1]] * gate[2 * kC + row[e >> 1]];
-      const float inv = plane_inv(warp_max(x));
-      if (lane == 0) ysc[quarter] = plane_scale(inv);
+        for (int e = 0; e < 4; ++e) x[n][e] *= gate[kRest * kC + row[e >> 1]] * gate[kBeta * kC + row[e >> 1]] * sk[e >> 1];
       __syncwarp();
-      store_rows<2>(yp, 2 * kGroup * kC, quarter * 2, x, inv, nullptr, 0);
+      put_sum(x, quarter, yp, ysc);
     }
     group_sync(pair);
     if (off && (threadIdx.x & 127) < kGroup) first[pair * kGroup + (threadIdx.x & 127)] = kC;
@@ -654,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[m][n][e] *= decay;
-    add_to_state<NP, DK>(s, kp, quarter, yp, ysc, sk);
+    add_to_state<NP, DK>(s, kp, quarter, yp, ysc);
     state_out(chunk + 1);
   }
   float* last = a.s_out + (long)bh * a.dk * a.dv;
@@ -682,9 +731,9 @@ struct OutputSmem {
   static constexpr int cols = 64;
   static constexpr int q = Planes<T>::n * kC * DK, p = 2 * kTile;  // elements
   static constexpr int s = 2 * cols * DK, e = 2 * cols * kC;
-  static constexpr int slice = s + e + 2 * 32;  // and the scales of S and E, four groups and quarters
+  static constexpr int slice = s + e + 2 * (16 + 4 * kC);  // and the scales of S (four groups and quarters) and of E
   static constexpr int buffers = (q + p + 2 * slice) * 2 > 96 * 1024 ? 1 : 2;
-  static constexpr int bytes = (q + p + buffers * slice) * 2 + kGates * kC * 4;
+  static constexpr int bytes = (q + p + buffers * slice) * 2 + (kBackward + 1) * kC * 4;
 };
 
 template <typename T, int DK>
@@ -697,34 +746,18 @@ __device__ __forceinline__ void output_load(f16* dst, const Problem& a, long nv,
     copy_async<2 * kGroup * DK * 2, kThreads>(dst + g * 2 * kGroup * DK, a.states + (first + g) * 2 * kGroup * DK);
     copy_async<2 * kGroup * kC * 2, kThreads>(dst + L::s + g * 2 * kGroup * kC, a.e + (first + g) * 2 * kGroup * kC);
   }
-  if (threadIdx.x < 8) {
-    const int g = threadIdx.x & 3;
+  if (threadIdx.x < 4 + 4 * 16) {
+    const int t = threadIdx.x - 4, g = t < 0 ? threadIdx.x : t >> 4;
     if (c0 + g * kGroup < a.dvp)
-      cp_async16(dst + L::s + L::e + threadIdx.x * 8, (threadIdx.x < 4 ? a.sscale : a.escale) + (first + g) * 4);
+      cp_async16(dst + L::s + L::e + threadIdx.x * 8, t < 0 ? a.sscale + (first + g) * 4 : a.escale + (first + g) * kC + (t & 15) * 4);
   }
   cp_async_commit();
 }
 
-// acc (two groups of 16 columns) += A B, one step of 16; both groups' scales are
-// scale[0] and scale[4].
-template <int NA, int TILE>
-__device__ __forceinline__ void output_step(float (&acc)[4][4], const uint32_t (&fa)[NA][4], uint32_t pb, const float* scale) {
-  uint32_t fb[2][4][2];
-  load_b<2, 4, true>(fb, pb, 2 * TILE * 2, TILE * 2);
-  float t[4][4];
-  mma_terms<NA, 2, 4>(t, fa, fb);
-#pragma unroll
-  for (int n = 0; n < 4; ++n) {
-    const float f = scale[(n >> 1) * 4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[n][e] += f * t[n][e];
-  }
-}
-
-// An element of P U (without the scales of P and B), for a chunk with an error that is not
-// finite: the zeros of P above its diagonal would spread it to earlier tokens.
-__device__ __noinline__ float output_element(const f16* pp, const f16* ep, int plane, const float* scale,
-                                             int i, int c) {
+// An element of P U, for a chunk with an error that is not finite: the zeros of P
+// above its diagonal would spread it to earlier tokens.
+__device__ __noinline__ float output_element(const f16* pp, const float* rows, const int* size, const f16* ep, int plane,
+                                             const float* scale, int i, int c) {
   float sum = 0.0f;
   for (int j = 0; j <= i; ++j) {
     const int ip = ((i >> 3) * 8 + (j >> 3)) * 64 + (i & 7) * 8 + (j & 7);
@@ -734,7 +767,7 @@ __device__ __noinline__ float output_element(const f16* pp, const f16* ep, int p
       u += __half2float(pp[p * kTile + ip]);
       w += __half2float(ep[p * plane + ie]);
     }
-    sum += fabsf(scale[j >> 4]) * (u * w);
+    sum += (rows[(j >> 4) * kC + i] * power_of(size[j] + 127)) * (fabsf(scale[j]) * (u * w));
   }
   return sum;
 }
@@ -755,7 +788,8 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
   wait_for_before();
   copy_async<L::q * 2, kThreads>(qp, a.qp + nk * L::q);
   copy_async<L::p * 2, kThreads>(pp, a.pp + nv * L::p);
-  copy_async<kGates * kC * 4, kThreads>(gate, a.gates + nv * kGates * kC);
+  copy_async<kBackward * kC * 4, kThreads>(gate, a.gates + nv * kGates * kC);
+  int* size = reinterpret_cast<int*>(gate + kBackward * kC);  // P's, with the exponents of beta
   output_load<T, DK>(slices, a, nv, 0);
   const int warp = threadIdx.x >> 5;
   // rows of 1 and 4 steps of P to two of the SM's quarters, of 2 and 3 to the others
@@ -768,12 +802,19 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
     cp_async_wait<0>();
     __syncthreads();
     if (c0 == 0) {
-      // P -> P B in place, eight columns at a time
-      const float ib = 1.0f / gate[5 * kC + 4];  // a power of two
+      // P -> P B in place, eight columns at a time, but for powers of two that
+      // leave |beta| in [1/2, 1]
+      if (threadIdx.x < kC) {
+        float& be = gate[kBeta * kC + threadIdx.x];
+        const int up = exponent_of(be) + 1;  // of the least power above it, biased
+        size[threadIdx.x] = reinterpret_cast<const int*>(gate)[kSizeP * kC + threadIdx.x] + up - 127;
+        be *= power_of(254 - up);
+      }
+      __syncthreads();
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int row = threadIdx.x + i * kThreads;  // of 8 elements
-        const float* be = gate + 2 * kC + ((row >> 3) & 7) * 8;
+        const float* be = gate + kBeta * kC + ((row >> 3) & 7) * 8;
         uint32_t r[2][4];
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
@@ -784,7 +825,7 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
         for (int j = 0; j < 4; ++j) {
           const float2 f = pair(r[0][j], r[1][j]);
           uint32_t w[2];
-          split2<2>(f.x * be[2 * j], f.y * be[2 * j + 1], ib, w);
+          split2<2>(f.x * be[2 * j], f.y * be[2 * j + 1], 1.0f, w);
           r[0][j] = w[0], r[1][j] = w[1];
         }
 #pragma unroll
@@ -802,7 +843,7 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
     const int cw = c0 + half * 32;  // this warp's columns; those it has are whole slices
     if (cw < a.dvp) {
       const float* fs = reinterpret_cast<const float*>(ep + L::e) + half * 8;
-      const float* fe = fs + 16;
+      const float* fe = reinterpret_cast<const float*>(ep + L::e) + 16 + half * 2 * kC;
       const f16* sg = sp + half * 4 * kGroup * DK;
       const f16* eg = ep + half * 4 * kGroup * kC;
       float x[4][4], y[4][4];
@@ -813,43 +854,80 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
         constexpr int per = DK / 64;  // steps to a scale
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
-          uint32_t fa[NP][4];
+          uint32_t fa[NP][4], fb[2][4][2];
 #pragma unroll
           for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], pa + kk * 256 + p * kC * DK * 2);
-          output_step<NP, kGroup * DK>(x, fa, pb + kk * 512, fs + kk / per);
+          load_b<2, 4, true>(fb, pb + kk * 512, 2 * kGroup * DK * 2, kGroup * DK * 2);
+          float t[4][4];
+          mma_terms<NP, 2, 4>(t, fa, fb);
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[n][e] += fs[kk / per + (n >> 1) * 4] * t[n][e];
         }
       }
       bool lost = false;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) lost |= fe[i] < 0.0f;
-      const float fy = gate[5 * kC + 1] * gate[5 * kC + 4];
+      for (int i = 0; i < 8; ++i) lost |= fe[i * 16] < 0.0f;
+      const float* rows_p = gate + kScaleP * kC;
       if (lost) {
 #pragma unroll
         for (int n = 0; n < 4; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            y[n][e] = output_element(pp, eg + (n >> 1) * 2 * kGroup * kC, kGroup * kC, fe + (n >> 1) * 4,
-                                         frag_row(m0, e >> 1), frag_col((n & 1) * 8) + (e & 1));
+            y[n][e] = output_element(pp, rows_p, size, eg + (n >> 1) * 2 * kGroup * kC, kGroup * kC, fe + (n >> 1) * kC,
+                                     frag_row(m0, e >> 1), frag_col((n & 1) * 8) + (e & 1));
       } else {
         const uint32_t pa = addr_a<kC, false>(pp, m0 / 8, 0), pb = addr_b<kGroup, true>(eg, 0, 0);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           if (kk > m0 / 16) break;
-          uint32_t fa[2][4];
+          uint32_t fp[2][4], fb[2][4][2];
 #pragma unroll
-          for (int p = 0; p < 2; ++p) ldm4<false>(fa[p], pa + kk * 256 + p * kTile * 2);
-          output_step<2, kGroup * kC>(y, fa, pb + kk * 512, fe + kk);
+          for (int p = 0; p < 2; ++p) ldm4<false>(fp[p], pa + kk * 256 + p * kTile * 2);
+          load_b<2, 4, true>(fb, pb + kk * 512, 2 * kGroup * kC * 2, kGroup * kC * 2);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const float* se = fe + g * kC;
+            auto weight = [&](int j) { return exponent_of(se[j]) + size[j]; };
+            const int c = kk * 16 + (threadIdx.x & 3) * 2;
+            const int w[4] = {weight(c), weight(c + 1), weight(c + 8), weight(c + 9)};
+            Weights f;
+            if (kk == m0 / 16) {
+              const int own[2] = {weight(frag_row(m0, 0)), weight(frag_row(m0, 1))};
+              f = diagonal_weights<false, false>(w, own);
+            } else {
+              f = whole_weights(w);
+            }
+            uint32_t fa[2][4], fg[2][2][2];
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) fa[p][i] = fp[p][i], fg[p][i >> 1][i & 1] = fb[p][2 * g + (i >> 1)][i & 1];
+              weigh(fa[p], f);
+            }
+            float t[2][4];
+            mma_terms<2, 2, 2>(t, fa, fg);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float r = rows_p[kk * kC + frag_row(m0, e)] * power_of(f.top[e]);
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                y[2 * g + n][2 * e] += r * t[n][2 * e];
+                y[2 * g + n][2 * e + 1] += r * t[n][2 * e + 1];
+              }
+            }
+          }
         }
       }
-      const float fx = a.scale * gate[5 * kC + 3];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = frag_row(m0, e);
-        const float f = gate[row] * fx;
+        const float f = gate[row] * gate[kScaleQ * kC + row] * a.scale;
         float2 z[4];
 #pragma unroll
         for (int n = 0; n < 4; ++n)
-          z[n] = make_float2(f * x[n][2 * e] + fy * y[n][2 * e], f * x[n][2 * e + 1] + fy * y[n][2 * e + 1]);
+          z[n] = make_float2(f * x[n][2 * e] + y[n][2 * e], f * x[n][2 * e + 1] + y[n][2 * e + 1]);
         set_row<T>(o + (long)row * a.Hv * a.dv + cw, a.dv - cw, vec, whole, row < rows, z);
       }
     }

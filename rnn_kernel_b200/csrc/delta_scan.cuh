@@ -58,41 +58,91 @@ __device__ __forceinline__ void times_state(float (&x)[2][4], const f16* kp, int
   }
 }
 
-// x += A B over steps [k0, k1): A a 64 x 64 tile (16 rows at m8, or transposed),
-// B 64 tokens x 16 columns as NB planes (`plane` bytes apart) with a scale for
-// each step.
-template <int NA, int NB, bool TA>
-__device__ __forceinline__ void times_tokens(float (&x)[2][4], const f16* A, int m8, const f16* B, int plane,
-                                             const float* scale, float factor, int k0, int k1) {
+// x += sign A B (UP: A^T B) for the 16 tokens of `quarter`, over the tokens up to
+// (from) them: A a lower 64 x 64 tile as planes, with the scales of its rows and
+// the sizes that its columns leave out; B 64 tokens x 16 columns as NB planes with
+// the exponents of its tokens' scales.  STRICT: A's diagonal is zero.
+template <int NB, bool UP, bool STRICT>
+__device__ __forceinline__ void times_tokens(float (&x)[2][4], const f16* A, const float* scale, const int* size, int quarter,
+                                             const f16* B, const int* exponent, float sign) {
+  constexpr int plane = 2 * kGroup * kC * 2;
+  const int lane = threadIdx.x & 31, c = (lane & 3) * 2, r = quarter * 16 + (lane >> 2);
+  // the exponents that a token of the sum brings
+  auto weight = [&](int t) {
+    return exponent[t] + (UP ? exponent_of(scale[quarter * kC + t]) - 127 : size[t]);
+  };
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) {
-    if (kk < k0 || kk >= k1) continue;
-    uint32_t fa[NA][4], fb[NB][2][2];
-    const uint32_t pa = addr_a<kC, TA>(A, m8, 2 * kk);
+    if (UP ? kk < quarter : kk > quarter) continue;
+    const int w[4] = {weight(kk * 16 + c), weight(kk * 16 + c + 1), weight(kk * 16 + c + 8), weight(kk * 16 + c + 9)};
+    Weights f;
+    if (kk == quarter) {
+      const int own[2] = {weight(r), weight(r + 8)};
+      f = diagonal_weights<UP, STRICT>(w, own);
+    } else {
+      f = whole_weights(w);
+    }
+    uint32_t fa[2][4], fb[NB][2][2];
+    const uint32_t pa = addr_a<kC, UP>(A, quarter * 2, 2 * kk);
 #pragma unroll
-    for (int p = 0; p < NA; ++p) ldm4<TA>(fa[p], pa + p * kTile * 2);
+    for (int p = 0; p < 2; ++p) {
+      ldm4<UP>(fa[p], pa + p * kTile * 2);
+      weigh(fa[p], f);
+    }
     load_b<NB, 2, true>(fb, addr_b<kGroup, true>(B, 2 * kk, 0), 0, plane);
     float t[2][4];
-    mma_terms<NA, NB, 2>(t, fa, fb);
-    const float f = factor * scale[kk];
+    mma_terms<2, NB, 2>(t, fa, fb);
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int e = 0; e < 2; ++e) {
+      const float g = sign * power_of(f.top[e]) * (UP ? power_of(size[r + 8 * e] + 127) : scale[kk * kC + r + 8 * e]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[n][e] += f * t[n][e];
+      for (int n = 0; n < 2; ++n) {
+        x[n][2 * e] += g * t[n][2 * e];
+        x[n][2 * e + 1] += g * t[n][2 * e + 1];
+      }
+    }
   }
 }
 
+// A warp's 16 tokens x 16 columns as NP planes with a scale for each token: planes
+// and exponents in shared memory and, if given, planes and scales in `out`.
+template <int NP>
+__device__ __forceinline__ void put_tokens(const float (&x)[2][4], int quarter, f16* tile, int* exponent, f16* out,
+                                           float* out_scale, bool& all_finite) {
+  float m[2];
+  row_max(x, m, all_finite);
+  const float inv[2] = {plane_inv(m[0]), plane_inv(m[1])};
+  const int lane = threadIdx.x & 31, r = quarter * 16 + (lane >> 2);
+  if ((lane & 3) == 0) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float s = plane_scale(inv[e]);
+      if (exponent) exponent[r + 8 * e] = exponent_of(s);
+      // below zero: the 16 tokens hold something that is not finite
+      if (out_scale) out_scale[r + 8 * e] = all_finite ? s : -s;
+    }
+  }
+  store_rows<NP>(tile, 2 * kGroup * kC, quarter * 2, x, inv, out, kGroup * kC);
+}
+
+// The same with one scale, for a sum over all of a chunk's tokens.
+__device__ __forceinline__ void put_sum(const float (&x)[2][4], int quarter, f16* tile, float* scale) {
+  const float i = plane_inv(warp_max(x)), inv[2] = {i, i};
+  if ((threadIdx.x & 31) == 0) scale[quarter] = plane_scale(i);
+  store_rows<2>(tile, 2 * kGroup * kC, quarter * 2, x, inv, nullptr, 0);
+}
+
 // s (this warp's quarter of the key columns x 16) += K^T X, X 64 tokens x 16
-// columns as two planes with a scale for each 16 tokens.
+// columns, with K's scales in it, as two planes with a scale for each 16 tokens.
 template <int NP, int DK>
 __device__ __forceinline__ void add_to_state(float (&s)[DK / 64][2][4], const f16* kp, int quarter, const f16* X,
-                                             const float* scale, float factor) {
+                                             const float* scale) {
   constexpr int MT = DK / 64;
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) {
     uint32_t fb[2][2][2];
     load_b<2, 2, true>(fb, addr_b<kGroup, true>(X, 2 * kk, 0), 0, 2 * kGroup * kC * 2);
-    const float f = factor * scale[kk];
+    const float f = scale[kk];
     float t[MT][2][4];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -135,10 +185,10 @@ __device__ __forceinline__ void put_state(const float (&s)[DK / 64][2][4], int q
         for (int e = 0; e < 4; ++e) m = max_finite(m, s[i][n][e]);
     m = warp_largest(m);
   }
-  const float inv = plane_inv(m);
+  const float i0 = plane_inv(m), inv[2] = {i0, i0};
   if ((threadIdx.x & 31) == 0) {
-    scale[quarter] = plane_scale(inv);
-    if (out) out_scale[quarter] = plane_scale(inv);
+    scale[quarter] = plane_scale(i0);
+    if (out) out_scale[quarter] = plane_scale(i0);
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i)

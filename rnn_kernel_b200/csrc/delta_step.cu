@@ -209,18 +209,18 @@ void lay_forward(Problem& a, const gru_delta_args& p, Arena& m) {
   a.states = m.take<f16>(nv * 2 * a.dvp * w);
   a.sscale = m.take<float>(nv * groups * 4);
   a.e = m.take<f16>(nv * 2 * a.dvp * kC);
-  a.escale = m.take<float>(nv * groups * 4);
+  a.escale = m.take<float>(nv * groups * kC);
 }
 
 void lay_backward(Problem& a, const gru_delta_args& p, Arena& m) {
   const size_t nk = (size_t)a.B * a.Hk * a.nc, nv = (size_t)a.B * a.Hv * a.nc, w = key_width(p);
   const size_t np = p.dtype == GRU_F32 ? 2 : 1, groups = a.dvp / kGroup;
   a.z = m.take<f16>(nv * 2 * a.dvp * kC);
-  a.zscale = m.take<float>(nv * groups * 4);
+  a.zscale = m.take<float>(nv * groups * kC);
   a.dstates = m.take<f16>(nv * 2 * a.dvp * w);
   a.dsscale = m.take<float>(nv * groups * 4);
   a.dop = m.take<f16>(nv * np * a.dvp * kC);
-  a.doscale = m.take<float>(nv * groups * 4);
+  a.doscale = m.take<float>(nv * groups * kC);
   a.dqk = m.take<float>(a.rep > 1 ? nk * 2 * kC * w : 0);
 }
 

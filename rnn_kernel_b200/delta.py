@@ -11,8 +11,13 @@ decay ``g_t`` and writing strength ``beta_t``, does::
 * :class:`GatedDelta` is the layer around them, with :class:`GRU`'s calling
   convention: ``(input, state) -> (output, state)``.
 
-q, k and v are FP32 or bf16, gates and states FP32; products and sums are FP32
-throughout.  Value heads may outnumber key heads (``Hv = n Hk``: value head h
+q, k and v are FP32 or bf16, gates and states FP32.  Sums are FP32; what the
+tensor cores multiply keeps 22 bits down to 2^-17 of the largest number that
+shares its scale, and 2^-39 of that below.  A token's head of q and of k has a
+scale of its own, and 16 of its values (of 16 neighbouring value columns) have:
+no token loses digits to another's size.  A value or key column far smaller than
+its neighbours does lose them to those: below 2^-17 of the largest of the 16
+value columns, or of the token's key.  Value heads may outnumber key heads (``Hv = n Hk``: value head h
 reads key head ``h // n``).  Shape problems raise ``ValueError``, device and
 dtype problems and CUDA failures ``RuntimeError``; there is no CPU fallback.
 """

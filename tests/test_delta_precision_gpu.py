@@ -24,3 +24,68 @@ def test_bf16_outputs_are_fp32_results_rounded_once(size, train):
         out, _ = gated_delta_rule(*x[:5], initial_state=x[5])
     want, _ = R.rule(*(t.detach() for t in x))
     assert float((out.detach() != want.bfloat16()).float().mean()) <= 0.01
+
+
+def plain(x, do=None, ds=None, dtype=torch.float64):
+    """The recurrence token by token in `dtype`: out, last state and, with do and ds, every input's gradient."""
+    x = [t.detach().to(dtype).requires_grad_(do is not None) for t in x]
+    q, k, v, g, beta, s = x
+    Hv, dk = v.shape[2], q.shape[3]
+    qr, kr = (t.repeat_interleave(Hv // t.shape[2], dim=2) for t in (q, k))
+    outs = []
+    for t in range(q.shape[1]):
+        s = s * g[:, t].exp()[..., None, None]
+        u = beta[:, t, :, None] * (v[:, t] - (s * kr[:, t, :, :, None]).sum(-2))
+        s = s + kr[:, t, :, :, None] * u[..., None, :]
+        outs.append((s * qr[:, t, :, :, None]).sum(-2) * dk ** -0.5)
+    out = torch.stack(outs, 1)
+    if do is None:
+        return out, s
+    return (out, s) + torch.autograd.grad((out, s), x, (do.to(dtype), ds.to(dtype)))
+
+
+NAMES = ("out", "state", "dq", "dk", "dv", "dg", "dbeta", "dstate")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("power", [20, 30, 40])
+@pytest.mark.parametrize("what", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("dk", [64, 128])
+def test_a_large_token_leaves_the_others_their_digits(what, power, dtype, dk):
+    """One token's q, k, v or output gradient is 2^20 to 2^40 times the others', amid its 16 tokens and its chunk.  Each
+    token's vectors (each stretch's numbers: before it, it, after it) are as exact as FP32 arithmetic leaves them.
+
+    The allowance, of a token's own size: 1e-5 in FP32 (2e-6 bounds whole tensors, see test_delta_gpu.py; a single token
+    may cancel a few times as much), 3e-3 where the result is bf16; and 16 times the error of the plain FP32 recurrence in
+    the same stretch (root mean square), since planes keep 22 bits of 24 and chunks take some four products in turn."""
+    T, t = 150, 75
+    x = list(R.inputs(1, T, 1, 2, dk, 48, dtype=dtype, seed=power))
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(power + 1)
+    do = torch.randn(1, T, 2, 48, device="cuda", generator=gen).to(dtype)
+    ds = torch.randn(1, 2, dk, 48, device="cuda", generator=gen)
+    for name, i in (("q", 0), ("k", 1), ("v", 2)):
+        if what == name:
+            x[i][:, t] *= 2.0 ** power
+    if what == "dout":
+        do[:, t] *= 2.0 ** power
+    mine = [y.clone().requires_grad_(True) for y in x]
+    out, last = gated_delta_rule(*mine[:5], initial_state=mine[5])
+    got = (out.detach(), last.detach()) + torch.autograd.grad((out, last), mine, (do, ds))
+    want, rough = plain(x, do, ds), plain(x, do, ds, torch.float32)
+    for name, a, b, c in zip(NAMES, got, want, rough):
+        assert torch.isfinite(a).all(), name
+        allowed = 3e-3 if a.dtype == torch.bfloat16 else 1e-5
+        a, c = a.double(), c.double()
+        if name in ("state", "dstate"):
+            assert float((a - b).norm()) <= allowed * float(b.norm()) + 16 * float((c - b).norm()), name
+            continue
+        for part in (slice(0, t), slice(t, t + 1), slice(t + 1, T)):
+            err, rerr, size = ((y[:, part]) for y in (a - b, c - b, b))
+            if name in ("dg", "dbeta"):  # numbers: a stretch of one head's
+                err, rerr, size = (y.norm(dim=1) for y in (err, rerr, size))
+            else:
+                err, rerr, size = (y.norm(dim=-1) for y in (err, rerr, size))
+            rough_rel = float((rerr / size).square().mean().sqrt())
+            worst = float((err / size).max())
+            assert worst <= allowed + 16 * rough_rel, (name, part, worst, rough_rel)
