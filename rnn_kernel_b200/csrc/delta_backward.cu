@@ -41,8 +41,8 @@ struct BackSmem {
   static constexpr int stage = 2 * (k + w) * 2 + kBackward * kC * 4;
   // two planes of two groups (of dO, NP): dS, B dU, e^G B Z, e^G dO; dO
   static constexpr int s = 4 * kGroup * DK, x = 4 * kGroup * kC, o = NP * 2 * kGroup * kC;
-  // scales of dS, e^G B Z and e^G dO, exponents of B dU's and dO's tokens
-  static constexpr int bytes = STAGES * stage + (s + 3 * x + o) * 2 + 3 * 8 * 4 + 4 * kC * 4;
+  // scales of dS, e^G B Z and e^G dO, weights of B dU's and dO's tokens
+  static constexpr int bytes = STAGES * stage + (s + 3 * x + o) * 2 + 3 * 8 * 4 + 4 * (kC * 2 + 4 * 4);
 };
 
 template <int NP, int DK>
@@ -78,9 +78,13 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
   f16* op = base + L::s + 3 * L::x + pair * kGroup * kC;
   float* scales = reinterpret_cast<float*>(base + L::s + 3 * L::x + L::o) + pair * 4;
   float *ssc = scales, *zsc = scales + 8, *qosc = scales + 16;
-  int* uex = reinterpret_cast<int*>(scales - pair * 4 + 24) + pair * kC;
-  int* oex = uex + 2 * kC;
-  bool all_finite;
+  int* utop = reinterpret_cast<int*>(scales - pair * 4 + 24) + pair * 4;
+  int* otop = utop + 8;
+  __half* ufactor = reinterpret_cast<__half*>(scales - pair * 4 + 40) + pair * kC;
+  __half* ofactor = ufactor + 2 * kC;
+  const int row[2] = {frag_row(quarter * 16, 0), frag_row(quarter * 16, 1)};  // this lane's tokens
+  int ow[2];    // exponents of their dO's scales and of P's rows
+  int next[2];  // those, of the chunk whose dO is loaded
 
   float d[MT][2][4];  // the gradient of the state after the chunk
   const float* ds = a.ds_out ? a.ds_out + (long)bh * a.dk * a.dv : nullptr;
@@ -103,6 +107,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
   auto load_dout = [&](int chunk) {
     const int t = chunk * kC + quarter * 16;
     od.start(dout + (dout ? t * stride : 0), stride, dout ? a.T - t : 0, cols, vec);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) next[e] = reinterpret_cast<const int*>(a.gates)[((nv0 + chunk) * kGates + kRowP) * kC + row[e]];
   };
   auto dout_tile = [&](float (&x)[2][4]) {
 #pragma unroll
@@ -118,8 +124,11 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
     float x[2][4];
     dout_tile(x);
     const long nv = nv0 + chunk;
-    put_tokens<NP>(x, quarter, op, oex, a.dop + (nv * groups + group) * NP * kGroup * kC,
-                   a.doscale + (nv * groups + group) * kC, all_finite);
+    put_tokens<NP>(x, quarter, op, ow, a.dop + (nv * groups + group) * NP * kGroup * kC,
+                   a.doscale + (nv * groups + group) * kC);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) ow[e] += next[e];
+    put_weights(ow, quarter, ofactor, otop);
   };
   auto state_out = [&](int chunk) {
     const long nv = nv0 + chunk;
@@ -144,10 +153,10 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
       buf ^= 1;
       back_load<NP, DK>(smem + buf * L::stage, a, nk0 + chunk - 1, nv - 1);
     }
-    const int* size = reinterpret_cast<const int*>(gate);
-    const int row[2] = {frag_row(quarter * 16, 0), frag_row(quarter * 16, 1)};
+    const int* whole = reinterpret_cast<const int*>(gate);
     const float sk[2] = {gate[kScaleK * kC + row[0]], gate[kScaleK * kC + row[1]]};
     float x[2][4], y[2][4];
+    Weights diagonal = diagonal_weights<true, false>(ow);
     // scale e^G dO, for Q^T
     dout_tile(x);
     if (chunk > 0) load_dout(chunk - 1);
@@ -162,17 +171,31 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[n][e] *= sk[e >> 1] * gate[kRest * kC + row[e >> 1]];
-    times_tokens<NP, true, false>(x, pp, gate + kScaleP * kC, size + kSizeP * kC, quarter, op, oex, 1.0f);
+    {
+      const int left[2] = {whole[kColumnP * kC + row[0]], whole[kColumnP * kC + row[1]]};
+      times_tokens<NP, true>(x, pp, left, quarter, op, diagonal, ofactor, otop, 1.0f);
+    }
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[n][e] = x[n][e] * gate[kBeta * kC + row[e >> 1]];
-    put_tokens<2>(y, quarter, up, uex, nullptr, nullptr, all_finite);
+    {
+      int w[2];
+      put_tokens<2>(y, quarter, up, w, nullptr, nullptr);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) w[e] += whole[kRowW * kC + row[e]];
+      put_weights(w, quarter, ufactor, utop);
+      diagonal = diagonal_weights<true, true>(w);
+    }
     group_sync(pair);
     // Z and dV
-    times_tokens<2, true, true>(x, wp, gate + kScaleW * kC, size + kSizeW * kC, quarter, up, uex, -1.0f);
-    put_tokens<2>(x, quarter, zp, nullptr, a.z + (nv * groups + group) * 2 * kGroup * kC,
-                  a.zscale + (nv * groups + group) * kC, all_finite);  // zp: on the way only
+    {
+      const int left[2] = {whole[kColumnW * kC + row[0]], whole[kColumnW * kC + row[1]]};
+      times_tokens<2, true>(x, wp, left, quarter, up, diagonal, ufactor, utop, -1.0f);
+      int w[2];
+      put_tokens<2>(x, quarter, zp, w, a.z + (nv * groups + group) * 2 * kGroup * kC,
+                    a.zscale + (nv * groups + group) * kC);  // zp: on the way only
+    }
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll

@@ -11,8 +11,8 @@
 // the largest, and 2^-39 of it below.
 //
 // What shares a scale.  Of K, Q, the errors and the gradients of outputs: a
-// token's head, or 16 value columns of it.  Of W and P: a token's 16 earlier
-// tokens, without those tokens' own sizes (Weights, below).  So no token's
+// token's head, or 16 value columns of it.  Of W and P: a token's row, without the
+// other tokens' own sizes and the decays between (Weights, below).  So no token's
 // result depends on another's magnitude but through the rule itself.  Of a state
 // and its gradient, which have no tokens: a quarter of the key columns x 16 value
 // columns; of what a chunk adds to a state: 16 tokens x 16 value columns.
@@ -46,15 +46,15 @@ enum Gate {
   kRest = 1,     // e^(G_end - G_i)
   kBeta = 2,
   kScaleK = 3,   // of the planes of K
-  kSizeW = 4,    // the exponents (integers) that W's columns leave out, see Weights
-  kScaleW = 5,   // of the planes of W, 4 rows: 16 columns each
-  kForward = 9,  // rows that the forward scan needs
-  kScaleQ = 9,
-  kScaleP = 10,  // as W's
-  kSizeP = 14,
-  kBackward = 15,
-  kLog = 15,     // G_i / log 2 as two floats
-  kGates = 17
+  kColumnW = 4,  // exponents (integers) of what the planes of W leave out, see Weights
+  kRowW = 5,
+  kForward = 6,  // rows that the forward scan needs
+  kScaleQ = 6,
+  kColumnP = 7,
+  kRowP = 8,
+  kBackward = 9,
+  kLog = 9,      // G_i / log 2 as two floats
+  kGates = 11
 };
 
 // Log decays below this count as this: e^-1000 is zero in FP32, and sums of 64
@@ -228,10 +228,11 @@ __device__ __forceinline__ void load_b(uint32_t (&fb)[NB][NT][2], uint32_t addr,
     }
 }
 
-// e^(G_i - G_j) from the two rows of logarithms.
-__device__ __forceinline__ float decay_between(const float* log, int i, int j) {
-  return exp2f((log[i] - log[j]) + (log[kC + i] - log[kC + j]));
+// The logarithm of e^(G_i - G_j), from its two rows, and that.
+__device__ __forceinline__ float log_between(const float* log, int i, int j) {
+  return (log[i] - log[j]) + (log[kC + i] - log[kC + j]);
 }
+__device__ __forceinline__ float decay_between(const float* log, int i, int j) { return exp2f(log_between(log, i, j)); }
 
 template <int NT>
 __device__ __forceinline__ void zero(float (&acc)[NT][4]) {
@@ -372,18 +373,22 @@ __device__ __forceinline__ void store_rows(f16* tile, int plane, int r8, const f
 }
 
 // ---------------------------------------------------------------------------
-// Products over tokens: sum_j A_ij x_j, A a token x token matrix (W or P, a 16 x
-// 16 tile of it), x_j tokens whose planes have a scale s_j each.
+// Products over tokens: sum_j A_ij x_j, A a token x token matrix (W or P), x_j
+// tokens whose planes have a scale s_j each.
 //
-// The planes of A leave out c_j = 2^Size_j, about |k_j| e^(G_J - G_j) with J the
-// last of j's 16 tokens (in W, where keys of any size multiply one another, the
-// largest that a column without that decay has in the rows' own measure):
-// A_ij = r_i c_j A'_ij, where r_i is a row's scale, and |A'_ij| spans little.  A tile
-// is then multiplied as A'_ij 2^(w_j - w), w_j the exponent of s_j c_j (of s_j
-// r_j, for sums over A's rows), w the largest of those that the row adds up: in the
-// tile on the diagonal only the tokens up to i (from i on), without i itself in W,
-// whose diagonal is zero.  What falls below FP16's range there is below 2^-24 of a
-// term of the largest size.
+// The planes of A leave out what its rows and columns differ by,
+//
+//   A_ij = 2^Row_i A'_ij 2^Column_j:
+//
+// 2^Column_j is about |k_j| e^-G_j (in W, where keys of any size multiply one another,
+// the largest that the column has in its rows' measure, for |k_j|), 2^Row_i what is
+// left, so that a row's largest A' has an FP16 number's size; the decays' exponents,
+// as large as they may be, are integers and only their differences are ever taken.  So
+// |A'_ij| spans little, and a 16 x 16 tile of it is multiplied as A'_ij 2^(w_j - w),
+// w_j the exponent of s_j 2^Column_j (of s_j 2^Row_j, for sums over A's rows), w the
+// largest of those that a row adds up: in the tile on the diagonal only the tokens up
+// to i (from i on), without i itself in W, whose diagonal is zero.  What falls below
+// FP16's range there is below 2^-24 of a term of the largest size.
 // ---------------------------------------------------------------------------
 
 // A lane's factors for an A fragment, {rows 0-7, 8-15} x {k = 0-7, 8-15}, and the
@@ -399,24 +404,35 @@ __device__ __forceinline__ __half2 two_powers(int a, int b) {
   return __floats2half2_rn(x, y);
 }
 
-// w: of tokens 2c, 2c + 1, 2c + 8, 2c + 9, c = lane & 3.
-__device__ __forceinline__ Weights whole_weights(const int (&w)[4]) {
+// What a warp's 16 tokens bring to tiles off the diagonal: factors and the exponent,
+// in shared memory.  own: the exponents of the lane's rows, lane / 4 and lane / 4 + 8.
+__device__ __forceinline__ void put_weights(const int (&own)[2], int quarter, __half* factor, int* top) {
+  const int lane = threadIdx.x & 31, m = __reduce_max_sync(0xffffffffu, max(own[0], own[1]));
+  if ((lane & 3) == 0) {
+    const __half2 f = two_powers(own[0] - m, own[1] - m);
+    factor[quarter * 16 + (lane >> 2)] = __low2half(f);
+    factor[quarter * 16 + (lane >> 2) + 8] = __high2half(f);
+  }
+  if (lane == 0) top[quarter] = m;
+}
+__device__ __forceinline__ Weights get_weights(int kk, const __half* factor, const int* top) {
   Weights r;
-  int top = max(max(w[0], w[1]), max(w[2], w[3]));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const int c = kk * 16 + (threadIdx.x & 3) * 2;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) r.f[0][k] = r.f[1][k] = two_powers(w[2 * k] - top, w[2 * k + 1] - top);
-  r.top[0] = r.top[1] = top;
+  for (int k = 0; k < 2; ++k) r.f[0][k] = r.f[1][k] = *reinterpret_cast<const __half2*>(factor + c + 8 * k);
+  r.top[0] = r.top[1] = top[kk];
   return r;
 }
 
-// own: of the lane's rows, lane / 4 and lane / 4 + 8.  The largest up to a row, or
-// from it on (DOWN), without it (STRICT).
+// For the tile on the diagonal, whose tokens are the warp's own: the largest up to a
+// row, or from it on (DOWN), without it (STRICT).
 template <bool DOWN, bool STRICT>
-__device__ __forceinline__ Weights diagonal_weights(const int (&w)[4], const int (&own)[2]) {
+__device__ __forceinline__ Weights diagonal_weights(const int (&own)[2]) {
   Weights r;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, from = (lane & 3) * 8;
+  // of tokens 2c, 2c + 1, 2c + 8, 2c + 9, c = lane & 3
+  const int w[4] = {__shfl_sync(0xffffffffu, own[0], from), __shfl_sync(0xffffffffu, own[0], from + 4),
+                    __shfl_sync(0xffffffffu, own[1], from), __shfl_sync(0xffffffffu, own[1], from + 4)};
   int a = own[DOWN ? 1 : 0], b = own[DOWN ? 0 : 1];  // the rows that count first, and the others
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) {
@@ -433,7 +449,7 @@ __device__ __forceinline__ Weights diagonal_weights(const int (&w)[4], const int
     const int x = DOWN ? __shfl_down_sync(0xffffffffu, a, 4) : __shfl_up_sync(0xffffffffu, a, 4);
     const int y = DOWN ? __shfl_down_sync(0xffffffffu, b, 4) : __shfl_up_sync(0xffffffffu, b, 4);
     const bool edge = DOWN ? lane >= 28 : lane < 4;
-    a = edge ? -1024 : x;  // nothing there
+    a = edge ? -(1 << 28) : x;  // nothing there
     b = edge ? all : y;
   }
   r.top[0] = DOWN ? b : a;

@@ -43,8 +43,8 @@ constexpr int kLd = 68;  // row length of the FP32 64 x 64 tiles: a multiple of 
 constexpr int kLx = 36;
 
 // The gates that prepare makes, in shared memory: e^G, e^(G_end - G), beta, the
-// exponents of P's columns and of the decays in them, and the logarithms.
-enum Local { kLocalSize = 3, kLocalTail = 4, kLocalLog = 5, kLocal = 7 };
+// exponents (integers) of e^G and of the keys, and the logarithms.
+enum Local { kLocalLevel = 3, kLocalKey = 4, kLocalLog = 5, kLocal = 7 };
 
 template <typename T, int DK>
 struct PrepareSmem {
@@ -53,8 +53,8 @@ struct PrepareSmem {
   static constexpr int tiles = (2 * kC * kLd + kC * kLx) * 4;  // N, W and X, over the planes once those are used up
   static constexpr int main = planes > tiles ? planes : tiles;
   // gates of two value heads, tokens whose key is not finite, the largest
-  // magnitudes of K's and Q's rows (then their scales), W's exponents
-  static constexpr int bytes = main + (2 * kLocal + 5) * kC * 4;
+  // magnitudes of K's and Q's rows (then their scales), P's rows', W's exponents
+  static constexpr int bytes = main + (2 * kLocal + 6) * kC * 4;
 };
 
 // acc += A B of FP32 tiles in shared memory, 16 rows from m0 and 8 columns
@@ -163,14 +163,10 @@ __device__ __forceinline__ void chunk_gates(const Problem& a, int b, int hv, int
     if (lane >= o) s += y;
   }
   const double end = __shfl_sync(0xffffffffu, s, 31);
-  // what the planes of P leave out of a token's column: its key's size, in those
-  // of its 16 tokens, and its decay up to the last of them (within bounds that keep
-  // the quotients finite)
+  // what the planes of P leave out of a token's column: its key's size, in the
+  // largest's, and its decay
   const int ke[2] = {exponent_of(key[2 * lane]), exponent_of(key[2 * lane + 1])};
-  int kmax = max(ke[0], ke[1]);
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) kmax = max(kmax, __shfl_xor_sync(0xffffffffu, kmax, o));
-  const double last = __shfl_sync(0xffffffffu, s, lane | 7);
+  const int kmax = __reduce_max_sync(0xffffffffu, max(ke[0], ke[1]));
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int i = 2 * lane + e;
@@ -181,9 +177,8 @@ __device__ __forceinline__ void chunk_gates(const Problem& a, int b, int hv, int
     const double g2 = gi * 1.4426950408889634;
     gates[kLocalLog * kC + i] = (float)g2;
     gates[(kLocalLog + 1) * kC + i] = (float)(g2 - (double)(float)g2);
-    const int decay = (int)fmin(fmax((last - gi) * 1.4426950408889634, -60.0), 60.0);
-    reinterpret_cast<int*>(gates)[kLocalSize * kC + i] = max(decay + max(ke[e] - kmax, -60), -100);
-    reinterpret_cast<int*>(gates)[kLocalTail * kC + i] = max(decay, -30);
+    reinterpret_cast<int*>(gates)[kLocalLevel * kC + i] = (int)floor(g2);
+    reinterpret_cast<int*>(gates)[kLocalKey * kC + i] = max(ke[e] - kmax, -60);
   }
 }
 
@@ -202,7 +197,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
   int* bad = reinterpret_cast<int*>(gates2 + 2 * kLocal * kC);  // tokens whose key is not finite
   float* ksc = reinterpret_cast<float*>(bad + kC);  // of K's rows and of Q's
   float* qsc = ksc + kC;
-  int* wrow = reinterpret_cast<int*>(qsc + kC);  // exponents of the largest of W's rows, and of its columns
+  float* prow = qsc + kC;                         // the largest of P's rows
+  int* wrow = reinterpret_cast<int*>(prow + kC);  // exponents of the largest of W's rows, and of its columns
   int* wcol = wrow + kC;
 
   let_next_start();
@@ -381,9 +377,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
     const int hv = h * a.rep + r;
     const long nv = ((long)b * a.Hv + hv) * a.nc + chunk;
     const float* gates = gates2 + (r & 1) * kLocal * kC;
-    const int* size = reinterpret_cast<const int*>(gates + kLocalSize * kC);
-    const int* tail = reinterpret_cast<const int*>(gates + kLocalTail * kC);
+    const int* level = reinterpret_cast<const int*>(gates + kLocalLevel * kC);
+    const int* key = reinterpret_cast<const int*>(gates + kLocalKey * kC);
     float* out = a.gates + nv * kGates * kC;
+    if (threadIdx.x < kC) prow[threadIdx.x] = 0.0f;
     __syncthreads();
     float pv[4][4];
 #pragma unroll
@@ -394,34 +391,38 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
         float nn[2];
 #pragma unroll
         for (int l = 0; l < 2; ++l) {
-          const float d = j + l <= i ? decay_between(gates + kLocalLog * kC, i, j + l) : 0.0f;
-          nn[l] = j + l < i ? ak[n][2 * e + l] * d : 0.0f;
-          pv[n][2 * e + l] = j + l <= i ? aq[n][2 * e + l] * (d * a.scale) * power_of(127 - size[j + l]) : 0.0f;
+          // the decay, and what of it P's planes hold
+          const float* log = gates + kLocalLog * kC;
+          const float g = log_between(log, i, j + l), left = g + (float)(level[j + l] - level[i]);
+          nn[l] = j + l < i ? ak[n][2 * e + l] * exp2f(g) : 0.0f;
+          pv[n][2 * e + l] = j + l <= i ? aq[n][2 * e + l] * (exp2f(left) * a.scale) * power_of(127 - key[j + l]) : 0.0f;
         }
         *reinterpret_cast<float2*>(N + i * kLd + j) = make_float2(nn[0], nn[1]);
       }
-    f16* pp = a.pp + nv * 2 * kTile;
-#pragma unroll
-    for (int n = 0; n < 4; n += 2)
+    if (n0 <= m0) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        // a row of a 16 x 16 tile, over four lanes
-        float m = max_finite(max_finite(0.0f, pv[n][2 * e]), pv[n][2 * e + 1]);
-        m = max_finite(max_finite(m, pv[n + 1][2 * e]), pv[n + 1][2 * e + 1]);
+        float m = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) m = max_finite(max_finite(m, pv[n][2 * e]), pv[n][2 * e + 1]);
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const float inv = plane_inv(m);
-        if ((lane & 3) == 0) out[(kScaleP + (n0 + n * 8) / 16) * kC + frag_row(m0, e)] = plane_scale(inv);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t w[2];
-          split2<2>(pv[n + h][2 * e], pv[n + h][2 * e + 1], inv, w);
-          const int at = ((m0 / 8 + e) * (kC / 8) + n0 / 8 + n + h) * 32 + lane;
-          reinterpret_cast<uint32_t*>(pp)[at] = w[0];
-          reinterpret_cast<uint32_t*>(pp + kTile)[at] = w[1];
-        }
+        if ((lane & 3) == 0) atomicMax(reinterpret_cast<int*>(prow + frag_row(m0, e)), __float_as_int(m));
       }
+    }
     __syncthreads();
+    f16* pp = a.pp + nv * 2 * kTile;
+    const float ip[2] = {plane_inv(prow[frag_row(m0, 0)]), plane_inv(prow[frag_row(m0, 1)])};
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        uint32_t w[2];
+        split2<2>(pv[n][2 * e], pv[n][2 * e + 1], ip[e], w);
+        const int at = ((m0 / 8 + e) * (kC / 8) + n0 / 8 + n) * 32 + lane;
+        reinterpret_cast<uint32_t*>(pp)[at] = w[0];
+        reinterpret_cast<uint32_t*>(pp + kTile)[at] = w[1];
+      }
     // W's 16 x 16 diagonal blocks, a thread per column: W_ic = N_ic - sum_j
     // N_ij beta_j W_jc, every row's term taken off as soon as it is known
     if (threadIdx.x < kC) {
@@ -458,50 +459,51 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
     // The exponents that W's columns leave out: the decays, and the largest of a
     // column in its rows' measure.  With keys of norm one that is about the key's
     // part; a larger key multiplies what later rows hold of earlier columns.
+    constexpr int kNone = -(1 << 28);
     {
       const int row = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
-      int m = -1024;
+      int m = kNone;
 #pragma unroll
       for (int y = 0; y < 16; y += 4) {
         const float4 f = *reinterpret_cast<const float4*>(W + row * kLd + c + y);
-        m = max(m, max(exponent_of(f.x) - tail[c + y], exponent_of(f.y) - tail[c + y + 1]));
-        m = max(m, max(exponent_of(f.z) - tail[c + y + 2], exponent_of(f.w) - tail[c + y + 3]));
+        const float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+          if (v[z] != 0.0f) m = max(m, exponent_of(v[z]) + level[c + y + z]);
       }
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      if ((threadIdx.x & 3) == 0) wrow[row] = m;
-      if (threadIdx.x < kC) wcol[threadIdx.x] = -1024;
+      if ((threadIdx.x & 3) == 0) wrow[row] = m == kNone ? 0 : m - level[row];
+      if (threadIdx.x < kC) wcol[threadIdx.x] = kNone;
     }
     __syncthreads();
     {
       const int c = threadIdx.x & (kC - 1), r1 = threadIdx.x / kC * 16;
-      int m = -1024;
+      int m = kNone;
 #pragma unroll
       for (int y = 0; y < 16; ++y) {
         const float f = W[(r1 + y) * kLd + c];
-        if (f != 0.0f) m = max(m, exponent_of(f) - wrow[r1 + y]);
+        if (f != 0.0f) m = max(m, exponent_of(f) - level[r1 + y] - wrow[r1 + y]);
       }
-      if (m > -1024) atomicMax(wcol + c, m);
+      if (m != kNone) atomicMax(wcol + c, m + level[c]);
     }
     __syncthreads();
-    // (W over it is no larger than its rows' largest over the decays)
-    auto size_w = [&](int c) { return min(max(wcol[c], -100), 60); };
-    // W's planes: a thread takes two rows of eight elements of the tile's blocks;
-    // the next block's same row, of the same scale, is another lane's
+    auto size_w = [&](int c) { return max(wcol[c], -100); };  // none is above zero
+    // W's planes: a thread takes two rows of eight elements of the tile's blocks.  A
+    // row's largest quotient has the exponent of wrow: the column that gave it is none
+    // larger in any row.
     f16* wp = a.wp + nv * 2 * kTile;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const int j = threadIdx.x + x * kThreads, blk = j >> 3, row = (blk / 8) * 8 + (j & 7), c8 = blk % 8;
       const float* f = W + row * kLd + c8 * 8;
-      float v[8], m = 0.0f;
+      const float inv = power_of(268 - max(wrow[row], 27));
+      float v[8];
 #pragma unroll
       for (int y = 0; y < 8; ++y) {
-        v[y] = f[y] * power_of(127 - size_w(c8 * 8 + y));
-        m = max_finite(m, v[y]);
+        const int c = c8 * 8 + y;
+        v[y] = f[y] * power_of(127 + level[c] - level[row] - size_w(c));
       }
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-      const float inv = plane_inv(m);
-      if (!(c8 & 1)) out[(kScaleW + c8 / 2) * kC + row] = plane_scale(inv);
       uint32_t w[4][2];
 #pragma unroll
       for (int y = 0; y < 4; ++y) split2<2>(v[2 * y], v[2 * y + 1], inv, w[y]);
@@ -515,9 +517,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
       out[kRest * kC + i] = gates[kC + i];
       out[kBeta * kC + i] = gates[2 * kC + i];
       out[kScaleK * kC + i] = ksc[i];
-      reinterpret_cast<int*>(out)[kSizeW * kC + i] = size_w(i);
+      int* whole = reinterpret_cast<int*>(out);
+      whole[kColumnW * kC + i] = size_w(i) - level[i];
+      whole[kRowW * kC + i] = max(wrow[i], 27) - 14 - 127 + level[i];
+      whole[kColumnP * kC + i] = key[i] - level[i];
+      whole[kRowP * kC + i] = exponent_of(plane_scale(plane_inv(prow[i]))) - 127 + level[i];
       out[kScaleQ * kC + i] = qsc[i];
-      reinterpret_cast<int*>(out)[kSizeP * kC + i] = size[i];
       out[kLog * kC + i] = gates[kLocalLog * kC + i];
       out[(kLog + 1) * kC + i] = gates[(kLocalLog + 1) * kC + i];
     }
@@ -549,8 +554,8 @@ struct ScanSmem {
   static constexpr int k = NP * kC * DK, w = 2 * kTile;  // elements
   static constexpr int stage = (k + w) * 2 + kForward * kC * 4;
   static constexpr int s = 4 * kGroup * DK, x = 4 * kGroup * kC;  // two planes of two groups
-  // scales of S and of U, exponents of B R's tokens, a token for each column
-  static constexpr int bytes = 2 * stage + (s + 2 * x) * 2 + 2 * 8 * 4 + 2 * kC * 4 + kSlice * 4;
+  // scales of S and of U, weights of B R's tokens, a token for each column
+  static constexpr int bytes = 2 * stage + (s + 2 * x) * 2 + 2 * 8 * 4 + 2 * (kC * 2 + 4 * 4) + kSlice * 4;
 };
 
 template <int NP, int DK>
@@ -580,8 +585,9 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
   float* scales = reinterpret_cast<float*>(base + L::s + 2 * L::x);
   float* ssc = scales + pair * 4;
   float* ysc = scales + 8 + pair * 4;
-  int* xex = reinterpret_cast<int*>(scales + 16) + pair * kC;
-  int* first = reinterpret_cast<int*>(scales + 16) + 2 * kC;  // of each column, the first token that is not finite
+  int* top = reinterpret_cast<int*>(scales + 16) + pair * 4;
+  __half* factor = reinterpret_cast<__half*>(scales + 24) + pair * kC;
+  int* first = reinterpret_cast<int*>(scales + 24 + kC);  // of each column, the first token that is not finite
 
   float s[MT][2][4];
   // a later range goes on from what the one before it left
@@ -626,6 +632,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
     const int row[2] = {frag_row(quarter * 16, 0), frag_row(quarter * 16, 1)};  // this lane's tokens
     const float sk[2] = {gate[kScaleK * kC + row[0]], gate[kScaleK * kC + row[1]]};
 
+    const int* whole = reinterpret_cast<const int*>(gate);
+    Weights diagonal;
     float x[2][4];
     times_state<NP, DK>(x, kp, quarter * 2, sp, ssc);
     // R, and the planes of B R
@@ -658,8 +666,12 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
 #pragma unroll
           for (int e = 0; e < 4; ++e) y[n][e] = finite(y[n][e]) && finite(x[n][e]) ? y[n][e] : 0.0f;
       }
-      bool all_finite;
-      put_tokens<2>(y, quarter, xp, xex, nullptr, nullptr, all_finite);
+      int w[2];
+      put_tokens<2>(y, quarter, xp, w, nullptr, nullptr);
+      w[0] += whole[kColumnW * kC + row[0]];
+      w[1] += whole[kColumnW * kC + row[1]];
+      put_weights(w, quarter, factor, top);
+      diagonal = diagonal_weights<false, true>(w);
     }
     off = group_sync_or(pair, off);
     if (off) {  // rare, and the same for the whole group
@@ -671,7 +683,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
       group_sync(pair);
     }
     // E
-    times_tokens<2, false, true>(x, wp, gate + kScaleW * kC, reinterpret_cast<const int*>(gate) + kSizeW * kC, quarter, xp, xex, -1.0f);
+    const int rw[2] = {whole[kRowW * kC + row[0]], whole[kRowW * kC + row[1]]};
+    times_tokens<2, false>(x, wp, rw, quarter, xp, diagonal, factor, top, -1.0f);
     if (off) {
       // a later token's error holds every earlier one's
 #pragma unroll
@@ -681,9 +694,9 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
           if (row[e >> 1] > first[pair * kGroup + frag_col(n * 8) + (e & 1)]) x[n][e] = __uint_as_float(0x7fffffffu);
     }
     {
-      bool all_finite;
-      put_tokens<2>(x, quarter, yp, nullptr, a.e + (nv * groups + group) * 2 * kGroup * kC,
-                    a.escale + (nv * groups + group) * kC, all_finite);  // yp: on the way only
+      int w[2];
+      put_tokens<2>(x, quarter, yp, w, a.e + (nv * groups + group) * 2 * kGroup * kC,
+                    a.escale + (nv * groups + group) * kC);  // yp: on the way only
     }
     // S <- e^G S + K^T (e^(G_end - G) U)
     {
@@ -733,7 +746,8 @@ struct OutputSmem {
   static constexpr int s = 2 * cols * DK, e = 2 * cols * kC;
   static constexpr int slice = s + e + 2 * (16 + 4 * kC);  // and the scales of S (four groups and quarters) and of E
   static constexpr int buffers = (q + p + 2 * slice) * 2 > 96 * 1024 ? 1 : 2;
-  static constexpr int bytes = (q + p + buffers * slice) * 2 + (kBackward + 1) * kC * 4;
+  // P's exponents, and of four groups' tokens the weights' exponents, factors and tops
+  static constexpr int bytes = (q + p + buffers * slice) * 2 + (kBackward + 1) * kC * 4 + 4 * (kC * 4 + kC * 2 + 4 * 4);
 };
 
 template <typename T, int DK>
@@ -756,7 +770,7 @@ __device__ __forceinline__ void output_load(f16* dst, const Problem& a, long nv,
 
 // An element of P U, for a chunk with an error that is not finite: the zeros of P
 // above its diagonal would spread it to earlier tokens.
-__device__ __noinline__ float output_element(const f16* pp, const float* rows, const int* size, const f16* ep, int plane,
+__device__ __noinline__ float output_element(const f16* pp, int row, const int* column, const f16* ep, int plane,
                                              const float* scale, int i, int c) {
   float sum = 0.0f;
   for (int j = 0; j <= i; ++j) {
@@ -767,7 +781,7 @@ __device__ __noinline__ float output_element(const f16* pp, const float* rows, c
       u += __half2float(pp[p * kTile + ip]);
       w += __half2float(ep[p * plane + ie]);
     }
-    sum += (rows[(j >> 4) * kC + i] * power_of(size[j] + 127)) * (fabsf(scale[j]) * (u * w));
+    sum += power_of(row + column[j] + 127) * (fabsf(scale[j]) * (u * w));
   }
   return sum;
 }
@@ -789,7 +803,11 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
   copy_async<L::q * 2, kThreads>(qp, a.qp + nk * L::q);
   copy_async<L::p * 2, kThreads>(pp, a.pp + nv * L::p);
   copy_async<kBackward * kC * 4, kThreads>(gate, a.gates + nv * kGates * kC);
-  int* size = reinterpret_cast<int*>(gate + kBackward * kC);  // P's, with the exponents of beta
+  const int* gates = reinterpret_cast<const int*>(gate);
+  int* column = reinterpret_cast<int*>(gate + kBackward * kC);  // P's, with the exponents of beta
+  int* weight = column + kC;
+  int* top = weight + 4 * kC;
+  __half* factor = reinterpret_cast<__half*>(top + 4 * 4);
   output_load<T, DK>(slices, a, nv, 0);
   const int warp = threadIdx.x >> 5;
   // rows of 1 and 4 steps of P to two of the SM's quarters, of 2 and 3 to the others
@@ -807,7 +825,7 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
       if (threadIdx.x < kC) {
         float& be = gate[kBeta * kC + threadIdx.x];
         const int up = exponent_of(be) + 1;  // of the least power above it, biased
-        size[threadIdx.x] = reinterpret_cast<const int*>(gate)[kSizeP * kC + threadIdx.x] + up - 127;
+        column[threadIdx.x] = gates[kColumnP * kC + threadIdx.x] + up - 127;
         be *= power_of(254 - up);
       }
       __syncthreads();
@@ -832,10 +850,21 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
         for (int p = 0; p < 2; ++p)
           reinterpret_cast<uint4*>(pp + p * kTile)[row] = make_uint4(r[p][0], r[p][1], r[p][2], r[p][3]);
       }
-      __syncthreads();
     }
     const f16* sp = slices + buf * L::slice;
     const f16* ep = sp + L::s;
+    {
+      // the weights of this slice's tokens: a thread has a group's token, half a warp
+      // its 16 tokens
+      const int w = exponent_of(reinterpret_cast<const float*>(ep + L::e)[16 + threadIdx.x]) + column[threadIdx.x & (kC - 1)];
+      int m = w;
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      weight[threadIdx.x] = w;
+      factor[threadIdx.x] = __low2half(two_powers(w - m, 0));
+      if ((threadIdx.x & 15) == 0) top[threadIdx.x >> 4] = m;
+    }
+    __syncthreads();
     if (L::buffers == 2 && c0 + L::cols < a.dvp) {
       buf ^= 1;
       output_load<T, DK>(slices + buf * L::slice, a, nv, c0 + L::cols);
@@ -869,14 +898,15 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
       bool lost = false;
 #pragma unroll
       for (int i = 0; i < 8; ++i) lost |= fe[i * 16] < 0.0f;
-      const float* rows_p = gate + kScaleP * kC;
+      const int row[2] = {frag_row(m0, 0), frag_row(m0, 1)};
+      const int row_p[2] = {gates[kRowP * kC + row[0]], gates[kRowP * kC + row[1]]};
       if (lost) {
 #pragma unroll
         for (int n = 0; n < 4; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            y[n][e] = output_element(pp, rows_p, size, eg + (n >> 1) * 2 * kGroup * kC, kGroup * kC, fe + (n >> 1) * kC,
-                                     frag_row(m0, e >> 1), frag_col((n & 1) * 8) + (e & 1));
+            y[n][e] = output_element(pp, row_p[e >> 1], column, eg + (n >> 1) * 2 * kGroup * kC, kGroup * kC,
+                                     fe + (n >> 1) * kC, row[e >> 1], frag_col((n & 1) * 8) + (e & 1));
       } else {
         const uint32_t pa = addr_a<kC, false>(pp, m0 / 8, 0), pb = addr_b<kGroup, true>(eg, 0, 0);
 #pragma unroll
@@ -888,16 +918,13 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
           load_b<2, 4, true>(fb, pb + kk * 512, 2 * kGroup * kC * 2, kGroup * kC * 2);
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
-            const float* se = fe + g * kC;
-            auto weight = [&](int j) { return exponent_of(se[j]) + size[j]; };
-            const int c = kk * 16 + (threadIdx.x & 3) * 2;
-            const int w[4] = {weight(c), weight(c + 1), weight(c + 8), weight(c + 9)};
+            const int group = half * 2 + g, *wg = weight + group * kC;
             Weights f;
             if (kk == m0 / 16) {
-              const int own[2] = {weight(frag_row(m0, 0)), weight(frag_row(m0, 1))};
-              f = diagonal_weights<false, false>(w, own);
+              const int own[2] = {wg[row[0]], wg[row[1]]};
+              f = diagonal_weights<false, false>(own);
             } else {
-              f = whole_weights(w);
+              f = get_weights(kk, factor + group * kC, top + group * 4);
             }
             uint32_t fa[2][4], fg[2][2][2];
 #pragma unroll
@@ -910,7 +937,7 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
             mma_terms<2, 2, 2>(t, fa, fg);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float r = rows_p[kk * kC + frag_row(m0, e)] * power_of(f.top[e]);
+              const float r = power_of(f.top[e] + row_p[e]);
 #pragma unroll
               for (int n = 0; n < 2; ++n) {
                 y[2 * g + n][2 * e] += r * t[n][2 * e];
@@ -922,13 +949,12 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = frag_row(m0, e);
-        const float f = gate[row] * gate[kScaleQ * kC + row] * a.scale;
+        const float f = gate[row[e]] * gate[kScaleQ * kC + row[e]] * a.scale;
         float2 z[4];
 #pragma unroll
         for (int n = 0; n < 4; ++n)
           z[n] = make_float2(f * x[n][2 * e] + y[n][2 * e], f * x[n][2 * e + 1] + y[n][2 * e + 1]);
-        set_row<T>(o + (long)row * a.Hv * a.dv + cw, a.dv - cw, vec, whole, row < rows, z);
+        set_row<T>(o + (long)row[e] * a.Hv * a.dv + cw, a.dv - cw, vec, whole, row[e] < rows, z);
       }
     }
     if (L::buffers == 1 && c0 + L::cols < a.dvp) {

@@ -59,29 +59,17 @@ __device__ __forceinline__ void times_state(float (&x)[2][4], const f16* kp, int
 }
 
 // x += sign A B (UP: A^T B) for the 16 tokens of `quarter`, over the tokens up to
-// (from) them: A a lower 64 x 64 tile as planes, with the scales of its rows and
-// the sizes that its columns leave out; B 64 tokens x 16 columns as NB planes with
-// the exponents of its tokens' scales.  STRICT: A's diagonal is zero.
-template <int NB, bool UP, bool STRICT>
-__device__ __forceinline__ void times_tokens(float (&x)[2][4], const f16* A, const float* scale, const int* size, int quarter,
-                                             const f16* B, const int* exponent, float sign) {
+// (from) them: A a lower 64 x 64 tile as planes; B 64 tokens x 16 columns as NB
+// planes, with the tokens' weights.  `own`: exponents of the lane's rows, A's Row (UP:
+// Column).
+template <int NB, bool UP>
+__device__ __forceinline__ void times_tokens(float (&x)[2][4], const f16* A, const int (&own)[2], int quarter, const f16* B,
+                                             const Weights& diagonal, const __half* factor, const int* top, float sign) {
   constexpr int plane = 2 * kGroup * kC * 2;
-  const int lane = threadIdx.x & 31, c = (lane & 3) * 2, r = quarter * 16 + (lane >> 2);
-  // the exponents that a token of the sum brings
-  auto weight = [&](int t) {
-    return exponent[t] + (UP ? exponent_of(scale[quarter * kC + t]) - 127 : size[t]);
-  };
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) {
     if (UP ? kk < quarter : kk > quarter) continue;
-    const int w[4] = {weight(kk * 16 + c), weight(kk * 16 + c + 1), weight(kk * 16 + c + 8), weight(kk * 16 + c + 9)};
-    Weights f;
-    if (kk == quarter) {
-      const int own[2] = {weight(r), weight(r + 8)};
-      f = diagonal_weights<UP, STRICT>(w, own);
-    } else {
-      f = whole_weights(w);
-    }
+    const Weights f = kk == quarter ? diagonal : get_weights(kk, factor, top);
     uint32_t fa[2][4], fb[NB][2][2];
     const uint32_t pa = addr_a<kC, UP>(A, quarter * 2, 2 * kk);
 #pragma unroll
@@ -94,7 +82,7 @@ __device__ __forceinline__ void times_tokens(float (&x)[2][4], const f16* A, con
     mma_terms<2, NB, 2>(t, fa, fb);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float g = sign * power_of(f.top[e]) * (UP ? power_of(size[r + 8 * e] + 127) : scale[kk * kC + r + 8 * e]);
+      const float g = sign * power_of(f.top[e] + own[e]);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         x[n][2 * e] += g * t[n][2 * e];
@@ -104,23 +92,22 @@ __device__ __forceinline__ void times_tokens(float (&x)[2][4], const f16* A, con
   }
 }
 
-// A warp's 16 tokens x 16 columns as NP planes with a scale for each token: planes
-// and exponents in shared memory and, if given, planes and scales in `out`.
+// A warp's 16 tokens x 16 columns as NP planes with a scale for each token, in shared
+// memory and, if given, in `out`; the exponents of the lane's scales.
 template <int NP>
-__device__ __forceinline__ void put_tokens(const float (&x)[2][4], int quarter, f16* tile, int* exponent, f16* out,
-                                           float* out_scale, bool& all_finite) {
+__device__ __forceinline__ void put_tokens(const float (&x)[2][4], int quarter, f16* tile, int (&exponent)[2], f16* out,
+                                           float* out_scale) {
   float m[2];
+  bool all_finite;
   row_max(x, m, all_finite);
   const float inv[2] = {plane_inv(m[0]), plane_inv(m[1])};
-  const int lane = threadIdx.x & 31, r = quarter * 16 + (lane >> 2);
-  if ((lane & 3) == 0) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float s = plane_scale(inv[e]);
-      if (exponent) exponent[r + 8 * e] = exponent_of(s);
-      // below zero: the 16 tokens hold something that is not finite
-      if (out_scale) out_scale[r + 8 * e] = all_finite ? s : -s;
-    }
+  for (int e = 0; e < 2; ++e) {
+    const float s = plane_scale(inv[e]);
+    exponent[e] = exponent_of(s);
+    // below zero: the 16 tokens hold something that is not finite
+    if (out_scale && (lane & 3) == 0) out_scale[quarter * 16 + (lane >> 2) + 8 * e] = all_finite ? s : -s;
   }
   store_rows<NP>(tile, 2 * kGroup * kC, quarter * 2, x, inv, out, kGroup * kC);
 }
