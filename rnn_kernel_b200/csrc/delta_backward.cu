@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
   const int row[2] = {frag_row(quarter * 16, 0), frag_row(quarter * 16, 1)};  // this lane's tokens
   int ow[2];    // exponents of their dO's scales and of P's rows
   int next[2];  // those, of the chunk whose dO is loaded
+  bool onarrow;
 
   float d[MT][2][4];  // the gradient of the state after the chunk
   const float* ds = a.ds_out ? a.ds_out + (long)bh * a.dk * a.dv : nullptr;
@@ -128,7 +129,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
                    a.doscale + (nv * groups + group) * kC);
 #pragma unroll
     for (int e = 0; e < 2; ++e) ow[e] += next[e];
-    put_weights(ow, quarter, ofactor, otop);
+    onarrow = put_weights(ow, quarter, ofactor, otop);
   };
   auto state_out = [&](int chunk) {
     const long nv = nv0 + chunk;
@@ -156,7 +157,6 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
     const int* whole = reinterpret_cast<const int*>(gate);
     const float sk[2] = {gate[kScaleK * kC + row[0]], gate[kScaleK * kC + row[1]]};
     float x[2][4], y[2][4];
-    Weights diagonal = diagonal_weights<true, false>(ow);
     // scale e^G dO, for Q^T
     dout_tile(x);
     if (chunk > 0) load_dout(chunk - 1);
@@ -173,26 +173,25 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
       for (int e = 0; e < 4; ++e) x[n][e] *= sk[e >> 1] * gate[kRest * kC + row[e >> 1]];
     {
       const int left[2] = {whole[kColumnP * kC + row[0]], whole[kColumnP * kC + row[1]]};
-      times_tokens<NP, true>(x, pp, left, quarter, op, diagonal, ofactor, otop, 1.0f);
+      times_tokens<NP, true, false>(x, pp, left, quarter, op, ow, onarrow, ofactor, otop, 1.0f);
     }
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[n][e] = x[n][e] * gate[kBeta * kC + row[e >> 1]];
+    int w[2];
+    bool narrow;
     {
-      int w[2];
       put_tokens<2>(y, quarter, up, w, nullptr, nullptr);
 #pragma unroll
       for (int e = 0; e < 2; ++e) w[e] += whole[kRowW * kC + row[e]];
-      put_weights(w, quarter, ufactor, utop);
-      diagonal = diagonal_weights<true, true>(w);
+      narrow = put_weights(w, quarter, ufactor, utop);
     }
     group_sync(pair);
     // Z and dV
     {
       const int left[2] = {whole[kColumnW * kC + row[0]], whole[kColumnW * kC + row[1]]};
-      times_tokens<2, true>(x, wp, left, quarter, up, diagonal, ufactor, utop, -1.0f);
-      int w[2];
+      times_tokens<2, true, true>(x, wp, left, quarter, up, w, narrow, ufactor, utop, -1.0f);
       put_tokens<2>(x, quarter, zp, w, a.z + (nv * groups + group) * 2 * kGroup * kC,
                     a.zscale + (nv * groups + group) * kC);  // zp: on the way only
     }

@@ -404,16 +404,23 @@ __device__ __forceinline__ __half2 two_powers(int a, int b) {
   return __floats2half2_rn(x, y);
 }
 
-// What a warp's 16 tokens bring to tiles off the diagonal: factors and the exponent,
-// in shared memory.  own: the exponents of the lane's rows, lane / 4 and lane / 4 + 8.
-__device__ __forceinline__ void put_weights(const int (&own)[2], int quarter, __half* factor, int* top) {
+// 16 tokens whose exponents are this close serve the tile on the diagonal as they
+// serve the others: A' in both planes times 2^-16 is still exact in FP16.
+constexpr int kNarrow = 16;
+
+// What a warp's 16 tokens bring to the tiles: factors and the exponent, in shared
+// memory; whether they are narrow.  own: the exponents of the lane's rows, lane / 4 and
+// lane / 4 + 8.
+__device__ __forceinline__ bool put_weights(const int (&own)[2], int quarter, __half* factor, int* top) {
   const int lane = threadIdx.x & 31, m = __reduce_max_sync(0xffffffffu, max(own[0], own[1]));
+  const int least = __reduce_min_sync(0xffffffffu, min(own[0], own[1]));
   if ((lane & 3) == 0) {
     const __half2 f = two_powers(own[0] - m, own[1] - m);
     factor[quarter * 16 + (lane >> 2)] = __low2half(f);
     factor[quarter * 16 + (lane >> 2) + 8] = __high2half(f);
   }
   if (lane == 0) top[quarter] = m;
+  return m - least <= kNarrow;
 }
 __device__ __forceinline__ Weights get_weights(int kk, const __half* factor, const int* top) {
   Weights r;
@@ -424,8 +431,8 @@ __device__ __forceinline__ Weights get_weights(int kk, const __half* factor, con
   return r;
 }
 
-// For the tile on the diagonal, whose tokens are the warp's own: the largest up to a
-// row, or from it on (DOWN), without it (STRICT).
+// For the tile on the diagonal, whose tokens are the warp's own, where they are not
+// narrow: the largest up to a row, or from it on (DOWN), without it (STRICT).
 template <bool DOWN, bool STRICT>
 __device__ __forceinline__ Weights diagonal_weights(const int (&own)[2]) {
   Weights r;

@@ -633,7 +633,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
     const float sk[2] = {gate[kScaleK * kC + row[0]], gate[kScaleK * kC + row[1]]};
 
     const int* whole = reinterpret_cast<const int*>(gate);
-    Weights diagonal;
+    int w[2];
+    bool narrow;
     float x[2][4];
     times_state<NP, DK>(x, kp, quarter * 2, sp, ssc);
     // R, and the planes of B R
@@ -666,12 +667,10 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
 #pragma unroll
           for (int e = 0; e < 4; ++e) y[n][e] = finite(y[n][e]) && finite(x[n][e]) ? y[n][e] : 0.0f;
       }
-      int w[2];
       put_tokens<2>(y, quarter, xp, w, nullptr, nullptr);
       w[0] += whole[kColumnW * kC + row[0]];
       w[1] += whole[kColumnW * kC + row[1]];
-      put_weights(w, quarter, factor, top);
-      diagonal = diagonal_weights<false, true>(w);
+      narrow = put_weights(w, quarter, factor, top);
     }
     off = group_sync_or(pair, off);
     if (off) {  // rare, and the same for the whole group
@@ -684,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
     }
     // E
     const int rw[2] = {whole[kRowW * kC + row[0]], whole[kRowW * kC + row[1]]};
-    times_tokens<2, false>(x, wp, rw, quarter, xp, diagonal, factor, top, -1.0f);
+    times_tokens<2, false, true>(x, wp, rw, quarter, xp, w, narrow, factor, top, -1.0f);
     if (off) {
       // a later token's error holds every earlier one's
 #pragma unroll
@@ -694,7 +693,6 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
           if (row[e >> 1] > first[pair * kGroup + frag_col(n * 8) + (e & 1)]) x[n][e] = __uint_as_float(0x7fffffffu);
     }
     {
-      int w[2];
       put_tokens<2>(x, quarter, yp, w, a.e + (nv * groups + group) * 2 * kGroup * kC,
                     a.escale + (nv * groups + group) * kC);  // yp: on the way only
     }
@@ -747,7 +745,7 @@ struct OutputSmem {
   static constexpr int slice = s + e + 2 * (16 + 4 * kC);  // and the scales of S (four groups and quarters) and of E
   static constexpr int buffers = (q + p + 2 * slice) * 2 > 96 * 1024 ? 1 : 2;
   // P's exponents, and of four groups' tokens the weights' exponents, factors and tops
-  static constexpr int bytes = (q + p + buffers * slice) * 2 + (kBackward + 1) * kC * 4 + 4 * (kC * 4 + kC * 2 + 4 * 4);
+  static constexpr int bytes = (q + p + buffers * slice) * 2 + (kBackward + 1) * kC * 4 + 4 * (kC * 4 + kC * 2 + 2 * 4 * 4);
 };
 
 template <typename T, int DK>
@@ -807,7 +805,8 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
   int* column = reinterpret_cast<int*>(gate + kBackward * kC);  // P's, with the exponents of beta
   int* weight = column + kC;
   int* top = weight + 4 * kC;
-  __half* factor = reinterpret_cast<__half*>(top + 4 * 4);
+  int* narrow = top + 4 * 4;
+  __half* factor = reinterpret_cast<__half*>(narrow + 4 * 4);
   output_load<T, DK>(slices, a, nv, 0);
   const int warp = threadIdx.x >> 5;
   // rows of 1 and 4 steps of P to two of the SM's quarters, of 2 and 3 to the others
@@ -857,12 +856,18 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
       // the weights of this slice's tokens: a thread has a group's token, half a warp
       // its 16 tokens
       const int w = exponent_of(reinterpret_cast<const float*>(ep + L::e)[16 + threadIdx.x]) + column[threadIdx.x & (kC - 1)];
-      int m = w;
+      int m = w, least = w;
 #pragma unroll
-      for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      for (int o = 1; o < 16; o <<= 1) {
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+      }
       weight[threadIdx.x] = w;
       factor[threadIdx.x] = __low2half(two_powers(w - m, 0));
-      if ((threadIdx.x & 15) == 0) top[threadIdx.x >> 4] = m;
+      if ((threadIdx.x & 15) == 0) {
+        top[threadIdx.x >> 4] = m;
+        narrow[threadIdx.x >> 4] = m - least <= kNarrow;
+      }
     }
     __syncthreads();
     if (L::buffers == 2 && c0 + L::cols < a.dvp) {
@@ -881,14 +886,23 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
       {
         const uint32_t pa = addr_a<DK, false>(qp, m0 / 8, 0), pb = addr_b<kGroup, true>(sg, 0, 0);
         constexpr int per = DK / 64;  // steps to a scale
+        float t[4][4];
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
           uint32_t fa[NP][4], fb[2][4][2];
 #pragma unroll
           for (int p = 0; p < NP; ++p) ldm4<false>(fa[p], pa + kk * 256 + p * kC * DK * 2);
           load_b<2, 4, true>(fb, pb + kk * 512, 2 * kGroup * DK * 2, kGroup * DK * 2);
-          float t[4][4];
-          mma_terms<NP, 2, 4>(t, fa, fb);
+          // a bf16 output adds the steps of one scale up on the tensor core
+          if (NP == 1 && kk % per != 0) {
+#pragma unroll
+            for (int p = 1; p >= 0; --p)
+#pragma unroll
+              for (int n = 0; n < 4; ++n) mma(t[n], fa[0], fb[p][n][0], fb[p][n][1]);
+          } else {
+            mma_terms<NP, 2, 4>(t, fa, fb);
+          }
+          if (NP == 1 && kk % per != per - 1) continue;
 #pragma unroll
           for (int n = 0; n < 4; ++n)
 #pragma unroll
@@ -920,7 +934,7 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
           for (int g = 0; g < 2; ++g) {
             const int group = half * 2 + g, *wg = weight + group * kC;
             Weights f;
-            if (kk == m0 / 16) {
+            if (kk == m0 / 16 && !narrow[group * 4 + kk]) {
               const int own[2] = {wg[row[0]], wg[row[1]]};
               f = diagonal_weights<false, false>(own);
             } else {

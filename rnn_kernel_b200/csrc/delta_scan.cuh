@@ -61,15 +61,16 @@ __device__ __forceinline__ void times_state(float (&x)[2][4], const f16* kp, int
 // x += sign A B (UP: A^T B) for the 16 tokens of `quarter`, over the tokens up to
 // (from) them: A a lower 64 x 64 tile as planes; B 64 tokens x 16 columns as NB
 // planes, with the tokens' weights.  `own`: exponents of the lane's rows, A's Row (UP:
-// Column).
-template <int NB, bool UP>
+// Column); w: of its rows as tokens of B, if they are not `narrow`.  STRICT: A's
+// diagonal is zero.
+template <int NB, bool UP, bool STRICT>
 __device__ __forceinline__ void times_tokens(float (&x)[2][4], const f16* A, const int (&own)[2], int quarter, const f16* B,
-                                             const Weights& diagonal, const __half* factor, const int* top, float sign) {
+                                             const int (&w)[2], bool narrow, const __half* factor, const int* top, float sign) {
   constexpr int plane = 2 * kGroup * kC * 2;
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) {
     if (UP ? kk < quarter : kk > quarter) continue;
-    const Weights f = kk == quarter ? diagonal : get_weights(kk, factor, top);
+    const Weights f = kk == quarter && !narrow ? diagonal_weights<UP, STRICT>(w) : get_weights(kk, factor, top);
     uint32_t fa[2][4], fb[NB][2][2];
     const uint32_t pa = addr_a<kC, UP>(A, quarter * 2, 2 * kk);
 #pragma unroll
