@@ -259,9 +259,10 @@ __device__ __forceinline__ float plane_inv(float m) {
 }
 __device__ __forceinline__ float plane_scale(float inv) { return __uint_as_float((254u << 23) - __float_as_uint(inv)); }
 
-// A power of two's exponent, biased, and back, to the nearest that there is.
+// A power of two's exponent, biased, and back: zero below FP32's normal numbers (a
+// decay of that size forgets), the largest above.
 __device__ __forceinline__ int exponent_of(float x) { return (int)((__float_as_uint(x) >> 23) & 0xffu); }
-__device__ __forceinline__ float power_of(int biased) { return __uint_as_float((unsigned)min(max(biased, 1), 254) << 23); }
+__device__ __forceinline__ float power_of(int biased) { return __uint_as_float((unsigned)min(max(biased, 0), 254) << 23); }
 
 // Two values (times inv) as planes, packed {low half: a, high half: b}.
 template <int NP>

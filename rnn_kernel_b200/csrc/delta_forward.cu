@@ -825,7 +825,7 @@ __global__ void __launch_bounds__(kThreads) delta_output_kernel(const Problem a,
         float& be = gate[kBeta * kC + threadIdx.x];
         const int up = exponent_of(be) + 1;  // of the least power above it, biased
         column[threadIdx.x] = gates[kColumnP * kC + threadIdx.x] + up - 127;
-        be *= power_of(254 - up);
+        be *= power_of(max(254 - up, 1));
       }
       __syncthreads();
 #pragma unroll

@@ -89,3 +89,30 @@ def test_a_large_token_leaves_the_others_their_digits(what, power, dtype, dk):
             rough_rel = float((rerr / size).square().mean().sqrt())
             worst = float((err / size).max())
             assert worst <= allowed + 16 * rough_rel, (name, part, worst, rough_rel)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("strength", [float("-inf"), -400.0])
+@pytest.mark.parametrize("t", [75, 80, 96])
+def test_nothing_comes_through_a_reset(t, dtype, strength):
+    """Tokens after a decay of zero (or one far below FP32) get the same bits whatever was before it, and however small
+    their own values are."""
+    T = 150
+    q, k, v, g, beta, s = R.inputs(1, T, 1, 2, 64, 48, dtype=dtype, seed=3)
+    g[:, t] = strength
+    v[:, t:] *= 2.0 ** -80
+    do, ds = torch.randn_like(v), torch.randn_like(s)
+    runs = []  # with other values before it, and other gradients from it on
+    for factor in (1.0, 2.0 ** 40):
+        w = v.clone()
+        w[:, :t] = torch.randn_like(w[:, :t]) * factor
+        d = do.clone()
+        d[:, :t] *= 2.0 ** -80
+        d[:, t:] = torch.randn_like(d[:, t:]) * factor  # which the gradients of earlier tokens must not see
+        w0, d1 = torch.randn_like(s) * factor, torch.randn_like(ds) * factor
+        x = [y.clone().requires_grad_(True) for y in (q, k, w, g, beta, w0)]
+        out, last = gated_delta_rule(*x[:5], initial_state=x[5])
+        runs.append((out.detach()[:, t:], last.detach(), torch.autograd.grad((out, last), x, (d, d1))))
+    (o, l, a), (o2, l2, b) = runs
+    assert torch.equal(o, o2) and torch.equal(l, l2) and float(o.abs().max()) > 0
+    assert torch.equal(a[2][:, :t], b[2][:, :t]) and torch.equal(a[5], b[5])  # dv before it, and the initial state's
