@@ -116,3 +116,41 @@ def test_nothing_comes_through_a_reset(t, dtype, strength):
     (o, l, a), (o2, l2, b) = runs
     assert torch.equal(o, o2) and torch.equal(l, l2) and float(o.abs().max()) > 0
     assert torch.equal(a[2][:, :t], b[2][:, :t]) and torch.equal(a[5], b[5])  # dv before it, and the initial state's
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [(2, 150, 1, 2, 64, 48), (1, 100, 2, 4, 128, 33), (1, 70, 1, 3, 40, 72)])
+def test_every_token_of_its_own_size(size, dtype):
+    """Values, queries, output gradients (2^-12 to 2^12), keys (2^-24 to 1) and strengths (2^-20 to 1) of every token's own
+    size.  The allowance is that of one large token, above; the plain recurrence's error is taken over all tokens."""
+    B, T, Hk, Hv, dk, dv = size
+    x = list(R.inputs(*size, dtype=dtype, seed=T))
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(T)
+
+    def powers(lo, hi, heads):
+        return torch.exp2(torch.randint(lo, hi + 1, (B, T, heads), device="cuda", generator=gen).float())
+
+    x[0] = (x[0].float() * powers(-12, 12, Hk)[..., None]).to(dtype)
+    x[1] = (x[1].float() * powers(-24, 0, Hk)[..., None]).to(dtype)
+    x[2] = (x[2].float() * powers(-12, 12, Hv)[..., None]).to(dtype)
+    x[4] = x[4] * powers(-20, 0, Hv)
+    do = (torch.randn(B, T, Hv, dv, device="cuda", generator=gen) * powers(-12, 12, Hv)[..., None]).to(dtype)
+    ds = torch.randn(B, Hv, dk, dv, device="cuda", generator=gen)
+    mine = [y.clone().requires_grad_(True) for y in x]
+    out, last = gated_delta_rule(*mine[:5], initial_state=mine[5])
+    got = (out.detach(), last.detach()) + torch.autograd.grad((out, last), mine, (do, ds))
+    want, rough = plain(x, do, ds), plain(x, do, ds, torch.float32)
+    for name, a, b, c in zip(NAMES, got, want, rough):
+        allowed = 3e-3 if a.dtype == torch.bfloat16 else 1e-5
+        err, rerr, length = a.double() - b, c.double() - b, b
+        if name in ("state", "dstate"):
+            err, rerr, length = (y.flatten(2).norm(dim=-1) for y in (err, rerr, length))
+        elif name in ("dg", "dbeta"):
+            # single numbers may cancel: a token's, among the eight around it
+            err, rerr, length = (y.square().unfold(1, 8, 1).sum(-1).sqrt() for y in (err, rerr, length))
+        else:
+            err, rerr, length = (y.norm(dim=-1) for y in (err, rerr, length))
+        rough_rel = float((rerr / length).square().mean().sqrt())
+        worst = float((err / length).max())
+        assert worst <= allowed + 16 * rough_rel, (name, worst, rough_rel)
