@@ -31,7 +31,7 @@ namespace {
 // scan: one CTA per (batch, value head, 32 value columns), last chunk first, in
 // the forward scan's division of work: eight warps, four quarters of the rows x
 // two groups of 16 columns, dS in registers, planes through shared memory
-// between three barriers a chunk (2048 chunks of heads of 128 x 128, bf16: 225 us;
+// between three barriers a chunk (2048 chunks of heads of 128 x 128, bf16: 260 us;
 // bound by the chain of four dependent products a chunk).
 // ---------------------------------------------------------------------------
 
@@ -245,10 +245,13 @@ __global__ void __launch_bounds__(kThreads, 2) delta_back_scan_kernel(const Prob
 // or two steps loading meanwhile.  A warp keeps 16 tokens x 32 key columns of
 // dQ, dK_row and dK_col, and of 16 or 32 tokens of dO U^T and Z U^T, in
 // registers: sixteen warps for 128 key columns, eight for 64, where two CTAs
-// then share an SM (2048 chunks of heads of 64, FP32: 165 us, with sixteen warps
-// of half the tile a fifth more; of 128, bf16: 299 us).  Bound by the latency of
-// products and barriers; the tensor pipe is a third busy, the most of any of
-// these kernels.
+// then share an SM (2048 chunks of heads of 64, FP32: 190 us, sixteen warps of half
+// the tile took a fifth more; of 128, bf16: 326 us).  Bound by the latency of products
+// and barriers; the tensor pipe is a third busy, the most of any of these kernels.
+//
+// dP' and M are summed over along both sides, so they are held twice: with the other
+// factor's scales in them and a scale a row, and the same a column.  One tile with one
+// scale would give a token the digits that the largest of 64 leaves it.
 // ---------------------------------------------------------------------------
 
 // A lower 64 x 64 matrix as its ten 16 x 16 tiles on and below the diagonal.
@@ -449,8 +452,8 @@ __global__ void __launch_bounds__(GradSmem<Planes<T>::n, DK>::threads, DK == 64 
         }
       };
       // of eight warps, half begin with what takes shared memory and no tensor core
-      // (training 64 x 512 437 us, 441 where all end with it; sixteen are spread by
-      // themselves: training 4 x 2048 757 us, 768)
+      // (training 64 x 512 505 us, 510 where all end with it; sixteen are spread by
+      // themselves)
       const bool early = split == 2 && (m0 & 16);
       if (early) state_dot();
       uint32_t fz[2][4], fe[2][4];

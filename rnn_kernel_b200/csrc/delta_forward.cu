@@ -36,7 +36,7 @@ struct Range {
 // a small grid one for each of those.
 // Latency-bound (a chain of small products between barriers), so it keeps its
 // shared memory small enough for several CTAs on an SM (2048 chunks of heads of
-// 128, two to a key head: 64 us).
+// 128, two to a key head: 76 us).
 // ---------------------------------------------------------------------------
 
 constexpr int kLd = 68;  // row length of the FP32 64 x 64 tiles: a multiple of 4, not of 32
@@ -538,15 +538,15 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * DK > 256 ? 2 : 3) delta_
 // x two groups of 16 columns.  The state stays in registers as FP32
 // accumulators; its planes, those of B R and of U go through shared memory
 // between three barriers a chunk (two of them among a group's four warps only),
-// every warp's quarter with its own scale, so that no scale needs an exchange of
-// its own.  K, W and the gates are loaded a
-// chunk ahead; so are the warp's values of V, into registers.
+// with scales of a warp's own quarter or tokens, so that no scale needs an
+// exchange of its own.  K, W and the gates are loaded a chunk ahead; so are the
+// warp's values of V, into registers.
 //
-// Bound by the chain of three dependent products a chunk (2.6 us at 128 x 128,
-// of which the tensor pipe is busy a quarter).  (With a warp to 16
-// columns that keeps its whole state in registers and needs no barrier, the
-// same work took 6.6 us a chunk at 128 x 128: one warp a scheduler hides none
-// of its 3200 instructions' latencies.)
+// Bound by the chain of three dependent products a chunk (3.2 us at 128 x 128, of
+// which the tensor pipe is busy a quarter; 2.6 with a scale to 16 tokens and one
+// plane of the states kept).  With a warp to 16 columns that keeps its whole state
+// in registers and needs no barrier, the same work took 6.6 us where this took
+// 2.6: one warp a scheduler hides none of its 3200 instructions' latencies.
 // ---------------------------------------------------------------------------
 
 template <int NP, int DK>
@@ -734,7 +734,8 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const Problem a
 // warp takes 16 tokens x 32 columns.  Every operand keeps both planes, whatever
 // the output's type: an FP32 result is rounded once, when it is stored (one
 // plane of each, 2^-12 of the operands' size, moved a tenth of the bf16 outputs
-// by their last bit).  Bound by the latency of its loads.
+// by their last bit).  2048 chunks of heads of 128 x 128, bf16: 78 us, with one
+// plane 46.  Bound by the latency of its loads; memory is a third busy.
 // ---------------------------------------------------------------------------
 
 template <typename T, int DK>
@@ -985,8 +986,8 @@ int run_prepare(const Problem& a, Range r, cudaStream_t stream) {
   LaunchScope scope(kKindDeltaRule, stream);
   const long ctas = (long)a.B * a.Hk * r.n;
   // While SMs are left over, a value head of its own CTA costs only the products of
-  // keys once more (a prompt of 77, 4 key and 8 value heads: 48.7 us from call to
-  // result, 53.6 with both in turn); in a full grid that would be work for nothing.
+  // keys once more (a prompt of 77, 4 key and 8 value heads: 48 us from call to
+  // result, 53 with both in turn); in a full grid that would be work for nothing.
   r.parts = ctas * a.rep <= 148 ? a.rep : 1;
   delta_prepare_kernel<T, DK><<<(unsigned)(ctas * r.parts), kThreads, bytes, stream>>>(a, r);
   GRU_CUDA_TRY(cudaGetLastError());
@@ -1021,8 +1022,8 @@ int run_output(const Problem& a, Range r, cudaStream_t stream) {
 // Worth its launches where those two take long themselves, from 2048 chunks of
 // heads on (about 0.1 ms of them at 128 x 128).
 // The first range's preparation and the last one's outputs have no scan beside
-// them, so those two are half as long (a prompt of 16384 900 us, in four equal
-// ranges 934, two 958, eight 985).
+// them, so those two are half as long (a prompt of 16384 1192 us, in four equal
+// ranges 1232, two 1244, six 1262, not cut 1765).
 constexpr int kEnds[] = {1, 3, 5, 6};  // of the ranges, in sixths of the chunks
 constexpr int kRanges = sizeof(kEnds) / sizeof(int);
 template <typename T, int DK>

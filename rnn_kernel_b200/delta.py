@@ -12,12 +12,13 @@ decay ``g_t`` and writing strength ``beta_t``, does::
   convention: ``(input, state) -> (output, state)``.
 
 q, k and v are FP32 or bf16, gates and states FP32.  Sums are FP32; what the
-tensor cores multiply keeps 22 bits down to 2^-17 of the largest number that
-shares its scale, and 2^-39 of that below.  A token's head of q and of k has a
-scale of its own, and 16 of its values (of 16 neighbouring value columns) have:
-no token loses digits to another's size.  A value or key column far smaller than
-its neighbours does lose them to those: below 2^-17 of the largest of the 16
-value columns, or of the token's key.  Value heads may outnumber key heads (``Hv = n Hk``: value head h
+tensor cores multiply keeps 22 bits of a number down to 2^-17 of the largest that
+shares its scale, and 2^-39 of that below.  A token's head of q or k has a scale,
+and so have 16 neighbouring value columns of a token; of a state, a quarter of its
+key columns x 16 value columns, and 16 tokens in what they add to it.  So tokens of
+any size leave one another their digits, except where a state holds them in
+different key columns; and a key or value column that is 2^17 times smaller than its
+neighbours loses digits to them.  Results are rounded to bf16 once.  Value heads may outnumber key heads (``Hv = n Hk``: value head h
 reads key head ``h // n``).  Shape problems raise ``ValueError``, device and
 dtype problems and CUDA failures ``RuntimeError``; there is no CPU fallback.
 """

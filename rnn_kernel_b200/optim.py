@@ -9,7 +9,8 @@ correction) in FP32 for FP32 or bf16 weights::
 
 ``state_bits=8`` holds each moment in one byte: blocks of 256 elements share an
 FP32 scale, codes are logarithmic with 3 mantissa bits, and rounding is
-stochastic from ``(seed, step, position)``, so a run repeats bit for bit.  A
+stochastic from ``(seed, step, position)``, so a run repeats bit for bit; ``eps``
+must be 2^-50 or more, since second moments below 2^-100 are held as zero.  A
 block that meets a gradient that is not finite has NaN moments from then on,
 as 32-bit moments of those elements would.  CUDA tensors only; there is no
 fallback.
@@ -101,8 +102,10 @@ class AdamW:
 
     ``params`` is an iterable of tensors, or of dicts with ``"params"`` and
     optionally ``"lr"`` and ``"weight_decay"``; ``param_groups`` holds them, and
-    a schedule may set a group's ``"lr"`` between steps.  Parameters without a
-    gradient are skipped and keep their own step count.
+    a schedule may set a group's ``"lr"`` between steps (the object is no
+    ``torch.optim.Optimizer``, which torch's schedulers ask for; its parameters
+    are fixed).  Parameters without a gradient are skipped and keep their own step
+    count.  Copies and pickles are optimizers of their own.
 
     ``capturable=True`` keeps the step count on the device, so that a step
     captured in a CUDA graph advances with every replay; the learning rates
