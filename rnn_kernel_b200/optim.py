@@ -181,28 +181,36 @@ class AdamW:
             if self._steady:
                 self._steps[:] = self._calls
             self._steady = False
+        before = self._calls, None if self._steady else self._steps.copy()
         self._calls += 1
         b1, b2 = self.betas
         dev = self.device.index
         scales = (None, None) if self.scale_avg is None else (self.scale_avg.data_ptr(), self.scale_sq.data_ptr())
         counter = None if self._device_step is None else self._device_step.data_ptr()
         scalars = None if self._scalars is None else self._scalars.data_ptr()
-        with _lib.on_device(dev):
-            stream = _lib.raw_stream(dev)
-            for table, without in zip(self._tables, missing):
-                entries, address = table.entries, table.address
-                if without is not None:
-                    entries = entries[~without]
-                    address = entries.ctypes.data
-                if not len(entries):
-                    continue
-                self._rates(table, entries, without)
-                _lib.check(lib.gru_adamw_step(
-                    address, len(entries), table.code, self.state_bits, self.exp_avg.data_ptr(),
-                    self.exp_avg_sq.data_ptr(), *scales, self.state_elems, b1, b2, self.eps, grad_scale, self.seed,
-                    self._calls, counter, scalars, stream), "gru_adamw_step")
-                counter = None  # counted once for all element types
-                table.copies = None
+        try:
+            with _lib.on_device(dev):
+                stream = _lib.raw_stream(dev)
+                for table, without in zip(self._tables, missing):
+                    entries, address = table.entries, table.address
+                    if without is not None:
+                        entries = entries[~without]
+                        address = entries.ctypes.data
+                    if not len(entries):
+                        continue
+                    self._rates(table, entries, without)
+                    _lib.check(lib.gru_adamw_step(
+                        address, len(entries), table.code, self.state_bits, self.exp_avg.data_ptr(),
+                        self.exp_avg_sq.data_ptr(), *scales, self.state_elems, b1, b2, self.eps, grad_scale, self.seed,
+                        self._calls, counter, scalars, stream), "gru_adamw_step")
+                    counter = None  # counted once for all element types
+                    table.copies = None
+        except Exception:
+            # a refused step is none: its number stays the next one's
+            self._calls = before[0]
+            if before[1] is not None:
+                self._steps[:] = before[1]
+            raise
         torch.autograd.graph.increment_version(self.params)
 
     def _rates(self, table, entries, without) -> None:

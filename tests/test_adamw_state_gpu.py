@@ -93,3 +93,24 @@ def test_trainer_steps_as_the_optimizer_over_its_parameters(bits):
         assert torch.equal(p.detach(), q.detach())
     if bits == 8:
         assert [n for _, n in trainer.optimizer.offsets()] == [p.numel() for p in m.parameters()]
+
+
+@pytest.mark.parametrize("missing", [False, True])
+def test_a_refused_step_is_not_counted(missing):
+    """The call refuses (a negative eps), the caller mends it: as if it had not been made."""
+    a, b = params_of([300, 40], seed=2), params_of([300, 40], seed=2)
+    oa, ob = AdamW(a, lr=1e-2, state_bits=8), AdamW(b, lr=1e-2, state_bits=8)
+    for t in range(4):
+        for ps in (a, b):
+            gradients(ps, t)
+            if missing and t == 1:
+                ps[1].grad = None
+        if t == 2:
+            eps, ob.eps = ob.eps, -1.0
+            with pytest.raises(RuntimeError, match="eps"):
+                ob.step()
+            ob.eps = eps
+        oa.step()
+        ob.step()
+    assert oa.state_dict()["steps"] == ob.state_dict()["steps"]
+    assert all(torch.equal(p.detach(), q.detach()) for p, q in zip(a, b))
