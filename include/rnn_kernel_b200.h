@@ -202,6 +202,110 @@ int gru_delta_backward(const gru_delta_args* args, const void* dout, const float
  * updated in place, out is dense [B, Hv, dv]. */
 int gru_delta_step(const gru_delta_args* args, float* state, void* out, void* stream);
 
+/* ---- Selective state space scan (no reference counterpart): a recurrent layer
+ * that keeps N numbers h per batch row and channel.  Per token, for channel d
+ * of group g = d / (D / G):
+ *   step = dt + dt_bias, through log(1 + e^.) if dt_softplus
+ *   h[n] = e^(step a[d, n]) h[n] + step x b[g, n]
+ *   out = (sum_n c[g, n] h[n] + skip x), times z / (1 + e^-z) with a gate z
+ * step * a <= 0 is asked for (decays).  x, dt, b, c, z, out and their gradients
+ * are of `dtype`, all else is FP32. ---- */
+typedef struct {
+  int dtype; /* GRU_F32 or GRU_BF16 */
+  int B, T, D, N, G; /* 1 <= N <= 64; D a multiple of G */
+  int dt_softplus;   /* 0 or 1 */
+  const void *x, *dt, *b, *c, *z; /* [B, T, D] (z may be NULL); b and c [B, T, G, N] */
+  const float* a;                 /* dense [D, N] */
+  const float *skip, *dt_bias;    /* [D], or NULL for zeros */
+  const float* initial_state;     /* dense [B, D, N], or NULL for zeros */
+  /* elements between batch rows and tokens (and groups); a token's channels and
+   * a group's states are consecutive */
+  long x_stride[2], dt_stride[2], z_stride[2], b_stride[3], c_stride[3];
+} gru_scan_args; /* host struct */
+
+/* Bytes that a training forward leaves for gru_scan_backward, and that call's
+ * workspace, from the sizes alone; 0 and an error text for sizes that they refuse. */
+size_t gru_scan_stash_bytes(const gru_scan_args* args);
+size_t gru_scan_workspace_bytes(const gru_scan_args* args);
+
+/* All T tokens: out dense [B, T, D], final_state dense [B, D, N].  stash:
+ * gru_scan_stash_bytes() bytes for a training forward, or NULL. */
+int gru_scan_forward(const gru_scan_args* args, void* out, float* final_state, void* stash, size_t stash_bytes,
+                     void* stream);
+
+/* Gradients (dense, overwritten) of everything that the forward read, from dout
+ * dense [B, T, D] and dfinal dense [B, D, N] (either NULL: zeros); dskip, ddt_bias
+ * and dinitial may be NULL, dz where z is.  args: the forward's. */
+int gru_scan_backward(const gru_scan_args* args, const void* dout, const float* dfinal, const void* stash,
+                      size_t stash_bytes, void* dx, void* ddt, float* da, void* db, void* dc, float* dskip, void* dz,
+                      float* ddt_bias, float* dinitial, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token (T = 1, initial_state unused): state dense [B, D, N] is updated in
+ * place, out is dense [B, D]. */
+int gru_scan_step(const gru_scan_args* args, float* state, void* out, void* stream);
+
+/* ---- Short causal convolution (no reference counterpart) of every channel with
+ * W weights of its own:
+ *   out_t = bias + sum_j weight[d, j] x_(t - W + 1 + j), through v / (1 + e^-v)
+ *   if activation = 1
+ * Tokens before the first are the initial state's, oldest first. ---- */
+typedef struct {
+  int dtype;        /* GRU_F32 or GRU_BF16: x, states, out and their gradients */
+  int weight_dtype; /* of weight, bias and their gradients: dtype or GRU_F32 */
+  int B, T, D, W;   /* 2 <= W <= 8 */
+  int activation;   /* 0 none, 1 silu */
+  const void* x;               /* [B, T, D], channels consecutive */
+  const void *weight, *bias;   /* dense [D, W]; [D] or NULL */
+  const void* initial_state;   /* dense [B, W - 1, D], or NULL for zeros */
+  long x_stride[2];            /* elements between batch rows and tokens */
+} gru_conv_args; /* host struct */
+
+/* Workspace of gru_conv_backward; 0 and an error text for refused sizes. */
+size_t gru_conv_workspace_bytes(const gru_conv_args* args);
+
+/* out dense [B, T, D]; final_state dense [B, W - 1, D]: the last W - 1 inputs, not
+ * in the initial state's memory. */
+int gru_conv_forward(const gru_conv_args* args, void* out, void* final_state, void* stream);
+
+/* Gradients (dense, overwritten) from dout dense [B, T, D] and dfinal dense
+ * [B, W - 1, D] (either NULL: zeros); dbias and dinitial may be NULL. */
+int gru_conv_backward(const gru_conv_args* args, const void* dout, const void* dfinal, void* dx, void* dweight,
+                      void* dbias, void* dinitial, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token (T = 1, initial_state unused): state dense [B, W - 1, D] is moved on in
+ * place, out is dense [B, D]. */
+int gru_conv_step(const gru_conv_args* args, void* state, void* out, void* stream);
+
+/* ---- Layer normalisation of rows, with a residual sum in front (no reference
+ * counterpart):
+ *   s = x + residual, in the residual's type (s = x without one)
+ *   out = (s - mean) / sqrt(variance + eps) weight + bias ---- */
+typedef struct {
+  int dtype;          /* GRU_F32 or GRU_BF16: x, out */
+  int residual_dtype; /* dtype or GRU_F32; dtype where there is no residual */
+  int weight_dtype;   /* dtype or GRU_F32 */
+  int width;          /* 1 .. 16384 */
+  float eps;
+  long rows;
+  long row_stride, residual_row_stride; /* elements between rows of x and of the residual */
+} gru_norm_args; /* host struct */
+
+/* Workspace of gru_layer_norm_backward; 0 and an error text for refused sizes. */
+size_t gru_layer_norm_workspace_bytes(const gru_norm_args* args);
+
+/* out dense [rows, width]; sum dense, with a residual; stats [3, rows] for the
+ * gradient (two parts of the mean, 1 / deviation), or NULL; bias may be NULL. */
+int gru_layer_norm_forward(const gru_norm_args* args, const void* x, const void* residual, const void* weight,
+                           const void* bias, void* out, void* sum, float* stats, void* stream);
+
+/* Gradients (dense, overwritten) from dout and dsum (of s's type; or NULL: zeros),
+ * both dense.  sum: s as the forward stored it, or x without a residual
+ * (row_stride: its rows').  dx is the gradient in x's type, dresidual the same in
+ * s's; either may be NULL, and dbias. */
+int gru_layer_norm_backward(const gru_norm_args* args, const void* sum, const void* weight, const float* stats,
+                            const void* dout, const void* dsum, void* dx, void* dresidual, void* dweight, void* dbias,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 /* Time chunks (no reference counterpart; a scheduling knob of this library).
  * When the time loops leave SMs idle (e.g. 104 of 148 at H = 256, B = 64),
  * gru_forward and gru_backward run the sequence as n consecutive chunks and
@@ -230,7 +334,8 @@ int gru_set_small_loops(int mode);
  * scripts/profile_a100_h256_step.py).  Kernel kinds: 0 input-projection GEMM,
  * 1 forward time loop, 2 backward time loop, 3 gradient products (dW, dx;
  * + split-K reduce), 4 bias-gradient column sums, 5 padding / transpose
- * copies, 6 MSE loss and its gradient, 7 AdamW, 8 gated delta rule. ---- */
+ * copies, 6 MSE loss and its gradient, 7 AdamW, 8 gated delta rule,
+ * 9 selective scan, 10 causal convolution, 11 layer norm. ---- */
 
 /* Device status word of the current device: 0 when every kernel so far ran
  * to completion, else GRU_STATUS_* bits (a bounded wait inside a time-loop

@@ -14,7 +14,18 @@ from .gru import (
     is_supported_gru,
 )
 from .loss import MSELossFunction, mse_loss
+from .norm import LayerNorm, LayerNormFunction, layer_norm
 from .optim import AdamW
+from .scan import (
+    CausalConvFunction,
+    RecurrentStack,
+    SelectiveScan,
+    SelectiveScanFunction,
+    causal_conv,
+    causal_conv_step,
+    selective_scan,
+    selective_step,
+)
 from .train import DataParallelTrainer, GraphedTrainStep, HostBatchPrefetcher, flatten_parameters_
 
 B200GRU = GRU
@@ -24,7 +35,18 @@ __all__ = [
     "GRU",
     "B200GRU",
     "GRUFunction",
+    "CausalConvFunction",
+    "LayerNorm",
+    "LayerNormFunction",
     "MAX_HIDDEN_SIZE",
+    "RecurrentStack",
+    "SelectiveScan",
+    "SelectiveScanFunction",
+    "causal_conv",
+    "causal_conv_step",
+    "layer_norm",
+    "selective_scan",
+    "selective_step",
     "DataParallelTrainer",
     "GraphedTrainStep",
     "GatedDelta",

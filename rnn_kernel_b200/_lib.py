@@ -38,6 +38,10 @@ _int = ctypes.c_int
 # gru_delta_args of include/rnn_kernel_b200.h, packed into bytes (which a call
 # takes as its pointer)
 DELTA_ARGS = struct.Struct("@7if6P15q")
+# gru_scan_args, gru_conv_args and gru_norm_args likewise
+SCAN_ARGS = struct.Struct("@7i9P12q")
+CONV_ARGS = struct.Struct("@7i4P2q")
+NORM_ARGS = struct.Struct("@4if3q")
 
 
 # name -> (restype, argtypes); mirrors include/rnn_kernel_b200.h
@@ -68,12 +72,24 @@ SIGNATURES = {
     "gru_delta_backward": (_int, [ctypes.c_void_p] * 4 + [_size_t] + [ctypes.c_void_p] * 7
                            + [_size_t, ctypes.c_void_p]),
     "gru_delta_step": (_int, [ctypes.c_void_p] * 4),
+    "gru_scan_stash_bytes": (_size_t, [ctypes.c_void_p]),
+    "gru_scan_workspace_bytes": (_size_t, [ctypes.c_void_p]),
+    "gru_scan_forward": (_int, [ctypes.c_void_p] * 4 + [_size_t, ctypes.c_void_p]),
+    "gru_scan_backward": (_int, [ctypes.c_void_p] * 4 + [_size_t] + [ctypes.c_void_p] * 10 + [_size_t, ctypes.c_void_p]),
+    "gru_scan_step": (_int, [ctypes.c_void_p] * 4),
+    "gru_conv_workspace_bytes": (_size_t, [ctypes.c_void_p]),
+    "gru_conv_forward": (_int, [ctypes.c_void_p] * 4),
+    "gru_conv_backward": (_int, [ctypes.c_void_p] * 8 + [_size_t, ctypes.c_void_p]),
+    "gru_conv_step": (_int, [ctypes.c_void_p] * 4),
+    "gru_layer_norm_workspace_bytes": (_size_t, [ctypes.c_void_p]),
+    "gru_layer_norm_forward": (_int, [ctypes.c_void_p] * 9),
+    "gru_layer_norm_backward": (_int, [ctypes.c_void_p] * 11 + [_size_t, ctypes.c_void_p]),
     "gru_timing_enable": (_int, [_int]),
     "gru_timing_collect": (_int, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int), _int]),
 }
 
 KERNEL_KINDS = ("input_gemm", "fwd_recurrent", "bwd_recurrent", "grad_gemm", "colsum", "layout", "loss", "optimizer",
-                "delta_rule")
+                "delta_rule", "selective_scan", "causal_conv", "layer_norm")
 
 
 def timing_enable(on: bool) -> None:

@@ -1,0 +1,407 @@
+// The short causal convolution of each channel with its own W weights, its
+// gradient and its single token (contract in include/rnn_kernel_b200.h).
+//
+//   p_t = bias + sum_j w_j x_{t-W+1+j};  y = p, or silu(p) = p sigmoid(p)
+//   e = dy silu'(p);  dx_t = sum_j w_j e_{t+W-1-j};  dw_j = sum_t e_t x_{t-W+1+j};  db = sum_t e_t
+//
+// Tokens before the first come from a state of W - 1 inputs.  A thread takes a
+// few neighbouring channels through a run of tokens with the last W - 1 inputs
+// in registers, so x is read once, but for the W - 1 tokens that two runs share.
+// The gradient keeps the last W errors too: e_t is final when x_t is read, and
+// with it dx_{t-W+1}.  Sums of dw and db go from a thread's registers over the
+// CTA's runs and then over the CTAs, in a fixed order.  Bound by memory.
+
+#include <algorithm>
+
+#include "row_ops.cuh"
+
+namespace gru {
+namespace {
+
+constexpr int kMinConv = 2, kMaxConv = 8;
+constexpr int kGradRuns = 8;    // runs of tokens of a gradient's CTA
+constexpr int kGradRun = 32;    // tokens of one of them
+
+struct Conv {
+  const void *x, *w, *bias, *s0;
+  void *y, *last;
+  // gradient
+  const void *dy, *dlast;
+  void *dx, *ds0;
+  float* part;  // [CTA of tokens][W + 1][D]
+  long xb, xt;  // elements between x's batch rows and tokens
+  int B, T, D, W, wtype, silu, run, runs;
+};
+
+// x at token t of a batch row, from the state before the first (T <= t: zero).
+template <typename T, int V>
+__device__ __forceinline__ void token(const Conv& a, int b, int c, int t, float (&v)[V]) {
+  if (t >= 0 && t < a.T) {
+    load_row<V>(static_cast<const T*>(a.x) + b * a.xb + t * a.xt + c, v);
+  } else if (t < 0 && a.s0) {
+    load_row<V>(static_cast<const T*>(a.s0) + ((long)b * (a.W - 1) + (a.W - 1 + t)) * a.D + c, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = 0.0f;
+  }
+}
+
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(256) conv_forward_kernel(const Conv a) {
+  const int vecs = a.D / V;
+  const long item = blockIdx.x * 256L + threadIdx.x;
+  const long rest = item / vecs;
+  const int c = (int)(item - rest * vecs) * V;
+  const int b = (int)(rest / a.runs);
+  if (b >= a.B) return;
+  const int t0 = (int)(rest - (long)b * a.runs) * a.run, t1 = min(t0 + a.run, a.T);
+  float w[V][W], bias[V], win[W][V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[e][j] = get(a.w, (long)(c + e) * W + j, a.wtype);
+    bias[e] = a.bias ? get(a.bias, c + e, a.wtype) : 0.0f;
+  }
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j) token<T, V>(a, b, c, t0 - (W - 1) + j, win[j]);
+  T* y = static_cast<T*>(a.y) + ((long)b * a.T + t0) * a.D + c;
+  constexpr int U = 4;  // tokens loaded together
+  for (int t = t0; t < t1; t += U) {
+    float x[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) token<T, V>(a, b, c, t + u, x[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float p[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        p[e] = bias[e];
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) p[e] = fmaf(w[e][j], win[j][e], p[e]);
+        p[e] = fmaf(w[e][W - 1], x[u][e], p[e]);
+        if (a.silu) p[e] *= sigmoid_of(p[e]);
+#pragma unroll
+        for (int j = 0; j + 1 < W - 1; ++j) win[j][e] = win[j + 1][e];
+        win[W - 2][e] = x[u][e];
+      }
+      if (t + u < t1) store_row<V>(y, p);
+      y += a.D;
+    }
+  }
+  if (t1 == a.T) {
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) {
+      float v[V];
+      token<T, V>(a, b, c, a.T - (W - 1) + j, v);
+      store_row<V>(static_cast<T*>(a.last) + ((long)b * (W - 1) + j) * a.D + c, v);
+    }
+  }
+}
+
+// A CTA: 32 lanes x V channels, kGradRuns runs of tokens, one a warp.
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(32 * kGradRuns) conv_backward_kernel(const Conv a) {
+  extern __shared__ float sums[];  // [run][W + 1][32 V]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int blocks = ceil_div(a.D, 32 * V);
+  const int cb = blockIdx.x % blocks;
+  const long rest = blockIdx.x / blocks;  // batch row and run group
+  const int groups = ceil_div(a.runs, kGradRuns);
+  const int b = (int)(rest / groups), run = (int)(rest - (long)b * groups) * kGradRuns + warp;
+  const int c = (cb * 32 + lane) * V;
+  float dw[V][W], db[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    db[e] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) dw[e][j] = 0.0f;
+  }
+  if (c < a.D && run < a.runs) {
+    const int t0 = run * a.run, t1 = min(t0 + a.run, a.T);
+    float w[V][W], bias[V], win[W][V], err[W][V];  // inputs up to t, errors up to t
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        w[e][j] = get(a.w, (long)(c + e) * W + j, a.wtype);
+        err[j][e] = 0.0f;
+      }
+      bias[e] = a.bias ? get(a.bias, c + e, a.wtype) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) token<T, V>(a, b, c, t0 - (W - 1) + j, win[j]);
+    const T* dy = static_cast<const T*>(a.dy);
+    // Errors of the W - 1 tokens behind the run belong to its dx; the first run's
+    // errors also go to the state.
+    constexpr int U = 4;
+    for (int t = t0; t < t1 + W - 1; t += U) {
+      float x[U][V], d[U][V];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        token<T, V>(a, b, c, t + u, x[u]);
+        if (dy && t + u < a.T) {
+          load_row<V>(dy + ((long)b * a.T + t + u) * a.D + c, d[u]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) d[u][e] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int now = t + u;
+        if (now >= t1 + W - 1) break;
+        float g[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          win[W - 1][e] = x[u][e];
+          float p = bias[e];
+#pragma unroll
+          for (int j = 0; j < W; ++j) p = fmaf(w[e][j], win[j][e], p);
+          float q = d[u][e];
+          if (a.silu) {
+            const float s = sigmoid_of(p);
+            q *= s * fmaf(p, 1.0f - s, 1.0f);
+          }
+          if (now >= a.T) q = 0.0f;
+          if (now < t1) {
+            db[e] += q;
+#pragma unroll
+            for (int j = 0; j < W; ++j) dw[e][j] = fmaf(q, win[j][e], dw[e][j]);
+          }
+#pragma unroll
+          for (int j = 0; j + 1 < W; ++j) {
+            win[j][e] = win[j + 1][e];
+            err[j][e] = err[j + 1][e];
+          }
+          err[W - 1][e] = q;
+          // dx of token now - W + 1, whose errors are err[0] .. err[W - 1]
+          g[e] = 0.0f;
+#pragma unroll
+          for (int j = 0; j < W; ++j) g[e] = fmaf(w[e][W - 1 - j], err[j][e], g[e]);
+        }
+        const int to = now - (W - 1);
+        if (to < t0 && t0 > 0) continue;  // an earlier run's
+        if (a.dlast && to >= a.T - (W - 1)) {
+          float s[V];
+          load_row<V>(static_cast<const T*>(a.dlast) + ((long)b * (W - 1) + to - (a.T - (W - 1))) * a.D + c, s);
+#pragma unroll
+          for (int e = 0; e < V; ++e) g[e] += s[e];
+        }
+        if (to >= 0) store_row<V>(static_cast<T*>(a.dx) + ((long)b * a.T + to) * a.D + c, g);
+        else if (a.ds0) store_row<V>(static_cast<T*>(a.ds0) + ((long)b * (W - 1) + (W - 1) + to) * a.D + c, g);
+      }
+    }
+  }
+  constexpr int C = 32 * V;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) sums[(warp * (W + 1) + j) * C + lane * V + e] = dw[e][j];
+    sums[(warp * (W + 1) + W) * C + lane * V + e] = db[e];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < (W + 1) * C; i += 32 * kGradRuns) {
+    const int col = cb * C + i % C;
+    if (col >= a.D) continue;
+    float s = sums[i];
+#pragma unroll
+    for (int r = 1; r < kGradRuns; ++r) s += sums[r * (W + 1) * C + i];
+    a.part[(rest * (W + 1) + i / C) * a.D + col] = s;
+  }
+}
+
+// One token: the state moves on by one input.
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(128) conv_step_kernel(const Conv a) {
+  const int vecs = a.D / V;
+  const long item = blockIdx.x * 128L + threadIdx.x;
+  const int b = (int)(item / vecs), c = (int)(item - (long)b * vecs) * V;
+  if (b >= a.B) return;
+  T* s = static_cast<T*>(a.last) + (long)b * (W - 1) * a.D + c;
+  float win[W][V], p[V];
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j) load_row<V>(s + (long)j * a.D, win[j]);
+  load_row<V>(static_cast<const T*>(a.x) + b * a.xb + c, win[W - 1]);
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j) store_row<V>(s + (long)j * a.D, win[j + 1]);
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    p[e] = a.bias ? get(a.bias, c + e, a.wtype) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) p[e] = fmaf(get(a.w, (long)(c + e) * W + j, a.wtype), win[j][e], p[e]);
+    if (a.silu) p[e] *= sigmoid_of(p[e]);
+  }
+  store_row<V>(static_cast<T*>(a.y) + (long)b * a.D + c, p);
+}
+
+struct StoreConv {
+  void *dw, *db;
+  int D, W, dtype;
+  __device__ __forceinline__ void operator()(long i, float x) const {
+    const long j = i / D, c = i - j * D;
+    if (j < W) put(dw, c * W + j, dtype, x);
+    else if (db) put(db, c, dtype, x);
+  }
+};
+
+enum Way { kForward, kBackward, kStep };
+
+template <typename T, int W, int V>
+int launch(const Conv& a, Way way, const StoreConv& store, cudaStream_t stream) {
+  if (way == kStep) {
+    LaunchScope scope(kKindCausalConv, stream);
+    conv_step_kernel<T, W, V><<<(unsigned)(((long)a.B * (a.D / V) + 127) / 128), 128, 0, stream>>>(a);
+  } else if (way == kForward) {
+    LaunchScope scope(kKindCausalConv, stream);
+    conv_forward_kernel<T, W, V><<<(unsigned)(((long)a.B * a.runs * (a.D / V) + 255) / 256), 256, 0, stream>>>(a);
+  } else {
+    LaunchScope scope(kKindCausalConv, stream, 2);
+    const int parts = a.B * ceil_div(a.runs, kGradRuns);
+    const size_t smem = sizeof(float) * kGradRuns * (W + 1) * 32 * V;
+    conv_backward_kernel<T, W, V><<<(unsigned)((long)parts * ceil_div(a.D, 32 * V)), 32 * kGradRuns, smem, stream>>>(a);
+    GRU_CUDA_TRY(cudaGetLastError());
+    const long cols = (W + 1L) * a.D;
+    return sum_parts(a.part, parts, cols, cols, store, stream);
+  }
+  GRU_CUDA_TRY(cudaGetLastError());
+  return GRU_OK;
+}
+
+// V: elements a thread; two where the window is long, for its registers' sake.
+template <typename T>
+int launch_any(const Conv& a, bool vec, Way way, const StoreConv& store, cudaStream_t stream) {
+#define GRU_CONV(WIDTH, V)                                                             \
+  if (a.W == WIDTH)                                                                  \
+    return vec ? launch<T, WIDTH, V>(a, way, store, stream) : launch<T, WIDTH, 1>(a, way, store, stream);
+  GRU_CONV(2, 4)
+  GRU_CONV(3, 4)
+  GRU_CONV(4, 4)
+  GRU_CONV(5, 2)
+  GRU_CONV(6, 2)
+  GRU_CONV(7, 2)
+  GRU_CONV(8, 2)
+#undef GRU_CONV
+  return GRU_ERR_UNSUPPORTED;
+}
+
+long grad_parts(const gru_conv_args& p) { return (long)p.B * ceil_div(ceil_div(p.T, kGradRun), kGradRuns); }
+
+int check(const char* me, const gru_conv_args* p) {
+  if (!p) return refuse(me, "null arguments");
+  if (!known(p->dtype) || !known(p->weight_dtype)) return refuse(me, "types must be GRU_F32 or GRU_BF16", GRU_ERR_UNSUPPORTED);
+  if (p->weight_dtype != p->dtype && p->weight_dtype != GRU_F32)
+    return refuse(me, "the weights must be FP32 or of x's type", GRU_ERR_UNSUPPORTED);
+  if (p->B < 0 || p->T < 0 || p->D < 1) return refuse(me, "need B >= 0, T >= 0 and D >= 1");
+  if (p->T > (1 << 30) || p->D > (1 << 24)) return refuse(me, "too many tokens or channels", GRU_ERR_UNSUPPORTED);
+  if (p->W < kMinConv || p->W > kMaxConv) return refuse(me, "the width must be in [2, 8]", GRU_ERR_UNSUPPORTED);
+  if (p->activation != 0 && p->activation != 1) return refuse(me, "activation must be 0 or 1", GRU_ERR_UNSUPPORTED);
+  // CTAs of the smallest pieces that a launch cuts the work into
+  const long runs = std::max(1L, (p->T + 7L) / 8);
+  if ((double)p->B * runs * p->D / 128 > 2e9) return refuse(me, "too large for one launch", GRU_ERR_UNSUPPORTED);
+  if (bits(p->x) & (elem_size(p->dtype) - 1) || bits(p->initial_state) & (elem_size(p->dtype) - 1) ||
+      bits(p->weight) & (elem_size(p->weight_dtype) - 1) || bits(p->bias) & (elem_size(p->weight_dtype) - 1))
+    return refuse(me, "a tensor is not aligned to its element size");
+  return GRU_OK;
+}
+
+void fill(Conv& a, const gru_conv_args& p) {
+  a.x = p.x, a.w = p.weight, a.bias = p.bias, a.s0 = p.initial_state;
+  a.xb = p.x_stride[0], a.xt = p.x_stride[1];
+  a.B = p.B, a.T = p.T, a.D = p.D, a.W = p.W, a.wtype = p.weight_dtype, a.silu = p.activation;
+}
+
+// Whether every row of the dense tensors and of x starts on the boundary that V
+// elements need.
+bool vectors(const gru_conv_args& p, uintptr_t all) {
+  const int v = p.W <= 4 ? 4 : 2;
+  return p.D % v == 0 && p.x_stride[0] % v == 0 && p.x_stride[1] % v == 0 && (all & (v * elem_size(p.dtype) - 1)) == 0;
+}
+
+}  // namespace
+}  // namespace gru
+
+using namespace gru;
+
+extern "C" size_t gru_conv_workspace_bytes(const gru_conv_args* p) {
+  if (check("gru_conv_workspace_bytes", p)) return 0;
+  return align_up(sizeof(float) * (size_t)grad_parts(*p) * (p->W + 1) * p->D, 256);
+}
+
+extern "C" int gru_conv_forward(const gru_conv_args* p, void* out, void* final_state, void* stream_) {
+  clear_error();
+  const char* me = "gru_conv_forward";
+  if (const int rc = check(me, p)) return rc;
+  if (p->B == 0) return GRU_OK;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  const uintptr_t es = elem_size(p->dtype);
+  if (!final_state || bits(final_state) & (es - 1)) return refuse(me, "null or misaligned final_state");
+  if (p->T == 0) {
+    const size_t n = es * p->B * (p->W - 1) * p->D;
+    if (!p->initial_state) GRU_CUDA_TRY(cudaMemsetAsync(final_state, 0, n, stream));
+    else if (p->initial_state != final_state)
+      GRU_CUDA_TRY(cudaMemcpyAsync(final_state, p->initial_state, n, cudaMemcpyDeviceToDevice, stream));
+    return GRU_OK;
+  }
+  if (!p->x || !p->weight || !out || bits(out) & (es - 1)) return refuse(me, "null tensor or misaligned out");
+  if (p->initial_state && p->initial_state == final_state) return refuse(me, "final_state must not be the initial state");
+  Conv a{};
+  fill(a, *p);
+  a.y = out, a.last = final_state;
+  const bool vec = vectors(*p, bits(p->x) | bits(p->initial_state) | bits(out) | bits(final_state));
+  // runs of 32 tokens, shorter ones where they would leave the GPU idle
+  const long lanes = (long)p->B * (p->D / (vec ? (p->W <= 4 ? 4 : 2) : 1));
+  a.run = 32;
+  while (a.run > 8 && lanes * ceil_div(p->T, a.run) < 148L * 1024) a.run /= 2;
+  a.runs = ceil_div(p->T, a.run);
+  return p->dtype == GRU_F32 ? launch_any<float>(a, vec, kForward, {}, stream) : launch_any<bf16>(a, vec, kForward, {}, stream);
+}
+
+extern "C" int gru_conv_backward(const gru_conv_args* p, const void* dout, const void* dfinal, void* dx, void* dweight,
+                                 void* dbias, void* dinitial, void* workspace, size_t workspace_bytes, void* stream_) {
+  clear_error();
+  const char* me = "gru_conv_backward";
+  if (const int rc = check(me, p)) return rc;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  const uintptr_t es = elem_size(p->dtype), ws = elem_size(p->weight_dtype);
+  if (!dweight || bits(dweight) & (ws - 1) || bits(dbias) & (ws - 1))
+    return refuse(me, "null or misaligned gradient of the weight");
+  if (bits(dout) & (es - 1) || bits(dfinal) & (es - 1) || bits(dx) & (es - 1) || bits(dinitial) & (es - 1))
+    return refuse(me, "a tensor is not aligned to its element size");
+  if (p->B == 0 || p->T == 0) {
+    GRU_CUDA_TRY(cudaMemsetAsync(dweight, 0, ws * p->D * p->W, stream));
+    if (dbias) GRU_CUDA_TRY(cudaMemsetAsync(dbias, 0, ws * p->D, stream));
+    const size_t n = es * p->B * (p->W - 1) * p->D;
+    if (n && dinitial && !dfinal) GRU_CUDA_TRY(cudaMemsetAsync(dinitial, 0, n, stream));
+    else if (n && dinitial && dfinal != dinitial)
+      GRU_CUDA_TRY(cudaMemcpyAsync(dinitial, dfinal, n, cudaMemcpyDeviceToDevice, stream));
+    return GRU_OK;
+  }
+  if (!p->x || !p->weight || !dx) return refuse(me, "null tensor");
+  if (!workspace || bits(workspace) & 15 || workspace_bytes < gru_conv_workspace_bytes(p))
+    return refuse(me, "workspace too small or not 16-byte aligned");
+  Conv a{};
+  fill(a, *p);
+  a.dy = dout, a.dlast = dfinal, a.dx = dx, a.ds0 = dinitial, a.part = static_cast<float*>(workspace);
+  a.run = kGradRun, a.runs = ceil_div(p->T, kGradRun);
+  const bool vec = vectors(*p, bits(p->x) | bits(p->initial_state) | bits(dout) | bits(dfinal) | bits(dx) | bits(dinitial));
+  const StoreConv store{dweight, dbias, p->D, p->W, p->weight_dtype};
+  return p->dtype == GRU_F32 ? launch_any<float>(a, vec, kBackward, store, stream)
+                             : launch_any<bf16>(a, vec, kBackward, store, stream);
+}
+
+extern "C" int gru_conv_step(const gru_conv_args* p, void* state, void* out, void* stream_) {
+  clear_error();
+  const char* me = "gru_conv_step";
+  if (const int rc = check(me, p)) return rc;
+  if (p->T != 1) return refuse(me, "T must be 1");
+  if (p->B == 0) return GRU_OK;
+  const uintptr_t es = elem_size(p->dtype);
+  if (!p->x || !p->weight || !state || !out || (bits(state) | bits(out)) & (es - 1))
+    return refuse(me, "null or misaligned tensor");
+  Conv a{};
+  fill(a, *p);
+  a.y = out, a.last = state;
+  const bool vec = vectors(*p, bits(p->x) | bits(state) | bits(out));
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  return p->dtype == GRU_F32 ? launch_any<float>(a, vec, kStep, {}, stream) : launch_any<bf16>(a, vec, kStep, {}, stream);
+}

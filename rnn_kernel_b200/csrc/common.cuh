@@ -24,7 +24,7 @@ void clear_error();
   } while (0)
 
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
-inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+constexpr int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // ---------------------------------------------------------------------------
 // Recurrent-kernel geometry.  One GRU layer's time loop runs on independent
@@ -193,7 +193,10 @@ enum KernelKind {
   kKindLoss = 6,        // MSE loss and its gradient
   kKindOptimizer = 7,   // AdamW
   kKindDeltaRule = 8,   // gated delta rule: forward, gradient, step
-  kKindCount = 9
+  kKindSelectiveScan = 9,  // selective scan: forward, gradient, step
+  kKindCausalConv = 10,    // short causal convolution: forward, gradient, step
+  kKindLayerNorm = 11,     // layer norm and its gradient
+  kKindCount = 12
 };
 
 class LaunchScope {

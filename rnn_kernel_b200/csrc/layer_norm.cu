@@ -1,0 +1,414 @@
+// Layer normalisation of rows, with the sum of a residual stream in front, and
+// its gradient (contract in include/rnn_kernel_b200.h).
+//
+//   s = x + residual (in the residual's type);  n = (s - mean) rstd;  y = n w + b
+//   ds += rstd (g - mean(g) - n mean(g n)) with g = dy w;  dw = sum dy n;  db = sum dy
+//
+// A row is in registers from its one read to its one write: a warp holds rows
+// of up to 1024 bf16 or 512 FP32 elements, a CTA longer ones, 16 bytes a thread
+// and load.  A first sum gives a mean that rounding leaves a little off where a row
+// has a large offset; the distances from it, which are exact there, give the
+// rest of the mean (`shift`) and the variance, so an offset costs no digits.  y is the norm of s as it is stored: the
+// gradient, which reads s again, sees the same numbers.  CTAs go over the rows
+// with the weights (and the sums of dw and db) in registers; the CTAs' sums are
+// added in a fixed order by a second launch.  Bound by memory.
+
+#include <algorithm>
+
+#include "row_ops.cuh"
+
+namespace gru {
+namespace {
+
+constexpr int kMaxWidth = 16384;
+constexpr int kNormCtas = 148 * 4;  // most CTAs of the gradient, whose sums the workspace holds
+
+struct Norm {
+  const void *x, *res, *w, *b;
+  void *y, *s;
+  float* stats;  // [3][rows]: the first mean, what it lacks, 1 / deviation
+  // gradient: s is read; x, y, res and b are unused
+  const void *dy, *ds;
+  void *dx, *dres;
+  float* part;  // [CTA][2][D]
+  long R, xs, rs, dys, dss;  // rows, and elements between them
+  int D, wtype;
+  float eps;
+};
+
+// Sums K numbers over the threads of a row.
+template <int K, bool CTA>
+__device__ __forceinline__ void row_sum(float (&v)[K], float* smem) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
+  if constexpr (CTA) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (lane == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) smem[k * 32 + warp] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = warp_sum(lane < warps ? smem[k * 32 + lane] : 0.0f);
+  }
+}
+
+// V elements a load, NV loads a thread; RES: there is a residual (type TR).
+template <typename TX, typename TR, bool RES, int V, int NV, bool CTA>
+__global__ void __launch_bounds__(1024) norm_forward_kernel(const Norm a) {
+  __shared__ float smem[2][64];
+  const int per = CTA ? blockDim.x : 32;
+  const int tid = CTA ? threadIdx.x : threadIdx.x & 31;
+  const long first = CTA ? blockIdx.x : (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const long step = CTA ? gridDim.x : (long)gridDim.x * (blockDim.x >> 5);
+  const float inv = 1.0f / (float)a.D;
+  float w[NV * V], b[NV * V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int c = (i * per + tid) * V + e;
+      w[i * V + e] = c < a.D ? get(a.w, c, a.wtype) : 0.0f;
+      b[i * V + e] = c < a.D && a.b ? get(a.b, c, a.wtype) : 0.0f;
+    }
+  for (long r = first; r < a.R; r += step) {
+    const TX* x = static_cast<const TX*>(a.x) + r * a.xs;
+    const TR* res = static_cast<const TR*>(a.res) + r * a.rs;
+    float v[NV][V], t[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * per + tid) * V;
+      if (c < a.D) {
+        load_row<V>(x + c, v[i]);
+        if (RES) load_row<V>(res + c, t[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[i][e] = t[i][e] = 0.0f;
+      }
+    }
+    float sum[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * per + tid) * V;
+      if (RES) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[i][e] = to_f32(from_f32<TR>(v[i][e] + t[i][e]));
+        if (c < a.D) store_row<V>(static_cast<TR*>(a.s) + r * a.D + c, v[i]);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[0] += v[i][e];
+    }
+    row_sum<1, CTA>(sum, smem[0]);
+    const float mean = sum[0] * inv;
+    float sums[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((i * per + tid) * V < a.D) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          v[i][e] -= mean;
+          sums[0] += v[i][e];
+          sums[1] += v[i][e] * v[i][e];
+        }
+      }
+    row_sum<2, CTA>(sums, smem[1]);
+    const float shift = sums[0] * inv;
+    const float var = sums[1] * inv - shift * shift;  // shift is small beside the deviation, or all but 0
+    const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + a.eps);
+    if (tid == 0 && a.stats) {
+      a.stats[r] = mean;
+      a.stats[a.R + r] = shift;
+      a.stats[2 * a.R + r] = rstd;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * per + tid) * V;
+      if (c >= a.D) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[i][e] = (v[i][e] - shift) * rstd * w[i * V + e] + b[i * V + e];
+      store_row<V>(static_cast<TX*>(a.y) + r * a.D + c, v[i]);
+    }
+  }
+}
+
+// TS: the type of s and ds (the residual's, or x's without one).
+template <typename TX, typename TS, int V, int NV, bool CTA>
+__global__ void __launch_bounds__(512) norm_backward_kernel(const Norm a) {
+  extern __shared__ float dyn[];
+  __shared__ float smem[2][64];
+  const int per = CTA ? blockDim.x : 32;
+  const int tid = CTA ? threadIdx.x : threadIdx.x & 31;
+  const long first = CTA ? blockIdx.x : (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const long step = CTA ? gridDim.x : (long)gridDim.x * (blockDim.x >> 5);
+  const float inv = 1.0f / (float)a.D;
+  float w[NV][V], dw[NV][V], db[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int c = (i * per + tid) * V + e;
+      w[i][e] = c < a.D ? get(a.w, c, a.wtype) : 0.0f;
+      dw[i][e] = db[i][e] = 0.0f;
+    }
+  int turn = 0;
+  for (long r = first; r < a.R; r += step, turn ^= 1) {
+    const TS* s = static_cast<const TS*>(a.s) + r * a.xs;
+    const TX* dy = static_cast<const TX*>(a.dy) + r * a.dys;
+    float n[NV][V], g[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * per + tid) * V;
+      if (c < a.D) {
+        load_row<V>(s + c, n[i]);
+        load_row<V>(dy + c, g[i]);
+      }
+    }
+    const float mean = a.stats[r], shift = a.stats[a.R + r], rstd = a.stats[2 * a.R + r];
+    float sums[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const bool in = (i * per + tid) * V < a.D;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        n[i][e] = in ? (n[i][e] - mean - shift) * rstd : 0.0f;
+        const float d = in ? g[i][e] : 0.0f;
+        db[i][e] += d;
+        dw[i][e] += d * n[i][e];
+        g[i][e] = d * w[i][e];
+        sums[0] += g[i][e];
+        sums[1] += g[i][e] * n[i][e];
+      }
+    }
+    row_sum<2, CTA>(sums, smem[turn]);
+    const float m0 = sums[0] * inv, m1 = sums[1] * inv;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * per + tid) * V;
+      if (c >= a.D) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e) g[i][e] = rstd * (g[i][e] - m0 - n[i][e] * m1);
+      if (a.ds) {
+        float t[V];
+        load_row<V>(static_cast<const TS*>(a.ds) + r * a.dss + c, t);
+#pragma unroll
+        for (int e = 0; e < V; ++e) g[i][e] += t[e];
+      }
+      if (a.dx) store_row<V>(static_cast<TX*>(a.dx) + r * a.D + c, g[i]);
+      if (a.dres) store_row<V>(static_cast<TS*>(a.dres) + r * a.D + c, g[i]);
+    }
+  }
+  float* part = a.part + (long)blockIdx.x * 2 * a.D;
+  if (CTA) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int c = (i * per + tid) * V + e;
+        if (c < a.D) part[c] = dw[i][e], part[a.D + c] = db[i][e];
+      }
+  } else {  // the warps' sums, in their order
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
+    float* mine = dyn + warp * 2 * a.D;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int c = (i * per + tid) * V + e;
+        if (c < a.D) mine[c] = dw[i][e], mine[a.D + c] = db[i][e];
+      }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * a.D; c += blockDim.x) {
+      float t = dyn[c];
+      for (int k = 1; k < warps; ++k) t += dyn[k * 2 * a.D + c];
+      part[c] = t;
+    }
+  }
+}
+
+struct StoreNorm {
+  void *dw, *db;
+  int D, dtype;
+  __device__ __forceinline__ void operator()(long c, float x) const {
+    if (c < D) put(dw, c, dtype, x);
+    else if (db) put(db, c - D, dtype, x);
+  }
+};
+
+// How a row is dealt out.
+struct Shape {
+  int nv, threads, rows;  // loads a thread, threads a CTA, rows a CTA at a time
+  bool cta;
+};
+// v elements a load: warps hold rows of up to 4 loads a lane; CTAs hold longer
+// ones in as many loads a thread as `most` threads need.
+Shape shape_of(int D, int v, int most) {
+  const int loads = ceil_div(D, v);
+  const int warp_loads = v == 1 ? 8 : 4;
+  Shape s;
+  s.cta = loads > 32 * warp_loads;
+  if (!s.cta) {
+    s.nv = 1;
+    while (s.nv * 32 < loads) s.nv *= 2;
+    s.threads = 128, s.rows = 4;
+    return s;
+  }
+  s.nv = v == 1 ? 8 : 1;
+  while (s.nv * 256 < loads && s.nv * v < 8) s.nv *= 2;
+  while (s.nv * most < loads) s.nv *= 2;
+  s.threads = (ceil_div(loads, s.nv) + 31) / 32 * 32, s.rows = 1;
+  return s;
+}
+
+template <typename TX, typename TR, bool RES, int V>
+int launch_forward(const Norm& a, cudaStream_t stream) {
+  const Shape s = shape_of(a.D, V, 1024);
+  const long need = (a.R + s.rows - 1) / s.rows;
+  const unsigned ctas = (unsigned)std::min<long>(need, (long)sms_here() * std::max(1, 2048 / s.threads));
+  LaunchScope scope(kKindLayerNorm, stream);
+#define GRU_NORM(NV, CTA)                                                                    \
+  if (s.nv == NV && s.cta == CTA) {                                                          \
+    norm_forward_kernel<TX, TR, RES, V, NV, CTA><<<ctas, s.threads, 0, stream>>>(a);         \
+    GRU_CUDA_TRY(cudaGetLastError());                                                        \
+    return GRU_OK;                                                                           \
+  }
+  GRU_NORM(1, false)
+  GRU_NORM(2, false)
+  GRU_NORM(4, false)
+  if constexpr (V == 1) {
+    GRU_NORM(8, false)
+    GRU_NORM(8, true)
+    GRU_NORM(16, true)
+  } else {
+    GRU_NORM(1, true)
+    GRU_NORM(2, true)
+    GRU_NORM(4, true)
+  }
+#undef GRU_NORM
+  return refuse("gru_layer_norm_forward", "no kernel for this width", GRU_ERR_UNSUPPORTED);
+}
+
+template <typename TX, typename TS, int V>
+int launch_backward(const Norm& a, const StoreNorm& store, cudaStream_t stream) {
+  const Shape s = shape_of(a.D, V, 512);
+  const long need = (a.R + s.rows - 1) / s.rows;
+  const long fit = std::min<long>(kNormCtas, (long)sms_here() * std::max(1, 1024 / s.threads));
+  const unsigned ctas = (unsigned)std::min(need, fit);
+  const size_t smem = s.cta ? 0 : sizeof(float) * 4 * 2 * a.D;
+  LaunchScope scope(kKindLayerNorm, stream, 2);
+#define GRU_NORM(NV, CTA)                                                                    \
+  if (s.nv == NV && s.cta == CTA) {                                                          \
+    norm_backward_kernel<TX, TS, V, NV, CTA><<<ctas, s.threads, smem, stream>>>(a);          \
+    GRU_CUDA_TRY(cudaGetLastError());                                                        \
+    return sum_parts(a.part, (int)ctas, 2L * a.D, 2L * a.D, store, stream);                  \
+  }
+  GRU_NORM(1, false)
+  GRU_NORM(2, false)
+  GRU_NORM(4, false)
+  if constexpr (V == 1) {
+    GRU_NORM(8, false)
+    GRU_NORM(8, true)
+    GRU_NORM(16, true)
+    GRU_NORM(32, true)
+  } else {
+    GRU_NORM(1, true)
+    GRU_NORM(2, true)
+    GRU_NORM(4, true)
+    if constexpr (V == 4) {
+      GRU_NORM(8, true)
+    }
+  }
+#undef GRU_NORM
+  return refuse("gru_layer_norm_backward", "no kernel for this width", GRU_ERR_UNSUPPORTED);
+}
+
+int check(const char* me, const gru_norm_args* p) {
+  if (!p) return refuse(me, "null arguments");
+  if (!known(p->dtype) || !known(p->residual_dtype) || !known(p->weight_dtype))
+    return refuse(me, "types must be GRU_F32 or GRU_BF16", GRU_ERR_UNSUPPORTED);
+  if ((p->residual_dtype != p->dtype && p->residual_dtype != GRU_F32) ||
+      (p->weight_dtype != p->dtype && p->weight_dtype != GRU_F32))
+    return refuse(me, "the residual and the weights must be FP32 or of x's type", GRU_ERR_UNSUPPORTED);
+  if (p->rows < 0 || p->width < 1) return refuse(me, "need rows >= 0 and width >= 1");
+  if (p->width > kMaxWidth) return refuse(me, "the width must be in [1, 16384]", GRU_ERR_UNSUPPORTED);
+  if (!(p->eps >= 0.0f)) return refuse(me, "eps must not be negative");
+  return GRU_OK;
+}
+
+bool misaligned(const void* p, int dtype) { return bits(p) & (elem_size(dtype) - 1); }
+
+}  // namespace
+}  // namespace gru
+
+using namespace gru;
+
+extern "C" size_t gru_layer_norm_workspace_bytes(const gru_norm_args* p) {
+  if (check("gru_layer_norm_workspace_bytes", p)) return 0;
+  return align_up(sizeof(float) * 2 * (size_t)p->width * (size_t)std::min<long>(kNormCtas, std::max(1L, p->rows)), 256);
+}
+
+extern "C" int gru_layer_norm_forward(const gru_norm_args* p, const void* x, const void* residual, const void* weight,
+                                      const void* bias, void* out, void* sum, float* stats, void* stream_) {
+  clear_error();
+  const char* me = "gru_layer_norm_forward";
+  if (const int rc = check(me, p)) return rc;
+  if (p->rows == 0) return GRU_OK;
+  if (!x || !weight || !out || (residual != nullptr) != (sum != nullptr))
+    return refuse(me, "null tensor, or a sum without a residual");
+  if (misaligned(x, p->dtype) || misaligned(out, p->dtype) || misaligned(residual, p->residual_dtype) ||
+      misaligned(sum, p->residual_dtype) || misaligned(weight, p->weight_dtype) || misaligned(bias, p->weight_dtype) ||
+      (bits(stats) & 3))
+    return refuse(me, "a tensor is not aligned to its element size");
+  Norm a{};
+  a.x = x, a.res = residual, a.w = weight, a.b = bias, a.y = out, a.s = sum, a.stats = stats;
+  a.R = p->rows, a.xs = p->row_stride, a.rs = p->residual_row_stride;
+  a.D = p->width, a.wtype = p->weight_dtype, a.eps = p->eps;
+  const int v = p->dtype == GRU_F32 ? 4 : 8;
+  const bool vec = a.D % v == 0 && a.xs % v == 0 && (!residual || a.rs % v == 0) &&
+                   ((bits(x) | bits(residual) | bits(out) | bits(sum)) & 15) == 0;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (p->dtype == GRU_F32) {
+    if (residual) return vec ? launch_forward<float, float, true, 4>(a, stream) : launch_forward<float, float, true, 1>(a, stream);
+    return vec ? launch_forward<float, float, false, 4>(a, stream) : launch_forward<float, float, false, 1>(a, stream);
+  }
+  if (!residual) return vec ? launch_forward<bf16, bf16, false, 8>(a, stream) : launch_forward<bf16, bf16, false, 1>(a, stream);
+  if (p->residual_dtype == GRU_F32)
+    return vec ? launch_forward<bf16, float, true, 8>(a, stream) : launch_forward<bf16, float, true, 1>(a, stream);
+  return vec ? launch_forward<bf16, bf16, true, 8>(a, stream) : launch_forward<bf16, bf16, true, 1>(a, stream);
+}
+
+extern "C" int gru_layer_norm_backward(const gru_norm_args* p, const void* sum, const void* weight, const float* stats,
+                                       const void* dout, const void* dsum, void* dx, void* dresidual,
+                                       void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream_) {
+  clear_error();
+  const char* me = "gru_layer_norm_backward";
+  if (const int rc = check(me, p)) return rc;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (!dweight || misaligned(dweight, p->weight_dtype) || misaligned(dbias, p->weight_dtype))
+    return refuse(me, "null or misaligned gradient of the weight");
+  if (p->rows == 0) {
+    const size_t n = elem_size(p->weight_dtype) * p->width;
+    GRU_CUDA_TRY(cudaMemsetAsync(dweight, 0, n, stream));
+    if (dbias) GRU_CUDA_TRY(cudaMemsetAsync(dbias, 0, n, stream));
+    return GRU_OK;
+  }
+  const int st = p->residual_dtype;  // s's type; x's without a residual
+  if (!sum || !weight || !stats || !dout) return refuse(me, "null tensor");
+  if (misaligned(sum, st) || misaligned(dsum, st) || misaligned(dresidual, st) || misaligned(dout, p->dtype) ||
+      misaligned(dx, p->dtype) || misaligned(weight, p->weight_dtype) || (bits(stats) & 3))
+    return refuse(me, "a tensor is not aligned to its element size");
+  if (!workspace || (bits(workspace) & 15) || workspace_bytes < gru_layer_norm_workspace_bytes(p))
+    return refuse(me, "workspace too small or not 16-byte aligned");
+  Norm a{};
+  a.s = const_cast<void*>(sum), a.w = weight, a.stats = const_cast<float*>(stats);
+  a.dy = dout, a.ds = dsum, a.dx = dx, a.dres = dresidual, a.part = static_cast<float*>(workspace);
+  a.R = p->rows, a.xs = p->row_stride, a.dys = a.dss = p->width;
+  a.D = p->width, a.wtype = p->weight_dtype, a.eps = p->eps;
+  const int v = p->dtype == GRU_F32 ? 4 : 8;
+  const bool vec = a.D % v == 0 && a.xs % v == 0 &&
+                   ((bits(sum) | bits(dout) | bits(dsum) | bits(dx) | bits(dresidual)) & 15) == 0;
+  const StoreNorm store{dweight, dbias, a.D, p->weight_dtype};
+  if (p->dtype == GRU_F32)
+    return vec ? launch_backward<float, float, 4>(a, store, stream) : launch_backward<float, float, 1>(a, store, stream);
+  if (st == GRU_F32)
+    return vec ? launch_backward<bf16, float, 8>(a, store, stream) : launch_backward<bf16, float, 1>(a, store, stream);
+  return vec ? launch_backward<bf16, bf16, 8>(a, store, stream) : launch_backward<bf16, bf16, 1>(a, store, stream);
+}

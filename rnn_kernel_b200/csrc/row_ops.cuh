@@ -1,0 +1,175 @@
+// What the selective scan, the causal convolution and the layer norm share:
+// loads and stores of FP32 or bf16 rows as FP32, the sigmoid, and the sum of
+// partial results in a fixed order.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include <string>
+
+#include "common.cuh"
+#include "../../include/rnn_kernel_b200.h"
+
+namespace gru {
+
+typedef __nv_bfloat16 bf16;
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(bf16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ bf16 from_f32<bf16>(float x) { return __float2bfloat16_rn(x); }
+
+// N consecutive elements, aligned to min(16, N * sizeof(T)) bytes.
+template <int N>
+__device__ __forceinline__ void load_row(const float* p, float (&v)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 r = *reinterpret_cast<const float4*>(p + i);
+      v[i] = r.x, v[i + 1] = r.y, v[i + 2] = r.z, v[i + 3] = r.w;
+    }
+  } else if constexpr (N == 2) {
+    const float2 r = *reinterpret_cast<const float2*>(p);
+    v[0] = r.x, v[1] = r.y;
+  } else {
+    static_assert(N == 1, "1, 2 or a multiple of 4");
+    v[0] = *p;
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_row(const bf16* p, float (&v)[N]) {
+  auto two = [&](int i, unsigned r) {
+    v[i] = __uint_as_float(r << 16);
+    v[i + 1] = __uint_as_float(r & 0xffff0000u);
+  };
+  if constexpr (N % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 8) {
+      const uint4 r = *reinterpret_cast<const uint4*>(p + i);
+      two(i, r.x), two(i + 2, r.y), two(i + 4, r.z), two(i + 6, r.w);
+    }
+  } else if constexpr (N == 4) {
+    const uint2 r = *reinterpret_cast<const uint2*>(p);
+    two(0, r.x), two(2, r.y);
+  } else if constexpr (N == 2) {
+    two(0, *reinterpret_cast<const unsigned*>(p));
+  } else {
+    static_assert(N == 1, "1, 2, 4 or a multiple of 8");
+    v[0] = __bfloat162float(*p);
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_row(float* p, const float (&v)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+  } else if constexpr (N == 2) {
+    *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+  } else {
+    static_assert(N == 1, "1, 2 or a multiple of 4");
+    *p = v[0];
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_row(bf16* p, const float (&v)[N]) {
+  auto two = [&](int i) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(v[i], v[i + 1]);
+    return *reinterpret_cast<const unsigned*>(&r);
+  };
+  if constexpr (N % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 8)
+      *reinterpret_cast<uint4*>(p + i) = make_uint4(two(i), two(i + 2), two(i + 4), two(i + 6));
+  } else if constexpr (N == 4) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(two(0), two(2));
+  } else if constexpr (N == 2) {
+    *reinterpret_cast<unsigned*>(p) = two(0);
+  } else {
+    static_assert(N == 1, "1, 2, 4 or a multiple of 8");
+    *p = __float2bfloat16_rn(v[0]);
+  }
+}
+
+// 1 / (1 + e^-x) by the hardware's exponential and quotient: within 2^-21 of
+// itself for |x| < 16, 0 below -88.
+__device__ __forceinline__ float sigmoid_of(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+// store(c, sum over p of part[p * stride + c]) for c < cols: FP64 sums in a
+// fixed order, so results do not change from run to run.
+constexpr int kSumRows = 8;
+template <typename Store>
+__global__ void __launch_bounds__(32 * kSumRows) sum_parts_kernel(const float* __restrict__ part, int parts, long stride,
+                                                                  long cols, Store store) {
+  __shared__ double s[kSumRows][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const long c = blockIdx.x * 32L + tx;
+  double acc = 0.0;
+  if (c < cols)
+#pragma unroll 4
+    for (int p = ty; p < parts; p += kSumRows) acc += (double)part[p * stride + c];
+  s[ty][tx] = acc;
+  __syncthreads();
+  if (ty == 0 && c < cols) {
+#pragma unroll
+    for (int r = 1; r < kSumRows; ++r) acc += s[r][tx];
+    store(c, (float)acc);
+  }
+}
+template <typename Store>
+int sum_parts(const float* part, int parts, long stride, long cols, Store store, cudaStream_t stream) {
+  sum_parts_kernel<<<(unsigned)((cols + 31) / 32), 32 * kSumRows, 0, stream>>>(part, parts, stride, cols, store);
+  GRU_CUDA_TRY(cudaGetLastError());
+  return GRU_OK;
+}
+
+// Writes x to FP32 or bf16 memory.
+__device__ __forceinline__ void put(void* p, long i, int dtype, float x) {
+  if (dtype == GRU_F32) static_cast<float*>(p)[i] = x;
+  else static_cast<bf16*>(p)[i] = __float2bfloat16_rn(x);
+}
+__device__ __forceinline__ float get(const void* p, long i, int dtype) {
+  return dtype == GRU_F32 ? static_cast<const float*>(p)[i] : __bfloat162float(static_cast<const bf16*>(p)[i]);
+}
+
+inline int refuse(const char* what, const char* msg, int code = GRU_ERR_INVALID) {
+  set_error(std::string(what) + ": " + msg);
+  return code;
+}
+inline uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+inline uintptr_t elem_size(int dtype) { return dtype == GRU_F32 ? 4 : 2; }
+inline bool known(int dtype) { return dtype == GRU_F32 || dtype == GRU_BF16; }
+
+// Hands out 256-byte aligned pieces of a buffer; with a null base it only
+// counts.
+struct Pieces {
+  char* base;
+  size_t used = 0;
+  float* floats(size_t n) {
+    float* p = base ? reinterpret_cast<float*>(base + used) : nullptr;
+    used += align_up(n * sizeof(float), 256);
+    return p;
+  }
+};
+
+// The SMs of the current device (148 where they cannot be read).
+inline int sms_here() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 148;
+  }
+  const int n = sm_count(dev);
+  return n > 0 ? n : 148;
+}
+
+}  // namespace gru

@@ -1,0 +1,13 @@
+// Launches of the selective scan's forward and gradient.
+#pragma once
+
+#include "scan_common.cuh"
+
+namespace gru {
+namespace scan {
+
+int forward(const Problem& p, int dtype, cudaStream_t stream);
+int backward(const Problem& p, int dtype, cudaStream_t stream);
+
+}  // namespace scan
+}  // namespace gru

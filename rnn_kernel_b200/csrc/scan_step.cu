@@ -1,0 +1,255 @@
+// The selective scan's single token (serving) and the C entry points of the whole
+// operator (contract in include/rnn_kernel_b200.h).
+//
+// One token reads a state [D, N] and writes it back.  A thread has four states
+// of a channel in registers from read to write, the lanes of a channel lie side
+// by side, and their sums of C h meet by shuffles.  HBM-bound: 8 N bytes a
+// channel, loaded and stored as used once.
+
+#include <algorithm>
+
+#include "scan_common.cuh"
+#include "scan_launch.cuh"
+
+namespace gru {
+namespace scan {
+namespace {
+
+constexpr int kStepThreads = 256;
+
+// LP: lanes of a channel; K: channels a thread takes one after another, whose
+// loads are in flight together.  vec: states lie in aligned fours.
+template <typename T, int LP, int K>
+__global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const Problem p, float* state, int vec, int blocks) {
+  constexpr int kSlots = kStepThreads / LP;
+  const int b = blockIdx.x / blocks, part = threadIdx.x % LP, slot = threadIdx.x / LP;
+  const int d0 = (blockIdx.x - b * blocks) * (kSlots * K) + slot;
+  const int n0 = 4 * part, left = p.N - n0;
+  float h[K][4], a[K][4];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int d = d0 + k * kSlots;
+    const float* s = state + ((long)b * p.D + d) * p.N + n0;
+    const float* r = p.a + (long)d * p.N + n0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[k][j] = a[k][j] = 0.0f;
+    if (d >= p.D) continue;
+    if (vec) {
+      if (left > 0) {
+        const float4 v = __ldcs(reinterpret_cast<const float4*>(s));
+        const float4 u = __ldg(reinterpret_cast<const float4*>(r));
+        h[k][0] = v.x, h[k][1] = v.y, h[k][2] = v.z, h[k][3] = v.w;
+        a[k][0] = u.x, a[k][1] = u.y, a[k][2] = u.z, a[k][3] = u.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < left) h[k][j] = s[j], a[k][j] = r[j];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int d = d0 + k * kSlots;
+    const bool in = d < p.D;
+    const int group = in ? d / p.R : 0;
+    const long db = in ? d : 0;
+    const float x = to_f32(static_cast<const T*>(p.x)[b * p.xs[0] + db]);
+    const float step = step_of(p, to_f32(static_cast<const T*>(p.dt)[b * p.dts[0] + db]), p.bias ? p.bias[db] : 0.0f);
+    const T* bm = static_cast<const T*>(p.b) + b * p.bs[0] + group * p.bs[2] + n0;
+    const T* cm = static_cast<const T*>(p.c) + b * p.cs[0] + group * p.cs[2] + n0;
+    float y = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float bv = j < left ? to_f32(bm[j]) : 0.0f, cv = j < left ? to_f32(cm[j]) : 0.0f;
+      h[k][j] = fmaf(exp2_of(step * decay_rate(a[k][j])), h[k][j], step * x * bv);
+      y = fmaf(cv, h[k][j], y);
+    }
+#pragma unroll
+    for (int o = LP / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    if (!in) continue;
+    float* s = state + ((long)b * p.D + d) * p.N + n0;
+    if (vec) {
+      if (left > 0) __stcs(reinterpret_cast<float4*>(s), make_float4(h[k][0], h[k][1], h[k][2], h[k][3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < left) s[j] = h[k][j];
+    }
+    if (part == 0) {
+      if (p.skip) y = fmaf(p.skip[d], x, y);
+      if (p.z) {
+        const float gate = to_f32(static_cast<const T*>(p.z)[b * p.zs[0] + d]);
+        y *= gate * sigmoid_of(gate);
+      }
+      static_cast<T*>(p.out)[(long)b * p.D + d] = from_f32<T>(y);
+    }
+  }
+}
+
+template <typename T, int LP, int K>
+int launch_step(const Problem& p, float* state, int vec, cudaStream_t stream) {
+  const int blocks = ceil_div(p.D, kStepThreads / LP * K);
+  LaunchScope scope(kKindSelectiveScan, stream);
+  scan_step_kernel<T, LP, K><<<(unsigned)((long)p.B * blocks), kStepThreads, 0, stream>>>(p, state, vec, blocks);
+  GRU_CUDA_TRY(cudaGetLastError());
+  return GRU_OK;
+}
+
+// Four channels a thread where that still gives every SM four CTAs.
+template <typename T>
+int step(const Problem& p, float* state, int vec, cudaStream_t stream) {
+  int lp = 1;
+  while (lp < p.ng) lp *= 2;
+  const bool four = (long)p.B * p.D * lp / (kStepThreads * 4) >= 4L * 148;
+#define GRU_STEP(LP) \
+  if (lp == LP) return four ? launch_step<T, LP, 4>(p, state, vec, stream) : launch_step<T, LP, 1>(p, state, vec, stream);
+  GRU_STEP(1)
+  GRU_STEP(2)
+  GRU_STEP(4)
+  GRU_STEP(8)
+  GRU_STEP(16)
+#undef GRU_STEP
+  return GRU_ERR_UNSUPPORTED;
+}
+
+enum Needs { kSizesOnly, kInputs };
+int check(const char* me, const gru_scan_args* p, Needs needs) {
+  if (!p) return refuse(me, "null arguments");
+  if (!known(p->dtype)) return refuse(me, "dtype must be GRU_F32 or GRU_BF16", GRU_ERR_UNSUPPORTED);
+  if (p->B < 0 || p->T < 0 || p->D < 1 || p->G < 1 || p->D % p->G != 0)
+    return refuse(me, "need B >= 0, T >= 0, and channels a multiple of the groups");
+  if (p->N < 1 || p->N > kMaxStates) return refuse(me, "the states must be in [1, 64]", GRU_ERR_UNSUPPORTED);
+  if (p->dt_softplus != 0 && p->dt_softplus != 1) return refuse(me, "dt_softplus must be 0 or 1");
+  const uintptr_t es = elem_size(p->dtype);
+  if ((bits(p->x) | bits(p->dt) | bits(p->b) | bits(p->c) | bits(p->z)) & (es - 1) ||
+      (bits(p->a) | bits(p->skip) | bits(p->dt_bias) | bits(p->initial_state)) & 3)
+    return refuse(me, "a tensor is not aligned to its element size");
+  if (needs == kInputs && p->B > 0 && p->T > 0 && (!p->x || !p->dt || !p->b || !p->c || !p->a)) return refuse(me, "null tensor");
+  const double tiles = (double)p->G * ((p->D / p->G + kLanes - 1) / kLanes);
+  if (p->B * tiles > 2e9 || (double)p->B * p->D * 16 > 4e11 || (double)p->B * p->T * p->G > 4e9 || p->T > (1 << 30) ||
+      p->D > (1 << 26))
+    return refuse(me, "too large for one launch", GRU_ERR_UNSUPPORTED);
+  return GRU_OK;
+}
+
+void fill(Problem& a, const gru_scan_args& p) {
+  a.x = p.x, a.dt = p.dt, a.b = p.b, a.c = p.c, a.z = p.z;
+  a.a = p.a, a.skip = p.skip, a.bias = p.dt_bias, a.s0 = p.initial_state;
+  for (int i = 0; i < 2; ++i) a.xs[i] = p.x_stride[i], a.dts[i] = p.dt_stride[i], a.zs[i] = p.z_stride[i];
+  for (int i = 0; i < 3; ++i) a.bs[i] = p.b_stride[i], a.cs[i] = p.c_stride[i];
+  a.B = p.B, a.T = p.T, a.D = p.D, a.N = p.N, a.G = p.G, a.R = p.D / p.G;
+  a.softplus = p.dt_softplus;
+  a.per_group = ceil_div(a.R, kLanes), a.tiles = a.per_group * a.G;
+  a.ng = ceil_div(a.N, kGroup);
+  a.nmarks = ceil_div(a.T, kMark);
+}
+
+void lay_marks(Problem& a, Pieces& m) { a.marks = m.floats((size_t)a.B * a.tiles * a.nmarks * a.ng * 4 * kLanes); }
+void lay_parts(Problem& a, Pieces& m) {
+  a.part_bc = m.floats((size_t)a.B * a.tiles * a.T * 2 * a.ng * 4);
+  a.part_a = m.floats((size_t)a.B * a.D * a.N);
+  a.part_ch = m.floats((size_t)a.B * 2 * a.D);
+}
+
+}  // namespace
+}  // namespace scan
+}  // namespace gru
+
+using namespace gru;
+using namespace gru::scan;
+
+extern "C" size_t gru_scan_stash_bytes(const gru_scan_args* p) {
+  if (check("gru_scan_stash_bytes", p, kSizesOnly)) return 0;
+  Problem a{};
+  fill(a, *p);
+  Pieces m{nullptr};
+  lay_marks(a, m);
+  return m.used;
+}
+
+extern "C" size_t gru_scan_workspace_bytes(const gru_scan_args* p) {
+  if (check("gru_scan_workspace_bytes", p, kSizesOnly)) return 0;
+  Problem a{};
+  fill(a, *p);
+  Pieces m{nullptr};
+  lay_parts(a, m);
+  return m.used;
+}
+
+extern "C" int gru_scan_forward(const gru_scan_args* p, void* out, float* final_state, void* stash, size_t stash_bytes,
+                                void* stream_) {
+  clear_error();
+  const char* me = "gru_scan_forward";
+  if (const int rc = check(me, p, kInputs)) return rc;
+  if (p->B == 0) return GRU_OK;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (!final_state || bits(final_state) & 3) return refuse(me, "null or misaligned final_state");
+  Problem a{};
+  fill(a, *p);
+  if (p->T == 0) {
+    const size_t n = sizeof(float) * (size_t)p->B * p->D * p->N;
+    if (!p->initial_state) GRU_CUDA_TRY(cudaMemsetAsync(final_state, 0, n, stream));
+    else if (p->initial_state != final_state)
+      GRU_CUDA_TRY(cudaMemcpyAsync(final_state, p->initial_state, n, cudaMemcpyDeviceToDevice, stream));
+    return GRU_OK;
+  }
+  if (!out || bits(out) & (elem_size(p->dtype) - 1)) return refuse(me, "null or misaligned out");
+  if (stash) {
+    Pieces m{static_cast<char*>(stash)};
+    lay_marks(a, m);
+    if (stash_bytes < m.used || bits(stash) & 15) return refuse(me, "stash too small or not 16-byte aligned");
+  }
+  a.out = out, a.last = final_state;
+  return forward(a, p->dtype, stream);
+}
+
+extern "C" int gru_scan_backward(const gru_scan_args* p, const void* dout, const float* dfinal, const void* stash,
+                                 size_t stash_bytes, void* dx, void* ddt, float* da, void* db, void* dc, float* dskip,
+                                 void* dz, float* ddt_bias, float* dinitial, void* workspace, size_t workspace_bytes,
+                                 void* stream_) {
+  clear_error();
+  const char* me = "gru_scan_backward";
+  if (const int rc = check(me, p, kInputs)) return rc;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  const uintptr_t es = elem_size(p->dtype);
+  if (!da || (bits(da) | bits(dskip) | bits(ddt_bias) | bits(dinitial) | bits(dfinal)) & 3 ||
+      (bits(dx) | bits(ddt) | bits(db) | bits(dc) | bits(dz) | bits(dout)) & (es - 1))
+    return refuse(me, "null or misaligned gradient");
+  Problem a{};
+  fill(a, *p);
+  if (p->B == 0 || p->T == 0) {
+    const size_t n = sizeof(float) * (size_t)p->B * p->D * p->N, wide = sizeof(float) * (size_t)p->D;
+    GRU_CUDA_TRY(cudaMemsetAsync(da, 0, wide * p->N, stream));
+    if (dskip) GRU_CUDA_TRY(cudaMemsetAsync(dskip, 0, wide, stream));
+    if (ddt_bias) GRU_CUDA_TRY(cudaMemsetAsync(ddt_bias, 0, wide, stream));
+    if (n && dinitial && !dfinal) GRU_CUDA_TRY(cudaMemsetAsync(dinitial, 0, n, stream));
+    else if (n && dinitial && dfinal != dinitial)
+      GRU_CUDA_TRY(cudaMemcpyAsync(dinitial, dfinal, n, cudaMemcpyDeviceToDevice, stream));
+    return GRU_OK;
+  }
+  if (!dx || !ddt || !db || !dc || (p->z && !dz)) return refuse(me, "null gradient");
+  Pieces m{static_cast<char*>(const_cast<void*>(stash))}, w{static_cast<char*>(workspace)};
+  lay_marks(a, m);
+  lay_parts(a, w);
+  if (!stash || stash_bytes < m.used || !workspace || workspace_bytes < w.used || (bits(stash) | bits(workspace)) & 15)
+    return refuse(me, "stash or workspace too small or not 16-byte aligned");
+  a.dout = dout, a.dlast = dfinal;
+  a.dx = dx, a.ddt = ddt, a.da = da, a.db = db, a.dc = dc, a.dskip = dskip, a.dz = dz, a.dbias = ddt_bias, a.ds0 = dinitial;
+  return backward(a, p->dtype, stream);
+}
+
+extern "C" int gru_scan_step(const gru_scan_args* p, float* state, void* out, void* stream_) {
+  clear_error();
+  const char* me = "gru_scan_step";
+  if (const int rc = check(me, p, kInputs)) return rc;
+  if (p->T != 1) return refuse(me, "T must be 1");
+  if (p->B == 0) return GRU_OK;
+  if (!state || !out || bits(state) & 3 || bits(out) & (elem_size(p->dtype) - 1))
+    return refuse(me, "null or misaligned state or out");
+  Problem a{};
+  fill(a, *p);
+  a.out = out;
+  const int vec = p->N % 4 == 0 && ((bits(state) | bits(p->a)) & 15) == 0;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  return p->dtype == GRU_F32 ? step<float>(a, state, vec, stream) : step<bf16>(a, state, vec, stream);
+}
