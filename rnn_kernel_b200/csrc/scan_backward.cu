@@ -9,16 +9,17 @@
 //   ddt_t = x_t sum_n B_t dh_t + sum_n A w_t,   w_t = dh_t a_t h_{t-1};   dA = sum_t dt_t w_t
 //
 // The forward's shape, backwards: a CTA owns 32 channels of one sequence, a lane
-// each, and goes over blocks of 64 tokens from the last to the first, 8 tokens a
-// warp.  The forward kept the state before each block.  For four states at a time a
+// each, and goes over blocks of 32 tokens from the last to the first, 8 tokens a
+// warp.  The forward kept the state before each block.  For two states at a time a
 // warp computes its tokens' decays once and from them its tokens' effect on the
 // state (P h + S) and on what is handed back (P r + R); both meet the other
 // warps' in shared memory, and the warp goes over its tokens forwards for h and
 // backwards for the gradients.  Sums over channels are butterflies over the
-// lanes in which each round halves the values, so that 64 values take 62
-// exchanges; the tiles' sums of dB and dC are added by a second launch, in a
-// fixed order, as are those over sequences of dA, dskip and dbias.
-// Bound by instructions.
+// lanes in which each round halves the values: 32 values (8 tokens, 2 states, dB
+// and dC) take 31 exchanges and leave a lane one sum.  The tiles' sums of dB and
+// dC are added by a second launch, in a fixed order, as are those over sequences
+// of dA, dskip and dbias.  Clusters share a sequence's blocks as in the forward.
+// Bound by instructions: some 22 per token, channel and state.
 
 #include <algorithm>
 
@@ -27,28 +28,39 @@
 
 namespace gru {
 namespace scan {
+
+__device__ int g_backward_status = 0;
+
 namespace {
 
-constexpr int kTok = 8;  // tokens of a warp
-constexpr int kWarps = kMark / kTok;
+constexpr int kTok = 8;            // tokens of a warp
+constexpr int kRow = kTok + 4;     // floats between two states' tokens in shared memory
+constexpr int kBlock = kWarps * kTok;
+constexpr int kResident = 4;       // CTAs an SM holds, by registers
+static_assert(kBlock == kMark, "the forward keeps the state before each block");
 
 // Shared memory in floats.
 struct Lay {
-  int bs, cs, ex, carry, rate, da, sums, total;
+  int bars, bs, cs, ex, carry, rate, da, rows, sums, total;
 };
 __host__ __device__ inline Lay layout(int ng) {
   Lay l;
   int n = 0;
-  l.bs = n, n += kMark * ng * 4;
-  l.cs = n, n += kMark * ng * 4;
-  l.ex = n, n += 2 * kWarps * 3 * kLanes * 4;
-  l.carry = n, n += 2 * ng * kLanes * 4;
-  l.rate = n, n += ng * kLanes * 4;
-  l.da = n, n += kWarps * ng * kLanes * 4;
+  l.bars = n, n += 2 * ng * 2;
+  n = (n + 3) / 4 * 4;
+  l.bs = n, n += kWarps * ng * 2 * kRow;
+  l.cs = n, n += kWarps * ng * 2 * kRow;
+  l.ex = n, n += 2 * kWarps * 3 * kLanes * 2;
+  l.carry = n, n += 2 * ng * kLanes * 2;
+  l.rate = n, n += ng * kLanes * 2;
+  l.da = n, n += kWarps * ng * kLanes * 2;
+  l.rows = n, n += kWarps * kTok * ng * 4;
   l.sums = n, n += 2 * kWarps * kLanes;
   l.total = n;
   return l;
 }
+
+__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
 
 // One round of the butterfly: lanes with `bit` keep the upper half of 2 M values
 // and hand over the lower, the others the other way around.
@@ -61,37 +73,51 @@ __device__ __forceinline__ void halve(float* v, int bit, bool upper) {
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(32 * kWarps, 1) scan_backward_kernel(const Problem p) {
+// Q: several CTAs share a tile, as a cluster.
+template <typename T, bool Q>
+__global__ void __launch_bounds__(32 * kWarps, kResident) scan_backward_kernel(const __grid_constant__ Problem p) {
   extern __shared__ __align__(16) float sm[];
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Lay l = layout(p.ng);
-  const int tile = blockIdx.x % p.tiles, b = blockIdx.x / p.tiles;
+  const int rank = Q ? (int)cluster_rank() : 0, peers = Q ? (int)cluster_size() : 1;
+  const int unit = blockIdx.x / peers, tile = unit % p.tiles, b = unit / p.tiles;
   const int group = tile / p.per_group, local = (tile - group * p.per_group) * kLanes + lane;
   const bool live = local < p.R;
   const int d = group * p.R + (live ? local : 0);
-  const int np = p.ng * 4;
-  float* bs = sm + l.bs + w * kTok * np;
-  float* cs = sm + l.cs + w * kTok * np;
-  float4* ex = reinterpret_cast<float4*>(sm + l.ex);
-  float4* carry = reinterpret_cast<float4*>(sm + l.carry);
-  float4* rate = reinterpret_cast<float4*>(sm + l.rate);
-  float4* das = reinterpret_cast<float4*>(sm + l.da) + w * p.ng * kLanes + lane;
+  float* bs = sm + l.bs + w * p.ng * 2 * kRow;
+  float* cs = sm + l.cs + w * p.ng * 2 * kRow;
+  float* rows = sm + l.rows + w * kTok * p.ng * 4;  // [token][dB, dC][state]
+  float2* ex = reinterpret_cast<float2*>(sm + l.ex) + lane;
+  float2* carry = reinterpret_cast<float2*>(sm + l.carry) + lane;
+  float2* rate = reinterpret_cast<float2*>(sm + l.rate) + lane;
+  float2* das = reinterpret_cast<float2*>(sm + l.da) + w * p.ng * kLanes + lane;
+  const uint32_t bars = smem_at(sm + l.bars);
 
   const float bias = p.bias ? p.bias[d] : 0.0f, skip = p.skip ? p.skip[d] : 0.0f;
-  const int blocks = ceil_div(p.T, kMark);
+  const int blocks = (p.T + kBlock - 1) / kBlock;
   for (int g = w; g < p.ng; g += kWarps) {
-    float r[4], s[4];
+    float r[2], s[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = 4 * g + j;
+    for (int j = 0; j < 2; ++j) {
+      const int n = 2 * g + j;
       r[j] = live && n < p.N ? decay_rate(p.a[(long)d * p.N + n]) : 0.0f;
       s[j] = live && n < p.N && p.dlast ? p.dlast[((long)b * p.D + d) * p.N + n] : 0.0f;
     }
-    rate[g * kLanes + lane] = make_float4(r[0], r[1], r[2], r[3]);
-    carry[g * kLanes + lane] = make_float4(s[0], s[1], s[2], s[3]);
+    rate[g * kLanes] = make_float2(r[0], r[1]);
+    if (rank == 0) carry[g * kLanes] = make_float2(s[0], s[1]);
   }
-  for (int g = 0; g < p.ng; ++g) das[g * kLanes] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int g = 0; g < p.ng; ++g) das[g * kLanes] = twice(0.0f);
+  if (Q) {  // the barrier of slot k & 1 counts the bytes of what is handed back to this CTA's k-th block
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < 2 * p.ng; ++i) bar_init(bars + 8 * i);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      for (int i = 0; i < 2 * p.ng; ++i)
+        if (rank == 0 && i < p.ng) bar_arrive(bars + 8 * i);  // the last state's gradient is there
+        else bar_expect(bars + 8 * i, kLanes * 8);
+    }
+    __syncthreads();
+    cluster_sync();
+  }
   const T* x = static_cast<const T*>(p.x) + b * p.xs[0] + d;
   const T* dt = static_cast<const T*>(p.dt) + b * p.dts[0] + d;
   const T* z = p.z ? static_cast<const T*>(p.z) + b * p.zs[0] + d : nullptr;
@@ -100,190 +126,241 @@ __global__ void __launch_bounds__(32 * kWarps, 1) scan_backward_kernel(const Pro
   const long dense = (long)b * p.T * p.D + d;
   const T* dout = p.dout ? static_cast<const T*>(p.dout) + dense : nullptr;
   float dskip = 0.0f, dbias = 0.0f;
-  __syncthreads();
+  if (!Q) __syncthreads();
 
   int turn = 0;
-  for (int i = blocks - 1; i >= 0; --i) {
-    const int t0 = i * kMark + w * kTok, here = min(max(p.T - t0, 0), kTok);
-    float step[kTok], xv[kTok], gy[kTok], sdt = 0.0f;
+  bool ok = true;
+  for (int step_i = rank, k = 0; step_i < blocks; step_i += peers, ++k) {
+    const int i = blocks - 1 - step_i;
+    const int t0 = i * kBlock + w * kTok, here = min(max(p.T - t0, 0), kTok);
+    float2 step[kTok / 2], du[kTok / 2], gy[kTok / 2];
+    float sdt = 0.0f;
+    {
+      float raw[kTok], xv[kTok], gv[kTok];
+      const T *px = x + t0 * p.xs[1], *pd = dt + t0 * p.dts[1], *pg = dout + (dout ? (long)t0 * p.D : 0);
 #pragma unroll
-    for (int t = 0; t < kTok; ++t) {
-      const bool in = live && t < here;
-      xv[t] = in ? to_f32(x[(t0 + t) * p.xs[1]]) : 0.0f;
-      step[t] = in ? to_f32(dt[(t0 + t) * p.dts[1]]) : 0.0f;
-      gy[t] = in && dout ? to_f32(dout[(long)(t0 + t) * p.D]) : 0.0f;
-    }
-    if (z)
-#pragma unroll
-      for (int t = 0; t < kTok; ++t) {
-        const float v = live && t < here ? to_f32(z[(t0 + t) * p.zs[1]]) : 0.0f;
-        gy[t] *= v * sigmoid_of(v);
+      for (int t = 0; t < kTok; ++t, px += p.xs[1], pd += p.dts[1], pg += p.D) {
+        const bool in = live && t < here;
+        xv[t] = in ? to_f32(*px) : 0.0f;
+        raw[t] = in ? to_f32(*pd) : 0.0f;
+        gv[t] = in && dout ? to_f32(*pg) : 0.0f;
       }
-    for (int k = lane; k < kTok * np; k += 32) {
-      const int t = k / np, n = k - t * np;
-      const bool in = t < here && n < p.N;
-      bs[k] = in ? to_f32(bm[(t0 + t) * p.bs[1] + n]) : 0.0f;
-      cs[k] = in ? to_f32(cm[(t0 + t) * p.cs[1] + n]) : 0.0f;
-    }
+      if (z) {
+        const T* pz = z + t0 * p.zs[1];
+        float zv[kTok];
 #pragma unroll
-    for (int t = 0; t < kTok; ++t) {
-      step[t] = live && t < here ? step_of(p, step[t], bias) : 0.0f;
-      sdt += step[t];
-    }
-    float y[kTok], sb[kTok], sa[kTok];
+        for (int t = 0; t < kTok; ++t, pz += p.zs[1]) zv[t] = live && t < here ? to_f32(*pz) : 0.0f;
 #pragma unroll
-    for (int t = 0; t < kTok; ++t) y[t] = sb[t] = sa[t] = 0.0f;
-    __syncwarp();
-    for (int g = 0; g < p.ng; ++g, turn ^= 1) {
-      const float4 rt4 = rate[g * kLanes + lane];
-      const float rt[4] = {rt4.x, rt4.y, rt4.z, rt4.w};
-      float a[kTok][4], s[4], r[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] = r[j] = 0.0f;
+        for (int t = 0; t < kTok; ++t) gv[t] *= zv[t] * sigmoid_of(zv[t]);
+      }
+      __syncwarp();
+      const int lanes = 1 << p.wide, n = lane & (lanes - 1);
+#pragma unroll 4
+      for (int e = lane; e < kTok << p.wide; e += 32) {
+        const int t = e >> p.wide, m = lanes <= 32 ? n : e & (lanes - 1);
+        const bool in = t < here && m < p.N;
+        const float bv = in ? to_f32(bm[(t0 + t) * p.bs[1] + m]) : 0.0f;
+        const float cv = in ? to_f32(cm[(t0 + t) * p.cs[1] + m]) : 0.0f;
+        if (m < 2 * p.ng) bs[m * kRow + t] = bv, cs[m * kRow + t] = cv;
+      }
 #pragma unroll
       for (int t = 0; t < kTok; ++t) {
-        const float4 b4 = *reinterpret_cast<const float4*>(bs + t * np + 4 * g);
-        const float bv[4] = {b4.x, b4.y, b4.z, b4.w}, du = step[t] * xv[t];
+        raw[t] = live && t < here ? step_of(p, raw[t], bias) : 0.0f;
+        sdt += raw[t];
+      }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          a[t][j] = exp2_of(step[t] * rt[j]);
-          s[j] = fmaf(a[t][j], s[j], du * bv[j]);
+      for (int t = 0; t < kTok / 2; ++t) {
+        step[t] = make_float2(raw[2 * t], raw[2 * t + 1]);
+        du[t] = __fmul2_rn(step[t], make_float2(xv[2 * t], xv[2 * t + 1]));
+        gy[t] = make_float2(gv[2 * t], gv[2 * t + 1]);
+      }
+    }
+    float2 y[kTok / 2], sb[kTok / 2], sa[kTok / 2];
+#pragma unroll
+    for (int t = 0; t < kTok / 2; ++t) y[t] = sb[t] = sa[t] = twice(0.0f);
+    __syncwarp();
+#pragma unroll 1
+    for (int g = 0; g < p.ng; ++g, turn ^= 1) {
+      const float2 rt = rate[g * kLanes];
+      const float2 mark = reinterpret_cast<const float2*>(p.marks)[(((long)unit * p.nmarks + i) * p.ng + g) * kLanes + lane];
+      float a[2][kTok], s[2], r[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float2 r2 = twice(j ? rt.y : rt.x);
+        const float4* b4 = reinterpret_cast<const float4*>(bs + (2 * g + j) * kRow);
+        const float4* c4 = reinterpret_cast<const float4*>(cs + (2 * g + j) * kRow);
+        s[j] = r[j] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < kTok / 4; ++t) {
+          const float4 v = b4[t];
+          const float2 e0 = __fmul2_rn(step[2 * t], r2), e1 = __fmul2_rn(step[2 * t + 1], r2);
+          const float2 v0 = __fmul2_rn(du[2 * t], make_float2(v.x, v.y)), v1 = __fmul2_rn(du[2 * t + 1], make_float2(v.z, v.w));
+          a[j][4 * t] = exp2_of(e0.x), a[j][4 * t + 1] = exp2_of(e0.y);
+          a[j][4 * t + 2] = exp2_of(e1.x), a[j][4 * t + 3] = exp2_of(e1.y);
+          s[j] = fmaf(a[j][4 * t], s[j], v0.x);
+          s[j] = fmaf(a[j][4 * t + 1], s[j], v0.y);
+          s[j] = fmaf(a[j][4 * t + 2], s[j], v1.x);
+          s[j] = fmaf(a[j][4 * t + 3], s[j], v1.y);
+        }
+#pragma unroll
+        for (int t = kTok / 4 - 1; t >= 0; --t) {
+          const float4 v = c4[t];
+          const float2 v0 = __fmul2_rn(gy[2 * t], make_float2(v.x, v.y)), v1 = __fmul2_rn(gy[2 * t + 1], make_float2(v.z, v.w));
+          r[j] = a[j][4 * t + 3] * (v1.y + r[j]);
+          r[j] = a[j][4 * t + 2] * (v1.x + r[j]);
+          r[j] = a[j][4 * t + 1] * (v0.y + r[j]);
+          r[j] = a[j][4 * t] * (v0.x + r[j]);
         }
       }
-#pragma unroll
-      for (int t = kTok - 1; t >= 0; --t) {
-        const float4 c4 = *reinterpret_cast<const float4*>(cs + t * np + 4 * g);
-        const float cv[4] = {c4.x, c4.y, c4.z, c4.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r[j] = a[t][j] * fmaf(cv[j], gy[t], r[j]);
-      }
-      float4* e = ex + turn * kWarps * 3 * kLanes;
-      e[(w * 3 + 0) * kLanes + lane] =
-          make_float4(exp2_of(sdt * rt[0]), exp2_of(sdt * rt[1]), exp2_of(sdt * rt[2]), exp2_of(sdt * rt[3]));
-      e[(w * 3 + 1) * kLanes + lane] = make_float4(s[0], s[1], s[2], s[3]);
-      e[(w * 3 + 2) * kLanes + lane] = make_float4(r[0], r[1], r[2], r[3]);
-      float4 h4 = reinterpret_cast<const float4*>(
-          p.marks)[((((long)b * p.tiles + tile) * p.nmarks + i) * p.ng + g) * kLanes + lane];
+      float2* e = ex + turn * kWarps * 3 * kLanes;
+      const float2 mine = make_float2(exp2_of(sdt * rt.x), exp2_of(sdt * rt.y));
+      e[(w * 3 + 0) * kLanes] = mine;
+      e[(w * 3 + 1) * kLanes] = make_float2(s[0], s[1]);
+      e[(w * 3 + 2) * kLanes] = make_float2(r[0], r[1]);
       __syncthreads();
-      float4 r4 = carry[(((blocks - 1 - i) & 1) * p.ng + g) * kLanes + lane];
-      for (int k = 0; k < w; ++k) {
-        const float4 q = e[(k * 3 + 0) * kLanes + lane], v = e[(k * 3 + 1) * kLanes + lane];
-        h4.x = fmaf(q.x, h4.x, v.x), h4.y = fmaf(q.y, h4.y, v.y), h4.z = fmaf(q.z, h4.z, v.z), h4.w = fmaf(q.w, h4.w, v.w);
-      }
-      for (int k = kWarps - 1; k > w; --k) {
-        const float4 q = e[(k * 3 + 0) * kLanes + lane], v = e[(k * 3 + 2) * kLanes + lane];
-        r4.x = fmaf(q.x, r4.x, v.x), r4.y = fmaf(q.y, r4.y, v.y), r4.z = fmaf(q.z, r4.z, v.z), r4.w = fmaf(q.w, r4.w, v.w);
-      }
-      const float h0[4] = {h4.x, h4.y, h4.z, h4.w};
-      float h[kTok][4];
-      r[0] = r4.x, r[1] = r4.y, r[2] = r4.z, r[3] = r4.w;
+      float2 h2 = mark, q = twice(1.0f), v = twice(0.0f);
 #pragma unroll
-      for (int t = 0; t < kTok; ++t) {
-        const float4 b4 = *reinterpret_cast<const float4*>(bs + t * np + 4 * g);
-        const float bv[4] = {b4.x, b4.y, b4.z, b4.w}, du = step[t] * xv[t];
+      for (int o = 0; o < kWarps - 1; ++o)
+        if (o < w) h2 = __ffma2_rn(e[(o * 3 + 0) * kLanes], h2, e[(o * 3 + 1) * kLanes]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[t][j] = fmaf(a[t][j], t ? h[t - 1][j] : h0[j], du * bv[j]);
+      for (int o = kWarps - 1; o > 0; --o)
+        if (o > w) {  // what the warps behind make of what is handed to the block
+          const float2 pr = e[(o * 3 + 0) * kLanes];
+          v = __ffma2_rn(pr, v, e[(o * 3 + 2) * kLanes]);
+          q = __fmul2_rn(pr, q);
+        }
+      const int slot = (k & 1) * p.ng + g;
+      if (Q && ok) ok = bar_wait(bars + 8 * slot, (k >> 1) & 1, &g_backward_status);
+      const float2 first = carry[slot * kLanes];
+      float2 back = __ffma2_rn(q, first, v);
+      if (w == 0) {  // for the block before
+        const float2 next = __ffma2_rn(mine, back, make_float2(r[0], r[1]));
+        if (Q) {
+          if (lane == 0 && step_i + 2 * peers < blocks) bar_expect(bars + 8 * slot, kLanes * 8);  // its use after the next
+          __syncwarp();
+          if (step_i + 1 < blocks) {
+            const int to = (rank + 1) % peers, slot_to = (((step_i + 1) / peers) & 1) * p.ng + g;
+            send(at_rank(smem_at(carry + slot_to * kLanes), to), next, at_rank(bars + 8 * slot_to, to));
+          }
+        } else {
+          carry[(((k + 1) & 1) * p.ng + g) * kLanes] = next;
+        }
       }
-      float4 da = das[g * kLanes];
-      float da4[4] = {da.x, da.y, da.z, da.w};
+      float h[2][kTok];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float4* b4 = reinterpret_cast<const float4*>(bs + (2 * g + j) * kRow);
+        float hv = j ? h2.y : h2.x;
+#pragma unroll
+        for (int t = 0; t < kTok / 4; ++t) {
+          const float4 bv = b4[t];
+          const float2 v0 = __fmul2_rn(du[2 * t], make_float2(bv.x, bv.y)), v1 = __fmul2_rn(du[2 * t + 1], make_float2(bv.z, bv.w));
+          h[j][4 * t] = fmaf(a[j][4 * t], hv, v0.x);
+          h[j][4 * t + 1] = fmaf(a[j][4 * t + 1], h[j][4 * t], v0.y);
+          h[j][4 * t + 2] = fmaf(a[j][4 * t + 2], h[j][4 * t + 1], v1.x);
+          hv = h[j][4 * t + 3] = fmaf(a[j][4 * t + 3], h[j][4 * t + 2], v1.y);
+        }
+      }
+      const float2 da = das[g * kLanes];
+      float2 da2[2] = {make_float2(da.x, 0.0f), make_float2(da.y, 0.0f)};
       float sums[kTok];
 #pragma unroll
-      for (int t = kTok - 1; t >= 0; --t) {
-        const float4 b4 = *reinterpret_cast<const float4*>(bs + t * np + 4 * g);
-        const float4 c4 = *reinterpret_cast<const float4*>(cs + t * np + 4 * g);
-        const float bv[4] = {b4.x, b4.y, b4.z, b4.w}, cv[4] = {c4.x, c4.y, c4.z, c4.w};
-        const float du = step[t] * xv[t];
-        float v[8];
+      for (int t = kTok / 2 - 1; t >= 0; --t) {
+        float2 vb[2], vc[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float dh = fmaf(cv[j], gy[t], r[j]);
-          y[t] = fmaf(cv[j], h[t][j], y[t]);
-          sb[t] = fmaf(bv[j], dh, sb[t]);
-          v[j] = dh * du;
-          v[4 + j] = gy[t] * h[t][j];
-          r[j] = a[t][j] * dh;
-          const float wt = r[j] * (t ? h[t - 1][j] : h0[j]);
-          sa[t] = fmaf(rt[j], wt, sa[t]);
-          da4[j] = fmaf(step[t], wt, da4[j]);
+        for (int j = 0; j < 2; ++j) {
+          const float2 bv = *reinterpret_cast<const float2*>(bs + (2 * g + j) * kRow + 2 * t);
+          const float2 cv = *reinterpret_cast<const float2*>(cs + (2 * g + j) * kRow + 2 * t);
+          float& rj = j ? back.y : back.x;
+          const float2 cg = __fmul2_rn(cv, gy[t]), hv = make_float2(h[j][2 * t], h[j][2 * t + 1]);
+          float2 dh, rr;
+          dh.y = cg.y + rj;
+          rr.y = a[j][2 * t + 1] * dh.y;
+          dh.x = cg.x + rr.y;
+          rr.x = rj = a[j][2 * t] * dh.x;
+          const float2 wt = make_float2(rr.x * (t ? h[j][2 * t - 1] : j ? h2.y : h2.x), rr.y * h[j][2 * t]);
+          y[t] = __ffma2_rn(cv, hv, y[t]);
+          sb[t] = __ffma2_rn(bv, dh, sb[t]);
+          sa[t] = __ffma2_rn(twice(j ? rt.y : rt.x), wt, sa[t]);
+          da2[j] = __ffma2_rn(step[t], wt, da2[j]);
+          vb[j] = __fmul2_rn(dh, du[t]);
+          vc[j] = __fmul2_rn(gy[t], hv);
         }
-        halve<4>(v, 16, lane & 16);
-        halve<2>(v, 8, lane & 8);
-        halve<1>(v, 4, lane & 4);
-        sums[t] = v[0];
+        float lo[4] = {vb[0].x, vb[1].x, vc[0].x, vc[1].x}, hi[4] = {vb[0].y, vb[1].y, vc[0].y, vc[1].y};
+        halve<2>(lo, 16, lane & 16), halve<2>(hi, 16, lane & 16);
+        halve<1>(lo, 8, lane & 8), halve<1>(hi, 8, lane & 8);
+        sums[2 * t] = lo[0], sums[2 * t + 1] = hi[0];
       }
-      das[g * kLanes] = make_float4(da4[0], da4[1], da4[2], da4[3]);
-      // a lane now holds dB (lane < 16) or dC of state (lane >> 2) & 3, for all
-      // tokens, over a quarter of the lanes each
-      halve<4>(sums, 2, lane & 2);
-      halve<2>(sums, 1, lane & 1);
-      {
-        const int t = (lane & 2 ? 4 : 0) + (lane & 1 ? 2 : 0);
-        float* part = p.part_bc + ((((long)b * p.tiles + tile) * p.T + t0 + t) * 2 + (lane >> 4)) * np + 4 * g + ((lane >> 2) & 3);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          if (t + k < here) part[(long)k * 2 * np] = sums[k];
-      }
-      if (w == 0) {
-        carry[(((blocks - i) & 1) * p.ng + g) * kLanes + lane] = make_float4(r[0], r[1], r[2], r[3]);
-        if (i == 0 && live && p.ds0) {
-          float* ds0 = p.ds0 + ((long)b * p.D + d) * p.N + 4 * g;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (4 * g + j < p.N) ds0[j] = r[j];
-        }
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < kTok; ++t) {
-      if (!live || t >= here) continue;
-      const long at = dense + (long)(t0 + t) * p.D;
-      const float g = p.skip ? skip * gy[t] : 0.0f;
-      static_cast<T*>(p.dx)[at] = from_f32<T>(fmaf(step[t], sb[t], g));
-      float raw = fmaf(xv[t], sb[t], sa[t] * 0.6931471805599453f);  // rt is A / ln 2
-      if (p.softplus) {
-        const float v = to_f32(dt[(t0 + t) * p.dts[1]]) + bias;
-        raw *= v > 20.0f ? 1.0f : 1.0f / (1.0f + expf(-v));
-      }
-      static_cast<T*>(p.ddt)[at] = from_f32<T>(raw);
-      dbias += raw;
-      dskip = fmaf(gy[t], xv[t], dskip);
-      if (z) {
-        const float v = to_f32(z[(t0 + t) * p.zs[1]]), s = sigmoid_of(v);
-        const float full = p.skip ? fmaf(skip, xv[t], y[t]) : y[t];
-        const float go = dout ? to_f32(dout[(long)(t0 + t) * p.D]) : 0.0f;
-        static_cast<T*>(p.dz)[at] = from_f32<T>(go * full * s * fmaf(v, 1.0f - s, 1.0f));
+      das[g * kLanes] = make_float2(da2[0].x + da2[0].y, da2[1].x + da2[1].y);
+      // a lane holds dB (lane < 16) or dC of state (lane >> 3) & 1, for all tokens,
+      // over an eighth of the lanes each
+      halve<4>(sums, 4, lane & 4);
+      halve<2>(sums, 2, lane & 2);
+      halve<1>(sums, 1, lane & 1);
+      rows[((lane & 7) * 2 + (lane >> 4)) * p.ng * 2 + 2 * g + ((lane >> 3) & 1)] = sums[0];
+      if (w == 0 && i == 0 && live && p.ds0) {
+        float* ds0 = p.ds0 + ((long)b * p.D + d) * p.N + 2 * g;
+        ds0[0] = back.x;
+        if (2 * g + 1 < p.N) ds0[1] = back.y;
       }
     }
     __syncwarp();
+    {
+      float* part = p.part_bc + ((long)unit * p.T + t0) * p.ng * 4;
+      for (int e = lane; e < here * p.ng * 4; e += 32) part[e] = rows[e];
+    }
+    if (!live) continue;
+    const T *px = x + t0 * p.xs[1], *pd = dt + t0 * p.dts[1];
+    long at = dense + (long)t0 * p.D;
+#pragma unroll
+    for (int t = 0; t < kTok; ++t, px += p.xs[1], pd += p.dts[1], at += p.D) {
+      if (t >= here) continue;
+      const float st = t & 1 ? step[t / 2].y : step[t / 2].x, gv = t & 1 ? gy[t / 2].y : gy[t / 2].x;
+      const float sbt = t & 1 ? sb[t / 2].y : sb[t / 2].x, sat = t & 1 ? sa[t / 2].y : sa[t / 2].x;
+      const float xt = to_f32(*px);
+      static_cast<T*>(p.dx)[at] = from_f32<T>(fmaf(st, sbt, p.skip ? skip * gv : 0.0f));
+      float raw = fmaf(xt, sbt, sat * 0.6931471805599453f);  // rate is A / ln 2
+      if (p.softplus) raw *= sigmoid_of(to_f32(*pd) + bias);
+      static_cast<T*>(p.ddt)[at] = from_f32<T>(raw);
+      dbias += raw;
+      dskip = fmaf(gv, xt, dskip);
+      if (z) {
+        const float v = to_f32(z[(t0 + t) * p.zs[1]]), g = sigmoid_of(v), yt = t & 1 ? y[t / 2].y : y[t / 2].x;
+        const float full = p.skip ? fmaf(skip, xt, yt) : yt, go = dout ? to_f32(dout[(long)(t0 + t) * p.D]) : 0.0f;
+        static_cast<T*>(p.dz)[at] = from_f32<T>(go * full * g * fmaf(v, 1.0f - g, 1.0f));
+      }
+    }
   }
   float* sums = sm + l.sums;
   sums[w * kLanes + lane] = dskip;
   sums[(kWarps + w) * kLanes + lane] = dbias;
   __syncthreads();
-  if (!live) return;
-  if (w < 2) {
-    float s = 0.0f;
-    for (int k = 0; k < kWarps; ++k) s += sums[(w * kWarps + k) * kLanes + lane];
-    p.part_ch[((long)b * 2 + w) * p.D + d] = s;
-  }
-  const float4* all = reinterpret_cast<const float4*>(sm + l.da) + lane;
-  for (int g = w; g < p.ng; g += kWarps) {
-    float4 s = all[g * kLanes];
-    for (int k = 1; k < kWarps; ++k) {
-      const float4 v = all[(k * p.ng + g) * kLanes];
-      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  if (live) {
+    const long at = (long)b * peers + rank;
+    if (w < 2) {
+      float s = 0.0f;
+      for (int o = 0; o < kWarps; ++o) s += sums[(w * kWarps + o) * kLanes + lane];
+      p.part_ch[(at * 2 + w) * p.D + d] = s;
     }
-    const float v[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (4 * g + j < p.N) p.part_a[((long)b * p.D + d) * p.N + 4 * g + j] = v[j];
+    const float2* all = reinterpret_cast<const float2*>(sm + l.da) + lane;
+    for (int g = w; g < p.ng; g += kWarps) {
+      float2 s = all[g * kLanes];
+      for (int o = 1; o < kWarps; ++o) {
+        const float2 v = all[(o * p.ng + g) * kLanes];
+        s.x += v.x, s.y += v.y;
+      }
+      float* part = p.part_a + (at * p.D + d) * p.N + 2 * g;
+      part[0] = s.x;
+      if (2 * g + 1 < p.N) part[1] = s.y;
+    }
   }
+  if (Q) cluster_sync();  // no CTA leaves while another may still write to it
 }
 
 // dB and dC: the sums over a group's tiles of 32 channels, in their order.
 template <typename T>
 __global__ void __launch_bounds__(256) sum_tiles_kernel(const Problem p) {
-  const int np = p.ng * 4;
+  const int np = p.ng * 2;
   const long i = blockIdx.x * 256L + threadIdx.x;  // (b, t, group, which, state)
   const long total = (long)p.B * p.T * p.G * 2 * np;
   if (i >= total) return;
@@ -322,19 +399,31 @@ struct StoreChannels {
 template <typename T>
 int launch_backward(const Problem& p, cudaStream_t stream) {
   const size_t smem = layout(p.ng).total * sizeof(float);
-  GRU_CUDA_TRY(cudaFuncSetAttribute(scan_backward_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const int q = backward_sharing(p);
   LaunchScope scope(kKindSelectiveScan, stream, 4);
-  scan_backward_kernel<T><<<(unsigned)((long)p.B * p.tiles), 32 * kWarps, smem, stream>>>(p);
-  GRU_CUDA_TRY(cudaGetLastError());
-  const long sums = (long)p.B * p.T * p.G * 2 * p.ng * 4;
+  const int rc = q > 1 ? launch_shared(scan_backward_kernel<T, true>, p, q, 32 * kWarps, smem, stream)
+                       : launch_shared(scan_backward_kernel<T, false>, p, 1, 32 * kWarps, smem, stream);
+  if (rc) return rc;
+  const long sums = (long)p.B * p.T * p.G * 2 * p.ng * 2;
   sum_tiles_kernel<T><<<(unsigned)((sums + 255) / 256), 256, 0, stream>>>(p);
   GRU_CUDA_TRY(cudaGetLastError());
   const long an = (long)p.D * p.N;
-  if (const int rc = sum_parts(p.part_a, p.B, an, an, StoreF32{p.da}, stream)) return rc;
-  return sum_parts(p.part_ch, p.B, 2L * p.D, 2L * p.D, StoreChannels{p.dskip, p.dbias, p.D}, stream);
+  if (const int rc = sum_parts(p.part_a, p.B * q, an, an, StoreF32{p.da}, stream)) return rc;
+  return sum_parts(p.part_ch, p.B * q, 2L * p.D, 2L * p.D, StoreChannels{p.dskip, p.dbias, p.D}, stream);
 }
 
 }  // namespace
+
+int backward_sharing(const Problem& p) { return sharing(p, (p.T + kBlock - 1) / kBlock, kResident); }
+
+int read_backward_status(int reset, int* status) {
+  GRU_CUDA_TRY(cudaMemcpyFromSymbol(status, g_backward_status, sizeof(int)));
+  if (reset) {
+    const int zero = 0;
+    GRU_CUDA_TRY(cudaMemcpyToSymbol(g_backward_status, &zero, sizeof(int)));
+  }
+  return GRU_OK;
+}
 
 int backward(const Problem& p, int dtype, cudaStream_t stream) {
   return dtype == GRU_F32 ? launch_backward<float>(p, stream) : launch_backward<bf16>(p, stream);

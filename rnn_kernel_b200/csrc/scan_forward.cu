@@ -3,14 +3,20 @@
 //   h[n] = e^{dt A[n]} h[n] + dt x B[n];   y = sum_n C[n] h[n] + skip x;   out = y silu(z)
 //
 // A CTA owns 32 channels of one sequence, a lane each, and goes over the time in
-// blocks; every warp has 16 tokens of a block.  For four states at a time a warp
-// computes its tokens' decays once (kept in registers), and from them what its
-// tokens make of a state: h -> P h + S with P = e^{A sum dt}.  The warps' P and S
-// meet in shared memory; each warp then has the state before its first token
-// from those ahead of it, and goes over its tokens again with that.  B and C are
-// broadcast reads of shared memory; the sum over n is the lane's own.
-// One exponential per token, channel and state (16 a cycle and SM) is what
-// bounds it.
+// blocks of 64 tokens, 16 a warp.  For two states at a time a warp computes its
+// tokens' decays once (kept in registers), and from them what its tokens make of
+// a state: h -> P h + S with P = e^{A sum dt}.  The warps' P and S meet in shared
+// memory; each warp then has the state before its first token from those ahead
+// of it, and goes over its tokens again with that.  Two neighbouring tokens share
+// each packed FP32 operation but the recurrence itself; B and C lie by state in
+// shared memory, so that one broadcast read serves four tokens of 32 channels.
+//
+// Where sequences and channels do not fill the GPU, up to eight CTAs of a cluster
+// share a sequence's channels and take its blocks in turn: a block's last state
+// goes to the next CTA's shared memory (st.async, counted by a barrier of the
+// receiver) as soon as the one before has come, two operations behind it; all
+// else of a block runs beside the other CTAs'.
+// One exponential per token, channel and state (16 a cycle and SM) is the bound.
 
 #include <algorithm>
 
@@ -19,57 +25,76 @@
 
 namespace gru {
 namespace scan {
+
+__device__ int g_forward_status = 0;
+
 namespace {
 
-constexpr int kTok = 16;  // tokens of a warp
+constexpr int kTok = 16;           // tokens of a warp
+constexpr int kRow = kTok + 4;     // floats between two states' tokens in shared memory
+constexpr int kBlock = kWarps * kTok;
+constexpr int kResident = 4;       // CTAs an SM holds, by registers
 
 // Shared memory in floats.
 struct Lay {
-  int dts, dus, bs, cs, ex, carry, rate, total;
+  int bars, bs, cs, ex, carry, rate, total;
 };
-__host__ __device__ inline Lay layout(int warps, int ng) {
+__host__ __device__ inline Lay layout(int ng) {
   Lay l;
   int n = 0;
-  l.dts = n, n += warps * kTok * kLanes;
-  l.dus = n, n += warps * kTok * kLanes;
-  l.bs = n, n += warps * kTok * ng * 4;
-  l.cs = n, n += warps * kTok * ng * 4;
-  l.ex = n, n += 2 * warps * 2 * kLanes * 4;
-  l.carry = n, n += 2 * ng * kLanes * 4;
-  l.rate = n, n += ng * kLanes * 4;
+  l.bars = n, n += 2 * ng * 2;
+  n = (n + 3) / 4 * 4;
+  l.bs = n, n += kWarps * ng * 2 * kRow;
+  l.cs = n, n += kWarps * ng * 2 * kRow;
+  l.ex = n, n += 2 * kWarps * 2 * kLanes * 2;
+  l.carry = n, n += 2 * ng * kLanes * 2;
+  l.rate = n, n += ng * kLanes * 2;
   l.total = n;
   return l;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256, 2) scan_forward_kernel(const Problem p) {
+__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
+
+// Q: several CTAs share a tile, as a cluster.
+template <typename T, bool Q>
+__global__ void __launch_bounds__(32 * kWarps, kResident) scan_forward_kernel(const __grid_constant__ Problem p) {
   extern __shared__ __align__(16) float sm[];
-  const int warps = blockDim.x >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Lay l = layout(warps, p.ng);
-  const int tile = blockIdx.x % p.tiles, b = blockIdx.x / p.tiles;
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Lay l = layout(p.ng);
+  const int rank = Q ? (int)cluster_rank() : 0, peers = Q ? (int)cluster_size() : 1;
+  const int unit = blockIdx.x / peers, tile = unit % p.tiles, b = unit / p.tiles;
   const int group = tile / p.per_group, local = (tile - group * p.per_group) * kLanes + lane;
   const bool live = local < p.R;
   const int d = group * p.R + (live ? local : 0);
-  const int np = p.ng * 4;
-  float* dts = sm + l.dts + w * kTok * kLanes + lane;
-  float* dus = sm + l.dus + w * kTok * kLanes + lane;
-  float* bs = sm + l.bs + w * kTok * np;
-  float* cs = sm + l.cs + w * kTok * np;
-  float4* ex = reinterpret_cast<float4*>(sm + l.ex);
-  float4* carry = reinterpret_cast<float4*>(sm + l.carry);
-  float4* rate = reinterpret_cast<float4*>(sm + l.rate);
+  float* bs = sm + l.bs + w * p.ng * 2 * kRow;
+  float* cs = sm + l.cs + w * p.ng * 2 * kRow;
+  float2* ex = reinterpret_cast<float2*>(sm + l.ex) + lane;
+  float2* carry = reinterpret_cast<float2*>(sm + l.carry) + lane;
+  float2* rate = reinterpret_cast<float2*>(sm + l.rate) + lane;
+  const uint32_t bars = smem_at(sm + l.bars);
 
   const float bias = p.bias ? p.bias[d] : 0.0f, skip = p.skip ? p.skip[d] : 0.0f;
-  for (int g = w; g < p.ng; g += warps) {
-    float r[4], s[4];
+  for (int g = w; g < p.ng; g += kWarps) {
+    float r[2], s[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = 4 * g + j;
+    for (int j = 0; j < 2; ++j) {
+      const int n = 2 * g + j;
       r[j] = live && n < p.N ? decay_rate(p.a[(long)d * p.N + n]) : 0.0f;
       s[j] = live && n < p.N && p.s0 ? p.s0[((long)b * p.D + d) * p.N + n] : 0.0f;
     }
-    rate[g * kLanes + lane] = make_float4(r[0], r[1], r[2], r[3]);
-    carry[g * kLanes + lane] = make_float4(s[0], s[1], s[2], s[3]);
+    rate[g * kLanes] = make_float2(r[0], r[1]);
+    if (rank == 0) carry[g * kLanes] = make_float2(s[0], s[1]);
+  }
+  if (Q) {  // the barrier of slot k & 1 counts the bytes of the state before this CTA's k-th block
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < 2 * p.ng; ++i) bar_init(bars + 8 * i);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      for (int i = 0; i < 2 * p.ng; ++i)
+        if (rank == 0 && i < p.ng) bar_arrive(bars + 8 * i);  // the initial state is there
+        else bar_expect(bars + 8 * i, kLanes * 8);
+    }
+    __syncthreads();
+    cluster_sync();
   }
   const T* x = static_cast<const T*>(p.x) + b * p.xs[0] + d;
   const T* dt = static_cast<const T*>(p.dt) + b * p.dts[0] + d;
@@ -77,114 +102,171 @@ __global__ void __launch_bounds__(256, 2) scan_forward_kernel(const Problem p) {
   const T* bm = static_cast<const T*>(p.b) + b * p.bs[0] + group * p.bs[2];
   const T* cm = static_cast<const T*>(p.c) + b * p.cs[0] + group * p.cs[2];
   T* out = static_cast<T*>(p.out) + (long)b * p.T * p.D + d;
-  __syncthreads();
+  if (!Q) __syncthreads();
 
   int turn = 0;
-  const int block = warps * kTok, blocks = ceil_div(p.T, block);
-  for (int i = 0; i < blocks; ++i) {
-    const int t0 = i * block + w * kTok, here = min(max(p.T - t0, 0), kTok);
-    float y[kTok], sdt = 0.0f;
+  bool ok = true;
+  const int blocks = (p.T + kBlock - 1) / kBlock;
+  for (int i = rank, k = 0; i < blocks; i += peers, ++k) {
+    const int t0 = i * kBlock + w * kTok, here = min(max(p.T - t0, 0), kTok);
+    float2 step[kTok / 2], du[kTok / 2], y[kTok / 2];
+    float sdt = 0.0f;
+    {
+      float raw[kTok], xv[kTok];
+      const T *px = x + t0 * p.xs[1], *pd = dt + t0 * p.dts[1];
 #pragma unroll
-    for (int t = 0; t < kTok; ++t) {
-      const bool in = live && t < here;
-      y[t] = in ? to_f32(x[(t0 + t) * p.xs[1]]) : 0.0f;
-      dts[t * kLanes] = in ? to_f32(dt[(t0 + t) * p.dts[1]]) : 0.0f;
-    }
-    for (int k = lane; k < kTok * np; k += 32) {
-      const int t = k / np, n = k - t * np;
-      const bool in = t < here && n < p.N;
-      bs[k] = in ? to_f32(bm[(t0 + t) * p.bs[1] + n]) : 0.0f;
-      cs[k] = in ? to_f32(cm[(t0 + t) * p.cs[1] + n]) : 0.0f;
-    }
+      for (int t = 0; t < kTok; ++t, px += p.xs[1], pd += p.dts[1]) {
+        const bool in = live && t < here;
+        xv[t] = in ? to_f32(*px) : 0.0f;
+        raw[t] = in ? to_f32(*pd) : 0.0f;
+      }
+      __syncwarp();
+      const int lanes = 1 << p.wide, n = lane & (lanes - 1);
+#pragma unroll 4
+      for (int e = lane; e < kTok << p.wide; e += 32) {  // wide >= 5: a lane keeps its n only if lanes <= 32
+        const int t = e >> p.wide, m = lanes <= 32 ? n : e & (lanes - 1);
+        const bool in = t < here && m < p.N;
+        const float bv = in ? to_f32(bm[(t0 + t) * p.bs[1] + m]) : 0.0f;
+        const float cv = in ? to_f32(cm[(t0 + t) * p.cs[1] + m]) : 0.0f;
+        if (m < 2 * p.ng) bs[m * kRow + t] = bv, cs[m * kRow + t] = cv;
+      }
 #pragma unroll
-    for (int t = 0; t < kTok; ++t) {
-      const float step = live && t < here ? step_of(p, dts[t * kLanes], bias) : 0.0f;
-      dts[t * kLanes] = step;
-      dus[t * kLanes] = step * y[t];
-      sdt += step;
-      y[t] *= skip;
-    }
-    if (!p.skip)
+      for (int t = 0; t < kTok; ++t) {
+        raw[t] = live && t < here ? step_of(p, raw[t], bias) : 0.0f;
+        sdt += raw[t];
+      }
 #pragma unroll
-      for (int t = 0; t < kTok; ++t) y[t] = 0.0f;
+      for (int t = 0; t < kTok / 2; ++t) {
+        step[t] = make_float2(raw[2 * t], raw[2 * t + 1]);
+        const float2 v = make_float2(xv[2 * t], xv[2 * t + 1]);
+        du[t] = __fmul2_rn(step[t], v);
+        y[t] = p.skip ? __fmul2_rn(twice(skip), v) : twice(0.0f);
+      }
+    }
     __syncwarp();
+#pragma unroll 1
     for (int g = 0; g < p.ng; ++g, turn ^= 1) {
-      const float4 rt = rate[g * kLanes + lane];
-      float a[kTok][4];
-      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float2 rt = rate[g * kLanes];
+      float a[2][kTok], s[2];
 #pragma unroll
-      for (int t = 0; t < kTok; ++t) {
-        const float step = dts[t * kLanes], du = dus[t * kLanes];
-        const float4 bv = *reinterpret_cast<const float4*>(bs + t * np + 4 * g);
-        a[t][0] = exp2_of(step * rt.x), a[t][1] = exp2_of(step * rt.y);
-        a[t][2] = exp2_of(step * rt.z), a[t][3] = exp2_of(step * rt.w);
-        s.x = fmaf(a[t][0], s.x, du * bv.x), s.y = fmaf(a[t][1], s.y, du * bv.y);
-        s.z = fmaf(a[t][2], s.z, du * bv.z), s.w = fmaf(a[t][3], s.w, du * bv.w);
-      }
-      float4* e = ex + turn * warps * 2 * kLanes;
-      e[(w * 2 + 0) * kLanes + lane] =
-          make_float4(exp2_of(sdt * rt.x), exp2_of(sdt * rt.y), exp2_of(sdt * rt.z), exp2_of(sdt * rt.w));
-      e[(w * 2 + 1) * kLanes + lane] = s;
-      __syncthreads();
-      float4 h = carry[((i & 1) * p.ng + g) * kLanes + lane];
-      for (int k = 0; k < w; ++k) {
-        const float4 q = e[(k * 2 + 0) * kLanes + lane], v = e[(k * 2 + 1) * kLanes + lane];
-        h.x = fmaf(q.x, h.x, v.x), h.y = fmaf(q.y, h.y, v.y), h.z = fmaf(q.z, h.z, v.z), h.w = fmaf(q.w, h.w, v.w);
-      }
-      if (p.marks && t0 % kMark == 0 && here > 0)
-        reinterpret_cast<float4*>(p.marks)[((((long)b * p.tiles + tile) * p.nmarks + t0 / kMark) * p.ng + g) * kLanes + lane] = h;
+      for (int j = 0; j < 2; ++j) {
+        const float2 r2 = twice(j ? rt.y : rt.x);
+        const float4* b4 = reinterpret_cast<const float4*>(bs + (2 * g + j) * kRow);
+        s[j] = 0.0f;
 #pragma unroll
-      for (int t = 0; t < kTok; ++t) {
-        const float du = dus[t * kLanes];
-        const float4 bv = *reinterpret_cast<const float4*>(bs + t * np + 4 * g);
-        const float4 cv = *reinterpret_cast<const float4*>(cs + t * np + 4 * g);
-        h.x = fmaf(a[t][0], h.x, du * bv.x), h.y = fmaf(a[t][1], h.y, du * bv.y);
-        h.z = fmaf(a[t][2], h.z, du * bv.z), h.w = fmaf(a[t][3], h.w, du * bv.w);
-        y[t] = fmaf(cv.x, h.x, y[t]), y[t] = fmaf(cv.y, h.y, y[t]);
-        y[t] = fmaf(cv.z, h.z, y[t]), y[t] = fmaf(cv.w, h.w, y[t]);
-      }
-      if (w == warps - 1) {
-        carry[(((i + 1) & 1) * p.ng + g) * kLanes + lane] = h;
-        if (i == blocks - 1 && live) {
-          float* last = p.last + ((long)b * p.D + d) * p.N + 4 * g;
-          const float v[4] = {h.x, h.y, h.z, h.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (4 * g + j < p.N) last[j] = v[j];
+        for (int t = 0; t < kTok / 4; ++t) {
+          const float4 v = b4[t];
+          const float2 e0 = __fmul2_rn(step[2 * t], r2), e1 = __fmul2_rn(step[2 * t + 1], r2);
+          const float2 v0 = __fmul2_rn(du[2 * t], make_float2(v.x, v.y)), v1 = __fmul2_rn(du[2 * t + 1], make_float2(v.z, v.w));
+          a[j][4 * t] = exp2_of(e0.x), a[j][4 * t + 1] = exp2_of(e0.y);
+          a[j][4 * t + 2] = exp2_of(e1.x), a[j][4 * t + 3] = exp2_of(e1.y);
+          s[j] = fmaf(a[j][4 * t], s[j], v0.x);
+          s[j] = fmaf(a[j][4 * t + 1], s[j], v0.y);
+          s[j] = fmaf(a[j][4 * t + 2], s[j], v1.x);
+          s[j] = fmaf(a[j][4 * t + 3], s[j], v1.y);
         }
       }
+      float2* e = ex + turn * kWarps * 2 * kLanes;
+      const float2 mine = make_float2(exp2_of(sdt * rt.x), exp2_of(sdt * rt.y));
+      e[(w * 2 + 0) * kLanes] = mine;
+      e[(w * 2 + 1) * kLanes] = make_float2(s[0], s[1]);
+      __syncthreads();
+      // what the warps ahead make of the block's first state
+      float2 q = twice(1.0f), v = twice(0.0f);
+#pragma unroll
+      for (int r = 0; r < kWarps - 1; ++r)
+        if (r < w) {
+          const float2 pr = e[(r * 2 + 0) * kLanes];
+          v = __ffma2_rn(pr, v, e[(r * 2 + 1) * kLanes]);
+          q = __fmul2_rn(pr, q);
+        }
+      const int slot = (k & 1) * p.ng + g;
+      if (Q && ok) ok = bar_wait(bars + 8 * slot, (k >> 1) & 1, &g_forward_status);
+      const float2 first = carry[slot * kLanes];
+      float2 h2 = __ffma2_rn(q, first, v);
+      if (w == kWarps - 1) {  // the state behind the block, for the next
+        const float2 next = __ffma2_rn(mine, h2, make_float2(s[0], s[1]));
+        if (Q) {
+          if (lane == 0 && i + 2 * peers < blocks) bar_expect(bars + 8 * slot, kLanes * 8);  // its use after the next
+          __syncwarp();
+          if (i + 1 < blocks) {
+            const int to = (rank + 1) % peers, slot_to = (((i + 1) / peers) & 1) * p.ng + g;
+            send(at_rank(smem_at(carry + slot_to * kLanes), to), next, at_rank(bars + 8 * slot_to, to));
+          }
+        } else {
+          carry[(((k + 1) & 1) * p.ng + g) * kLanes] = next;
+        }
+      }
+      if (p.marks && t0 % kMark == 0 && here > 0)
+        reinterpret_cast<float2*>(p.marks)[(((long)unit * p.nmarks + t0 / kMark) * p.ng + g) * kLanes + lane] = h2;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float4* b4 = reinterpret_cast<const float4*>(bs + (2 * g + j) * kRow);
+        const float4* c4 = reinterpret_cast<const float4*>(cs + (2 * g + j) * kRow);
+        float h = j ? h2.y : h2.x;
+#pragma unroll
+        for (int t = 0; t < kTok / 4; ++t) {
+          const float4 bv = b4[t], cv = c4[t];
+          const float2 v0 = __fmul2_rn(du[2 * t], make_float2(bv.x, bv.y)), v1 = __fmul2_rn(du[2 * t + 1], make_float2(bv.z, bv.w));
+          float2 h0, h1;
+          h0.x = fmaf(a[j][4 * t], h, v0.x);
+          h0.y = fmaf(a[j][4 * t + 1], h0.x, v0.y);
+          h1.x = fmaf(a[j][4 * t + 2], h0.y, v1.x);
+          h1.y = fmaf(a[j][4 * t + 3], h1.x, v1.y);
+          h = h1.y;
+          y[2 * t] = __ffma2_rn(make_float2(cv.x, cv.y), h0, y[2 * t]);
+          y[2 * t + 1] = __ffma2_rn(make_float2(cv.z, cv.w), h1, y[2 * t + 1]);
+        }
+        s[j] = h;
+      }
+      if (w == kWarps - 1 && i == blocks - 1 && live) {
+        float* last = p.last + ((long)b * p.D + d) * p.N + 2 * g;
+        last[0] = s[0];
+        if (2 * g + 1 < p.N) last[1] = s[1];
+      }
+    }
+    if (!live) continue;
+    T* po = out + (long)t0 * p.D;
+    if (z) {
+      const T* pz = z + t0 * p.zs[1];
+      float zv[kTok];
+#pragma unroll
+      for (int t = 0; t < kTok; ++t, pz += p.zs[1]) zv[t] = t < here ? to_f32(*pz) : 0.0f;
+#pragma unroll
+      for (int t = 0; t < kTok; ++t) {
+        float& v = t & 1 ? y[t / 2].y : y[t / 2].x;
+        v *= zv[t] * sigmoid_of(zv[t]);
+      }
     }
 #pragma unroll
-    for (int t = 0; t < kTok; ++t) {
-      if (!live || t >= here) continue;
-      float v = y[t];
-      if (z) {
-        const float gate = to_f32(z[(t0 + t) * p.zs[1]]);
-        v *= gate * sigmoid_of(gate);
-      }
-      out[(long)(t0 + t) * p.D] = from_f32<T>(v);
-    }
-    __syncwarp();
+    for (int t = 0; t < kTok; ++t, po += p.D)
+      if (t < here) *po = from_f32<T>(t & 1 ? y[t / 2].y : y[t / 2].x);
   }
+  if (Q) cluster_sync();  // no CTA leaves while another may still write to it
+}
+
+template <typename T>
+int launch_forward(const Problem& p, cudaStream_t stream) {
+  const size_t smem = layout(p.ng).total * sizeof(float);
+  const int q = sharing(p, (p.T + kBlock - 1) / kBlock, kResident);
+  LaunchScope scope(kKindSelectiveScan, stream);
+  if (q > 1) return launch_shared(scan_forward_kernel<T, true>, p, q, 32 * kWarps, smem, stream);
+  return launch_shared(scan_forward_kernel<T, false>, p, 1, 32 * kWarps, smem, stream);
 }
 
 }  // namespace
 
-template <typename T>
-int launch_forward(const Problem& p, cudaStream_t stream) {
-  int warps = std::min(8, ceil_div(p.T, kTok));
-  const size_t most = 227 * 1024;
-  while (warps > 1 && layout(warps, p.ng).total * sizeof(float) > most) warps /= 2;
-  const size_t smem = layout(warps, p.ng).total * sizeof(float);
-  GRU_CUDA_TRY(cudaFuncSetAttribute(scan_forward_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  LaunchScope scope(kKindSelectiveScan, stream);
-  scan_forward_kernel<T><<<(unsigned)((long)p.B * p.tiles), warps * 32, smem, stream>>>(p);
-  GRU_CUDA_TRY(cudaGetLastError());
-  return GRU_OK;
-}
-
 int forward(const Problem& p, int dtype, cudaStream_t stream) {
   return dtype == GRU_F32 ? launch_forward<float>(p, stream) : launch_forward<bf16>(p, stream);
+}
+
+int read_forward_status(int reset, int* status) {
+  GRU_CUDA_TRY(cudaMemcpyFromSymbol(status, g_forward_status, sizeof(int)));
+  if (reset) {
+    const int zero = 0;
+    GRU_CUDA_TRY(cudaMemcpyToSymbol(g_forward_status, &zero, sizeof(int)));
+  }
+  return GRU_OK;
 }
 
 }  // namespace scan

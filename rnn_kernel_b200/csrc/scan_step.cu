@@ -99,7 +99,7 @@ int launch_step(const Problem& p, float* state, int vec, cudaStream_t stream) {
 template <typename T>
 int step(const Problem& p, float* state, int vec, cudaStream_t stream) {
   int lp = 1;
-  while (lp < p.ng) lp *= 2;
+  while (lp * 4 < p.N) lp *= 2;
   const bool four = (long)p.B * p.D * lp / (kStepThreads * 4) >= 4L * 148;
 #define GRU_STEP(LP) \
   if (lp == LP) return four ? launch_step<T, LP, 4>(p, state, vec, stream) : launch_step<T, LP, 1>(p, state, vec, stream);
@@ -141,14 +141,17 @@ void fill(Problem& a, const gru_scan_args& p) {
   a.softplus = p.dt_softplus;
   a.per_group = ceil_div(a.R, kLanes), a.tiles = a.per_group * a.G;
   a.ng = ceil_div(a.N, kGroup);
+  a.wide = 0;
+  while ((1 << a.wide) < a.N || a.wide < 1) ++a.wide;
   a.nmarks = ceil_div(a.T, kMark);
 }
 
-void lay_marks(Problem& a, Pieces& m) { a.marks = m.floats((size_t)a.B * a.tiles * a.nmarks * a.ng * 4 * kLanes); }
+void lay_marks(Problem& a, Pieces& m) { a.marks = m.floats((size_t)a.B * a.tiles * a.nmarks * a.ng * kGroup * kLanes); }
 void lay_parts(Problem& a, Pieces& m) {
-  a.part_bc = m.floats((size_t)a.B * a.tiles * a.T * 2 * a.ng * 4);
-  a.part_a = m.floats((size_t)a.B * a.D * a.N);
-  a.part_ch = m.floats((size_t)a.B * 2 * a.D);
+  a.part_bc = m.floats((size_t)a.B * a.tiles * a.T * 2 * a.ng * kGroup);
+  const size_t q = backward_sharing(a);
+  a.part_a = m.floats(q * a.B * a.D * a.N);
+  a.part_ch = m.floats(q * a.B * 2 * a.D);
 }
 
 }  // namespace
