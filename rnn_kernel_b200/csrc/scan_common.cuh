@@ -8,7 +8,6 @@ namespace gru {
 namespace scan {
 
 constexpr int kMaxStates = 64;
-constexpr int kGroup = 2;        // states a lane works on at a time
 constexpr int kLanes = 32;       // channels of a CTA, one a lane
 constexpr int kWarps = 4;        // warps of a CTA, neighbouring pieces of the time
 constexpr int kMark = 32;        // tokens between two states that the forward keeps for the gradient
@@ -19,7 +18,7 @@ struct Problem {
   long xs[2], dts[2], zs[2], bs[3], cs[3];  // batch, token (, group)
   void* out;
   float* last;
-  float* marks;  // [B][tiles][mark][state group][32] float2: states at the tokens 0, kMark, ...
+  float* marks;  // [B][tiles][mark][state, padded][32]: states at the tokens 0, kMark, ...
   // gradient
   const void* dout;
   const float* dlast;
@@ -30,9 +29,10 @@ struct Problem {
   float* part_ch;  // [B][CTA of a tile][2][D]: of skip and dt_bias
   int B, T, D, N, G, R;  // R: channels of a group
   int softplus;
+  int pairs, dpairs;  // rows of x, dt and z, and of dout, lie on 4-byte boundaries
   int per_group, tiles;  // tiles of 32 channels in a group, and in all
-  int ng;                // groups of states: ceil(N / 2)
-  int wide;              // log2 of the states rounded up to a power of two
+  int np;                // states rounded up to a multiple of four
+  int wide;              // log2 of the states rounded up to a power of two, at least 4
   int nmarks;
 };
 
@@ -49,32 +49,129 @@ __device__ __forceinline__ float decay_rate(float a) {
   return r < -3.0e38f ? -3.0e38f : r > 3.0e38f ? 3.0e38f : r;
 }
 
+__device__ __forceinline__ float rcp_of(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float x, float y) {  // NaN where either is
+  float z;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
+
 // log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x|.  With s = e / (2 + e), at
 // most 1/3, log(1 + e) = 2 artanh(s) = 2 (s + s^3 / 3 + s^5 / 5 + ...), whose
-// terms after s^13 sum to less than 2^-24 of it: as exact for small e as for
-// large, in 2 special and some 14 plain operations (log1pf(expf(x)): about 60,
-// which made a third of the forward's instructions).
-__device__ __forceinline__ float softplus_of(float x) {
-  const float ax = fminf(fabsf(x), 120.0f), t = ax * -1.4426950408889634f;
-  const float lost = fmaf(ax, -1.4426950408889634f, -t);  // of the exponent by its rounding
-  float e = exp2_of(t);
-  e = fmaf(e, lost * 0.6931471805599453f, e);
-  const float s = __fdividef(e, 2.0f + e), q = s * s;
-  float r = fmaf(q, 1.0f / 15.0f, 1.0f / 13.0f);
-  r = fmaf(q, r, 1.0f / 11.0f);
-  r = fmaf(q, r, 1.0f / 9.0f);
-  r = fmaf(q, r, 1.0f / 7.0f);
-  r = fmaf(q, r, 1.0f / 5.0f);
-  r = fmaf(q, r, 1.0f / 3.0f);
-  r = fmaf(q * r, s, s);
-  return x == x ? fmaxf(x, 0.0f) + 2.0f * r : x;
+// terms after s^15 sum to less than 2^-26 of it: as exact for small e as for
+// large, in 2 special and some 10 packed operations (log1pf(expf(x)) takes about
+// 60, which made a third of the forward's instructions).
+__device__ __forceinline__ float2 softplus_of(float2 x) {
+  const float2 ax = make_float2(fminf(fabsf(x.x), 120.0f), fminf(fabsf(x.y), 120.0f));
+  const float2 t = __fmul2_rn(ax, twice(-1.4426950408889634f));
+  // what the exponent lost by its rounding
+  const float2 lost = __ffma2_rn(ax, twice(-1.4426950408889634f), make_float2(-t.x, -t.y));
+  float2 e = make_float2(exp2_of(t.x), exp2_of(t.y));
+  e = __ffma2_rn(e, __fmul2_rn(lost, twice(0.6931471805599453f)), e);
+  const float2 den = __fadd2_rn(e, twice(2.0f));
+  const float2 s = __fmul2_rn(e, make_float2(rcp_of(den.x), rcp_of(den.y))), q = __fmul2_rn(s, s);
+  float2 r = __ffma2_rn(q, twice(1.0f / 15.0f), twice(1.0f / 13.0f));
+  r = __ffma2_rn(q, r, twice(1.0f / 11.0f));
+  r = __ffma2_rn(q, r, twice(1.0f / 9.0f));
+  r = __ffma2_rn(q, r, twice(1.0f / 7.0f));
+  r = __ffma2_rn(q, r, twice(1.0f / 5.0f));
+  r = __ffma2_rn(q, r, twice(1.0f / 3.0f));
+  r = __ffma2_rn(__fmul2_rn(q, r), s, s);
+  return __ffma2_rn(twice(2.0f), r, make_float2(max_nan(x.x, 0.0f), max_nan(x.y, 0.0f)));
+}
+// The step sizes of two raw values.
+__device__ __forceinline__ float2 step_of(int softplus, float2 raw, float bias) {
+  raw = __fadd2_rn(raw, twice(bias));
+  return softplus ? softplus_of(raw) : raw;
+}
+// 1 / (1 + e^-x), as sigmoid_of
+__device__ __forceinline__ float2 sigmoid_of2(float2 x) {
+  const float2 t = __fmul2_rn(x, twice(-1.4426950408889634f));
+  const float2 d = __fadd2_rn(make_float2(exp2_of(t.x), exp2_of(t.y)), twice(1.0f));
+  return make_float2(rcp_of(d.x), rcp_of(d.y));
 }
 
-// The step size of a raw value.
-__device__ __forceinline__ float step_of(const Problem& p, float raw, float bias) {
-  raw += bias;
-  return p.softplus ? softplus_of(raw) : raw;
+// ---- a warp's tokens of a tensor [token][channel], through shared memory ----
+
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits for all but the last N issued.
+template <int N>
+__device__ __forceinline__ void copies_done() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+
+// TOK tokens x 32 channels from src (the tile's first channel of the first token,
+// `stride` elements a token) to dst [TOK][32]; tokens from `here` on and channels
+// from `width` on read as zero.  `async`: rows lie on 4-byte boundaries and the
+// width fills 4-byte pieces, so the copy can run behind the warp's work (finished
+// by copies_done() and a __syncwarp()); otherwise it is done at once.
+template <typename T, int TOK>
+__device__ __forceinline__ void fetch_rows(const T* src, long stride, int here, int width, bool async, T* dst) {
+  const int lane = threadIdx.x & 31;
+  constexpr int kPer = 4 / sizeof(T), kLanesRow = kLanes / kPer, kRows = 32 / kLanesRow;
+  if (async) {
+    const int row = lane / kLanesRow, c = (lane % kLanesRow) * kPer;
+    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(dst + row * kLanes + c));
+#pragma unroll
+    for (int t = 0; t < TOK; t += kRows) {
+      const int at = t + row;
+      const bool in = at < here && c < width;
+      const T* from = in ? src + at * stride + c : src;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + t * kLanes * (int)sizeof(T)), "l"(from),
+                   "r"(in ? 4 : 0)
+                   : "memory");
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < TOK; ++t)
+      dst[t * kLanes + lane] = t < here && lane < width ? src[t * stride + lane] : from_f32<T>(0.0f);
+  }
+}
+
+// A warp's rows of B and C [token][state], as FP32 by state: row n holds the
+// tokens, ROW floats apart; states from N on are zero.  load() leaves them in
+// registers, so that the loads run behind other work, up to store().
+template <typename T, int TOK, int ROW>
+struct FewRows {
+  static constexpr int kMost = TOK * kMaxStates / 32;
+  // states past the first 16 tokens x 16 are loaded and stored in turns
+  static constexpr int kHeld = TOK / 2;
+  T b[kHeld], c[kHeld];
+  __device__ __forceinline__ void at(const Problem& p, int i, int* t, int* n) const {
+    const int e = i * 32 + (threadIdx.x & 31);
+    *t = e >> p.wide, *n = e & ((1 << p.wide) - 1);
+  }
+  __device__ __forceinline__ void load(const Problem& p, const T* bm, const T* cm, int here, int first) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      int t, n;
+      at(p, first + i, &t, &n);
+      const bool in = t < here && n < p.N;
+      b[i] = in ? bm[t * p.bs[1] + n] : from_f32<T>(0.0f);
+      c[i] = in ? cm[t * p.cs[1] + n] : from_f32<T>(0.0f);
+    }
+  }
+  __device__ __forceinline__ void store(const Problem& p, float* bs, float* cs, int rows, int first) const {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      int t, n;
+      at(p, first + i, &t, &n);
+      if (t < TOK && n < rows) bs[n * ROW + t] = to_f32(b[i]), cs[n * ROW + t] = to_f32(c[i]);
+    }
+  }
+  // what does not fit the registers
+  __device__ __forceinline__ void rest(const Problem& p, const T* bm, const T* cm, int here, float* bs, float* cs, int rows) {
+    for (int first = kHeld; first * 32 < TOK << p.wide; first += kHeld) {
+      load(p, bm, cm, here, first);
+      store(p, bs, cs, rows, first);
+    }
+  }
+};
 
 // ---- clusters: CTAs of one sequence and tile that take its blocks in turn ----
 

@@ -35,46 +35,64 @@ constexpr int kRow = kTok + 4;     // floats between two states' tokens in share
 constexpr int kBlock = kWarps * kTok;
 constexpr int kResident = 4;       // CTAs an SM holds, by registers
 
-// Shared memory in floats.
+// Shared memory in floats; ng: pairs of states, elem: bytes of an element.
 struct Lay {
-  int bars, bs, cs, ex, carry, rate, total;
+  int bars, in, bs, cs, ex, carry, rate, total;
 };
-__host__ __device__ inline Lay layout(int ng) {
+__host__ __device__ inline Lay layout(int ng, int elem) {
   Lay l;
   int n = 0;
-  l.bars = n, n += 2 * ng * 2;
-  n = (n + 3) / 4 * 4;
+  l.bars = n, n += (2 * ng * 2 + 3) / 4 * 4;
+  l.in = n, n += kWarps * 3 * kTok * kLanes * elem / 4;
   l.bs = n, n += kWarps * ng * 2 * kRow;
   l.cs = n, n += kWarps * ng * 2 * kRow;
-  l.ex = n, n += 2 * kWarps * 2 * kLanes * 2;
+  l.ex = n, n += 2 * kWarps * kLanes * 4;
   l.carry = n, n += 2 * ng * kLanes * 2;
   l.rate = n, n += ng * kLanes * 2;
   l.total = n;
   return l;
 }
 
-__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
-
 // Q: several CTAs share a tile, as a cluster.
 template <typename T, bool Q>
 __global__ void __launch_bounds__(32 * kWarps, kResident) scan_forward_kernel(const __grid_constant__ Problem p) {
   extern __shared__ __align__(16) float sm[];
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Lay l = layout(p.ng);
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, ng = (p.N + 1) / 2;
+  const Lay l = layout(ng, sizeof(T));
   const int rank = Q ? (int)cluster_rank() : 0, peers = Q ? (int)cluster_size() : 1;
   const int unit = blockIdx.x / peers, tile = unit % p.tiles, b = unit / p.tiles;
-  const int group = tile / p.per_group, local = (tile - group * p.per_group) * kLanes + lane;
-  const bool live = local < p.R;
-  const int d = group * p.R + (live ? local : 0);
-  float* bs = sm + l.bs + w * p.ng * 2 * kRow;
-  float* cs = sm + l.cs + w * p.ng * 2 * kRow;
-  float2* ex = reinterpret_cast<float2*>(sm + l.ex) + lane;
+  const int group = tile / p.per_group, c0 = (tile - group * p.per_group) * kLanes;
+  const int width = min(p.R - c0, kLanes), d0 = group * p.R + c0;
+  const bool live = lane < width;
+  const int d = d0 + (live ? lane : 0);
+  T* xs = reinterpret_cast<T*>(sm + l.in) + w * 3 * kTok * kLanes;  // x, dt, z
+  T *ds = xs + kTok * kLanes, *zs = ds + kTok * kLanes;
+  float* bs = sm + l.bs + w * ng * 2 * kRow;
+  float* cs = sm + l.cs + w * ng * 2 * kRow;
+  float4* ex = reinterpret_cast<float4*>(sm + l.ex) + lane;
   float2* carry = reinterpret_cast<float2*>(sm + l.carry) + lane;
   float2* rate = reinterpret_cast<float2*>(sm + l.rate) + lane;
   const uint32_t bars = smem_at(sm + l.bars);
 
+  const T* x = static_cast<const T*>(p.x) + b * p.xs[0] + d0;
+  const T* dt = static_cast<const T*>(p.dt) + b * p.dts[0] + d0;
+  const T* z = p.z ? static_cast<const T*>(p.z) + b * p.zs[0] + d0 : nullptr;
+  const T* bm = static_cast<const T*>(p.b) + b * p.bs[0] + group * p.bs[2];
+  const T* cm = static_cast<const T*>(p.c) + b * p.cs[0] + group * p.cs[2];
+  T* out = static_cast<T*>(p.out) + (long)b * p.T * p.D + d;
+  const bool async = p.pairs && (sizeof(T) == 4 || width % 2 == 0);
+  auto fetch = [&](const T* src, long stride, int i, T* dst) {
+    const int t0 = i * kBlock + w * kTok;
+    if (t0 < p.T) fetch_rows<T, kTok>(src + t0 * stride, stride, p.T - t0, width, async, dst);
+  };
+  fetch(x, p.xs[1], rank, xs);
+  fetch(dt, p.dts[1], rank, ds);
+  copies_issued();  // x and dt, then z, block after block: what is waited for is always the last but one
+  if (z) fetch(z, p.zs[1], rank, zs);
+  copies_issued();
+
   const float bias = p.bias ? p.bias[d] : 0.0f, skip = p.skip ? p.skip[d] : 0.0f;
-  for (int g = w; g < p.ng; g += kWarps) {
+  for (int g = w; g < ng; g += kWarps) {
     float r[2], s[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -87,22 +105,17 @@ __global__ void __launch_bounds__(32 * kWarps, kResident) scan_forward_kernel(co
   }
   if (Q) {  // the barrier of slot k & 1 counts the bytes of the state before this CTA's k-th block
     if (threadIdx.x == 0) {
-      for (int i = 0; i < 2 * p.ng; ++i) bar_init(bars + 8 * i);
+      for (int i = 0; i < 2 * ng; ++i) bar_init(bars + 8 * i);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-      for (int i = 0; i < 2 * p.ng; ++i)
-        if (rank == 0 && i < p.ng) bar_arrive(bars + 8 * i);  // the initial state is there
+      for (int i = 0; i < 2 * ng; ++i)
+        if (rank == 0 && i < ng) bar_arrive(bars + 8 * i);  // the initial state is there
         else bar_expect(bars + 8 * i, kLanes * 8);
     }
     __syncthreads();
     cluster_sync();
+  } else {
+    __syncthreads();
   }
-  const T* x = static_cast<const T*>(p.x) + b * p.xs[0] + d;
-  const T* dt = static_cast<const T*>(p.dt) + b * p.dts[0] + d;
-  const T* z = p.z ? static_cast<const T*>(p.z) + b * p.zs[0] + d : nullptr;
-  const T* bm = static_cast<const T*>(p.b) + b * p.bs[0] + group * p.bs[2];
-  const T* cm = static_cast<const T*>(p.c) + b * p.cs[0] + group * p.cs[2];
-  T* out = static_cast<T*>(p.out) + (long)b * p.T * p.D + d;
-  if (!Q) __syncthreads();
 
   int turn = 0;
   bool ok = true;
@@ -112,40 +125,33 @@ __global__ void __launch_bounds__(32 * kWarps, kResident) scan_forward_kernel(co
     float2 step[kTok / 2], du[kTok / 2], y[kTok / 2];
     float sdt = 0.0f;
     {
-      float raw[kTok], xv[kTok];
-      const T *px = x + t0 * p.xs[1], *pd = dt + t0 * p.dts[1];
-#pragma unroll
-      for (int t = 0; t < kTok; ++t, px += p.xs[1], pd += p.dts[1]) {
-        const bool in = live && t < here;
-        xv[t] = in ? to_f32(*px) : 0.0f;
-        raw[t] = in ? to_f32(*pd) : 0.0f;
-      }
+      FewRows<T, kTok, kRow> few;
+      const T *pb = bm + t0 * p.bs[1], *pc = cm + t0 * p.cs[1];
+      few.load(p, pb, pc, here, 0);
+      copies_done<1>();
       __syncwarp();
-      const int lanes = 1 << p.wide, n = lane & (lanes - 1);
-#pragma unroll 4
-      for (int e = lane; e < kTok << p.wide; e += 32) {  // wide >= 5: a lane keeps its n only if lanes <= 32
-        const int t = e >> p.wide, m = lanes <= 32 ? n : e & (lanes - 1);
-        const bool in = t < here && m < p.N;
-        const float bv = in ? to_f32(bm[(t0 + t) * p.bs[1] + m]) : 0.0f;
-        const float cv = in ? to_f32(cm[(t0 + t) * p.cs[1] + m]) : 0.0f;
-        if (m < 2 * p.ng) bs[m * kRow + t] = bv, cs[m * kRow + t] = cv;
-      }
-#pragma unroll
-      for (int t = 0; t < kTok; ++t) {
-        raw[t] = live && t < here ? step_of(p, raw[t], bias) : 0.0f;
-        sdt += raw[t];
-      }
 #pragma unroll
       for (int t = 0; t < kTok / 2; ++t) {
-        step[t] = make_float2(raw[2 * t], raw[2 * t + 1]);
-        const float2 v = make_float2(xv[2 * t], xv[2 * t + 1]);
-        du[t] = __fmul2_rn(step[t], v);
+        const float2 v = make_float2(to_f32(xs[2 * t * kLanes + lane]), to_f32(xs[(2 * t + 1) * kLanes + lane]));
+        float2 s = step_of(p.softplus, make_float2(to_f32(ds[2 * t * kLanes + lane]), to_f32(ds[(2 * t + 1) * kLanes + lane])), bias);
+        if (here < kTok) s.x = 2 * t < here ? s.x : 0.0f, s.y = 2 * t + 1 < here ? s.y : 0.0f;
+        step[t] = s;
+        du[t] = __fmul2_rn(s, v);
+        if (here < kTok) du[t].x = 2 * t < here ? du[t].x : 0.0f, du[t].y = 2 * t + 1 < here ? du[t].y : 0.0f;
         y[t] = p.skip ? __fmul2_rn(twice(skip), v) : twice(0.0f);
+        sdt += s.x + s.y;
       }
+      few.store(p, bs, cs, 2 * ng, 0);
+      few.rest(p, pb, pc, here, bs, cs, 2 * ng);
+      __syncwarp();
+      if (i + peers < blocks) {
+        fetch(x, p.xs[1], i + peers, xs);
+        fetch(dt, p.dts[1], i + peers, ds);
+      }
+      copies_issued();
     }
-    __syncwarp();
 #pragma unroll 1
-    for (int g = 0; g < p.ng; ++g, turn ^= 1) {
+    for (int g = 0; g < ng; ++g, turn ^= 1) {
       const float2 rt = rate[g * kLanes];
       float a[2][kTok], s[2];
 #pragma unroll
@@ -166,21 +172,20 @@ __global__ void __launch_bounds__(32 * kWarps, kResident) scan_forward_kernel(co
           s[j] = fmaf(a[j][4 * t + 3], s[j], v1.y);
         }
       }
-      float2* e = ex + turn * kWarps * 2 * kLanes;
+      float4* e = ex + turn * kWarps * kLanes;
       const float2 mine = make_float2(exp2_of(sdt * rt.x), exp2_of(sdt * rt.y));
-      e[(w * 2 + 0) * kLanes] = mine;
-      e[(w * 2 + 1) * kLanes] = make_float2(s[0], s[1]);
+      e[w * kLanes] = make_float4(mine.x, mine.y, s[0], s[1]);
       __syncthreads();
       // what the warps ahead make of the block's first state
       float2 q = twice(1.0f), v = twice(0.0f);
 #pragma unroll
       for (int r = 0; r < kWarps - 1; ++r)
         if (r < w) {
-          const float2 pr = e[(r * 2 + 0) * kLanes];
-          v = __ffma2_rn(pr, v, e[(r * 2 + 1) * kLanes]);
-          q = __fmul2_rn(pr, q);
+          const float4 o = e[r * kLanes];
+          v = __ffma2_rn(make_float2(o.x, o.y), v, make_float2(o.z, o.w));
+          q = __fmul2_rn(make_float2(o.x, o.y), q);
         }
-      const int slot = (k & 1) * p.ng + g;
+      const int slot = (k & 1) * ng + g;
       if (Q && ok) ok = bar_wait(bars + 8 * slot, (k >> 1) & 1, &g_forward_status);
       const float2 first = carry[slot * kLanes];
       float2 h2 = __ffma2_rn(q, first, v);
@@ -190,15 +195,17 @@ __global__ void __launch_bounds__(32 * kWarps, kResident) scan_forward_kernel(co
           if (lane == 0 && i + 2 * peers < blocks) bar_expect(bars + 8 * slot, kLanes * 8);  // its use after the next
           __syncwarp();
           if (i + 1 < blocks) {
-            const int to = (rank + 1) % peers, slot_to = (((i + 1) / peers) & 1) * p.ng + g;
+            const int to = (rank + 1) % peers, slot_to = (((i + 1) / peers) & 1) * ng + g;
             send(at_rank(smem_at(carry + slot_to * kLanes), to), next, at_rank(bars + 8 * slot_to, to));
           }
         } else {
-          carry[(((k + 1) & 1) * p.ng + g) * kLanes] = next;
+          carry[(((k + 1) & 1) * ng + g) * kLanes] = next;
         }
       }
-      if (p.marks && t0 % kMark == 0 && here > 0)
-        reinterpret_cast<float2*>(p.marks)[(((long)unit * p.nmarks + t0 / kMark) * p.ng + g) * kLanes + lane] = h2;
+      if (p.marks && t0 % kMark == 0 && here > 0) {
+        float* mark = p.marks + (((long)unit * p.nmarks + t0 / kMark) * p.np + 2 * g) * kLanes + lane;
+        mark[0] = h2.x, mark[kLanes] = h2.y;
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const float4* b4 = reinterpret_cast<const float4*>(bs + (2 * g + j) * kRow);
@@ -225,29 +232,37 @@ __global__ void __launch_bounds__(32 * kWarps, kResident) scan_forward_kernel(co
         if (2 * g + 1 < p.N) last[1] = s[1];
       }
     }
-    if (!live) continue;
-    T* po = out + (long)t0 * p.D;
+    copies_done<1>();
+    __syncwarp();
     if (z) {
-      const T* pz = z + t0 * p.zs[1];
-      float zv[kTok];
 #pragma unroll
-      for (int t = 0; t < kTok; ++t, pz += p.zs[1]) zv[t] = t < here ? to_f32(*pz) : 0.0f;
+      for (int t = 0; t < kTok / 2; ++t) {
+        const float2 v = make_float2(to_f32(zs[2 * t * kLanes + lane]), to_f32(zs[(2 * t + 1) * kLanes + lane]));
+        y[t] = __fmul2_rn(y[t], __fmul2_rn(v, sigmoid_of2(v)));
+      }
+      __syncwarp();
+      if (i + peers < blocks) fetch(z, p.zs[1], i + peers, zs);
+    }
+    copies_issued();
+    if (live) {
+      T* po = out + (long)t0 * p.D;
+      if (here == kTok) {
 #pragma unroll
-      for (int t = 0; t < kTok; ++t) {
-        float& v = t & 1 ? y[t / 2].y : y[t / 2].x;
-        v *= zv[t] * sigmoid_of(zv[t]);
+        for (int t = 0; t < kTok; ++t, po += p.D) *po = from_f32<T>(t & 1 ? y[t / 2].y : y[t / 2].x);
+      } else {
+#pragma unroll
+        for (int t = 0; t < kTok; ++t, po += p.D)
+          if (t < here) *po = from_f32<T>(t & 1 ? y[t / 2].y : y[t / 2].x);
       }
     }
-#pragma unroll
-    for (int t = 0; t < kTok; ++t, po += p.D)
-      if (t < here) *po = from_f32<T>(t & 1 ? y[t / 2].y : y[t / 2].x);
+    __syncwarp();
   }
   if (Q) cluster_sync();  // no CTA leaves while another may still write to it
 }
 
 template <typename T>
 int launch_forward(const Problem& p, cudaStream_t stream) {
-  const size_t smem = layout(p.ng).total * sizeof(float);
+  const size_t smem = layout((p.N + 1) / 2, sizeof(T)).total * sizeof(float);
   const int q = sharing(p, (p.T + kBlock - 1) / kBlock, kResident);
   LaunchScope scope(kKindSelectiveScan, stream);
   if (q > 1) return launch_shared(scan_forward_kernel<T, true>, p, q, 32 * kWarps, smem, stream);

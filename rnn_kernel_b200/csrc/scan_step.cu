@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const Problem p
     const int group = in ? d / p.R : 0;
     const long db = in ? d : 0;
     const float x = to_f32(static_cast<const T*>(p.x)[b * p.xs[0] + db]);
-    const float step = step_of(p, to_f32(static_cast<const T*>(p.dt)[b * p.dts[0] + db]), p.bias ? p.bias[db] : 0.0f);
+    const float step = step_of(p.softplus, twice(to_f32(static_cast<const T*>(p.dt)[b * p.dts[0] + db])), p.bias ? p.bias[db] : 0.0f).x;
     const T* bm = static_cast<const T*>(p.b) + b * p.bs[0] + group * p.bs[2] + n0;
     const T* cm = static_cast<const T*>(p.c) + b * p.cs[0] + group * p.cs[2] + n0;
     float y = 0.0f;
@@ -139,16 +139,19 @@ void fill(Problem& a, const gru_scan_args& p) {
   for (int i = 0; i < 3; ++i) a.bs[i] = p.b_stride[i], a.cs[i] = p.c_stride[i];
   a.B = p.B, a.T = p.T, a.D = p.D, a.N = p.N, a.G = p.G, a.R = p.D / p.G;
   a.softplus = p.dt_softplus;
+  const int per = p.dtype == GRU_F32 ? 1 : 2;
+  a.pairs = ((bits(p.x) | bits(p.dt) | bits(p.z)) & 3) == 0 && a.R % per == 0;
+  for (int i = 0; i < 2; ++i) a.pairs = a.pairs && p.x_stride[i] % per == 0 && p.dt_stride[i] % per == 0 && p.z_stride[i] % per == 0;
   a.per_group = ceil_div(a.R, kLanes), a.tiles = a.per_group * a.G;
-  a.ng = ceil_div(a.N, kGroup);
-  a.wide = 0;
-  while ((1 << a.wide) < a.N || a.wide < 1) ++a.wide;
+  a.np = ceil_div(a.N, 4) * 4;
+  a.wide = 2;
+  while ((1 << a.wide) < a.N) ++a.wide;
   a.nmarks = ceil_div(a.T, kMark);
 }
 
-void lay_marks(Problem& a, Pieces& m) { a.marks = m.floats((size_t)a.B * a.tiles * a.nmarks * a.ng * kGroup * kLanes); }
+void lay_marks(Problem& a, Pieces& m) { a.marks = m.floats((size_t)a.B * a.tiles * a.nmarks * a.np * kLanes); }
 void lay_parts(Problem& a, Pieces& m) {
-  a.part_bc = m.floats((size_t)a.B * a.tiles * a.T * 2 * a.ng * kGroup);
+  a.part_bc = m.floats((size_t)a.B * a.tiles * a.T * 2 * a.np);
   const size_t q = backward_sharing(a);
   a.part_a = m.floats(q * a.B * a.D * a.N);
   a.part_ch = m.floats(q * a.B * 2 * a.D);
@@ -237,6 +240,7 @@ extern "C" int gru_scan_backward(const gru_scan_args* p, const void* dout, const
   if (!stash || stash_bytes < m.used || !workspace || workspace_bytes < w.used || (bits(stash) | bits(workspace)) & 15)
     return refuse(me, "stash or workspace too small or not 16-byte aligned");
   a.dout = dout, a.dlast = dfinal;
+  a.dpairs = (bits(dout) & 3) == 0 && (p->dtype == GRU_F32 || p->D % 2 == 0);
   a.dx = dx, a.ddt = ddt, a.da = da, a.db = db, a.dc = dc, a.dskip = dskip, a.dz = dz, a.dbias = ddt_bias, a.ds0 = dinitial;
   return backward(a, p->dtype, stream);
 }
