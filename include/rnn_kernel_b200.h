@@ -218,20 +218,21 @@ typedef struct {
   const float* a;                 /* dense [D, N] */
   const float *skip, *dt_bias;    /* [D], or NULL for zeros */
   const float* initial_state;     /* dense [B, D, N], or NULL for zeros */
-  /* elements between batch rows and tokens (and groups); a token's channels and
-   * a group's states are consecutive */
+  /* elements between batch rows and tokens (less than 2^31 bytes) (and groups); a
+   * token's channels and a group's states are consecutive */
   long x_stride[2], dt_stride[2], z_stride[2], b_stride[3], c_stride[3];
 } gru_scan_args; /* host struct */
 
-/* Bytes that a training forward leaves for gru_scan_backward, and that call's
- * workspace, from the sizes alone; 0 and an error text for sizes that they refuse. */
+/* Bytes that a training forward leaves for gru_scan_backward, and the workspace
+ * of that (backward != 0) or of a forward (which may be 0), from the sizes alone;
+ * 0 and an error text for sizes that they refuse. */
 size_t gru_scan_stash_bytes(const gru_scan_args* args);
-size_t gru_scan_workspace_bytes(const gru_scan_args* args);
+size_t gru_scan_workspace_bytes(const gru_scan_args* args, int backward);
 
 /* All T tokens: out dense [B, T, D], final_state dense [B, D, N].  stash:
  * gru_scan_stash_bytes() bytes for a training forward, or NULL. */
 int gru_scan_forward(const gru_scan_args* args, void* out, float* final_state, void* stash, size_t stash_bytes,
-                     void* stream);
+                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gradients (dense, overwritten) of everything that the forward read, from dout
  * dense [B, T, D] and dfinal dense [B, D, N] (either NULL: zeros); dskip, ddt_bias

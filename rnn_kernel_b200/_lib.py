@@ -73,8 +73,8 @@ SIGNATURES = {
                            + [_size_t, ctypes.c_void_p]),
     "gru_delta_step": (_int, [ctypes.c_void_p] * 4),
     "gru_scan_stash_bytes": (_size_t, [ctypes.c_void_p]),
-    "gru_scan_workspace_bytes": (_size_t, [ctypes.c_void_p]),
-    "gru_scan_forward": (_int, [ctypes.c_void_p] * 4 + [_size_t, ctypes.c_void_p]),
+    "gru_scan_workspace_bytes": (_size_t, [ctypes.c_void_p, _int]),
+    "gru_scan_forward": (_int, [ctypes.c_void_p] * 4 + [_size_t, ctypes.c_void_p, _size_t, ctypes.c_void_p]),
     "gru_scan_backward": (_int, [ctypes.c_void_p] * 4 + [_size_t] + [ctypes.c_void_p] * 10 + [_size_t, ctypes.c_void_p]),
     "gru_scan_step": (_int, [ctypes.c_void_p] * 4),
     "gru_conv_workspace_bytes": (_size_t, [ctypes.c_void_p]),

@@ -367,10 +367,6 @@ int gru_device_status(int reset) {
   int st = 0, st2 = 0;
   if (read_device_status(reset, &st) != GRU_OK) return -1;
   if (read_gemm_status(reset, &st2) != GRU_OK) return -1;
-  st |= st2;
-  if (scan::read_forward_status(reset, &st2) != GRU_OK) return -1;
-  st |= st2;
-  if (scan::read_backward_status(reset, &st2) != GRU_OK) return -1;
   return st | st2;
 }
 

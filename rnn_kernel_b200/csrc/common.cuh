@@ -147,10 +147,6 @@ int tc_gemm_sum(const TcGemmArgs* a, int n, const float* const* part, const long
                 cudaStream_t stream, int kind);
 bool tc_rows_ok(const TcGemmArgs& a);
 int read_gemm_status(int reset, int* status);
-namespace scan {
-int read_forward_status(int reset, int* status);
-int read_backward_status(int reset, int* status);
-}  // namespace scan
 
 // Transpose a [rows, cols] matrix into [cols, ldd] (columns rows .. ldd zeroed).
 int transpose(const float* src, int rows, int cols, float* dst, int ldd, cudaStream_t stream);

@@ -9,17 +9,17 @@
 //   ddt_t = x_t sum_n B_t dh_t + sum_n A w_t,   w_t = dh_t a_t h_{t-1};   dA = sum_t dt_t w_t
 //
 // The forward's shape, backwards: a CTA owns 32 channels of one sequence, a lane
-// each, and goes over blocks of 32 tokens from the last to the first, 8 tokens a
-// warp.  The forward kept the state before each block.  For four states at a time a
-// warp computes its tokens' decays once and from them its tokens' effect on the
-// state (P h + S) and on what is handed back (P r + R); both meet the other
-// warps' in shared memory, and the warp goes over its tokens forwards for h and
-// backwards for the gradients.  Sums over channels are butterflies over the
-// lanes in which each round halves the values: 64 values (8 tokens, 4 states, dB
-// and dC) take 62 exchanges and leave a lane two sums.  The tiles' sums of dB and
-// dC are added by a second launch, in a fixed order, as are those over sequences
-// of dA, dskip and dbias.  Clusters share a sequence's blocks as in the forward.
-// Bound by instructions: some 22 per token, channel and state.
+// each, a warp two states at a time (twice two above 32 states), and goes over
+// blocks of 16 tokens from the last to the first.  The forward kept the state
+// before each block; from it a warp computes its states at the block's tokens,
+// with the decays, in registers, and then goes over the tokens backwards.  The
+// warps' shares of y, sum_n B dh and sum_n A w meet in shared memory, where two
+// tokens a warp are finished.  Sums over channels are butterflies over the lanes in
+// which each round halves the values: 64 values (16 tokens, 2 states, dB and dC)
+// take 62 exchanges and leave a lane two sums.  The tiles' sums of dB and dC are
+// added by a second launch, in a fixed order, as are those over sequences of dA,
+// dskip and dbias.  Segments as in the forward.  Bound by instructions: some 26
+// per token, channel and state, of them 8 for the sums over channels.
 
 #include <algorithm>
 
@@ -29,41 +29,24 @@
 namespace gru {
 namespace scan {
 
-__device__ int g_backward_status = 0;
-
 namespace {
 
-constexpr int kTok = 8;            // tokens of a warp
-constexpr int kRow = kTok + 4;     // floats between two states' tokens in shared memory
-constexpr int kBlock = kWarps * kTok;
-constexpr int kResident = 3;       // CTAs an SM holds, by registers
-static_assert(kBlock == kMark, "the forward keeps the state before each block");
-
-// Shared memory in floats; np: states, padded; elem: bytes of an element.
+// Shared memory in floats.
 struct Lay {
-  int bars, in, bs, cs, ex, carry, rate, da, rows, sums, total;
+  int step, du, gy, bs, cs, part, sums, total;
 };
-__host__ __device__ inline Lay layout(int np, int elem) {
+__host__ __device__ inline Lay layout(int warps, int np) {
   Lay l;
   int n = 0;
-  l.bars = n, n += np;
-  l.in = n, n += 2 * kWarps * 4 * kTok * kLanes * elem / 4;
-  l.bs = n, n += kWarps * np * kRow;
-  l.cs = n, n += kWarps * np * kRow;
-  l.ex = n, n += 2 * kWarps * 3 * kLanes * 4;
-  l.carry = n, n += 2 * np * kLanes;
-  l.rate = n, n += np * kLanes;
-  l.da = n, n += kWarps * np * kLanes;
-  l.rows = n, n += kWarps * kTok * np * 2;
-  l.sums = n, n += 2 * kWarps * kLanes;
+  l.step = n, n += kBlock * kLanes;
+  l.du = n, n += kBlock * kLanes;
+  l.gy = n, n += kBlock * kLanes;
+  l.bs = n, n += np * kRow;
+  l.cs = n, n += np * kRow;
+  l.part = n, n += warps * 3 * kBlock * kLanes;  // y, sum B dh, sum A w
+  l.sums = n, n += 2 * warps * kLanes;
   l.total = n;
   return l;
-}
-
-__device__ __forceinline__ float4 fma4(float4 x, float4 y, float4 z) {
-  const float2 a = __ffma2_rn(make_float2(x.x, x.y), make_float2(y.x, y.y), make_float2(z.x, z.y));
-  const float2 b = __ffma2_rn(make_float2(x.z, x.w), make_float2(y.z, y.w), make_float2(z.z, z.w));
-  return make_float4(a.x, a.y, b.x, b.y);
 }
 
 // One round of the butterfly: lanes with `bit` keep the upper half of 2 M values
@@ -77,342 +60,310 @@ __device__ __forceinline__ void halve(float* v, int bit, bool upper) {
   }
 }
 
-// Q: several CTAs share a tile, as a cluster.
-template <typename T, bool Q>
-__global__ void __launch_bounds__(32 * kWarps, kResident) scan_backward_kernel(const __grid_constant__ Problem p) {
+// GW: pairs of states of a warp.  SUM: only what the segments hand back.  MOST, ONE,
+// W and K as in the forward.
+template <typename T, int GW, bool SUM, int MOST, bool ONE, int W, int K>
+__global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kernel(const __grid_constant__ Problem p) {
   extern __shared__ __align__(16) float sm[];
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, ng = p.np / 4;
-  const Lay l = layout(p.np, sizeof(T));
-  const int rank = Q ? (int)cluster_rank() : 0, peers = Q ? (int)cluster_size() : 1;
-  const int unit = blockIdx.x / peers, tile = unit % p.tiles, b = unit / p.tiles;
-  const int group = tile / p.per_group, c0 = (tile - group * p.per_group) * kLanes;
-  const int width = min(p.R - c0, kLanes), d0 = group * p.R + c0;
-  const bool live = lane < width;
-  const int d = d0 + (live ? lane : 0);
-  constexpr int kTile = kTok * kLanes;
-  T* in0 = reinterpret_cast<T*>(sm + l.in) + w * 8 * kTile;  // two buffers of x, dt, dout, z
-  float* bs = sm + l.bs + w * p.np * kRow;
-  float* cs = sm + l.cs + w * p.np * kRow;
-  float* rows = sm + l.rows + w * kTok * p.np * 2;  // [token][dB, dC][state]
-  float4* ex = reinterpret_cast<float4*>(sm + l.ex) + lane;
-  float4* carry = reinterpret_cast<float4*>(sm + l.carry) + lane;
-  float4* rate = reinterpret_cast<float4*>(sm + l.rate) + lane;
-  float4* das = reinterpret_cast<float4*>(sm + l.da) + w * ng * kLanes + lane;
-  const uint32_t bars = smem_at(sm + l.bars);
+  const int warps = W ? W : blockDim.x >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Lay l = layout(warps, p.np);
+  const Place q = place(p);
+  if (SUM && q.seg == 0) return;
+  const T* x = static_cast<const T*>(p.x) + q.b * p.xb + q.d;
+  const T* dt = static_cast<const T*>(p.dt) + q.b * p.dtb + q.d;
+  const T* z = p.z ? static_cast<const T*>(p.z) + q.b * p.zb + q.d : nullptr;
+  const T* bm = static_cast<const T*>(p.b) + q.b * p.bb + q.group * p.bg;
+  const T* cm = static_cast<const T*>(p.c) + q.b * p.cb + q.group * p.cg;
+  const long dense = (long)q.b * p.T * p.D + q.d;
+  const T* dout = p.dout ? static_cast<const T*>(p.dout) + dense : nullptr;
+  const float bias = p.bias ? p.bias[q.d] : 0.0f, skip = p.skip ? p.skip[q.d] : 0.0f;
 
-  const T* x = static_cast<const T*>(p.x) + b * p.xs[0] + d0;
-  const T* dt = static_cast<const T*>(p.dt) + b * p.dts[0] + d0;
-  const T* z = p.z ? static_cast<const T*>(p.z) + b * p.zs[0] + d0 : nullptr;
-  const T* bm = static_cast<const T*>(p.b) + b * p.bs[0] + group * p.bs[2];
-  const T* cm = static_cast<const T*>(p.c) + b * p.cs[0] + group * p.cs[2];
-  const T* dout = p.dout ? static_cast<const T*>(p.dout) + (long)b * p.T * p.D + d0 : nullptr;
-  const int blocks = (p.T + kBlock - 1) / kBlock;
-  const bool async = p.pairs && (sizeof(T) == 4 || width % 2 == 0);
-  auto fetch = [&](int i, T* to) {
-    const int t0 = i * kBlock + w * kTok, here = p.T - t0;
-    if (here <= 0) return;
-    fetch_rows<T, kTok>(x + t0 * p.xs[1], p.xs[1], here, width, async, to);
-    fetch_rows<T, kTok>(dt + t0 * p.dts[1], p.dts[1], here, width, async, to + kTile);
-    if (dout) fetch_rows<T, kTok>(dout + (long)t0 * p.D, p.D, here, width, async && p.dpairs, to + 2 * kTile);
-    if (z) fetch_rows<T, kTok>(z + t0 * p.zs[1], p.zs[1], here, width, async, to + 3 * kTile);
+  // states 2 (g warps + w) and the next
+  float rt[GW][2], back[GW][2];
+  float2 da[GW][2];
+#pragma unroll
+  for (int g = 0; g < GW; ++g)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int n = 2 * (g * warps + w) + j;
+      const bool in = q.live && n < p.N;
+      rt[g][j] = in ? decay_rate(p.a[(long)q.d * p.N + n]) : 0.0f;
+      back[g][j] = !SUM && in && p.dlast ? p.dlast[((long)q.b * p.D + q.d) * p.N + n] : 0.0f;
+      da[g][j] = twice(0.0f);
+    }
+  if (!SUM)
+    for (int s = p.segs - 1; s > q.seg; --s) {
+      const long at = (long)q.unit * p.segs + s;
+      const float steps = p.seg_steps[at * kLanes + lane];
+#pragma unroll
+      for (int g = 0; g < GW; ++g)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int n = 2 * (g * warps + w) + j;
+          if (n < p.np)
+            back[g][j] = fmaf(exp2_of(rt[g][j] * steps), back[g][j], p.seg_sums[(at * p.np + n) * kLanes + lane]);
+        }
+    }
+
+  Pair<T> nx, nd, nz, ng;  // a pair of the next block's tokens; of this one's below
+  Pair<T> cx, cd, cz, cg;
+  Few<T, K> few;
+  few.init(p, bm, cm);
+  const int lastt = q.end - 1;
+  auto load = [&](int t, Pair<T>& px, Pair<T>& pd, Pair<T>& pz, Pair<T>& pg) {
+    px.load(x, p.xst, t, lastt);
+    pd.load(dt, p.dtst, t, lastt);
+    if (z) pz.load(z, p.zst, t, lastt);
+    if (dout) pg.load(dout, p.ost, t, lastt);
   };
-  fetch(blocks - 1 - rank, in0);
-  copies_issued();
-
-  const float bias = p.bias ? p.bias[d] : 0.0f, skip = p.skip ? p.skip[d] : 0.0f;
-  for (int g = w; g < ng; g += kWarps) {
-    float r[4], s[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = 4 * g + j;
-      r[j] = live && n < p.N ? decay_rate(p.a[(long)d * p.N + n]) : 0.0f;
-      s[j] = live && n < p.N && p.dlast ? p.dlast[((long)b * p.D + d) * p.N + n] : 0.0f;
+  const bool first_pair = !ONE || w < kBlock / 2;
+  auto prefetch = [&](int t0) {
+    if (first_pair) load(t0 + 2 * w, nx, nd, nz, ng);
+    few.load(p, t0, lastt);
+  };
+  auto prepare_pair = [&](const Pair<T>& px, const Pair<T>& pd, const Pair<T>& pz, const Pair<T>& pg, int t, int at) {
+    const bool a = q.live && t <= lastt, b = q.live && t < lastt;
+    const float s0 = a ? step_of(p.softplus, to_f32(pd.x), bias) : 0.0f;
+    const float s1 = b ? step_of(p.softplus, to_f32(pd.y), bias) : 0.0f;
+    float g0 = a && dout ? to_f32(pg.x) : 0.0f, g1 = b && dout ? to_f32(pg.y) : 0.0f;
+    if (z) {
+      const float z0 = to_f32(pz.x), z1 = to_f32(pz.y);
+      g0 = a ? g0 * (z0 * gate_of(z0)) : 0.0f, g1 = b ? g1 * (z1 * gate_of(z1)) : 0.0f;
     }
-    rate[g * kLanes] = make_float4(r[0], r[1], r[2], r[3]);
-    if (rank == 0) carry[g * kLanes] = make_float4(s[0], s[1], s[2], s[3]);
-  }
-  for (int g = 0; g < ng; ++g) das[g * kLanes] = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (Q) {  // the barrier of slot k & 1 counts the bytes of what is handed back to this CTA's k-th block
-    if (threadIdx.x == 0) {
-      for (int i = 0; i < 2 * ng; ++i) bar_init(bars + 8 * i);
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-      for (int i = 0; i < 2 * ng; ++i)
-        if (rank == 0 && i < ng) bar_arrive(bars + 8 * i);  // the last state's gradient is there
-        else bar_expect(bars + 8 * i, kLanes * 16);
-    }
-    __syncthreads();
-    cluster_sync();
-  } else {
-    __syncthreads();
-  }
-  float dskip = 0.0f, dbias = 0.0f;
-
-  int turn = 0;
-  bool ok = true;
-  for (int from = rank, k = 0; from < blocks; from += peers, ++k) {
-    const int i = blocks - 1 - from;
-    const int t0 = i * kBlock + w * kTok, here = min(max(p.T - t0, 0), kTok);
-    const T* in = in0 + (k & 1) * 4 * kTile;
-    float2 step[kTok / 2], du[kTok / 2], gy[kTok / 2];
-    float sdt = 0.0f;
-    {
-      FewRows<T, kTok, kRow> few;
-      const T *pb = bm + t0 * p.bs[1], *pc = cm + t0 * p.cs[1];
-      few.load(p, pb, pc, here, 0);
-      copies_done<0>();
-      __syncwarp();
-      auto pair = [&](int which, int t) {
-        const T* at = in + which * kTile + 2 * t * kLanes + lane;
-        return make_float2(to_f32(at[0]), to_f32(at[kLanes]));
-      };
-#pragma unroll
-      for (int t = 0; t < kTok / 2; ++t) {
-        step[t] = step_of(p.softplus, pair(1, t), bias);
-        du[t] = __fmul2_rn(step[t], pair(0, t));
-        gy[t] = dout ? pair(2, t) : twice(0.0f);
-        if (z) {
-          const float2 v = pair(3, t);
-          gy[t] = __fmul2_rn(gy[t], __fmul2_rn(v, sigmoid_of2(v)));
-        }
-        if (here < kTok) {
-          if (2 * t >= here) step[t].x = du[t].x = gy[t].x = 0.0f;
-          if (2 * t + 1 >= here) step[t].y = du[t].y = gy[t].y = 0.0f;
-        }
-        sdt += step[t].x + step[t].y;
+    pair_in(sm + l.step, at) = make_float2(s0, s1);
+    pair_in(sm + l.du, at) = make_float2(a ? s0 * to_f32(px.x) : 0.0f, b ? s1 * to_f32(px.y) : 0.0f);
+    pair_in(sm + l.gy, at) = make_float2(g0, g1);
+  };
+  auto prepare = [&](int t0) {
+    if (first_pair) prepare_pair(nx, nd, nz, ng, t0 + 2 * w, pair_at(2 * w, lane));
+    if (!ONE)
+      for (int u = w + warps; u < kBlock / 2; u += warps) {
+        Pair<T> px, pd, pz, pg;
+        load(t0 + 2 * u, px, pd, pz, pg);
+        prepare_pair(px, pd, pz, pg, t0 + 2 * u, pair_at(2 * u, lane));
       }
-      few.store(p, bs, cs, p.np, 0);
-      few.rest(p, pb, pc, here, bs, cs, p.np);
+    few.store(sm + l.bs, sm + l.cs, t0, lastt);
+    cx = nx, cd = nd, cz = nz, cg = ng;
+  };
+  float dskip = 0.0f, dbias = 0.0f;
+  // A token's sums over the states, and what follows from them.
+  auto finish_token = [&](T px, T pd, T pz, T pg, float y, float sb, float sa, float gy, float step, int t) {
+    const float xv = to_f32(px);
+    const float gx = fmaf(step, sb, p.skip ? skip * gy : 0.0f);
+    float raw = fmaf(xv, sb, sa * 0.6931471805599453f);  // rt is A / ln 2
+    if (p.softplus) raw *= gate_of(to_f32(pd) + bias);
+    const long at = dense + (long)t * p.D;
+    static_cast<T*>(p.dx)[at] = from_f32<T>(gx), static_cast<T*>(p.ddt)[at] = from_f32<T>(raw);
+    if (z) {
+      const float v = to_f32(pz), s = gate_of(v), full = p.skip ? fmaf(skip, xv, y) : y, go = dout ? to_f32(pg) : 0.0f;
+      static_cast<T*>(p.dz)[at] = from_f32<T>(go * full * (s * fmaf(v, 1.0f - s, 1.0f)));
     }
-    if (from + peers < blocks) fetch(i - peers, in0 + (~k & 1) * 4 * kTile);
-    copies_issued();
-    float2 y[kTok / 2], sb[kTok / 2], sa[kTok / 2];
+    dbias += raw, dskip = fmaf(gy, xv, dskip);
+  };
+  // part: [quad][y, sum B dh, sum A w][warp][lane]
+  auto finish_pair = [&](const Pair<T>& px, const Pair<T>& pd, const Pair<T>& pz, const Pair<T>& pg, int u, int t) {
+    float2 sum[3];
 #pragma unroll
-    for (int t = 0; t < kTok / 2; ++t) y[t] = sb[t] = sa[t] = twice(0.0f);
-    __syncwarp();
-#pragma unroll 1
-    for (int g = 0; g < ng; ++g, turn ^= 1) {
-      const float4 rt4 = rate[g * kLanes];
-      const float rt[4] = {rt4.x, rt4.y, rt4.z, rt4.w};
-      float a[4][kTok], s[4], r[4], mark[4];
-      const float* kept = p.marks + (((long)unit * p.nmarks + i) * p.np + 4 * g) * kLanes + lane;
+    for (int i = 0; i < 3; ++i) {
+      sum[i] = twice(0.0f);
+      if (i == 0 && !z) continue;
+      const float* part = sm + l.part + (((u >> 1) * 3 + i) * warps * kLanes + lane) * 4 + 2 * (u & 1);
+#pragma unroll (W ? W : 4)
+      for (int k = 0; k < warps; ++k) sum[i] = __fadd2_rn(sum[i], *reinterpret_cast<const float2*>(part + k * 4 * kLanes));
+    }
+    if (!q.live) return;
+    const int at = pair_at(2 * u, lane);
+    const float2 gy = pair_in(sm + l.gy, at), step = pair_in(sm + l.step, at);
+    finish_token(px.x, pd.x, pz.x, pg.x, sum[0].x, sum[1].x, sum[2].x, gy.x, step.x, t);
+    if (t < lastt) finish_token(px.y, pd.y, pz.y, pg.y, sum[0].y, sum[1].y, sum[2].y, gy.y, step.y, t + 1);
+  };
+  auto finish = [&](int t0) {
+    if (first_pair && t0 + 2 * w <= lastt) finish_pair(cx, cd, cz, cg, w, t0 + 2 * w);
+    if (!ONE)
+      for (int u = w + warps; u < kBlock / 2 && t0 + 2 * u <= lastt; u += warps) {
+        Pair<T> px, pd, pz, pg;
+        load(t0 + 2 * u, px, pd, pz, pg);
+        finish_pair(px, pd, pz, pg, u, t0 + 2 * u);
+      }
+  };
+
+  const float4* step = reinterpret_cast<const float4*>(sm + l.step) + lane;
+  const float4* du = reinterpret_cast<const float4*>(sm + l.du) + lane;
+  const float4* gy = reinterpret_cast<const float4*>(sm + l.gy) + lane;
+  float total = 0.0f;
+  const int start = q.first + (q.end - 1 - q.first) / kBlock * kBlock;  // the last block
+  // the marks of this warp's first state; its lanes' rows of partial sums
+  const float* mark = p.marks + (((long)q.unit * p.nmarks + start / kBlock) * p.np + 2 * w) * kLanes + lane;
+  float* bc = p.part_bc + (((long)q.unit * p.np + 2 * w + ((lane >> 3) & 1)) * 2 + (lane >> 4)) * p.T;
+  const int mine = (lane & 4 ? 8 : 0) + (lane & 2 ? 4 : 0) + (lane & 1 ? 2 : 0);
+  prefetch(start);
+  prepare(start);
+  if (start > q.first) prefetch(start - kBlock);
+  __syncthreads();
+  for (int t0 = start; t0 >= q.first; t0 -= kBlock) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mark[j] = 4 * g + j < p.N ? kept[j * kLanes] : 0.0f;
+    for (int g = 0; g < GW; ++g) {
+      const int n0 = 2 * (g * warps + w);
+      const float* bs = sm + l.bs + n0 * kRow;
+      const float* cs = sm + l.cs + n0 * kRow;
+      if (GW > 1 && n0 >= p.np) {  // no such states: nothing to add
+        continue;
+      }
+      float a[2][kBlock], h[2][kBlock], h0[2] = {0.0f, 0.0f};
+      if (!SUM) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 r2 = twice(rt[j]);
-        const float4* b4 = reinterpret_cast<const float4*>(bs + (4 * g + j) * kRow);
-        const float4* c4 = reinterpret_cast<const float4*>(cs + (4 * g + j) * kRow);
-        s[j] = r[j] = 0.0f;
+        for (int j = 0; j < 2; ++j) h0[j] = n0 + j < p.N ? mark[(g * 2 * warps + j) * kLanes] : 0.0f;
+      }
 #pragma unroll
-        for (int t = 0; t < kTok / 4; ++t) {
-          const float4 v = b4[t];
-          const float2 e0 = __fmul2_rn(step[2 * t], r2), e1 = __fmul2_rn(step[2 * t + 1], r2);
-          const float2 v0 = __fmul2_rn(du[2 * t], make_float2(v.x, v.y)), v1 = __fmul2_rn(du[2 * t + 1], make_float2(v.z, v.w));
+      for (int t = 0; t < kBlock / 4; ++t) {
+        const float4 s = step[t * kLanes], u = du[t * kLanes];
+        if (SUM) total += (s.x + s.y) + (s.z + s.w);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float2 e0 = __fmul2_rn(make_float2(s.x, s.y), twice(rt[g][j]));
+          const float2 e1 = __fmul2_rn(make_float2(s.z, s.w), twice(rt[g][j]));
           a[j][4 * t] = exp2_of(e0.x), a[j][4 * t + 1] = exp2_of(e0.y);
           a[j][4 * t + 2] = exp2_of(e1.x), a[j][4 * t + 3] = exp2_of(e1.y);
-          s[j] = fmaf(a[j][4 * t], s[j], v0.x);
-          s[j] = fmaf(a[j][4 * t + 1], s[j], v0.y);
-          s[j] = fmaf(a[j][4 * t + 2], s[j], v1.x);
-          s[j] = fmaf(a[j][4 * t + 3], s[j], v1.y);
-        }
-#pragma unroll
-        for (int t = kTok / 4 - 1; t >= 0; --t) {
-          const float4 v = c4[t];
-          const float2 v0 = __fmul2_rn(gy[2 * t], make_float2(v.x, v.y)), v1 = __fmul2_rn(gy[2 * t + 1], make_float2(v.z, v.w));
-          r[j] = a[j][4 * t + 3] * (v1.y + r[j]);
-          r[j] = a[j][4 * t + 2] * (v1.x + r[j]);
-          r[j] = a[j][4 * t + 1] * (v0.y + r[j]);
-          r[j] = a[j][4 * t] * (v0.x + r[j]);
-        }
-      }
-      float4* e = ex + turn * kWarps * 3 * kLanes;
-      const float4 mine = make_float4(exp2_of(sdt * rt[0]), exp2_of(sdt * rt[1]), exp2_of(sdt * rt[2]), exp2_of(sdt * rt[3]));
-      e[(w * 3 + 0) * kLanes] = mine;
-      e[(w * 3 + 1) * kLanes] = make_float4(s[0], s[1], s[2], s[3]);
-      e[(w * 3 + 2) * kLanes] = make_float4(r[0], r[1], r[2], r[3]);
-      __syncthreads();
-      float4 h4 = make_float4(mark[0], mark[1], mark[2], mark[3]);
-      float4 q = make_float4(1.f, 1.f, 1.f, 1.f), v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int o = 0; o < kWarps - 1; ++o)
-        if (o < w) h4 = fma4(e[(o * 3 + 0) * kLanes], h4, e[(o * 3 + 1) * kLanes]);
-#pragma unroll
-      for (int o = kWarps - 1; o > 0; --o)
-        if (o > w) {  // what the warps behind make of what is handed to the block
-          const float4 pr = e[(o * 3 + 0) * kLanes];
-          v = fma4(pr, v, e[(o * 3 + 2) * kLanes]);
-          q.x *= pr.x, q.y *= pr.y, q.z *= pr.z, q.w *= pr.w;
-        }
-      const int slot = (k & 1) * ng + g;
-      if (Q && ok) ok = bar_wait(bars + 8 * slot, (k >> 1) & 1, &g_backward_status);
-      const float4 back4 = fma4(q, carry[slot * kLanes], v);
-      if (w == 0) {  // for the block before
-        const float4 next = fma4(mine, back4, make_float4(r[0], r[1], r[2], r[3]));
-        if (Q) {
-          if (lane == 0 && from + 2 * peers < blocks) bar_expect(bars + 8 * slot, kLanes * 16);  // its use after the next
-          __syncwarp();
-          if (from + 1 < blocks) {
-            const int to = (rank + 1) % peers, slot_to = (((from + 1) / peers) & 1) * ng + g;
-            const uint32_t there = at_rank(smem_at(carry + slot_to * kLanes), to), bar = at_rank(bars + 8 * slot_to, to);
-            send(there, make_float2(next.x, next.y), bar);
-            send(there + 8, make_float2(next.z, next.w), bar);
+          if (!SUM) {
+            const float4 bv = *reinterpret_cast<const float4*>(bs + j * kRow + 4 * t);
+            const float2 v0 = __fmul2_rn(make_float2(u.x, u.y), make_float2(bv.x, bv.y));
+            const float2 v1 = __fmul2_rn(make_float2(u.z, u.w), make_float2(bv.z, bv.w));
+            h[j][4 * t] = fmaf(a[j][4 * t], t ? h[j][t ? 4 * t - 1 : 0] : h0[j], v0.x);
+            h[j][4 * t + 1] = fmaf(a[j][4 * t + 1], h[j][4 * t], v0.y);
+            h[j][4 * t + 2] = fmaf(a[j][4 * t + 2], h[j][4 * t + 1], v1.x);
+            h[j][4 * t + 3] = fmaf(a[j][4 * t + 3], h[j][4 * t + 2], v1.y);
           }
-        } else {
-          carry[(((k + 1) & 1) * ng + g) * kLanes] = next;
         }
       }
-      const float h0[4] = {h4.x, h4.y, h4.z, h4.w};
-      float h[4][kTok];
+      float sums[kBlock];
+      float2 da2[2] = {twice(0.0f), twice(0.0f)};  // of the block: short sums first
+      float4* part = reinterpret_cast<float4*>(sm + l.part) + w * kLanes + lane;
+      const int next = warps * kLanes;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4* b4 = reinterpret_cast<const float4*>(bs + (4 * g + j) * kRow);
-        float hv = h0[j];
-#pragma unroll
-        for (int t = 0; t < kTok / 4; ++t) {
-          const float4 bv = b4[t];
-          const float2 v0 = __fmul2_rn(du[2 * t], make_float2(bv.x, bv.y)), v1 = __fmul2_rn(du[2 * t + 1], make_float2(bv.z, bv.w));
-          h[j][4 * t] = fmaf(a[j][4 * t], hv, v0.x);
-          h[j][4 * t + 1] = fmaf(a[j][4 * t + 1], h[j][4 * t], v0.y);
-          h[j][4 * t + 2] = fmaf(a[j][4 * t + 2], h[j][4 * t + 1], v1.x);
-          hv = h[j][4 * t + 3] = fmaf(a[j][4 * t + 3], h[j][4 * t + 2], v1.y);
+      for (int t = kBlock / 4 - 1; t >= 0; --t) {
+        const float4 s = step[t * kLanes], u = du[t * kLanes], gv = gy[t * kLanes];
+        float2 y0 = twice(0.0f), y1 = y0, b0 = y0, b1 = y0, w0 = y0, w1 = y0;
+        if (!SUM && g > 0) {
+          const float4 py = part[3 * t * next], pb = part[(3 * t + 1) * next], pw = part[(3 * t + 2) * next];
+          y0 = make_float2(py.x, py.y), y1 = make_float2(py.z, py.w), b0 = make_float2(pb.x, pb.y), b1 = make_float2(pb.z, pb.w);
+          w0 = make_float2(pw.x, pw.y), w1 = make_float2(pw.z, pw.w);
         }
-      }
-      const float4 da = das[g * kLanes];
-      float2 da2[4] = {{da.x, 0.0f}, {da.y, 0.0f}, {da.z, 0.0f}, {da.w, 0.0f}};
-      float sums[kTok], back[4] = {back4.x, back4.y, back4.z, back4.w};
+        float v[16];  // [dB, dC][state][token]
 #pragma unroll
-      for (int t = kTok / 2 - 1; t >= 0; --t) {
-        float lo[8], hi[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 bv = *reinterpret_cast<const float2*>(bs + (4 * g + j) * kRow + 2 * t);
-          const float2 cv = *reinterpret_cast<const float2*>(cs + (4 * g + j) * kRow + 2 * t);
-          const float2 cg = __fmul2_rn(cv, gy[t]), hv = make_float2(h[j][2 * t], h[j][2 * t + 1]);
-          float2 dh, rr;
-          dh.y = cg.y + back[j];
-          rr.y = a[j][2 * t + 1] * dh.y;
-          dh.x = cg.x + rr.y;
-          rr.x = back[j] = a[j][2 * t] * dh.x;
-          const float2 wt = make_float2(rr.x * (t ? h[j][2 * t - 1] : h0[j]), rr.y * h[j][2 * t]);
-          y[t] = __ffma2_rn(cv, hv, y[t]);
-          sb[t] = __ffma2_rn(bv, dh, sb[t]);
-          sa[t] = __ffma2_rn(twice(rt[j]), wt, sa[t]);
-          da2[j] = __ffma2_rn(step[t], wt, da2[j]);
-          const float2 vb = __fmul2_rn(dh, du[t]), vc = __fmul2_rn(gy[t], hv);
-          lo[j] = vb.x, hi[j] = vb.y, lo[4 + j] = vc.x, hi[4 + j] = vc.y;
+        for (int j = 0; j < 2; ++j) {
+          const float4 cv = *reinterpret_cast<const float4*>(cs + j * kRow + 4 * t);
+          const float2 c0 = make_float2(cv.x, cv.y), c1 = make_float2(cv.z, cv.w);
+          const float2 g0 = make_float2(gv.x, gv.y), g1 = make_float2(gv.z, gv.w);
+          const float2 cg0 = __fmul2_rn(c0, g0), cg1 = __fmul2_rn(c1, g1);
+          float2 d0, d1, r0, r1;
+          d1.y = cg1.y + back[g][j];
+          r1.y = a[j][4 * t + 3] * d1.y;
+          d1.x = cg1.x + r1.y;
+          r1.x = a[j][4 * t + 2] * d1.x;
+          d0.y = cg0.y + r1.x;
+          r0.y = a[j][4 * t + 1] * d0.y;
+          d0.x = cg0.x + r0.y;
+          r0.x = back[g][j] = a[j][4 * t] * d0.x;
+          if (SUM) continue;
+          const float4 bv = *reinterpret_cast<const float4*>(bs + j * kRow + 4 * t);
+          const float2 h01 = make_float2(h[j][4 * t], h[j][4 * t + 1]), h23 = make_float2(h[j][4 * t + 2], h[j][4 * t + 3]);
+          r0.x *= t ? h[j][t ? 4 * t - 1 : 0] : h0[j];  // w
+          r0.y *= h01.x, r1.x *= h01.y, r1.y *= h23.x;
+          y0 = __ffma2_rn(c0, h01, y0), y1 = __ffma2_rn(c1, h23, y1);
+          b0 = __ffma2_rn(make_float2(bv.x, bv.y), d0, b0), b1 = __ffma2_rn(make_float2(bv.z, bv.w), d1, b1);
+          w0 = __ffma2_rn(twice(rt[g][j]), r0, w0), w1 = __ffma2_rn(twice(rt[g][j]), r1, w1);
+          da2[j] = __ffma2_rn(make_float2(s.x, s.y), r0, da2[j]);
+          da2[j] = __ffma2_rn(make_float2(s.z, s.w), r1, da2[j]);
+          const float2 vb0 = __fmul2_rn(d0, make_float2(u.x, u.y)), vb1 = __fmul2_rn(d1, make_float2(u.z, u.w));
+          const float2 vc0 = __fmul2_rn(g0, h01), vc1 = __fmul2_rn(g1, h23);
+          v[4 * j] = vb0.x, v[4 * j + 1] = vb0.y, v[4 * j + 2] = vb1.x, v[4 * j + 3] = vb1.y;
+          v[8 + 4 * j] = vc0.x, v[9 + 4 * j] = vc0.y, v[10 + 4 * j] = vc1.x, v[11 + 4 * j] = vc1.y;
         }
-        halve<4>(lo, 16, lane & 16), halve<4>(hi, 16, lane & 16);
-        halve<2>(lo, 8, lane & 8), halve<2>(hi, 8, lane & 8);
-        halve<1>(lo, 4, lane & 4), halve<1>(hi, 4, lane & 4);
-        sums[2 * t] = lo[0], sums[2 * t + 1] = hi[0];
+        if (SUM) continue;
+        part[3 * t * next] = make_float4(y0.x, y0.y, y1.x, y1.y);
+        part[(3 * t + 1) * next] = make_float4(b0.x, b0.y, b1.x, b1.y);
+        part[(3 * t + 2) * next] = make_float4(w0.x, w0.y, w1.x, w1.y);
+        halve<8>(v, 16, lane & 16);
+        halve<4>(v, 8, lane & 8);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[4 * t + e] = v[e];
       }
-      das[g * kLanes] = make_float4(da2[0].x + da2[0].y, da2[1].x + da2[1].y, da2[2].x + da2[2].y, da2[3].x + da2[3].y);
-      // a lane holds dB (lane < 16) or dC of state (lane >> 2) & 3, for all tokens,
-      // over a quarter of the lanes each
+      if (SUM) continue;
+      da[g][0] = __fadd2_rn(da[g][0], da2[0]), da[g][1] = __fadd2_rn(da[g][1], da2[1]);
+      // a lane holds dB (lane < 16) or dC of state (lane >> 3) & 1, for all tokens,
+      // over an eighth of the lanes each
+      halve<8>(sums, 4, lane & 4);
       halve<4>(sums, 2, lane & 2);
       halve<2>(sums, 1, lane & 1);
-      {
-        const int t = (lane & 2 ? 4 : 0) + (lane & 1 ? 2 : 0);
-        float* to = rows + (t * 2 + (lane >> 4)) * p.np + 4 * g + ((lane >> 2) & 3);
-        to[0] = sums[0], to[2 * p.np] = sums[1];
-      }
-      if (w == 0 && i == 0 && live && p.ds0) {
-        float* ds0 = p.ds0 + ((long)b * p.D + d) * p.N + 4 * g;
+      const int t = t0 + mine;
+      float* to = bc + (long)g * 4 * warps * p.T + t;
+      if (t <= lastt) to[0] = sums[0];
+      if (t < lastt) to[1] = sums[1];
+    }
+    mark -= p.np * kLanes;
+    __syncthreads();
+    if (!SUM) finish(t0);
+    if (t0 > q.first) {
+      // finish() reads this block's steps and gradients of its own pairs, which
+      // are the pairs that prepare() overwrites
+      prepare(t0 - kBlock);
+      if (t0 - kBlock > q.first) prefetch(t0 - 2 * kBlock);
+    }
+    __syncthreads();
+  }
+  if (SUM) {
+    const long at = (long)q.unit * p.segs + q.seg;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (4 * g + j < p.N) ds0[j] = back[j];
-      }
-    }
-    __syncwarp();
-    {
-      float4* part = reinterpret_cast<float4*>(p.part_bc + ((long)unit * p.T + t0) * p.np * 2);
-      for (int e = lane; e < here * p.np / 2; e += 32) part[e] = reinterpret_cast<const float4*>(rows)[e];
-    }
-    if (live) {
-      const long at0 = ((long)b * p.T + t0) * p.D + d;
-      T* dx = static_cast<T*>(p.dx) + at0;
-      T* ddt = static_cast<T*>(p.ddt) + at0;
-      T* dz = z ? static_cast<T*>(p.dz) + at0 : nullptr;
+    for (int g = 0; g < GW; ++g)
 #pragma unroll
-      for (int t = 0; t < kTok / 2; ++t) {
-        auto pair = [&](int which) {
-          const T* at = in + which * kTile + 2 * t * kLanes + lane;
-          return make_float2(to_f32(at[0]), to_f32(at[kLanes]));
-        };
-        const float2 xv = pair(0);
-        const float2 gx = __ffma2_rn(step[t], sb[t], p.skip ? __fmul2_rn(twice(skip), gy[t]) : twice(0.0f));
-        float2 raw = __ffma2_rn(xv, sb[t], __fmul2_rn(sa[t], twice(0.6931471805599453f)));  // rate is A / ln 2
-        if (p.softplus) raw = __fmul2_rn(raw, sigmoid_of2(__fadd2_rn(pair(1), twice(bias))));
-        float2 gz = twice(0.0f);
-        if (z) {
-          const float2 v = pair(3), s = sigmoid_of2(v), full = p.skip ? __ffma2_rn(twice(skip), xv, y[t]) : y[t];
-          const float2 go = dout ? pair(2) : twice(0.0f), one = __ffma2_rn(v, make_float2(1.0f - s.x, 1.0f - s.y), twice(1.0f));
-          gz = __fmul2_rn(__fmul2_rn(go, full), __fmul2_rn(s, one));
-        }
-        if (2 * t < here) {
-          const long at = (long)(2 * t) * p.D;
-          dx[at] = from_f32<T>(gx.x), ddt[at] = from_f32<T>(raw.x);
-          if (z) dz[at] = from_f32<T>(gz.x);
-          dbias += raw.x, dskip = fmaf(gy[t].x, xv.x, dskip);
-        }
-        if (2 * t + 1 < here) {
-          const long at = (long)(2 * t + 1) * p.D;
-          dx[at] = from_f32<T>(gx.y), ddt[at] = from_f32<T>(raw.y);
-          if (z) dz[at] = from_f32<T>(gz.y);
-          dbias += raw.y, dskip = fmaf(gy[t].y, xv.y, dskip);
-        }
+      for (int j = 0; j < 2; ++j) {
+        const int n = 2 * (g * warps + w) + j;
+        if (n < p.np) p.seg_sums[(at * p.np + n) * kLanes + lane] = back[g][j];
       }
-    }
-    __syncwarp();
+    if (w == 0) p.seg_steps[at * kLanes + lane] = total / GW;
+    return;
   }
   float* sums = sm + l.sums;
   sums[w * kLanes + lane] = dskip;
-  sums[(kWarps + w) * kLanes + lane] = dbias;
+  sums[(warps + w) * kLanes + lane] = dbias;
   __syncthreads();
-  if (live) {
-    const long at = (long)b * peers + rank;
-    if (w < 2) {
-      float s = 0.0f;
-      for (int o = 0; o < kWarps; ++o) s += sums[(w * kWarps + o) * kLanes + lane];
-      p.part_ch[(at * 2 + w) * p.D + d] = s;
-    }
-    const float4* all = reinterpret_cast<const float4*>(sm + l.da) + lane;
-    for (int g = w; g < ng; g += kWarps) {
-      float4 s = all[g * kLanes];
-      for (int o = 1; o < kWarps; ++o) {
-        const float4 v = all[(o * ng + g) * kLanes];
-        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-      }
-      float* part = p.part_a + (at * p.D + d) * p.N + 4 * g;
-      const float v[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (4 * g + j < p.N) part[j] = v[j];
-    }
+  if (!q.live) return;
+  const long at = (long)q.b * p.segs + q.seg;
+  for (int k = w; k < 2; k += warps) {
+    float s = 0.0f;
+    for (int o = 0; o < warps; ++o) s += sums[(k * warps + o) * kLanes + lane];
+    p.part_ch[(at * 2 + k) * p.D + q.d] = s;
   }
-  if (Q) cluster_sync();  // no CTA leaves while another may still write to it
+#pragma unroll
+  for (int g = 0; g < GW; ++g)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int n = 2 * (g * warps + w) + j;
+      if (n >= p.N) continue;
+      p.part_a[(at * p.D + q.d) * p.N + n] = da[g][j].x + da[g][j].y;
+      if (q.seg == 0 && p.ds0) p.ds0[((long)q.b * p.D + q.d) * p.N + n] = back[g][j];
+    }
 }
 
-// dB and dC: the sums over a group's tiles of 32 channels, in their order.
+// dB and dC: the sums over a group's tiles of 32 channels, in their order.  A
+// thread has a token, so that the partial sums are read along the time.
 template <typename T>
 __global__ void __launch_bounds__(256) sum_tiles_kernel(const Problem p) {
-  const int np = p.np;
-  const long i = blockIdx.x * 256L + threadIdx.x;  // (b, t, group, which, state)
-  const long total = (long)p.B * p.T * p.G * 2 * np;
-  if (i >= total) return;
-  const int n = (int)(i % np);
-  long rest = i / np;
+  const long i = blockIdx.x * 256L + threadIdx.x;  // (b, group, state, which, t)
+  const long t = i % p.T;
+  long rest = i / p.T;
   const int which = (int)(rest % 2);
   rest /= 2;
+  const int n = (int)(rest % p.N);
+  rest /= p.N;
   const int group = (int)(rest % p.G);
-  rest /= p.G;
-  const long t = rest % p.T, b = rest / p.T;
-  if (n >= p.N) return;
-  const long row = 2L * np;
-  const float* part = p.part_bc + ((b * p.tiles + (long)group * p.per_group) * p.T + t) * row + which * np + n;
+  const long b = rest / p.G;
+  if (b >= p.B) return;
+  const long tile = (long)p.np * 2 * p.T;
+  const float* part = p.part_bc + (b * p.tiles + (long)group * p.per_group) * tile + ((long)n * 2 + which) * p.T + t;
   double s = 0.0;
-#pragma unroll 4
-  for (int k = 0; k < p.per_group; ++k) s += (double)part[k * p.T * row];
+#pragma unroll 8
+  for (int k = 0; k < p.per_group; ++k) s += (double)part[k * tile];
   static_cast<T*>(which ? p.dc : p.db)[((b * p.T + t) * p.G + group) * p.N + n] = from_f32<T>((float)s);
 }
 
@@ -432,37 +383,39 @@ struct StoreChannels {
   }
 };
 
-template <typename T>
+template <typename T, int GW, int MOST, bool ONE, int W, int K>
 int launch_backward(const Problem& p, cudaStream_t stream) {
-  const size_t smem = layout(p.np, sizeof(T)).total * sizeof(float);
-  const int q = backward_sharing(p);
-  LaunchScope scope(kKindSelectiveScan, stream, 4);
-  const int rc = q > 1 ? launch_shared(scan_backward_kernel<T, true>, p, q, 32 * kWarps, smem, stream)
-                       : launch_shared(scan_backward_kernel<T, false>, p, 1, 32 * kWarps, smem, stream);
-  if (rc) return rc;
-  const long sums = (long)p.B * p.T * p.G * 2 * p.np;
+  const int warps = ceil_div(p.N, 2 * GW);
+  const size_t smem = layout(warps, p.np).total * sizeof(float);
+  const unsigned ctas = (unsigned)((long)p.B * p.tiles * p.segs);
+  LaunchScope scope(kKindSelectiveScan, stream, p.segs > 1 ? 5 : 4);
+  if (p.segs > 1) {
+    GRU_CUDA_TRY(cudaFuncSetAttribute(scan_backward_kernel<T, GW, true, MOST, ONE, W, K>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    scan_backward_kernel<T, GW, true, MOST, ONE, W, K><<<ctas, 32 * warps, smem, stream>>>(p);
+    GRU_CUDA_TRY(cudaGetLastError());
+  }
+  GRU_CUDA_TRY(cudaFuncSetAttribute(scan_backward_kernel<T, GW, false, MOST, ONE, W, K>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  scan_backward_kernel<T, GW, false, MOST, ONE, W, K><<<ctas, 32 * warps, smem, stream>>>(p);
+  GRU_CUDA_TRY(cudaGetLastError());
+  const long sums = (long)p.B * p.T * p.G * 2 * p.N;
   sum_tiles_kernel<T><<<(unsigned)((sums + 255) / 256), 256, 0, stream>>>(p);
   GRU_CUDA_TRY(cudaGetLastError());
   const long an = (long)p.D * p.N;
-  if (const int rc = sum_parts(p.part_a, p.B * q, an, an, StoreF32{p.da}, stream)) return rc;
-  return sum_parts(p.part_ch, p.B * q, 2L * p.D, 2L * p.D, StoreChannels{p.dskip, p.dbias, p.D}, stream);
+  if (const int rc = sum_parts(p.part_a, p.B * p.segs, an, an, StoreF32{p.da}, stream)) return rc;
+  return sum_parts(p.part_ch, p.B * p.segs, 2L * p.D, 2L * p.D, StoreChannels{p.dskip, p.dbias, p.D}, stream);
+}
+
+template <typename T>
+int backward_of(const Problem& p, cudaStream_t stream) {
+  if (p.N <= 14) return launch_backward<T, 1, 256, false, 0, 2>(p, stream);
+  if (p.N <= 16) return launch_backward<T, 1, 256, true, 8, 1>(p, stream);
+  return p.N <= 32 ? launch_backward<T, 1, 512, true, 0, 2>(p, stream) : launch_backward<T, 2, 512, true, 0, 4>(p, stream);
 }
 
 }  // namespace
 
-int backward_sharing(const Problem& p) { return sharing(p, (p.T + kBlock - 1) / kBlock, kResident); }
-
-int read_backward_status(int reset, int* status) {
-  GRU_CUDA_TRY(cudaMemcpyFromSymbol(status, g_backward_status, sizeof(int)));
-  if (reset) {
-    const int zero = 0;
-    GRU_CUDA_TRY(cudaMemcpyToSymbol(g_backward_status, &zero, sizeof(int)));
-  }
-  return GRU_OK;
-}
-
 int backward(const Problem& p, int dtype, cudaStream_t stream) {
-  return dtype == GRU_F32 ? launch_backward<float>(p, stream) : launch_backward<bf16>(p, stream);
+  return dtype == GRU_F32 ? backward_of<float>(p, stream) : backward_of<bf16>(p, stream);
 }
 
 }  // namespace scan

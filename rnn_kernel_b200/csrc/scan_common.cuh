@@ -9,31 +9,35 @@ namespace scan {
 
 constexpr int kMaxStates = 64;
 constexpr int kLanes = 32;       // channels of a CTA, one a lane
-constexpr int kWarps = 4;        // warps of a CTA, neighbouring pieces of the time
-constexpr int kMark = 32;        // tokens between two states that the forward keeps for the gradient
+constexpr int kBlock = 16;       // tokens of a block
+constexpr int kRow = kBlock + 4; // floats between two states' tokens in shared memory
 
 struct Problem {
   const void *x, *dt, *b, *c, *z;
   const float *a, *skip, *bias, *s0;
-  long xs[2], dts[2], zs[2], bs[3], cs[3];  // batch, token (, group)
+  long xb, dtb, zb, bb, cb, bg, cg;   // elements between batch rows, and groups
+  int xst, dtst, zst, bst, cst, ost;  // bytes between tokens; ost: of dense rows
   void* out;
   float* last;
-  float* marks;  // [B][tiles][mark][state, padded][32]: states at the tokens 0, kMark, ...
+  float* marks;  // [B][tiles][mark][state, padded][32]: states before each block
   // gradient
   const void* dout;
   const float* dlast;
   void *dx, *ddt, *dz, *db, *dc;
   float *da, *dskip, *dbias, *ds0;
-  float* part_bc;  // [B][tiles][T][2][padded N]
-  float* part_a;   // [B][CTA of a tile][D][N]
-  float* part_ch;  // [B][CTA of a tile][2][D]: of skip and dt_bias
+  float* part_bc;  // [B][tiles][padded N][dB, dC][T]
+  float* part_a;   // [B][segment][D][N]
+  float* part_ch;  // [B][segment][2][D]: of skip and dt_bias
+  // a segment's effect on a state that passes it: S or R, and its sum of steps
+  float* seg_sums;   // [B][tiles][segment][state, padded][32]
+  float* seg_steps;  // [B][tiles][segment][32]
   int B, T, D, N, G, R;  // R: channels of a group
   int softplus;
-  int pairs, dpairs;  // rows of x, dt and z, and of dout, lie on 4-byte boundaries
   int per_group, tiles;  // tiles of 32 channels in a group, and in all
   int np;                // states rounded up to a multiple of four
   int wide;              // log2 of the states rounded up to a power of two, at least 4
   int nmarks;
+  int segs, len;         // segments of the time, and their tokens (a multiple of kBlock)
 };
 
 __device__ __forceinline__ float exp2_of(float x) {
@@ -64,178 +68,108 @@ __device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
 // log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x|.  With s = e / (2 + e), at
 // most 1/3, log(1 + e) = 2 artanh(s) = 2 (s + s^3 / 3 + s^5 / 5 + ...), whose
 // terms after s^15 sum to less than 2^-26 of it: as exact for small e as for
-// large, in 2 special and some 10 packed operations (log1pf(expf(x)) takes about
-// 60, which made a third of the forward's instructions).
-__device__ __forceinline__ float2 softplus_of(float2 x) {
-  const float2 ax = make_float2(fminf(fabsf(x.x), 120.0f), fminf(fabsf(x.y), 120.0f));
-  const float2 t = __fmul2_rn(ax, twice(-1.4426950408889634f));
-  // what the exponent lost by its rounding
-  const float2 lost = __ffma2_rn(ax, twice(-1.4426950408889634f), make_float2(-t.x, -t.y));
-  float2 e = make_float2(exp2_of(t.x), exp2_of(t.y));
-  e = __ffma2_rn(e, __fmul2_rn(lost, twice(0.6931471805599453f)), e);
-  const float2 den = __fadd2_rn(e, twice(2.0f));
-  const float2 s = __fmul2_rn(e, make_float2(rcp_of(den.x), rcp_of(den.y))), q = __fmul2_rn(s, s);
-  float2 r = __ffma2_rn(q, twice(1.0f / 15.0f), twice(1.0f / 13.0f));
-  r = __ffma2_rn(q, r, twice(1.0f / 11.0f));
-  r = __ffma2_rn(q, r, twice(1.0f / 9.0f));
-  r = __ffma2_rn(q, r, twice(1.0f / 7.0f));
-  r = __ffma2_rn(q, r, twice(1.0f / 5.0f));
-  r = __ffma2_rn(q, r, twice(1.0f / 3.0f));
-  r = __ffma2_rn(__fmul2_rn(q, r), s, s);
-  return __ffma2_rn(twice(2.0f), r, make_float2(max_nan(x.x, 0.0f), max_nan(x.y, 0.0f)));
+// large, in 2 special and some 16 plain operations (log1pf(expf(x)) takes about 60,
+// which made a third of the forward's instructions).  Not packed: the constants
+// would have to be moved into pairs of registers.
+__device__ __forceinline__ float softplus_of(float x) {
+  const float ax = fminf(fabsf(x), 120.0f), t = ax * -1.4426950408889634f;
+  const float lost = fmaf(ax, -1.4426950408889634f, -t);  // of the exponent by its rounding
+  float e = exp2_of(t);
+  e = fmaf(e, lost * 0.6931471805599453f, e);
+  const float s = e * rcp_of(e + 2.0f), q = s * s;
+  float r = fmaf(q, 1.0f / 15.0f, 1.0f / 13.0f);
+  r = fmaf(q, r, 1.0f / 11.0f);
+  r = fmaf(q, r, 1.0f / 9.0f);
+  r = fmaf(q, r, 1.0f / 7.0f);
+  r = fmaf(q, r, 1.0f / 5.0f);
+  r = fmaf(q, r, 1.0f / 3.0f);
+  r = fmaf(q * r, s, s);
+  return fmaf(2.0f, r, max_nan(x, 0.0f));
 }
-// The step sizes of two raw values.
-__device__ __forceinline__ float2 step_of(int softplus, float2 raw, float bias) {
-  raw = __fadd2_rn(raw, twice(bias));
+// The step size of a raw value.
+__device__ __forceinline__ float step_of(int softplus, float raw, float bias) {
+  raw += bias;
   return softplus ? softplus_of(raw) : raw;
 }
-// 1 / (1 + e^-x), as sigmoid_of
-__device__ __forceinline__ float2 sigmoid_of2(float2 x) {
-  const float2 t = __fmul2_rn(x, twice(-1.4426950408889634f));
-  const float2 d = __fadd2_rn(make_float2(exp2_of(t.x), exp2_of(t.y)), twice(1.0f));
-  return make_float2(rcp_of(d.x), rcp_of(d.y));
+// 1 / (1 + e^-x), as sigmoid_of but for the last bits
+__device__ __forceinline__ float gate_of(float x) { return rcp_of(1.0f + exp2_of(x * -1.4426950408889634f)); }
+
+// The tile of 32 channels and the range of tokens of a CTA.
+struct Place {
+  int seg, unit, b, group, d, local;  // local: the lane's channel in its group
+  int first, end;                     // tokens
+  bool live;                          // the lane has a channel
+};
+__device__ __forceinline__ Place place(const Problem& p) {
+  Place q;
+  q.seg = blockIdx.x % p.segs, q.unit = blockIdx.x / p.segs;
+  const int tile = q.unit % p.tiles;
+  q.b = q.unit / p.tiles;
+  q.group = tile / p.per_group;
+  q.local = (tile - q.group * p.per_group) * kLanes + (threadIdx.x & 31);
+  q.live = q.local < p.R;
+  q.d = q.group * p.R + (q.live ? q.local : 0);
+  q.first = q.seg * p.len, q.end = min(q.first + p.len, p.T);
+  return q;
 }
 
-// ---- a warp's tokens of a tensor [token][channel], through shared memory ----
-
-__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// Waits for all but the last N issued.
-template <int N>
-__device__ __forceinline__ void copies_done() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Byte offset `token` rows of `stride` bytes on: one wide multiply-add.
+template <typename T>
+__device__ __forceinline__ T* row_at(T* base, int token, int stride) {
+  return reinterpret_cast<T*>(reinterpret_cast<uintptr_t>(base) + (long)token * stride);
 }
 
-// TOK tokens x 32 channels from src (the tile's first channel of the first token,
-// `stride` elements a token) to dst [TOK][32]; tokens from `here` on and channels
-// from `width` on read as zero.  `async`: rows lie on 4-byte boundaries and the
-// width fills 4-byte pieces, so the copy can run behind the warp's work (finished
-// by copies_done() and a __syncwarp()); otherwise it is done at once.
-template <typename T, int TOK>
-__device__ __forceinline__ void fetch_rows(const T* src, long stride, int here, int width, bool async, T* dst) {
-  const int lane = threadIdx.x & 31;
-  constexpr int kPer = 4 / sizeof(T), kLanesRow = kLanes / kPer, kRows = 32 / kLanesRow;
-  if (async) {
-    const int row = lane / kLanesRow, c = (lane % kLanesRow) * kPer;
-    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(dst + row * kLanes + c));
-#pragma unroll
-    for (int t = 0; t < TOK; t += kRows) {
-      const int at = t + row;
-      const bool in = at < here && c < width;
-      const T* from = in ? src + at * stride + c : src;
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + t * kLanes * (int)sizeof(T)), "l"(from),
-                   "r"(in ? 4 : 0)
-                   : "memory");
-    }
-  } else {
-#pragma unroll
-    for (int t = 0; t < TOK; ++t)
-      dst[t * kLanes + lane] = t < here && lane < width ? src[t * stride + lane] : from_f32<T>(0.0f);
+// Two neighbouring tokens of a lane's channel from src (the channel's first
+// token), as stored; the last token again where there are no more (a load without
+// a branch does not wait for its value).
+template <typename T>
+struct Pair {
+  T x, y;
+  __device__ __forceinline__ void load(const T* src, int stride, int t, int last) {
+    x = *row_at(src, min(t, last), stride);
+    y = *row_at(src, min(t + 1, last), stride);
   }
-}
-
-// A warp's rows of B and C [token][state], as FP32 by state: row n holds the
-// tokens, ROW floats apart; states from N on are zero.  load() leaves them in
-// registers, so that the loads run behind other work, up to store().
-template <typename T, int TOK, int ROW>
-struct FewRows {
-  static constexpr int kMost = TOK * kMaxStates / 32;
-  // states past the first 16 tokens x 16 are loaded and stored in turns
-  static constexpr int kHeld = TOK / 2;
-  T b[kHeld], c[kHeld];
-  __device__ __forceinline__ void at(const Problem& p, int i, int* t, int* n) const {
-    const int e = i * 32 + (threadIdx.x & 31);
-    *t = e >> p.wide, *n = e & ((1 << p.wide) - 1);
-  }
-  __device__ __forceinline__ void load(const Problem& p, const T* bm, const T* cm, int here, int first) {
+};
+// A block's B and C [token][state], K elements of each a thread at most, from
+// memory to rows of shared memory by state (kRow floats apart; states from N on and
+// tokens behind the last are zero).
+template <typename T, int K>
+struct Few {
+  const T *bm[K], *cm[K];  // this thread's state of the first token
+  int token[K], to[K];     // of a block; where in shared memory, or -1
+  T b[K], c[K];
+  __device__ __forceinline__ void init(const Problem& p, const T* bm0, const T* cm0) {
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      int t, n;
-      at(p, first + i, &t, &n);
-      const bool in = t < here && n < p.N;
-      b[i] = in ? bm[t * p.bs[1] + n] : from_f32<T>(0.0f);
-      c[i] = in ? cm[t * p.cs[1] + n] : from_f32<T>(0.0f);
+    for (int i = 0; i < K; ++i) {
+      const int e = threadIdx.x + i * blockDim.x, n = e & ((1 << p.wide) - 1);
+      token[i] = e >> p.wide;
+      to[i] = token[i] < kBlock && n < p.np ? n * kRow + token[i] : -1;
+      bm[i] = bm0 + min(n, p.N - 1), cm[i] = cm0 + min(n, p.N - 1);
+      if (n >= p.N) token[i] = 1 << 30;  // never there: zero
     }
   }
-  __device__ __forceinline__ void store(const Problem& p, float* bs, float* cs, int rows, int first) const {
+  __device__ __forceinline__ void load(const Problem& p, int t0, int last) {
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      int t, n;
-      at(p, first + i, &t, &n);
-      if (t < TOK && n < rows) bs[n * ROW + t] = to_f32(b[i]), cs[n * ROW + t] = to_f32(c[i]);
+    for (int i = 0; i < K; ++i) {
+      const int t = min(t0 + token[i], last);
+      b[i] = *row_at(bm[i], t, p.bst);
+      c[i] = *row_at(cm[i], t, p.cst);
     }
   }
-  // what does not fit the registers
-  __device__ __forceinline__ void rest(const Problem& p, const T* bm, const T* cm, int here, float* bs, float* cs, int rows) {
-    for (int first = kHeld; first * 32 < TOK << p.wide; first += kHeld) {
-      load(p, bm, cm, here, first);
-      store(p, bs, cs, rows, first);
-    }
+  __device__ __forceinline__ void store(float* bs, float* cs, int t0, int last) const {
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+      if (to[i] >= 0) {
+        const bool in = t0 + token[i] <= last;
+        bs[to[i]] = in ? to_f32(b[i]) : 0.0f;
+        cs[to[i]] = in ? to_f32(c[i]) : 0.0f;
+      }
   }
 };
 
-// ---- clusters: CTAs of one sequence and tile that take its blocks in turn ----
-
-__device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void bar_init(uint32_t bar) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// Eight bytes to another CTA's memory, counted by its barrier.
-__device__ __forceinline__ void send(uint32_t to, float2 v, uint32_t bar) {
-  const unsigned long long w = (unsigned long long)__float_as_uint(v.y) << 32 | __float_as_uint(v.x);
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(to), "l"(w), "r"(bar)
-               : "memory");
-}
-__device__ __forceinline__ bool bar_done(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Waits at most two seconds; after that the status word says so, the caller
-// waits no more, and the launch's results are invalid.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int* status) {
-  if (bar_done(bar, parity)) return true;
-  unsigned long long t0, t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-  for (;;) {
-    for (int i = 0; i < 64; ++i)
-      if (bar_done(bar, parity)) return true;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    if (t - t0 > 2000000000ull) {
-      atomicOr(status, GRU_STATUS_WAIT_TIMEOUT);
-      return false;
-    }
-  }
-}
+// Rows of four tokens, [quad][lane] float4: the float2 of tokens t and t + 1.
+__device__ __forceinline__ int pair_at(int t, int lane) { return ((t >> 2) * kLanes + lane) * 4 + (t & 2); }
+__device__ __forceinline__ float2& pair_in(float* rows, int at) { return *reinterpret_cast<float2*>(rows + at); }
 
 }  // namespace scan
 }  // namespace gru

@@ -53,10 +53,10 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const Problem p
     const bool in = d < p.D;
     const int group = in ? d / p.R : 0;
     const long db = in ? d : 0;
-    const float x = to_f32(static_cast<const T*>(p.x)[b * p.xs[0] + db]);
-    const float step = step_of(p.softplus, twice(to_f32(static_cast<const T*>(p.dt)[b * p.dts[0] + db])), p.bias ? p.bias[db] : 0.0f).x;
-    const T* bm = static_cast<const T*>(p.b) + b * p.bs[0] + group * p.bs[2] + n0;
-    const T* cm = static_cast<const T*>(p.c) + b * p.cs[0] + group * p.cs[2] + n0;
+    const float x = to_f32(static_cast<const T*>(p.x)[b * p.xb + db]);
+    const float step = step_of(p.softplus, to_f32(static_cast<const T*>(p.dt)[b * p.dtb + db]), p.bias ? p.bias[db] : 0.0f);
+    const T* bm = static_cast<const T*>(p.b) + b * p.bb + group * p.bg + n0;
+    const T* cm = static_cast<const T*>(p.c) + b * p.cb + group * p.cg + n0;
     float y = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const Problem p
     if (part == 0) {
       if (p.skip) y = fmaf(p.skip[d], x, y);
       if (p.z) {
-        const float gate = to_f32(static_cast<const T*>(p.z)[b * p.zs[0] + d]);
+        const float gate = to_f32(static_cast<const T*>(p.z)[b * p.zb + d]);
         y *= gate * sigmoid_of(gate);
       }
       static_cast<T*>(p.out)[(long)b * p.D + d] = from_f32<T>(y);
@@ -125,6 +125,9 @@ int check(const char* me, const gru_scan_args* p, Needs needs) {
       (bits(p->a) | bits(p->skip) | bits(p->dt_bias) | bits(p->initial_state)) & 3)
     return refuse(me, "a tensor is not aligned to its element size");
   if (needs == kInputs && p->B > 0 && p->T > 0 && (!p->x || !p->dt || !p->b || !p->c || !p->a)) return refuse(me, "null tensor");
+  for (const long s : {p->x_stride[1], p->dt_stride[1], p->z_stride[1], p->b_stride[1], p->c_stride[1]})
+    if (s < 0 || s * (long)es > 0x7fffffffL)
+      return refuse(me, "tokens must be less than 2^31 bytes apart", GRU_ERR_UNSUPPORTED);
   const double tiles = (double)p->G * ((p->D / p->G + kLanes - 1) / kLanes);
   if (p->B * tiles > 2e9 || (double)p->B * p->D * 16 > 4e11 || (double)p->B * p->T * p->G > 4e9 || p->T > (1 << 30) ||
       p->D > (1 << 26))
@@ -135,26 +138,52 @@ int check(const char* me, const gru_scan_args* p, Needs needs) {
 void fill(Problem& a, const gru_scan_args& p) {
   a.x = p.x, a.dt = p.dt, a.b = p.b, a.c = p.c, a.z = p.z;
   a.a = p.a, a.skip = p.skip, a.bias = p.dt_bias, a.s0 = p.initial_state;
-  for (int i = 0; i < 2; ++i) a.xs[i] = p.x_stride[i], a.dts[i] = p.dt_stride[i], a.zs[i] = p.z_stride[i];
-  for (int i = 0; i < 3; ++i) a.bs[i] = p.b_stride[i], a.cs[i] = p.c_stride[i];
+  const int es = (int)elem_size(p.dtype);
+  a.xb = p.x_stride[0], a.dtb = p.dt_stride[0], a.zb = p.z_stride[0], a.bb = p.b_stride[0], a.cb = p.c_stride[0];
+  a.bg = p.b_stride[2], a.cg = p.c_stride[2];
+  a.xst = (int)(p.x_stride[1] * es), a.dtst = (int)(p.dt_stride[1] * es), a.zst = (int)(p.z_stride[1] * es);
+  a.bst = (int)(p.b_stride[1] * es), a.cst = (int)(p.c_stride[1] * es), a.ost = p.D * es;
   a.B = p.B, a.T = p.T, a.D = p.D, a.N = p.N, a.G = p.G, a.R = p.D / p.G;
   a.softplus = p.dt_softplus;
-  const int per = p.dtype == GRU_F32 ? 1 : 2;
-  a.pairs = ((bits(p.x) | bits(p.dt) | bits(p.z)) & 3) == 0 && a.R % per == 0;
-  for (int i = 0; i < 2; ++i) a.pairs = a.pairs && p.x_stride[i] % per == 0 && p.dt_stride[i] % per == 0 && p.z_stride[i] % per == 0;
   a.per_group = ceil_div(a.R, kLanes), a.tiles = a.per_group * a.G;
   a.np = ceil_div(a.N, 4) * 4;
   a.wide = 2;
   while ((1 << a.wide) < a.N) ++a.wide;
-  a.nmarks = ceil_div(a.T, kMark);
+  a.nmarks = ceil_div(a.T, kBlock);
+}
+
+// Segments of the time.  One pass of `full` warps an SM keeps it about
+// w / (w + 8) busy with w of them; more than one segment costs a first pass of some
+// 0.7 of the work over all but one of them.
+void cut(Problem& a, int full) {
+  const double beside = (double)a.B * a.tiles * ceil_div(a.N, a.N <= 32 ? 2 : 4) / 148.0;
+  double best = 0.0;
+  a.segs = 1;
+  for (int s = 1; s <= 64 && (s == 1 || a.T / s >= 4 * kBlock); s *= 2) {
+    const double w = std::min(beside * s, (double)full);
+    const double cost = (1.0 + 0.7 * (s - 1) / s) * (w + 8.0) / w;
+    if (s == 1 || cost < 0.95 * best) best = cost, a.segs = s;
+  }
+  a.len = ceil_div(ceil_div(a.T, a.segs), kBlock) * kBlock;
+  a.segs = std::max(1, ceil_div(a.T, a.len > 0 ? a.len : 1));
 }
 
 void lay_marks(Problem& a, Pieces& m) { a.marks = m.floats((size_t)a.B * a.tiles * a.nmarks * a.np * kLanes); }
-void lay_parts(Problem& a, Pieces& m) {
+void lay_segments(Problem& a, Pieces& m) {
+  const size_t n = a.segs > 1 ? (size_t)a.B * a.tiles * a.segs * kLanes : 0;
+  a.seg_sums = m.floats(n * a.np);
+  a.seg_steps = m.floats(n);
+}
+void lay_forward(Problem& a, Pieces& m) {
+  cut(a, 24);
+  lay_segments(a, m);
+}
+void lay_backward(Problem& a, Pieces& m) {
+  cut(a, 16);
+  lay_segments(a, m);
   a.part_bc = m.floats((size_t)a.B * a.tiles * a.T * 2 * a.np);
-  const size_t q = backward_sharing(a);
-  a.part_a = m.floats(q * a.B * a.D * a.N);
-  a.part_ch = m.floats(q * a.B * 2 * a.D);
+  a.part_a = m.floats((size_t)a.segs * a.B * a.D * a.N);
+  a.part_ch = m.floats((size_t)a.segs * a.B * 2 * a.D);
 }
 
 }  // namespace
@@ -173,17 +202,18 @@ extern "C" size_t gru_scan_stash_bytes(const gru_scan_args* p) {
   return m.used;
 }
 
-extern "C" size_t gru_scan_workspace_bytes(const gru_scan_args* p) {
+extern "C" size_t gru_scan_workspace_bytes(const gru_scan_args* p, int backward) {
   if (check("gru_scan_workspace_bytes", p, kSizesOnly)) return 0;
   Problem a{};
   fill(a, *p);
   Pieces m{nullptr};
-  lay_parts(a, m);
+  if (backward) lay_backward(a, m);
+  else lay_forward(a, m);
   return m.used;
 }
 
 extern "C" int gru_scan_forward(const gru_scan_args* p, void* out, float* final_state, void* stash, size_t stash_bytes,
-                                void* stream_) {
+                                void* workspace, size_t workspace_bytes, void* stream_) {
   clear_error();
   const char* me = "gru_scan_forward";
   if (const int rc = check(me, p, kInputs)) return rc;
@@ -205,6 +235,10 @@ extern "C" int gru_scan_forward(const gru_scan_args* p, void* out, float* final_
     lay_marks(a, m);
     if (stash_bytes < m.used || bits(stash) & 15) return refuse(me, "stash too small or not 16-byte aligned");
   }
+  Pieces m{static_cast<char*>(workspace)};
+  lay_forward(a, m);
+  if (m.used && (!workspace || workspace_bytes < m.used || bits(workspace) & 15))
+    return refuse(me, "workspace too small or not 16-byte aligned");
   a.out = out, a.last = final_state;
   return forward(a, p->dtype, stream);
 }
@@ -236,11 +270,10 @@ extern "C" int gru_scan_backward(const gru_scan_args* p, const void* dout, const
   if (!dx || !ddt || !db || !dc || (p->z && !dz)) return refuse(me, "null gradient");
   Pieces m{static_cast<char*>(const_cast<void*>(stash))}, w{static_cast<char*>(workspace)};
   lay_marks(a, m);
-  lay_parts(a, w);
+  lay_backward(a, w);
   if (!stash || stash_bytes < m.used || !workspace || workspace_bytes < w.used || (bits(stash) | bits(workspace)) & 15)
     return refuse(me, "stash or workspace too small or not 16-byte aligned");
   a.dout = dout, a.dlast = dfinal;
-  a.dpairs = (bits(dout) & 3) == 0 && (p->dtype == GRU_F32 || p->D % 2 == 0);
   a.dx = dx, a.ddt = ddt, a.da = da, a.db = db, a.dc = dc, a.dskip = dskip, a.dz = dz, a.dbias = ddt_bias, a.ds0 = dinitial;
   return backward(a, p->dtype, stream);
 }

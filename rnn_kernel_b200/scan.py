@@ -46,6 +46,12 @@ def _dense_last(t):
     return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _near(t):
+    """_dense_last of [B, T, ...], with tokens less than 2^31 bytes apart, as the scan asks for."""
+    t = _dense_last(t)
+    return t if t is None or t.stride(1) * t.element_size() < 1 << 31 else t.contiguous()
+
+
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
@@ -91,10 +97,10 @@ def _check(name, x, dt, A, B, C, skip, z, dt_bias, state, lead):
 
 @functools.lru_cache(maxsize=4096)
 def _sizes(code, B, T, D, N, G):
-    """Bytes of the stash and of the backward's workspace."""
+    """Bytes of the stash, the forward's workspace and the backward's."""
     lib = _lib.load()
     a = _lib.SCAN_ARGS.pack(code, B, T, D, N, G, 0, *[0] * 21)
-    return lib.gru_scan_stash_bytes(a), lib.gru_scan_workspace_bytes(a)
+    return lib.gru_scan_stash_bytes(a), lib.gru_scan_workspace_bytes(a, 0), lib.gru_scan_workspace_bytes(a, 1)
 
 
 def _args(code, softplus, x, dt, A, B, C, skip, z, dt_bias, state):
@@ -107,15 +113,17 @@ def _args(code, softplus, x, dt, A, B, C, skip, z, dt_bias, state):
 
 def _scan_forward(code, dev, x, dt, A, B, C, skip, z, dt_bias, softplus, state, train):
     """out, the last state, the inputs as they were read and, to train, what the gradient needs besides them."""
-    x, dt, B, C, z = (_dense_last(t) for t in (x, dt, B, C, z))
+    x, dt, B, C, z = (_near(t) for t in (x, dt, B, C, z))
     A, skip, dt_bias, state = (_dense(t) for t in (A, skip, dt_bias, state))
     (b, T, D), (_, N) = x.shape, A.shape
     with _lib.on_device(dev):
         out, last = x.new_empty((b, T, D)), A.new_empty((b, D, N))
-        stash_bytes = _sizes(code, b, T, D, N, B.shape[2])[0] if train else 0
+        stash_bytes, ws_bytes, _ = _sizes(code, b, T, D, N, B.shape[2])
         stash = A.new_empty(stash_bytes // 4) if train else None
+        ws = A.new_empty(ws_bytes // 4) if ws_bytes else None
         _lib.check(_lib.load().gru_scan_forward(_args(code, softplus, x, dt, A, B, C, skip, z, dt_bias, state), out.data_ptr(),
-                                                last.data_ptr(), _ptr(stash), stash_bytes, _lib.raw_stream(dev)), "gru_scan_forward")
+                                                last.data_ptr(), _ptr(stash), stash_bytes if train else 0, _ptr(ws), ws_bytes,
+                                                _lib.raw_stream(dev)), "gru_scan_forward")
     return out, last, (x, dt, A, B, C, skip, z, dt_bias, stash)
 
 
@@ -136,7 +144,7 @@ class SelectiveScanFunction(torch.autograd.Function):
         x, dt, A, B, C, skip, z, dt_bias, stash = ctx.saved_tensors
         (b, T, D), (_, N), G = x.shape, A.shape, B.shape[2]
         dev = x.get_device()
-        stash_bytes, ws_bytes = _sizes(ctx.code, b, T, D, N, G)
+        stash_bytes, _, ws_bytes = _sizes(ctx.code, b, T, D, N, G)
         with _lib.on_device(dev):
             dout, dlast = _dense(dout), _dense(dlast)
             dx, ddt = x.new_empty((b, T, D)), x.new_empty((b, T, D))
