@@ -10,6 +10,8 @@ namespace scan {
 constexpr int kMaxStates = 64;
 constexpr int kLanes = 32;       // channels of a CTA, one a lane
 constexpr int kBlock = 16;       // tokens of a block
+constexpr int kQuads = kBlock / 4;
+constexpr int kStates = 4;       // states of a warp
 constexpr int kRow = kBlock + 4; // floats between two states' tokens in shared memory
 
 struct Problem {
@@ -33,6 +35,7 @@ struct Problem {
   float* seg_steps;  // [B][tiles][segment][32]
   int B, T, D, N, G, R;  // R: channels of a group
   int softplus;
+  int wide_rows, wide_dout, wide_few;  // rows of x, dt and z, of dout, and of B and C lie on 16-byte boundaries
   int per_group, tiles;  // tiles of 32 channels in a group, and in all
   int np;                // states rounded up to a multiple of four
   int wide;              // log2 of the states rounded up to a power of two, at least 4
@@ -98,6 +101,7 @@ __device__ __forceinline__ float gate_of(float x) { return rcp_of(1.0f + exp2_of
 struct Place {
   int seg, unit, b, group, d, local;  // local: the lane's channel in its group
   int first, end;                     // tokens
+  int d0, width;                      // the tile's first channel, and its channels
   bool live;                          // the lane has a channel
 };
 __device__ __forceinline__ Place place(const Problem& p) {
@@ -108,7 +112,8 @@ __device__ __forceinline__ Place place(const Problem& p) {
   q.group = tile / p.per_group;
   q.local = (tile - q.group * p.per_group) * kLanes + (threadIdx.x & 31);
   q.live = q.local < p.R;
-  q.d = q.group * p.R + (q.live ? q.local : 0);
+  q.d0 = q.group * p.R + q.local - (int)(threadIdx.x & 31), q.width = min(p.R - (q.d0 - q.group * p.R), kLanes);
+  q.d = q.live ? q.group * p.R + q.local : q.d0;
   q.first = q.seg * p.len, q.end = min(q.first + p.len, p.T);
   return q;
 }
@@ -119,57 +124,77 @@ __device__ __forceinline__ T* row_at(T* base, int token, int stride) {
   return reinterpret_cast<T*>(reinterpret_cast<uintptr_t>(base) + (long)token * stride);
 }
 
-// Two neighbouring tokens of a lane's channel from src (the channel's first
-// token), as stored; the last token again where there are no more (a load without
-// a branch does not wait for its value).
-template <typename T>
-struct Pair {
-  T x, y;
-  __device__ __forceinline__ void load(const T* src, int stride, int t, int last) {
-    x = *row_at(src, min(t, last), stride);
-    y = *row_at(src, min(t + 1, last), stride);
-  }
-};
-// A block's B and C [token][state], K elements of each a thread at most, from
-// memory to rows of shared memory by state (kRow floats apart; states from N on and
-// tokens behind the last are zero).
-template <typename T, int K>
-struct Few {
-  const T *bm[K], *cm[K];  // this thread's state of the first token
-  int token[K], to[K];     // of a block; where in shared memory, or -1
-  T b[K], c[K];
-  __device__ __forceinline__ void init(const Problem& p, const T* bm0, const T* cm0) {
-#pragma unroll
-    for (int i = 0; i < K; ++i) {
-      const int e = threadIdx.x + i * blockDim.x, n = e & ((1 << p.wide) - 1);
-      token[i] = e >> p.wide;
-      to[i] = token[i] < kBlock && n < p.np ? n * kRow + token[i] : -1;
-      bm[i] = bm0 + min(n, p.N - 1), cm[i] = cm0 + min(n, p.N - 1);
-      if (n >= p.N) token[i] = 1 << 30;  // never there: zero
-    }
-  }
-  __device__ __forceinline__ void load(const Problem& p, int t0, int last) {
-#pragma unroll
-    for (int i = 0; i < K; ++i) {
-      const int t = min(t0 + token[i], last);
-      b[i] = *row_at(bm[i], t, p.bst);
-      c[i] = *row_at(cm[i], t, p.cst);
-    }
-  }
-  __device__ __forceinline__ void store(float* bs, float* cs, int t0, int last) const {
-#pragma unroll
-    for (int i = 0; i < K; ++i)
-      if (to[i] >= 0) {
-        const bool in = t0 + token[i] <= last;
-        bs[to[i]] = in ? to_f32(b[i]) : 0.0f;
-        cs[to[i]] = in ? to_f32(c[i]) : 0.0f;
-      }
-  }
-};
+// ---- a block's inputs, as stored, in shared memory --------------------------------
 
-// Rows of four tokens, [quad][lane] float4: the float2 of tokens t and t + 1.
-__device__ __forceinline__ int pair_at(int t, int lane) { return ((t >> 2) * kLanes + lane) * 4 + (t & 2); }
-__device__ __forceinline__ float2& pair_in(float* rows, int at) { return *reinterpret_cast<float2*>(rows + at); }
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+               "l"(from)
+               : "memory");
+}
+// This thread's copies are there (other threads' after a barrier).
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Tokens t0 .. t0 + 15 of a tile's channels, from src (its first channel at token
+// 0), to dst [token][32]; the last token again where there are no more.  Pieces of
+// 16 bytes that arrive behind the CTA's work where all rows lie on their boundaries
+// (wide), elements otherwise; channels from `width` on are not written.
+template <typename T>
+__device__ __forceinline__ void fetch_rows(T* dst, const T* src, int stride, int t0, int last, int width, bool wide) {
+  if (wide) {
+    constexpr int kPer = 16 / sizeof(T), kPieces = kLanes / kPer;
+    for (int e = threadIdx.x; e < kBlock * kPieces; e += blockDim.x) {
+      const int t = e / kPieces, c = (e % kPieces) * kPer;
+      if (c < width) copy16(dst + t * kLanes + c, row_at(src + c, min(t0 + t, last), stride));
+    }
+  } else {
+    for (int e = threadIdx.x; e < kBlock * kLanes; e += blockDim.x) {
+      const int t = e / kLanes, c = e % kLanes;
+      if (c < width) dst[e] = *row_at(src + c, min(t0 + t, last), stride);
+    }
+  }
+}
+// The same for N states of B or C: dst [token][N].
+template <typename T>
+__device__ __forceinline__ void fetch_few(T* dst, const T* src, int stride, int t0, int last, int N, bool wide) {
+  if (wide) {
+    const int pieces = N * (int)sizeof(T) / 16;
+    for (int e = threadIdx.x; e < kBlock * pieces; e += blockDim.x) {
+      const int t = e / pieces, c = (e - t * pieces) * (16 / (int)sizeof(T));
+      copy16(dst + t * N + c, row_at(src + c, min(t0 + t, last), stride));
+    }
+  } else {
+    for (int e = threadIdx.x; e < kBlock * N; e += blockDim.x) {
+      const int t = e / N;
+      dst[e] = *row_at(src + (e - t * N), min(t0 + t, last), stride);
+    }
+  }
+}
+// From there to FP32 rows by state (kRow floats apart): states from N on and tokens
+// behind the last are zero.
+template <typename T>
+__device__ __forceinline__ void turn_few(const Problem& p, const T* b, const T* c, float* bs, float* cs, int np, int left) {
+  for (int e = threadIdx.x; e < kBlock << p.wide; e += blockDim.x) {
+    const int t = e >> p.wide, n = e & ((1 << p.wide) - 1);
+    if (n >= np) continue;
+    const bool in = t < left && n < p.N;
+    bs[n * kRow + t] = in ? to_f32(b[t * p.N + n]) : 0.0f;
+    cs[n * kRow + t] = in ? to_f32(c[t * p.N + n]) : 0.0f;
+  }
+}
+// Four tokens of the lane's channel.
+template <typename T>
+__device__ __forceinline__ void quad_of(const T* rows, int u, int lane, float (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = to_f32(rows[(4 * u + i) * kLanes + lane]);
+}
+
+__device__ __forceinline__ float4 as4(const float (&v)[4]) { return make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ float2 lo(float4 v) { return make_float2(v.x, v.y); }
+__device__ __forceinline__ float2 hi(float4 v) { return make_float2(v.z, v.w); }
+__device__ __forceinline__ float4 add4(float4 a, float4 b) {
+  const float2 x = __fadd2_rn(lo(a), lo(b)), y = __fadd2_rn(hi(a), hi(b));
+  return make_float4(x.x, x.y, y.x, y.y);
+}
 
 }  // namespace scan
 }  // namespace gru

@@ -143,6 +143,14 @@ void fill(Problem& a, const gru_scan_args& p) {
   a.bg = p.b_stride[2], a.cg = p.c_stride[2];
   a.xst = (int)(p.x_stride[1] * es), a.dtst = (int)(p.dt_stride[1] * es), a.zst = (int)(p.z_stride[1] * es);
   a.bst = (int)(p.b_stride[1] * es), a.cst = (int)(p.c_stride[1] * es), a.ost = p.D * es;
+  auto on16 = [&](const void* at, const long* stride, int n) {
+    bool ok = (bits(at) & 15) == 0;
+    for (int i = 0; i < n; ++i) ok = ok && stride[i] * es % 16 == 0;
+    return ok;
+  };
+  a.wide_rows = on16(p.x, p.x_stride, 2) && on16(p.dt, p.dt_stride, 2) && (!p.z || on16(p.z, p.z_stride, 2)) &&
+                p.D / p.G * es % 16 == 0;
+  a.wide_few = on16(p.b, p.b_stride, 3) && on16(p.c, p.c_stride, 3) && p.N * es % 16 == 0;
   a.B = p.B, a.T = p.T, a.D = p.D, a.N = p.N, a.G = p.G, a.R = p.D / p.G;
   a.softplus = p.dt_softplus;
   a.per_group = ceil_div(a.R, kLanes), a.tiles = a.per_group * a.G;
@@ -156,7 +164,7 @@ void fill(Problem& a, const gru_scan_args& p) {
 // w / (w + 8) busy with w of them; more than one segment costs a first pass of some
 // 0.7 of the work over all but one of them.
 void cut(Problem& a, int full) {
-  const double beside = (double)a.B * a.tiles * ceil_div(a.N, a.N <= 32 ? 2 : 4) / 148.0;
+  const double beside = (double)a.B * a.tiles * (a.np / kStates) / 148.0;
   double best = 0.0;
   a.segs = 1;
   for (int s = 1; s <= 64 && (s == 1 || a.T / s >= 4 * kBlock); s *= 2) {
@@ -274,6 +282,7 @@ extern "C" int gru_scan_backward(const gru_scan_args* p, const void* dout, const
   if (!stash || stash_bytes < m.used || !workspace || workspace_bytes < w.used || (bits(stash) | bits(workspace)) & 15)
     return refuse(me, "stash or workspace too small or not 16-byte aligned");
   a.dout = dout, a.dlast = dfinal;
+  a.wide_dout = (bits(dout) & 15) == 0;  // its rows are D elements apart, as wide as wide_rows asks for
   a.dx = dx, a.ddt = ddt, a.da = da, a.db = db, a.dc = dc, a.dskip = dskip, a.dz = dz, a.dbias = ddt_bias, a.ds0 = dinitial;
   return backward(a, p->dtype, stream);
 }
