@@ -8,20 +8,19 @@
 //   dx_t = skip gy_t + dt_t sum_n B_t dh_t
 //   ddt_t = x_t sum_n B_t dh_t + sum_n A w_t,   w_t = dh_t a_t h_{t-1};   dA = sum_t dt_t w_t
 //
-// The forward's shape, backwards: a CTA owns 32 channels of one sequence, a lane
-// each, a warp four states, and goes over blocks of 16 tokens from the last to the
-// first.  The forward kept the state before each block; from it a warp computes its
-// states at eight tokens, with the decays, in registers, and then goes over the
-// tokens backwards, first for the later eight (for them it passes the earlier ones
-// once more: half an exponential, where twice as many kept states would cost as
-// much in memory traffic).  The warps' shares of y, sum_n B dh and sum_n A w meet in
-// shared memory, where each warp finishes four tokens.  Sums over channels are
-// butterflies over the lanes in which each round halves the values: 64 values (8
-// tokens, 4 states, dB and dC) take 62 exchanges and leave a lane two sums.  The
-// tiles' sums of dB and dC are added by a second launch, in a fixed order, as are
-// those over sequences of dA, dskip and dbias.  Segments as in the forward.
-// Bound by instructions, 8 of them per token, channel and state for the sums over
-// channels.
+// The forward's shape, backwards: a CTA owns 64 channels of one sequence, two a
+// lane, a warp two states (twice two above 32), and goes over blocks of 16 tokens
+// from the last to the first.  The forward kept the state before each block; from
+// it a warp computes its states at eight tokens, with the decays, in registers, and
+// then goes over the tokens backwards, first for the later eight (for them it passes
+// the earlier ones once more: half an exponential, where twice as many kept states
+// would cost as much in memory traffic).  The warps' shares of y, sum_n B dh and
+// sum_n A w meet in shared memory, where each warp finishes a token.  Sums over
+// channels: the lane's two, then butterflies over the lanes in which each round
+// halves the values: 32 values (8 tokens, 2 states, dB and dC) take 31 exchanges and
+// leave a lane one sum.  The tiles' sums of dB and dC are added by a second launch,
+// in a fixed order, as are those over sequences of dA, dskip and dbias.  Segments as
+// in the forward.  Bound by instructions, and by shared memory's wavefronts.
 
 #include <algorithm>
 
@@ -35,27 +34,26 @@ namespace {
 
 constexpr int kHalf = kBlock / 2;
 
-// Shared memory in floats.
+// Shared memory in floats; elem: bytes of an element.
 struct Lay {
   int step, du, gy, xs, sg, gz, bs, cs, part, marks, in, few, sums, total;
 };
-__host__ __device__ inline Lay layout(int warps, int N, int elem) {
-  const int np = warps * kStates;
+__host__ __device__ inline Lay layout(int warps, int np, int N, int elem) {
   Lay l;
   int n = 0;
-  l.step = n, n += kBlock * kLanes;
-  l.du = n, n += kBlock * kLanes;  // dt x
-  l.gy = n, n += kBlock * kLanes;  // gradient of y
-  l.xs = n, n += kBlock * kLanes;
-  l.sg = n, n += kBlock * kLanes;  // softplus'
-  l.gz = n, n += kBlock * kLanes;  // dout silu'(z)
+  l.step = n, n += kBlock * kTile;
+  l.du = n, n += kBlock * kTile;  // dt x
+  l.gy = n, n += kBlock * kTile;  // gradient of y
+  l.xs = n, n += kBlock * kTile;
+  l.sg = n, n += kBlock * kTile;  // softplus'
+  l.gz = n, n += kBlock * kTile;  // dout silu'(z)
   l.bs = n, n += np * kRow;
   l.cs = n, n += np * kRow;
-  l.part = n, n += warps * 3 * kBlock * kLanes;  // [quad][y, sum B dh, sum A w][warp][lane] float4
-  l.marks = n, n += np * kLanes;
-  l.in = n, n += 4 * kBlock * kLanes * elem / 4;
+  l.part = n, n += warps * 3 * kHalf * kTile;  // [pair of tokens][y, sum B dh, sum A w][warp][lane] float4
+  l.marks = n, n += np * kTile;
+  l.in = n, n += 4 * kBlock * kTile * elem / 4;
   l.few = n, n += 2 * kBlock * N * elem / 4;
-  l.sums = n, n += 2 * warps * kLanes;
+  l.sums = n, n += 2 * warps * kTile;
   l.total = n;
   return l;
 }
@@ -71,12 +69,13 @@ __device__ __forceinline__ void halve(float* v, int bit, bool upper) {
   }
 }
 
-// SUM: only what the segments hand back.  MOST and W as in the forward.
-template <typename T, bool SUM, int MOST, int W>
-__global__ void __launch_bounds__(MOST, MOST == 128 ? 3 : 1) scan_backward_kernel(const __grid_constant__ Problem p) {
+// GW: pairs of states of a warp.  SUM: only what the segments hand back.  MOST and W
+// as in the forward.
+template <typename T, int GW, bool SUM, int MOST, int W>
+__global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kernel(const __grid_constant__ Problem p) {
   extern __shared__ __align__(16) float sm[];
-  const int warps = W ? W : blockDim.x >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31, np = warps * kStates;
-  const Lay l = layout(warps, p.N, sizeof(T));
+  const int threads = W ? 32 * W : blockDim.x, warps = W ? W : threads >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Lay l = layout(warps, p.np, p.N, sizeof(T));
   const Place q = place(p);
   if (SUM && q.seg == 0) return;
   const T* x = static_cast<const T*>(p.x) + q.b * p.xb + q.d0;
@@ -84,66 +83,77 @@ __global__ void __launch_bounds__(MOST, MOST == 128 ? 3 : 1) scan_backward_kerne
   const T* z = p.z ? static_cast<const T*>(p.z) + q.b * p.zb + q.d0 : nullptr;
   const T* bm = static_cast<const T*>(p.b) + q.b * p.bb + q.group * p.bg;
   const T* cm = static_cast<const T*>(p.c) + q.b * p.cb + q.group * p.cg;
-  const long dense = (long)q.b * p.T * p.D + q.d;
   const T* dout = p.dout ? static_cast<const T*>(p.dout) + (long)q.b * p.T * p.D + q.d0 : nullptr;
-  const float bias = p.bias ? p.bias[q.d] : 0.0f, skip = p.skip ? p.skip[q.d] : 0.0f;
-  const int lastt = q.end - 1, n0 = kStates * w;
+  const long dense = (long)q.b * p.T * p.D + q.d;
+  const float2 bias = two_of(p.bias, q), skip = two_of(p.skip, q);
+  const int lastt = q.end - 1;
   T* in = reinterpret_cast<T*>(sm + l.in);
   T* few = reinterpret_cast<T*>(sm + l.few);
-  constexpr int kTile = kBlock * kLanes;
+  constexpr int kRows = kBlock * kTile;
+  Feed<T> feed;
+  feed.init(p, q, bm, cm);
   auto fetch = [&](int t0) {
-    fetch_rows(in, x, p.xst, t0, lastt, q.width, p.wide_rows);
-    fetch_rows(in + kTile, dt, p.dtst, t0, lastt, q.width, p.wide_rows);
-    if (z) fetch_rows(in + 2 * kTile, z, p.zst, t0, lastt, q.width, p.wide_rows);
-    if (dout) fetch_rows(in + 3 * kTile, dout, p.ost, t0, lastt, q.width, p.wide_rows && p.wide_dout);
-    fetch_few(few, bm, p.bst, t0, lastt, p.N, p.wide_few);
-    fetch_few(few + kBlock * p.N, cm, p.cst, t0, lastt, p.N, p.wide_few);
+    feed.row(in, x, p.xst, t0, lastt, q.width, true);
+    feed.row(in + kRows, dt, p.dtst, t0, lastt, q.width, true);
+    if (z) feed.row(in + 2 * kRows, z, p.zst, t0, lastt, q.width, true);
+    if (dout) feed.row(in + 3 * kRows, dout, p.ost, t0, lastt, q.width, p.wide_dout);
+    feed.bc(p, few, bm, cm, t0, lastt);
   };
   auto fetch_marks = [&](int t0) {
-    const float4* from = reinterpret_cast<const float4*>(p.marks + ((long)q.unit * p.nmarks + t0 / kBlock) * np * kLanes);
-    for (int e = threadIdx.x; e < np * kLanes / 4; e += blockDim.x) copy16(reinterpret_cast<float4*>(sm + l.marks) + e, from + e);
+    const float4* from = reinterpret_cast<const float4*>(p.marks + ((long)q.unit * p.nmarks + t0 / kBlock) * p.np * kTile);
+    for (int e = threadIdx.x; e < p.np * kTile / 4; e += threads) copy16(reinterpret_cast<float4*>(sm + l.marks) + e, from + e);
   };
   const int start = q.first + (lastt - q.first) / kBlock * kBlock;  // the last block
   fetch(start);
   if (!SUM) fetch_marks(start);
 
-  float rt[kStates], back[kStates], da[kStates];
+  // states 2 (g warps + w) and the next
+  float2 rt[GW][2], back[GW][2], da[GW][2];
 #pragma unroll
-  for (int j = 0; j < kStates; ++j) {
-    const bool in = q.live && n0 + j < p.N;
-    rt[j] = in ? decay_rate(p.a[(long)q.d * p.N + n0 + j]) : 0.0f;
-    back[j] = !SUM && in && p.dlast ? p.dlast[((long)q.b * p.D + q.d) * p.N + n0 + j] : 0.0f;
-    da[j] = 0.0f;
-  }
+  for (int g = 0; g < GW; ++g)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int n = 2 * (g * warps + w) + j;
+      const float2 a = two_of(p.a, q, n, p.N);
+      rt[g][j] = make_float2(decay_rate(a.x), decay_rate(a.y));
+      back[g][j] = SUM ? twice(0.0f) : two_of(p.dlast ? p.dlast + (long)q.b * p.D * p.N : nullptr, q, n, p.N);
+      da[g][j] = twice(0.0f);
+    }
   if (!SUM)
     for (int s = p.segs - 1; s > q.seg; --s) {
       const long at = (long)q.unit * p.segs + s;
-      const float steps = p.seg_steps[at * kLanes + lane];
+      const float2 steps = both(p.seg_steps + at * kTile, 0, lane);
 #pragma unroll
-      for (int j = 0; j < kStates; ++j)
-        back[j] = fmaf(exp2_of(rt[j] * steps), back[j], p.seg_sums[(at * p.np + n0 + j) * kLanes + lane]);
+      for (int g = 0; g < GW; ++g)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int n = min(2 * (g * warps + w) + j, p.np - 1);
+          back[g][j] = __ffma2_rn(exp2_of(__fmul2_rn(rt[g][j], steps)), back[g][j],
+                                  both(p.seg_sums + (at * p.np + n) * kTile, 0, lane));
+        }
     }
 
-  float4* rows = reinterpret_cast<float4*>(sm) + lane;  // [array][quad][lane]
+  float4* rows = reinterpret_cast<float4*>(sm) + lane;  // [array][pair of tokens][lane]
   const int a_step = l.step / 4, a_du = l.du / 4, a_gy = l.gy / 4, a_xs = l.xs / 4, a_sg = l.sg / 4, a_gz = l.gz / 4;
   float4* shares = reinterpret_cast<float4*>(sm + l.part) + lane;
-  // What four tokens have per channel.
+  // What two tokens have per channel.
   auto prepare = [&](int t0) {
-    for (int u = w; u < kQuads; u += warps) {
-      const int t = t0 + 4 * u;
+    for (int u = w; u < kPairs; u += warps) {
+      const int t = t0 + 2 * u;
       float s[4], v[4], g[4] = {0.0f, 0.0f, 0.0f, 0.0f}, xv[4], sg[4], gz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      quad_of(in, u, lane, xv);
-      quad_of(in + kTile, u, lane, s);
-      if (dout) quad_of(in + 3 * kTile, u, lane, g);
+      four(in, u, lane, xv);
+      four(in + kRows, u, lane, s);
+      if (dout) four(in + 3 * kRows, u, lane, g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sg[i] = p.softplus ? gate_of(s[i] + bias) : 1.0f;
-        s[i] = step_of(p.softplus, s[i], bias);
+        const float bi = i & 1 ? bias.y : bias.x;
+        sg[i] = p.softplus ? gate_of(s[i] + bi) : 1.0f;
+        s[i] = step_of(p.softplus, s[i], bi);
         v[i] = s[i] * xv[i];
       }
       if (z) {
         float zv[4];
-        quad_of(in + 2 * kTile, u, lane, zv);
+        four(in + 2 * kRows, u, lane, zv);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float c = gate_of(zv[i]);
@@ -151,183 +161,170 @@ __global__ void __launch_bounds__(MOST, MOST == 128 ? 3 : 1) scan_backward_kerne
           g[i] *= zv[i] * c;
         }
       }
-      if (!q.live || t + 3 > lastt)
+      if (!q.second || t + 1 > lastt)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (!q.live || t + i > lastt) s[i] = v[i] = g[i] = 0.0f;
+          if (!(i & 1 ? q.second : q.live) || t + i / 2 > lastt) s[i] = v[i] = g[i] = 0.0f;
       float4* to = rows + u * kLanes;
       to[a_step] = as4(s), to[a_du] = as4(v), to[a_gy] = as4(g);
       if (!SUM) to[a_xs] = as4(xv), to[a_sg] = as4(sg), to[a_gz] = as4(gz);
       if (W) break;
     }
-    turn_few(p, few, few + kBlock * p.N, sm + l.bs, sm + l.cs, np, q.end - t0);
+    turn_few(p, few, sm + l.bs, sm + l.cs, p.np, q.end - t0);
   };
-  float dskip = 0.0f, dbias = 0.0f;
-  // Four tokens' sums over the states, and what follows from them.
-  auto finish_quad = [&](int u, int t) {
-    float4 sum[3];
+  float2 dskip = twice(0.0f), dbias = twice(0.0f);
+  // A half's tokens' sums over the states, and what follows from them; a token a warp.
+  auto finish = [&](int t0, int half) {
+    for (int e = w; e < kHalf; e += warps) {
+      const int t = t0 + half * kHalf + e;
+      if (t > lastt) break;
+      float2 sum[3];
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const float4* part = shares + (u * 3 + i) * warps * kLanes;
-      sum[i] = part[0];
+      for (int i = 0; i < 3; ++i) {
+        const float2* part = reinterpret_cast<const float2*>(shares + ((e / 2) * 3 + i) * warps * kLanes) + (e & 1);
+        sum[i] = part[0];
 #pragma unroll (W ? W : 4)
-      for (int k = 1; k < warps; ++k) sum[i] = add4(sum[i], part[k * kLanes]);
-    }
-    if (!q.live) return;
-    const float4* of = rows + u * kLanes;
-    const float4 s4 = of[a_step], g4 = of[a_gy], x4 = of[a_xs], sg4 = of[a_sg], gz4 = of[a_gz];
-    const float y[4] = {sum[0].x, sum[0].y, sum[0].z, sum[0].w}, sb[4] = {sum[1].x, sum[1].y, sum[1].z, sum[1].w};
-    const float sa[4] = {sum[2].x, sum[2].y, sum[2].z, sum[2].w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
-    const float g[4] = {g4.x, g4.y, g4.z, g4.w}, xv[4] = {x4.x, x4.y, x4.z, x4.w}, sg[4] = {sg4.x, sg4.y, sg4.z, sg4.w};
-    const float gz[4] = {gz4.x, gz4.y, gz4.z, gz4.w};
-    T* dx = row_at(static_cast<T*>(p.dx) + dense, t, p.ost);
-    T* ddt = row_at(static_cast<T*>(p.ddt) + dense, t, p.ost);
-    T* dz = z ? row_at(static_cast<T*>(p.dz) + dense, t, p.ost) : nullptr;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (t + i > lastt) break;
-      const float raw = fmaf(xv[i], sb[i], sa[i] * 0.6931471805599453f) * sg[i];  // rt is A / ln 2
-      *row_at(dx, i, p.ost) = from_f32<T>(fmaf(s[i], sb[i], p.skip ? skip * g[i] : 0.0f));
-      *row_at(ddt, i, p.ost) = from_f32<T>(raw);
-      if (z) *row_at(dz, i, p.ost) = from_f32<T>(gz[i] * (p.skip ? fmaf(skip, xv[i], y[i]) : y[i]));
-      dbias += raw, dskip = fmaf(g[i], xv[i], dskip);
-    }
-  };
-  auto finish = [&](int t0) {
-    for (int u = w; u < kQuads; u += warps) {
-      finish_quad(u, t0 + 4 * u);
-      if (W) break;
+        for (int k = 1; k < warps; ++k) sum[i] = __fadd2_rn(sum[i], part[2 * k * kLanes]);
+      }
+      auto of = [&](int a) {
+        return reinterpret_cast<const float2*>(rows + a + (half * (kHalf / 2) + e / 2) * kLanes)[e & 1];
+      };
+      const float2 s = of(a_step), g = of(a_gy), xv = of(a_xs), sg = of(a_sg);
+      const float2 y = sum[0], sb = sum[1], sa = sum[2];
+      const float2 raw = __fmul2_rn(__ffma2_rn(xv, sb, __fmul2_rn(sa, twice(0.6931471805599453f))), sg);  // rt is A / ln 2
+      const float2 gx = __ffma2_rn(s, sb, p.skip ? __fmul2_rn(skip, g) : twice(0.0f));
+      put_both(row_at(static_cast<T*>(p.dx) + dense, t, p.ost), gx.x, gx.y, q, p.even_out);
+      put_both(row_at(static_cast<T*>(p.ddt) + dense, t, p.ost), raw.x, raw.y, q, p.even_out);
+      if (z) {
+        const float2 dz = __fmul2_rn(of(a_gz), p.skip ? __ffma2_rn(skip, xv, y) : y);
+        put_both(row_at(static_cast<T*>(p.dz) + dense, t, p.ost), dz.x, dz.y, q, p.even_out);
+      }
+      dbias = __fadd2_rn(dbias, raw), dskip = __ffma2_rn(g, xv, dskip);
     }
   };
 
-  const float* bs = sm + l.bs + n0 * kRow;
-  const float* cs = sm + l.cs + n0 * kRow;
-  float total = 0.0f;
-  // the lanes' rows of partial sums
-  float* bc = p.part_bc + (((long)q.unit * p.np + n0 + ((lane >> 2) & 3)) * 2 + (lane >> 4)) * p.T;
-  const int mine = (lane & 2 ? 4 : 0) + (lane & 1 ? 2 : 0);
+  float2 total = twice(0.0f);
+  // the lanes' rows of partial sums, and their token of a half
+  float* bc = p.part_bc + (((long)q.unit * p.np + 2 * w + ((lane >> 3) & 1)) * 2 + (lane >> 4)) * p.T;
   copies_done();
   __syncthreads();
   prepare(start);
   __syncthreads();
   for (int t0 = start; t0 >= q.first; t0 -= kBlock) {
     const bool more = t0 > q.first;
-    // what a quad's tokens make of the warp's states; their decays and states are kept at a, h
-    float a[kStates][kHalf], h[kStates][kHalf];
-    auto scan = [&](int t, float (&st)[kStates], bool keep, int at) {
-      const float4 s = rows[a_step + t * kLanes], u = rows[a_du + t * kLanes];
-#pragma unroll
-      for (int j = 0; j < kStates; ++j) {
-        const float4 bv = *reinterpret_cast<const float4*>(bs + j * kRow + 4 * t);
-        const float2 e0 = __fmul2_rn(lo(s), twice(rt[j])), e1 = __fmul2_rn(hi(s), twice(rt[j]));
-        const float2 v0 = __fmul2_rn(lo(u), lo(bv)), v1 = __fmul2_rn(hi(u), hi(bv));
-        const float c[4] = {exp2_of(e0.x), exp2_of(e0.y), exp2_of(e1.x), exp2_of(e1.y)}, v[4] = {v0.x, v0.y, v1.x, v1.y};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          st[j] = fmaf(c[i], st[j], v[i]);
-          if (keep) a[j][at + i] = c[i], h[j][at + i] = st[j];
-        }
-      }
-    };
-    float h0[kStates];
-    if (!SUM) {
-#pragma unroll
-      for (int j = 0; j < kStates; ++j) h0[j] = sm[l.marks + (n0 + j) * kLanes + lane];
-    }
     if (more) fetch(t0 - kBlock);
-#pragma unroll
+#pragma unroll 1
     for (int half = 1; half >= 0; --half) {
-      constexpr int kQ = kHalf / 4;
-      float before[kStates];  // the state before these tokens
-      if (!SUM) {
-        float st[kStates];
 #pragma unroll
-        for (int j = 0; j < kStates; ++j) st[j] = h0[j];
-        if (half)
-#pragma unroll
-          for (int t = 0; t < kQ; ++t) scan(t, st, false, 0);
-#pragma unroll
-        for (int j = 0; j < kStates; ++j) before[j] = st[j];
-#pragma unroll
-        for (int t = 0; t < kQ; ++t) scan(half * kQ + t, st, true, 4 * t);
-      }
-      float sums[kHalf];
-      float2 da2[kStates];
-#pragma unroll
-      for (int j = 0; j < kStates; ++j) da2[j] = twice(0.0f);
-#pragma unroll
-      for (int tt = kQ - 1; tt >= 0; --tt) {
-        const int t = half * kQ + tt;
-        const float4 s = rows[a_step + t * kLanes], gv = rows[a_gy + t * kLanes];
+      for (int g = 0; g < GW; ++g) {
+        const int n0 = 2 * (g * warps + w);
+        if (GW > 1 && n0 >= p.np) continue;  // no such states: nothing to add
+        const float* bs = sm + l.bs + n0 * kRow;
+        const float* cs = sm + l.cs + n0 * kRow;
+        const float4* step = rows + a_step + half * (kHalf / 2) * kLanes;
         if (SUM) {
-          total += (s.x + s.y) + (s.z + s.w);
+          const float4* gy = rows + a_gy + half * (kHalf / 2) * kLanes;
 #pragma unroll
-          for (int j = 0; j < kStates; ++j) {
-            const float4 cv = *reinterpret_cast<const float4*>(cs + j * kRow + 4 * t);
-            back[j] = exp2_of(s.w * rt[j]) * fmaf(cv.w, gv.w, back[j]);
-            back[j] = exp2_of(s.z * rt[j]) * fmaf(cv.z, gv.z, back[j]);
-            back[j] = exp2_of(s.y * rt[j]) * fmaf(cv.y, gv.y, back[j]);
-            back[j] = exp2_of(s.x * rt[j]) * fmaf(cv.x, gv.x, back[j]);
+          for (int t = kHalf / 2 - 1; t >= 0; --t) {
+            const float4 s = step[t * kLanes], gv = gy[t * kLanes];
+            if (g == 0) total = __fadd2_rn(total, __fadd2_rn(lo(s), hi(s)));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float4 cv = *reinterpret_cast<const float4*>(cs + j * kRow + 4 * (half * (kHalf / 2) + t));
+              float2& r = back[g][j];
+              r = __fmul2_rn(exp2_of(__fmul2_rn(hi(s), rt[g][j])), __ffma2_rn(hi(cv), hi(gv), r));
+              r = __fmul2_rn(exp2_of(__fmul2_rn(lo(s), rt[g][j])), __ffma2_rn(lo(cv), lo(gv), r));
+            }
           }
           continue;
         }
-        const float4 u = rows[a_du + t * kLanes];
-        float2 y0 = twice(0.0f), y1 = y0, b0 = y0, b1 = y0, w0 = y0, w1 = y0;
-        float v[kStates * 4];  // [state][token]: of dB in the lower lanes, of dC in the upper
+        float2 a[2][kHalf], h[2][kHalf], before[2];
 #pragma unroll
-        for (int j = 0; j < kStates; ++j) {
-          const float4 cv = *reinterpret_cast<const float4*>(cs + j * kRow + 4 * t);
-          const float4 bv = *reinterpret_cast<const float4*>(bs + j * kRow + 4 * t);
-          const float* aj = &a[j][4 * tt];
-          const float2 h01 = make_float2(h[j][4 * tt], h[j][4 * tt + 1]), h23 = make_float2(h[j][4 * tt + 2], h[j][4 * tt + 3]);
-          const float2 g0 = __fmul2_rn(lo(cv), lo(gv)), g1 = __fmul2_rn(hi(cv), hi(gv));
-          float2 d0, d1, r0, r1;
-          d1.y = g1.y + back[j];
-          r1.y = aj[3] * d1.y;
-          d1.x = g1.x + r1.y;
-          r1.x = aj[2] * d1.x;
-          d0.y = g0.y + r1.x;
-          r0.y = aj[1] * d0.y;
-          d0.x = g0.x + r0.y;
-          r0.x = back[j] = aj[0] * d0.x;
-          r0.x *= tt ? h[j][tt ? 4 * tt - 1 : 0] : before[j];  // w
-          r0.y *= h01.x, r1.x *= h01.y, r1.y *= h23.x;
-          y0 = __ffma2_rn(lo(cv), h01, y0), y1 = __ffma2_rn(hi(cv), h23, y1);
-          b0 = __ffma2_rn(lo(bv), d0, b0), b1 = __ffma2_rn(hi(bv), d1, b1);
-          w0 = __ffma2_rn(twice(rt[j]), r0, w0), w1 = __ffma2_rn(twice(rt[j]), r1, w1);
-          da2[j] = __ffma2_rn(lo(s), r0, da2[j]);
-          da2[j] = __ffma2_rn(hi(s), r1, da2[j]);
-          const float2 vb0 = __fmul2_rn(d0, lo(u)), vb1 = __fmul2_rn(d1, hi(u));
-          const float2 vc0 = __fmul2_rn(lo(gv), h01), vc1 = __fmul2_rn(hi(gv), h23);
-          float m[8] = {vb0.x, vb0.y, vb1.x, vb1.y, vc0.x, vc0.y, vc1.x, vc1.y};
-          halve<4>(m, 16, lane & 16);
+        for (int j = 0; j < 2; ++j) before[j] = both(sm + l.marks + (n0 + j) * kTile, 0, lane);
+        if (half) {  // pass the earlier eight
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[4 * j + i] = m[i];
+          for (int t = 0; t < kHalf / 2; ++t) {
+            const float4 s = rows[a_step + t * kLanes], u = rows[a_du + t * kLanes];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float4 bv = *reinterpret_cast<const float4*>(bs + j * kRow + 4 * t);
+              before[j] = __ffma2_rn(exp2_of(__fmul2_rn(lo(s), rt[g][j])), before[j], __fmul2_rn(lo(u), lo(bv)));
+              before[j] = __ffma2_rn(exp2_of(__fmul2_rn(hi(s), rt[g][j])), before[j], __fmul2_rn(hi(u), hi(bv)));
+            }
+          }
         }
-        shares[(3 * t + 0) * warps * kLanes + w * kLanes] = make_float4(y0.x, y0.y, y1.x, y1.y);
-        shares[(3 * t + 1) * warps * kLanes + w * kLanes] = make_float4(b0.x, b0.y, b1.x, b1.y);
-        shares[(3 * t + 2) * warps * kLanes + w * kLanes] = make_float4(w0.x, w0.y, w1.x, w1.y);
-        halve<8>(v, 8, lane & 8);
-        halve<4>(v, 4, lane & 4);
+        bs += 4 * half * (kHalf / 2), cs += 4 * half * (kHalf / 2);
+        const float4* du = rows + a_du + half * (kHalf / 2) * kLanes;
+        const float4* gy = rows + a_gy + half * (kHalf / 2) * kLanes;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sums[4 * tt + i] = v[i];
+        for (int t = 0; t < kHalf / 2; ++t) {
+          const float4 s = step[t * kLanes], u = du[t * kLanes];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float4 bv = *reinterpret_cast<const float4*>(bs + j * kRow + 4 * t);
+            a[j][2 * t] = exp2_of(__fmul2_rn(lo(s), rt[g][j]));
+            a[j][2 * t + 1] = exp2_of(__fmul2_rn(hi(s), rt[g][j]));
+            h[j][2 * t] = __ffma2_rn(a[j][2 * t], t ? h[j][t ? 2 * t - 1 : 0] : before[j], __fmul2_rn(lo(u), lo(bv)));
+            h[j][2 * t + 1] = __ffma2_rn(a[j][2 * t + 1], h[j][2 * t], __fmul2_rn(hi(u), hi(bv)));
+          }
+        }
+        float sums[kHalf];
+        float2 da2[2] = {twice(0.0f), twice(0.0f)};  // of the half: short sums first
+#pragma unroll
+        for (int t = kHalf / 2 - 1; t >= 0; --t) {
+          const float4 s = step[t * kLanes], u = du[t * kLanes], gv = gy[t * kLanes];
+          float4* share = shares + (t * 3 * warps + w) * kLanes;
+          float2 y0 = twice(0.0f), y1 = y0, b0 = y0, b1 = y0, w0 = y0, w1 = y0;
+          if (g > 0) {
+            y0 = lo(share[0]), y1 = hi(share[0]), b0 = lo(share[warps * kLanes]), b1 = hi(share[warps * kLanes]);
+            w0 = lo(share[2 * warps * kLanes]), w1 = hi(share[2 * warps * kLanes]);
+          }
+          float v[8];  // [dB, dC][state][token]
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float4 cv = *reinterpret_cast<const float4*>(cs + j * kRow + 4 * t);
+            const float4 bv = *reinterpret_cast<const float4*>(bs + j * kRow + 4 * t);
+            const float2 h0 = h[j][2 * t], h1 = h[j][2 * t + 1], hb = t ? h[j][t ? 2 * t - 1 : 0] : before[j];
+            const float2 d1 = __ffma2_rn(hi(cv), hi(gv), back[g][j]);
+            const float2 r1 = __fmul2_rn(a[j][2 * t + 1], d1);
+            const float2 d0 = __ffma2_rn(lo(cv), lo(gv), r1);
+            back[g][j] = __fmul2_rn(a[j][2 * t], d0);
+            const float2 q1 = __fmul2_rn(r1, h0), q0 = __fmul2_rn(back[g][j], hb);  // w
+            y0 = __ffma2_rn(lo(cv), h0, y0), y1 = __ffma2_rn(hi(cv), h1, y1);
+            b0 = __ffma2_rn(lo(bv), d0, b0), b1 = __ffma2_rn(hi(bv), d1, b1);
+            w0 = __ffma2_rn(rt[g][j], q0, w0), w1 = __ffma2_rn(rt[g][j], q1, w1);
+            da2[j] = __ffma2_rn(lo(s), q0, da2[j]), da2[j] = __ffma2_rn(hi(s), q1, da2[j]);
+            v[2 * j] = fmaf(d0.y, u.y, d0.x * u.x), v[2 * j + 1] = fmaf(d1.y, u.w, d1.x * u.z);
+            v[4 + 2 * j] = fmaf(h0.y, gv.y, h0.x * gv.x), v[5 + 2 * j] = fmaf(h1.y, gv.w, h1.x * gv.z);
+          }
+          share[0] = as4(y0, y1), share[warps * kLanes] = as4(b0, b1), share[2 * warps * kLanes] = as4(w0, w1);
+          halve<4>(v, 16, lane & 16);
+          halve<2>(v, 8, lane & 8);
+          sums[2 * t] = v[0], sums[2 * t + 1] = v[1];
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) da[g][j] = __fadd2_rn(da[g][j], da2[j]);
+        // a lane holds dB (lane < 16) or dC of state (lane >> 3) & 1, for all eight
+        // tokens, over an eighth of the lanes each
+        halve<4>(sums, 4, lane & 4);
+        halve<2>(sums, 2, lane & 2);
+        halve<1>(sums, 1, lane & 1);
+        const int t = t0 + half * kHalf + (lane & 7);
+        if (t <= lastt) bc[(long)g * 4 * warps * p.T + t] = sums[0];
       }
       if (SUM) continue;
-#pragma unroll
-      for (int j = 0; j < kStates; ++j) da[j] += da2[j].x + da2[j].y;  // short sums first
-      // a lane holds dB (lane < 16) or dC of state (lane >> 2) & 3, for all eight
-      // tokens, over a quarter of the lanes each
-      halve<4>(sums, 2, lane & 2);
-      halve<2>(sums, 1, lane & 1);
-      const int t = t0 + half * kHalf + mine;
-      if (t <= lastt) bc[t] = sums[0];
-      if (t < lastt) bc[t + 1] = sums[1];
+      if (half == 0) copies_done();
+      __syncthreads();
+      finish(t0, half);
+      if (half) __syncthreads();
     }
-    copies_done();
-    __syncthreads();
-    if (!SUM && more) fetch_marks(t0 - kBlock);
-    if (!SUM) finish(t0);
-    // finish() reads the quads of this block that prepare() overwrites: the warp's own
+    if (SUM) {
+      copies_done();
+      __syncthreads();
+    } else if (more) {
+      fetch_marks(t0 - kBlock);
+    }
+    __syncthreads();  // finish() reads rows that prepare() overwrites
     if (more) prepare(t0 - kBlock);
     copies_done();
     __syncthreads();
@@ -335,31 +332,36 @@ __global__ void __launch_bounds__(MOST, MOST == 128 ? 3 : 1) scan_backward_kerne
   if (SUM) {
     const long at = (long)q.unit * p.segs + q.seg;
 #pragma unroll
-    for (int j = 0; j < kStates; ++j) p.seg_sums[(at * p.np + n0 + j) * kLanes + lane] = back[j];
-    if (w == 0) p.seg_steps[at * kLanes + lane] = total;
+    for (int g = 0; g < GW; ++g)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int n = 2 * (g * warps + w) + j;
+        if (n < p.np) *reinterpret_cast<float2*>(p.seg_sums + (at * p.np + n) * kTile + 2 * lane) = back[g][j];
+      }
+    if (w == 0) *reinterpret_cast<float2*>(p.seg_steps + at * kTile + 2 * lane) = total;
     return;
   }
-  float* sums = sm + l.sums;
-  sums[w * kLanes + lane] = dskip;
-  sums[(warps + w) * kLanes + lane] = dbias;
+  float2* sums = reinterpret_cast<float2*>(sm + l.sums) + lane;
+  sums[w * kLanes] = dskip;
+  sums[(warps + w) * kLanes] = dbias;
   __syncthreads();
-  if (!q.live) return;
   const long at = (long)q.b * p.segs + q.seg;
   for (int k = w; k < 2; k += warps) {
-    float s = 0.0f;
-    for (int o = 0; o < warps; ++o) s += sums[(k * warps + o) * kLanes + lane];
-    p.part_ch[(at * 2 + k) * p.D + q.d] = s;
+    float2 s = twice(0.0f);
+    for (int o = 0; o < warps; ++o) s = __fadd2_rn(s, sums[(k * warps + o) * kLanes]);
+    put_two(p.part_ch + (at * 2 + k) * p.D, q, 0, 1, s);
   }
 #pragma unroll
-  for (int j = 0; j < kStates; ++j) {
-    const int n = n0 + j;
-    if (n >= p.N) continue;
-    p.part_a[(at * p.D + q.d) * p.N + n] = da[j];
-    if (q.seg == 0 && p.ds0) p.ds0[((long)q.b * p.D + q.d) * p.N + n] = back[j];
-  }
+  for (int g = 0; g < GW; ++g)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int n = 2 * (g * warps + w) + j;
+      put_two(p.part_a + at * p.D * p.N, q, n, p.N, da[g][j]);
+      if (q.seg == 0 && p.ds0) put_two(p.ds0 + (long)q.b * p.D * p.N, q, n, p.N, back[g][j]);
+    }
 }
 
-// dB and dC: the sums over a group's tiles of 32 channels, in their order.  A
+// dB and dC: the sums over a group's tiles of 64 channels, in their order.  A
 // thread has a token, so that the partial sums are read along the time.
 template <typename T>
 __global__ void __launch_bounds__(256) sum_tiles_kernel(const Problem p) {
@@ -397,19 +399,19 @@ struct StoreChannels {
   }
 };
 
-template <typename T, int MOST, int W>
+template <typename T, int GW, int MOST, int W>
 int launch_backward(const Problem& p, cudaStream_t stream) {
-  const int warps = p.np / kStates;
-  const size_t smem = layout(warps, p.N, sizeof(T)).total * sizeof(float);
+  const int warps = p.np / (2 * GW);
+  const size_t smem = layout(warps, p.np, p.N, sizeof(T)).total * sizeof(float);
   const unsigned ctas = (unsigned)((long)p.B * p.tiles * p.segs);
   LaunchScope scope(kKindSelectiveScan, stream, p.segs > 1 ? 5 : 4);
   if (p.segs > 1) {
-    auto kernel = scan_backward_kernel<T, true, MOST, W>;
+    auto kernel = scan_backward_kernel<T, GW, true, MOST, W>;
     GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     kernel<<<ctas, 32 * warps, smem, stream>>>(p);
     GRU_CUDA_TRY(cudaGetLastError());
   }
-  auto kernel = scan_backward_kernel<T, false, MOST, W>;
+  auto kernel = scan_backward_kernel<T, GW, false, MOST, W>;
   GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   kernel<<<ctas, 32 * warps, smem, stream>>>(p);
   GRU_CUDA_TRY(cudaGetLastError());
@@ -423,8 +425,9 @@ int launch_backward(const Problem& p, cudaStream_t stream) {
 
 template <typename T>
 int backward_of(const Problem& p, cudaStream_t stream) {
-  if (p.np == 16) return launch_backward<T, 128, 4>(p, stream);
-  return p.np < 16 ? launch_backward<T, 128, 0>(p, stream) : launch_backward<T, 512, 0>(p, stream);
+  if (p.np == 16) return launch_backward<T, 1, 256, 8>(p, stream);
+  if (p.np < 16) return launch_backward<T, 1, 256, 0>(p, stream);
+  return p.np <= 32 ? launch_backward<T, 1, 512, 0>(p, stream) : launch_backward<T, 2, 512, 0>(p, stream);
 }
 
 }  // namespace

@@ -8,11 +8,11 @@ namespace gru {
 namespace scan {
 
 constexpr int kMaxStates = 64;
-constexpr int kLanes = 32;       // channels of a CTA, one a lane
+constexpr int kLanes = 32;
+constexpr int kTile = 64;        // channels of a CTA: two neighbours a lane
 constexpr int kBlock = 16;       // tokens of a block
-constexpr int kQuads = kBlock / 4;
-constexpr int kStates = 4;       // states of a warp
-constexpr int kRow = kBlock + 4; // floats between two states' tokens in shared memory
+constexpr int kPairs = kBlock / 2;
+constexpr int kRow = 2 * kBlock + 4;  // floats between two states' tokens in shared memory, each twice
 
 struct Problem {
   const void *x, *dt, *b, *c, *z;
@@ -21,7 +21,7 @@ struct Problem {
   int xst, dtst, zst, bst, cst, ost;  // bytes between tokens; ost: of dense rows
   void* out;
   float* last;
-  float* marks;  // [B][tiles][mark][state, padded][32]: states before each block
+  float* marks;  // [B][tiles][block][state, padded][64]: states before each block
   // gradient
   const void* dout;
   const float* dlast;
@@ -31,12 +31,13 @@ struct Problem {
   float* part_a;   // [B][segment][D][N]
   float* part_ch;  // [B][segment][2][D]: of skip and dt_bias
   // a segment's effect on a state that passes it: S or R, and its sum of steps
-  float* seg_sums;   // [B][tiles][segment][state, padded][32]
-  float* seg_steps;  // [B][tiles][segment][32]
+  float* seg_sums;   // [B][tiles][segment][state, padded][64]
+  float* seg_steps;  // [B][tiles][segment][64]
   int B, T, D, N, G, R;  // R: channels of a group
   int softplus;
   int wide_rows, wide_dout, wide_few;  // rows of x, dt and z, of dout, and of B and C lie on 16-byte boundaries
-  int per_group, tiles;  // tiles of 32 channels in a group, and in all
+  int even_out;  // neighbouring channels of dense tensors can be stored together
+  int per_group, tiles;  // tiles of 64 channels in a group, and in all
   int np;                // states rounded up to a multiple of four
   int wide;              // log2 of the states rounded up to a power of two, at least 4
   int nmarks;
@@ -97,25 +98,41 @@ __device__ __forceinline__ float step_of(int softplus, float raw, float bias) {
 // 1 / (1 + e^-x), as sigmoid_of but for the last bits
 __device__ __forceinline__ float gate_of(float x) { return rcp_of(1.0f + exp2_of(x * -1.4426950408889634f)); }
 
-// The tile of 32 channels and the range of tokens of a CTA.
+// The tile of channels and the range of tokens of a CTA.
 struct Place {
-  int seg, unit, b, group, d, local;  // local: the lane's channel in its group
-  int first, end;                     // tokens
-  int d0, width;                      // the tile's first channel, and its channels
-  bool live;                          // the lane has a channel
+  int seg, unit, b, group;
+  int first, end;     // tokens
+  int d0, width;      // the tile's first channel, and its channels
+  int d;              // the lane's first channel (the tile's where it has none)
+  bool live, second;  // the lane has a channel, and its neighbour
 };
 __device__ __forceinline__ Place place(const Problem& p) {
   Place q;
   q.seg = blockIdx.x % p.segs, q.unit = blockIdx.x / p.segs;
-  const int tile = q.unit % p.tiles;
+  const int tile = q.unit % p.tiles, c = 2 * (threadIdx.x & 31);
   q.b = q.unit / p.tiles;
   q.group = tile / p.per_group;
-  q.local = (tile - q.group * p.per_group) * kLanes + (threadIdx.x & 31);
-  q.live = q.local < p.R;
-  q.d0 = q.group * p.R + q.local - (int)(threadIdx.x & 31), q.width = min(p.R - (q.d0 - q.group * p.R), kLanes);
-  q.d = q.live ? q.group * p.R + q.local : q.d0;
+  const int in_group = (tile - q.group * p.per_group) * kTile;
+  q.d0 = q.group * p.R + in_group;
+  q.width = min(p.R - in_group, kTile);
+  q.live = c < q.width, q.second = c + 1 < q.width;
+  q.d = q.d0 + (q.live ? c : 0);
   q.first = q.seg * p.len, q.end = min(q.first + p.len, p.T);
   return q;
+}
+// A parameter [D] of the lane's channels; 0 where there are none.
+__device__ __forceinline__ float2 two_of(const float* v, const Place& q) {
+  return make_float2(v && q.live ? v[q.d] : 0.0f, v && q.second ? v[q.d + 1] : 0.0f);
+}
+// And a matrix [D, N]'s (or [B, D, N]'s from its batch row).
+__device__ __forceinline__ float2 two_of(const float* v, const Place& q, int n, int N) {
+  const bool in = v && n < N;
+  return make_float2(in && q.live ? v[(long)q.d * N + n] : 0.0f, in && q.second ? v[(long)(q.d + 1) * N + n] : 0.0f);
+}
+__device__ __forceinline__ void put_two(float* v, const Place& q, int n, int N, float2 x) {
+  if (n >= N) return;
+  if (q.live) v[(long)q.d * N + n] = x.x;
+  if (q.second) v[(long)(q.d + 1) * N + n] = x.y;
 }
 
 // Byte offset `token` rows of `stride` bytes on: one wide multiply-add.
@@ -134,67 +151,108 @@ __device__ __forceinline__ void copy16(void* to, const void* from) {
 // This thread's copies are there (other threads' after a barrier).
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// Tokens t0 .. t0 + 15 of a tile's channels, from src (its first channel at token
-// 0), to dst [token][32]; the last token again where there are no more.  Pieces of
-// 16 bytes that arrive behind the CTA's work where all rows lie on their boundaries
-// (wide), elements otherwise; channels from `width` on are not written.
+// Brings a block's rows of up to four tensors [token][channel] and of B and C
+// [token][state] from memory to shared memory, as they are stored: [token][64] and
+// [token][N]; the last token again where there are no more.  Pieces of 16 bytes that
+// arrive behind the CTA's work, each thread one of them, where all rows lie on their
+// boundaries and there are threads enough; elements otherwise.  Channels past the
+// tile's width are not written.
 template <typename T>
-__device__ __forceinline__ void fetch_rows(T* dst, const T* src, int stride, int t0, int last, int width, bool wide) {
-  if (wide) {
-    constexpr int kPer = 16 / sizeof(T), kPieces = kLanes / kPer;
-    for (int e = threadIdx.x; e < kBlock * kPieces; e += blockDim.x) {
-      const int t = e / kPieces, c = (e % kPieces) * kPer;
-      if (c < width) copy16(dst + t * kLanes + c, row_at(src + c, min(t0 + t, last), stride));
-    }
-  } else {
-    for (int e = threadIdx.x; e < kBlock * kLanes; e += blockDim.x) {
-      const int t = e / kLanes, c = e % kLanes;
-      if (c < width) dst[e] = *row_at(src + c, min(t0 + t, last), stride);
+struct Feed {
+  static constexpr int kPer = 16 / (int)sizeof(T), kPieces = kTile / kPer;
+  bool rows, few;      // by pieces
+  int token, at;       // of this thread's piece
+  bool has;
+  const T* few_src;    // its piece of B or C
+  int few_token, few_at, few_stride;
+  bool few_has;
+  __device__ __forceinline__ void init(const Problem& p, const Place& q, const T* bm, const T* cm) {
+    const int e = threadIdx.x;
+    rows = p.wide_rows && (int)blockDim.x >= kBlock * kPieces;
+    token = e / kPieces, at = (e % kPieces) * kPer;
+    has = e < kBlock * kPieces && at < q.width;
+    const int pieces = p.N / kPer;
+    few = p.wide_few && (int)blockDim.x >= 2 * kBlock * pieces;
+    few_has = false;
+    if (few) {
+      const bool c = e >= kBlock * pieces;
+      const int f = c ? e - kBlock * pieces : e;
+      few_has = f < kBlock * pieces;
+      few_token = f / pieces;
+      const int n = (f - few_token * pieces) * kPer;
+      few_src = (c ? cm : bm) + n;
+      few_stride = c ? p.cst : p.bst;
+      few_at = (c ? kBlock * p.N : 0) + few_token * p.N + n;
     }
   }
-}
-// The same for N states of B or C: dst [token][N].
-template <typename T>
-__device__ __forceinline__ void fetch_few(T* dst, const T* src, int stride, int t0, int last, int N, bool wide) {
-  if (wide) {
-    const int pieces = N * (int)sizeof(T) / 16;
-    for (int e = threadIdx.x; e < kBlock * pieces; e += blockDim.x) {
-      const int t = e / pieces, c = (e - t * pieces) * (16 / (int)sizeof(T));
-      copy16(dst + t * N + c, row_at(src + c, min(t0 + t, last), stride));
-    }
-  } else {
-    for (int e = threadIdx.x; e < kBlock * N; e += blockDim.x) {
-      const int t = e / N;
-      dst[e] = *row_at(src + (e - t * N), min(t0 + t, last), stride);
+  __device__ __forceinline__ void row(T* dst, const T* src, int stride, int t0, int last, int width, bool wide) const {
+    if (rows && wide) {
+      if (has) copy16(dst + token * kTile + at, row_at(src + at, min(t0 + token, last), stride));
+    } else {
+      for (int e = threadIdx.x; e < kBlock * kTile; e += blockDim.x) {
+        const int t = e / kTile, c = e % kTile;
+        if (c < width) dst[e] = *row_at(src + c, min(t0 + t, last), stride);
+      }
     }
   }
-}
-// From there to FP32 rows by state (kRow floats apart): states from N on and tokens
-// behind the last are zero.
+  __device__ __forceinline__ void bc(const Problem& p, T* dst, const T* bm, const T* cm, int t0, int last) const {
+    if (few) {
+      if (few_has) copy16(dst + few_at, row_at(few_src, min(t0 + few_token, last), few_stride));
+    } else {
+      for (int e = threadIdx.x; e < kBlock * p.N; e += blockDim.x) {
+        const int t = e / p.N, n = e - t * p.N, from = min(t0 + t, last);
+        dst[e] = *row_at(bm + n, from, p.bst);
+        dst[kBlock * p.N + e] = *row_at(cm + n, from, p.cst);
+      }
+    }
+  }
+};
+// B and C from there to FP32 rows by state, each number twice (an operand of two
+// channels), kRow floats apart: states from N on and tokens behind the last are zero.
 template <typename T>
-__device__ __forceinline__ void turn_few(const Problem& p, const T* b, const T* c, float* bs, float* cs, int np, int left) {
+__device__ __forceinline__ void turn_few(const Problem& p, const T* raw, float* bs, float* cs, int np, int left) {
   for (int e = threadIdx.x; e < kBlock << p.wide; e += blockDim.x) {
     const int t = e >> p.wide, n = e & ((1 << p.wide) - 1);
     if (n >= np) continue;
     const bool in = t < left && n < p.N;
-    bs[n * kRow + t] = in ? to_f32(b[t * p.N + n]) : 0.0f;
-    cs[n * kRow + t] = in ? to_f32(c[t * p.N + n]) : 0.0f;
+    const float b = in ? to_f32(raw[t * p.N + n]) : 0.0f, c = in ? to_f32(raw[(kBlock + t) * p.N + n]) : 0.0f;
+    *reinterpret_cast<float2*>(bs + n * kRow + 2 * t) = make_float2(b, b);
+    *reinterpret_cast<float2*>(cs + n * kRow + 2 * t) = make_float2(c, c);
   }
 }
-// Four tokens of the lane's channel.
+// The lane's channels of one token, and of two.
+__device__ __forceinline__ float2 both(const float* rows, int t, int lane) {
+  return *reinterpret_cast<const float2*>(rows + t * kTile + 2 * lane);
+}
+__device__ __forceinline__ float2 both(const bf16* rows, int t, int lane) {
+  const unsigned r = *reinterpret_cast<const unsigned*>(rows + t * kTile + 2 * lane);
+  return make_float2(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
+}
 template <typename T>
-__device__ __forceinline__ void quad_of(const T* rows, int u, int lane, float (&v)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = to_f32(rows[(4 * u + i) * kLanes + lane]);
+__device__ __forceinline__ void four(const T* rows, int u, int lane, float (&v)[4]) {
+  const float2 a = both(rows, 2 * u, lane), b = both(rows, 2 * u + 1, lane);
+  v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+}
+// Stores the lane's channels of one token of a dense tensor.
+template <typename T>
+__device__ __forceinline__ void put_both(T* at, float x, float y, const Place& q, bool even) {
+  if (even) {
+    if (q.live) {
+      const float v[2] = {x, y};
+      store_row<2>(at, v);
+    }
+  } else {
+    if (q.live) at[0] = from_f32<T>(x);
+    if (q.second) at[1] = from_f32<T>(y);
+  }
 }
 
 __device__ __forceinline__ float4 as4(const float (&v)[4]) { return make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ float4 as4(float2 a, float2 b) { return make_float4(a.x, a.y, b.x, b.y); }
 __device__ __forceinline__ float2 lo(float4 v) { return make_float2(v.x, v.y); }
 __device__ __forceinline__ float2 hi(float4 v) { return make_float2(v.z, v.w); }
-__device__ __forceinline__ float4 add4(float4 a, float4 b) {
-  const float2 x = __fadd2_rn(lo(a), lo(b)), y = __fadd2_rn(hi(a), hi(b));
-  return make_float4(x.x, x.y, y.x, y.y);
-}
+__device__ __forceinline__ float4 add4(float4 a, float4 b) { return as4(__fadd2_rn(lo(a), lo(b)), __fadd2_rn(hi(a), hi(b))); }
+__device__ __forceinline__ float2 exp2_of(float2 v) { return make_float2(exp2_of(v.x), exp2_of(v.y)); }
 
 }  // namespace scan
 }  // namespace gru

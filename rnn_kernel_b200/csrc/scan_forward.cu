@@ -2,15 +2,15 @@
 //
 //   h[n] = e^{dt A[n]} h[n] + dt x B[n];   y = sum_n C[n] h[n] + skip x;   out = y silu(z)
 //
-// A CTA owns 32 channels of one sequence, a lane each; every warp has four of the
-// states and goes through all tokens with them in registers, so that each decay is
-// computed once and nothing is exchanged along the time.  What a token has per
-// channel (the step by softplus, dt x, the gate) is worked out by one warp for
-// all, four tokens at a time, and passes through shared memory, as do B and C (by
-// state: one broadcast read serves four tokens of 32 channels) and the warps'
-// shares of y.  Blocks of 16 tokens: the next one's inputs are copied in beside a
-// block's scan; between two barriers its outputs are finished and they are prepared.
-// Neighbouring tokens share a packed FP32 operation in all but the recurrence.
+// A CTA owns 64 channels of one sequence, two neighbours a lane, which share every
+// packed FP32 operation; every warp has two (four above 32) of the states and goes
+// through all tokens with them in registers, so that each decay is computed once
+// and nothing is exchanged along the time.  What a token has per channel (the step
+// by softplus, dt x, the gate) is worked out by one warp for all, two tokens at a
+// time, and passes through shared memory, as do B and C (each number twice: one
+// broadcast read serves two tokens of 64 channels) and the warps' shares of y.
+// Blocks of 16 tokens: the next one's inputs are copied in beside a block's scan;
+// between two barriers its outputs are finished and they are prepared.
 //
 // Sequences too few to fill the GPU are cut into segments: a first launch finds
 // what each makes of a state (h -> e^{A sum dt} h + S), then all segments run side
@@ -30,29 +30,29 @@ namespace {
 struct Lay {
   int step, du, bs, cs, part, in, few, total;
 };
-__host__ __device__ inline Lay layout(int warps, int N, int elem) {
-  const int np = warps * kStates;
+__host__ __device__ inline Lay layout(int warps, int np, int N, int elem) {
   Lay l;
   int n = 0;
-  l.step = n, n += kBlock * kLanes;
-  l.du = n, n += kBlock * kLanes;
+  l.step = n, n += kBlock * kTile;
+  l.du = n, n += kBlock * kTile;
   l.bs = n, n += np * kRow;
   l.cs = n, n += np * kRow;
-  l.part = n, n += warps * kBlock * kLanes;  // [quad][warp][lane] float4
-  l.in = n, n += 3 * kBlock * kLanes * elem / 4;
+  l.part = n, n += warps * kBlock * kTile;  // [pair of tokens][warp][lane] float4
+  l.in = n, n += 3 * kBlock * kTile * elem / 4;
   l.few = n, n += 2 * kBlock * N * elem / 4;
   l.total = n;
   return l;
 }
 
-// SUM: only what the segments make of a state.  MOST: threads at most.  W: the
-// warps, where they are known (4, for the usual 16 states: addresses are constants
-// then, and each warp has one quad of tokens to prepare and finish), or 0.
-template <typename T, bool SUM, int MOST, int W>
-__global__ void __launch_bounds__(MOST, MOST == 128 ? 6 : 1) scan_forward_kernel(const __grid_constant__ Problem p) {
+// SG: states of a warp.  SUM: only what the segments make of a state.  MOST: threads
+// at most.  W: the warps, where they are known (8, for the usual 16 states: addresses
+// are constants then, and each warp has one pair of tokens to prepare and finish),
+// or 0.
+template <typename T, int SG, bool SUM, int MOST, int W>
+__global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : 1) scan_forward_kernel(const __grid_constant__ Problem p) {
   extern __shared__ __align__(16) float sm[];
-  const int warps = W ? W : blockDim.x >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31, np = warps * kStates;
-  const Lay l = layout(warps, p.N, sizeof(T));
+  const int threads = W ? 32 * W : blockDim.x, warps = W ? W : threads >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Lay l = layout(warps, p.np, p.N, sizeof(T));
   const Place q = place(p);
   if (SUM && q.seg == p.segs - 1) return;
   const T* x = static_cast<const T*>(p.x) + q.b * p.xb + q.d0;
@@ -61,108 +61,98 @@ __global__ void __launch_bounds__(MOST, MOST == 128 ? 6 : 1) scan_forward_kernel
   const T* bm = static_cast<const T*>(p.b) + q.b * p.bb + q.group * p.bg;
   const T* cm = static_cast<const T*>(p.c) + q.b * p.cb + q.group * p.cg;
   T* out = static_cast<T*>(p.out) + (long)q.b * p.T * p.D + q.d;
-  const float bias = p.bias ? p.bias[q.d] : 0.0f, skip = p.skip ? p.skip[q.d] : 0.0f;
-  const int lastt = q.end - 1, n0 = kStates * w;
+  const float2 bias = two_of(p.bias, q), skip = two_of(p.skip, q);
+  const int lastt = q.end - 1, n0 = SG * w;
   T* in = reinterpret_cast<T*>(sm + l.in);
   T* few = reinterpret_cast<T*>(sm + l.few);
-  constexpr int kTile = kBlock * kLanes;
+  constexpr int kRows = kBlock * kTile;
+  Feed<T> feed;
+  feed.init(p, q, bm, cm);
   auto fetch = [&](int t0) {
-    fetch_rows(in, x, p.xst, t0, lastt, q.width, p.wide_rows);
-    fetch_rows(in + kTile, dt, p.dtst, t0, lastt, q.width, p.wide_rows);
-    if (z) fetch_rows(in + 2 * kTile, z, p.zst, t0, lastt, q.width, p.wide_rows);
-    fetch_few(few, bm, p.bst, t0, lastt, p.N, p.wide_few);
-    fetch_few(few + kBlock * p.N, cm, p.cst, t0, lastt, p.N, p.wide_few);
+    feed.row(in, x, p.xst, t0, lastt, q.width, true);
+    feed.row(in + kRows, dt, p.dtst, t0, lastt, q.width, true);
+    if (z) feed.row(in + 2 * kRows, z, p.zst, t0, lastt, q.width, true);
+    feed.bc(p, few, bm, cm, t0, lastt);
   };
   fetch(q.first);
 
-  float rt[kStates], h[kStates];
+  float2 rt[SG], h[SG];
 #pragma unroll
-  for (int j = 0; j < kStates; ++j) {
-    const bool in = q.live && n0 + j < p.N;
-    rt[j] = in ? decay_rate(p.a[(long)q.d * p.N + n0 + j]) : 0.0f;
-    h[j] = !SUM && in && p.s0 ? p.s0[((long)q.b * p.D + q.d) * p.N + n0 + j] : 0.0f;
+  for (int j = 0; j < SG; ++j) {
+    const float2 a = two_of(p.a, q, n0 + j, p.N);
+    rt[j] = make_float2(decay_rate(a.x), decay_rate(a.y));
+    h[j] = SUM ? twice(0.0f) : two_of(p.s0 ? p.s0 + (long)q.b * p.D * p.N : nullptr, q, n0 + j, p.N);
   }
   if (!SUM)
     for (int s = 0; s < q.seg; ++s) {
       const long at = (long)q.unit * p.segs + s;
-      const float steps = p.seg_steps[at * kLanes + lane];
+      const float2 steps = both(p.seg_steps + at * kTile, 0, lane);
 #pragma unroll
-      for (int j = 0; j < kStates; ++j)
-        h[j] = fmaf(exp2_of(rt[j] * steps), h[j], p.seg_sums[(at * p.np + n0 + j) * kLanes + lane]);
+      for (int j = 0; j < SG; ++j)
+        h[j] = __ffma2_rn(exp2_of(__fmul2_rn(rt[j], steps)), h[j], both(p.seg_sums + (at * p.np + n0 + j) * kTile, 0, lane));
     }
 
-  float4* step = reinterpret_cast<float4*>(sm + l.step) + lane;
+  float4* step = reinterpret_cast<float4*>(sm + l.step) + lane;  // [pair of tokens][lane]
   float4* du = reinterpret_cast<float4*>(sm + l.du) + lane;
   float4* part = reinterpret_cast<float4*>(sm + l.part) + lane;
   const float* bs = sm + l.bs + n0 * kRow;
   const float* cs = sm + l.cs + n0 * kRow;
-  // What finish() needs of the warp's first quad; the inputs are overwritten before.
+  // What finish() needs of the warp's first pair; the inputs are overwritten before.
   float own[4], gate[4];
-  auto outer = [&](int u, float (&o)[4], float (&g)[4]) {
-    quad_of(in, u, lane, o);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = p.skip ? o[i] * skip : 0.0f;
-    if (z) {
-      quad_of(in + 2 * kTile, u, lane, g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) g[i] *= gate_of(g[i]);
-    }
-  };
   auto prepare = [&](int t0) {
-    for (int u = w; u < kQuads; u += warps) {
+    for (int u = w; u < kPairs; u += warps) {
       float s[4], v[4];
-      quad_of(in + kTile, u, lane, s);
-      quad_of(in, u, lane, v);
+      four(in + kRows, u, lane, s);
+      four(in, u, lane, v);
+      if (!SUM && u == w) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) own[i] = p.skip ? (i & 1 ? skip.y : skip.x) * v[i] : 0.0f;
+        if (z) {
+          four(in + 2 * kRows, u, lane, gate);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) gate[i] *= gate_of(gate[i]);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[i] = step_of(p.softplus, s[i], bias);
+        s[i] = step_of(p.softplus, s[i], i & 1 ? bias.y : bias.x);
         v[i] *= s[i];
       }
-      if (!q.live || t0 + 4 * u + 3 > lastt)  // lanes without a channel keep states of zero
+      // tokens that are not there, and lanes without a channel, whose states stay zero
+      if (!q.second || t0 + 2 * u + 1 > lastt)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (!q.live || t0 + 4 * u + i > lastt) s[i] = v[i] = 0.0f;
+          if (!(i & 1 ? q.second : q.live) || t0 + 2 * u + i / 2 > lastt) s[i] = v[i] = 0.0f;
       step[u * kLanes] = as4(s), du[u * kLanes] = as4(v);
-      if (!SUM && u == w) outer(u, own, gate);
       if (W) break;
     }
-    turn_few(p, few, few + kBlock * p.N, sm + l.bs, sm + l.cs, np, q.end - t0);
+    turn_few(p, few, sm + l.bs, sm + l.cs, p.np, q.end - t0);
   };
   auto finish = [&](int t0) {
-    for (int u = w; u < kQuads; u += warps) {
-      const int t = t0 + 4 * u;
+    for (int u = w; u < kPairs; u += warps) {
+      const int t = t0 + 2 * u;
+      if (t > lastt) break;
       float4 sum = part[u * warps * kLanes];
 #pragma unroll (W ? W : 4)
       for (int k = 1; k < warps; ++k) sum = add4(sum, part[(u * warps + k) * kLanes]);
-      float y[4] = {sum.x, sum.y, sum.z, sum.w}, o[4], g[4];
+      float y[4] = {sum.x, sum.y, sum.z, sum.w};
       if (u == w) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = own[i], g[i] = gate[i];
-      } else {  // fewer warps than quads: from memory once more
+        for (int i = 0; i < 4; ++i) y[i] = z ? (y[i] + own[i]) * gate[i] : y[i] + own[i];
+      } else if (q.live) {  // fewer warps than pairs: from memory once more
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int at = min(t + i, lastt);
-          o[i] = p.skip ? skip * to_f32(*row_at(x + q.d - q.d0, at, p.xst)) : 0.0f;
-          g[i] = z ? to_f32(*row_at(z + q.d - q.d0, at, p.zst)) : 0.0f;
-          g[i] *= gate_of(g[i]);
+          const int at = min(t + i / 2, lastt), c = q.d - q.d0 + (i & 1 ? q.second : 0);
+          if (p.skip) y[i] = fmaf(i & 1 ? skip.y : skip.x, to_f32(*row_at(x + c, at, p.xst)), y[i]);
+          if (z) {
+            const float g = to_f32(*row_at(z + c, at, p.zst));
+            y[i] *= g * gate_of(g);
+          }
         }
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        y[i] += o[i];
-        if (z) y[i] *= g[i];
-      }
-      if (q.live) {
-        T* to = row_at(out, t, p.ost);
-        if (t + 3 <= lastt) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) *row_at(to, i, p.ost) = from_f32<T>(y[i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (t + i <= lastt) *row_at(to, i, p.ost) = from_f32<T>(y[i]);
-        }
-      }
+      T* to = row_at(out, t, p.ost);
+      put_both(to, y[0], y[1], q, p.even_out);
+      if (t < lastt) put_both(to + p.D, y[2], y[3], q, p.even_out);
       if (W) break;
     }
   };
@@ -171,39 +161,35 @@ __global__ void __launch_bounds__(MOST, MOST == 128 ? 6 : 1) scan_forward_kernel
   __syncthreads();
   prepare(q.first);
   __syncthreads();
-  float total = 0.0f;
-  float* mark = p.marks + (((long)q.unit * p.nmarks + q.first / kBlock) * p.np + n0) * kLanes + lane;
+  float2 total = twice(0.0f);
+  float* mark = p.marks + (((long)q.unit * p.nmarks + q.first / kBlock) * p.np + n0) * kTile + 2 * lane;
   for (int t0 = q.first; t0 <= lastt; t0 += kBlock) {
     const bool more = t0 + kBlock <= lastt;
     if (more) fetch(t0 + kBlock);
     if (!SUM && p.marks) {
 #pragma unroll
-      for (int j = 0; j < kStates; ++j) mark[j * kLanes] = h[j];
-      mark += p.np * kLanes;
+      for (int j = 0; j < SG; ++j) *reinterpret_cast<float2*>(mark + j * kTile) = h[j];
+      mark += p.np * kTile;
     }
 #pragma unroll
-    for (int t = 0; t < kQuads; ++t) {
+    for (int t = 0; t < kPairs; ++t) {
       const float4 s = step[t * kLanes], u = du[t * kLanes];
       float2 y0 = twice(0.0f), y1 = twice(0.0f);
-      if (SUM) total += (s.x + s.y) + (s.z + s.w);
+      if (SUM) total = __fadd2_rn(total, __fadd2_rn(lo(s), hi(s)));
 #pragma unroll
-      for (int j = 0; j < kStates; ++j) {
+      for (int j = 0; j < SG; ++j) {
         const float4 bv = *reinterpret_cast<const float4*>(bs + j * kRow + 4 * t);
-        const float2 e0 = __fmul2_rn(lo(s), twice(rt[j])), e1 = __fmul2_rn(hi(s), twice(rt[j]));
-        const float2 v0 = __fmul2_rn(lo(u), lo(bv)), v1 = __fmul2_rn(hi(u), hi(bv));
-        float2 h0, h1;
-        h0.x = fmaf(exp2_of(e0.x), h[j], v0.x);
-        h0.y = fmaf(exp2_of(e0.y), h0.x, v0.y);
-        h1.x = fmaf(exp2_of(e1.x), h0.y, v1.x);
-        h1.y = fmaf(exp2_of(e1.y), h1.x, v1.y);
-        h[j] = h1.y;
+        const float2 a0 = exp2_of(__fmul2_rn(lo(s), rt[j])), a1 = exp2_of(__fmul2_rn(hi(s), rt[j]));
+        const float2 h0 = __ffma2_rn(a0, h[j], __fmul2_rn(lo(u), lo(bv)));
+        const float2 h1 = __ffma2_rn(a1, h0, __fmul2_rn(hi(u), hi(bv)));
+        h[j] = h1;
         if (!SUM) {
           const float4 cv = *reinterpret_cast<const float4*>(cs + j * kRow + 4 * t);
           y0 = __ffma2_rn(lo(cv), h0, y0);
           y1 = __ffma2_rn(hi(cv), h1, y1);
         }
       }
-      if (!SUM) part[(t * warps + w) * kLanes] = make_float4(y0.x, y0.y, y1.x, y1.y);
+      if (!SUM) part[(t * warps + w) * kLanes] = as4(y0, y1);
     }
     copies_done();
     __syncthreads();
@@ -214,29 +200,28 @@ __global__ void __launch_bounds__(MOST, MOST == 128 ? 6 : 1) scan_forward_kernel
   if (SUM) {
     const long at = (long)q.unit * p.segs + q.seg;
 #pragma unroll
-    for (int j = 0; j < kStates; ++j) p.seg_sums[(at * p.np + n0 + j) * kLanes + lane] = h[j];
-    if (w == 0) p.seg_steps[at * kLanes + lane] = total;
-  } else if (q.seg == p.segs - 1 && q.live) {
-    float* last = p.last + ((long)q.b * p.D + q.d) * p.N + n0;
+    for (int j = 0; j < SG; ++j)
+      *reinterpret_cast<float2*>(p.seg_sums + (at * p.np + n0 + j) * kTile + 2 * lane) = h[j];
+    if (w == 0) *reinterpret_cast<float2*>(p.seg_steps + at * kTile + 2 * lane) = total;
+  } else if (q.seg == p.segs - 1) {
 #pragma unroll
-    for (int j = 0; j < kStates; ++j)
-      if (n0 + j < p.N) last[j] = h[j];
+    for (int j = 0; j < SG; ++j) put_two(p.last + (long)q.b * p.D * p.N, q, n0 + j, p.N, h[j]);
   }
 }
 
-template <typename T, int MOST, int W>
+template <typename T, int SG, int MOST, int W>
 int launch_forward(const Problem& p, cudaStream_t stream) {
-  const int warps = p.np / kStates;
-  const size_t smem = layout(warps, p.N, sizeof(T)).total * sizeof(float);
+  const int warps = p.np / SG;
+  const size_t smem = layout(warps, p.np, p.N, sizeof(T)).total * sizeof(float);
   const unsigned ctas = (unsigned)((long)p.B * p.tiles * p.segs);
   LaunchScope scope(kKindSelectiveScan, stream, p.segs > 1 ? 2 : 1);
   if (p.segs > 1) {
-    auto kernel = scan_forward_kernel<T, true, MOST, W>;
+    auto kernel = scan_forward_kernel<T, SG, true, MOST, W>;
     GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     kernel<<<ctas, 32 * warps, smem, stream>>>(p);
     GRU_CUDA_TRY(cudaGetLastError());
   }
-  auto kernel = scan_forward_kernel<T, false, MOST, W>;
+  auto kernel = scan_forward_kernel<T, SG, false, MOST, W>;
   GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   kernel<<<ctas, 32 * warps, smem, stream>>>(p);
   GRU_CUDA_TRY(cudaGetLastError());
@@ -245,8 +230,9 @@ int launch_forward(const Problem& p, cudaStream_t stream) {
 
 template <typename T>
 int forward_of(const Problem& p, cudaStream_t stream) {
-  if (p.np == 16) return launch_forward<T, 128, 4>(p, stream);
-  return p.np < 16 ? launch_forward<T, 128, 0>(p, stream) : launch_forward<T, 512, 0>(p, stream);
+  if (p.np == 16) return launch_forward<T, 2, 256, 8>(p, stream);
+  if (p.np < 16) return launch_forward<T, 2, 256, 0>(p, stream);
+  return p.np <= 32 ? launch_forward<T, 2, 512, 0>(p, stream) : launch_forward<T, 4, 512, 0>(p, stream);
 }
 
 }  // namespace

@@ -128,7 +128,7 @@ int check(const char* me, const gru_scan_args* p, Needs needs) {
   for (const long s : {p->x_stride[1], p->dt_stride[1], p->z_stride[1], p->b_stride[1], p->c_stride[1]})
     if (s < 0 || s * (long)es > 0x7fffffffL)
       return refuse(me, "tokens must be less than 2^31 bytes apart", GRU_ERR_UNSUPPORTED);
-  const double tiles = (double)p->G * ((p->D / p->G + kLanes - 1) / kLanes);
+  const double tiles = (double)p->G * ((p->D / p->G + kTile - 1) / kTile);
   if (p->B * tiles > 2e9 || (double)p->B * p->D * 16 > 4e11 || (double)p->B * p->T * p->G > 4e9 || p->T > (1 << 30) ||
       p->D > (1 << 26))
     return refuse(me, "too large for one launch", GRU_ERR_UNSUPPORTED);
@@ -153,7 +153,7 @@ void fill(Problem& a, const gru_scan_args& p) {
   a.wide_few = on16(p.b, p.b_stride, 3) && on16(p.c, p.c_stride, 3) && p.N * es % 16 == 0;
   a.B = p.B, a.T = p.T, a.D = p.D, a.N = p.N, a.G = p.G, a.R = p.D / p.G;
   a.softplus = p.dt_softplus;
-  a.per_group = ceil_div(a.R, kLanes), a.tiles = a.per_group * a.G;
+  a.per_group = ceil_div(a.R, kTile), a.tiles = a.per_group * a.G;
   a.np = ceil_div(a.N, 4) * 4;
   a.wide = 2;
   while ((1 << a.wide) < a.N) ++a.wide;
@@ -164,7 +164,7 @@ void fill(Problem& a, const gru_scan_args& p) {
 // w / (w + 8) busy with w of them; more than one segment costs a first pass of some
 // 0.7 of the work over all but one of them.
 void cut(Problem& a, int full) {
-  const double beside = (double)a.B * a.tiles * (a.np / kStates) / 148.0;
+  const double beside = (double)a.B * a.tiles * (a.np <= 32 ? a.np / 2 : a.np / 4) / 148.0;
   double best = 0.0;
   a.segs = 1;
   for (int s = 1; s <= 64 && (s == 1 || a.T / s >= 4 * kBlock); s *= 2) {
@@ -176,9 +176,12 @@ void cut(Problem& a, int full) {
   a.segs = std::max(1, ceil_div(a.T, a.len > 0 ? a.len : 1));
 }
 
-void lay_marks(Problem& a, Pieces& m) { a.marks = m.floats((size_t)a.B * a.tiles * a.nmarks * a.np * kLanes); }
+// Whether the lanes' two channels of dense tensors start on a boundary of two elements.
+int even(const Problem& a, int dtype, uintptr_t all) { return a.R % 2 == 0 && (all & (2 * elem_size(dtype) - 1)) == 0; }
+
+void lay_marks(Problem& a, Pieces& m) { a.marks = m.floats((size_t)a.B * a.tiles * a.nmarks * a.np * kTile); }
 void lay_segments(Problem& a, Pieces& m) {
-  const size_t n = a.segs > 1 ? (size_t)a.B * a.tiles * a.segs * kLanes : 0;
+  const size_t n = a.segs > 1 ? (size_t)a.B * a.tiles * a.segs * kTile : 0;
   a.seg_sums = m.floats(n * a.np);
   a.seg_steps = m.floats(n);
 }
@@ -248,6 +251,7 @@ extern "C" int gru_scan_forward(const gru_scan_args* p, void* out, float* final_
   if (m.used && (!workspace || workspace_bytes < m.used || bits(workspace) & 15))
     return refuse(me, "workspace too small or not 16-byte aligned");
   a.out = out, a.last = final_state;
+  a.even_out = even(a, p->dtype, bits(out));
   return forward(a, p->dtype, stream);
 }
 
@@ -282,6 +286,7 @@ extern "C" int gru_scan_backward(const gru_scan_args* p, const void* dout, const
   if (!stash || stash_bytes < m.used || !workspace || workspace_bytes < w.used || (bits(stash) | bits(workspace)) & 15)
     return refuse(me, "stash or workspace too small or not 16-byte aligned");
   a.dout = dout, a.dlast = dfinal;
+  a.even_out = even(a, p->dtype, bits(dx) | bits(ddt) | bits(dz));
   a.wide_dout = (bits(dout) & 15) == 0;  // its rows are D elements apart, as wide as wide_rows asks for
   a.dx = dx, a.ddt = ddt, a.da = da, a.db = db, a.dc = dc, a.dskip = dskip, a.dz = dz, a.dbias = ddt_bias, a.ds0 = dinitial;
   return backward(a, p->dtype, stream);
