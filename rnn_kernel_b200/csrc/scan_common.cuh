@@ -154,9 +154,9 @@ __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;
 // Brings a block's rows of up to four tensors [token][channel] and of B and C
 // [token][state] from memory to shared memory, as they are stored: [token][64] and
 // [token][N]; the last token again where there are no more.  Pieces of 16 bytes that
-// arrive behind the CTA's work, each thread one of them, where all rows lie on their
-// boundaries and there are threads enough; elements otherwise.  Channels past the
-// tile's width are not written.
+// arrive behind the CTA's work, where all rows lie on their
+// boundaries (for B and C: and there are threads enough); elements otherwise.
+// Channels past the tile's width are not written.
 template <typename T>
 struct Feed {
   static constexpr int kPer = 16 / (int)sizeof(T), kPieces = kTile / kPer;
@@ -168,9 +168,9 @@ struct Feed {
   bool few_has;
   __device__ __forceinline__ void init(const Problem& p, const Place& q, const T* bm, const T* cm) {
     const int e = threadIdx.x;
-    rows = p.wide_rows && (int)blockDim.x >= kBlock * kPieces;
+    rows = p.wide_rows;
     token = e / kPieces, at = (e % kPieces) * kPer;
-    has = e < kBlock * kPieces && at < q.width;
+    has = at < q.width;
     const int pieces = p.N / kPer;
     few = p.wide_few && (int)blockDim.x >= 2 * kBlock * pieces;
     few_has = false;
@@ -187,7 +187,9 @@ struct Feed {
   }
   __device__ __forceinline__ void row(T* dst, const T* src, int stride, int t0, int last, int width, bool wide) const {
     if (rows && wide) {
-      if (has) copy16(dst + token * kTile + at, row_at(src + at, min(t0 + token, last), stride));
+      if (has)
+        for (int t = token; t < kBlock; t += blockDim.x / kPieces)
+          copy16(dst + t * kTile + at, row_at(src + at, min(t0 + t, last), stride));
     } else {
       for (int e = threadIdx.x; e < kBlock * kTile; e += blockDim.x) {
         const int t = e / kTile, c = e % kTile;

@@ -49,7 +49,7 @@ __host__ __device__ inline Lay layout(int warps, int np, int N, int elem) {
 // are constants then, and each warp has one pair of tokens to prepare and finish),
 // or 0.
 template <typename T, int SG, bool SUM, int MOST, int W>
-__global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : 1) scan_forward_kernel(const __grid_constant__ Problem p) {
+__global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : MOST == 128 ? 5 : 1) scan_forward_kernel(const __grid_constant__ Problem p) {
   extern __shared__ __align__(16) float sm[];
   const int threads = W ? 32 * W : blockDim.x, warps = W ? W : threads >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Lay l = layout(warps, p.np, p.N, sizeof(T));
@@ -97,20 +97,27 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : 1) scan_forward_kernel
   float4* part = reinterpret_cast<float4*>(sm + l.part) + lane;
   const float* bs = sm + l.bs + n0 * kRow;
   const float* cs = sm + l.cs + n0 * kRow;
-  // What finish() needs of the warp's first pair; the inputs are overwritten before.
-  float own[4], gate[4];
+  // What finish() needs of the warp's first pairs; the inputs are overwritten before.
+  constexpr int kOwn = W ? (kPairs + W - 1) / W : 1;
+  float own[kOwn][4], gate[kOwn][4];
   auto prepare = [&](int t0) {
-    for (int u = w; u < kPairs; u += warps) {
+#pragma unroll
+    for (int k = 0; k < (W ? kOwn : kPairs); ++k) {
+      const int u = w + k * warps;
+      if (u >= kPairs) break;
       float s[4], v[4];
       four(in + kRows, u, lane, s);
       four(in, u, lane, v);
-      if (!SUM && u == w) {
+      if (!SUM && k < kOwn) {
+        constexpr int kLast = kOwn - 1;
+        float(&o)[4] = own[k < kOwn ? k : kLast];
+        float(&g)[4] = gate[k < kOwn ? k : kLast];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) own[i] = p.skip ? (i & 1 ? skip.y : skip.x) * v[i] : 0.0f;
+        for (int i = 0; i < 4; ++i) o[i] = p.skip ? (i & 1 ? skip.y : skip.x) * v[i] : 0.0f;
         if (z) {
-          four(in + 2 * kRows, u, lane, gate);
+          four(in + 2 * kRows, u, lane, g);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) gate[i] *= gate_of(gate[i]);
+          for (int i = 0; i < 4; ++i) g[i] *= gate_of(g[i]);
         }
       }
 #pragma unroll
@@ -124,21 +131,24 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : 1) scan_forward_kernel
         for (int i = 0; i < 4; ++i)
           if (!(i & 1 ? q.second : q.live) || t0 + 2 * u + i / 2 > lastt) s[i] = v[i] = 0.0f;
       step[u * kLanes] = as4(s), du[u * kLanes] = as4(v);
-      if (W) break;
     }
     turn_few(p, few, sm + l.bs, sm + l.cs, p.np, q.end - t0);
   };
   auto finish = [&](int t0) {
-    for (int u = w; u < kPairs; u += warps) {
-      const int t = t0 + 2 * u;
-      if (t > lastt) break;
+#pragma unroll
+    for (int k = 0; k < (W ? kOwn : kPairs); ++k) {
+      const int u = w + k * warps, t = t0 + 2 * u;
+      if (u >= kPairs || t > lastt) break;
       float4 sum = part[u * warps * kLanes];
 #pragma unroll (W ? W : 4)
-      for (int k = 1; k < warps; ++k) sum = add4(sum, part[(u * warps + k) * kLanes]);
+      for (int i = 1; i < warps; ++i) sum = add4(sum, part[(u * warps + i) * kLanes]);
       float y[4] = {sum.x, sum.y, sum.z, sum.w};
-      if (u == w) {
+      if (k < kOwn) {
+        constexpr int kLast = kOwn - 1;
+        const float(&o)[4] = own[k < kOwn ? k : kLast];
+        const float(&g)[4] = gate[k < kOwn ? k : kLast];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = z ? (y[i] + own[i]) * gate[i] : y[i] + own[i];
+        for (int i = 0; i < 4; ++i) y[i] = z ? (y[i] + o[i]) * g[i] : y[i] + o[i];
       } else if (q.live) {  // fewer warps than pairs: from memory once more
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -153,7 +163,6 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : 1) scan_forward_kernel
       T* to = row_at(out, t, p.ost);
       put_both(to, y[0], y[1], q, p.even_out);
       if (t < lastt) put_both(to + p.D, y[2], y[3], q, p.even_out);
-      if (W) break;
     }
   };
 
@@ -230,7 +239,7 @@ int launch_forward(const Problem& p, cudaStream_t stream) {
 
 template <typename T>
 int forward_of(const Problem& p, cudaStream_t stream) {
-  if (p.np == 16) return launch_forward<T, 2, 256, 8>(p, stream);
+  if (p.np == 16) return launch_forward<T, 4, 128, 4>(p, stream);
   if (p.np < 16) return launch_forward<T, 2, 256, 0>(p, stream);
   return p.np <= 32 ? launch_forward<T, 2, 512, 0>(p, stream) : launch_forward<T, 4, 512, 0>(p, stream);
 }
