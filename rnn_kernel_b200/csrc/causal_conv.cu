@@ -5,11 +5,14 @@
 //   e = dy silu'(p);  dx_t = sum_j w_j e_{t+W-1-j};  dw_j = sum_t e_t x_{t-W+1+j};  db = sum_t e_t
 //
 // Tokens before the first come from a state of W - 1 inputs.  A thread takes a
-// few neighbouring channels through a run of tokens with the last W - 1 inputs
-// in registers, so x is read once, but for the W - 1 tokens that two runs share.
-// The gradient keeps the last W errors too: e_t is final when x_t is read, and
-// with it dx_{t-W+1}.  Sums of dw and db go from a thread's registers over the
-// CTA's runs and then over the CTAs, in a fixed order.  Bound by memory.
+// few neighbouring channels through a run of tokens with the last W inputs in
+// registers (the loop goes W tokens at a time, so that none of them is moved), so x
+// is read once, but for the W - 1 tokens that two runs share.  The gradient keeps
+// the last W errors too: e_t is final when x_t is read, and with it dx_{t-W+1}.
+// Sums of dw and db go from a thread's registers over the CTA's runs and then over
+// the CTAs, in a fixed order.  Loads have no branch around them, which would wait for
+// each: rows past the ends are the last one again, and their numbers dropped.
+// Bound by memory.
 
 #include <algorithm>
 
@@ -33,18 +36,56 @@ struct Conv {
   int B, T, D, W, wtype, silu, run, runs;
 };
 
-// x at token t of a batch row, from the state before the first (T <= t: zero).
-template <typename T, int V>
-__device__ __forceinline__ void token(const Conv& a, int b, int c, int t, float (&v)[V]) {
-  if (t >= 0 && t < a.T) {
-    load_row<V>(static_cast<const T*>(a.x) + b * a.xb + t * a.xt + c, v);
-  } else if (t < 0 && a.s0) {
-    load_row<V>(static_cast<const T*>(a.s0) + ((long)b * (a.W - 1) + (a.W - 1 + t)) * a.D + c, v);
+// a[e] b[e] + c[e], neighbours packed.
+template <int V>
+__device__ __forceinline__ void fma_into(float (&c)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float2 r = __ffma2_rn(make_float2(a[e], a[e + 1]), make_float2(b[e], b[e + 1]), make_float2(c[e], c[e + 1]));
+      c[e] = r.x, c[e + 1] = r.y;
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = 0.0f;
+    for (int e = 0; e < V; ++e) c[e] = fmaf(a[e], b[e], c[e]);
   }
 }
+
+// A thread's channels c .. c + V - 1 of batch row b.
+template <typename T, int W, int V>
+struct Run {
+  const T *x, *s0;  // rows of tokens 0
+  float w[W][V], bias[V], win[W][V];  // the input of token t at win[t mod W], counted from the run's first
+  __device__ __forceinline__ Run(const Conv& a, int b, int c) {
+    x = static_cast<const T*>(a.x) + b * a.xb + c;
+    s0 = a.s0 ? static_cast<const T*>(a.s0) + ((long)b * (W - 1) + W - 1) * a.D + c : nullptr;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) w[j][e] = get(a.w, (long)(c + e) * W + j, a.wtype);
+      bias[e] = a.bias ? get(a.bias, c + e, a.wtype) : 0.0f;
+    }
+  }
+  // Token t, which may lie before the first.
+  __device__ __forceinline__ void any(const Conv& a, int t, float (&v)[V]) const {
+    const T* at = t < 0 && s0 ? s0 + (long)t * a.D : x + (long)min(max(t, 0), a.T - 1) * a.xt;
+    load_row<V>(at, v);
+    if (t < 0 && !s0)
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = 0.0f;
+  }
+  __device__ __forceinline__ void start(const Conv& a, int t0) {
+#pragma unroll
+    for (int j = 1; j < W; ++j) any(a, t0 - W + j, win[j]);
+  }
+  // The sum for token u of a turn.
+  __device__ __forceinline__ void sum(int u, float (&p)[V]) const {
+#pragma unroll
+    for (int e = 0; e < V; ++e) p[e] = bias[e];
+#pragma unroll
+    for (int j = 0; j < W; ++j) fma_into(p, w[j], win[(u + 1 + j) % W]);
+  }
+};
 
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(256) conv_forward_kernel(const Conv a) {
@@ -55,35 +96,31 @@ __global__ void __launch_bounds__(256) conv_forward_kernel(const Conv a) {
   const int b = (int)(rest / a.runs);
   if (b >= a.B) return;
   const int t0 = (int)(rest - (long)b * a.runs) * a.run, t1 = min(t0 + a.run, a.T);
-  float w[V][W], bias[V], win[W][V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) w[e][j] = get(a.w, (long)(c + e) * W + j, a.wtype);
-    bias[e] = a.bias ? get(a.bias, c + e, a.wtype) : 0.0f;
-  }
-#pragma unroll
-  for (int j = 0; j < W - 1; ++j) token<T, V>(a, b, c, t0 - (W - 1) + j, win[j]);
+  Run<T, W, V> r(a, b, c);
+  r.start(a, t0);
   T* y = static_cast<T*>(a.y) + ((long)b * a.T + t0) * a.D + c;
-  constexpr int U = 4;  // tokens loaded together
-  for (int t = t0; t < t1; t += U) {
-    float x[U][V];
+  float next[W][V];
+  auto load = [&](int t) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) token<T, V>(a, b, c, t + u, x[u]);
+    for (int u = 0; u < W; ++u) load_row<V>(r.x + (long)min(t + u, a.T - 1) * a.xt, next[u]);
+  };
+  load(t0);
+  for (int t = t0; t < t1; t += W) {
+    float x[W][V];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < W; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[u][e] = next[u][e];
+    if (t + W < t1) load(t + W);
+#pragma unroll
+    for (int u = 0; u < W; ++u) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) r.win[u][e] = x[u][e];
       float p[V];
+      r.sum(u, p);
+      if (a.silu)
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        p[e] = bias[e];
-#pragma unroll
-        for (int j = 0; j < W - 1; ++j) p[e] = fmaf(w[e][j], win[j][e], p[e]);
-        p[e] = fmaf(w[e][W - 1], x[u][e], p[e]);
-        if (a.silu) p[e] *= sigmoid_of(p[e]);
-#pragma unroll
-        for (int j = 0; j + 1 < W - 1; ++j) win[j][e] = win[j + 1][e];
-        win[W - 2][e] = x[u][e];
-      }
+        for (int e = 0; e < V; ++e) p[e] *= sigmoid_of(p[e]);
       if (t + u < t1) store_row<V>(y, p);
       y += a.D;
     }
@@ -92,7 +129,7 @@ __global__ void __launch_bounds__(256) conv_forward_kernel(const Conv a) {
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) {
       float v[V];
-      token<T, V>(a, b, c, a.T - (W - 1) + j, v);
+      r.any(a, a.T - (W - 1) + j, v);
       store_row<V>(static_cast<T*>(a.last) + ((long)b * (W - 1) + j) * a.D + c, v);
     }
   }
@@ -101,104 +138,97 @@ __global__ void __launch_bounds__(256) conv_forward_kernel(const Conv a) {
 // A CTA: 32 lanes x V channels, kGradRuns runs of tokens, one a warp.
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(32 * kGradRuns) conv_backward_kernel(const Conv a) {
-  extern __shared__ float sums[];  // [run][W + 1][32 V]
+  extern __shared__ __align__(16) float sums[];  // [run][W + 1][32 V]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int blocks = ceil_div(a.D, 32 * V);
+  const int blocks = (a.D + 32 * V - 1) / (32 * V);
   const int cb = blockIdx.x % blocks;
   const long rest = blockIdx.x / blocks;  // batch row and run group
-  const int groups = ceil_div(a.runs, kGradRuns);
+  const int groups = (a.runs + kGradRuns - 1) / kGradRuns;
   const int b = (int)(rest / groups), run = (int)(rest - (long)b * groups) * kGradRuns + warp;
   const int c = (cb * 32 + lane) * V;
-  float dw[V][W], db[V];
+  float dw[W][V], db[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     db[e] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < W; ++j) dw[e][j] = 0.0f;
+    for (int j = 0; j < W; ++j) dw[j][e] = 0.0f;
   }
   if (c < a.D && run < a.runs) {
     const int t0 = run * a.run, t1 = min(t0 + a.run, a.T);
-    float w[V][W], bias[V], win[W][V], err[W][V];  // inputs up to t, errors up to t
+    Run<T, W, V> r(a, b, c);
+    r.start(a, t0);
+    float err[W][V];  // the error of token t at err[t mod W]
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
+    for (int j = 0; j < W; ++j)
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        w[e][j] = get(a.w, (long)(c + e) * W + j, a.wtype);
-        err[j][e] = 0.0f;
+      for (int e = 0; e < V; ++e) err[j][e] = 0.0f;
+    const long dense = (long)b * a.T * a.D + c;
+    const T* dy = a.dy ? static_cast<const T*>(a.dy) + dense : nullptr;
+    float xn[W][V], dn[W][V];
+    auto load = [&](int t) {
+#pragma unroll
+      for (int u = 0; u < W; ++u) {
+        const long at = min(t + u, a.T - 1);
+        load_row<V>(r.x + at * a.xt, xn[u]);
+        if (dy) load_row<V>(dy + at * a.D, dn[u]);
       }
-      bias[e] = a.bias ? get(a.bias, c + e, a.wtype) : 0.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < W - 1; ++j) token<T, V>(a, b, c, t0 - (W - 1) + j, win[j]);
-    const T* dy = static_cast<const T*>(a.dy);
+    };
+    load(t0);
     // Errors of the W - 1 tokens behind the run belong to its dx; the first run's
     // errors also go to the state.
-    constexpr int U = 4;
-    for (int t = t0; t < t1 + W - 1; t += U) {
-      float x[U][V], d[U][V];
+    const int end = t1 + W - 1;
+    for (int t = t0; t < end; t += W) {
+      float x[W][V], d[W][V];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        token<T, V>(a, b, c, t + u, x[u]);
-        if (dy && t + u < a.T) {
-          load_row<V>(dy + ((long)b * a.T + t + u) * a.D + c, d[u]);
-        } else {
+      for (int u = 0; u < W; ++u)
 #pragma unroll
-          for (int e = 0; e < V; ++e) d[u][e] = 0.0f;
-        }
-      }
+        for (int e = 0; e < V; ++e) x[u][e] = xn[u][e], d[u][e] = dy ? dn[u][e] : 0.0f;
+      if (t + W < end) load(t + W);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
+      for (int u = 0; u < W; ++u) {
         const int now = t + u;
-        if (now >= t1 + W - 1) break;
-        float g[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) r.win[u][e] = x[u][e];
+        float q[V], p[V];
+        r.sum(u, p);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          win[W - 1][e] = x[u][e];
-          float p = bias[e];
-#pragma unroll
-          for (int j = 0; j < W; ++j) p = fmaf(w[e][j], win[j][e], p);
-          float q = d[u][e];
+          q[e] = d[u][e];
           if (a.silu) {
-            const float s = sigmoid_of(p);
-            q *= s * fmaf(p, 1.0f - s, 1.0f);
+            const float s = sigmoid_of(p[e]);
+            q[e] *= s * fmaf(p[e], 1.0f - s, 1.0f);
           }
-          if (now >= a.T) q = 0.0f;
-          if (now < t1) {
-            db[e] += q;
-#pragma unroll
-            for (int j = 0; j < W; ++j) dw[e][j] = fmaf(q, win[j][e], dw[e][j]);
-          }
-#pragma unroll
-          for (int j = 0; j + 1 < W; ++j) {
-            win[j][e] = win[j + 1][e];
-            err[j][e] = err[j + 1][e];
-          }
-          err[W - 1][e] = q;
-          // dx of token now - W + 1, whose errors are err[0] .. err[W - 1]
-          g[e] = 0.0f;
-#pragma unroll
-          for (int j = 0; j < W; ++j) g[e] = fmaf(w[e][W - 1 - j], err[j][e], g[e]);
+          if (now >= a.T) q[e] = 0.0f;
         }
+        if (now < t1) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) db[e] += q[e];
+#pragma unroll
+          for (int j = 0; j < W; ++j) fma_into(dw[j], q, r.win[(u + 1 + j) % W]);
+        }
+        float g[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) err[u][e] = q[e], g[e] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) fma_into(g, r.w[W - 1 - j], err[(u + 1 + j) % W]);
+        // dx of token now - W + 1
         const int to = now - (W - 1);
-        if (to < t0 && t0 > 0) continue;  // an earlier run's
+        if (now >= end || (to < t0 && t0 > 0)) continue;  // past the run, or an earlier one's
         if (a.dlast && to >= a.T - (W - 1)) {
           float s[V];
           load_row<V>(static_cast<const T*>(a.dlast) + ((long)b * (W - 1) + to - (a.T - (W - 1))) * a.D + c, s);
 #pragma unroll
           for (int e = 0; e < V; ++e) g[e] += s[e];
         }
-        if (to >= 0) store_row<V>(static_cast<T*>(a.dx) + ((long)b * a.T + to) * a.D + c, g);
+        if (to >= 0) store_row<V>(static_cast<T*>(a.dx) + dense + (long)to * a.D, g);
         else if (a.ds0) store_row<V>(static_cast<T*>(a.ds0) + ((long)b * (W - 1) + (W - 1) + to) * a.D + c, g);
       }
     }
   }
   constexpr int C = 32 * V;
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) sums[(warp * (W + 1) + j) * C + lane * V + e] = dw[e][j];
-    sums[(warp * (W + 1) + W) * C + lane * V + e] = db[e];
-  }
+  for (int j = 0; j < W; ++j) store_row<V>(sums + (warp * (W + 1) + j) * C + lane * V, dw[j]);
+  store_row<V>(sums + (warp * (W + 1) + W) * C + lane * V, db);
   __syncthreads();
   for (int i = threadIdx.x; i < (W + 1) * C; i += 32 * kGradRuns) {
     const int col = cb * C + i % C;

@@ -6,7 +6,7 @@
 //
 // A row is in registers from its one read to its one write: a warp holds rows
 // of up to 1024 bf16 or 512 FP32 elements, a CTA longer ones, 16 bytes a thread
-// and load.  A first sum gives a mean that rounding leaves a little off where a row
+// and load; the next row's loads are under way meanwhile.  A first sum gives a mean that rounding leaves a little off where a row
 // has a large offset; the distances from it, which are exact there, give the
 // rest of the mean (`shift`) and the variance, so an offset costs no digits.  y is the norm of s as it is stored: the
 // gradient, which reads s again, sees the same numbers.  CTAs go over the rows
@@ -70,21 +70,34 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const Norm a) {
       w[i * V + e] = c < a.D ? get(a.w, c, a.wtype) : 0.0f;
       b[i * V + e] = c < a.D && a.b ? get(a.b, c, a.wtype) : 0.0f;
     }
-  for (long r = first; r < a.R; r += step) {
+  Raw<TX, V> xn[NV];
+  Raw<TR, V> tn[NV];
+  auto load = [&](long r) {
     const TX* x = static_cast<const TX*>(a.x) + r * a.xs;
     const TR* res = static_cast<const TR*>(a.res) + r * a.rs;
-    float v[NV][V], t[NV][V];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * per + tid) * V;
       if (c < a.D) {
-        load_row<V>(x + c, v[i]);
-        if (RES) load_row<V>(res + c, t[i]);
+        xn[i].load(x + c);
+        if (RES) tn[i].load(res + c);
+      }
+    }
+  };
+  if (first < a.R) load(first);
+  for (long r = first; r < a.R; r += step) {
+    float v[NV][V], t[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if ((i * per + tid) * V < a.D) {
+        xn[i].get(v[i]);
+        if (RES) tn[i].get(t[i]);
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) v[i][e] = t[i][e] = 0.0f;
       }
     }
+    if (r + step < a.R) load(r + step);
     float sum[1] = {0.0f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -149,20 +162,37 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(const Norm a) {
       w[i][e] = c < a.D ? get(a.w, c, a.wtype) : 0.0f;
       dw[i][e] = db[i][e] = 0.0f;
     }
-  int turn = 0;
-  for (long r = first; r < a.R; r += step, turn ^= 1) {
+  Raw<TS, V> sn[NV], dn[NV];
+  Raw<TX, V> gn[NV];
+  float stats[3];
+  auto load = [&](long r) {
     const TS* s = static_cast<const TS*>(a.s) + r * a.xs;
     const TX* dy = static_cast<const TX*>(a.dy) + r * a.dys;
-    float n[NV][V], g[NV][V];
+    const TS* ds = static_cast<const TS*>(a.ds) + r * a.dss;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * per + tid) * V;
       if (c < a.D) {
-        load_row<V>(s + c, n[i]);
-        load_row<V>(dy + c, g[i]);
+        sn[i].load(s + c);
+        gn[i].load(dy + c);
+        if (a.ds) dn[i].load(ds + c);
       }
     }
-    const float mean = a.stats[r], shift = a.stats[a.R + r], rstd = a.stats[2 * a.R + r];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) stats[k] = a.stats[k * a.R + r];
+  };
+  if (first < a.R) load(first);
+  int turn = 0;
+  for (long r = first; r < a.R; r += step, turn ^= 1) {
+    float n[NV][V], g[NV][V], ds[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      sn[i].get(n[i]);
+      gn[i].get(g[i]);
+      if (a.ds) dn[i].get(ds[i]);
+    }
+    const float mean = stats[0], shift = stats[1], rstd = stats[2];
+    if (r + step < a.R) load(r + step);
     float sums[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -186,12 +216,9 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(const Norm a) {
       if (c >= a.D) continue;
 #pragma unroll
       for (int e = 0; e < V; ++e) g[i][e] = rstd * (g[i][e] - m0 - n[i][e] * m1);
-      if (a.ds) {
-        float t[V];
-        load_row<V>(static_cast<const TS*>(a.ds) + r * a.dss + c, t);
+      if (a.ds)
 #pragma unroll
-        for (int e = 0; e < V; ++e) g[i][e] += t[e];
-      }
+        for (int e = 0; e < V; ++e) g[i][e] += ds[i][e];
       if (a.dx) store_row<V>(static_cast<TX*>(a.dx) + r * a.D + c, g[i]);
       if (a.dres) store_row<V>(static_cast<TS*>(a.dres) + r * a.D + c, g[i]);
     }

@@ -104,30 +104,68 @@ __device__ __forceinline__ float warp_sum(float x) {
   return x;
 }
 
+// N consecutive elements as they are stored, so that a load can be under way
+// while the numbers before it are worked on.
+template <typename T, int N>
+struct Raw {
+  static constexpr int kBytes = N * (int)sizeof(T), kWords = kBytes / 4;
+  static_assert(N == 1 || kBytes == 8 || kBytes % 16 == 0, "one element, or whole accesses");
+  unsigned v[kWords > 0 ? kWords : 1];
+  T one;
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (N == 1) {
+      one = *p;
+    } else if constexpr (kBytes == 8) {
+      const uint2 r = *reinterpret_cast<const uint2*>(p);
+      v[0] = r.x, v[1] = r.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 r = reinterpret_cast<const uint4*>(p)[i / 4];
+        v[i] = r.x, v[i + 1] = r.y, v[i + 2] = r.z, v[i + 3] = r.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[N]) const {
+    if constexpr (N == 1) {
+      f[0] = to_f32(one);
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = __uint_as_float(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) f[2 * i] = __uint_as_float(v[i] << 16), f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+    }
+  }
+};
+
 // store(c, sum over p of part[p * stride + c]) for c < cols: FP64 sums in a
-// fixed order, so results do not change from run to run.
-constexpr int kSumRows = 8;
-template <typename Store>
-__global__ void __launch_bounds__(32 * kSumRows) sum_parts_kernel(const float* __restrict__ part, int parts, long stride,
-                                                                  long cols, Store store) {
-  __shared__ double s[kSumRows][33];
+// fixed order, so results do not change from run to run.  ROWS threads share a
+// column.
+template <typename Store, int ROWS>
+__global__ void __launch_bounds__(32 * ROWS) sum_parts_kernel(const float* __restrict__ part, int parts, long stride,
+                                                              long cols, Store store) {
+  __shared__ double s[ROWS][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const long c = blockIdx.x * 32L + tx;
   double acc = 0.0;
   if (c < cols)
-#pragma unroll 4
-    for (int p = ty; p < parts; p += kSumRows) acc += (double)part[p * stride + c];
+#pragma unroll 8
+    for (int p = ty; p < parts; p += ROWS) acc += (double)part[p * stride + c];
   s[ty][tx] = acc;
   __syncthreads();
-  if (ty == 0 && c < cols) {
 #pragma unroll
-    for (int r = 1; r < kSumRows; ++r) acc += s[r][tx];
-    store(c, (float)acc);
+  for (int n = ROWS / 2; n > 0; n /= 2) {
+    if (ty < n) s[ty][tx] += s[ty + n][tx];
+    __syncthreads();
   }
+  if (ty == 0 && c < cols) store(c, (float)s[0][tx]);
 }
 template <typename Store>
 int sum_parts(const float* part, int parts, long stride, long cols, Store store, cudaStream_t stream) {
-  sum_parts_kernel<<<(unsigned)((cols + 31) / 32), 32 * kSumRows, 0, stream>>>(part, parts, stride, cols, store);
+  const unsigned ctas = (unsigned)((cols + 31) / 32);
+  if (parts > 32) sum_parts_kernel<Store, 32><<<ctas, 1024, 0, stream>>>(part, parts, stride, cols, store);
+  else sum_parts_kernel<Store, 4><<<ctas, 128, 0, stream>>>(part, parts, stride, cols, store);
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
 }

@@ -50,22 +50,27 @@ __device__ __forceinline__ float exp2_of(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max_nan(float x, float y) {  // NaN where either is
+  float z;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+__device__ __forceinline__ float min_nan(float x, float y) {
+  float z;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+
 // A in powers of two, kept finite: a token that is not there has dt = 0, and
 // 0 * infinity would make its decay NaN, not 1.
 __device__ __forceinline__ float decay_rate(float a) {
-  const float r = a * 1.4426950408889634f;
-  return r < -3.0e38f ? -3.0e38f : r > 3.0e38f ? 3.0e38f : r;
+  return min_nan(max_nan(a * 1.4426950408889634f, -3.0e38f), 3.0e38f);
 }
 
 __device__ __forceinline__ float rcp_of(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-__device__ __forceinline__ float max_nan(float x, float y) {  // NaN where either is
-  float z;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
-  return z;
 }
 __device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
 

@@ -18,55 +18,62 @@ namespace {
 constexpr int kStepThreads = 256;
 
 // LP: lanes of a channel; K: channels a thread takes one after another, whose
-// loads are in flight together.  vec: states lie in aligned fours.
+// loads are in flight together.  vec: states, and groups of B and C, lie in aligned
+// fours.
 template <typename T, int LP, int K>
 __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const Problem p, float* state, int vec, int blocks) {
   constexpr int kSlots = kStepThreads / LP;
   const int b = blockIdx.x / blocks, part = threadIdx.x % LP, slot = threadIdx.x / LP;
   const int d0 = (blockIdx.x - b * blocks) * (kSlots * K) + slot;
   const int n0 = 4 * part, left = p.N - n0;
-  float h[K][4], a[K][4];
+  float h[K][4], a[K][4], x[K], dt[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int d = d0 + k * kSlots;
+    const int d = min(d0 + k * kSlots, p.D - 1);  // loads without a branch; the last channel is not written twice
     const float* s = state + ((long)b * p.D + d) * p.N + n0;
     const float* r = p.a + (long)d * p.N + n0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) h[k][j] = a[k][j] = 0.0f;
-    if (d >= p.D) continue;
+    x[k] = to_f32(static_cast<const T*>(p.x)[b * p.xb + d]);
+    dt[k] = to_f32(static_cast<const T*>(p.dt)[b * p.dtb + d]);
     if (vec) {
-      if (left > 0) {
-        const float4 v = __ldcs(reinterpret_cast<const float4*>(s));
-        const float4 u = __ldg(reinterpret_cast<const float4*>(r));
-        h[k][0] = v.x, h[k][1] = v.y, h[k][2] = v.z, h[k][3] = v.w;
-        a[k][0] = u.x, a[k][1] = u.y, a[k][2] = u.z, a[k][3] = u.w;
-      }
+      const int at = left > 0 ? 0 : -n0;  // lanes without states read the channel's first
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(s + at));
+      const float4 u = __ldg(reinterpret_cast<const float4*>(r + at));
+      h[k][0] = v.x, h[k][1] = v.y, h[k][2] = v.z, h[k][3] = v.w;
+      a[k][0] = u.x, a[k][1] = u.y, a[k][2] = u.z, a[k][3] = u.w;
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < left) h[k][j] = s[j], a[k][j] = r[j];
+      for (int j = 0; j < 4; ++j) h[k][j] = j < left ? s[j] : 0.0f, a[k][j] = j < left ? r[j] : 0.0f;
     }
   }
+  float bv[4], cv[4];
+  int group = -1;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int d = d0 + k * kSlots;
-    const bool in = d < p.D;
-    const int group = in ? d / p.R : 0;
-    const long db = in ? d : 0;
-    const float x = to_f32(static_cast<const T*>(p.x)[b * p.xb + db]);
-    const float step = step_of(p.softplus, to_f32(static_cast<const T*>(p.dt)[b * p.dtb + db]), p.bias ? p.bias[db] : 0.0f);
-    const T* bm = static_cast<const T*>(p.b) + b * p.bb + group * p.bg + n0;
-    const T* cm = static_cast<const T*>(p.c) + b * p.cb + group * p.cg + n0;
+    const int d = min(d0 + k * kSlots, p.D - 1);
+    const int g = p.G == 1 ? 0 : d / p.R;
+    if (g != group) {
+      group = g;
+      const T* bm = static_cast<const T*>(p.b) + b * p.bb + g * p.bg + n0;
+      const T* cm = static_cast<const T*>(p.c) + b * p.cb + g * p.cg + n0;
+      if (vec && left > 0) {
+        load_row<4>(bm, bv);
+        load_row<4>(cm, cv);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bv[j] = j < left ? to_f32(bm[j]) : 0.0f, cv[j] = j < left ? to_f32(cm[j]) : 0.0f;
+      }
+    }
+    const float step = step_of(p.softplus, dt[k], p.bias ? p.bias[d] : 0.0f), du = step * x[k];
     float y = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float bv = j < left ? to_f32(bm[j]) : 0.0f, cv = j < left ? to_f32(cm[j]) : 0.0f;
-      h[k][j] = fmaf(exp2_of(step * decay_rate(a[k][j])), h[k][j], step * x * bv);
-      y = fmaf(cv, h[k][j], y);
+      h[k][j] = fmaf(exp2_of(step * decay_rate(a[k][j])), h[k][j], du * bv[j]);
+      y = fmaf(cv[j], h[k][j], y);
     }
+    if (left <= 0) y = 0.0f;
 #pragma unroll
     for (int o = LP / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (!in) continue;
+    if (d0 + k * kSlots >= p.D) continue;
     float* s = state + ((long)b * p.D + d) * p.N + n0;
     if (vec) {
       if (left > 0) __stcs(reinterpret_cast<float4*>(s), make_float4(h[k][0], h[k][1], h[k][2], h[k][3]));
@@ -76,10 +83,10 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const Problem p
         if (j < left) s[j] = h[k][j];
     }
     if (part == 0) {
-      if (p.skip) y = fmaf(p.skip[d], x, y);
+      if (p.skip) y = fmaf(p.skip[d], x[k], y);
       if (p.z) {
         const float gate = to_f32(static_cast<const T*>(p.z)[b * p.zb + d]);
-        y *= gate * sigmoid_of(gate);
+        y *= gate * gate_of(gate);
       }
       static_cast<T*>(p.out)[(long)b * p.D + d] = from_f32<T>(y);
     }
@@ -303,7 +310,9 @@ extern "C" int gru_scan_step(const gru_scan_args* p, float* state, void* out, vo
   Problem a{};
   fill(a, *p);
   a.out = out;
-  const int vec = p->N % 4 == 0 && ((bits(state) | bits(p->a)) & 15) == 0;
+  const uintptr_t four = 4 * elem_size(p->dtype) - 1;
+  const int vec = p->N % 4 == 0 && ((bits(state) | bits(p->a)) & 15) == 0 && ((bits(p->b) | bits(p->c)) & four) == 0 &&
+                  (p->b_stride[0] | p->b_stride[2] | p->c_stride[0] | p->c_stride[2]) % 4 == 0;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   return p->dtype == GRU_F32 ? step<float>(a, state, vec, stream) : step<bf16>(a, state, vec, stream);
 }
