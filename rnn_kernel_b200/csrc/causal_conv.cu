@@ -33,7 +33,7 @@ struct Conv {
   void *dx, *ds0;
   float* part;  // [CTA of tokens][W + 1][D]
   long xb, xt;  // elements between x's batch rows and tokens
-  int B, T, D, W, wtype, silu, run, runs;
+  int B, T, D, W, wtype, wvec, silu, run, runs;  // wvec: weights lie on boundaries of V elements
 };
 
 // a[e] b[e] + c[e], neighbours packed.
@@ -51,6 +51,21 @@ __device__ __forceinline__ void fma_into(float (&c)[V], const float (&a)[V], con
   }
 }
 
+// The weights of channels c .. c + V - 1.
+template <int W, int V>
+__device__ __forceinline__ void weights(const Conv& a, int c, float (&w)[W][V], float (&bias)[V]) {
+  float flat[W][V];  // V channels x W weights, as they lie
+#pragma unroll
+  for (int i = 0; i < W; ++i) get_row<V>(a.w, (long)c * W + i * V, a.wtype, a.wvec, flat[i]);
+  get_row<V>(a.bias ? a.bias : a.w, c, a.wtype, a.wvec, bias);
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[j][e] = flat[(e * W + j) / V][(e * W + j) % V];
+    if (!a.bias) bias[e] = 0.0f;
+  }
+}
+
 // A thread's channels c .. c + V - 1 of batch row b.
 template <typename T, int W, int V>
 struct Run {
@@ -59,12 +74,7 @@ struct Run {
   __device__ __forceinline__ Run(const Conv& a, int b, int c) {
     x = static_cast<const T*>(a.x) + b * a.xb + c;
     s0 = a.s0 ? static_cast<const T*>(a.s0) + ((long)b * (W - 1) + W - 1) * a.D + c : nullptr;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-#pragma unroll
-      for (int j = 0; j < W; ++j) w[j][e] = get(a.w, (long)(c + e) * W + j, a.wtype);
-      bias[e] = a.bias ? get(a.bias, c + e, a.wtype) : 0.0f;
-    }
+    weights<W, V>(a, c, w, bias);
   }
   // Token t, which may lie before the first.
   __device__ __forceinline__ void any(const Conv& a, int t, float (&v)[V]) const {
@@ -248,7 +258,8 @@ __global__ void __launch_bounds__(128) conv_step_kernel(const Conv a) {
   const int b = (int)(item / vecs), c = (int)(item - (long)b * vecs) * V;
   if (b >= a.B) return;
   T* s = static_cast<T*>(a.last) + (long)b * (W - 1) * a.D + c;
-  float win[W][V], p[V];
+  float win[W][V], w[W][V], p[V];
+  weights<W, V>(a, c, w, p);
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) load_row<V>(s + (long)j * a.D, win[j]);
   load_row<V>(static_cast<const T*>(a.x) + b * a.xb + c, win[W - 1]);
@@ -256,9 +267,8 @@ __global__ void __launch_bounds__(128) conv_step_kernel(const Conv a) {
   for (int j = 0; j < W - 1; ++j) store_row<V>(s + (long)j * a.D, win[j + 1]);
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    p[e] = a.bias ? get(a.bias, c + e, a.wtype) : 0.0f;
 #pragma unroll
-    for (int j = 0; j < W; ++j) p[e] = fmaf(get(a.w, (long)(c + e) * W + j, a.wtype), win[j][e], p[e]);
+    for (int j = 0; j < W; ++j) p[e] = fmaf(w[j][e], win[j][e], p[e]);
     if (a.silu) p[e] *= sigmoid_of(p[e]);
   }
   store_row<V>(static_cast<T*>(a.y) + (long)b * a.D + c, p);
@@ -338,6 +348,8 @@ void fill(Conv& a, const gru_conv_args& p) {
   a.x = p.x, a.w = p.weight, a.bias = p.bias, a.s0 = p.initial_state;
   a.xb = p.x_stride[0], a.xt = p.x_stride[1];
   a.B = p.B, a.T = p.T, a.D = p.D, a.W = p.W, a.wtype = p.weight_dtype, a.silu = p.activation;
+  const int v = p.W <= 4 ? 4 : 2;
+  a.wvec = ((bits(p.weight) | bits(p.bias)) & (v * elem_size(p.weight_dtype) - 1)) == 0;
 }
 
 // Whether every row of the dense tensors and of x starts on the boundary that V

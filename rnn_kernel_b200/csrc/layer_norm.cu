@@ -32,7 +32,7 @@ struct Norm {
   void *dx, *dres;
   float* part;  // [CTA][2][D]
   long R, xs, rs, dys, dss;  // rows, and elements between them
-  int D, wtype;
+  int D, wtype, wvec;  // wvec: the weights lie on boundaries of a load
   float eps;
 };
 
@@ -61,15 +61,16 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const Norm a) {
   const long first = CTA ? blockIdx.x : (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const long step = CTA ? gridDim.x : (long)gridDim.x * (blockDim.x >> 5);
   const float inv = 1.0f / (float)a.D;
-  float w[NV * V], b[NV * V];
+  float w[NV][V], b[NV][V];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    const int c = min((i * per + tid) * V, a.D - V);  // threads past the row read its last
+    get_row<V>(a.w, c, a.wtype, a.wvec, w[i]);
+    get_row<V>(a.b ? a.b : a.w, c, a.wtype, a.wvec, b[i]);
+    if (!a.b)
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int c = (i * per + tid) * V + e;
-      w[i * V + e] = c < a.D ? get(a.w, c, a.wtype) : 0.0f;
-      b[i * V + e] = c < a.D && a.b ? get(a.b, c, a.wtype) : 0.0f;
-    }
+      for (int e = 0; e < V; ++e) b[i][e] = 0.0f;
+  }
   Raw<TX, V> xn[NV];
   Raw<TR, V> tn[NV];
   auto load = [&](long r) {
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const Norm a) {
       const int c = (i * per + tid) * V;
       if (c >= a.D) continue;
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[i][e] = (v[i][e] - shift) * rstd * w[i * V + e] + b[i * V + e];
+      for (int e = 0; e < V; ++e) v[i][e] = (v[i][e] - shift) * rstd * w[i][e] + b[i][e];
       store_row<V>(static_cast<TX*>(a.y) + r * a.D + c, v[i]);
     }
   }
@@ -155,13 +156,11 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(const Norm a) {
   const float inv = 1.0f / (float)a.D;
   float w[NV][V], dw[NV][V], db[NV][V];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    get_row<V>(a.w, min((i * per + tid) * V, a.D - V), a.wtype, a.wvec, w[i]);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int c = (i * per + tid) * V + e;
-      w[i][e] = c < a.D ? get(a.w, c, a.wtype) : 0.0f;
-      dw[i][e] = db[i][e] = 0.0f;
-    }
+    for (int e = 0; e < V; ++e) dw[i][e] = db[i][e] = 0.0f;
+  }
   Raw<TS, V> sn[NV], dn[NV];
   Raw<TX, V> gn[NV];
   float stats[3];
@@ -391,6 +390,7 @@ extern "C" int gru_layer_norm_forward(const gru_norm_args* p, const void* x, con
   const int v = p->dtype == GRU_F32 ? 4 : 8;
   const bool vec = a.D % v == 0 && a.xs % v == 0 && (!residual || a.rs % v == 0) &&
                    ((bits(x) | bits(residual) | bits(out) | bits(sum)) & 15) == 0;
+  a.wvec = vec && ((bits(weight) | bits(bias)) & 15) == 0;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (p->dtype == GRU_F32) {
     if (residual) return vec ? launch_forward<float, float, true, 4>(a, stream) : launch_forward<float, float, true, 1>(a, stream);
@@ -432,6 +432,7 @@ extern "C" int gru_layer_norm_backward(const gru_norm_args* p, const void* sum, 
   const int v = p->dtype == GRU_F32 ? 4 : 8;
   const bool vec = a.D % v == 0 && a.xs % v == 0 &&
                    ((bits(sum) | bits(dout) | bits(dsum) | bits(dx) | bits(dresidual)) & 15) == 0;
+  a.wvec = vec && (bits(weight) & 15) == 0;
   const StoreNorm store{dweight, dbias, a.D, p->weight_dtype};
   if (p->dtype == GRU_F32)
     return vec ? launch_backward<float, float, 4>(a, store, stream) : launch_backward<float, float, 1>(a, store, stream);

@@ -179,6 +179,30 @@ __device__ __forceinline__ float get(const void* p, long i, int dtype) {
   return dtype == GRU_F32 ? static_cast<const float*>(p)[i] : __bfloat162float(static_cast<const bf16*>(p)[i]);
 }
 
+// N elements of a parameter from i on as FP32.  whole: they lie on a boundary of
+// min(16, N elements) bytes.  One branch on the type around all loads: a branch
+// around each would wait for each (16 of them took 10 us at a kernel's start).
+template <int N>
+__device__ __forceinline__ void get_row(const void* p, long i, int dtype, bool whole, float (&v)[N]) {
+  if (dtype == GRU_F32) {
+    const float* f = static_cast<const float*>(p) + i;
+    if (whole) {
+      load_row<N>(f, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = f[e];
+    }
+  } else {
+    const bf16* f = static_cast<const bf16*>(p) + i;
+    if (whole) {
+      load_row<N>(f, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = __bfloat162float(f[e]);
+    }
+  }
+}
+
 inline int refuse(const char* what, const char* msg, int code = GRU_ERR_INVALID) {
   set_error(std::string(what) + ": " + msg);
   return code;

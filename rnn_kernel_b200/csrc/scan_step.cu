@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const Problem p
   const int b = blockIdx.x / blocks, part = threadIdx.x % LP, slot = threadIdx.x / LP;
   const int d0 = (blockIdx.x - b * blocks) * (kSlots * K) + slot;
   const int n0 = 4 * part, left = p.N - n0;
-  float h[K][4], a[K][4], x[K], dt[K];
+  float h[K][4], a[K][4], x[K], dt[K], z[K], bias[K], skip[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int d = min(d0 + k * kSlots, p.D - 1);  // loads without a branch; the last channel is not written twice
@@ -34,6 +34,9 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const Problem p
     const float* r = p.a + (long)d * p.N + n0;
     x[k] = to_f32(static_cast<const T*>(p.x)[b * p.xb + d]);
     dt[k] = to_f32(static_cast<const T*>(p.dt)[b * p.dtb + d]);
+    z[k] = to_f32(p.z ? static_cast<const T*>(p.z)[b * p.zb + d] : static_cast<const T*>(p.x)[b * p.xb + d]);
+    bias[k] = *(p.bias ? p.bias + d : p.a);
+    skip[k] = *(p.skip ? p.skip + d : p.a);
     if (vec) {
       const int at = left > 0 ? 0 : -n0;  // lanes without states read the channel's first
       const float4 v = __ldcs(reinterpret_cast<const float4*>(s + at));
@@ -63,7 +66,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const Problem p
         for (int j = 0; j < 4; ++j) bv[j] = j < left ? to_f32(bm[j]) : 0.0f, cv[j] = j < left ? to_f32(cm[j]) : 0.0f;
       }
     }
-    const float step = step_of(p.softplus, dt[k], p.bias ? p.bias[d] : 0.0f), du = step * x[k];
+    const float step = step_of(p.softplus, dt[k], p.bias ? bias[k] : 0.0f), du = step * x[k];
     float y = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -83,11 +86,8 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const Problem p
         if (j < left) s[j] = h[k][j];
     }
     if (part == 0) {
-      if (p.skip) y = fmaf(p.skip[d], x[k], y);
-      if (p.z) {
-        const float gate = to_f32(static_cast<const T*>(p.z)[b * p.zb + d]);
-        y *= gate * gate_of(gate);
-      }
+      if (p.skip) y = fmaf(skip[k], x[k], y);
+      if (p.z) y *= z[k] * gate_of(z[k]);
       static_cast<T*>(p.out)[(long)b * p.D + d] = from_f32<T>(y);
     }
   }
