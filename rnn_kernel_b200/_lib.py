@@ -8,10 +8,12 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import importlib.machinery
 import importlib.util
 import struct
 import threading
+import warnings
 from pathlib import Path
 
 import torch
@@ -211,7 +213,7 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
 
 
 def host():
-    """The Python module of csrc/host_tensors.cpp (built first if needed); raises where it cannot be built or loaded."""
+    """The Python module of csrc/host_*.cpp (built first if needed); raises where it cannot be built or loaded."""
     global _host
     with _lock:
         if _host is None:
@@ -221,6 +223,20 @@ def host():
             loader.exec_module(module)
             _host = module
         return _host
+
+
+@functools.lru_cache(maxsize=1)
+def operators():
+    """The module above with the library's entries, for the usual calls of the scan, the convolution and the norm; None
+    (said once) where it cannot be built: their Python does the same."""
+    try:
+        module, lib = host(), load()
+        module.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in SIGNATURES})
+        return module
+    except Exception as e:  # no compiler, no headers, a module that does not load
+        warnings.warn(f"the scan, the convolution and the norm are called in Python, some 10 us more a call: the module _host "
+                      f"is not available ({e})")
+        return None
 
 
 def last_error() -> str:

@@ -3,11 +3,12 @@
 ``python -m rnn_kernel_b200.build`` (or ``build()``) compiles every ``.cu`` in
 ``csrc/`` with nvcc into one shared library next to this file.  The library
 has a plain C ABI (``include/rnn_kernel_b200.h``) and is loaded with ctypes.
-``csrc/host_tensors.cpp`` becomes the Python module ``_host`` beside it
-(``build_host()``), which reads torch tensors' addresses for AdamW.  The library
-needs nvcc alone; the module needs a C++ compiler and the headers of the
-installed Python and torch, and carries both versions in its file's name, so
-that after an upgrade of either a new one is built and the old one left alone.
+``csrc/host_*.cpp`` become the Python module ``_host`` beside it
+(``build_host()``), which reads torch tensors' addresses for AdamW and makes the
+usual calls of the newer operators.  The library needs nvcc alone; the module
+needs a C++ compiler and the headers of CUDA and the installed Python and torch,
+and carries the versions of these two in its file's name, so that after an
+upgrade of either a new one is built and the old one left alone.
 """
 from __future__ import annotations
 
@@ -30,7 +31,7 @@ if VARIANT not in ("", "timeline"):
     raise ValueError(f"RNN_KERNEL_B200_VARIANT must be unset or 'timeline', got {VARIANT!r}")
 LIB_NAME = "librnn_kernel_b200_timeline.so" if VARIANT else "librnn_kernel_b200.so"
 LIB_PATH = PKG / LIB_NAME
-HOST_SOURCE = CSRC / "host_tensors.cpp"
+HOST_SOURCES = [CSRC / "host_tensors.cpp", CSRC / "host_operators.cpp"]
 VARIANT_FLAGS = ["-DGRU_TIMELINE"] if VARIANT == "timeline" else []
 
 NVCC_FLAGS = [
@@ -71,18 +72,20 @@ def host_path() -> Path:
 
 
 def build_host(force: bool = False, verbose: bool = False) -> Path:
-    """Compiles the module ``_host`` if it is missing or older than its source."""
+    """Compiles the module ``_host`` if it is missing or older than a source of its."""
     import torch
 
     path = host_path()
-    if not force and not _stale(path, [HOST_SOURCE]):
+    if not force and not _stale(path, [*HOST_SOURCES, *CSRC.glob("host_*.h")]):
         return path
     base = Path(torch.__file__).parent
     tmp = path.with_name(f"{path.name}.{os.getpid()}.so.tmp")  # ranks may build at the same time
-    include = [base / "include", base / "include/torch/csrc/api/include", sysconfig.get_paths()["include"]]
+    cuda = Path(nvcc_path()).resolve().parent.parent
+    include = [base / "include", base / "include/torch/csrc/api/include", sysconfig.get_paths()["include"], cuda / "include"]
     cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{i}" for i in include),
-           str(HOST_SOURCE), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-o", str(tmp)]
+           *map(str, HOST_SOURCES), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-o", str(tmp)]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)
@@ -110,4 +113,4 @@ if __name__ == "__main__":
     try:
         build_host(force="--force" in sys.argv, verbose=True)
     except (OSError, subprocess.CalledProcessError) as e:
-        print(f"the module _host was not built ({e}); AdamW reads its tensors in Python", file=sys.stderr)
+        print(f"the module _host was not built ({e}); its calls are made in Python", file=sys.stderr)

@@ -5,6 +5,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/rnn_kernel_b200.h"
+#include "host_operators.h"
 
 namespace {
 
@@ -45,4 +46,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, null
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__host() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddFunctions(m, operator_methods()) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -176,6 +176,11 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
                residual: Optional[torch.Tensor] = None):
     """The norm of x over its last dimension; with a ``residual`` of x's shape, ``(norm of x + residual, x + residual)``."""
     eps = float(eps)
+    fast = _lib.operators()
+    if fast is not None and forward_ad._current_level < 0:
+        got = fast.layer_norm(x, weight, bias, eps, residual)
+        if got is not None:
+            return got
     if _differentiated(x, weight, bias, residual):
         out, s = LayerNormFunction.apply(x, weight, bias, residual, eps)
     else:

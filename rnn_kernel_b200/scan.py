@@ -30,6 +30,7 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _lib
 from .norm import LayerNorm, _check_device, _differentiated, _first_derivatives, _no_tangents
@@ -39,6 +40,12 @@ CONV_SIZES = range(2, 9)
 
 _DTYPES = {torch.float32: _lib.GRU_F32, torch.bfloat16: _lib.GRU_BF16}
 _ACTIVATIONS = {None: 0, "silu": 1}
+
+
+def _fast(name, *args):
+    """The call by the module in C++, or None where it leaves it to Python."""
+    module = _lib.operators()
+    return None if module is None or forward_ad._current_level >= 0 else getattr(module, name)(*args)
 
 
 def _dense_last(t):
@@ -174,6 +181,9 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     last dimension are free.
     """
     softplus = bool(dt_softplus)
+    got = _fast("selective_scan", x, dt, A, B, C, skip, z, dt_bias, softplus, initial_state)
+    if got is not None:
+        return got
     if _differentiated(x, dt, A, B, C, skip, z, dt_bias, initial_state):
         return SelectiveScanFunction.apply(x, dt, A, B, C, skip, z, dt_bias, softplus, initial_state)
     code, dev = _check("selective_scan", x, dt, A, B, C, skip, z, dt_bias, initial_state, 2)
@@ -187,6 +197,9 @@ def selective_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
 
     ``x``, ``dt``, ``z``: [B, D]; ``B``, ``C``: [B, G, N].  No gradient.
     """
+    got = _fast("selective_step", x, dt, A, B, C, state, skip, z, dt_bias, bool(dt_softplus))
+    if got is not None:
+        return got
     code, dev = _check("selective_step", x, dt, A, B, C, skip, z, dt_bias, state, 1)
     _no_tangents("selective_step", x, dt, A, B, C, skip, z, dt_bias, state)
     if not state.is_contiguous():
@@ -201,7 +214,8 @@ def selective_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     with _lib.on_device(dev):
         out = x.new_empty((b, D))
         _lib.check(_lib.load().gru_scan_step(a, state.data_ptr(), out.data_ptr(), _lib.raw_stream(dev)), "gru_scan_step")
-    torch.autograd.graph.increment_version(state)
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)
     return out
 
 
@@ -284,6 +298,9 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     ``x``: [B, T, D], strides free but the last; ``weight``: [D, W], 2 <= W <= 8; ``activation``: None or
     "silu"; ``initial_state``: the W - 1 inputs before the first, oldest first (default zeros).
     """
+    got = _fast("causal_conv", x, weight, bias, activation, initial_state)
+    if got is not None:
+        return got
     if _differentiated(x, weight, bias, initial_state):
         return CausalConvFunction.apply(x, weight, bias, activation, initial_state)
     code, dev = _check_conv("causal_conv", x, weight, bias, initial_state, activation, 2)
@@ -293,6 +310,9 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
 def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor, bias: Optional[torch.Tensor] = None,
                      activation: Optional[str] = None) -> torch.Tensor:
     """One token, ``x`` [B, D] -> [B, D]; ``state`` [B, W - 1, D] (contiguous) is moved on in place.  No gradient."""
+    got = _fast("causal_conv_step", x, weight, state, bias, activation)
+    if got is not None:
+        return got
     code, dev = _check_conv("causal_conv_step", x, weight, bias, state, activation, 1)
     _no_tangents("causal_conv_step", x, weight, bias, state)
     if not state.is_contiguous():
@@ -303,7 +323,8 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor,
     with _lib.on_device(dev):
         out = x.new_empty(x.shape)
         _lib.check(_lib.load().gru_conv_step(a, state.data_ptr(), out.data_ptr(), _lib.raw_stream(dev)), "gru_conv_step")
-    torch.autograd.graph.increment_version(state)
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)
     return out
 
 

@@ -1,8 +1,20 @@
 """Plain 64-bit selective scan, causal convolution and layer norm for the tests (torch, any device; differentiable by autograd)."""
 import math
 
+import pytest
 import torch
 import torch.nn.functional as F
+
+from rnn_kernel_b200 import _lib
+
+
+@pytest.fixture(autouse=True, params=["C++", "Python"])
+def caller(request, monkeypatch):
+    """Every test that imports this runs with the calls made by the module in C++ and with those made in Python."""
+    if request.param == "Python":
+        monkeypatch.setattr(_lib, "operators", lambda: None)
+    else:
+        assert _lib.operators() is not None
 
 
 def scan(x, dt, A, B, C, skip=None, z=None, dt_bias=None, dt_softplus=False, initial_state=None):

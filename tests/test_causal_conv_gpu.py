@@ -11,6 +11,7 @@ import torch
 from rnn_kernel_b200 import causal_conv, causal_conv_step
 
 from . import scan_reference as R
+from .scan_reference import caller  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 

@@ -6,6 +6,7 @@ import torch.nn.functional as F
 from rnn_kernel_b200 import GRU, DataParallelTrainer, GatedDelta, GraphedTrainStep, RecurrentStack, SelectiveScan
 
 from . import scan_reference as R
+from .scan_reference import caller  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
