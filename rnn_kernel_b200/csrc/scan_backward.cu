@@ -49,8 +49,8 @@ __host__ __device__ inline Lay layout(int warps, int np, int N, int elem) {
   l.gz = n, n += kBlock * kTile;  // dout silu'(z)
   l.bs = n, n += np * kRow;
   l.cs = n, n += np * kRow;
-  l.part = n, n += warps * 3 * kHalf * kTile;  // [pair of tokens][y, sum B dh, sum A w][warp][lane] float4
-  l.marks = n, n += np * kTile;
+  l.part = n, n += warps * 3 * kHalf * kTile;  // [token][y, sum B dh, sum A w][warp][lane] float2
+  l.marks = n, n += 2 * np * kTile;  // of this block and the next
   l.in = n, n += 4 * kBlock * kTile * elem / 4;
   l.few = n, n += 2 * kBlock * N * elem / 4;
   l.sums = n, n += 2 * warps * kTile;
@@ -91,21 +91,21 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
   T* few = reinterpret_cast<T*>(sm + l.few);
   constexpr int kRows = kBlock * kTile;
   Feed<T> feed;
-  feed.init(p, q, bm, cm);
+  feed.init(p, bm, cm);
   auto fetch = [&](int t0) {
-    feed.row(in, x, p.xst, t0, lastt, q.width, true);
-    feed.row(in + kRows, dt, p.dtst, t0, lastt, q.width, true);
-    if (z) feed.row(in + 2 * kRows, z, p.zst, t0, lastt, q.width, true);
-    if (dout) feed.row(in + 3 * kRows, dout, p.ost, t0, lastt, q.width, p.wide_dout);
+    feed.row(in, x, p.xst, t0, lastt, q.width, p.row_piece);
+    feed.row(in + kRows, dt, p.dtst, t0, lastt, q.width, p.row_piece);
+    if (z) feed.row(in + 2 * kRows, z, p.zst, t0, lastt, q.width, p.row_piece);
+    if (dout) feed.row(in + 3 * kRows, dout, p.ost, t0, lastt, q.width, p.dout_piece);
     feed.bc(p, few, bm, cm, t0, lastt);
   };
-  auto fetch_marks = [&](int t0) {
+  auto fetch_marks = [&](int t0, int buf) {
     const float4* from = reinterpret_cast<const float4*>(p.marks + ((long)q.unit * p.nmarks + t0 / kBlock) * p.np * kTile);
-    for (int e = threadIdx.x; e < p.np * kTile / 4; e += threads) copy16(reinterpret_cast<float4*>(sm + l.marks) + e, from + e);
+    for (int e = threadIdx.x; e < p.np * kTile / 4; e += threads) copy<16>(reinterpret_cast<float4*>(sm + l.marks + buf * p.np * kTile) + e, from + e);
   };
   const int start = q.first + (lastt - q.first) / kBlock * kBlock;  // the last block
   fetch(start);
-  if (!SUM) fetch_marks(start);
+  if (!SUM) fetch_marks(start, 0);
 
   // states 2 (g warps + w) and the next
   float2 rt[GW][2], back[GW][2], da[GW][2];
@@ -134,8 +134,9 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
     }
 
   float4* rows = reinterpret_cast<float4*>(sm) + lane;  // [array][pair of tokens][lane]
-  const int a_step = l.step / 4, a_du = l.du / 4, a_gy = l.gy / 4, a_xs = l.xs / 4, a_sg = l.sg / 4, a_gz = l.gz / 4;
-  float4* shares = reinterpret_cast<float4*>(sm + l.part) + lane;
+  const int a_step = l.step / 4, a_du = l.du / 4, a_gy = l.gy / 4;
+  float2* shares = reinterpret_cast<float2*>(sm + l.part) + lane;
+  float2* ends = reinterpret_cast<float2*>(sm) + lane;  // [array][token][lane], of what finish() alone reads
   // What two tokens have per channel.
   auto prepare = [&](int t0) {
     for (int u = w; u < kPairs; u += warps) {
@@ -167,7 +168,14 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
           if (!(i & 1 ? q.second : q.live) || t + i / 2 > lastt) s[i] = v[i] = g[i] = 0.0f;
       float4* to = rows + u * kLanes;
       to[a_step] = as4(s), to[a_du] = as4(v), to[a_gy] = as4(g);
-      if (!SUM) to[a_xs] = as4(xv), to[a_sg] = as4(sg), to[a_gz] = as4(gz);
+      if (!SUM)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float2* at = ends + (2 * u + i) * kLanes;
+          at[l.xs / 2] = make_float2(xv[2 * i], xv[2 * i + 1]);
+          at[l.sg / 2] = make_float2(sg[2 * i], sg[2 * i + 1]);
+          at[l.gz / 2] = make_float2(gz[2 * i], gz[2 * i + 1]);
+        }
       if (W) break;
     }
     turn_few(p, few, sm + l.bs, sm + l.cs, p.np, q.end - t0);
@@ -181,22 +189,23 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
       float2 sum[3];
 #pragma unroll
       for (int i = 0; i < 3; ++i) {
-        const float2* part = reinterpret_cast<const float2*>(shares + ((e / 2) * 3 + i) * warps * kLanes) + (e & 1);
+        const float2* part = shares + (e * 3 + i) * warps * kLanes;
         sum[i] = part[0];
 #pragma unroll (W ? W : 4)
-        for (int k = 1; k < warps; ++k) sum[i] = __fadd2_rn(sum[i], part[2 * k * kLanes]);
+        for (int k = 1; k < warps; ++k) sum[i] = __fadd2_rn(sum[i], part[k * kLanes]);
       }
       auto of = [&](int a) {
         return reinterpret_cast<const float2*>(rows + a + (half * (kHalf / 2) + e / 2) * kLanes)[e & 1];
       };
-      const float2 s = of(a_step), g = of(a_gy), xv = of(a_xs), sg = of(a_sg);
+      const float2* end = ends + (half * kHalf + e) * kLanes;
+      const float2 s = of(a_step), g = of(a_gy), xv = end[l.xs / 2], sg = end[l.sg / 2];
       const float2 y = sum[0], sb = sum[1], sa = sum[2];
       const float2 raw = __fmul2_rn(__ffma2_rn(xv, sb, __fmul2_rn(sa, twice(0.6931471805599453f))), sg);  // rt is A / ln 2
       const float2 gx = __ffma2_rn(s, sb, p.skip ? __fmul2_rn(skip, g) : twice(0.0f));
       put_both(row_at(static_cast<T*>(p.dx) + dense, t, p.ost), gx.x, gx.y, q, p.even_out);
       put_both(row_at(static_cast<T*>(p.ddt) + dense, t, p.ost), raw.x, raw.y, q, p.even_out);
       if (z) {
-        const float2 dz = __fmul2_rn(of(a_gz), p.skip ? __ffma2_rn(skip, xv, y) : y);
+        const float2 dz = __fmul2_rn(end[l.gz / 2], p.skip ? __ffma2_rn(skip, xv, y) : y);
         put_both(row_at(static_cast<T*>(p.dz) + dense, t, p.ost), dz.x, dz.y, q, p.even_out);
       }
       dbias = __fadd2_rn(dbias, raw), dskip = __ffma2_rn(g, xv, dskip);
@@ -210,9 +219,13 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
   __syncthreads();
   prepare(start);
   __syncthreads();
-  for (int t0 = start; t0 >= q.first; t0 -= kBlock) {
+  int buf = 0;
+  for (int t0 = start; t0 >= q.first; t0 -= kBlock, buf ^= 1) {
     const bool more = t0 > q.first;
-    if (more) fetch(t0 - kBlock);
+    if (more) {
+      fetch(t0 - kBlock);
+      if (!SUM) fetch_marks(t0 - kBlock, buf ^ 1);
+    }
 #pragma unroll 1
     for (int half = 1; half >= 0; --half) {
 #pragma unroll
@@ -240,7 +253,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
         }
         float2 a[2][kHalf], h[2][kHalf], before[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) before[j] = both(sm + l.marks + (n0 + j) * kTile, 0, lane);
+        for (int j = 0; j < 2; ++j) before[j] = both(sm + l.marks + (buf * p.np + n0 + j) * kTile, 0, lane);
         if (half) {  // pass the earlier eight
 #pragma unroll
           for (int t = 0; t < kHalf / 2; ++t) {
@@ -273,11 +286,12 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
 #pragma unroll
         for (int t = kHalf / 2 - 1; t >= 0; --t) {
           const float4 s = step[t * kLanes], u = du[t * kLanes], gv = gy[t * kLanes];
-          float4* share = shares + (t * 3 * warps + w) * kLanes;
+          float2* share0 = shares + (2 * t * 3 * warps + w) * kLanes;  // of the tokens 2 t and 2 t + 1
+          float2* share1 = share0 + 3 * warps * kLanes;
           float2 y0 = twice(0.0f), y1 = y0, b0 = y0, b1 = y0, w0 = y0, w1 = y0;
           if (g > 0) {
-            y0 = lo(share[0]), y1 = hi(share[0]), b0 = lo(share[warps * kLanes]), b1 = hi(share[warps * kLanes]);
-            w0 = lo(share[2 * warps * kLanes]), w1 = hi(share[2 * warps * kLanes]);
+            y0 = share0[0], b0 = share0[warps * kLanes], w0 = share0[2 * warps * kLanes];
+            y1 = share1[0], b1 = share1[warps * kLanes], w1 = share1[2 * warps * kLanes];
           }
           float v[8];  // [dB, dC][state][token]
 #pragma unroll
@@ -297,7 +311,8 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
             v[2 * j] = fmaf(d0.y, u.y, d0.x * u.x), v[2 * j + 1] = fmaf(d1.y, u.w, d1.x * u.z);
             v[4 + 2 * j] = fmaf(h0.y, gv.y, h0.x * gv.x), v[5 + 2 * j] = fmaf(h1.y, gv.w, h1.x * gv.z);
           }
-          share[0] = as4(y0, y1), share[warps * kLanes] = as4(b0, b1), share[2 * warps * kLanes] = as4(w0, w1);
+          share0[0] = y0, share0[warps * kLanes] = b0, share0[2 * warps * kLanes] = w0;
+          share1[0] = y1, share1[warps * kLanes] = b1, share1[2 * warps * kLanes] = w1;
           halve<4>(v, 16, lane & 16);
           halve<2>(v, 8, lane & 8);
           sums[2 * t] = v[0], sums[2 * t + 1] = v[1];
@@ -318,15 +333,9 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
       finish(t0, half);
       if (half) __syncthreads();
     }
-    if (SUM) {
-      copies_done();
-      __syncthreads();
-    } else if (more) {
-      fetch_marks(t0 - kBlock);
-    }
+    if (SUM) copies_done();
     __syncthreads();  // finish() reads rows that prepare() overwrites
     if (more) prepare(t0 - kBlock);
-    copies_done();
     __syncthreads();
   }
   if (SUM) {

@@ -35,7 +35,9 @@ struct Problem {
   float* seg_steps;  // [B][tiles][segment][64]
   int B, T, D, N, G, R;  // R: channels of a group
   int softplus;
-  int wide_rows, wide_dout, wide_few;  // rows of x, dt and z, of dout, and of B and C lie on 16-byte boundaries
+  // bytes of the pieces in which rows of x, dt and z, of dout, and of B and C are
+  // copied: 16 or 4 where all lie on such boundaries, else 0 (single elements)
+  int row_piece, dout_piece, few_piece;
   int even_out;  // neighbouring channels of dense tensors can be stored together
   int per_group, tiles;  // tiles of 64 channels in a group, and in all
   int np;                // states rounded up to a multiple of four
@@ -148,36 +150,31 @@ __device__ __forceinline__ T* row_at(T* base, int token, int stride) {
 
 // ---- a block's inputs, as stored, in shared memory --------------------------------
 
-__device__ __forceinline__ void copy16(void* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))),
-               "l"(from)
-               : "memory");
+template <int BYTES>
+__device__ __forceinline__ void copy(void* to, const void* from) {
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(from) : "memory");
 }
 // This thread's copies are there (other threads' after a barrier).
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Brings a block's rows of up to four tensors [token][channel] and of B and C
 // [token][state] from memory to shared memory, as they are stored: [token][64] and
-// [token][N]; the last token again where there are no more.  Pieces of 16 bytes that
-// arrive behind the CTA's work, where all rows lie on their
-// boundaries (for B and C: and there are threads enough); elements otherwise.
-// Channels past the tile's width are not written.
+// [token][N]; the last token again where there are no more.  Pieces of 16 bytes, or
+// of 4, that arrive behind the CTA's work, as all rows' boundaries allow; elements
+// (16-bit ones at odd places), which do not, otherwise.  Channels past the tile's
+// width are not written.
 template <typename T>
 struct Feed {
-  static constexpr int kPer = 16 / (int)sizeof(T), kPieces = kTile / kPer;
-  bool rows, few;      // by pieces
-  int token, at;       // of this thread's piece
-  bool has;
-  const T* few_src;    // its piece of B or C
+  bool few;            // B and C by pieces of 16 bytes, one a thread
+  const T* few_src;
   int few_token, few_at, few_stride;
   bool few_has;
-  __device__ __forceinline__ void init(const Problem& p, const Place& q, const T* bm, const T* cm) {
-    const int e = threadIdx.x;
-    rows = p.wide_rows;
-    token = e / kPieces, at = (e % kPieces) * kPer;
-    has = at < q.width;
-    const int pieces = p.N / kPer;
-    few = p.wide_few && (int)blockDim.x >= 2 * kBlock * pieces;
+  __device__ __forceinline__ void init(const Problem& p, const T* bm, const T* cm) {
+    constexpr int kPer = 16 / (int)sizeof(T);
+    const int e = threadIdx.x, pieces = p.N / kPer;
+    few = p.few_piece == 16 && (int)blockDim.x >= 2 * kBlock * pieces;
     few_has = false;
     if (few) {
       const bool c = e >= kBlock * pieces;
@@ -190,27 +187,45 @@ struct Feed {
       few_at = (c ? kBlock * p.N : 0) + few_token * p.N + n;
     }
   }
-  __device__ __forceinline__ void row(T* dst, const T* src, int stride, int t0, int last, int width, bool wide) const {
-    if (rows && wide) {
-      if (has)
-        for (int t = token; t < kBlock; t += blockDim.x / kPieces)
-          copy16(dst + t * kTile + at, row_at(src + at, min(t0 + t, last), stride));
+  // BYTES of a piece; rows of kTile.
+  template <int BYTES>
+  __device__ __forceinline__ void pieces(T* dst, const T* src, int stride, int t0, int last, int width) const {
+    constexpr int kPer = BYTES / (int)sizeof(T), kPieces = kTile / kPer;
+    const int at = (threadIdx.x % kPieces) * kPer;  // blockDim is a multiple of 32, and so of kPieces or its half
+    if (kPieces <= 32) {
+      if (at < width)
+        for (int t = threadIdx.x / kPieces; t < kBlock; t += blockDim.x / kPieces)
+          copy<BYTES>(dst + t * kTile + at, row_at(src + at, min(t0 + t, last), stride));
     } else {
-      for (int e = threadIdx.x; e < kBlock * kTile; e += blockDim.x) {
-        const int t = e / kTile, c = e % kTile;
-        if (c < width) dst[e] = *row_at(src + c, min(t0 + t, last), stride);
+      for (int e = threadIdx.x; e < kBlock * kPieces; e += blockDim.x) {
+        const int t = e / kPieces, c = (e % kPieces) * kPer;
+        if (c < width) copy<BYTES>(dst + t * kTile + c, row_at(src + c, min(t0 + t, last), stride));
       }
     }
   }
+  __device__ __forceinline__ void row(T* dst, const T* src, int stride, int t0, int last, int width, int piece) const {
+    if (piece == 16) pieces<16>(dst, src, stride, t0, last, width);
+    else if (piece == 4) pieces<4>(dst, src, stride, t0, last, width);
+    else
+#pragma unroll 4
+      for (int e = threadIdx.x; e < kBlock * kTile; e += blockDim.x) {
+        const int t = e / kTile, c = e % kTile;
+        dst[e] = *row_at(src + min(c, width - 1), min(t0 + t, last), stride);
+      }
+  }
   __device__ __forceinline__ void bc(const Problem& p, T* dst, const T* bm, const T* cm, int t0, int last) const {
     if (few) {
-      if (few_has) copy16(dst + few_at, row_at(few_src, min(t0 + few_token, last), few_stride));
-    } else {
-      for (int e = threadIdx.x; e < kBlock * p.N; e += blockDim.x) {
-        const int t = e / p.N, n = e - t * p.N, from = min(t0 + t, last);
-        dst[e] = *row_at(bm + n, from, p.bst);
-        dst[kBlock * p.N + e] = *row_at(cm + n, from, p.cst);
-      }
+      if (few_has) copy<16>(dst + few_at, row_at(few_src, min(t0 + few_token, last), few_stride));
+      return;
+    }
+    const int each = p.few_piece ? 4 / (int)sizeof(T) : 1, count = p.N / each;
+#pragma unroll 2
+    for (int e = threadIdx.x; e < kBlock * count; e += blockDim.x) {
+      const int t = e / count, n = (e - t * count) * each, from = min(t0 + t, last);
+      const T *b = row_at(bm + n, from, p.bst), *c = row_at(cm + n, from, p.cst);
+      T *tb = dst + t * p.N + n, *tc = tb + kBlock * p.N;
+      if (p.few_piece) copy<4>(tb, b), copy<4>(tc, c);
+      else tb[0] = *b, tc[0] = *c;
     }
   }
 };

@@ -67,11 +67,11 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : MOST == 128 ? 5 : 1) s
   T* few = reinterpret_cast<T*>(sm + l.few);
   constexpr int kRows = kBlock * kTile;
   Feed<T> feed;
-  feed.init(p, q, bm, cm);
+  feed.init(p, bm, cm);
   auto fetch = [&](int t0) {
-    feed.row(in, x, p.xst, t0, lastt, q.width, true);
-    feed.row(in + kRows, dt, p.dtst, t0, lastt, q.width, true);
-    if (z) feed.row(in + 2 * kRows, z, p.zst, t0, lastt, q.width, true);
+    feed.row(in, x, p.xst, t0, lastt, q.width, p.row_piece);
+    feed.row(in + kRows, dt, p.dtst, t0, lastt, q.width, p.row_piece);
+    if (z) feed.row(in + 2 * kRows, z, p.zst, t0, lastt, q.width, p.row_piece);
     feed.bc(p, few, bm, cm, t0, lastt);
   };
   fetch(q.first);

@@ -7,6 +7,8 @@
 // channel, loaded and stored as used once.
 
 #include <algorithm>
+#include <initializer_list>
+#include <utility>
 
 #include "scan_common.cuh"
 #include "scan_launch.cuh"
@@ -142,6 +144,21 @@ int check(const char* me, const gru_scan_args* p, Needs needs) {
   return GRU_OK;
 }
 
+// The widest piece (16 or 4 bytes, else 0) whose boundaries all rows of the tensors
+// lie on, and `inner` elements fill.
+int piece_of(std::initializer_list<std::pair<const void*, const long*>> all, int strides, long inner, int es) {
+  for (const int n : {16, 4}) {
+    bool ok = inner * es % n == 0;
+    for (const auto& t : all) {
+      if (!t.first) continue;
+      ok = ok && bits(t.first) % n == 0;
+      for (int i = 0; i < strides; ++i) ok = ok && t.second[i] * es % n == 0;
+    }
+    if (ok) return n;
+  }
+  return 0;
+}
+
 void fill(Problem& a, const gru_scan_args& p) {
   a.x = p.x, a.dt = p.dt, a.b = p.b, a.c = p.c, a.z = p.z;
   a.a = p.a, a.skip = p.skip, a.bias = p.dt_bias, a.s0 = p.initial_state;
@@ -150,14 +167,8 @@ void fill(Problem& a, const gru_scan_args& p) {
   a.bg = p.b_stride[2], a.cg = p.c_stride[2];
   a.xst = (int)(p.x_stride[1] * es), a.dtst = (int)(p.dt_stride[1] * es), a.zst = (int)(p.z_stride[1] * es);
   a.bst = (int)(p.b_stride[1] * es), a.cst = (int)(p.c_stride[1] * es), a.ost = p.D * es;
-  auto on16 = [&](const void* at, const long* stride, int n) {
-    bool ok = (bits(at) & 15) == 0;
-    for (int i = 0; i < n; ++i) ok = ok && stride[i] * es % 16 == 0;
-    return ok;
-  };
-  a.wide_rows = on16(p.x, p.x_stride, 2) && on16(p.dt, p.dt_stride, 2) && (!p.z || on16(p.z, p.z_stride, 2)) &&
-                p.D / p.G * es % 16 == 0;
-  a.wide_few = on16(p.b, p.b_stride, 3) && on16(p.c, p.c_stride, 3) && p.N * es % 16 == 0;
+  a.row_piece = piece_of({{p.x, p.x_stride}, {p.dt, p.dt_stride}, {p.z, p.z_stride}}, 2, p.D / p.G, es);
+  a.few_piece = piece_of({{p.b, p.b_stride}, {p.c, p.c_stride}}, 3, p.N, es);
   a.B = p.B, a.T = p.T, a.D = p.D, a.N = p.N, a.G = p.G, a.R = p.D / p.G;
   a.softplus = p.dt_softplus;
   a.per_group = ceil_div(a.R, kTile), a.tiles = a.per_group * a.G;
@@ -167,17 +178,19 @@ void fill(Problem& a, const gru_scan_args& p) {
   a.nmarks = ceil_div(a.T, kBlock);
 }
 
-// Segments of the time.  One pass of `full` warps an SM keeps it about
-// w / (w + 8) busy with w of them; more than one segment costs a first pass of some
-// 0.7 of the work over all but one of them.
-void cut(Problem& a, int full) {
+// Segments of the time.  One pass with w warps an SM keeps it about w / (w + 8)
+// busy, up to `full` of them; more than one segment costs a first pass of `pre` of
+// the work over all but one of them.  (4 sequences of 2048 tokens, 2048 channels:
+// forward 356 us in one segment, 280 in four, 253 in eight; gradient 728, 662, 624.
+// 64 of 512 tokens, 512 channels: 176 and 547 in one, 237 and 584 in two.)
+void cut(Problem& a, int full, double pre) {
   const double beside = (double)a.B * a.tiles * (a.np <= 32 ? a.np / 2 : a.np / 4) / 148.0;
   double best = 0.0;
   a.segs = 1;
-  for (int s = 1; s <= 64 && (s == 1 || a.T / s >= 4 * kBlock); s *= 2) {
+  for (int s = 1; s <= 64 && (s == 1 || a.T / s >= kBlock); s *= 2) {
     const double w = std::min(beside * s, (double)full);
-    const double cost = (1.0 + 0.7 * (s - 1) / s) * (w + 8.0) / w;
-    if (s == 1 || cost < 0.95 * best) best = cost, a.segs = s;
+    const double cost = (1.0 + pre * (s - 1) / s) * (w + 8.0) / w;
+    if (s == 1 || cost < 0.97 * best) best = cost, a.segs = s;
   }
   a.len = ceil_div(ceil_div(a.T, a.segs), kBlock) * kBlock;
   a.segs = std::max(1, ceil_div(a.T, a.len > 0 ? a.len : 1));
@@ -193,11 +206,11 @@ void lay_segments(Problem& a, Pieces& m) {
   a.seg_steps = m.floats(n);
 }
 void lay_forward(Problem& a, Pieces& m) {
-  cut(a, 24);
+  cut(a, 40, 0.5);
   lay_segments(a, m);
 }
 void lay_backward(Problem& a, Pieces& m) {
-  cut(a, 16);
+  cut(a, 32, 0.25);
   lay_segments(a, m);
   a.part_bc = m.floats((size_t)a.B * a.tiles * a.T * 2 * a.np);
   a.part_a = m.floats((size_t)a.segs * a.B * a.D * a.N);
@@ -294,7 +307,8 @@ extern "C" int gru_scan_backward(const gru_scan_args* p, const void* dout, const
     return refuse(me, "stash or workspace too small or not 16-byte aligned");
   a.dout = dout, a.dlast = dfinal;
   a.even_out = even(a, p->dtype, bits(dx) | bits(ddt) | bits(dz));
-  a.wide_dout = (bits(dout) & 15) == 0;  // its rows are D elements apart, as wide as wide_rows asks for
+  const long rows[2] = {p->D, p->D};  // with the groups' channels, all that dout's rows add up from
+  a.dout_piece = piece_of({{dout, rows}}, 2, p->D / p->G, (int)es);
   a.dx = dx, a.ddt = ddt, a.da = da, a.db = db, a.dc = dc, a.dskip = dskip, a.dz = dz, a.dbias = ddt_bias, a.ds0 = dinitial;
   return backward(a, p->dtype, stream);
 }
