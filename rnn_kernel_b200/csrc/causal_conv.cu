@@ -15,6 +15,7 @@
 // Bound by memory.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "row_ops.cuh"
 
@@ -98,7 +99,7 @@ struct Run {
 };
 
 template <typename T, int W, int V>
-__global__ void __launch_bounds__(256) conv_forward_kernel(const Conv a) {
+__global__ void __launch_bounds__(256, V > 2 ? 3 : 2) conv_forward_kernel(const Conv a) {
   const int vecs = a.D / V;
   const long item = blockIdx.x * 256L + threadIdx.x;
   const long rest = item / vecs;
@@ -109,19 +110,18 @@ __global__ void __launch_bounds__(256) conv_forward_kernel(const Conv a) {
   Run<T, W, V> r(a, b, c);
   r.start(a, t0);
   T* y = static_cast<T*>(a.y) + ((long)b * a.T + t0) * a.D + c;
-  float next[W][V];
-  auto load = [&](int t) {
+  Raw<T, V> next[2][W];  // two turns ahead
+  auto load = [&](int t, Raw<T, V>(&to)[W]) {
 #pragma unroll
-    for (int u = 0; u < W; ++u) load_row<V>(r.x + (long)min(t + u, a.T - 1) * a.xt, next[u]);
+    for (int u = 0; u < W; ++u) to[u].load(r.x + (long)min(t + u, a.T - 1) * a.xt);
   };
-  load(t0);
-  for (int t = t0; t < t1; t += W) {
+  load(t0, next[0]);
+  load(t0 + W, next[1]);
+  auto turn = [&](int t, Raw<T, V>(&raw)[W]) {
     float x[W][V];
 #pragma unroll
-    for (int u = 0; u < W; ++u)
-#pragma unroll
-      for (int e = 0; e < V; ++e) x[u][e] = next[u][e];
-    if (t + W < t1) load(t + W);
+    for (int u = 0; u < W; ++u) raw[u].get(x[u]);
+    if (t + 2 * W < t1) load(t + 2 * W, raw);
 #pragma unroll
     for (int u = 0; u < W; ++u) {
 #pragma unroll
@@ -134,6 +134,10 @@ __global__ void __launch_bounds__(256) conv_forward_kernel(const Conv a) {
       if (t + u < t1) store_row<V>(y, p);
       y += a.D;
     }
+  };
+  for (int t = t0; t < t1; t += 2 * W) {
+    turn(t, next[0]);
+    if (t + W < t1) turn(t + W, next[1]);
   }
   if (t1 == a.T) {
 #pragma unroll
@@ -174,28 +178,36 @@ __global__ void __launch_bounds__(32 * kGradRuns) conv_backward_kernel(const Con
       for (int e = 0; e < V; ++e) err[j][e] = 0.0f;
     const long dense = (long)b * a.T * a.D + c;
     const T* dy = a.dy ? static_cast<const T*>(a.dy) + dense : nullptr;
-    float xn[W][V], dn[W][V];
+    Raw<T, V> xn[W], dn[W];  // a turn ahead
     auto load = [&](int t) {
 #pragma unroll
       for (int u = 0; u < W; ++u) {
         const long at = min(t + u, a.T - 1);
-        load_row<V>(r.x + at * a.xt, xn[u]);
-        if (dy) load_row<V>(dy + at * a.D, dn[u]);
+        xn[u].load(r.x + at * a.xt);
+        if (dy) dn[u].load(dy + at * a.D);
       }
     };
     load(t0);
     // Errors of the W - 1 tokens behind the run belong to its dx; the first run's
     // errors also go to the state.
     const int end = t1 + W - 1;
-    for (int t = t0; t < end; t += W) {
+    // W tokens from t on.  INNER: all of them, and those that their dx belongs to, are
+    // this run's, and no state's.
+    auto turn = [&](int t, auto inner) {
+      constexpr bool INNER = decltype(inner)::value;
       float x[W][V], d[W][V];
 #pragma unroll
-      for (int u = 0; u < W; ++u)
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[u][e] = xn[u][e], d[u][e] = dy ? dn[u][e] : 0.0f;
-      if (t + W < end) load(t + W);
-#pragma unroll
       for (int u = 0; u < W; ++u) {
+        xn[u].get(x[u]);
+        dn[u].get(d[u]);
+        if (!dy)
+#pragma unroll
+          for (int e = 0; e < V; ++e) d[u][e] = 0.0f;
+      }
+      if (t + W < end) load(t + W);
+      T* dx = static_cast<T*>(a.dx) + dense + (long)(t - (W - 1)) * a.D;
+#pragma unroll
+      for (int u = 0; u < W; ++u, dx += a.D) {
         const int now = t + u;
 #pragma unroll
         for (int e = 0; e < V; ++e) r.win[u][e] = x[u][e];
@@ -208,9 +220,9 @@ __global__ void __launch_bounds__(32 * kGradRuns) conv_backward_kernel(const Con
             const float s = sigmoid_of(p[e]);
             q[e] *= s * fmaf(p[e], 1.0f - s, 1.0f);
           }
-          if (now >= a.T) q[e] = 0.0f;
+          if (!INNER && now >= a.T) q[e] = 0.0f;
         }
-        if (now < t1) {
+        if (INNER || now < t1) {
 #pragma unroll
           for (int e = 0; e < V; ++e) db[e] += q[e];
 #pragma unroll
@@ -221,6 +233,10 @@ __global__ void __launch_bounds__(32 * kGradRuns) conv_backward_kernel(const Con
         for (int e = 0; e < V; ++e) err[u][e] = q[e], g[e] = 0.0f;
 #pragma unroll
         for (int j = 0; j < W; ++j) fma_into(g, r.w[W - 1 - j], err[(u + 1 + j) % W]);
+        if (INNER) {
+          store_row<V>(dx, g);
+          continue;
+        }
         // dx of token now - W + 1
         const int to = now - (W - 1);
         if (now >= end || (to < t0 && t0 > 0)) continue;  // past the run, or an earlier one's
@@ -230,10 +246,14 @@ __global__ void __launch_bounds__(32 * kGradRuns) conv_backward_kernel(const Con
 #pragma unroll
           for (int e = 0; e < V; ++e) g[e] += s[e];
         }
-        if (to >= 0) store_row<V>(static_cast<T*>(a.dx) + dense + (long)to * a.D, g);
+        if (to >= 0) store_row<V>(dx, g);
         else if (a.ds0) store_row<V>(static_cast<T*>(a.ds0) + ((long)b * (W - 1) + (W - 1) + to) * a.D + c, g);
       }
-    }
+    };
+    turn(t0, std::false_type{});
+    int t = t0 + W;
+    for (; t + W <= t1 && t + W <= a.T - (W - 1); t += W) turn(t, std::true_type{});
+    for (; t < end; t += W) turn(t, std::false_type{});
   }
   constexpr int C = 32 * V;
 #pragma unroll

@@ -47,8 +47,17 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* smem) {
 #pragma unroll
       for (int k = 0; k < K; ++k) smem[k * 32 + warp] = v[k];
     __syncthreads();
+    if (warps <= 8) {  // eight lanes hold the warps' sums, four times over
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = warp_sum(lane < warps ? smem[k * 32 + lane] : 0.0f);
+      for (int k = 0; k < K; ++k) {
+        v[k] = (lane & 7) < warps ? smem[k * 32 + (lane & 7)] : 0.0f;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] = warp_sum(lane < warps ? smem[k * 32 + lane] : 0.0f);
+    }
   }
 }
 
@@ -105,8 +114,9 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const Norm a) {
       const int c = (i * per + tid) * V;
       if (RES) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[i][e] = to_f32(from_f32<TR>(v[i][e] + t[i][e]));
+        for (int e = 0; e < V; ++e) v[i][e] += t[i][e];
         if (c < a.D) store_row<V>(static_cast<TR*>(a.s) + r * a.D + c, v[i]);
+        round_row<TR, V>(v[i]);
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) sum[0] += v[i][e];
@@ -127,7 +137,7 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const Norm a) {
     row_sum<2, CTA>(sums, smem[1]);
     const float shift = sums[0] * inv;
     const float var = sums[1] * inv - shift * shift;  // shift is small beside the deviation, or all but 0
-    const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + a.eps);
+    const float rstd = rsqrtf((var < 0.0f ? 0.0f : var) + a.eps);
     if (tid == 0 && a.stats) {
       a.stats[r] = mean;
       a.stats[a.R + r] = shift;
@@ -264,13 +274,15 @@ struct Shape {
   int nv, threads, rows;  // loads a thread, threads a CTA, rows a CTA at a time
   bool cta;
 };
-// v elements a load: warps hold rows of up to 4 loads a lane; CTAs hold longer
-// ones in as many loads a thread as `most` threads need.
-Shape shape_of(int D, int v, int most) {
+// v elements a load: warps hold rows of up to 4 loads a lane, where there are rows
+// enough for four of them on every SM; CTAs hold the others in as many loads a thread
+// as `most` threads need, with some 16 elements a thread for the forward's sake (its
+// sums over a row's threads cost as much as eight elements' other work).
+Shape shape_of(int D, int v, int most, long rows, int each) {
   const int loads = ceil_div(D, v);
   const int warp_loads = v == 1 ? 8 : 4;
   Shape s;
-  s.cta = loads > 32 * warp_loads;
+  s.cta = loads > 32 * warp_loads || (v > 1 && loads > 32 && rows < 4 * 148);
   if (!s.cta) {
     s.nv = 1;
     while (s.nv * 32 < loads) s.nv *= 2;
@@ -278,7 +290,7 @@ Shape shape_of(int D, int v, int most) {
     return s;
   }
   s.nv = v == 1 ? 8 : 1;
-  while (s.nv * 256 < loads && s.nv * v < 8) s.nv *= 2;
+  while (s.nv * 32 < loads && s.nv * v < each && rows >= 148) s.nv *= 2;
   while (s.nv * most < loads) s.nv *= 2;
   s.threads = (ceil_div(loads, s.nv) + 31) / 32 * 32, s.rows = 1;
   return s;
@@ -286,7 +298,7 @@ Shape shape_of(int D, int v, int most) {
 
 template <typename TX, typename TR, bool RES, int V>
 int launch_forward(const Norm& a, cudaStream_t stream) {
-  const Shape s = shape_of(a.D, V, 1024);
+  const Shape s = shape_of(a.D, V, 1024, a.R, 16);
   const long need = (a.R + s.rows - 1) / s.rows;
   const unsigned ctas = (unsigned)std::min<long>(need, (long)sms_here() * std::max(1, 2048 / s.threads));
   LaunchScope scope(kKindLayerNorm, stream);
@@ -314,7 +326,7 @@ int launch_forward(const Norm& a, cudaStream_t stream) {
 
 template <typename TX, typename TS, int V>
 int launch_backward(const Norm& a, const StoreNorm& store, cudaStream_t stream) {
-  const Shape s = shape_of(a.D, V, 512);
+  const Shape s = shape_of(a.D, V, 512, a.R, 8);
   const long need = (a.R + s.rows - 1) / s.rows;
   const long fit = std::min<long>(kNormCtas, (long)sms_here() * std::max(1, 1024 / s.threads));
   const unsigned ctas = (unsigned)std::min(need, fit);

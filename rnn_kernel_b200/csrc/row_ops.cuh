@@ -94,6 +94,24 @@ __device__ __forceinline__ void store_row(bf16* p, const float (&v)[N]) {
   }
 }
 
+// The numbers that T would hold.
+template <typename T, int N>
+__device__ __forceinline__ void round_row(float (&v)[N]) {
+  if constexpr (sizeof(T) == 2) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const __nv_bfloat162 r = __floats2bfloat162_rn(v[i], v[i + 1]);
+        const unsigned w = *reinterpret_cast<const unsigned*>(&r);
+        v[i] = __uint_as_float(w << 16), v[i + 1] = __uint_as_float(w & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = to_f32(from_f32<T>(v[i]));
+    }
+  }
+}
+
 // 1 / (1 + e^-x) by the hardware's exponential and quotient: within 2^-21 of
 // itself for |x| < 16, 0 below -88.
 __device__ __forceinline__ float sigmoid_of(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
@@ -109,12 +127,14 @@ __device__ __forceinline__ float warp_sum(float x) {
 template <typename T, int N>
 struct Raw {
   static constexpr int kBytes = N * (int)sizeof(T), kWords = kBytes / 4;
-  static_assert(N == 1 || kBytes == 8 || kBytes % 16 == 0, "one element, or whole accesses");
+  static_assert(N == 1 || kBytes == 4 || kBytes == 8 || kBytes % 16 == 0, "one element, or whole accesses");
   unsigned v[kWords > 0 ? kWords : 1];
   T one;
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (N == 1) {
       one = *p;
+    } else if constexpr (kBytes == 4) {
+      v[0] = *reinterpret_cast<const unsigned*>(p);
     } else if constexpr (kBytes == 8) {
       const uint2 r = *reinterpret_cast<const uint2*>(p);
       v[0] = r.x, v[1] = r.y;

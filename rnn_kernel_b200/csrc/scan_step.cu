@@ -19,26 +19,27 @@ namespace {
 
 constexpr int kStepThreads = 256;
 
-// LP: lanes of a channel; K: channels a thread takes one after another, whose
-// loads are in flight together.  vec: states, and groups of B and C, lie in aligned
-// fours.
+// LP: lanes of a channel; K <= LP: channels a thread takes one after another, whose
+// loads are in flight together.  The k-th lane of a channel's works out the step and
+// the gate of the k-th channel for all.  vec: states, and groups of B and C, lie in
+// aligned fours.
 template <typename T, int LP, int K>
-__global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const Problem p, float* state, int vec, int blocks) {
+__global__ void __launch_bounds__(kStepThreads, 3) scan_step_kernel(const Problem p, float* state, int vec, int blocks) {
+  static_assert(K <= LP, "a lane for every channel");
   constexpr int kSlots = kStepThreads / LP;
-  const int b = blockIdx.x / blocks, part = threadIdx.x % LP, slot = threadIdx.x / LP;
+  const int b = blockIdx.x / blocks, part = threadIdx.x % LP, slot = threadIdx.x / LP, lane = threadIdx.x & 31;
   const int d0 = (blockIdx.x - b * blocks) * (kSlots * K) + slot;
   const int n0 = 4 * part, left = p.N - n0;
-  float h[K][4], a[K][4], x[K], dt[K], z[K], bias[K], skip[K];
+  const int mine = min(d0 + (part % K) * kSlots, p.D - 1);
+  const float x = to_f32(static_cast<const T*>(p.x)[b * p.xb + mine]), raw = to_f32(static_cast<const T*>(p.dt)[b * p.dtb + mine]);
+  const float z = to_f32(p.z ? static_cast<const T*>(p.z)[b * p.zb + mine] : static_cast<const T*>(p.x)[b * p.xb + mine]);
+  const float bias = *(p.bias ? p.bias + mine : p.a), skip = *(p.skip ? p.skip + mine : p.a);
+  float h[K][4], a[K][4];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int d = min(d0 + k * kSlots, p.D - 1);  // loads without a branch; the last channel is not written twice
     const float* s = state + ((long)b * p.D + d) * p.N + n0;
     const float* r = p.a + (long)d * p.N + n0;
-    x[k] = to_f32(static_cast<const T*>(p.x)[b * p.xb + d]);
-    dt[k] = to_f32(static_cast<const T*>(p.dt)[b * p.dtb + d]);
-    z[k] = to_f32(p.z ? static_cast<const T*>(p.z)[b * p.zb + d] : static_cast<const T*>(p.x)[b * p.xb + d]);
-    bias[k] = *(p.bias ? p.bias + d : p.a);
-    skip[k] = *(p.skip ? p.skip + d : p.a);
     if (vec) {
       const int at = left > 0 ? 0 : -n0;  // lanes without states read the channel's first
       const float4 v = __ldcs(reinterpret_cast<const float4*>(s + at));
@@ -50,7 +51,8 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const Problem p
       for (int j = 0; j < 4; ++j) h[k][j] = j < left ? s[j] : 0.0f, a[k][j] = j < left ? r[j] : 0.0f;
     }
   }
-  float bv[4], cv[4];
+  const float step = step_of(p.softplus, raw, p.bias ? bias : 0.0f), du = step * x;
+  float bv[4], cv[4], own = 0.0f;
   int group = -1;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -68,16 +70,18 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const Problem p
         for (int j = 0; j < 4; ++j) bv[j] = j < left ? to_f32(bm[j]) : 0.0f, cv[j] = j < left ? to_f32(cm[j]) : 0.0f;
       }
     }
-    const float step = step_of(p.softplus, dt[k], p.bias ? bias[k] : 0.0f), du = step * x[k];
+    const int from = (lane & ~(LP - 1)) + k;
+    const float sk = __shfl_sync(0xffffffffu, step, from), uk = __shfl_sync(0xffffffffu, du, from);
     float y = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      h[k][j] = fmaf(exp2_of(step * decay_rate(a[k][j])), h[k][j], du * bv[j]);
+      h[k][j] = fmaf(exp2_of(sk * decay_rate(a[k][j])), h[k][j], uk * bv[j]);
       y = fmaf(cv[j], h[k][j], y);
     }
     if (left <= 0) y = 0.0f;
 #pragma unroll
     for (int o = LP / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    if (part == k) own = y;
     if (d0 + k * kSlots >= p.D) continue;
     float* s = state + ((long)b * p.D + d) * p.N + n0;
     if (vec) {
@@ -87,11 +91,11 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const Problem p
       for (int j = 0; j < 4; ++j)
         if (j < left) s[j] = h[k][j];
     }
-    if (part == 0) {
-      if (p.skip) y = fmaf(skip[k], x[k], y);
-      if (p.z) y *= z[k] * gate_of(z[k]);
-      static_cast<T*>(p.out)[(long)b * p.D + d] = from_f32<T>(y);
-    }
+  }
+  if (part < K && d0 + part * kSlots < p.D) {
+    if (p.skip) own = fmaf(skip, x, own);
+    if (p.z) own *= z * gate_of(z);
+    static_cast<T*>(p.out)[(long)b * p.D + mine] = from_f32<T>(own);
   }
 }
 
@@ -104,19 +108,20 @@ int launch_step(const Problem& p, float* state, int vec, cudaStream_t stream) {
   return GRU_OK;
 }
 
-// Four channels a thread where that still gives every SM four CTAs.
+// Four channels a thread (as many as a channel has lanes, where those are fewer),
+// where that still gives every SM four CTAs.
 template <typename T>
 int step(const Problem& p, float* state, int vec, cudaStream_t stream) {
   int lp = 1;
   while (lp * 4 < p.N) lp *= 2;
   const bool four = (long)p.B * p.D * lp / (kStepThreads * 4) >= 4L * 148;
-#define GRU_STEP(LP) \
-  if (lp == LP) return four ? launch_step<T, LP, 4>(p, state, vec, stream) : launch_step<T, LP, 1>(p, state, vec, stream);
-  GRU_STEP(1)
-  GRU_STEP(2)
-  GRU_STEP(4)
-  GRU_STEP(8)
-  GRU_STEP(16)
+#define GRU_STEP(LP, K) \
+  if (lp == LP) return four ? launch_step<T, LP, K>(p, state, vec, stream) : launch_step<T, LP, 1>(p, state, vec, stream);
+  GRU_STEP(1, 1)
+  GRU_STEP(2, 2)
+  GRU_STEP(4, 4)
+  GRU_STEP(8, 4)
+  GRU_STEP(16, 4)
 #undef GRU_STEP
   return GRU_ERR_UNSUPPORTED;
 }
