@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(256, V > 2 ? 3 : 2) conv_forward_kernel(const 
 
 // A CTA: 32 lanes x V channels, kGradRuns runs of tokens, one a warp.
 template <typename T, int W, int V>
-__global__ void __launch_bounds__(32 * kGradRuns) conv_backward_kernel(const Conv a) {
+__global__ void __launch_bounds__(32 * kGradRuns, W <= 4 ? 2 : 1) conv_backward_kernel(const Conv a) {
   extern __shared__ __align__(16) float sums[];  // [run][W + 1][32 V]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int blocks = (a.D + 32 * V - 1) / (32 * V);

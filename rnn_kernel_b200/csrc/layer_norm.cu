@@ -61,6 +61,64 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* smem) {
   }
 }
 
+// Elementwise on V neighbours, two in an operation: V is 1 or even.
+template <int V>
+__device__ __forceinline__ void add_to(float (&v)[V], float c) {
+  if constexpr (V == 1) v[0] += c;
+  else
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float2 r = __fadd2_rn(make_float2(v[e], v[e + 1]), make_float2(c, c));
+      v[e] = r.x, v[e + 1] = r.y;
+    }
+}
+template <int V>
+__device__ __forceinline__ void scale(float (&v)[V], float c) {
+  if constexpr (V == 1) v[0] *= c;
+  else
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float2 r = __fmul2_rn(make_float2(v[e], v[e + 1]), make_float2(c, c));
+      v[e] = r.x, v[e + 1] = r.y;
+    }
+}
+template <int V>
+__device__ __forceinline__ void add_row(float (&v)[V], const float (&w)[V]) {
+  if constexpr (V == 1) v[0] += w[0];
+  else
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float2 r = __fadd2_rn(make_float2(v[e], v[e + 1]), make_float2(w[e], w[e + 1]));
+      v[e] = r.x, v[e + 1] = r.y;
+    }
+}
+// v = a b + c
+template <int V>
+__device__ __forceinline__ void fma_row(float (&v)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+  if constexpr (V == 1) v[0] = fmaf(a[0], b[0], c[0]);
+  else
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float2 r = __ffma2_rn(make_float2(a[e], a[e + 1]), make_float2(b[e], b[e + 1]), make_float2(c[e], c[e + 1]));
+      v[e] = r.x, v[e + 1] = r.y;
+    }
+}
+// acc += a, and acc += a b, as two sums (of odd and even places).
+template <int V>
+__device__ __forceinline__ void sum_into(float2& acc, const float (&a)[V]) {
+  if constexpr (V == 1) acc.x += a[0];
+  else
+#pragma unroll
+    for (int e = 0; e < V; e += 2) acc = __fadd2_rn(acc, make_float2(a[e], a[e + 1]));
+}
+template <int V>
+__device__ __forceinline__ void dot_into(float2& acc, const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V == 1) acc.x = fmaf(a[0], b[0], acc.x);
+  else
+#pragma unroll
+    for (int e = 0; e < V; e += 2) acc = __ffma2_rn(make_float2(a[e], a[e + 1]), make_float2(b[e], b[e + 1]), acc);
+}
+
 // V elements a load, NV loads a thread; RES: there is a residual (type TR).
 template <typename TX, typename TR, bool RES, int V, int NV, bool CTA>
 __global__ void __launch_bounds__(1024) norm_forward_kernel(const Norm a) {
@@ -108,32 +166,29 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const Norm a) {
       }
     }
     if (r + step < a.R) load(r + step);
-    float sum[1] = {0.0f};
+    float2 acc = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * per + tid) * V;
       if (RES) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[i][e] += t[i][e];
+        add_row<V>(v[i], t[i]);
         if (c < a.D) store_row<V>(static_cast<TR*>(a.s) + r * a.D + c, v[i]);
         round_row<TR, V>(v[i]);
       }
-#pragma unroll
-      for (int e = 0; e < V; ++e) sum[0] += v[i][e];
+      sum_into<V>(acc, v[i]);
     }
+    float sum[1] = {acc.x + acc.y};
     row_sum<1, CTA>(sum, smem[0]);
     const float mean = sum[0] * inv;
-    float sums[2] = {0.0f, 0.0f};
+    float2 first_sum = make_float2(0.0f, 0.0f), square = first_sum;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if ((i * per + tid) * V < a.D) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          v[i][e] -= mean;
-          sums[0] += v[i][e];
-          sums[1] += v[i][e] * v[i][e];
-        }
+        add_to<V>(v[i], -mean);
+        sum_into<V>(first_sum, v[i]);
+        dot_into<V>(square, v[i], v[i]);
       }
+    float sums[2] = {first_sum.x + first_sum.y, square.x + square.y};
     row_sum<2, CTA>(sums, smem[1]);
     const float shift = sums[0] * inv;
     const float var = sums[1] * inv - shift * shift;  // shift is small beside the deviation, or all but 0
@@ -147,8 +202,9 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const Norm a) {
     for (int i = 0; i < NV; ++i) {
       const int c = (i * per + tid) * V;
       if (c >= a.D) continue;
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[i][e] = (v[i][e] - shift) * rstd * w[i][e] + b[i][e];
+      add_to<V>(v[i], -shift);
+      scale<V>(v[i], rstd);
+      fma_row<V>(v[i], v[i], w[i], b[i]);
       store_row<V>(static_cast<TX*>(a.y) + r * a.D + c, v[i]);
     }
   }
@@ -202,32 +258,33 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(const Norm a) {
     }
     const float mean = stats[0], shift = stats[1], rstd = stats[2];
     if (r + step < a.R) load(r + step);
-    float sums[2] = {0.0f, 0.0f};
+    float2 gs = make_float2(0.0f, 0.0f), gn_ = gs;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const bool in = (i * per + tid) * V < a.D;
+      if ((i * per + tid) * V >= a.D) continue;
+      add_to<V>(n[i], -mean);
+      add_to<V>(n[i], -shift);
+      scale<V>(n[i], rstd);
+      add_row<V>(db[i], g[i]);
+      fma_row<V>(dw[i], g[i], n[i], dw[i]);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        n[i][e] = in ? (n[i][e] - mean - shift) * rstd : 0.0f;
-        const float d = in ? g[i][e] : 0.0f;
-        db[i][e] += d;
-        dw[i][e] += d * n[i][e];
-        g[i][e] = d * w[i][e];
-        sums[0] += g[i][e];
-        sums[1] += g[i][e] * n[i][e];
-      }
+      for (int e = 0; e < V; ++e) g[i][e] *= w[i][e];
+      sum_into<V>(gs, g[i]);
+      dot_into<V>(gn_, g[i], n[i]);
     }
+    float sums[2] = {gs.x + gs.y, gn_.x + gn_.y};
     row_sum<2, CTA>(sums, smem[turn]);
-    const float m0 = sums[0] * inv, m1 = sums[1] * inv;
+    const float m0 = -sums[0] * inv * rstd, m1 = -sums[1] * inv * rstd;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * per + tid) * V;
       if (c >= a.D) continue;
-#pragma unroll
-      for (int e = 0; e < V; ++e) g[i][e] = rstd * (g[i][e] - m0 - n[i][e] * m1);
-      if (a.ds)
-#pragma unroll
-        for (int e = 0; e < V; ++e) g[i][e] += ds[i][e];
+      // rstd g - rstd mean(g) - n rstd mean(g n) (+ ds)
+      scale<V>(g[i], rstd);
+      add_to<V>(g[i], m0);
+      scale<V>(n[i], m1);
+      add_row<V>(g[i], n[i]);
+      if (a.ds) add_row<V>(g[i], ds[i]);
       if (a.dx) store_row<V>(static_cast<TX*>(a.dx) + r * a.D + c, g[i]);
       if (a.dres) store_row<V>(static_cast<TS*>(a.dres) + r * a.D + c, g[i]);
     }
@@ -276,9 +333,8 @@ struct Shape {
 };
 // v elements a load: warps hold rows of up to 4 loads a lane, where there are rows
 // enough for four of them on every SM; CTAs hold the others in as many loads a thread
-// as `most` threads need, with some 16 elements a thread for the forward's sake (its
-// sums over a row's threads cost as much as eight elements' other work).
-Shape shape_of(int D, int v, int most, long rows, int each) {
+// as `most` threads need, eight elements a thread where that takes no more than 256 of them.
+Shape shape_of(int D, int v, int most, long rows) {
   const int loads = ceil_div(D, v);
   const int warp_loads = v == 1 ? 8 : 4;
   Shape s;
@@ -290,7 +346,8 @@ Shape shape_of(int D, int v, int most, long rows, int each) {
     return s;
   }
   s.nv = v == 1 ? 8 : 1;
-  while (s.nv * 32 < loads && s.nv * v < each && rows >= 148) s.nv *= 2;
+  while (s.nv * 32 < loads && s.nv * v < 8 && rows >= 148) s.nv *= 2;
+  if (s.nv * 256 < loads) s.nv *= 2;
   while (s.nv * most < loads) s.nv *= 2;
   s.threads = (ceil_div(loads, s.nv) + 31) / 32 * 32, s.rows = 1;
   return s;
@@ -298,7 +355,7 @@ Shape shape_of(int D, int v, int most, long rows, int each) {
 
 template <typename TX, typename TR, bool RES, int V>
 int launch_forward(const Norm& a, cudaStream_t stream) {
-  const Shape s = shape_of(a.D, V, 1024, a.R, 16);
+  const Shape s = shape_of(a.D, V, 1024, a.R);
   const long need = (a.R + s.rows - 1) / s.rows;
   const unsigned ctas = (unsigned)std::min<long>(need, (long)sms_here() * std::max(1, 2048 / s.threads));
   LaunchScope scope(kKindLayerNorm, stream);
@@ -326,7 +383,7 @@ int launch_forward(const Norm& a, cudaStream_t stream) {
 
 template <typename TX, typename TS, int V>
 int launch_backward(const Norm& a, const StoreNorm& store, cudaStream_t stream) {
-  const Shape s = shape_of(a.D, V, 512, a.R, 8);
+  const Shape s = shape_of(a.D, V, 512, a.R);
   const long need = (a.R + s.rows - 1) / s.rows;
   const long fit = std::min<long>(kNormCtas, (long)sms_here() * std::max(1, 1024 / s.threads));
   const unsigned ctas = (unsigned)std::min(need, fit);
