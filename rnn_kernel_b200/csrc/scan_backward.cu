@@ -237,18 +237,25 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
         const float4* step = rows + a_step + half * (kHalf / 2) * kLanes;
         if (SUM) {
           const float4* gy = rows + a_gy + half * (kHalf / 2) * kLanes;
+          float2 behind[2] = {back[g][0], back[g][1]}, all[2] = {twice(1.0f), twice(1.0f)}, steps = twice(0.0f);
 #pragma unroll
           for (int t = kHalf / 2 - 1; t >= 0; --t) {
             const float4 s = step[t * kLanes], gv = gy[t * kLanes];
-            if (g == 0) total = __fadd2_rn(total, __fadd2_rn(lo(s), hi(s)));
+            steps = __fadd2_rn(steps, __fadd2_rn(lo(s), hi(s)));
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const float4 cv = *reinterpret_cast<const float4*>(cs + j * kRow + 4 * (half * (kHalf / 2) + t));
               float2& r = back[g][j];
-              r = __fmul2_rn(exp2_of(__fmul2_rn(hi(s), rt[g][j])), __ffma2_rn(hi(cv), hi(gv), r));
-              r = __fmul2_rn(exp2_of(__fmul2_rn(lo(s), rt[g][j])), __ffma2_rn(lo(cv), lo(gv), r));
+              const float2 a0 = exp2_of(__fmul2_rn(lo(s), rt[g][j])), a1 = exp2_of(__fmul2_rn(hi(s), rt[g][j]));
+              r = __fmul2_rn(a1, __ffma2_rn(hi(cv), hi(gv), r));
+              r = __fmul2_rn(a0, __ffma2_rn(lo(cv), lo(gv), r));
+              all[j] = __fmul2_rn(all[j], __fmul2_rn(a0, a1));
             }
           }
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            back[g][j] = carried(back[g][j], behind[j], exp2_of(__fmul2_rn(rt[g][j], steps)), all[j]);
+          if (g == 0) total = __fadd2_rn(total, steps);
           continue;
         }
         float2 a[2][kHalf], h[2][kHalf], before[2];
@@ -269,9 +276,12 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
         bs += 4 * half * (kHalf / 2), cs += 4 * half * (kHalf / 2);
         const float4* du = rows + a_du + half * (kHalf / 2) * kLanes;
         const float4* gy = rows + a_gy + half * (kHalf / 2) * kLanes;
+        // what is handed back is carried over the tokens as the forward carries a state
+        float2 behind[2] = {back[g][0], back[g][1]}, all[2] = {twice(1.0f), twice(1.0f)}, steps = twice(0.0f);
 #pragma unroll
         for (int t = 0; t < kHalf / 2; ++t) {
           const float4 s = step[t * kLanes], u = du[t * kLanes];
+          steps = __fadd2_rn(steps, __fadd2_rn(lo(s), hi(s)));
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const float4 bv = *reinterpret_cast<const float4*>(bs + j * kRow + 4 * t);
@@ -279,6 +289,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
             a[j][2 * t + 1] = exp2_of(__fmul2_rn(hi(s), rt[g][j]));
             h[j][2 * t] = __ffma2_rn(a[j][2 * t], t ? h[j][t ? 2 * t - 1 : 0] : before[j], __fmul2_rn(lo(u), lo(bv)));
             h[j][2 * t + 1] = __ffma2_rn(a[j][2 * t + 1], h[j][2 * t], __fmul2_rn(hi(u), hi(bv)));
+            all[j] = __fmul2_rn(all[j], __fmul2_rn(a[j][2 * t], a[j][2 * t + 1]));
           }
         }
         float sums[kHalf];
@@ -318,7 +329,10 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
           sums[2 * t] = v[0], sums[2 * t + 1] = v[1];
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) da[g][j] = __fadd2_rn(da[g][j], da2[j]);
+        for (int j = 0; j < 2; ++j) {
+          da[g][j] = __fadd2_rn(da[g][j], da2[j]);
+          back[g][j] = carried(back[g][j], behind[j], exp2_of(__fmul2_rn(rt[g][j], steps)), all[j]);
+        }
         // a lane holds dB (lane < 16) or dC of state (lane >> 3) & 1, for all eight
         // tokens, over an eighth of the lanes each
         halve<4>(sums, 4, lane & 4);

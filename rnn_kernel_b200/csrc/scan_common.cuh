@@ -274,6 +274,11 @@ __device__ __forceinline__ float4 as4(float2 a, float2 b) { return make_float4(a
 __device__ __forceinline__ float2 lo(float4 v) { return make_float2(v.x, v.y); }
 __device__ __forceinline__ float2 hi(float4 v) { return make_float2(v.z, v.w); }
 __device__ __forceinline__ float4 add4(float4 a, float4 b) { return as4(__fadd2_rn(lo(a), lo(b)), __fadd2_rn(hi(a), hi(b))); }
+// A state behind some tokens, its part from before them carried by `decay` and not
+// by the product of the tokens' decays.
+__device__ __forceinline__ float2 carried(float2 state, float2 before, float2 decay, float2 product) {
+  return __ffma2_rn(__fadd2_rn(decay, make_float2(-product.x, -product.y)), before, state);
+}
 __device__ __forceinline__ float2 exp2_of(float2 v) { return make_float2(exp2_of(v.x), exp2_of(v.y)); }
 
 }  // namespace scan

@@ -12,6 +12,12 @@
 // Blocks of 16 tokens: the next one's inputs are copied in beside a block's scan;
 // between two barriers its outputs are finished and they are prepared.
 //
+// The hardware's exponential is off by up to 2^-22, to one side for neighbouring
+// arguments, and a state that remembers a thousand tokens would gather that a
+// thousand times (3e-6 of it).  So a block's start is carried over the block by
+// e^{A sum dt} and not by the product of its decays: the difference of the two, of
+// the start, is put in at the block's end (4e-7).
+//
 // Sequences too few to fill the GPU are cut into segments: a first launch finds
 // what each makes of a state (h -> e^{A sum dt} h + S), then all segments run side
 // by side, each putting the segments ahead of it together first.
@@ -180,11 +186,14 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : MOST == 128 ? 5 : 1) s
       for (int j = 0; j < SG; ++j) *reinterpret_cast<float2*>(mark + j * kTile) = h[j];
       mark += p.np * kTile;
     }
+    float2 before[SG], all[SG], steps = twice(0.0f);  // the start, the product of decays, the sum of steps
+#pragma unroll
+    for (int j = 0; j < SG; ++j) before[j] = h[j], all[j] = twice(1.0f);
 #pragma unroll
     for (int t = 0; t < kPairs; ++t) {
       const float4 s = step[t * kLanes], u = du[t * kLanes];
       float2 y0 = twice(0.0f), y1 = twice(0.0f);
-      if (SUM) total = __fadd2_rn(total, __fadd2_rn(lo(s), hi(s)));
+      steps = __fadd2_rn(steps, __fadd2_rn(lo(s), hi(s)));
 #pragma unroll
       for (int j = 0; j < SG; ++j) {
         const float4 bv = *reinterpret_cast<const float4*>(bs + j * kRow + 4 * t);
@@ -192,6 +201,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : MOST == 128 ? 5 : 1) s
         const float2 h0 = __ffma2_rn(a0, h[j], __fmul2_rn(lo(u), lo(bv)));
         const float2 h1 = __ffma2_rn(a1, h0, __fmul2_rn(hi(u), hi(bv)));
         h[j] = h1;
+        all[j] = __fmul2_rn(all[j], __fmul2_rn(a0, a1));
         if (!SUM) {
           const float4 cv = *reinterpret_cast<const float4*>(cs + j * kRow + 4 * t);
           y0 = __ffma2_rn(lo(cv), h0, y0);
@@ -200,6 +210,9 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : MOST == 128 ? 5 : 1) s
       }
       if (!SUM) part[(t * warps + w) * kLanes] = as4(y0, y1);
     }
+#pragma unroll
+    for (int j = 0; j < SG; ++j) h[j] = carried(h[j], before[j], exp2_of(__fmul2_rn(rt[j], steps)), all[j]);
+    if (SUM) total = __fadd2_rn(total, steps);
     copies_done();
     __syncthreads();
     if (!SUM) finish(t0);
