@@ -76,8 +76,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
   extern __shared__ __align__(16) float sm[];
   const int threads = W ? 32 * W : blockDim.x, warps = W ? W : threads >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Lay l = layout(warps, p.np, p.N, sizeof(T));
-  const Place q = place(p);
-  if (SUM && q.seg == 0) return;
+  const Place q = place(p, SUM ? p.segs - 1 : p.segs, SUM ? 1 : 0);
   const T* x = static_cast<const T*>(p.x) + q.b * p.xb + q.d0;
   const T* dt = static_cast<const T*>(p.dt) + q.b * p.dtb + q.d0;
   const T* z = p.z ? static_cast<const T*>(p.z) + q.b * p.zb + q.d0 : nullptr;
@@ -120,6 +119,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
       da[g][j] = twice(0.0f);
     }
   if (!SUM)
+#pragma unroll 4
     for (int s = p.segs - 1; s > q.seg; --s) {
       const long at = (long)q.unit * p.segs + s;
       const float2 steps = both(p.seg_steps + at * kTile, 0, lane);
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int n = min(2 * (g * warps + w) + j, p.np - 1);
-          back[g][j] = __ffma2_rn(exp2_of(__fmul2_rn(rt[g][j], steps)), back[g][j],
+          back[g][j] = __ffma2_rn(passed(rt[g][j], steps), back[g][j],
                                   both(p.seg_sums + (at * p.np + n) * kTile, 0, lane));
         }
     }
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
           }
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            back[g][j] = carried(back[g][j], behind[j], exp2_of(__fmul2_rn(rt[g][j], steps)), all[j]);
+            back[g][j] = carried(back[g][j], behind[j], passed(rt[g][j], steps), all[j]);
           if (g == 0) total = __fadd2_rn(total, steps);
           continue;
         }
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           da[g][j] = __fadd2_rn(da[g][j], da2[j]);
-          back[g][j] = carried(back[g][j], behind[j], exp2_of(__fmul2_rn(rt[g][j], steps)), all[j]);
+          back[g][j] = carried(back[g][j], behind[j], passed(rt[g][j], steps), all[j]);
         }
         // a lane holds dB (lane < 16) or dC of state (lane >> 3) & 1, for all eight
         // tokens, over an eighth of the lanes each
@@ -424,19 +424,19 @@ struct StoreChannels {
 
 template <typename T, int GW, int MOST, int W>
 int launch_backward(const Problem& p, cudaStream_t stream) {
-  const int warps = p.np / (2 * GW);
+  const int warps = backward_warps(p.np);
   const size_t smem = layout(warps, p.np, p.N, sizeof(T)).total * sizeof(float);
-  const unsigned ctas = (unsigned)((long)p.B * p.tiles * p.segs);
+  const long units = (long)p.B * p.tiles;
   LaunchScope scope(kKindSelectiveScan, stream, p.segs > 1 ? 5 : 4);
   if (p.segs > 1) {
     auto kernel = scan_backward_kernel<T, GW, true, MOST, W>;
     GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kernel<<<ctas, 32 * warps, smem, stream>>>(p);
+    kernel<<<(unsigned)(units * (p.segs - 1)), 32 * warps, smem, stream>>>(p);
     GRU_CUDA_TRY(cudaGetLastError());
   }
   auto kernel = scan_backward_kernel<T, GW, false, MOST, W>;
   GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kernel<<<ctas, 32 * warps, smem, stream>>>(p);
+  kernel<<<(unsigned)(units * p.segs), 32 * warps, smem, stream>>>(p);
   GRU_CUDA_TRY(cudaGetLastError());
   const long sums = (long)p.B * p.T * p.G * 2 * p.N;
   sum_tiles_kernel<T><<<(unsigned)((sums + 255) / 256), 256, 0, stream>>>(p);
@@ -454,6 +454,8 @@ int backward_of(const Problem& p, cudaStream_t stream) {
 }
 
 }  // namespace
+
+int backward_warps(int np) { return np <= 32 ? np / 2 : np / 4; }
 
 int backward(const Problem& p, int dtype, cudaStream_t stream) {
   return dtype == GRU_F32 ? backward_of<float>(p, stream) : backward_of<bf16>(p, stream);

@@ -113,9 +113,10 @@ struct Place {
   int d;              // the lane's first channel (the tile's where it has none)
   bool live, second;  // the lane has a channel, and its neighbour
 };
-__device__ __forceinline__ Place place(const Problem& p) {
+// segs: of them that the launch takes, from `from` on.
+__device__ __forceinline__ Place place(const Problem& p, int segs, int from) {
   Place q;
-  q.seg = blockIdx.x % p.segs, q.unit = blockIdx.x / p.segs;
+  q.unit = blockIdx.x / segs, q.seg = from + blockIdx.x - q.unit * segs;
   const int tile = q.unit % p.tiles, c = 2 * (threadIdx.x & 31);
   q.b = q.unit / p.tiles;
   q.group = tile / p.per_group;
@@ -274,12 +275,21 @@ __device__ __forceinline__ float4 as4(float2 a, float2 b) { return make_float4(a
 __device__ __forceinline__ float2 lo(float4 v) { return make_float2(v.x, v.y); }
 __device__ __forceinline__ float2 hi(float4 v) { return make_float2(v.z, v.w); }
 __device__ __forceinline__ float4 add4(float4 a, float4 b) { return as4(__fadd2_rn(lo(a), lo(b)), __fadd2_rn(hi(a), hi(b))); }
-// A state behind some tokens, its part from before them carried by `decay` and not
-// by the product of the tokens' decays.
-__device__ __forceinline__ float2 carried(float2 state, float2 before, float2 decay, float2 product) {
-  return __ffma2_rn(__fadd2_rn(decay, make_float2(-product.x, -product.y)), before, state);
-}
 __device__ __forceinline__ float2 exp2_of(float2 v) { return make_float2(exp2_of(v.x), exp2_of(v.y)); }
+
+constexpr float kMost = 3.0e38f;
+// The decay over tokens whose steps sum to `steps`.  Finite: a state that is zero
+// stays so, where each token's own decay would have left it zero.
+__device__ __forceinline__ float2 passed(float2 rate, float2 steps) {
+  const float2 d = exp2_of(__fmul2_rn(rate, steps));
+  return make_float2(fminf(d.x, kMost), fminf(d.y, kMost));
+}
+// A state behind some tokens, its part from before them carried by `decay` and not
+// by the product of the tokens' decays (unless that overflowed, where A is positive).
+__device__ __forceinline__ float2 carried(float2 state, float2 before, float2 decay, float2 product) {
+  const float2 d = __fadd2_rn(decay, make_float2(-product.x, -product.y));
+  return __ffma2_rn(make_float2(fabsf(d.x) <= kMost ? d.x : 0.0f, fabsf(d.y) <= kMost ? d.y : 0.0f), before, state);
+}
 
 }  // namespace scan
 }  // namespace gru

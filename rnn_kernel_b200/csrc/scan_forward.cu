@@ -59,8 +59,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : MOST == 128 ? 5 : 1) s
   extern __shared__ __align__(16) float sm[];
   const int threads = W ? 32 * W : blockDim.x, warps = W ? W : threads >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Lay l = layout(warps, p.np, p.N, sizeof(T));
-  const Place q = place(p);
-  if (SUM && q.seg == p.segs - 1) return;
+  const Place q = place(p, SUM ? p.segs - 1 : p.segs, 0);
   const T* x = static_cast<const T*>(p.x) + q.b * p.xb + q.d0;
   const T* dt = static_cast<const T*>(p.dt) + q.b * p.dtb + q.d0;
   const T* z = p.z && !SUM ? static_cast<const T*>(p.z) + q.b * p.zb + q.d0 : nullptr;
@@ -90,12 +89,13 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : MOST == 128 ? 5 : 1) s
     h[j] = SUM ? twice(0.0f) : two_of(p.s0 ? p.s0 + (long)q.b * p.D * p.N : nullptr, q, n0 + j, p.N);
   }
   if (!SUM)
+#pragma unroll 4
     for (int s = 0; s < q.seg; ++s) {
       const long at = (long)q.unit * p.segs + s;
       const float2 steps = both(p.seg_steps + at * kTile, 0, lane);
 #pragma unroll
       for (int j = 0; j < SG; ++j)
-        h[j] = __ffma2_rn(exp2_of(__fmul2_rn(rt[j], steps)), h[j], both(p.seg_sums + (at * p.np + n0 + j) * kTile, 0, lane));
+        h[j] = __ffma2_rn(passed(rt[j], steps), h[j], both(p.seg_sums + (at * p.np + n0 + j) * kTile, 0, lane));
     }
 
   float4* step = reinterpret_cast<float4*>(sm + l.step) + lane;  // [pair of tokens][lane]
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : MOST == 128 ? 5 : 1) s
       if (!SUM) part[(t * warps + w) * kLanes] = as4(y0, y1);
     }
 #pragma unroll
-    for (int j = 0; j < SG; ++j) h[j] = carried(h[j], before[j], exp2_of(__fmul2_rn(rt[j], steps)), all[j]);
+    for (int j = 0; j < SG; ++j) h[j] = carried(h[j], before[j], passed(rt[j], steps), all[j]);
     if (SUM) total = __fadd2_rn(total, steps);
     copies_done();
     __syncthreads();
@@ -235,20 +235,24 @@ template <typename T, int SG, int MOST, int W>
 int launch_forward(const Problem& p, cudaStream_t stream) {
   const int warps = p.np / SG;
   const size_t smem = layout(warps, p.np, p.N, sizeof(T)).total * sizeof(float);
-  const unsigned ctas = (unsigned)((long)p.B * p.tiles * p.segs);
+  const long units = (long)p.B * p.tiles;
   LaunchScope scope(kKindSelectiveScan, stream, p.segs > 1 ? 2 : 1);
   if (p.segs > 1) {
     auto kernel = scan_forward_kernel<T, SG, true, MOST, W>;
     GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kernel<<<ctas, 32 * warps, smem, stream>>>(p);
+    kernel<<<(unsigned)(units * (p.segs - 1)), 32 * warps, smem, stream>>>(p);
     GRU_CUDA_TRY(cudaGetLastError());
   }
   auto kernel = scan_forward_kernel<T, SG, false, MOST, W>;
   GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kernel<<<ctas, 32 * warps, smem, stream>>>(p);
+  kernel<<<(unsigned)(units * p.segs), 32 * warps, smem, stream>>>(p);
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
 }
+
+// States of a warp: four, so that few warps share the work of a token; two where
+// there are few states, for threads to copy and prepare with.
+int states_of_warp(int np) { return np == 16 || np > 32 ? 4 : 2; }
 
 template <typename T>
 int forward_of(const Problem& p, cudaStream_t stream) {
@@ -258,6 +262,8 @@ int forward_of(const Problem& p, cudaStream_t stream) {
 }
 
 }  // namespace
+
+int forward_warps(int np) { return np / states_of_warp(np); }
 
 int forward(const Problem& p, int dtype, cudaStream_t stream) {
   return dtype == GRU_F32 ? forward_of<float>(p, stream) : forward_of<bf16>(p, stream);

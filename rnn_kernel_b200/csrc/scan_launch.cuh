@@ -6,6 +6,9 @@
 namespace gru {
 namespace scan {
 
+// Warps of a CTA of either pass, for this many states.
+int forward_warps(int np);
+int backward_warps(int np);
 int forward(const Problem& p, int dtype, cudaStream_t stream);
 int backward(const Problem& p, int dtype, cudaStream_t stream);
 

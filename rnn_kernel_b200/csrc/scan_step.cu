@@ -183,22 +183,33 @@ void fill(Problem& a, const gru_scan_args& p) {
   a.nmarks = ceil_div(a.T, kBlock);
 }
 
-// Segments of the time.  One pass with w warps an SM keeps it about w / (w + 8)
-// busy, up to `full` of them; more than one segment costs a first pass of `pre` of
-// the work over all but one of them.  (4 sequences of 2048 tokens, 2048 channels:
-// forward 356 us in one segment, 280 in four, 253 in eight; gradient 728, 662, 624.
-// 64 of 512 tokens, 512 channels: 176 and 547 in one, 237 and 584 in two.)
-void cut(Problem& a, int full, double pre) {
-  const double beside = (double)a.B * a.tiles * (a.np <= 32 ? a.np / 2 : a.np / 4) / 148.0;
+// Segments of the time: as many as take the least time, by what a pass measured.  An
+// SM that is given c CTAs of w warps, r at once, takes c + 9.5 / w ceil(c / r) for a
+// token of them (9.5 / w: the latencies that the warps beside do not hide), and a CTA
+// takes 17 tokens' time to start, and a third of one's for each segment ahead of it.
+// More than one segment needs a first pass over all but one, with `pre` of the work.
+// (Fitted to some 100 forwards and 50 gradients of 1 to 128 segments, which it gives
+// to about 5 %: 16384 tokens of 512 channels, 1 / 8 / 64 segments 2699 / 537 / 156 us;
+// 4 sequences of 2048, 2048 channels, 1 / 4 / 16 segments 360 / 264 / 250 us and 797 /
+// 696 / 672 of the gradient; 64 of 512, 512 channels, 1 / 2 segments 184 / 234 and
+// 578 / 619 us.)
+void cut(Problem& a, int warps, int resident, double pre) {
+  const long units = (long)a.B * a.tiles;
+  const int few = std::max(1, ceil_div(a.T, kBlock)), most = std::min(few, 128);
+  auto pass = [&](long ctas) {
+    const long c = (ctas + 147) / 148;
+    return (double)c + 9.5 / warps * (double)((c + resident - 1) / resident);
+  };
   double best = 0.0;
-  a.segs = 1;
-  for (int s = 1; s <= 64 && (s == 1 || a.T / s >= kBlock); s *= 2) {
-    const double w = std::min(beside * s, (double)full);
-    const double cost = (1.0 + pre * (s - 1) / s) * (w + 8.0) / w;
-    if (s == 1 || cost < 0.97 * best) best = cost, a.segs = s;
+  a.segs = 1, a.len = few * kBlock;
+  for (int i = 0, s = 1, tried = 0; a.T > 0 && tried < most; ++i, s = i % 2 ? 2 << i / 2 : 3 << (i / 2 - 1)) {  // 1, 2, 3, 4, 6, 8, 12 ...
+    tried = std::min(s, most);
+    const int len = ceil_div(ceil_div(a.T, tried), kBlock) * kBlock, segs = ceil_div(a.T, len);
+    double cost = (len + 17.0 + 0.3 * (segs - 1)) * pass(units * segs);
+    if (segs > 1) cost += 10.0 + pre * (len + 17.0) * pass(units * (segs - 1));
+    if (i == 0 || cost < 1.03 * best) a.segs = segs, a.len = len;  // of as good ones the finer, which balances better
+    if (i == 0 || cost < best) best = cost;
   }
-  a.len = ceil_div(ceil_div(a.T, a.segs), kBlock) * kBlock;
-  a.segs = std::max(1, ceil_div(a.T, a.len > 0 ? a.len : 1));
 }
 
 // Whether the lanes' two channels of dense tensors start on a boundary of two elements.
@@ -211,11 +222,11 @@ void lay_segments(Problem& a, Pieces& m) {
   a.seg_steps = m.floats(n);
 }
 void lay_forward(Problem& a, Pieces& m) {
-  cut(a, 40, 0.5);
+  cut(a, forward_warps(a.np), a.np == 16 ? 5 : a.np < 16 ? 3 : 1, 0.56);
   lay_segments(a, m);
 }
 void lay_backward(Problem& a, Pieces& m) {
-  cut(a, 32, 0.25);
+  cut(a, backward_warps(a.np), a.np <= 16 ? 2 : 1, 0.22);
   lay_segments(a, m);
   a.part_bc = m.floats((size_t)a.B * a.tiles * a.T * 2 * a.np);
   a.part_a = m.floats((size_t)a.segs * a.B * a.D * a.N);

@@ -246,6 +246,21 @@ def test_decays_that_forget_everything():
     close(got[1], want[1], torch.float32)
 
 
+@pytest.mark.parametrize("T", [16, 17, 300, 2100])
+def test_a_zero_state_stays_zero_where_it_would_grow(T):
+    """A is positive here, and the product of the decays overflows; nothing enters the state before the last token, whose
+    share of it is dt x B = B, without a rounding."""
+    kw = R.scan_inputs(1, T, 40, 5, 1, gate=False, skip=False, bias=False, state=False)
+    kw["x"].zero_()
+    kw["x"][:, -1] = 1.0
+    kw["dt"].fill_(1.0)
+    kw["A"].fill_(20.0)
+    out, last = selective_scan(**{**kw, "dt_softplus": False})
+    assert torch.equal(last, kw["B"][:, -1].float().expand(1, 40, 5))
+    assert float(out[:, :-1].abs().max()) == 0
+    close(out[:, -1], (kw["B"].double() * kw["C"].double())[:, -1].sum(-1).expand(1, 40), torch.float32)
+
+
 @pytest.mark.parametrize("name", ["x", "dt", "B", "C", "z"])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_bad_numbers_reach_no_earlier_token_and_no_other_sequence(name, bad):
