@@ -24,7 +24,6 @@ namespace {
 
 constexpr int kMinConv = 2, kMaxConv = 8;
 constexpr int kGradRuns = 8;    // runs of tokens of a gradient's CTA
-constexpr int kGradRun = 32;    // tokens of one of them
 
 struct Conv {
   const void *x, *w, *bias, *s0;
@@ -49,6 +48,21 @@ __device__ __forceinline__ void fma_into(float (&c)[V], const float (&a)[V], con
   } else {
 #pragma unroll
     for (int e = 0; e < V; ++e) c[e] = fmaf(a[e], b[e], c[e]);
+  }
+}
+
+// a[e] *= b[e], neighbours packed.
+template <int V>
+__device__ __forceinline__ void mul_into(float (&a)[V], const float (&b)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float2 r = __fmul2_rn(make_float2(a[e], a[e + 1]), make_float2(b[e], b[e + 1]));
+      a[e] = r.x, a[e + 1] = r.y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) a[e] *= b[e];
   }
 }
 
@@ -117,20 +131,22 @@ __global__ void __launch_bounds__(256, V > 2 ? 3 : 2) conv_forward_kernel(const 
   };
   load(t0, next[0]);
   load(t0 + W, next[1]);
+  // Each input goes where the oldest of the window was, and the one that follows it two
+  // turns later is asked for.
   auto turn = [&](int t, Raw<T, V>(&raw)[W]) {
-    float x[W][V];
-#pragma unroll
-    for (int u = 0; u < W; ++u) raw[u].get(x[u]);
-    if (t + 2 * W < t1) load(t + 2 * W, raw);
+    const bool more = t + 2 * W < t1;
 #pragma unroll
     for (int u = 0; u < W; ++u) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) r.win[u][e] = x[u][e];
+      raw[u].get(r.win[u]);
+      if (more) raw[u].load(r.x + (long)min(t + 2 * W + u, a.T - 1) * a.xt);
       float p[V];
       r.sum(u, p);
-      if (a.silu)
+      if (a.silu) {
+        float g[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) p[e] *= sigmoid_of(p[e]);
+        for (int e = 0; e < V; ++e) g[e] = sigmoid_of(p[e]);
+        mul_into(p, g);
+      }
       if (t + u < t1) store_row<V>(y, p);
       y += a.D;
     }
@@ -179,49 +195,44 @@ __global__ void __launch_bounds__(32 * kGradRuns, W <= 4 ? 2 : 1) conv_backward_
     const long dense = (long)b * a.T * a.D + c;
     const T* dy = a.dy ? static_cast<const T*>(a.dy) + dense : nullptr;
     Raw<T, V> xn[W], dn[W];  // a turn ahead
-    auto load = [&](int t) {
-#pragma unroll
-      for (int u = 0; u < W; ++u) {
-        const long at = min(t + u, a.T - 1);
-        xn[u].load(r.x + at * a.xt);
-        if (dy) dn[u].load(dy + at * a.D);
-      }
+    auto load = [&](int t, int u) {
+      const long at = min(t + u, a.T - 1);
+      xn[u].load(r.x + at * a.xt);
+      if (dy) dn[u].load(dy + at * a.D);
     };
-    load(t0);
+#pragma unroll
+    for (int u = 0; u < W; ++u) load(t0, u);
     // Errors of the W - 1 tokens behind the run belong to its dx; the first run's
     // errors also go to the state.
     const int end = t1 + W - 1;
     // W tokens from t on.  INNER: all of them, and those that their dx belongs to, are
-    // this run's, and no state's.
+    // this run's, and no state's; and there is a dy.
     auto turn = [&](int t, auto inner) {
       constexpr bool INNER = decltype(inner)::value;
-      float x[W][V], d[W][V];
-#pragma unroll
-      for (int u = 0; u < W; ++u) {
-        xn[u].get(x[u]);
-        dn[u].get(d[u]);
-        if (!dy)
-#pragma unroll
-          for (int e = 0; e < V; ++e) d[u][e] = 0.0f;
-      }
-      if (t + W < end) load(t + W);
+      const bool more = t + W < end;
       T* dx = static_cast<T*>(a.dx) + dense + (long)(t - (W - 1)) * a.D;
 #pragma unroll
       for (int u = 0; u < W; ++u, dx += a.D) {
         const int now = t + u;
+        xn[u].get(r.win[u]);
+        float (&q)[V] = err[u];
+        dn[u].get(q);
+        if (more) load(t + W, u);
+        if (!INNER && !dy)
 #pragma unroll
-        for (int e = 0; e < V; ++e) r.win[u][e] = x[u][e];
-        float q[V], p[V];
-        r.sum(u, p);
+          for (int e = 0; e < V; ++e) q[e] = 0.0f;
+        if (a.silu) {  // s + p s (1 - s)
+          float p[V], s[V], n[V];
+          r.sum(u, p);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          q[e] = d[u][e];
-          if (a.silu) {
-            const float s = sigmoid_of(p[e]);
-            q[e] *= s * fmaf(p[e], 1.0f - s, 1.0f);
-          }
-          if (!INNER && now >= a.T) q[e] = 0.0f;
+          for (int e = 0; e < V; ++e) s[e] = sigmoid_of(p[e]), n[e] = 1.0f - s[e];
+          mul_into(p, s);
+          fma_into(s, p, n);
+          mul_into(q, s);
         }
+        if (!INNER && now >= a.T)
+#pragma unroll
+          for (int e = 0; e < V; ++e) q[e] = 0.0f;
         if (INNER || now < t1) {
 #pragma unroll
           for (int e = 0; e < V; ++e) db[e] += q[e];
@@ -230,7 +241,7 @@ __global__ void __launch_bounds__(32 * kGradRuns, W <= 4 ? 2 : 1) conv_backward_
         }
         float g[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) err[u][e] = q[e], g[e] = 0.0f;
+        for (int e = 0; e < V; ++e) g[e] = 0.0f;
 #pragma unroll
         for (int j = 0; j < W; ++j) fma_into(g, r.w[W - 1 - j], err[(u + 1 + j) % W]);
         if (INNER) {
@@ -252,7 +263,8 @@ __global__ void __launch_bounds__(32 * kGradRuns, W <= 4 ? 2 : 1) conv_backward_
     };
     turn(t0, std::false_type{});
     int t = t0 + W;
-    for (; t + W <= t1 && t + W <= a.T - (W - 1); t += W) turn(t, std::true_type{});
+    if (dy)
+      for (; t + W <= t1 && t + W <= a.T - (W - 1); t += W) turn(t, std::true_type{});
     for (; t < end; t += W) turn(t, std::false_type{});
   }
   constexpr int C = 32 * V;
@@ -344,7 +356,33 @@ int launch_any(const Conv& a, bool vec, Way way, const StoreConv& store, cudaStr
   return GRU_ERR_UNSUPPORTED;
 }
 
-long grad_parts(const gru_conv_args& p) { return (long)p.B * ceil_div(ceil_div(p.T, kGradRun), kGradRuns); }
+// The tokens of a run, of T that `units` pieces of work each have: of the runs that
+// fill the GPU once, twice and so on, those that take the least, at `extra` tokens'
+// time besides its own for a run.  side: runs of a CTA; resident: CTAs of an SM.  Not
+// below 8 tokens.  (4 x 2048 tokens, 4096 channels: forward in runs of 76, once the GPU,
+// 37 us, of 32 39, of 128 43; gradient in runs of 128, once, 71 us, of 32 or 64 77.)
+int run_of(long units, int side, int resident, int T, int extra) {
+  const long slots = 148L * resident, most = (T + 7) / 8;
+  long best = 0;
+  int run = T;
+  for (long k = 1; k <= 8; ++k) {
+    const long runs = std::min(std::max(k * slots * side / units, 1L), most);
+    const int len = (int)((T + runs - 1) / runs);
+    const long ctas = (units * ceil_div(T, len) + side - 1) / side;
+    const long cost = (ctas + slots - 1) / slots * (len + extra);
+    if (k == 1 || cost < best) best = cost, run = len;
+  }
+  return run;
+}
+// A gradient's: its CTAs take 8 runs of one batch row and 32 lanes.  The same whether
+// or not the tensors' boundaries let a lane have several channels.
+int grad_run(const gru_conv_args& p) {
+  const long units = (long)p.B * ceil_div(p.D, p.W <= 4 ? 128 : 64);
+  return run_of(units, 1, p.W <= 4 ? 2 : 1, ceil_div(p.T, kGradRuns), p.W + 3);
+}
+long grad_parts(const gru_conv_args& p) {
+  return p.T > 0 && p.B > 0 ? (long)p.B * ceil_div(ceil_div(p.T, grad_run(p)), kGradRuns) : 0;
+}
 
 int check(const char* me, const gru_conv_args* p) {
   if (!p) return refuse(me, "null arguments");
@@ -410,10 +448,8 @@ extern "C" int gru_conv_forward(const gru_conv_args* p, void* out, void* final_s
   fill(a, *p);
   a.y = out, a.last = final_state;
   const bool vec = vectors(*p, bits(p->x) | bits(p->initial_state) | bits(out) | bits(final_state));
-  // runs of 32 tokens, shorter ones where they would leave the GPU idle
-  const long lanes = (long)p->B * (p->D / (vec ? (p->W <= 4 ? 4 : 2) : 1));
-  a.run = 32;
-  while (a.run > 8 && lanes * ceil_div(p->T, a.run) < 148L * 1024) a.run /= 2;
+  const int v = vec ? (p->W <= 4 ? 4 : 2) : 1;
+  a.run = run_of((long)p->B * (p->D / v), 256, v > 2 ? 3 : 2, p->T, p->W + 3);
   a.runs = ceil_div(p->T, a.run);
   return p->dtype == GRU_F32 ? launch_any<float>(a, vec, kForward, {}, stream) : launch_any<bf16>(a, vec, kForward, {}, stream);
 }
@@ -444,7 +480,7 @@ extern "C" int gru_conv_backward(const gru_conv_args* p, const void* dout, const
   Conv a{};
   fill(a, *p);
   a.dy = dout, a.dlast = dfinal, a.dx = dx, a.ds0 = dinitial, a.part = static_cast<float*>(workspace);
-  a.run = kGradRun, a.runs = ceil_div(p->T, kGradRun);
+  a.run = grad_run(*p), a.runs = ceil_div(p->T, a.run);
   const bool vec = vectors(*p, bits(p->x) | bits(p->initial_state) | bits(dout) | bits(dfinal) | bits(dx) | bits(dinitial));
   const StoreConv store{dweight, dbias, p->D, p->W, p->weight_dtype};
   return p->dtype == GRU_F32 ? launch_any<float>(a, vec, kBackward, store, stream)

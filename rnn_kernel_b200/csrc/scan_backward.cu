@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float bi = i & 1 ? bias.y : bias.x;
-        sg[i] = p.softplus ? gate_of(s[i] + bi) : 1.0f;
+        sg[i] = p.softplus ? sigmoid_of(s[i] + bi) : 1.0f;
         s[i] = step_of(p.softplus, s[i], bi);
         v[i] = s[i] * xv[i];
       }
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
         four(in + 2 * kRows, u, lane, zv);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float c = gate_of(zv[i]);
+          const float c = sigmoid_of(zv[i]);
           gz[i] = g[i] * (c * fmaf(zv[i], 1.0f - c, 1.0f));
           g[i] *= zv[i] * c;
         }

@@ -46,12 +46,6 @@ struct Problem {
   int segs, len;         // segments of the time, and their tokens (a multiple of kBlock)
 };
 
-__device__ __forceinline__ float exp2_of(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ float max_nan(float x, float y) {  // NaN where either is
   float z;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
@@ -69,11 +63,6 @@ __device__ __forceinline__ float decay_rate(float a) {
   return min_nan(max_nan(a * 1.4426950408889634f, -3.0e38f), 3.0e38f);
 }
 
-__device__ __forceinline__ float rcp_of(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
 
 // log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x|.  With s = e / (2 + e), at
@@ -102,9 +91,6 @@ __device__ __forceinline__ float step_of(int softplus, float raw, float bias) {
   raw += bias;
   return softplus ? softplus_of(raw) : raw;
 }
-// 1 / (1 + e^-x), as sigmoid_of but for the last bits
-__device__ __forceinline__ float gate_of(float x) { return rcp_of(1.0f + exp2_of(x * -1.4426950408889634f)); }
-
 // The tile of channels and the range of tokens of a CTA.
 struct Place {
   int seg, unit, b, group;
@@ -275,6 +261,7 @@ __device__ __forceinline__ float4 as4(float2 a, float2 b) { return make_float4(a
 __device__ __forceinline__ float2 lo(float4 v) { return make_float2(v.x, v.y); }
 __device__ __forceinline__ float2 hi(float4 v) { return make_float2(v.z, v.w); }
 __device__ __forceinline__ float4 add4(float4 a, float4 b) { return as4(__fadd2_rn(lo(a), lo(b)), __fadd2_rn(hi(a), hi(b))); }
+using gru::exp2_of;
 __device__ __forceinline__ float2 exp2_of(float2 v) { return make_float2(exp2_of(v.x), exp2_of(v.y)); }
 
 constexpr float kMost = 3.0e38f;

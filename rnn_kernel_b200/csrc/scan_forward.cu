@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : MOST == 128 ? 5 : 1) s
         if (z) {
           four(in + 2 * kRows, u, lane, g);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) g[i] *= gate_of(g[i]);
+          for (int i = 0; i < 4; ++i) g[i] *= sigmoid_of(g[i]);
         }
       }
 #pragma unroll
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : MOST == 128 ? 5 : 1) s
           if (p.skip) y[i] = fmaf(i & 1 ? skip.y : skip.x, to_f32(*row_at(x + c, at, p.xst)), y[i]);
           if (z) {
             const float g = to_f32(*row_at(z + c, at, p.zst));
-            y[i] *= g * gate_of(g);
+            y[i] *= g * sigmoid_of(g);
           }
         }
       }

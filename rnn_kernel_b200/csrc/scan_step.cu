@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kStepThreads, 3) scan_step_kernel(const Proble
   }
   if (part < K && d0 + part * kSlots < p.D) {
     if (p.skip) own = fmaf(skip, x, own);
-    if (p.z) own *= z * gate_of(z);
+    if (p.z) own *= z * sigmoid_of(z);
     static_cast<T*>(p.out)[(long)b * p.D + mine] = from_f32<T>(own);
   }
 }
