@@ -28,8 +28,7 @@ struct Problem {
   void *dx, *ddt, *dz, *db, *dc;
   float *da, *dskip, *dbias, *ds0;
   float* part_bc;  // [B][tiles][padded N][dB, dC][T]
-  float* part_a;   // [B][segment][D][N]
-  float* part_ch;  // [B][segment][2][D]: of skip and dt_bias
+  float* part;     // [B][segment]: of dA [D][N], of dskip and dbias [2][D]
   // a segment's effect on a state that passes it: S or R, and its sum of steps
   float* seg_sums;   // [B][tiles][segment][state, padded][64]
   float* seg_steps;  // [B][tiles][segment][64]

@@ -229,8 +229,7 @@ void lay_backward(Problem& a, Pieces& m) {
   cut(a, backward_warps(a.np), a.np <= 16 ? 2 : 1, 0.22);
   lay_segments(a, m);
   a.part_bc = m.floats((size_t)a.B * a.tiles * a.T * 2 * a.np);
-  a.part_a = m.floats((size_t)a.segs * a.B * a.D * a.N);
-  a.part_ch = m.floats((size_t)a.segs * a.B * 2 * a.D);
+  a.part = m.floats((size_t)a.segs * a.B * a.D * (a.N + 2));
 }
 
 }  // namespace
