@@ -206,9 +206,6 @@ __device__ __forceinline__ void put(void* p, long i, int dtype, float x) {
   if (dtype == GRU_F32) static_cast<float*>(p)[i] = x;
   else static_cast<bf16*>(p)[i] = __float2bfloat16_rn(x);
 }
-__device__ __forceinline__ float get(const void* p, long i, int dtype) {
-  return dtype == GRU_F32 ? static_cast<const float*>(p)[i] : __bfloat162float(static_cast<const bf16*>(p)[i]);
-}
 
 // N elements of a parameter from i on as FP32.  whole: they lie on a boundary of
 // min(16, N elements) bytes.  One branch on the type around all loads: a branch

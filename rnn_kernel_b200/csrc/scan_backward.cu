@@ -20,7 +20,13 @@
 // halves the values: 32 values (8 tokens, 2 states, dB and dC) take 31 exchanges and
 // leave a lane one sum.  The tiles' sums of dB and dC are added by a second launch,
 // in a fixed order, as are those over sequences of dA, dskip and dbias.  Segments as
-// in the forward.  Bound by instructions, and by shared memory's wavefronts.
+// in the forward.
+//
+// 64 sequences of 512 tokens, 512 channels, 16 states, FP32: 551 us; its exponentials
+// would take 87, its memory 72.  Bound by instructions and their latencies (issue slots
+// 51 % with the 16 warps an SM that 128 registers a thread allow; shared memory's
+// wavefronts 62 %).  Left out in turn, the finishing of tokens took 92 us of it, the
+// preparation 60, copies 42, the earlier tokens' second pass 28, the butterflies 28.
 
 #include <algorithm>
 
