@@ -286,28 +286,54 @@ __global__ void __launch_bounds__(32 * kGradRuns, W <= 4 ? 2 : 1) conv_backward_
   }
 }
 
-// One token: the state moves on by one input.
-template <typename T, int W, int V>
+// One token: the state moves on by one input.  A thread has its channels' weights for
+// ROWS sequences, whose loads are in flight together.
+template <typename T, int W, int V, int ROWS>
 __global__ void __launch_bounds__(128) conv_step_kernel(const Conv a) {
   const int vecs = a.D / V;
   const long item = blockIdx.x * 128L + threadIdx.x;
-  const int b = (int)(item / vecs), c = (int)(item - (long)b * vecs) * V;
-  if (b >= a.B) return;
-  T* s = static_cast<T*>(a.last) + (long)b * (W - 1) * a.D + c;
-  float win[W][V], w[W][V], p[V];
-  weights<W, V>(a, c, w, p);
+  const long group = item / vecs;
+  const int b0 = (int)group * ROWS, c = (int)(item - group * vecs) * V;
+  if (b0 >= a.B) return;
+  float w[W][V], bias[V];
+  Raw<T, V> in[ROWS][W];
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) load_row<V>(s + (long)j * a.D, win[j]);
-  load_row<V>(static_cast<const T*>(a.x) + b * a.xb + c, win[W - 1]);
+  for (int k = 0; k < ROWS; ++k) {
+    const int b = min(b0 + k, a.B - 1);
+    const T* s = static_cast<const T*>(a.last) + (long)b * (W - 1) * a.D + c;
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) store_row<V>(s + (long)j * a.D, win[j + 1]);
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) p[e] = fmaf(w[j][e], win[j][e], p[e]);
-    if (a.silu) p[e] *= sigmoid_of(p[e]);
+    for (int j = 0; j < W - 1; ++j) in[k][j].load(s + (long)j * a.D);
+    in[k][W - 1].load(static_cast<const T*>(a.x) + b * a.xb + c);
   }
-  store_row<V>(static_cast<T*>(a.y) + (long)b * a.D + c, p);
+  weights<W, V>(a, c, w, bias);
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    if (k > 0 && b0 + k >= a.B) break;
+    T* s = static_cast<T*>(a.last) + (long)(b0 + k) * (W - 1) * a.D + c;
+    float p[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) p[e] = bias[e];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      float v[V];
+      in[k][j].get(v);
+      fma_into(p, w[j], v);
+      if (j > 0) store_row<V>(s + (long)(j - 1) * a.D, v);
+    }
+    if (a.silu) {
+      float g[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) g[e] = sigmoid_of(p[e]);
+      mul_into(p, g);
+    }
+    store_row<V>(static_cast<T*>(a.y) + (long)(b0 + k) * a.D + c, p);
+  }
+}
+
+template <typename T, int W, int V, int ROWS>
+void launch_step(const Conv& a, cudaStream_t stream) {
+  const long threads = (long)((a.B + ROWS - 1) / ROWS) * (a.D / V);
+  conv_step_kernel<T, W, V, ROWS><<<(unsigned)((threads + 127) / 128), 128, 0, stream>>>(a);
 }
 
 struct StoreConv {
@@ -326,7 +352,10 @@ template <typename T, int W, int V>
 int launch(const Conv& a, Way way, const StoreConv& store, cudaStream_t stream) {
   if (way == kStep) {
     LaunchScope scope(kKindCausalConv, stream);
-    conv_step_kernel<T, W, V><<<(unsigned)(((long)a.B * (a.D / V) + 127) / 128), 128, 0, stream>>>(a);
+    // four sequences a thread where that leaves three CTAs for an SM (4096 channels, 4
+    // weights, bf16, one and four a thread: 256 sequences 5.5 and 3.7 us, 512 8.8 and 5.4)
+    if ((long)a.B * (a.D / V) >= 4L * 128 * 3 * 148) launch_step<T, W, V, 4>(a, stream);
+    else launch_step<T, W, V, 1>(a, stream);
   } else if (way == kForward) {
     LaunchScope scope(kKindCausalConv, stream);
     conv_forward_kernel<T, W, V><<<(unsigned)(((long)a.B * a.runs * (a.D / V) + 255) / 256), 256, 0, stream>>>(a);
@@ -363,14 +392,14 @@ int launch_any(const Conv& a, bool vec, Way way, const StoreConv& store, cudaStr
 // The tokens of a run, of T that `units` pieces of work each have: of the runs that
 // fill the GPU once, twice and so on, those that take the least, at `extra` tokens'
 // time besides its own for a run.  side: runs of a CTA; resident: CTAs of an SM.  Not
-// below 8 tokens.  (4 x 2048 tokens, 4096 channels: forward in runs of 76, once the GPU,
+// below 8 tokens nor above `longest`.  (4 x 2048 tokens, 4096 channels: forward in runs of 76, once the GPU,
 // 37 us, of 32 39, of 128 43; gradient in runs of 128, once, 71 us, of 32 or 64 77.)
-int run_of(long units, int side, int resident, int T, int extra) {
-  const long slots = 148L * resident, most = (T + 7) / 8;
+int run_of(long units, int side, int resident, int T, int longest, int extra) {
+  const long slots = 148L * resident, most = (T + 7) / 8, least = (T + longest - 1) / longest;
   long best = 0;
   int run = T;
   for (long k = 1; k <= 8; ++k) {
-    const long runs = std::min(std::max(k * slots * side / units, 1L), most);
+    const long runs = std::min(std::max(k * slots * side / units, least), most);
     const int len = (int)((T + runs - 1) / runs);
     const long ctas = (units * ceil_div(T, len) + side - 1) / side;
     const long cost = (ctas + slots - 1) / slots * (len + extra);
@@ -379,10 +408,11 @@ int run_of(long units, int side, int resident, int T, int extra) {
   return run;
 }
 // A gradient's: its CTAs take 8 runs of one batch row and 32 lanes.  The same whether
-// or not the tensors' boundaries let a lane have several channels.
+// or not the tensors' boundaries let a lane have several channels.  A thread adds up
+// at most 512 tokens of dw in FP32 (an error of about 256^0.5 2^-25 = 5e-7 of it).
 int grad_run(const gru_conv_args& p) {
   const long units = (long)p.B * ceil_div(p.D, p.W <= 4 ? 128 : 64);
-  return run_of(units, 1, p.W <= 4 ? 2 : 1, ceil_div(p.T, kGradRuns), p.W + 3);
+  return run_of(units, 1, p.W <= 4 ? 2 : 1, ceil_div(p.T, kGradRuns), 512, p.W + 3);
 }
 long grad_parts(const gru_conv_args& p) {
   return p.T > 0 && p.B > 0 ? (long)p.B * ceil_div(ceil_div(p.T, grad_run(p)), kGradRuns) : 0;
@@ -453,7 +483,7 @@ extern "C" int gru_conv_forward(const gru_conv_args* p, void* out, void* final_s
   a.y = out, a.last = final_state;
   const bool vec = vectors(*p, bits(p->x) | bits(p->initial_state) | bits(out) | bits(final_state));
   const int v = vec ? (p->W <= 4 ? 4 : 2) : 1;
-  a.run = run_of((long)p->B * (p->D / v), 256, v > 2 ? 3 : 2, p->T, p->W + 3);
+  a.run = run_of((long)p->B * (p->D / v), 256, v > 2 ? 3 : 2, p->T, p->T, p->W + 3);
   a.runs = ceil_div(p->T, a.run);
   return p->dtype == GRU_F32 ? launch_any<float>(a, vec, kForward, {}, stream) : launch_any<bf16>(a, vec, kForward, {}, stream);
 }

@@ -2,8 +2,8 @@
 channels, strides, states, gradients and the single token.
 
 Tolerances (relative 2-norm).  FP32 outputs: a sum of at most 8 products (4e-7 at the worst), the sigmoid (2^-21), and for the
-weights' gradients FP32 sums over at most 256 tokens before FP64 ones (their errors average out below 256^0.5 2^-24 = 1e-6):
-2e-6.  bf16 outputs: the last rounding is at
+weights' gradients FP32 sums over at most 512 tokens, then over 8 of those sums, before FP64 ones (an error of 2^-25 of the
+sum so far at each, which average out to 256^0.5 2^-25 = 5e-7): 2e-6.  bf16 outputs: the last rounding is at
 most half a step of 2^-7, that is 2^-8 of each element and so of the 2-norm, on top of 2e-6."""
 import pytest
 import torch
@@ -73,6 +73,32 @@ def test_values_and_gradients(size, types):
     true = torch.autograd.grad(want, R.tensors(plain), [g.double() for g in grads])
     for n, a, t in zip([n for n, t in kw.items() if isinstance(t, torch.Tensor)], got, true):
         close(a, t, kw[n].dtype, n)
+
+
+@pytest.mark.parametrize("size", [(1, 1100, 18944, 4), (2, 700, 9001, 3), (1, 900, 9472, 8)])
+def test_values_and_gradients_with_long_runs(size):
+    """Channels enough to fill the GPU, so that a thread takes many turns."""
+    kw = inputs(*size, seed=sum(size))
+    mine, plain = R.leaves(kw), R.leaves(kw, wide=True)
+    outs, want = causal_conv(**mine), R.conv(**plain)
+    close(outs[0], want[0], torch.float32, "out")
+    assert torch.equal(outs[1], want[1].float())
+    grads = [torch.randn_like(o) for o in outs]
+    got = torch.autograd.grad(outs, R.tensors(mine), grads)
+    true = torch.autograd.grad(want, R.tensors(plain), [g.double() for g in grads])
+    for n, a, t in zip([n for n, t in kw.items() if isinstance(t, torch.Tensor)], got, true):
+        close(a, t, torch.float32, n)
+
+
+@pytest.mark.parametrize("size", [(225, 4096, 4), (229, 1001, 5), (230, 2048, 8)])
+def test_a_step_of_many_sequences(size):
+    B, D, W = size
+    kw = inputs(B, 1, D, W, torch.bfloat16, seed=B)
+    state = kw.pop("initial_state")
+    want, last = R.conv(initial_state=state, **kw)
+    x = kw.pop("x")
+    close(causal_conv_step(x[:, 0], state=state, **kw), want[:, 0], torch.bfloat16)
+    assert torch.equal(state, last.to(torch.bfloat16))
 
 
 @pytest.mark.parametrize("W", range(2, 9))
