@@ -229,14 +229,16 @@ typedef struct {
 size_t gru_scan_stash_bytes(const gru_scan_args* args);
 size_t gru_scan_workspace_bytes(const gru_scan_args* args, int backward);
 
-/* All T tokens: out dense [B, T, D], final_state dense [B, D, N].  stash:
- * gru_scan_stash_bytes() bytes for a training forward, or NULL. */
+/* All T tokens: out dense [B, T, D], final_state dense [B, D, N], not in the
+ * initial state's memory.  stash: gru_scan_stash_bytes() bytes for a training
+ * forward, or NULL. */
 int gru_scan_forward(const gru_scan_args* args, void* out, float* final_state, void* stash, size_t stash_bytes,
                      void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gradients (dense, overwritten) of everything that the forward read, from dout
  * dense [B, T, D] and dfinal dense [B, D, N] (either NULL: zeros); dskip, ddt_bias
- * and dinitial may be NULL, dz where z is.  args: the forward's. */
+ * and dinitial may be NULL, dz where z is; dinitial is not in dfinal's memory.
+ * args: the forward's. */
 int gru_scan_backward(const gru_scan_args* args, const void* dout, const float* dfinal, const void* stash,
                       size_t stash_bytes, void* dx, void* ddt, float* da, void* db, void* dc, float* dskip, void* dz,
                       float* ddt_bias, float* dinitial, void* workspace, size_t workspace_bytes, void* stream);

@@ -17,6 +17,7 @@
 #include <torch/csrc/utils/object_ptr.h>
 
 #include <atomic>
+#include <climits>
 #include <cmath>
 #include <string>
 
@@ -75,7 +76,13 @@ bool take(PyObject* o, Tensor* t, bool none_too = false) {
   if (o == Py_None) return none_too;
   if (!THPVariable_CheckExact(o)) return false;
   *t = THPVariable_Unpack(o);
-  return t->layout() == at::kStrided;
+  return t->layout() == at::kStrided && !t->is_neg();
+}
+// Whether the C structs' sizes hold x's.
+bool counted(const Tensor& x) {
+  for (const int64_t n : x.sizes())
+    if (n > INT_MAX) return false;
+  return true;
 }
 bool on(const Tensor& t, const Tensor& like, at::ScalarType type) {
   return t.device() == like.device() && t.scalar_type() == type;
@@ -213,7 +220,7 @@ gru_scan_args scan_args(const Tensor& x, const Tensor& dt, const Tensor& A, cons
 bool scan_usual(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Tensor& skip,
                 const Tensor& z, const Tensor& bias, const Tensor& state, int64_t lead) {
   const auto type = x.scalar_type();
-  if (!x.is_cuda() || !usual(type) || x.dim() != lead + 1 || A.dim() != 2 || B.dim() != lead + 2) return false;
+  if (!x.is_cuda() || !usual(type) || x.dim() != lead + 1 || !counted(x) || A.dim() != 2 || B.dim() != lead + 2) return false;
   const int64_t D = x.size(-1), G = B.size(-2), N = B.size(-1);
   if (D < 1 || G < 1 || D % G || N < 1 || N > 64) return false;
   if (!on(dt, x, type) || dt.sizes() != x.sizes() || (z.defined() && (!on(z, x, type) || z.sizes() != x.sizes()))) return false;
@@ -286,7 +293,7 @@ gru_conv_args conv_args(const Tensor& x, const Tensor& weight, const Tensor& bia
 }
 bool conv_usual(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& state, int64_t lead) {
   const auto type = x.scalar_type();
-  if (!x.is_cuda() || !usual(type) || x.dim() != lead + 1 || weight.dim() != 2) return false;
+  if (!x.is_cuda() || !usual(type) || x.dim() != lead + 1 || !counted(x) || weight.dim() != 2) return false;
   const int64_t D = x.size(-1), W = weight.size(1);
   const auto wtype = weight.scalar_type();
   if (D < 1 || W < 2 || W > 8 || weight.size(0) != D || !weight.is_contiguous() || weight.device() != x.device()) return false;

@@ -277,6 +277,8 @@ extern "C" int gru_scan_forward(const gru_scan_args* p, void* out, float* final_
       GRU_CUDA_TRY(cudaMemcpyAsync(final_state, p->initial_state, n, cudaMemcpyDeviceToDevice, stream));
     return GRU_OK;
   }
+  // several segments read the one while the last writes the other
+  if (p->initial_state == final_state) return refuse(me, "final_state must not be the initial state");
   if (!out || bits(out) & (elem_size(p->dtype) - 1)) return refuse(me, "null or misaligned out");
   if (stash) {
     Pieces m{static_cast<char*>(stash)};
@@ -317,6 +319,7 @@ extern "C" int gru_scan_backward(const gru_scan_args* p, const void* dout, const
     return GRU_OK;
   }
   if (!dx || !ddt || !db || !dc || (p->z && !dz)) return refuse(me, "null gradient");
+  if (dinitial && dinitial == dfinal) return refuse(me, "dinitial must not be dfinal");
   Pieces m{static_cast<char*>(const_cast<void*>(stash))}, w{static_cast<char*>(workspace)};
   lay_marks(a, m);
   lay_backward(a, w);

@@ -31,6 +31,12 @@ _DTYPES = {torch.float32: _lib.GRU_F32, torch.bfloat16: _lib.GRU_BF16}
 _supported: dict = {}  # device index -> whether it is a B200
 
 
+def _check_plain(name, *tensors):
+    """Numbers are read as they lie in memory."""
+    if any(t is not None and t.is_neg() for t in tensors):
+        raise RuntimeError(f"{name}: a tensor has a pending negation; give its resolve_neg().")
+
+
 def _check_device(name, dev, *tensors):
     """All tensors on CUDA device ``dev``, a B200."""
     for t in tensors:
@@ -100,6 +106,7 @@ def _check(x, weight, bias, residual, eps):
         if residual is not None and residual.dtype not in (dtype, torch.float32):
             raise RuntimeError(f"{name}: the residual must be float32 or of x's type.")
     _check_device(name, dev)
+    _check_plain(name, x, weight, bias, residual)
     return dev
 
 

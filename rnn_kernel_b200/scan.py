@@ -33,7 +33,7 @@ import torch.nn as nn
 from torch.autograd import forward_ad
 
 from . import _lib
-from .norm import LayerNorm, _check_device, _differentiated, _first_derivatives, _no_tangents
+from .norm import LayerNorm, _check_device, _check_plain, _differentiated, _first_derivatives, _no_tangents
 
 MAX_STATES = 64
 CONV_SIZES = range(2, 9)
@@ -57,6 +57,11 @@ def _near(t):
     """_dense_last of [B, T, ...], with tokens less than 2^31 bytes apart, as the scan asks for."""
     t = _dense_last(t)
     return t if t is None or t.stride(1) * t.element_size() < 1 << 31 else t.contiguous()
+
+
+def _check_counts(name, x):
+    if any(n >= 1 << 31 for n in x.shape):
+        raise ValueError(f"{name}: each of x's sizes must be below 2^31.")
 
 
 def _ptr(t):
@@ -91,9 +96,11 @@ def _check(name, x, dt, A, B, C, skip, z, dt_bias, state, lead):
         raise ValueError(f"{name}: skip and dt_bias must have shape ({D},).")
     if state is not None and state.shape != (x.shape[0], D, N):
         raise ValueError(f"{name}: the state must have shape {(x.shape[0], D, N)}.")
+    _check_counts(name, x)
     dev = x.get_device()
     rest = [t for t in (skip, dt_bias, state) if t is not None]
     _check_device(name, dev, dt, A, B, C, z, *rest)
+    _check_plain(name, x, dt, A, B, C, z, *rest)
     code = _DTYPES.get(x.dtype)
     if code is None or any(t is not None and t.dtype != x.dtype for t in (dt, B, C, z)):
         raise RuntimeError(f"{name}: x, dt, B, C and z must all be float32 or all bfloat16.")
@@ -235,8 +242,10 @@ def _check_conv(name, x, weight, bias, state, activation, lead):
         raise ValueError(f"{name}: the weight's size must be in [{CONV_SIZES[0]}, {CONV_SIZES[-1]}].")
     if state is not None and state.shape != (x.shape[0], W - 1, D):
         raise ValueError(f"{name}: the state must have shape {(x.shape[0], W - 1, D)}.")
+    _check_counts(name, x)
     dev = x.get_device()
     _check_device(name, dev, weight, bias, state)
+    _check_plain(name, x, weight, bias, state)
     code = _DTYPES.get(x.dtype)
     if code is None or (state is not None and state.dtype != x.dtype):
         raise RuntimeError(f"{name}: x and the state must both be float32 or both bfloat16.")

@@ -7,8 +7,9 @@ about 1000 for the inputs here: 32 * 2^-22 = 8e-6, and 1e-5 leaves room for the 
 the last rounding is at most half a step of 2^-7, that is 2^-8 of each element and so of the 2-norm, on top of 1e-5."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
-from rnn_kernel_b200 import selective_scan, selective_step
+from rnn_kernel_b200 import causal_conv, layer_norm, selective_scan, selective_step
 
 from . import scan_reference as R
 from .scan_reference import caller  # noqa: F401
@@ -42,6 +43,8 @@ SIZES = [
     (1, 1030, 64, 16, 1),
     (5, 128, 9, 1, 3),
     (1, 2100, 5, 33, 1),
+    (2, 90, 130, 32, 1),
+    (1, 300, 64, 24, 1),
 ]
 OPTIONS = [dict(), dict(gate=False), dict(skip=False, bias=False), dict(gate=False, skip=False, state=False)]
 
@@ -359,6 +362,29 @@ def test_streams_and_graphs():
     assert torch.equal(eager[0], want[0][0])
 
 
+def test_saved_tensors_through_hooks_and_checkpoints():
+    kw = R.scan_inputs(2, 70, 64, 16, 2, seed=30)
+    w, b = torch.randn(2, 64, device="cuda")
+    cw = torch.randn(64, 4, device="cuda")
+
+    def run(x, A, cw, w):
+        y, s = layer_norm(x, w, b, residual=x)
+        u, _ = causal_conv(y, cw, None, "silu")
+        return selective_scan(**{**kw, "x": u, "A": A})[0] + s
+
+    def grads(how):
+        leaves = [t.clone().requires_grad_() for t in (kw["x"], kw["A"], cw, w)]
+        out = how(*leaves)
+        return (out, *torch.autograd.grad(out, leaves, torch.ones_like(out)))
+
+    want = grads(run)
+    with torch.autograd.graph.save_on_cpu():
+        kept = grads(run)
+    again = grads(lambda *t: torch.utils.checkpoint.checkpoint(run, *t, use_reentrant=False))
+    for got in (kept, again):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_refusals():
     kw = R.scan_inputs(2, 6, 8, 4, 2)
     one = {n: v[:, 0] if n in ("x", "dt", "B", "C", "z") else v for n, v in kw.items() if n != "initial_state"}
@@ -373,3 +399,9 @@ def test_refusals():
         selective_step(state=s.transpose(1, 2).contiguous().transpose(1, 2), **one)
     with pytest.raises(RuntimeError):
         selective_step(state=s.bfloat16(), **one)
+    # numbers that torch would negate when it reads them
+    for call in (lambda: selective_scan(**{**kw, "x": torch._neg_view(kw["x"])}), lambda: selective_step(state=torch._neg_view(s), **one),
+                 lambda: causal_conv(torch._neg_view(kw["x"]), torch.ones(8, 4, device="cuda")),
+                 lambda: layer_norm(torch._neg_view(kw["x"]), torch.ones(8, device="cuda"))):
+        with pytest.raises(RuntimeError, match="negation"):
+            call()

@@ -49,8 +49,9 @@ def test_scan_entries_refuse(bad):
 
 def test_scan_entries_refuse_null_misaligned_and_small():
     lib = _lib.load()
-    p = (64,) * 9  # addresses that are never read: the calls fail before
+    p = (64,) * 8 + (128,)  # addresses that are never read: the calls fail before
     assert lib.gru_scan_forward(scan(), 64, 64, 0, 0, 0, 0, 0) in BAD  # null tensors
+    assert lib.gru_scan_forward(scan(pointers=p), 64, 128, 0, 0, 0, 0, 0) in BAD and "initial state" in _lib.last_error()
     assert lib.gru_scan_forward(scan(pointers=p), 0, 64, 0, 0, 0, 0, 0) in BAD
     assert lib.gru_scan_forward(scan(pointers=p), 64, 0, 0, 0, 0, 0, 0) in BAD
     assert lib.gru_scan_forward(scan(pointers=p), 64, 64, 64, 16, 0, 0, 0) in BAD  # a small stash
@@ -59,10 +60,11 @@ def test_scan_entries_refuse_null_misaligned_and_small():
     assert lib.gru_scan_forward(scan(T=5000, pointers=p), 64, 64, 0, 0, 0, 0, 0) in BAD  # no workspace
     assert lib.gru_scan_forward(scan(T=5000, pointers=p), 64, 64, 0, 0, 64, 16, 0) in BAD
     grads = [64] * 9
-    assert lib.gru_scan_backward(scan(pointers=p), 64, 64, 64, 1 << 40, *grads, 64, 16, 0) in BAD
-    assert lib.gru_scan_backward(scan(pointers=p), 64, 64, 64, 16, *grads, 64, 1 << 40, 0) in BAD
+    assert lib.gru_scan_backward(scan(pointers=p), 64, 128, 64, 1 << 40, *grads, 64, 16, 0) in BAD
+    assert lib.gru_scan_backward(scan(pointers=p), 64, 128, 64, 16, *grads, 64, 1 << 40, 0) in BAD
+    assert lib.gru_scan_backward(scan(pointers=p), 64, 64, 64, 1 << 40, *grads, 64, 1 << 40, 0) in BAD and "dfinal" in _lib.last_error()
     for i in (0, 1, 2, 3, 4, 6):  # dx, ddt, da, db, dc, dz
-        assert lib.gru_scan_backward(scan(pointers=p), 64, 64, 64, 1 << 40, *grads[:i], 0, *grads[i + 1:], 64, 1 << 40, 0) in BAD
+        assert lib.gru_scan_backward(scan(pointers=p), 64, 128, 64, 1 << 40, *grads[:i], 0, *grads[i + 1:], 64, 1 << 40, 0) in BAD
     assert lib.gru_scan_step(scan(pointers=p), 64, 64, 0) in BAD and "T must be 1" in _lib.last_error()
     assert lib.gru_scan_step(scan(T=1, pointers=p), 0, 64, 0) in BAD
     assert lib.gru_scan_step(scan(T=1, B=0), 0, 0, 0) == _lib.GRU_OK == lib.gru_scan_forward(scan(B=0), 0, 0, 0, 0, 0, 0, 0)
