@@ -6,9 +6,9 @@ has a plain C ABI (``include/rnn_kernel_b200.h``) and is loaded with ctypes.
 ``csrc/host_*.cpp`` become the Python module ``_host`` beside it
 (``build_host()``), which reads torch tensors' addresses for AdamW and makes the
 usual calls of the newer operators.  The library needs nvcc alone; the module
-needs a C++ compiler and the headers of CUDA and the installed Python and torch,
-and carries the versions of these two in its file's name, so that after an
-upgrade of either a new one is built and the old one left alone.
+needs a C++ compiler and the headers of the installed Python and torch (and of
+CUDA, for the newer operators), and carries both versions in its file's name, so
+that after an upgrade of either a new one is built and the old one left alone.
 """
 from __future__ import annotations
 
@@ -71,6 +71,17 @@ def host_path() -> Path:
     return PKG / f"_host-torch{torch.__version__}{sysconfig.get_config_var('EXT_SUFFIX')}"
 
 
+def host_parts(torch_base: Path) -> tuple[list[Path], list[str]]:
+    """The module's sources and what they need besides torch: AdamW's part alone, without CUDA's headers or torch's part for it."""
+    try:
+        headers = Path(nvcc_path()).resolve().parent.parent / "include"
+    except RuntimeError:
+        headers = Path("/usr/local/cuda/include")
+    if (headers / "cuda_runtime_api.h").exists() and (torch_base / "lib" / "libc10_cuda.so").exists():
+        return HOST_SOURCES, [f"-I{headers}", "-lc10_cuda"]
+    return HOST_SOURCES[:1], ["-DGRU_TENSORS_ONLY"]
+
+
 def build_host(force: bool = False, verbose: bool = False) -> Path:
     """Compiles the module ``_host`` if it is missing or older than a source of its."""
     import torch
@@ -80,12 +91,11 @@ def build_host(force: bool = False, verbose: bool = False) -> Path:
         return path
     base = Path(torch.__file__).parent
     tmp = path.with_name(f"{path.name}.{os.getpid()}.so.tmp")  # ranks may build at the same time
-    cuda = Path(nvcc_path()).resolve().parent.parent
-    include = [base / "include", base / "include/torch/csrc/api/include", sysconfig.get_paths()["include"], cuda / "include"]
+    include = [base / "include", base / "include/torch/csrc/api/include", sysconfig.get_paths()["include"]]
+    files, cuda = host_parts(base)
     cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{i}" for i in include),
-           *map(str, HOST_SOURCES), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
-           "-o", str(tmp)]
+           *map(str, files), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", *cuda, "-o", str(tmp)]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)

@@ -48,6 +48,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, null
 
 PyMODINIT_FUNC PyInit__host() {
   PyObject* m = PyModule_Create(&module);
+#ifndef GRU_TENSORS_ONLY
   if (m && PyModule_AddFunctions(m, operator_methods()) < 0) Py_CLEAR(m);
+#endif
   return m;
 }

@@ -3,7 +3,7 @@ and of the Python ones, the layers' parameters."""
 import pytest
 import torch
 
-from rnn_kernel_b200 import (LayerNorm, RecurrentStack, SelectiveScan, _lib, causal_conv, causal_conv_step, layer_norm,
+from rnn_kernel_b200 import (LayerNorm, RecurrentStack, SelectiveScan, _lib, build, causal_conv, causal_conv_step, layer_norm,
                              selective_scan, selective_step)
 
 BAD = (_lib.GRU_ERR_INVALID, _lib.GRU_ERR_UNSUPPORTED)
@@ -144,6 +144,11 @@ def test_python_entries_refuse_shapes_and_cpu_tensors():
                 dict(x=torch.zeros(2, 0), weight=torch.zeros(0)), dict(x=torch.zeros(1, 16385), weight=torch.zeros(16385))):
         with pytest.raises(ValueError):
             layer_norm(**{**dict(x=x, weight=torch.zeros(8)), **bad})
+
+
+def test_the_host_module_without_cuda_headers_is_adamws_alone(tmp_path):
+    files, flags = build.host_parts(tmp_path)  # no libc10_cuda there
+    assert [f.name for f in files] == ["host_tensors.cpp"] and flags == ["-DGRU_TENSORS_ONLY"]
 
 
 def test_layers():
