@@ -224,8 +224,8 @@ typedef struct {
 } gru_scan_args; /* host struct */
 
 /* Bytes that a training forward leaves for gru_scan_backward, and the workspace
- * of that (backward != 0) or of a forward (which may be 0), from the sizes alone;
- * 0 and an error text for sizes that they refuse. */
+ * of that (backward != 0) or of a forward (which may be 0), from the sizes and from
+ * whether there is a z; 0 and an error text for sizes that they refuse. */
 size_t gru_scan_stash_bytes(const gru_scan_args* args);
 size_t gru_scan_workspace_bytes(const gru_scan_args* args, int backward);
 

@@ -14,18 +14,20 @@
 // it a warp computes its states at eight tokens, with the decays, in registers, and
 // then goes over the tokens backwards, first for the later eight (for them it passes
 // the earlier ones once more: half an exponential, where twice as many kept states
-// would cost as much in memory traffic).  The warps' shares of y, sum_n B dh and
-// sum_n A w meet in shared memory, where each warp finishes a token.  Sums over
+// would cost as much in memory traffic), and what the gate multiplied, for dz.  The
+// warps' shares of sum_n B dh and sum_n A w meet in shared memory, where each warp
+// finishes a token.  Sums over
 // channels: the lane's two, then butterflies over the lanes in which each round
 // halves the values: 32 values (8 tokens, 2 states, dB and dC) take 31 exchanges and
 // leave a lane one sum.  The tiles' sums of dB and dC are added by a second launch,
 // in a fixed order, as are those over sequences of dA, dskip and dbias.  Segments as
 // in the forward.
 //
-// 64 sequences of 512 tokens, 512 channels, 16 states, FP32: 551 us; its exponentials
-// would take 87, its memory 72.  Bound by instructions and their latencies (issue slots
-// 51 % with the 16 warps an SM that 128 registers a thread allow; shared memory's
-// wavefronts 62 %).  Left out in turn, the finishing of tokens took 92 us of it, the
+// 64 sequences of 512 tokens, 512 channels, 16 states, FP32: 510 us; its exponentials
+// would take 87, its memory 82.  Bound by instructions and their latencies (issue slots
+// 50 % with the 16 warps an SM that 128 registers a thread allow; shared memory's
+// wavefronts 60 %).  It took 551 when it made what the gate multiplied once more, instead
+// of reading it; left out in turn, the finishing of tokens then took 92 us, the
 // preparation 60, copies 42, the earlier tokens' second pass 28, the butterflies 28.
 
 #include <algorithm>
@@ -42,7 +44,7 @@ constexpr int kHalf = kBlock / 2;
 
 // Shared memory in floats; elem: bytes of an element.
 struct Lay {
-  int step, du, gy, xs, sg, gz, bs, cs, part, marks, in, few, sums, total;
+  int step, du, gy, xs, sg, bs, cs, part, marks, in, kept, few, sums, total;
 };
 __host__ __device__ inline Lay layout(int warps, int np, int N, int elem) {
   Lay l;
@@ -52,12 +54,12 @@ __host__ __device__ inline Lay layout(int warps, int np, int N, int elem) {
   l.gy = n, n += kBlock * kTile;  // gradient of y
   l.xs = n, n += kBlock * kTile;
   l.sg = n, n += kBlock * kTile;  // softplus'
-  l.gz = n, n += kBlock * kTile;  // dout silu'(z)
   l.bs = n, n += np * kRow;
   l.cs = n, n += np * kRow;
-  l.part = n, n += warps * 3 * kHalf * kTile;  // [token][y, sum B dh, sum A w][warp][lane] float2
+  l.part = n, n += warps * 2 * kHalf * kTile;  // [token][sum B dh, sum A w][warp][lane] float2
   l.marks = n, n += 2 * np * kTile;  // of this block and the next
   l.in = n, n += 4 * kBlock * kTile * elem / 4;
+  l.kept = n, n += kBlock * kTile;
   l.few = n, n += 2 * kBlock * N * elem / 4;
   l.sums = n, n += 2 * warps * kTile;
   l.total = n;
@@ -90,6 +92,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
   const T* cm = static_cast<const T*>(p.c) + q.b * p.cb + q.group * p.cg;
   const T* dout = p.dout ? static_cast<const T*>(p.dout) + (long)q.b * p.T * p.D + q.d0 : nullptr;
   const long dense = (long)q.b * p.T * p.D + q.d;
+  const float* kept = z && !SUM ? p.sums + (long)q.b * p.T * p.D + q.d0 : nullptr;
   const float2 bias = two_of(p.bias, q), skip = two_of(p.skip, q);
   const int lastt = q.end - 1;
   T* in = reinterpret_cast<T*>(sm + l.in);
@@ -97,11 +100,13 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
   constexpr int kRows = kBlock * kTile;
   Feed<T> feed;
   feed.init(p, bm, cm);
+  Feed<float> feed_kept;
   auto fetch = [&](int t0) {
     feed.row(in, x, p.xst, t0, lastt, q.width, p.row_piece);
     feed.row(in + kRows, dt, p.dtst, t0, lastt, q.width, p.row_piece);
     if (z) feed.row(in + 2 * kRows, z, p.zst, t0, lastt, q.width, p.row_piece);
     if (dout) feed.row(in + 3 * kRows, dout, p.ost, t0, lastt, q.width, p.dout_piece);
+    if (kept) feed_kept.row(sm + l.kept, kept, p.D * 4, t0, lastt, q.width, p.sums_piece);
     feed.bc(p, few, bm, cm, t0, lastt);
   };
   auto fetch_marks = [&](int t0, int buf) {
@@ -147,7 +152,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
   auto prepare = [&](int t0) {
     for (int u = w; u < kPairs; u += warps) {
       const int t = t0 + 2 * u;
-      float s[4], v[4], g[4] = {0.0f, 0.0f, 0.0f, 0.0f}, xv[4], sg[4], gz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float s[4], v[4], g[4] = {0.0f, 0.0f, 0.0f, 0.0f}, xv[4], sg[4];
       four(in, u, lane, xv);
       four(in + kRows, u, lane, s);
       if (dout) four(in + 3 * kRows, u, lane, g);
@@ -159,13 +164,19 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
         v[i] = s[i] * xv[i];
       }
       if (z) {
-        float zv[4];
+        float zv[4], y[4];
         four(in + 2 * kRows, u, lane, zv);
+        if (!SUM) four(sm + l.kept, u, lane, y);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float c = sigmoid_of(zv[i]);
-          gz[i] = g[i] * (c * fmaf(zv[i], 1.0f - c, 1.0f));
+          if (!SUM) y[i] *= g[i] * (c * fmaf(zv[i], 1.0f - c, 1.0f));
           g[i] *= zv[i] * c;
+        }
+        if (!SUM && t <= lastt) {
+          T* dz = row_at(static_cast<T*>(p.dz) + dense, t, p.ost);
+          put_both(dz, y[0], y[1], q, p.even_out);
+          if (t < lastt) put_both(dz + p.D, y[2], y[3], q, p.even_out);
         }
       }
       if (!q.second || t + 1 > lastt)
@@ -180,7 +191,6 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
           float2* at = ends + (2 * u + i) * kLanes;
           at[l.xs / 2] = make_float2(xv[2 * i], xv[2 * i + 1]);
           at[l.sg / 2] = make_float2(sg[2 * i], sg[2 * i + 1]);
-          at[l.gz / 2] = make_float2(gz[2 * i], gz[2 * i + 1]);
         }
       if (W) break;
     }
@@ -192,10 +202,10 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
     for (int e = w; e < kHalf; e += warps) {
       const int t = t0 + half * kHalf + e;
       if (t > lastt) break;
-      float2 sum[3];
+      float2 sum[2];
 #pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        const float2* part = shares + (e * 3 + i) * warps * kLanes;
+      for (int i = 0; i < 2; ++i) {
+        const float2* part = shares + (e * 2 + i) * warps * kLanes;
         sum[i] = part[0];
 #pragma unroll (W ? W : 4)
         for (int k = 1; k < warps; ++k) sum[i] = __fadd2_rn(sum[i], part[k * kLanes]);
@@ -205,15 +215,11 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
       };
       const float2* end = ends + (half * kHalf + e) * kLanes;
       const float2 s = of(a_step), g = of(a_gy), xv = end[l.xs / 2], sg = end[l.sg / 2];
-      const float2 y = sum[0], sb = sum[1], sa = sum[2];
+      const float2 sb = sum[0], sa = sum[1];
       const float2 raw = __fmul2_rn(__ffma2_rn(xv, sb, __fmul2_rn(sa, twice(0.6931471805599453f))), sg);  // rt is A / ln 2
       const float2 gx = __ffma2_rn(s, sb, p.skip ? __fmul2_rn(skip, g) : twice(0.0f));
       put_both(row_at(static_cast<T*>(p.dx) + dense, t, p.ost), gx.x, gx.y, q, p.even_out);
       put_both(row_at(static_cast<T*>(p.ddt) + dense, t, p.ost), raw.x, raw.y, q, p.even_out);
-      if (z) {
-        const float2 dz = __fmul2_rn(end[l.gz / 2], p.skip ? __ffma2_rn(skip, xv, y) : y);
-        put_both(row_at(static_cast<T*>(p.dz) + dense, t, p.ost), dz.x, dz.y, q, p.even_out);
-      }
       dbias = __fadd2_rn(dbias, raw), dskip = __ffma2_rn(g, xv, dskip);
     }
   };
@@ -303,12 +309,12 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
 #pragma unroll
         for (int t = kHalf / 2 - 1; t >= 0; --t) {
           const float4 s = step[t * kLanes], u = du[t * kLanes], gv = gy[t * kLanes];
-          float2* share0 = shares + (2 * t * 3 * warps + w) * kLanes;  // of the tokens 2 t and 2 t + 1
-          float2* share1 = share0 + 3 * warps * kLanes;
-          float2 y0 = twice(0.0f), y1 = y0, b0 = y0, b1 = y0, w0 = y0, w1 = y0;
+          float2* share0 = shares + (2 * t * 2 * warps + w) * kLanes;  // of the tokens 2 t and 2 t + 1
+          float2* share1 = share0 + 2 * warps * kLanes;
+          float2 b0 = twice(0.0f), b1 = b0, w0 = b0, w1 = b0;
           if (g > 0) {
-            y0 = share0[0], b0 = share0[warps * kLanes], w0 = share0[2 * warps * kLanes];
-            y1 = share1[0], b1 = share1[warps * kLanes], w1 = share1[2 * warps * kLanes];
+            b0 = share0[0], w0 = share0[warps * kLanes];
+            b1 = share1[0], w1 = share1[warps * kLanes];
           }
           float v[8];  // [dB, dC][state][token]
 #pragma unroll
@@ -321,15 +327,14 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
             const float2 d0 = __ffma2_rn(lo(cv), lo(gv), r1);
             back[g][j] = __fmul2_rn(a[j][2 * t], d0);
             const float2 q1 = __fmul2_rn(r1, h0), q0 = __fmul2_rn(back[g][j], hb);  // w
-            y0 = __ffma2_rn(lo(cv), h0, y0), y1 = __ffma2_rn(hi(cv), h1, y1);
             b0 = __ffma2_rn(lo(bv), d0, b0), b1 = __ffma2_rn(hi(bv), d1, b1);
             w0 = __ffma2_rn(rt[g][j], q0, w0), w1 = __ffma2_rn(rt[g][j], q1, w1);
             da2[j] = __ffma2_rn(lo(s), q0, da2[j]), da2[j] = __ffma2_rn(hi(s), q1, da2[j]);
             v[2 * j] = fmaf(d0.y, u.y, d0.x * u.x), v[2 * j + 1] = fmaf(d1.y, u.w, d1.x * u.z);
             v[4 + 2 * j] = fmaf(h0.y, gv.y, h0.x * gv.x), v[5 + 2 * j] = fmaf(h1.y, gv.w, h1.x * gv.z);
           }
-          share0[0] = y0, share0[warps * kLanes] = b0, share0[2 * warps * kLanes] = w0;
-          share1[0] = y1, share1[warps * kLanes] = b1, share1[2 * warps * kLanes] = w1;
+          share0[0] = b0, share0[warps * kLanes] = w0;
+          share1[0] = b1, share1[warps * kLanes] = w1;
           halve<4>(v, 16, lane & 16);
           halve<2>(v, 8, lane & 8);
           sums[2 * t] = v[0], sums[2 * t + 1] = v[1];

@@ -21,7 +21,9 @@ struct Problem {
   int xst, dtst, zst, bst, cst, ost;  // bytes between tokens; ost: of dense rows
   void* out;
   float* last;
+  // what a training forward keeps
   float* marks;  // [B][tiles][block][state, padded][64]: states before each block
+  float* sums;   // [B][T][D], with a gate: what it multiplies
   // gradient
   const void* dout;
   const float* dlast;
@@ -36,8 +38,9 @@ struct Problem {
   int softplus;
   // bytes of the pieces in which rows of x, dt and z, of dout, and of B and C are
   // copied: 16 or 4 where all lie on such boundaries, else 0 (single elements)
-  int row_piece, dout_piece, few_piece;
-  int even_out;  // neighbouring channels of dense tensors can be stored together
+  int row_piece, dout_piece, sums_piece, few_piece;
+  int even_out;   // neighbouring channels of dense tensors can be stored together
+  int even_sums;  // and those of sums
   int per_group, tiles;  // tiles of 64 channels in a group, and in all
   int np;                // states rounded up to a multiple of four
   int wide;              // log2 of the states rounded up to a power of two, at least 4

@@ -156,24 +156,30 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : MOST == 128 ? 5 : 1) s
       float4 sum = part[u * warps * kLanes];
 #pragma unroll (W ? W : 4)
       for (int i = 1; i < warps; ++i) sum = add4(sum, part[(u * warps + i) * kLanes]);
-      float y[4] = {sum.x, sum.y, sum.z, sum.w};
+      float y[4] = {sum.x, sum.y, sum.z, sum.w}, g[4];
       if (k < kOwn) {
         constexpr int kLast = kOwn - 1;
-        const float(&o)[4] = own[k < kOwn ? k : kLast];
-        const float(&g)[4] = gate[k < kOwn ? k : kLast];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = z ? (y[i] + o[i]) * g[i] : y[i] + o[i];
+        for (int i = 0; i < 4; ++i) y[i] += own[k < kOwn ? k : kLast][i], g[i] = gate[k < kOwn ? k : kLast][i];
       } else if (q.live) {  // fewer warps than pairs: from memory once more
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int at = min(t + i / 2, lastt), c = q.d - q.d0 + (i & 1 ? q.second : 0);
           if (p.skip) y[i] = fmaf(i & 1 ? skip.y : skip.x, to_f32(*row_at(x + c, at, p.xst)), y[i]);
           if (z) {
-            const float g = to_f32(*row_at(z + c, at, p.zst));
-            y[i] *= g * sigmoid_of(g);
+            g[i] = to_f32(*row_at(z + c, at, p.zst));
+            g[i] *= sigmoid_of(g[i]);
           }
         }
       }
+      if (p.sums) {
+        float* kept = p.sums + ((long)q.b * p.T + t) * p.D + q.d;
+        put_both(kept, y[0], y[1], q, p.even_sums);
+        if (t < lastt) put_both(kept + p.D, y[2], y[3], q, p.even_sums);
+      }
+      if (z)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] *= g[i];
       T* to = row_at(out, t, p.ost);
       put_both(to, y[0], y[1], q, p.even_out);
       if (t < lastt) put_both(to + p.D, y[2], y[3], q, p.even_out);

@@ -217,7 +217,13 @@ void cut(Problem& a, int warps, int resident, double pre) {
 // Whether the lanes' two channels of dense tensors start on a boundary of two elements.
 int even(const Problem& a, int dtype, uintptr_t all) { return a.R % 2 == 0 && (all & (2 * elem_size(dtype) - 1)) == 0; }
 
-void lay_marks(Problem& a, Pieces& m) { a.marks = m.floats((size_t)a.B * a.tiles * a.nmarks * a.np * kTile); }
+void lay_stash(Problem& a, Pieces& m) {
+  a.marks = m.floats((size_t)a.B * a.tiles * a.nmarks * a.np * kTile);
+  a.sums = a.z ? m.floats((size_t)a.B * a.T * a.D) : nullptr;
+  a.even_sums = a.R % 2 == 0;
+  const long rows[2] = {a.D, a.D};
+  a.sums_piece = piece_of({{a.sums, rows}}, 2, a.R, sizeof(float));
+}
 void lay_segments(Problem& a, Pieces& m) {
   const size_t n = a.segs > 1 ? (size_t)a.B * a.tiles * a.segs * kTile : 0;
   a.seg_sums = m.floats(n * a.np);
@@ -246,7 +252,7 @@ extern "C" size_t gru_scan_stash_bytes(const gru_scan_args* p) {
   Problem a{};
   fill(a, *p);
   Pieces m{nullptr};
-  lay_marks(a, m);
+  lay_stash(a, m);
   return m.used;
 }
 
@@ -282,7 +288,7 @@ extern "C" int gru_scan_forward(const gru_scan_args* p, void* out, float* final_
   if (!out || bits(out) & (elem_size(p->dtype) - 1)) return refuse(me, "null or misaligned out");
   if (stash) {
     Pieces m{static_cast<char*>(stash)};
-    lay_marks(a, m);
+    lay_stash(a, m);
     if (stash_bytes < m.used || bits(stash) & 15) return refuse(me, "stash too small or not 16-byte aligned");
   }
   Pieces m{static_cast<char*>(workspace)};
@@ -321,7 +327,7 @@ extern "C" int gru_scan_backward(const gru_scan_args* p, const void* dout, const
   if (!dx || !ddt || !db || !dc || (p->z && !dz)) return refuse(me, "null gradient");
   if (dinitial && dinitial == dfinal) return refuse(me, "dinitial must not be dfinal");
   Pieces m{static_cast<char*>(const_cast<void*>(stash))}, w{static_cast<char*>(workspace)};
-  lay_marks(a, m);
+  lay_stash(a, m);
   lay_backward(a, w);
   if (!stash || stash_bytes < m.used || !workspace || workspace_bytes < w.used || (bits(stash) | bits(workspace)) & 15)
     return refuse(me, "stash or workspace too small or not 16-byte aligned");

@@ -110,10 +110,10 @@ def _check(name, x, dt, A, B, C, skip, z, dt_bias, state, lead):
 
 
 @functools.lru_cache(maxsize=4096)
-def _sizes(code, B, T, D, N, G):
+def _sizes(code, B, T, D, N, G, gated):
     """Bytes of the stash, the forward's workspace and the backward's."""
     lib = _lib.load()
-    a = _lib.SCAN_ARGS.pack(code, B, T, D, N, G, 0, *[0] * 21)
+    a = _lib.SCAN_ARGS.pack(code, B, T, D, N, G, 0, 0, 0, 0, 0, 16 * gated, *[0] * 16)  # a gate's address, which is not read
     return lib.gru_scan_stash_bytes(a), lib.gru_scan_workspace_bytes(a, 0), lib.gru_scan_workspace_bytes(a, 1)
 
 
@@ -132,7 +132,7 @@ def _scan_forward(code, dev, x, dt, A, B, C, skip, z, dt_bias, softplus, state, 
     (b, T, D), (_, N) = x.shape, A.shape
     with _lib.on_device(dev):
         out, last = x.new_empty((b, T, D)), A.new_empty((b, D, N))
-        stash_bytes, ws_bytes, _ = _sizes(code, b, T, D, N, B.shape[2])
+        stash_bytes, ws_bytes, _ = _sizes(code, b, T, D, N, B.shape[2], z is not None)
         stash = A.new_empty(stash_bytes // 4) if train else None
         ws = A.new_empty(ws_bytes // 4) if ws_bytes else None
         _lib.check(_lib.load().gru_scan_forward(_args(code, softplus, x, dt, A, B, C, skip, z, dt_bias, state), out.data_ptr(),
@@ -158,7 +158,7 @@ class SelectiveScanFunction(torch.autograd.Function):
         x, dt, A, B, C, skip, z, dt_bias, stash = ctx.saved_tensors
         (b, T, D), (_, N), G = x.shape, A.shape, B.shape[2]
         dev = x.get_device()
-        stash_bytes, _, ws_bytes = _sizes(ctx.code, b, T, D, N, G)
+        stash_bytes, _, ws_bytes = _sizes(ctx.code, b, T, D, N, G, z is not None)
         with _lib.on_device(dev):
             dout, dlast = _dense(dout), _dense(dlast)
             dx, ddt = x.new_empty((b, T, D)), x.new_empty((b, T, D))

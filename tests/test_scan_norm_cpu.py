@@ -29,6 +29,8 @@ def test_sizes_without_gpu():
     lib = _lib.load()
     one = lib.gru_scan_stash_bytes(scan(T=64))
     assert one > 0 and one % 256 == 0 and one < lib.gru_scan_stash_bytes(scan(T=65)) < 2 * one
+    # a gate keeps what it multiplies
+    assert lib.gru_scan_stash_bytes(scan(T=64, pointers=(0,) * 4 + (64,) + (0,) * 4)) == one + 4 * 2 * 64 * 64
     assert lib.gru_scan_workspace_bytes(scan(), 1) > 0
     # long sequences of few channels are cut into segments, which a forward remembers too
     assert lib.gru_scan_workspace_bytes(scan(T=5), 0) == 0 < lib.gru_scan_workspace_bytes(scan(T=5000), 0)
