@@ -9,7 +9,7 @@
 //   ddt_t = x_t sum_n B_t dh_t + sum_n A w_t,   w_t = dh_t a_t h_{t-1};   dA = sum_t dt_t w_t
 //
 // The forward's shape, backwards: a CTA owns 64 channels of one sequence, two a
-// lane, a warp two states (twice two above 32), and goes over blocks of 16 tokens
+// lane, a warp two states (twice two above 16), and goes over blocks of 16 tokens
 // from the last to the first.  The forward kept the state before each block; from
 // it a warp computes its states at eight tokens, with the decays, in registers, and
 // then goes over the tokens backwards, first for the later eight (for them it passes
@@ -77,10 +77,10 @@ __device__ __forceinline__ void halve(float* v, int bit, bool upper) {
   }
 }
 
-// GW: pairs of states of a warp.  SUM: only what the segments hand back.  MOST and W
+// GW: pairs of states of a warp.  SUM: only what the segments hand back.  MOST, OCC and W
 // as in the forward.
-template <typename T, int GW, bool SUM, int MOST, int W>
-__global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kernel(const __grid_constant__ Problem p) {
+template <typename T, int GW, bool SUM, int MOST, int OCC, int W>
+__global__ void __launch_bounds__(MOST, OCC) scan_backward_kernel(const __grid_constant__ Problem p) {
   extern __shared__ __align__(16) float sm[];
   const int threads = W ? 32 * W : blockDim.x, warps = W ? W : threads >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Lay l = layout(warps, p.np, p.N, sizeof(T));
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
           at[l.xs / 2] = make_float2(xv[2 * i], xv[2 * i + 1]);
           at[l.sg / 2] = make_float2(sg[2 * i], sg[2 * i + 1]);
         }
-      if (W) break;
+      if (W >= kPairs) break;
     }
     turn_few(p, few, sm + l.bs, sm + l.cs, p.np, q.end - t0);
   };
@@ -243,7 +243,6 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) scan_backward_kerne
 #pragma unroll
       for (int g = 0; g < GW; ++g) {
         const int n0 = 2 * (g * warps + w);
-        if (GW > 1 && n0 >= p.np) continue;  // no such states: nothing to add
         const float* bs = sm + l.bs + n0 * kRow;
         const float* cs = sm + l.cs + n0 * kRow;
         const float4* step = rows + a_step + half * (kHalf / 2) * kLanes;
@@ -451,19 +450,19 @@ struct StoreSums {  // dA, then dskip, then dbias
   }
 };
 
-template <typename T, int GW, int MOST, int W>
+template <typename T, int GW, int MOST, int OCC, int W>
 int launch_backward(const Problem& p, cudaStream_t stream) {
-  const int warps = backward_warps(p.np);
+  const int warps = p.np / (2 * GW);
   const size_t smem = layout(warps, p.np, p.N, sizeof(T)).total * sizeof(float);
   const long units = (long)p.B * p.tiles;
   LaunchScope scope(kKindSelectiveScan, stream, p.segs > 1 ? 4 : 3);
   if (p.segs > 1) {
-    auto kernel = scan_backward_kernel<T, GW, true, MOST, W>;
+    auto kernel = scan_backward_kernel<T, GW, true, MOST, OCC, W>;
     GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     kernel<<<(unsigned)(units * (p.segs - 1)), 32 * warps, smem, stream>>>(p);
     GRU_CUDA_TRY(cudaGetLastError());
   }
-  auto kernel = scan_backward_kernel<T, GW, false, MOST, W>;
+  auto kernel = scan_backward_kernel<T, GW, false, MOST, OCC, W>;
   GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   kernel<<<(unsigned)(units * p.segs), 32 * warps, smem, stream>>>(p);
   GRU_CUDA_TRY(cudaGetLastError());
@@ -474,16 +473,25 @@ int launch_backward(const Problem& p, cudaStream_t stream) {
   return sum_parts(p.part, p.B * p.segs, cols, cols, StoreSums{p.da, p.dskip, p.dbias, an, p.D}, stream);
 }
 
+// Two pairs of states a warp, one after the other, from 20 states on, where that many
+// warps leave room for two CTAs (64 sequences of 512 tokens, 512 channels, 32 states:
+// 1013 us, 1081 with a pair a warp; 16 states 562 and 517).  As many CTAs an SM as
+// shared memory and 128 registers a thread allow.
 template <typename T>
 int backward_of(const Problem& p, cudaStream_t stream) {
-  if (p.np == 16) return launch_backward<T, 1, 256, 8>(p, stream);
-  if (p.np < 16) return launch_backward<T, 1, 256, 0>(p, stream);
-  return p.np <= 32 ? launch_backward<T, 1, 512, 0>(p, stream) : launch_backward<T, 2, 512, 0>(p, stream);
+  if (p.np == 4) return launch_backward<T, 1, 64, 4, 2>(p, stream);
+  if (p.np == 8) return launch_backward<T, 1, 128, 3, 4>(p, stream);
+  if (p.np == 12) return launch_backward<T, 1, 192, 2, 6>(p, stream);
+  if (p.np == 16) return launch_backward<T, 1, 256, 2, 8>(p, stream);
+  if (p.np < 32) return launch_backward<T, 2, 224, 2, 0>(p, stream);
+  if (p.np == 32) return launch_backward<T, 2, 256, 2, 8>(p, stream);
+  if (p.np == 64) return launch_backward<T, 2, 512, 1, 16>(p, stream);
+  return launch_backward<T, 2, 512, 1, 0>(p, stream);
 }
 
 }  // namespace
 
-int backward_warps(int np) { return np <= 32 ? np / 2 : np / 4; }
+Fit backward_fit(int np) { return {np <= 16 ? np / 2 : np / 4, np == 4 ? 4 : np == 8 ? 3 : np <= 32 ? 2 : 1}; }
 
 int backward(const Problem& p, int dtype, cudaStream_t stream) {
   return dtype == GRU_F32 ? backward_of<float>(p, stream) : backward_of<bf16>(p, stream);

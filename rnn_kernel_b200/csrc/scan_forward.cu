@@ -3,7 +3,7 @@
 //   h[n] = e^{dt A[n]} h[n] + dt x B[n];   y = sum_n C[n] h[n] + skip x;   out = y silu(z)
 //
 // A CTA owns 64 channels of one sequence, two neighbours a lane, which share every
-// packed FP32 operation; every warp has four (two, below 16) of the states and goes
+// packed FP32 operation; every warp has four (two, below 12) of the states and goes
 // through all tokens with them in registers, so that each decay is computed once
 // and nothing is exchanged along the time.  What a token has per channel (the step
 // by softplus, dt x, the gate) is worked out by one warp for all, two tokens at a
@@ -59,11 +59,10 @@ __host__ __device__ inline Lay layout(int warps, int np, int N, int elem) {
 }
 
 // SG: states of a warp.  SUM: only what the segments make of a state.  MOST: threads
-// at most.  W: the warps, where they are known (4 here and 8 in the gradient, for the
-// usual 16 states: addresses are constants then, and what finish() needs stays in
-// registers), or 0.
-template <typename T, int SG, bool SUM, int MOST, int W>
-__global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : MOST == 128 ? 5 : 1) scan_forward_kernel(const __grid_constant__ Problem p) {
+// at most.  OCC: CTAs of an SM.  W: the warps, where they are known (addresses are
+// constants then, and what finish() needs stays in registers), or 0.
+template <typename T, int SG, bool SUM, int MOST, int OCC, int W>
+__global__ void __launch_bounds__(MOST, OCC) scan_forward_kernel(const __grid_constant__ Problem p) {
   extern __shared__ __align__(16) float sm[];
   const int threads = W ? 32 * W : blockDim.x, warps = W ? W : threads >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Lay l = layout(warps, p.np, p.N, sizeof(T));
@@ -245,41 +244,50 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : MOST == 128 ? 5 : 1) s
   }
 }
 
-template <typename T, int SG, int MOST, int W>
+template <typename T, int SG, int MOST, int OCC, int W>
 int launch_forward(const Problem& p, cudaStream_t stream) {
   const int warps = p.np / SG;
   const size_t smem = layout(warps, p.np, p.N, sizeof(T)).total * sizeof(float);
   const long units = (long)p.B * p.tiles;
   LaunchScope scope(kKindSelectiveScan, stream, p.segs > 1 ? 2 : 1);
   if (p.segs > 1) {
-    auto kernel = scan_forward_kernel<T, SG, true, MOST, W>;
+    auto kernel = scan_forward_kernel<T, SG, true, MOST, OCC, W>;
     GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     kernel<<<(unsigned)(units * (p.segs - 1)), 32 * warps, smem, stream>>>(p);
     GRU_CUDA_TRY(cudaGetLastError());
   }
-  auto kernel = scan_forward_kernel<T, SG, false, MOST, W>;
+  auto kernel = scan_forward_kernel<T, SG, false, MOST, OCC, W>;
   GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   kernel<<<(unsigned)(units * p.segs), 32 * warps, smem, stream>>>(p);
   GRU_CUDA_TRY(cudaGetLastError());
   return GRU_OK;
 }
 
-// States of a warp: four, which share a token's loads and its share of y; two below 16
+// States of a warp: four, which share a token's loads and its share of y; two below 12
 // states, for threads to copy and prepare with.  (64 sequences of 512 tokens, 512
-// channels, four and two states a warp: 8 states 204 and 157 us, 12 states 202 and
-// 181, 16 states 187 and 210, 32 states 337 and 390.)
-int states_of_warp(int np) { return np < 16 ? 2 : 4; }
-
+// channels, four and two states a warp: 8 states 156 and 115 us, 12 states 162 and
+// 205, 16 states 187 and 210, 32 states 337 and 390.)  As many CTAs an SM as leave a
+// thread some 110 to 128 registers: 80 for one or two CTAs more took 199 us instead of
+// 172 at 16 states, 358 instead of 299 at 32.  Known warps where the states are usual
+// (8 states 135 us with any number of warps, 115 with four).
 template <typename T>
 int forward_of(const Problem& p, cudaStream_t stream) {
-  if (p.np == 16) return launch_forward<T, 4, 128, 4>(p, stream);
-  if (p.np < 16) return launch_forward<T, 2, 256, 0>(p, stream);
-  return p.np <= 32 ? launch_forward<T, 4, 256, 0>(p, stream) : launch_forward<T, 4, 512, 0>(p, stream);
+  if (p.np == 4) return launch_forward<T, 2, 64, 7, 2>(p, stream);
+  if (p.np == 8) return launch_forward<T, 2, 128, 4, 4>(p, stream);
+  if (p.np == 12) return launch_forward<T, 4, 96, 5, 3>(p, stream);
+  if (p.np == 16) return launch_forward<T, 4, 128, 4, 4>(p, stream);
+  if (p.np < 32) return launch_forward<T, 4, 224, 3, 0>(p, stream);
+  if (p.np == 32) return launch_forward<T, 4, 256, 2, 8>(p, stream);
+  if (p.np == 64) return launch_forward<T, 4, 512, 1, 16>(p, stream);
+  return launch_forward<T, 4, 512, 1, 0>(p, stream);
 }
 
 }  // namespace
 
-int forward_warps(int np) { return np / states_of_warp(np); }
+// Warps of a CTA, and CTAs of an SM, as above.
+Fit forward_fit(int np) {
+  return {np < 12 ? np / 2 : np / 4, np == 4 ? 7 : np == 8 ? 4 : np == 12 ? 5 : np == 16 ? 4 : np < 32 ? 3 : np == 32 ? 2 : 1};
+}
 
 int forward(const Problem& p, int dtype, cudaStream_t stream) {
   return dtype == GRU_F32 ? forward_of<float>(p, stream) : forward_of<bf16>(p, stream);

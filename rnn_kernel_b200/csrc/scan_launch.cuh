@@ -6,9 +6,11 @@
 namespace gru {
 namespace scan {
 
-// Warps of a CTA of either pass, for this many states.
-int forward_warps(int np);
-int backward_warps(int np);
+struct Fit {
+  int warps, resident;  // of a CTA, and CTAs of an SM
+};
+Fit forward_fit(int np);  // np: the states rounded up to a multiple of four
+Fit backward_fit(int np);
 int forward(const Problem& p, int dtype, cudaStream_t stream);
 int backward(const Problem& p, int dtype, cudaStream_t stream);
 

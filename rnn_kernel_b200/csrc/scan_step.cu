@@ -195,12 +195,12 @@ void fill(Problem& a, const gru_scan_args& p) {
 // 4 sequences of 2048, 2048 channels, 1 / 4 / 16 segments 360 / 264 / 250 us and 797 /
 // 696 / 672 of the gradient; 64 of 512, 512 channels, 1 / 2 segments 184 / 234 and
 // 578 / 619 us.)
-void cut(Problem& a, int warps, int resident, double pre) {
+void cut(Problem& a, Fit fit, double pre) {
   const long units = (long)a.B * a.tiles;
   const int few = std::max(1, ceil_div(a.T, kBlock)), most = std::min(few, 128);
   auto pass = [&](long ctas) {
     const long c = (ctas + 147) / 148;
-    return (double)c + 9.5 / warps * (double)((c + resident - 1) / resident);
+    return (double)c + 9.5 / fit.warps * (double)((c + fit.resident - 1) / fit.resident);
   };
   double best = 0.0;
   a.segs = 1, a.len = few * kBlock;
@@ -230,11 +230,11 @@ void lay_segments(Problem& a, Pieces& m) {
   a.seg_steps = m.floats(n);
 }
 void lay_forward(Problem& a, Pieces& m) {
-  cut(a, forward_warps(a.np), a.np == 16 ? 5 : a.np <= 32 ? 3 : 1, 0.56);
+  cut(a, forward_fit(a.np), 0.56);
   lay_segments(a, m);
 }
 void lay_backward(Problem& a, Pieces& m) {
-  cut(a, backward_warps(a.np), a.np <= 16 ? 2 : 1, 0.22);
+  cut(a, backward_fit(a.np), 0.22);
   lay_segments(a, m);
   a.part_bc = m.floats((size_t)a.B * a.tiles * a.T * 2 * a.np);
   a.part = m.floats((size_t)a.segs * a.B * a.D * (a.N + 2));

@@ -45,6 +45,9 @@ SIZES = [
     (1, 2100, 5, 33, 1),
     (2, 90, 130, 32, 1),
     (1, 300, 64, 24, 1),
+    (2, 130, 70, 10, 2),
+    (1, 700, 64, 12, 1),
+    (3, 40, 66, 8, 1),
 ]
 OPTIONS = [dict(), dict(gate=False), dict(skip=False, bias=False), dict(gate=False, skip=False, state=False)]
 
