@@ -23,13 +23,13 @@
 // by side, each putting the segments ahead of it together first.
 //
 // The floor is one exponential per token, channel and state (16 a cycle and SM).  64
-// sequences of 512 tokens, 512 channels, 16 states, FP32: 185 us, of which the
-// exponentials would take 58 and memory 41.  No unit is full (issue slots 46 %,
-// exponentials 42 %, shared memory 51 %): the latencies of a token's chain, with the 14
-// warps an SM that this many sequences make.  16384 tokens of 2048 channels in 64
-// segments, bf16: 191 us the first pass (exponentials 70 % busy), 303 the second.
-// Left out in turn, exponentials, copies, preparation and B and C took 20 to 30 us of
-// the 185 each, finish() and the blocks' carrying 12 to 14.
+// sequences of 512 tokens, 512 channels, 16 states, FP32: 173 us, of which the
+// exponentials would take 58 and memory 41.  No unit is full (issue slots 52 %,
+// exponentials 46 %, shared memory 54 %): the latencies of a token's chain, with the 13
+// warps an SM that its registers allow.  16384 tokens of 2048 channels in 32 segments,
+// bf16: 195 us the first pass (exponentials 71 % busy), 283 the second.  Left out in
+// turn, exponentials, copies, preparation and B and C took 20 to 30 us each of 185,
+// finish() and the blocks' carrying 12 to 14.
 
 #include <algorithm>
 
