@@ -242,6 +242,9 @@ __global__ void __launch_bounds__(MOST, OCC) scan_backward_kernel(const __grid_c
     for (int half = 1; half >= 0; --half) {
 #pragma unroll
       for (int g = 0; g < GW; ++g) {
+        // one pair's work behind the other's: mixed by the compiler, its registers went to
+        // memory (32 states 1164 us instead of 954)
+        if (g > 0) __syncwarp();
         const int n0 = 2 * (g * warps + w);
         const float* bs = sm + l.bs + n0 * kRow;
         const float* cs = sm + l.cs + n0 * kRow;
@@ -475,7 +478,7 @@ int launch_backward(const Problem& p, cudaStream_t stream) {
 
 // Two pairs of states a warp, one after the other, from 20 states on, where that many
 // warps leave room for two CTAs (64 sequences of 512 tokens, 512 channels, 32 states:
-// 1013 us, 1081 with a pair a warp; 16 states 562 and 517).  As many CTAs an SM as
+// 954 us, 1081 with a pair a warp; 16 states 562 and 517).  As many CTAs an SM as
 // shared memory and 128 registers a thread allow.
 template <typename T>
 int backward_of(const Problem& p, cudaStream_t stream) {

@@ -191,10 +191,10 @@ void fill(Problem& a, const gru_scan_args& p) {
 // takes 17 tokens' time to start, and a third of one's for each segment ahead of it.
 // More than one segment needs a first pass over all but one, with `pre` of the work.
 // (Fitted to some 100 forwards and 50 gradients of 1 to 128 segments, which it gives
-// to about 5 %: 16384 tokens of 512 channels, 1 / 8 / 64 segments 2699 / 537 / 156 us;
-// 4 sequences of 2048, 2048 channels, 1 / 4 / 16 segments 360 / 264 / 250 us and 797 /
-// 696 / 672 of the gradient; 64 of 512, 512 channels, 1 / 2 segments 184 / 234 and
-// 578 / 619 us.)
+// to about 5 %; its choices take at most 4 % more than the best ones.  16384 tokens of
+// 512 channels, 1 / 8 / 64 segments: 2404 / 495 / 150 us; 4 sequences of 2048, 2048
+// channels, 1 / 4 / 8 segments 332 / 250 / 246 us and 674 / 624 / 592 of the gradient;
+// 64 of 512, 512 channels, 1 / 2 segments 168 / 217 and 514 / 561 us.)
 void cut(Problem& a, Fit fit, double pre) {
   const long units = (long)a.B * a.tiles;
   const int few = std::max(1, ceil_div(a.T, kBlock)), most = std::min(few, 128);
