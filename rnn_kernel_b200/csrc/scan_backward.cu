@@ -305,6 +305,7 @@ __global__ void __launch_bounds__(MOST, OCC) scan_backward_kernel(const __grid_c
             h[j][2 * t + 1] = __ffma2_rn(a[j][2 * t + 1], h[j][2 * t], __fmul2_rn(hi(u), hi(bv)));
             all[j] = __fmul2_rn(all[j], __fmul2_rn(a[j][2 * t], a[j][2 * t + 1]));
           }
+          __syncwarp();  // a pair of tokens after another, for the registers' sake (516 -> 509 us)
         }
         float sums[kHalf];
         float2 da2[2] = {twice(0.0f), twice(0.0f)};  // of the half: short sums first
