@@ -23,7 +23,7 @@
 // in a fixed order, as are those over sequences of dA, dskip and dbias.  Segments as
 // in the forward.
 //
-// 64 sequences of 512 tokens, 512 channels, 16 states, FP32: 510 us; its exponentials
+// 64 sequences of 512 tokens, 512 channels, 16 states, FP32: 500 us; its exponentials
 // would take 87, its memory 82.  Bound by instructions and their latencies (issue slots
 // 50 % with the 16 warps an SM that 128 registers a thread allow; shared memory's
 // wavefronts 60 %).  It took 551 when it made what the gate multiplied once more, instead
