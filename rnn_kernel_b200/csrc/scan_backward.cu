@@ -77,9 +77,9 @@ __device__ __forceinline__ void halve(float* v, int bit, bool upper) {
   }
 }
 
-// GW: pairs of states of a warp.  SUM: only what the segments hand back.  MOST, OCC and W
-// as in the forward.
-template <typename T, int GW, bool SUM, int MOST, int OCC, int W>
+// GW: pairs of states of a warp.  SUM: only what the segments hand back.  PADS, MOST, OCC
+// and W as in the forward.
+template <typename T, int GW, bool SUM, bool PADS, int MOST, int OCC, int W>
 __global__ void __launch_bounds__(MOST, OCC) scan_backward_kernel(const __grid_constant__ Problem p) {
   extern __shared__ __align__(16) float sm[];
   const int threads = W ? 32 * W : blockDim.x, warps = W ? W : threads >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(MOST, OCC) scan_backward_kernel(const __grid_c
             back[g][j] = __fmul2_rn(a[j][2 * t], d0);
             const float2 q1 = __fmul2_rn(r1, h0), q0 = __fmul2_rn(back[g][j], hb);  // w
             b0 = __ffma2_rn(lo(bv), d0, b0), b1 = __ffma2_rn(hi(bv), d1, b1);
-            w0 = __ffma2_rn(rt[g][j], q0, w0), w1 = __ffma2_rn(rt[g][j], q1, w1);
+            if (!PADS || n0 + j < p.N) w0 = __ffma2_rn(rt[g][j], q0, w0), w1 = __ffma2_rn(rt[g][j], q1, w1);
             da2[j] = __ffma2_rn(lo(s), q0, da2[j]), da2[j] = __ffma2_rn(hi(s), q1, da2[j]);
             v[2 * j] = fmaf(d0.y, u.y, d0.x * u.x), v[2 * j + 1] = fmaf(d1.y, u.w, d1.x * u.z);
             v[4 + 2 * j] = fmaf(h0.y, gv.y, h0.x * gv.x), v[5 + 2 * j] = fmaf(h1.y, gv.w, h1.x * gv.z);
@@ -461,12 +461,12 @@ int launch_backward(const Problem& p, cudaStream_t stream) {
   const long units = (long)p.B * p.tiles;
   LaunchScope scope(kKindSelectiveScan, stream, p.segs > 1 ? 4 : 3);
   if (p.segs > 1) {
-    auto kernel = scan_backward_kernel<T, GW, true, MOST, OCC, W>;
+    auto kernel = scan_backward_kernel<T, GW, true, false, MOST, OCC, W>;
     GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     kernel<<<(unsigned)(units * (p.segs - 1)), 32 * warps, smem, stream>>>(p);
     GRU_CUDA_TRY(cudaGetLastError());
   }
-  auto kernel = scan_backward_kernel<T, GW, false, MOST, OCC, W>;
+  auto kernel = p.N == p.np ? scan_backward_kernel<T, GW, false, false, MOST, OCC, W> : scan_backward_kernel<T, GW, false, true, MOST, OCC, W>;
   GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   kernel<<<(unsigned)(units * p.segs), 32 * warps, smem, stream>>>(p);
   GRU_CUDA_TRY(cudaGetLastError());

@@ -58,10 +58,12 @@ __host__ __device__ inline Lay layout(int warps, int np, int N, int elem) {
   return l;
 }
 
-// SG: states of a warp.  SUM: only what the segments make of a state.  MOST: threads
+// SG: states of a warp.  SUM: only what the segments make of a state.  PADS: some of
+// them are not there (an infinite dt x times their B of 0 makes NaN of them, which
+// is kept out of y; asked for every state it took 2 % where all are there).  MOST: threads
 // at most.  OCC: CTAs of an SM.  W: the warps, where they are known (addresses are
 // constants then, and what finish() needs stays in registers), or 0.
-template <typename T, int SG, bool SUM, int MOST, int OCC, int W>
+template <typename T, int SG, bool SUM, bool PADS, int MOST, int OCC, int W>
 __global__ void __launch_bounds__(MOST, OCC) scan_forward_kernel(const __grid_constant__ Problem p) {
   extern __shared__ __align__(16) float sm[];
   const int threads = W ? 32 * W : blockDim.x, warps = W ? W : threads >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -215,7 +217,7 @@ __global__ void __launch_bounds__(MOST, OCC) scan_forward_kernel(const __grid_co
         const float2 h1 = __ffma2_rn(a1, h0, __fmul2_rn(hi(u), hi(bv)));
         h[j] = h1;
         all[j] = __fmul2_rn(all[j], __fmul2_rn(a0, a1));
-        if (!SUM) {
+        if (!SUM && (!PADS || n0 + j < p.N)) {
           const float4 cv = *reinterpret_cast<const float4*>(cs + j * kRow + 4 * t);
           y0 = __ffma2_rn(lo(cv), h0, y0);
           y1 = __ffma2_rn(hi(cv), h1, y1);
@@ -251,12 +253,12 @@ int launch_forward(const Problem& p, cudaStream_t stream) {
   const long units = (long)p.B * p.tiles;
   LaunchScope scope(kKindSelectiveScan, stream, p.segs > 1 ? 2 : 1);
   if (p.segs > 1) {
-    auto kernel = scan_forward_kernel<T, SG, true, MOST, OCC, W>;
+    auto kernel = scan_forward_kernel<T, SG, true, false, MOST, OCC, W>;
     GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     kernel<<<(unsigned)(units * (p.segs - 1)), 32 * warps, smem, stream>>>(p);
     GRU_CUDA_TRY(cudaGetLastError());
   }
-  auto kernel = scan_forward_kernel<T, SG, false, MOST, OCC, W>;
+  auto kernel = p.N == p.np ? scan_forward_kernel<T, SG, false, false, MOST, OCC, W> : scan_forward_kernel<T, SG, false, true, MOST, OCC, W>;
   GRU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   kernel<<<(unsigned)(units * p.segs), 32 * warps, smem, stream>>>(p);
   GRU_CUDA_TRY(cudaGetLastError());

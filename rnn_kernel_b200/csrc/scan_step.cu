@@ -78,9 +78,8 @@ __global__ void __launch_bounds__(kStepThreads, 3) scan_step_kernel(const Proble
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       h[k][j] = fmaf(exp2_of(sk * decay_rate(a[k][j])), h[k][j], uk * bv[j]);
-      y = fmaf(cv[j], h[k][j], y);
+      if (j < left) y = fmaf(cv[j], h[k][j], y);  // an infinite dt x makes NaN of states that are not there
     }
-    if (left <= 0) y = 0.0f;
 #pragma unroll
     for (int o = LP / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
     if (part == k) own = y;
