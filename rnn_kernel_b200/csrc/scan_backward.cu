@@ -139,8 +139,8 @@ __global__ void __launch_bounds__(MOST, OCC) scan_backward_kernel(const __grid_c
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int n = min(2 * (g * warps + w) + j, p.np - 1);
-          back[g][j] = __ffma2_rn(passed(rt[g][j], steps), back[g][j],
-                                  both(p.seg_sums + (at * p.np + n) * kTile, 0, lane));
+          back[g][j] = behind_segment(back[g][j], passed(rt[g][j], steps),
+                                      both(p.seg_sums + (at * p.np + n) * kTile, 0, lane));
         }
     }
 

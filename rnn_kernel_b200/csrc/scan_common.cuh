@@ -2,6 +2,8 @@
 // include/rnn_kernel_b200.h).
 #pragma once
 
+#include <math_constants.h>
+
 #include "row_ops.cuh"
 
 namespace gru {
@@ -275,9 +277,18 @@ __device__ __forceinline__ float2 passed(float2 rate, float2 steps) {
 }
 // A state behind some tokens, its part from before them carried by `decay` and not
 // by the product of the tokens' decays (unless that overflowed, where A is positive).
+// An infinite state has no such difference (0 or a negative number of infinities is
+// NaN): it stays as the tokens left it.
 __device__ __forceinline__ float2 carried(float2 state, float2 before, float2 decay, float2 product) {
-  const float2 d = __fadd2_rn(decay, make_float2(-product.x, -product.y));
-  return __ffma2_rn(make_float2(fabsf(d.x) <= kMost ? d.x : 0.0f, fabsf(d.y) <= kMost ? d.y : 0.0f), before, state);
+  const float2 d = __fadd2_rn(decay, make_float2(-product.x, -product.y)), r = __ffma2_rn(d, before, state);
+  return make_float2(fabsf(r.x) <= kMost ? r.x : state.x, fabsf(r.y) <= kMost ? r.y : state.y);
+}
+// A state behind a segment that adds `sum` to it.  Its decay may be below the least FP32
+// number where no token's is, so an infinity is not multiplied by it.
+__device__ __forceinline__ float2 behind_segment(float2 state, float2 decay, float2 sum) {
+  const float2 r = __ffma2_rn(decay, state, sum);
+  return make_float2(fabsf(state.x) == CUDART_INF_F ? state.x + sum.x : r.x,
+                     fabsf(state.y) == CUDART_INF_F ? state.y + sum.y : r.y);
 }
 
 }  // namespace scan

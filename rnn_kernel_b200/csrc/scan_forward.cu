@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(MOST, OCC) scan_forward_kernel(const __grid_co
       const float2 steps = both(p.seg_steps + at * kTile, 0, lane);
 #pragma unroll
       for (int j = 0; j < SG; ++j)
-        h[j] = __ffma2_rn(passed(rt[j], steps), h[j], both(p.seg_sums + (at * p.np + n0 + j) * kTile, 0, lane));
+        h[j] = behind_segment(h[j], passed(rt[j], steps), both(p.seg_sums + (at * p.np + n0 + j) * kTile, 0, lane));
     }
 
   float4* step = reinterpret_cast<float4*>(sm + l.step) + lane;  // [pair of tokens][lane]

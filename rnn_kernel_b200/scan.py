@@ -18,9 +18,9 @@ x, dt, B, C and z are all FP32 or all bf16; A, skip, dt_bias and states are FP32
 The convolution's weights are FP32 or of x's type, its state of x's type.  All
 arithmetic is FP32 (the convolution's weight gradients end in FP64 sums) and
 results are rounded to bf16 once.  ``step * A`` must not be positive: states
-decay.  Decays below 2^-126 count as 0.  Shape problems raise ``ValueError``,
-device and dtype problems and CUDA failures ``RuntimeError``; there is no CPU
-fallback.
+decay.  Decays below 2^-126 count as 0.  A state that has become infinite stays
+so.  Shape problems raise ``ValueError``, device and dtype problems and CUDA
+failures ``RuntimeError``; there is no CPU fallback.
 """
 from __future__ import annotations
 
