@@ -4,8 +4,8 @@
 //
 // Each function takes what its Python namesake takes, positionally, and gives its
 // result, or None for a call that it leaves to Python: tensors that have to be
-// copied first, and all that is refused, which Python explains.  Gradients are
-// autograd functions; their own derivatives raise.
+// copied first, calls that torch.jit.trace records, and all that is refused, which
+// Python explains.  Gradients are autograd functions; their own derivatives raise.
 
 #include "host_operators.h"
 
@@ -14,6 +14,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/object_ptr.h>
 
 #include <atomic>
@@ -71,6 +72,12 @@ bool supported(int device) {
   return k > 0;
 }
 
+// Whether a call is of the usual kind: as many arguments as it takes, an entry to call, and
+// no trace being recorded, which would hold the allocations alone.
+template <typename F>
+bool ready(Py_ssize_t n, Py_ssize_t takes, F entry) {
+  return n == takes && entry && !torch::jit::tracer::isTracing();
+}
 // A plain tensor, or None where that is allowed (an undefined one then).
 bool take(PyObject* o, Tensor* t, bool none_too = false) {
   if (o == Py_None) return none_too;
@@ -357,7 +364,7 @@ bool changed_in_place(const Tensor& t) {
 PyObject* layer_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Tensor x, weight, bias, residual;
-  if (n != 5 || !lib.norm_forward || !take(o[0], &x) || !take(o[1], &weight) || !take(o[2], &bias, true) ||
+  if (!ready(n, 5, lib.norm_forward) || !take(o[0], &x) || !take(o[1], &weight) || !take(o[2], &bias, true) ||
       !PyFloat_Check(o[3]) || !take(o[4], &residual, true))
     Py_RETURN_NONE;
   const double eps = PyFloat_AS_DOUBLE(o[3]);
@@ -388,7 +395,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
 PyObject* selective_scan(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Tensor x, dt, A, B, C, skip, z, bias, state;
-  if (n != 10 || !lib.scan_forward || !take(o[0], &x) || !take(o[1], &dt) || !take(o[2], &A) || !take(o[3], &B) || !take(o[4], &C) ||
+  if (!ready(n, 10, lib.scan_forward) || !take(o[0], &x) || !take(o[1], &dt) || !take(o[2], &A) || !take(o[3], &B) || !take(o[4], &C) ||
       !take(o[5], &skip, true) || !take(o[6], &z, true) || !take(o[7], &bias, true) || !PyBool_Check(o[8]) || !take(o[9], &state, true))
     Py_RETURN_NONE;
   if (!scan_usual(x, dt, A, B, C, skip, z, bias, state, 2)) Py_RETURN_NONE;
@@ -411,7 +418,7 @@ PyObject* selective_scan(PyObject*, PyObject* const* o, Py_ssize_t n) {
 PyObject* selective_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Tensor x, dt, A, B, C, skip, z, bias, state;
-  if (n != 10 || !lib.scan_step || !take(o[0], &x) || !take(o[1], &dt) || !take(o[2], &A) || !take(o[3], &B) || !take(o[4], &C) ||
+  if (!ready(n, 10, lib.scan_step) || !take(o[0], &x) || !take(o[1], &dt) || !take(o[2], &A) || !take(o[3], &B) || !take(o[4], &C) ||
       !take(o[5], &state) || !take(o[6], &skip, true) || !take(o[7], &z, true) || !take(o[8], &bias, true) || !PyBool_Check(o[9]))
     Py_RETURN_NONE;
   if (!scan_usual(x, dt, A, B, C, skip, z, bias, state, 1)) Py_RETURN_NONE;
@@ -433,7 +440,7 @@ PyObject* selective_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
 PyObject* causal_conv(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Tensor x, weight, bias, state;
-  if (n != 5 || !lib.conv_forward || !take(o[0], &x) || !take(o[1], &weight) || !take(o[2], &bias, true) || !take(o[4], &state, true))
+  if (!ready(n, 5, lib.conv_forward) || !take(o[0], &x) || !take(o[1], &weight) || !take(o[2], &bias, true) || !take(o[4], &state, true))
     Py_RETURN_NONE;
   const int activation = activation_of(o[3]);
   if (activation < 0 || !conv_usual(x, weight, bias, state, 2)) Py_RETURN_NONE;
@@ -455,7 +462,7 @@ PyObject* causal_conv(PyObject*, PyObject* const* o, Py_ssize_t n) {
 PyObject* causal_conv_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Tensor x, weight, bias, state;
-  if (n != 5 || !lib.conv_step || !take(o[0], &x) || !take(o[1], &weight) || !take(o[2], &state) || !take(o[3], &bias, true)) Py_RETURN_NONE;
+  if (!ready(n, 5, lib.conv_step) || !take(o[0], &x) || !take(o[1], &weight) || !take(o[2], &state) || !take(o[3], &bias, true)) Py_RETURN_NONE;
   const int activation = activation_of(o[4]);
   if (activation < 0 || !conv_usual(x, weight, bias, state, 1)) Py_RETURN_NONE;
   const gru_conv_args a = conv_args(x, weight, bias, activation, Tensor());
