@@ -239,6 +239,12 @@ def operators():
         return None
 
 
+def traced() -> bool:
+    """Whether torch.jit.trace records this call: it sees torch's operations, allocations among them, and autograd functions, but
+    not the library's calls."""
+    return torch._C._get_tracing_state() is not None
+
+
 def last_error() -> str:
     msg = load().gru_last_error()
     return msg.decode() if msg else ""

@@ -186,7 +186,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     needed = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
-    if needed or _forward_mode():  # the Function refuses tangents
+    if needed or _forward_mode() or _lib.traced():  # the Function refuses tangents; a trace's replay calls it again
         return GatedDeltaRuleFunction.apply(q, k, v, g, beta, initial_state, scale)
     code = _check("gated_delta_rule", q, k, v, g, beta, initial_state, 2)
     out, last, _ = _forward(code, q, k, v, g, beta, initial_state, scale, False)
@@ -202,6 +202,8 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     code = _check("gated_delta_step", q, k, v, g, beta, state, 1)
     if _forward_mode() and any(forward_ad.unpack_dual(t).tangent is not None for t in (q, k, v, g, beta, state)):
         raise RuntimeError("gated_delta_step has no derivative.")
+    if _lib.traced():
+        raise RuntimeError("gated_delta_step cannot be traced: it updates its state in place.")
     if not state.is_contiguous():
         raise ValueError("gated_delta_step: the state is updated in place and must be contiguous.")
     q, k, v = _dense_heads(q), _dense_heads(k), _dense_heads(v)

@@ -178,6 +178,8 @@ class GRUFunction(torch.autograd.Function):
 def gru_forward_inference(x, h0, weight_ih, weight_hh, bias_ih, bias_hh):
     """No-stash forward of one layer (ref ``_a100_gru_forward_inference``, ``:583-617``)."""
     with torch.no_grad():
+        if _lib.traced():  # a trace's replay calls the Function again
+            return GRUFunction.apply(x, h0, weight_ih, weight_hh, bias_ih, bias_hh)
         out, hn, _, _ = _forward_impl(x, h0, weight_ih, weight_hh, bias_ih, bias_hh, False)
     return out, hn
 

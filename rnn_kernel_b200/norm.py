@@ -71,21 +71,16 @@ def _first_derivatives(name, grads):
     return tuple(grads)
 
 
-def _traced():
-    """Whether torch.jit.trace records this call: it sees torch's operations, allocations among them, and autograd functions."""
-    return torch._C._get_tracing_state() is not None
-
-
 def _differentiated(*tensors):
     """Whether a call has to go through autograd: gradients asked for, a level of forward mode (which the Functions refuse), or a
     trace (whose replay calls the Function again)."""
-    return forward_ad._current_level >= 0 or _traced() or (
+    return forward_ad._current_level >= 0 or _lib.traced() or (
         torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
 
 
 def _no_tangents(name, *tensors):
     """For calls without a derivative, which are no autograd functions and change a state in place."""
-    if _traced():
+    if _lib.traced():
         raise RuntimeError(f"{name} cannot be traced: it updates its state in place.")
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError(f"{name} has no derivative.")
