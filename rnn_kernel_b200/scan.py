@@ -440,5 +440,11 @@ class RecurrentStack(nn.Module):
 
     @torch.no_grad()
     def step(self, x: torch.Tensor, states) -> torch.Tensor:
-        """One token of every sequence, [batch, width], through layers that have a step; states are updated in place."""
+        """One token of every sequence, [batch, width], through layers that have a step (:class:`GRU` has none: RuntimeError);
+        states are updated in place.  Layers ahead of one that refuses its own state have moved theirs on."""
+        if len(states) < len(self.layers):
+            raise ValueError(f"RecurrentStack.step: {len(self.layers)} states are needed, one for each layer; there are {len(states)}.")
+        for layer in self.layers:
+            if not callable(getattr(layer, "step", None)):
+                raise RuntimeError(f"RecurrentStack.step: {type(layer).__name__} has no step.")
         return self._run(x, lambda i, y: self.layers[i].step(y, states[i]))
