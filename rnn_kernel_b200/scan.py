@@ -376,9 +376,12 @@ class SelectiveScan(nn.Module):
         self.out_proj = nn.Linear(inner, self.output_size, bias=False)
 
     def init_state(self, batch: int, dtype: Optional[torch.dtype] = None):
-        """Zeros; ``dtype`` is the convolution's (default: the projection's own)."""
+        """Zeros; ``dtype`` is the convolution's (default: that of the projection's output, which autocast sets)."""
         like = self.in_proj.weight
-        return (torch.zeros(batch, self.conv_size - 1, self.inner_size, dtype=like.dtype if dtype is None else dtype, device=like.device),
+        kind = like.device.type
+        if dtype is None:
+            dtype = torch.get_autocast_dtype(kind) if torch.is_autocast_enabled(kind) else like.dtype
+        return (torch.zeros(batch, self.conv_size - 1, self.inner_size, dtype=dtype, device=like.device),
                 torch.zeros(batch, self.inner_size, self.state_size, dtype=torch.float32, device=like.device))
 
     def _inputs(self, x, z):
