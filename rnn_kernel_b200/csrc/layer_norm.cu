@@ -381,7 +381,9 @@ int launch_forward(const Norm& a, cudaStream_t stream) {
   } else {
     GRU_NORM(1, true)
     GRU_NORM(2, true)
-    GRU_NORM(4, true)
+    if constexpr (V == 4) {  // two loads of eight hold the longest row
+      GRU_NORM(4, true)
+    }
   }
 #undef GRU_NORM
   return refuse("gru_layer_norm_forward", "no kernel for this width", GRU_ERR_UNSUPPORTED);

@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(MOST, OCC) scan_backward_kernel(const __grid_c
       for (int g = 0; g < GW; ++g)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int n = min(2 * (g * warps + w) + j, p.np - 1);
+          const int n = 2 * (g * warps + w) + j;
           back[g][j] = behind_segment(back[g][j], passed(rt[g][j], steps),
                                       both(p.seg_sums + (at * p.np + n) * kTile, 0, lane));
         }
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(MOST, OCC) scan_backward_kernel(const __grid_c
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int n = 2 * (g * warps + w) + j;
-        if (n < p.np) *reinterpret_cast<float2*>(p.seg_sums + (at * p.np + n) * kTile + 2 * lane) = back[g][j];
+        *reinterpret_cast<float2*>(p.seg_sums + (at * p.np + n) * kTile + 2 * lane) = back[g][j];
       }
     if (w == 0) *reinterpret_cast<float2*>(p.seg_steps + at * kTile + 2 * lane) = total;
     return;
