@@ -372,7 +372,10 @@ int launch(const Conv& a, Way way, const StoreConv& store, cudaStream_t stream) 
   return GRU_OK;
 }
 
-// V: elements a thread; two where the window is long, for its registers' sake.
+// V: elements a thread; two where the window is long, for its registers' sake.  (Four were
+// chosen by bf16 times.  In FP32 W = 4 spills 108 bytes in the forward and 360 in the gradient:
+// 4 x 2048 tokens of 4096 channels 70 and 130 us, timed with the launches, where bytes take
+// 41 and 62.)
 template <typename T>
 int launch_any(const Conv& a, bool vec, Way way, const StoreConv& store, cudaStream_t stream) {
 #define GRU_CONV(WIDTH, V)                                                             \
@@ -392,8 +395,10 @@ int launch_any(const Conv& a, bool vec, Way way, const StoreConv& store, cudaStr
 // The tokens of a run, of T that `units` pieces of work each have: of the runs that
 // fill the GPU once, twice and so on, those that take the least, at `extra` tokens'
 // time besides its own for a run.  side: runs of a CTA; resident: CTAs of an SM.  Not
-// below 8 tokens nor above `longest`.  (4 x 2048 tokens, 4096 channels: forward in runs of 76, once the GPU,
-// 37 us, of 32 39, of 128 43; gradient in runs of 128, once, 71 us, of 32 or 64 77.)
+// above `longest`, and not more runs than eighths of T, so of 5 tokens at least where T
+// is more.  (4 x 2048 tokens of 4096 channels, bf16, timed with the launches and the sum, which
+// the file's head leaves out: forward in runs of 76, once the GPU, 37 us, of 32 39, of 64
+// or 128 43; gradient in runs of 128, once, 71 us, of 32 or 64 77.)
 int run_of(long units, int side, int resident, int T, int longest, int extra) {
   const long slots = 148L * resident, most = (T + 7) / 8, least = (T + longest - 1) / longest;
   long best = 0;
@@ -407,7 +412,10 @@ int run_of(long units, int side, int resident, int T, int longest, int extra) {
   }
   return run;
 }
-// A gradient's: its CTAs take 8 runs of one batch row and 32 lanes.  The same whether
+// A gradient's: its CTAs take 8 runs of one batch row and 32 lanes, so that short sequences
+// have runs down to a token, one for each warp (4096 channels, bf16: 64 x 8 tokens 42 us in
+// runs of 1 or of 8, 64 x 72 75 us in runs of 9, 114 in runs of 8, whose last one takes a
+// CTA).  The same whether
 // or not the tensors' boundaries let a lane have several channels.  A thread adds up
 // at most 512 tokens of dw in FP32 (an error of about 256^0.5 2^-25 = 5e-7 of it).
 int grad_run(const gru_conv_args& p) {

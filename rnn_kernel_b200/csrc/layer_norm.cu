@@ -4,9 +4,11 @@
 //   s = x + residual (in the residual's type);  n = (s - mean) rstd;  y = n w + b
 //   ds += rstd (g - mean(g) - n mean(g n)) with g = dy w;  dw = sum dy n;  db = sum dy
 //
-// A row is in registers from its one read to its one write: a warp holds rows
+// A row is read and written once and held between: a warp holds rows
 // of up to 1024 bf16 or 512 FP32 elements, a CTA longer ones, 16 bytes a thread
-// and load; the next row's loads are under way meanwhile.  A first sum gives a mean
+// and load; the next row's loads are under way meanwhile.  One or two loads a thread stay in
+// registers, but for bf16 rows of two loads with a residual; forms of more loads spill, the warps'
+// most, as all are compiled for CTAs of 1024 threads (gradient: 512).  A first sum gives a mean
 // that rounding leaves a little off where a row has a large offset; the distances
 // from it, which are exact there, give the rest of the mean (`shift`) and the
 // variance, so an offset costs no digits.  y is the norm of s as it is stored: the
@@ -17,7 +19,9 @@
 // Bound by memory: 8192 rows of 2048 with a residual, bf16, forward 26 us (134 MB, 79 %
 // of the copy rate), gradient 36 (134 MB, 57 %: two CTAs an SM by their registers, and
 // a barrier a row); 32768 rows of 256, FP32, forward 12 us (67 MB, 85 %), gradient 17
-// (101 MB, 89 %).
+// (101 MB, 89 %).  By local memory where registers are spilled: 8192 rows with a residual,
+// timed with the launches, of 768 bf16 78 and 56 us (50 MB each, 8 us; gradient 178
+// with an FP32 residual), of 4096 61 and 114 (268 MB, 41 us).
 
 #include <algorithm>
 

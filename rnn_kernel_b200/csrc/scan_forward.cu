@@ -25,8 +25,8 @@
 // The floor is one exponential per token, channel and state (16 a cycle and SM).  64
 // sequences of 512 tokens, 512 channels, 16 states, FP32: 173 us, of which the
 // exponentials would take 58 and memory 41.  No unit is full (issue slots 52 %,
-// exponentials 46 %, shared memory 54 %): the latencies of a token's chain, with the 13
-// warps an SM that its registers allow.  16384 tokens of 2048 channels in 32 segments,
+// exponentials 46 %, shared memory 54 %): the latencies of a token's chain, with 12.7
+// warps an SM on average (registers allow 16; the 512 CTAs are 13.8).  16384 tokens of 2048 channels in 32 segments,
 // bf16: 195 us the first pass (exponentials 71 % busy), 283 the second.  Left out in
 // turn, exponentials, copies, preparation and B and C took 20 to 30 us each of 185,
 // finish() and the blocks' carrying 12 to 14.
@@ -269,8 +269,10 @@ int launch_forward(const Problem& p, cudaStream_t stream) {
 // states, for threads to copy and prepare with.  (64 sequences of 512 tokens, 512
 // channels, four and two states a warp: 8 states 156 and 115 us, 12 states 162 and
 // 205, 16 states 187 and 210, 32 states 337 and 390.)  As many CTAs an SM as leave a
-// thread some 110 to 128 registers: 80 for one or two CTAs more took 199 us instead of
-// 172 at 16 states, 358 instead of 299 at 32.  Known warps where the states are usual
+// thread some 110 to 128 registers, of which 8 to 44 bytes are spilled: 80 for one or two
+// CTAs more took 199 us instead of 172 at 16 states, 358 instead of 299 at 32.  (17 to 28
+// states have three CTAs and 80 registers all the same, and spill 124 bytes; two were not
+// measured there.)  Known warps where the states are usual
 // (8 states 135 us with any number of warps, 115 with four).
 template <typename T>
 int forward_of(const Problem& p, cudaStream_t stream) {
