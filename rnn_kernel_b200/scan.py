@@ -380,7 +380,8 @@ class SelectiveScan(nn.Module):
         like = self.in_proj.weight
         kind = like.device.type
         if dtype is None:
-            dtype = torch.get_autocast_dtype(kind) if torch.is_autocast_enabled(kind) else like.dtype
+            cast = torch.amp.is_autocast_available(kind) and torch.is_autocast_enabled(kind)
+            dtype = torch.get_autocast_dtype(kind) if cast else like.dtype
         return (torch.zeros(batch, self.conv_size - 1, self.inner_size, dtype=dtype, device=like.device),
                 torch.zeros(batch, self.inner_size, self.state_size, dtype=torch.float32, device=like.device))
 

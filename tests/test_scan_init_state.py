@@ -17,6 +17,7 @@ def test_types():
     with torch.autocast("cpu", torch.bfloat16, enabled=False):
         assert m.init_state(2)[0].dtype == torch.float32
     assert m.bfloat16().init_state(2)[0].dtype == torch.bfloat16
+    assert SelectiveScan(16).to("meta").init_state(2)[0].device.type == "meta"  # which has no autocast
 
 
 @pytest.mark.gpu
