@@ -59,8 +59,9 @@ __host__ __device__ inline Lay layout(int warps, int np, int N, int elem) {
 }
 
 // SG: states of a warp.  SUM: only what the segments make of a state.  PADS: some of
-// them are not there (an infinite dt x times their B of 0 makes NaN of them, which
-// is kept out of y; asked for every state it took 2 % where all are there).  MOST: threads
+// them are not there (an infinite dt x times their B of 0 makes NaN of them, and in
+// the gradient an infinite gradient of y times their C: that is kept out of the sums over
+// states, which took 2 % where all are there and were asked for).  MOST: threads
 // at most.  OCC: CTAs of an SM.  W: the warps, where they are known (addresses are
 // constants then, and what finish() needs stays in registers), or 0.
 template <typename T, int SG, bool SUM, bool PADS, int MOST, int OCC, int W>

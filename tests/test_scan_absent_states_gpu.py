@@ -1,6 +1,6 @@
-"""States are worked on in fours; those that a call does not have stay out of its results where dt x is infinite.  B, C and the
-outputs' gradients are positive and there is no skip, so an infinity meets none of the other sign.  Finite numbers are held to 1e-5, as the scan's own
-tests derive it."""
+"""States are worked on in fours; those that a call does not have stay out of its results where dt x or an output's
+gradient is infinite.  B, C and the outputs' gradients are positive and there is no skip, so an infinity meets none of the
+other sign.  Finite numbers are held to 1e-5, as the scan's own tests derive it."""
 import pytest
 import torch
 
@@ -43,6 +43,22 @@ def test_values_and_gradients(N):
     got = torch.autograd.grad(outs, [mine[n] for n in names], d)
     true = torch.autograd.grad(want, [plain[n] for n in names], [t.double() for t in d])
     assert bool(true[1][1, 1:, 3].isinf().all())
+    for a, b in zip(got, true):
+        same(a, b)
+
+
+@pytest.mark.parametrize("N", [1, 2, 3, 4, 5, 7, 11, 13, 18, 27, 30, 33, 62])
+def test_an_infinite_gradient(N):
+    kw = inputs(3, N)
+    kw["x"][1, 0, 3] = 1.0
+    mine, plain = R.leaves(kw), R.leaves(kw, wide=True)
+    outs, want = selective_scan(**mine), R.scan(**plain)
+    names = ("x", "initial_state")
+    d = [torch.rand_like(o) + 0.1 for o in outs]
+    d[0][1, 2, 3] = INF
+    got = torch.autograd.grad(outs, [mine[n] for n in names], d)
+    true = torch.autograd.grad(want, [plain[n] for n in names], [t.double() for t in d])
+    assert bool(true[0][1, :, 3].isinf().all()) and bool(true[1][1, 3].isinf().all())
     for a, b in zip(got, true):
         same(a, b)
 
