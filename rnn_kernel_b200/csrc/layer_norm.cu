@@ -6,9 +6,9 @@
 //
 // A row is read and written once and held between: a warp holds rows
 // of up to 1024 bf16 or 512 FP32 elements, a CTA longer ones, 16 bytes a thread
-// and load; the next row's loads are under way meanwhile.  One or two loads a thread stay in
-// registers, but for bf16 rows of two loads with a residual; forms of more loads spill, the warps'
-// most, as all are compiled for CTAs of 1024 threads (gradient: 512).  A first sum gives a mean
+// and load; the next row's loads are under way meanwhile.  One load a thread stays
+// in registers, and two of FP32; the other forms spill, the warps' most, as all are compiled
+// for CTAs of 1024 threads (gradient: 512).  A first sum gives a mean
 // that rounding leaves a little off where a row has a large offset; the distances
 // from it, which are exact there, give the rest of the mean (`shift`) and the
 // variance, so an offset costs no digits.  y is the norm of s as it is stored: the
